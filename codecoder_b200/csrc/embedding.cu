@@ -1,0 +1,534 @@
+// Token embedding with any number of tokens: the lookup with a scale, and its weight gradient by sorted tokens.
+//
+//   lookup    y[i, :] = scale W[ids[i], :]                              (a zero row where ids[i] is outside [0, V))
+//   gradient  dW[v, :] = scale sum over i with ids[i] = v of gy[i, :]   (ids outside [0, V) contribute nothing)
+//
+// The products and sums are fp32 and rounded once to the output's type.  The gradient is deterministic: the positions
+// are sorted stably by token (least-significant-digit radix sort), and the sorted rows are summed in that order.
+#include <algorithm>
+#include <string>
+
+#include <cuda_fp16.h>
+
+#include "bpc.h"
+#include "bpc_common.cuh"
+#include "bpc_internal.h"
+
+namespace bpc {
+
+namespace {
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+
+template <typename T>
+__device__ __forceinline__ T from_f32(float x);
+template <>
+__device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
+
+// VEC elements moved as one access
+template <typename T, int VEC>
+struct alignas(sizeof(T) * VEC) Pack {
+  T v[VEC];
+};
+
+// ---------------------------------------------------------------------------------------------------------------
+// lookup: one thread per VEC channels of a row
+template <typename I, typename TW, typename TY, int VEC>
+__global__ void __launch_bounds__(256) embed_lookup_kernel(const I* __restrict__ ids, const TW* __restrict__ w,
+                                                           TY* __restrict__ y, int64_t units, int V, int CV,
+                                                           int64_t ldw, float scale) {
+  for (int64_t u = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; u < units;
+       u += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+    const int64_t row = u / CV;
+    const int c = static_cast<int>(u - row * CV) * VEC;
+    const int64_t id = ids[row];
+    Pack<TY, VEC> o;
+    if (id >= 0 && id < V) {
+      const Pack<TW, VEC> x = *reinterpret_cast<const Pack<TW, VEC>*>(w + id * ldw + c);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) o.v[e] = from_f32<TY>(scale * to_f32(x.v[e]));
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) o.v[e] = from_f32<TY>(0.f);
+    }
+    *reinterpret_cast<Pack<TY, VEC>*>(y + u * VEC) = o;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Stable radix sort of the positions by token, kDigitBits bits a pass: per-tile digit counts, one scan per digit over
+// the tiles, then each tile places its keys.  Positions whose id is outside [0, V) get key V: they sort to the end.
+constexpr int kDigitBits = 8;
+constexpr int kBins = 1 << kDigitBits;
+constexpr int kSortThreads = 256;
+constexpr int kSortWarps = kSortThreads / 32;
+constexpr int kSortRounds = 16;                           // keys per thread
+constexpr int kSortTile = kSortThreads * kSortRounds;
+
+template <typename I>
+__device__ __forceinline__ int token_key(I id, int V) {
+  return id >= 0 && static_cast<int64_t>(id) < V ? static_cast<int>(id) : V;
+}
+
+// src: the ids (first pass) or the previous pass's keys, which are in [0, V] already
+template <typename I>
+__global__ void __launch_bounds__(kSortThreads) sort_count_kernel(const I* __restrict__ src, int64_t n, int V, int shift,
+                                                                  int* __restrict__ counts, int tiles) {
+  __shared__ int cnt[kBins];
+  for (int b = threadIdx.x; b < kBins; b += kSortThreads) cnt[b] = 0;
+  __syncthreads();
+  const int64_t base = static_cast<int64_t>(blockIdx.x) * kSortTile;
+#pragma unroll
+  for (int r = 0; r < kSortRounds; ++r) {
+    const int64_t i = base + r * kSortThreads + threadIdx.x;
+    const bool ok = i < n;
+    const unsigned act = __ballot_sync(0xffffffffu, ok);
+    if (ok) {
+      const int digit = (token_key(src[i], V) >> shift) & (kBins - 1);
+      const unsigned same = __match_any_sync(act, digit);
+      if ((threadIdx.x & 31) == __ffs(same) - 1) atomicAdd(&cnt[digit], __popc(same));
+    }
+  }
+  __syncthreads();
+  for (int b = threadIdx.x; b < kBins; b += kSortThreads) counts[static_cast<int64_t>(b) * tiles + blockIdx.x] = cnt[b];
+}
+
+// One block per digit: its counts over the tiles become exclusive sums; totals[digit] their sum.
+__global__ void __launch_bounds__(256) sort_scan_kernel(int* __restrict__ counts, int* __restrict__ totals, int tiles) {
+  __shared__ int warp_sum[8];
+  int* row = counts + static_cast<int64_t>(blockIdx.x) * tiles;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int carry = 0;
+  for (int t0 = 0; t0 < tiles; t0 += 256) {
+    const int t = t0 + threadIdx.x;
+    const int v = t < tiles ? row[t] : 0;
+    int s = v;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, s, d);
+      if (lane >= d) s += o;
+    }
+    if (lane == 31) warp_sum[warp] = s;
+    __syncthreads();
+    int before = carry, all = 0;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      if (w < warp) before += warp_sum[w];
+      all += warp_sum[w];
+    }
+    if (t < tiles) row[t] = before + s - v;
+    carry += all;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) totals[blockIdx.x] = carry;
+}
+
+// Places a tile's keys.  Each warp takes a run of kSortRounds x 32 consecutive keys in order, so ranks by (warp, round,
+// lane) keep the order of equal digits.  perm_in null: the first pass (position i itself).
+template <typename I>
+__global__ void __launch_bounds__(kSortThreads) sort_place_kernel(const I* __restrict__ src,
+                                                                  const int* __restrict__ perm_in, int64_t n, int V,
+                                                                  int shift, const int* __restrict__ offsets,
+                                                                  const int* __restrict__ totals, int tiles,
+                                                                  int* __restrict__ key_out, int* __restrict__ perm_out) {
+  __shared__ int cnt[kSortWarps][kBins];
+  __shared__ int warp_sum[kSortWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int b = threadIdx.x; b < kSortWarps * kBins; b += kSortThreads) (&cnt[0][0])[b] = 0;
+  __syncthreads();
+  const int64_t base = static_cast<int64_t>(blockIdx.x) * kSortTile + warp * (kSortRounds * 32) + lane;
+  int key[kSortRounds], rank[kSortRounds];
+#pragma unroll
+  for (int r = 0; r < kSortRounds; ++r) {
+    const int64_t i = base + r * 32;
+    key[r] = i < n ? token_key(src[i], V) : -1;
+  }
+#pragma unroll
+  for (int r = 0; r < kSortRounds; ++r) {
+    const bool ok = key[r] >= 0;
+    const unsigned act = __ballot_sync(0xffffffffu, ok);
+    rank[r] = 0;
+    if (ok) {
+      const int digit = (key[r] >> shift) & (kBins - 1);
+      const unsigned same = __match_any_sync(act, digit);
+      const int before = cnt[warp][digit];
+      rank[r] = before + __popc(same & ((1u << lane) - 1));
+      __syncwarp(act);
+      if (lane == __ffs(same) - 1) cnt[warp][digit] = before + __popc(same);
+    }
+    __syncwarp();
+  }
+  __syncthreads();
+  {
+    // first place of each digit: the digits below it, then this digit's earlier tiles, then its earlier warps
+    static_assert(kBins == kSortThreads, "one thread per digit");
+    const int b = threadIdx.x;
+    const int v = totals[b];
+    int s = v;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, s, d);
+      if (lane >= d) s += o;
+    }
+    if (lane == 31) warp_sum[warp] = s;
+    __syncthreads();
+    int at = s - v + offsets[static_cast<int64_t>(b) * tiles + blockIdx.x];
+    for (int w = 0; w < warp; ++w) at += warp_sum[w];
+#pragma unroll
+    for (int w = 0; w < kSortWarps; ++w) {
+      const int c = cnt[w][b];
+      cnt[w][b] = at;
+      at += c;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < kSortRounds; ++r) {
+    if (key[r] >= 0) {
+      const int64_t i = base + r * 32;
+      const int at = cnt[warp][(key[r] >> shift) & (kBins - 1)] + rank[r];
+      key_out[at] = key[r];
+      perm_out[at] = perm_in ? perm_in[i] : static_cast<int>(i);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// The segmented sum.  V row ends and n sorted rows form one path of V + n steps (a row end follows the last row of its
+// token), cut into equal runs of `items` steps, one per worker, so that a token with millions of rows and a million
+// tokens without any both spread evenly; every row of dW is written once, the empty ones as zeros.  A token whose rows
+// cross workers: each worker but the one at its end leaves a partial sum in tail[], the last one leaves its own in
+// head[], and wgrad_join_kernel adds them in order.
+struct MergeArgs {
+  const int* key;      // (n,) sorted
+  const int* perm;     // (n,) the rows in that order
+  int64_t n, items, workers;
+  int V, C, G;         // G lanes per worker
+  int64_t ldg;
+  float scale;
+  void* dw;
+  int dw_dtype;
+  float* head;         // (workers, C)
+  float* tail;
+  int* head_token;     // (workers,) the token of head[], or -1
+};
+
+// tokens finished within the first d steps of the path
+__device__ __forceinline__ int64_t path_search(const int* __restrict__ key, int64_t n, int V, int64_t d) {
+  int64_t lo = d > n ? d - n : 0, hi = d < V ? d : V;      // lo holds: every row consumed
+  while (lo < hi) {
+    const int64_t mid = (lo + hi + 1) >> 1;
+    // token mid - 1 is finished before step d iff the next row belongs to a later one
+    if (d - mid >= n || key[d - mid] >= mid) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+template <int VEC>
+__device__ __forceinline__ void store_row(void* dw, int dtype, int64_t at, const float* acc, float scale) {
+  if (dtype == BPC_DTYPE_F32) {
+    Pack<float, VEC < 4 ? VEC : 4>* p = reinterpret_cast<Pack<float, VEC < 4 ? VEC : 4>*>(static_cast<float*>(dw) + at);
+#pragma unroll
+    for (int e = 0; e < VEC; e += 4) {
+      Pack<float, VEC < 4 ? VEC : 4> o;
+#pragma unroll
+      for (int f = 0; f < (VEC < 4 ? VEC : 4); ++f) o.v[f] = scale * acc[e + f];
+      p[e / 4] = o;
+    }
+  } else if (dtype == BPC_DTYPE_BF16) {
+    Pack<__nv_bfloat16, VEC> o;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) o.v[e] = __float2bfloat16_rn(scale * acc[e]);
+    *reinterpret_cast<Pack<__nv_bfloat16, VEC>*>(static_cast<__nv_bfloat16*>(dw) + at) = o;
+  } else {
+    Pack<__half, VEC> o;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) o.v[e] = __float2half_rn(scale * acc[e]);
+    *reinterpret_cast<Pack<__half, VEC>*>(static_cast<__half*>(dw) + at) = o;
+  }
+}
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256) wgrad_merge_kernel(const T* __restrict__ gy, MergeArgs a) {
+  constexpr int kRows = 8;                                // rows whose loads are in flight per worker
+  const int per_block = 256 / a.G;
+  const int64_t w = blockIdx.x * static_cast<int64_t>(per_block) + threadIdx.x / a.G;
+  const int c = (blockIdx.y * a.G + threadIdx.x % a.G) * VEC;
+  if (w >= a.workers) return;
+  const bool on = c < a.C;
+  const int64_t end = a.V + a.n;
+  const int64_t d0 = min(end, w * a.items), d1 = min(end, d0 + a.items);
+  const int64_t i0 = path_search(a.key, a.n, a.V, d0), i1 = path_search(a.key, a.n, a.V, d1);
+  const int64_t j0 = d0 - i0, j1 = d1 - i1;
+  bool open = j0 > 0 && i0 < a.V && a.key[j0 - 1] == i0;   // token i0 began in an earlier worker
+  if (on && c == 0) a.head_token[w] = open && i1 > i0 ? static_cast<int>(i0) : -1;
+  float acc[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
+  int64_t tok = i0;
+  auto flush = [&]() {
+    if (on) {
+      if (open) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) a.head[w * a.C + c + e] = acc[e];
+      } else {
+        store_row<VEC>(a.dw, a.dw_dtype, tok * a.C + c, acc, a.scale);
+      }
+    }
+    open = false;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
+    ++tok;
+  };
+  for (int64_t j = j0; j < j1; j += kRows) {
+    int k[kRows];
+    Pack<T, VEC> x[kRows];
+#pragma unroll
+    for (int u = 0; u < kRows; ++u) {
+      k[u] = a.V;
+      if (j + u < j1) {
+        k[u] = a.key[j + u];
+        if (on && k[u] < a.V) x[u] = *reinterpret_cast<const Pack<T, VEC>*>(gy + a.perm[j + u] * a.ldg + c);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kRows; ++u) {
+      if (k[u] < a.V) {                                    // key V: a position without a token, or past the end
+        while (tok < k[u]) flush();
+        if (on) {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) acc[e] += to_f32(x[u].v[e]);
+        }
+      }
+    }
+  }
+  while (tok < i1) flush();
+  if (on && i1 < a.V && j1 > 0 && a.key[j1 - 1] == i1) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) a.tail[w * a.C + c + e] = acc[e];
+  }
+}
+
+// One block per worker that ended a token begun before it: the tails of the workers since the token's first row, in
+// order, then its own head.
+__global__ void __launch_bounds__(256) wgrad_join_kernel(MergeArgs a) {
+  const int64_t w = blockIdx.x;
+  const int t = a.head_token[w];
+  if (t < 0) return;
+  int64_t lo = 0, hi = a.n;                                // first row of token t
+  while (lo < hi) {
+    const int64_t mid = (lo + hi) >> 1;
+    if (a.key[mid] < t) lo = mid + 1;
+    else hi = mid;
+  }
+  const int64_t first = (lo + t) / a.items;
+  for (int c = threadIdx.x; c < a.C; c += 256) {
+    float s = 0.f;
+    for (int64_t v = first; v < w; ++v) s += a.tail[v * a.C + c];
+    s += a.head[w * a.C + c];
+    store_row<1>(a.dw, a.dw_dtype, static_cast<int64_t>(t) * a.C + c, &s, a.scale);
+  }
+}
+
+int dtype_size(int32_t dtype) { return dtype == BPC_DTYPE_F32 ? 4 : dtype == BPC_DTYPE_BF16 || dtype == BPC_DTYPE_F16 ? 2 : 0; }
+
+// Workspace layout of the gradient
+struct WgradPlan {
+  int passes, tiles, G;
+  int64_t items, workers;
+  size_t key[2], perm[2], counts, totals, head, tail, head_token, bytes;
+};
+
+WgradPlan wgrad_plan(int64_t n, int32_t V, int32_t C) {
+  WgradPlan p;
+  int bits = 1;
+  while (bits < 32 && (static_cast<int64_t>(1) << bits) <= V) ++bits;      // keys are in [0, V]
+  p.passes = (bits + kDigitBits - 1) / kDigitBits;
+  p.tiles = static_cast<int>((n + kSortTile - 1) / kSortTile);
+  p.G = 1;
+  while (p.G < 32 && p.G * 8 < C) p.G *= 2;
+  // about 16 warps of workers per SM, of at least 32 steps
+  const int64_t target = static_cast<int64_t>(num_sms()) * 16 * (32 / p.G);
+  p.items = std::max<int64_t>(32, (V + n + target - 1) / target);
+  p.workers = (V + n + p.items - 1) / p.items;
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t r = at;
+    at += (bytes + 255) & ~static_cast<size_t>(255);
+    return r;
+  };
+  for (int k = 0; k < 2; ++k) {
+    p.key[k] = take(sizeof(int) * n);
+    p.perm[k] = take(sizeof(int) * n);
+  }
+  p.counts = take(sizeof(int) * kBins * static_cast<size_t>(p.tiles));
+  p.totals = take(sizeof(int) * kBins);
+  p.head = take(sizeof(float) * p.workers * C);
+  p.tail = take(sizeof(float) * p.workers * C);
+  p.head_token = take(sizeof(int) * p.workers);
+  p.bytes = at;
+  return p;
+}
+
+int launched(const char* what) {
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? 0 : fail(BPC_ERR_LAUNCH, std::string(what) + " launch: " + cudaGetErrorString(e));
+}
+
+template <typename I, typename TW, typename TY>
+int lookup_launch(const void* ids, const void* w, void* y, int64_t n, int V, int C, int64_t ldw, float scale,
+                  cudaStream_t s) {
+  constexpr int kVec = 16 / (sizeof(TW) > sizeof(TY) ? sizeof(TW) : sizeof(TY));
+  const bool wide = C % kVec == 0 && ldw % kVec == 0 && reinterpret_cast<uintptr_t>(w) % (kVec * sizeof(TW)) == 0 &&
+                    reinterpret_cast<uintptr_t>(y) % (kVec * sizeof(TY)) == 0;
+  const int CV = wide ? C / kVec : C;
+  const int64_t units = n * CV;
+  const int grid = static_cast<int>(std::min<int64_t>((units + 255) / 256, static_cast<int64_t>(num_sms()) * 8));
+  if (wide)
+    embed_lookup_kernel<I, TW, TY, kVec><<<grid, 256, 0, s>>>(static_cast<const I*>(ids), static_cast<const TW*>(w),
+                                                              static_cast<TY*>(y), units, V, CV, ldw, scale);
+  else
+    embed_lookup_kernel<I, TW, TY, 1><<<grid, 256, 0, s>>>(static_cast<const I*>(ids), static_cast<const TW*>(w),
+                                                           static_cast<TY*>(y), units, V, CV, ldw, scale);
+  return launched("embed_lookup_kernel");
+}
+
+template <typename I, typename TW>
+int lookup_by_y(const void* ids, const void* w, void* y, int64_t n, int V, int C, int64_t ldw, float scale,
+                int32_t y_dtype, cudaStream_t s) {
+  if (y_dtype == BPC_DTYPE_F32) return lookup_launch<I, TW, float>(ids, w, y, n, V, C, ldw, scale, s);
+  if (y_dtype == BPC_DTYPE_BF16) return lookup_launch<I, TW, __nv_bfloat16>(ids, w, y, n, V, C, ldw, scale, s);
+  return lookup_launch<I, TW, __half>(ids, w, y, n, V, C, ldw, scale, s);
+}
+
+template <typename I>
+int lookup_by_w(const void* ids, const void* w, void* y, int64_t n, int V, int C, int64_t ldw, float scale,
+                int32_t w_dtype, int32_t y_dtype, cudaStream_t s) {
+  if (w_dtype == BPC_DTYPE_F32) return lookup_by_y<I, float>(ids, w, y, n, V, C, ldw, scale, y_dtype, s);
+  if (w_dtype == BPC_DTYPE_BF16) return lookup_by_y<I, __nv_bfloat16>(ids, w, y, n, V, C, ldw, scale, y_dtype, s);
+  return lookup_by_y<I, __half>(ids, w, y, n, V, C, ldw, scale, y_dtype, s);
+}
+
+template <typename I>
+int sort_pass(const I* src, const int* perm_in, int64_t n, int V, int shift, int tiles, int* counts, int* totals,
+              int* key_out, int* perm_out, cudaStream_t s) {
+  sort_count_kernel<I><<<tiles, kSortThreads, 0, s>>>(src, n, V, shift, counts, tiles);
+  if (int e = launched("sort_count_kernel")) return e;
+  sort_scan_kernel<<<kBins, 256, 0, s>>>(counts, totals, tiles);
+  if (int e = launched("sort_scan_kernel")) return e;
+  sort_place_kernel<I><<<tiles, kSortThreads, 0, s>>>(src, perm_in, n, V, shift, counts, totals, tiles, key_out,
+                                                      perm_out);
+  return launched("sort_place_kernel");
+}
+
+template <typename T>
+int merge_launch(const void* gy, MergeArgs a, cudaStream_t s) {
+  constexpr int kVec = 16 / sizeof(T);
+  const bool wide = a.C % kVec == 0 && a.ldg % kVec == 0 && reinterpret_cast<uintptr_t>(gy) % 16 == 0 &&
+                    reinterpret_cast<uintptr_t>(a.dw) % 16 == 0;
+  const int vec = wide ? kVec : 1;
+  const int64_t blocks = (a.workers + 256 / a.G - 1) / (256 / a.G);
+  const dim3 grid(static_cast<unsigned>(blocks), (a.C + a.G * vec - 1) / (a.G * vec));
+  if (wide)
+    wgrad_merge_kernel<T, kVec><<<grid, 256, 0, s>>>(static_cast<const T*>(gy), a);
+  else
+    wgrad_merge_kernel<T, 1><<<grid, 256, 0, s>>>(static_cast<const T*>(gy), a);
+  if (int e = launched("wgrad_merge_kernel")) return e;
+  wgrad_join_kernel<<<static_cast<unsigned>(a.workers), 256, 0, s>>>(a);
+  return launched("wgrad_join_kernel");
+}
+
+int embed_check(const void* ids, int32_t id_bytes, int64_t n, int32_t V, int32_t C, int64_t stride, int32_t in_dtype,
+                int32_t out_dtype) {
+  if (n < 0 || n > 0x7fffffffLL || V < 1 || V > 0x7ffffffe || C < 1 || C > (1 << 20))
+    return fail(BPC_ERR_ARG, "0 <= n < 2^31 positions, 1 <= V < 2^31 - 1 tokens, 1 <= C <= 2^20 channels");
+  if (id_bytes != 4 && id_bytes != 8) return fail(BPC_ERR_ARG, "ids must be int32 or int64 (id_bytes 4 or 8)");
+  if (!dtype_size(in_dtype) || !dtype_size(out_dtype)) return fail(BPC_ERR_ARG, "dtype must be f32, bf16 or f16");
+  if (stride < C) return fail(BPC_ERR_ARG, "row stride smaller than the channel count");
+  if (reinterpret_cast<uintptr_t>(ids) % id_bytes) return fail(BPC_ERR_ARG, "ids are not aligned to their type");
+  return 0;
+}
+
+}  // namespace
+
+}  // namespace bpc
+
+using namespace bpc;
+
+extern "C" int bpc_embed_lookup(const void* ids, int32_t id_bytes, const void* w, void* y, int64_t n, int32_t V,
+                                int32_t C, int64_t w_stride, float scale, int32_t w_dtype, int32_t y_dtype,
+                                bpc_stream_t stream) {
+  if (int e = embed_check(ids, id_bytes, n, V, C, w_stride, w_dtype, y_dtype)) return e;
+  if (n == 0) return 0;
+  if (!ids || !w || !y) return fail(BPC_ERR_ARG, "null buffer");
+  if (reinterpret_cast<uintptr_t>(w) % dtype_size(w_dtype) || reinterpret_cast<uintptr_t>(y) % dtype_size(y_dtype))
+    return fail(BPC_ERR_ARG, "w and y must be aligned to their types");
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (id_bytes == 8) return lookup_by_w<int64_t>(ids, w, y, n, V, C, w_stride, scale, w_dtype, y_dtype, s);
+  return lookup_by_w<int32_t>(ids, w, y, n, V, C, w_stride, scale, w_dtype, y_dtype, s);
+}
+
+extern "C" size_t bpc_embed_wgrad_workspace_size(int64_t n, int32_t V, int32_t C) {
+  if (n < 1 || n > 0x7fffffffLL || V < 1 || V > 0x7ffffffe || C < 1 || C > (1 << 20)) return 0;
+  return wgrad_plan(n, V, C).bytes;
+}
+
+extern "C" int bpc_embed_wgrad(const void* gy, const void* ids, int32_t id_bytes, void* dw, void* workspace,
+                               size_t workspace_bytes, int64_t n, int32_t V, int32_t C, int64_t gy_stride, float scale,
+                               int32_t gy_dtype, int32_t dw_dtype, bpc_stream_t stream) {
+  if (int e = embed_check(ids, id_bytes, n, V, C, gy_stride, gy_dtype, dw_dtype)) return e;
+  if (!dw) return fail(BPC_ERR_ARG, "null dw");
+  if (reinterpret_cast<uintptr_t>(dw) % dtype_size(dw_dtype)) return fail(BPC_ERR_ARG, "dw must be aligned to its type");
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (n == 0) {
+    cudaError_t e = cudaMemsetAsync(dw, 0, static_cast<size_t>(V) * C * dtype_size(dw_dtype), s);
+    return e == cudaSuccess ? 0 : fail(BPC_ERR_LAUNCH, std::string("cudaMemsetAsync: ") + cudaGetErrorString(e));
+  }
+  if (!gy || !ids || !workspace) return fail(BPC_ERR_ARG, "null buffer");
+  if (reinterpret_cast<uintptr_t>(gy) % dtype_size(gy_dtype)) return fail(BPC_ERR_ARG, "gy must be aligned to its type");
+  if (reinterpret_cast<uintptr_t>(workspace) & 15) return fail(BPC_ERR_ARG, "the workspace must be 16-byte aligned");
+  const WgradPlan p = wgrad_plan(n, V, C);
+  if (workspace_bytes < p.bytes) return fail(BPC_ERR_SPACE, "embedding gradient workspace too small");
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  int* key[2] = {reinterpret_cast<int*>(ws + p.key[0]), reinterpret_cast<int*>(ws + p.key[1])};
+  int* perm[2] = {reinterpret_cast<int*>(ws + p.perm[0]), reinterpret_cast<int*>(ws + p.perm[1])};
+  int* counts = reinterpret_cast<int*>(ws + p.counts);
+  int* totals = reinterpret_cast<int*>(ws + p.totals);
+  for (int k = 0; k < p.passes; ++k) {
+    int e;
+    if (k == 0 && id_bytes == 8)
+      e = sort_pass(static_cast<const int64_t*>(ids), nullptr, n, V, 0, p.tiles, counts, totals, key[0], perm[0], s);
+    else if (k == 0)
+      e = sort_pass(static_cast<const int32_t*>(ids), nullptr, n, V, 0, p.tiles, counts, totals, key[0], perm[0], s);
+    else
+      e = sort_pass(static_cast<const int*>(key[(k - 1) & 1]), perm[(k - 1) & 1], n, V, k * kDigitBits, p.tiles, counts,
+                    totals, key[k & 1], perm[k & 1], s);
+    if (e) return e;
+  }
+  MergeArgs a;
+  a.key = key[(p.passes - 1) & 1];
+  a.perm = perm[(p.passes - 1) & 1];
+  a.n = n;
+  a.items = p.items;
+  a.workers = p.workers;
+  a.V = V;
+  a.C = C;
+  a.G = p.G;
+  a.ldg = gy_stride;
+  a.scale = scale;
+  a.dw = dw;
+  a.dw_dtype = dw_dtype;
+  a.head = reinterpret_cast<float*>(ws + p.head);
+  a.tail = reinterpret_cast<float*>(ws + p.tail);
+  a.head_token = reinterpret_cast<int*>(ws + p.head_token);
+  if (gy_dtype == BPC_DTYPE_F32) return merge_launch<float>(gy, a, s);
+  if (gy_dtype == BPC_DTYPE_BF16) return merge_launch<__nv_bfloat16>(gy, a, s);
+  return merge_launch<__half>(gy, a, s);
+}

@@ -33,7 +33,8 @@ enum {
   BPC_ERR_SPACE = 6     /* the workspace is smaller than bpc_predecoder_workspace_size() */
 };
 
-enum { BPC_DTYPE_F32 = 0, BPC_DTYPE_BF16 = 1 };
+/* BPC_DTYPE_F16: the embedding lookup, its gradient and the gradient norm only. */
+enum { BPC_DTYPE_F32 = 0, BPC_DTYPE_BF16 = 1, BPC_DTYPE_F16 = 2 };
 
 /* Library version, (major << 16) | minor. */
 BPC_API int bpc_version(void);
@@ -135,6 +136,39 @@ BPC_API size_t bpc_embed_tokens_bwd_workspace_size(int32_t C);
 BPC_API int bpc_embed_tokens_bwd(const uint8_t* det, const uint8_t* check_type, const float* g, const void* g_bf16,
                                  float* dE, void* workspace, size_t workspace_bytes, int64_t B, int32_t N, int32_t C,
                                  bpc_stream_t stream);
+
+/* Token embedding with any number of tokens (the Cascade network's stem, nn.Embedding of cascade_net.py:279-285, and
+ * any larger table), forward and weight gradient:
+ *   bpc_embed_lookup  y[i, :] = scale W[ids[i], :], a zero row where ids[i] is outside [0, V)
+ *   bpc_embed_wgrad   dW[v, :] = scale sum over i with ids[i] = v of gy[i, :]; ids outside [0, V) contribute nothing,
+ *                     tokens without a row get zeros
+ * ids (n) int32 or int64 (id_bytes 4 or 8); W (V, C) with rows w_stride elements apart, y (n, C); gy (n, C) with rows
+ * gy_stride elements apart, dW (V, C).  Each of W, y, gy, dW is f32, bf16 or f16; products and sums are fp32, rounded
+ * once.  The gradient sorts the positions by token and adds each token's rows in a fixed order (deterministic); its
+ * workspace holds the sorted positions and partial sums, bpc_embed_wgrad_workspace_size(n, V, C) bytes on the current
+ * device, 16-byte aligned.  n < 2^31, V < 2^31 - 1, C <= 2^20; every buffer aligned to its type. */
+BPC_API int bpc_embed_lookup(const void* ids, int32_t id_bytes, const void* w, void* y, int64_t n, int32_t V, int32_t C,
+                             int64_t w_stride, float scale, int32_t w_dtype, int32_t y_dtype, bpc_stream_t stream);
+BPC_API size_t bpc_embed_wgrad_workspace_size(int64_t n, int32_t V, int32_t C);
+BPC_API int bpc_embed_wgrad(const void* gy, const void* ids, int32_t id_bytes, void* dw, void* workspace,
+                            size_t workspace_bytes, int64_t n, int32_t V, int32_t C, int64_t gy_stride, float scale,
+                            int32_t gy_dtype, int32_t dw_dtype, bpc_stream_t stream);
+
+/* The 2-norm over every element of a list of n tensors, and clipping the list by it (the gradient clipping of the
+ * reference's training step, cascade_train.py:292-320):
+ *   bpc_grad_norm   *norm = sqrt(sum_t sum_i g_t[i]^2)
+ *   bpc_clip_grads  the same, and out_t[i] = g_t[i] min(1, max_norm / (norm + 1e-6)); out[t] may be tensors[t] (in place)
+ * tensors, out, numel, dtype, out_dtype: host arrays of n entries, read during the call; numel[t] contiguous elements
+ * of f32, bf16 or f16 each, aligned to the type (no wider alignment needed); outputs must not overlap another tensor of
+ * the list.  norm: one fp32 on the device.  Squares and the sum are fp64, in a fixed order.  An infinite norm scales by
+ * zero (an infinite element becomes NaN), a NaN norm makes every output NaN.  max_norm >= 0.  workspace:
+ * bpc_grad_norm_workspace_size(n) bytes on the current device, 8-byte aligned. */
+BPC_API size_t bpc_grad_norm_workspace_size(int32_t n);
+BPC_API int bpc_grad_norm(const void* const* tensors, const int64_t* numel, const int32_t* dtype, int32_t n, float* norm,
+                          void* workspace, size_t workspace_bytes, bpc_stream_t stream);
+BPC_API int bpc_clip_grads(const void* const* tensors, void* const* out, const int64_t* numel, const int32_t* dtype,
+                           const int32_t* out_dtype, int32_t n, double max_norm, float* norm, void* workspace,
+                           size_t workspace_bytes, bpc_stream_t stream);
 
 /* The training network's X/Z head and its loss, one pass each way (the head linear(h_d, W, b) under bf16 autocast and
  * the mean BCE-with-logits of the reference's training step, cascade_train.py:292-320):
