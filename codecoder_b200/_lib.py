@@ -98,6 +98,7 @@ SIGNATURES = {
 }
 
 _lib = None
+_torch = None
 
 
 def lib() -> ctypes.CDLL:
@@ -113,6 +114,25 @@ def lib() -> ctypes.CDLL:
             f.argtypes = args
         _lib = L
     return _lib
+
+
+def torch_ops():
+    """The host side of the embedding and gradient-norm operators (csrc/torch_ops.cpp), bound to lib()'s entry points."""
+    global _torch
+    if _torch is None:
+        path = os.path.join(_PKG, "_torch_ops.so")
+        if not os.path.exists(path):
+            raise RuntimeError(f"{path} is missing: build it with `python -m codecoder_b200.build`")
+        import importlib.util
+
+        import torch  # noqa: F401  (its libraries must be loaded first)
+        spec = importlib.util.spec_from_file_location("_torch_ops", path)
+        m = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(m)
+        L = lib()
+        m.bind({name: ctypes.cast(getattr(L, name), c_vp).value for name in SIGNATURES})
+        _torch = m
+    return _torch
 
 
 def last_error() -> str:

@@ -1,10 +1,11 @@
-"""Build libbpc.so (the C-ABI library with every CUDA kernel) in-tree for sm_100a.
+"""Build libbpc.so (the C-ABI library with every CUDA kernel) in-tree for sm_100a, and _torch_ops.so beside it.
 
     python -m codecoder_b200.build            # or __graft_entry__.build()
 
 Each csrc/*.cu is compiled by nvcc with -gencode arch=compute_100a,code=sm_100a into _build/, then linked into
 codecoder_b200/libbpc.so with the static CUDA runtime, so the library loads on a machine without a GPU (the driver is
-only opened on first use)."""
+only opened on first use).  csrc/torch_ops.cpp, the host side of the embedding and gradient-norm operators on torch
+tensors, is compiled by g++ against the installed torch into codecoder_b200/_torch_ops.so."""
 from __future__ import annotations
 
 import concurrent.futures as cf
@@ -17,6 +18,8 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 REPO = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 OUT = os.path.join(PKG, "libbpc.so")
+TORCH_SRC = os.path.join(CSRC, "torch_ops.cpp")
+TORCH_OUT = os.path.join(PKG, "_torch_ops.so")
 BUILD = os.path.join(REPO, "_build")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -35,41 +38,73 @@ def sources() -> list[str]:
     return sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".cu"))
 
 
+def _header() -> str:
+    return os.path.join(REPO, "include", "bpc.h")
+
+
+def _older(out: str, deps: list[str]) -> bool:
+    return not os.path.exists(out) or any(os.path.getmtime(d) > os.path.getmtime(out) for d in deps if os.path.exists(d))
+
+
 def _needs_build() -> bool:
-    if not os.path.exists(OUT):
-        return True
-    t = os.path.getmtime(OUT)
-    deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)] + [os.path.join(REPO, "include", "bpc.h")]
-    return any(os.path.getmtime(d) > t for d in deps if os.path.exists(d))
+    return _older(OUT, [os.path.join(CSRC, f) for f in os.listdir(CSRC) if not f.endswith(".cpp")] + [_header()])
 
 
-def build(force: bool = False, verbose: bool = False) -> str:
-    if not force and not _needs_build():
-        return OUT
+def _run(cmd: list[str], what: str) -> str:
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{what} failed:\n{r.stdout}\n{r.stderr}")
+    return r.stderr
+
+
+def build_torch_ops() -> str:
+    """Compile csrc/torch_ops.cpp against the headers and libraries of the installed torch: with g++, the compiler nvcc
+    uses, whatever $CXX says (another one may bring its own C++ runtime into the process)."""
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(os.path.abspath(torch.__file__))
+    inc = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           sysconfig.get_paths()["include"], os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include"),
+           os.path.join(REPO, "include")]
+    tmp = TORCH_OUT + ".tmp"
+    _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+          "-DTORCH_EXTENSION_NAME=_torch_ops", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+          *[f"-isystem{d}" for d in inc], TORCH_SRC, "-o", tmp, "-L", os.path.join(root, "lib"), "-lc10", "-lc10_cuda",
+          "-ltorch_cpu", "-ltorch_python"], f"g++ on {TORCH_SRC}")
+    os.replace(tmp, TORCH_OUT)
+    return TORCH_OUT
+
+
+def build_lib(verbose: bool = False) -> str:
     os.makedirs(BUILD, exist_ok=True)
     cc = nvcc()
-    objs = []
 
     def one(src):
         obj = os.path.join(BUILD, os.path.basename(src)[:-3] + ".o")
         cmd = [cc, *ARCH, *FLAGS, "-c", src, "-o", obj]
         if verbose:
             cmd.insert(1, "-Xptxas=-v")
-        r = subprocess.run(cmd, capture_output=True, text=True)
-        if r.returncode != 0:
-            raise RuntimeError(f"nvcc failed on {src}:\n{r.stdout}\n{r.stderr}")
+        err = _run(cmd, f"nvcc on {src}")
         if verbose:
-            sys.stderr.write(r.stderr)
+            sys.stderr.write(err)
         return obj
 
     with cf.ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as ex:
         objs = list(ex.map(one, sources()))
     tmp = OUT + ".tmp"
-    cmd = [cc, *ARCH, "-shared", "-cudart", "static", "-o", tmp, *objs, "-lrt", "-ldl", "-lpthread"]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+    _run([cc, *ARCH, "-shared", "-cudart", "static", "-o", tmp, *objs, "-lrt", "-ldl", "-lpthread"], "link")
     os.replace(tmp, OUT)
+    return OUT
+
+
+def build(force: bool = False, verbose: bool = False) -> str:
+    with cf.ThreadPoolExecutor(max_workers=1) as ex:
+        host = ex.submit(build_torch_ops) if force or _older(TORCH_OUT, [TORCH_SRC, _header()]) else None
+        if force or _needs_build():
+            build_lib(verbose)
+        if host is not None:
+            host.result()
     return OUT
 
 

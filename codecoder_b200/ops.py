@@ -16,16 +16,11 @@ cascade_train.py:292-320).
 """
 from __future__ import annotations
 
-from array import array
-
 import torch
 
 from . import _lib
 
 _DTYPES = {torch.bfloat16: _lib.BPC_DTYPE_BF16, torch.float32: _lib.BPC_DTYPE_F32}
-# the embedding lookup, its gradient and the gradient norm also take fp16
-_FLOAT_DTYPES = {**_DTYPES, torch.float16: _lib.BPC_DTYPE_F16}
-_ID_BYTES = {torch.int32: 4, torch.int64: 8}
 
 
 # True: the fused steps' forward runs the op and its GELU / residual pass in one launch where the wide-tile kernel
@@ -529,56 +524,12 @@ class HeadBCEB200(torch.autograd.Function):
         return dh, dW.to(ctx.dtypes[0]), db.to(ctx.dtypes[1]), None
 
 
-def _on_device(device, fn, *args):
-    """fn(*args) with `device` current: the library takes the current device's SM count and launches there."""
-    if device.index == torch.cuda.current_device():
-        return fn(*args)
-    with torch.cuda.device(device):
-        return fn(*args)
-
-
-def _same_device(*ts):
-    _check_cuda(*ts)
-    if any(t.device != ts[0].device for t in ts):
-        raise ValueError("tensors are on different devices")
-
-
-def _row_view(t):
-    """A (rows, C) tensor and its row stride, without a copy where the channels are contiguous."""
-    rows, C = t.shape
-    if C > 1 and t.stride(1) != 1 or rows > 1 and t.stride(0) < C:
-        t = t.contiguous()
-    return t, t.stride(0) if rows > 1 else C
-
-
-def _check_embedding(ids, floats, out_dtype):
-    if ids.dtype not in _ID_BYTES:
-        raise TypeError(f"token ids must be int32 or int64, got {ids.dtype}")
-    if floats.dtype not in _FLOAT_DTYPES or out_dtype not in _FLOAT_DTYPES:
-        raise TypeError(f"embeddings are fp32, bf16 or fp16, got {floats.dtype} -> {out_dtype}")
-
-
 def embed_lookup(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
                  dtype: torch.dtype | None = None) -> torch.Tensor:
     """scale weight[ids] (C ABI bpc_embed_lookup): ids (...) int32 or int64, weight (V, C) fp32, bf16 or fp16 ->
     (..., C) in `dtype` (default: weight's), the product in fp32 and rounded once.  An id outside [0, V) reads a zero
     row, as gmm's idx does: -1 marks a padded position."""
-    _same_device(weight, ids)
-    dtype = weight.dtype if dtype is None else dtype
-    _check_embedding(ids, weight, dtype)
-    if weight.dim() != 2:
-        raise ValueError("embed_lookup: weight must be (V, C)")
-    V, C = weight.shape
-    y = torch.empty(*ids.shape, C, device=weight.device, dtype=dtype)
-    if y.numel() == 0:
-        return y
-    ids = ids.contiguous()
-    weight, ld = _row_view(weight)
-    rc = _on_device(weight.device, _lib.lib().bpc_embed_lookup, ids.data_ptr(), _ID_BYTES[ids.dtype],
-                    weight.data_ptr(), y.data_ptr(), ids.numel(), V, C, ld, float(scale), _FLOAT_DTYPES[weight.dtype],
-                    _FLOAT_DTYPES[dtype], _stream_ptr(weight.device))
-    _lib.check(rc, "bpc_embed_lookup")
-    return y
+    return _lib.torch_ops().embed_lookup(ids, weight, scale, dtype)
 
 
 def embed_wgrad(gy: torch.Tensor, ids: torch.Tensor, n_tokens: int, scale: float = 1.0,
@@ -586,27 +537,7 @@ def embed_wgrad(gy: torch.Tensor, ids: torch.Tensor, n_tokens: int, scale: float
     """The weight gradient of embed_lookup (C ABI bpc_embed_wgrad): gy (..., C), ids (...) -> dW (n_tokens, C) in
     `dtype`, dW[v] = scale sum over ids == v of gy, summed in fp32 in a fixed order (deterministic) and rounded once.
     Ids outside [0, n_tokens) contribute nothing; tokens that do not occur get zeros."""
-    _same_device(gy, ids)
-    _check_embedding(ids, gy, dtype)
-    if gy.dim() != ids.dim() + 1 or gy.shape[:-1] != ids.shape:
-        raise ValueError("embed_wgrad: gy must be ids' shape with the channels added")
-    V, C = int(n_tokens), gy.shape[-1]
-    dw = torch.empty(V, C, device=gy.device, dtype=dtype)
-    if C == 0:
-        return dw
-    n = ids.numel()
-    ids = ids.contiguous()
-    gy, ld = _row_view(gy.reshape(n, C))
-    return _on_device(gy.device, _embed_wgrad, gy, ld, ids, dw, n, V, C, float(scale))
-
-
-def _embed_wgrad(gy, ld, ids, dw, n, V, C, scale):
-    L = _lib.lib()
-    ws = torch.empty(int(L.bpc_embed_wgrad_workspace_size(n, V, C)), device=gy.device, dtype=torch.uint8)
-    rc = L.bpc_embed_wgrad(gy.data_ptr(), ids.data_ptr(), _ID_BYTES[ids.dtype], dw.data_ptr(), ws.data_ptr(), ws.numel(),
-                           n, V, C, ld, scale, _FLOAT_DTYPES[gy.dtype], _FLOAT_DTYPES[dw.dtype], _stream_ptr(gy.device))
-    _lib.check(rc, "bpc_embed_wgrad")
-    return dw
+    return _lib.torch_ops().embed_wgrad(gy, ids, n_tokens, scale, dtype)
 
 
 class EmbeddingB200(torch.autograd.Function):
@@ -634,71 +565,11 @@ def embedding(ids, weight, scale=1.0, dtype=None):
     return EmbeddingB200.apply(ids, weight, scale, dtype)
 
 
-def _is_dense(t) -> bool:
-    """Whether t's elements fill one run of memory in some order of its dimensions."""
-    want = 1
-    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
-        if stride != want:
-            return False
-        want *= size
-    return True
-
-
-def _tensor_list(what, ts):
-    """Host arrays (addresses, element counts, dtypes) of a list of dense tensors on one GPU."""
-    if not ts:
-        raise ValueError(f"{what} needs at least one tensor")
-    _check_cuda(ts[0])
-    dev = ts[0].get_device()
-    for t in ts:
-        if t.get_device() != dev:
-            raise ValueError(f"{what}: tensors are on different devices")
-        if not t.is_contiguous() and not _is_dense(t):
-            raise ValueError(f"{what}: a tensor with gaps or overlaps between its elements (strides {t.stride()})")
-    try:
-        dtypes = array("i", [_FLOAT_DTYPES[t.dtype] for t in ts])
-    except KeyError as e:
-        raise TypeError(f"{what} takes fp32, bf16 and fp16 tensors, got {e.args[0]}") from None
-    return (array("Q", map(torch.Tensor.data_ptr, ts)), array("q", map(torch.Tensor.numel, ts)), dtypes)
-
-
-def _addr(a):
-    return a.buffer_info()[0]
-
-
-def _mark_written(ts):
-    """Tell autograd that the kernels wrote these tensors (inference tensors have no version to count)."""
-    try:
-        torch.autograd.graph.increment_version(ts)
-    except RuntimeError:
-        for t in ts:
-            if not t.is_inference():
-                torch.autograd.graph.increment_version(t)
-
-
 def grad_norm(tensors) -> torch.Tensor:
     """The 2-norm over every element of a list of fp32, bf16 or fp16 tensors (C ABI bpc_grad_norm) as an fp32 scalar on
-    the device: squares and sum in fp64 in a fixed order.  Not differentiable."""
-    ts = list(tensors)
-    ptrs, numel, dtypes = _tensor_list("grad_norm", ts)
-    return _on_device(ts[0].device, _norm_call, ts[0].device, ptrs, numel, dtypes, None)
-
-
-def _norm_call(device, ptrs, numel, dtypes, clip):
-    L = _lib.lib()
-    n = len(ptrs)
-    ws = torch.empty(int(L.bpc_grad_norm_workspace_size(n)), device=device, dtype=torch.uint8)
-    norm = torch.empty((), device=device, dtype=torch.float32)
-    st = _stream_ptr(device)
-    if clip is None:
-        rc = L.bpc_grad_norm(_addr(ptrs), _addr(numel), _addr(dtypes), n, norm.data_ptr(), ws.data_ptr(), ws.numel(), st)
-        _lib.check(rc, "bpc_grad_norm")
-    else:
-        out_ptrs, out_dtypes, max_norm = clip
-        rc = L.bpc_clip_grads(_addr(ptrs), _addr(out_ptrs), _addr(numel), _addr(dtypes), _addr(out_dtypes), n, max_norm,
-                              norm.data_ptr(), ws.data_ptr(), ws.numel(), st)
-        _lib.check(rc, "bpc_clip_grads")
-    return norm
+    the device: squares and sum in fp64 in a fixed order.  Dense tensors only (any order of dimensions).  Not
+    differentiable."""
+    return _lib.torch_ops().grad_norm(tensors if type(tensors) is list else list(tensors))
 
 
 def clip_grads(tensors, max_norm: float, out=None) -> torch.Tensor:
@@ -707,23 +578,8 @@ def clip_grads(tensors, max_norm: float, out=None) -> torch.Tensor:
     into `out`: tensors of the same shapes and strides, each fp32, bf16 or fp16 (say the fp32 master gradients of bf16
     ones).  No output may share memory with another tensor of the list.  An infinite norm scales by zero, a NaN norm
     makes every gradient NaN, as torch.nn.utils.clip_grad_norm_ does."""
-    ts = list(tensors)
-    ptrs, numel, dtypes = _tensor_list("clip_grads", ts)
-    if out is None:
-        outs, out_ptrs, out_dtypes = ts, ptrs, dtypes
-    else:
-        outs = list(out)
-        if len(outs) != len(ts) or any(o.shape != t.shape for o, t in zip(outs, ts)):
-            raise ValueError("clip_grads: out must hold one tensor of the same shape per gradient")
-        out_ptrs, _, out_dtypes = _tensor_list("clip_grads", outs)
-        if outs[0].get_device() != ts[0].get_device():
-            raise ValueError("clip_grads: tensors are on different devices")
-        if any(o.stride() != t.stride() for o, t in zip(outs, ts) if not (o.is_contiguous() and t.is_contiguous())):
-            raise ValueError("clip_grads: out must have the gradients' strides")
-    norm = _on_device(ts[0].device, _norm_call, ts[0].device, ptrs, numel, dtypes,
-                      (out_ptrs, out_dtypes, float(max_norm)))
-    _mark_written(outs)
-    return norm
+    return _lib.torch_ops().clip_grads(tensors if type(tensors) is list else list(tensors), max_norm,
+                                       out if out is None or type(out) is list else list(out))
 
 
 def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:

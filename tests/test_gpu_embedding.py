@@ -290,5 +290,5 @@ def test_refusals():
         ops.embed_wgrad(gy.view(7, 4, 10), ids, 9)
     with pytest.raises(TypeError, match="fp32"):
         ops.embed_wgrad(gy.double(), ids, 9)
-    with pytest.raises(RuntimeError, match="tokens"):
+    with pytest.raises(ValueError, match="tokens"):
         ops.embed_wgrad(gy, ids, 0)

@@ -153,7 +153,7 @@ def test_refusals():
         ops.grad_norm([x[:, :20]])
     with pytest.raises(ValueError, match="gaps or overlaps"):
         ops.clip_grads([x[:, :1].expand(40, 50)], 1.0)
-    with pytest.raises(TypeError, match="float64"):
+    with pytest.raises(TypeError, match="takes dense"):
         ops.grad_norm([x, x.double()])
     with pytest.raises(ValueError, match="different devices"):
         ops.grad_norm([x, x.cpu()])

@@ -136,13 +136,3 @@ def test_python_refusals():
     with pytest.raises(ValueError, match="at least one"):
         ops.clip_grads(iter([]), 1.0)
     assert float(ops.clip_grad_norm_([torch.nn.Parameter(w)], 1.0)) == 0.0      # no gradients: nothing to do
-
-
-def test_dense_layouts_are_told_from_views_with_gaps():
-    x = torch.zeros(4, 6, 5)
-    for t in (x, x.transpose(0, 2), x[2], x[:, :1], x[1:3], x.new_zeros(7, 1).expand(7, 1), x.permute(1, 0, 2)):
-        want = t.is_contiguous() or t.transpose(0, -1).is_contiguous() or t.permute(*range(t.dim())).is_contiguous()
-        if want:
-            assert ops._is_dense(t)
-    assert ops._is_dense(x.permute(1, 0, 2)) and ops._is_dense(x.transpose(0, 2))
-    assert not ops._is_dense(x[:, :3]) and not ops._is_dense(x[..., ::2]) and not ops._is_dense(x[:, :1].expand(4, 6, 5))
