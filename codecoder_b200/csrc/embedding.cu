@@ -37,6 +37,22 @@ struct alignas(sizeof(T) * VEC) Pack {
   T v[VEC];
 };
 
+// a pack as one access of its whole size
+template <int BYTES>
+struct Word;
+template <> struct Word<16> { typedef uint4 type; };
+template <> struct Word<8> { typedef uint2 type; };
+template <> struct Word<4> { typedef uint32_t type; };
+template <> struct Word<2> { typedef uint16_t type; };
+
+template <typename P>
+__device__ __forceinline__ P load_pack(const void* p) {
+  const auto w = *static_cast<const typename Word<sizeof(P)>::type*>(p);
+  P x;
+  memcpy(&x, &w, sizeof(P));
+  return x;
+}
+
 // ---------------------------------------------------------------------------------------------------------------
 // lookup: one thread per VEC channels of a row
 template <typename I, typename TW, typename TY, int VEC>
@@ -337,6 +353,220 @@ __global__ void __launch_bounds__(256) wgrad_join_kernel(MergeArgs a) {
   }
 }
 
+// ---------------------------------------------------------------------------------------------------------------
+// Few tokens (V <= kFewTokens; the detector tokens of this library's networks are 4 or 5): no sort.  The rows are read
+// once in their own order.  A ninth warp copies them ahead into a ring of shared memory (bulk copies: the bytes in
+// flight depend neither on registers nor on the load units).  The threads of the other eight lie along a row's pieces
+// of VEC channels and several rows; each keeps one sum per token in registers and adds its piece under one predicate per
+// token.  A block adds its threads' sums in order, wgrad_few_join_kernel the blocks' in fp64.
+constexpr int kFewTokens = 8;
+constexpr int kFewThreads = 256;                          // that add
+constexpr int kFewStages = 4;                             // of 64 bytes per adding thread: 64 KB
+constexpr int kFewBlocksPerSm = 3;
+constexpr uint64_t kFewTimeoutNs = 2000000000ull;         // bound of every wait
+
+enum FewMode : int {
+  kFewWhole = 0,       // a stage's rows are one run of memory: one bulk copy
+  kFewRows = 1,        // one per row (16-byte pieces at a row stride, or a slice of the channels)
+  kFewDirect = 2,      // not aligned for bulk copies: the rows are read from global memory
+};
+
+struct FewPlan {
+  int vec, mode;
+  int pieces;          // of vec channels per row and slice
+  int rows_at_once;    // kFewThreads / pieces
+  int slices;          // of the channels (gridDim.y)
+  int batch;           // rows of a stage
+  uint32_t pitch;      // bytes from row to row in shared memory
+  int64_t blocks, rows_per_block;
+};
+
+struct FewArgs {
+  FewPlan p;
+  const void* gy;
+  const void* ids;
+  int id_bytes;
+  int64_t n, ldg;
+  int V, C;
+  float scale;
+  void* dw;
+  int dw_dtype;
+  float* partial;      // (gridDim.x, V, C), unused when one block covers the rows
+  int* status;         // watchdog word of the op entry points
+};
+
+__device__ __forceinline__ int small_token(const int32_t* p) { return __ldg(p); }
+__device__ __forceinline__ int small_token(const int64_t* p) {
+  const int2 w = __ldg(reinterpret_cast<const int2*>(p));
+  return w.y == 0 ? w.x : -1;                              // an id that does not fit 32 bits is none
+}
+
+template <int VEC>
+__device__ __forceinline__ void add_if(float (&s)[VEC], const float (&x)[VEC], int t, int v) {
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) s[e] = t == v ? s[e] + x[e] : s[e];
+}
+
+template <typename T, typename I, int VEC, int NV>
+__global__ void __launch_bounds__(kFewThreads + 32) wgrad_few_kernel(const __grid_constant__ FewArgs a) {
+  extern __shared__ uint4 few_smem_base[];
+  __shared__ __align__(8) uint64_t full[kFewStages], empty[kFewStages];
+  __shared__ int abort;
+  typedef Pack<T, VEC> Piece;
+  constexpr int kRows = 64 / sizeof(Piece);                // rows per thread and stage
+  constexpr int kAhead = 4;                                // rows whose tokens are read ahead
+  const FewPlan& p = a.p;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t r0 = blockIdx.x * p.rows_per_block;
+  const int rows = static_cast<int>(min(a.n - r0, p.rows_per_block));
+  const int c0 = blockIdx.y * p.pieces * VEC;
+  const int width = min(p.pieces * VEC, a.C - c0);         // channels of this slice
+  const T* gp = static_cast<const T*>(a.gy) + r0 * a.ldg + c0;
+  const int TY = p.rows_at_once, batch = kRows * TY;
+  const int copied = p.mode == kFewDirect ? 0 : rows / batch;          // the stages that pass through the ring
+  volatile int* gave_up = &abort;
+  if (tid == 0) {
+    abort = 0;
+    for (int k = 0; k < kFewStages; ++k) {
+      mbar_init(smem_u32(&full[k]), 1);
+      mbar_init(smem_u32(&empty[k]), kFewThreads / 32);
+    }
+    fence_mbar_init();
+  }
+  __syncthreads();
+  if (warp == kFewThreads / 32) {
+    const uint32_t ring = smem_u32(few_smem_base), row_bytes = width * sizeof(T);
+    for (int k = 0; k < copied; ++k) {
+      const int q = k % kFewStages;
+      if (k >= kFewStages && !mbar_wait(smem_u32(&empty[q]), (k / kFewStages - 1) & 1, gave_up, a.status, kFewTimeoutNs))
+        break;
+      __syncwarp();
+      const uint32_t dst = ring + q * batch * p.pitch, bar = smem_u32(&full[q]);
+      const T* src = gp + static_cast<int64_t>(k) * batch * a.ldg;
+      if (lane == 0) mbar_arrive_expect_tx(bar, batch * row_bytes);
+      __syncwarp();
+      if (p.mode == kFewWhole) {
+        if (lane == 0) bulk_load(dst, src, batch * row_bytes, bar);
+      } else {
+        for (int r = lane; r < batch; r += 32) bulk_load(dst + r * p.pitch, src + r * a.ldg, row_bytes, bar);
+      }
+    }
+    __syncthreads();
+    // after a wait that ran out: copies under way still write this block's memory, give them as long again
+    if (abort && lane == 0) {
+      volatile int never = 0;
+      for (int q = 0; q < kFewStages && q < copied; ++q)
+        mbar_wait(smem_u32(&full[q]), ((copied - 1 - q) / kFewStages) & 1, &never, nullptr, kFewTimeoutNs);
+    }
+    __syncthreads();
+    return;
+  }
+
+  float s[NV][VEC];
+#pragma unroll
+  for (int v = 0; v < NV; ++v)
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) s[v][e] = 0.f;
+  const int x = tid % p.pieces, y = tid / p.pieces;
+  const bool on = y < TY && x * VEC < width;
+  const auto add = [&](const Piece piece, int t) {         // a token of V or more meets no sum that is read
+    float f[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) f[e] = to_f32(piece.v[e]);
+#pragma unroll
+    for (int v = 0; v < NV; ++v) add_if(s[v], f, t, v);
+  };
+  const I* idp = static_cast<const I*>(a.ids) + r0 + (on ? y : 0);
+  int next[kAhead];                                        // the tokens of this thread's next rows
+  const auto tokens = [&](int r) {                         // rows r, r + TY .. of this thread's stages: all in range
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) next[u] = small_token(idp + (r + u * TY));
+  };
+  const char* const mine = reinterpret_cast<const char*>(few_smem_base) + y * p.pitch + x * sizeof(Piece);
+  const uint32_t row_step = TY * p.pitch, stage_step = batch * p.pitch;
+  if (copied) tokens(0);
+  uint32_t q = 0, parity = 0;
+  for (int k = 0; k < copied; ++k) {
+    if (!mbar_wait(smem_u32(&full[q]), parity, gave_up, a.status, kFewTimeoutNs)) break;
+    const char* at = mine + q * stage_step;
+#pragma unroll
+    for (int j = 0; j < kRows; j += kAhead) {
+      int t[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) t[u] = next[u];
+      if (j + kAhead < kRows || k + 1 < copied) tokens((j + kAhead) * TY);
+      if (on) {
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) add(load_pack<Piece>(at + (j + u) * row_step), t[u]);
+      }
+    }
+    idp += batch;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&empty[q]));
+    if (++q == kFewStages) {
+      q = 0;
+      parity ^= 1;
+    }
+  }
+  if (on) {                                                // what does not fill a stage
+    for (int r = copied * batch + y; r < rows; r += TY)
+      add(load_pack<Piece>(gp + static_cast<int64_t>(r) * a.ldg + x * VEC),
+          small_token(static_cast<const I*>(a.ids) + r0 + r));
+  }
+  __syncthreads();                                         // the ring is read: its memory takes the sums
+  __syncthreads();
+  float* sums = reinterpret_cast<float*>(few_smem_base);   // (V, VEC, kFewThreads)
+#pragma unroll
+  for (int v = 0; v < NV; ++v)
+    if (v < a.V)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) sums[(v * VEC + e) * kFewThreads + tid] = s[v][e];
+  asm volatile("bar.sync 1, %0;" ::"n"(kFewThreads) : "memory");            // the eight warps that add
+  for (int i = tid; i < a.V * p.pieces; i += kFewThreads) {
+    const int v = i / p.pieces, xx = i - v * p.pieces;
+    if (xx * VEC >= width) continue;
+    float o[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const float* q = sums + (v * VEC + e) * kFewThreads + xx;
+      o[e] = 0.f;
+      for (int yy = 0; yy < p.rows_at_once; ++yy) o[e] += q[yy * p.pieces];
+    }
+    const int cc = c0 + xx * VEC;
+    if (gridDim.x == 1) {
+      store_row<VEC>(a.dw, a.dw_dtype, static_cast<int64_t>(v) * a.C + cc, o, a.scale);
+    } else {
+      float* out = a.partial + (static_cast<int64_t>(blockIdx.x) * a.V + v) * a.C + cc;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) out[e] = o[e];
+    }
+  }
+}
+
+// 32 sums a block, its warps each a fixed share of the blocks' partial sums, in fp64
+__global__ void __launch_bounds__(1024) wgrad_few_join_kernel(const float* __restrict__ partial, int blocks, int n,
+                                                              float scale, void* dw, int dw_dtype) {
+  __shared__ double red[32][33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int i = blockIdx.x * 32 + lane;
+  double s = 0.0;
+  if (i < n) {
+#pragma unroll 8
+    for (int b = warp; b < blocks; b += 32) s += partial[static_cast<int64_t>(b) * n + i];
+  }
+  red[warp][lane] = s;
+  __syncthreads();
+  // transposed: warp w now holds the 32 shares of sum w
+  s = red[lane][warp];
+#pragma unroll
+  for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+  const int o = blockIdx.x * 32 + warp;
+  if (lane == 0 && o < n) {
+    const float f = static_cast<float>(s);
+    store_row<1>(dw, dw_dtype, o, &f, scale);
+  }
+}
+
 int dtype_size(int32_t dtype) { return dtype == BPC_DTYPE_F32 ? 4 : dtype == BPC_DTYPE_BF16 || dtype == BPC_DTYPE_F16 ? 2 : 0; }
 
 // Workspace layout of the gradient
@@ -345,6 +575,47 @@ struct WgradPlan {
   int64_t items, workers;
   size_t key[2], perm[2], counts, totals, head, tail, head_token, bytes;
 };
+
+// Few tokens: how a block reads its rows, by alignment and row length.
+FewPlan few_plan(const void* gy, const void* dw, int64_t n, int C, int64_t ldg, int size) {
+  FewPlan p;
+  const auto fits = [&](int vec) {
+    return C % vec == 0 && ldg % vec == 0 && reinterpret_cast<uintptr_t>(gy) % (vec * size) == 0 &&
+           reinterpret_cast<uintptr_t>(dw) % 16 == 0;
+  };
+  p.vec = 16 / size;
+  while (p.vec > 1 && !fits(p.vec)) p.vec /= 2;
+  const int units = (C + p.vec - 1) / p.vec;
+  p.slices = (units + kFewThreads - 1) / kFewThreads;
+  p.pieces = (units + p.slices - 1) / p.slices;
+  p.rows_at_once = kFewThreads / p.pieces;
+  p.pitch = static_cast<uint32_t>(p.pieces) * p.vec * size;
+  // 64 bytes per thread and stage: narrower pieces take more rows, so that every whole stage begins on 16 bytes
+  p.batch = p.rows_at_once * (64 / (p.vec * size));
+  if (reinterpret_cast<uintptr_t>(gy) % 16) p.mode = kFewDirect;
+  else if (ldg == C && p.slices == 1) p.mode = kFewWhole;
+  else if (p.vec * size == 16) p.mode = kFewRows;
+  else p.mode = kFewDirect;
+  // a whole number of stages per block, unless there are too few rows to fill the GPU that way; at least 8 rows, and a
+  // multiple of 8, which begins on 16 bytes too
+  const int64_t most = std::max<int64_t>(1, kFewBlocksPerSm * num_sms() / p.slices);
+  int64_t per = (n + most - 1) / most;
+  if (per >= 2 * p.batch) per = (per + p.batch - 1) / p.batch * p.batch;
+  p.rows_per_block = (per + 7) / 8 * 8;
+  p.blocks = (n + p.rows_per_block - 1) / p.rows_per_block;
+  return p;
+}
+
+// the ring, or the block's sums after it
+int few_smem(const FewPlan& p, int V) {
+  const int ring = p.mode == kFewDirect ? 0 : static_cast<int>(kFewStages * p.batch * p.pitch);
+  return std::max(ring, V * kFewThreads * 4 * p.vec);
+}
+
+// the most blocks that few_plan cuts n rows into
+size_t few_bytes(int64_t n, int32_t V, int32_t C) {
+  return sizeof(float) * V * C * static_cast<size_t>(std::min<int64_t>((n + 7) / 8, kFewBlocksPerSm * static_cast<int64_t>(num_sms())));
+}
 
 WgradPlan wgrad_plan(int64_t n, int32_t V, int32_t C) {
   WgradPlan p;
@@ -445,6 +716,45 @@ int merge_launch(const void* gy, MergeArgs a, cudaStream_t s) {
   return launched("wgrad_join_kernel");
 }
 
+template <typename T, typename I, int VEC, int NV>
+int few_launch_tokens(const FewArgs& a, cudaStream_t s) {
+  const auto fn = wgrad_few_kernel<T, I, VEC, NV>;
+  const int smem = few_smem(a.p, a.V);
+  if (int e = allow_smem(reinterpret_cast<const void*>(fn), smem)) return e;
+  fn<<<dim3(static_cast<unsigned>(a.p.blocks), a.p.slices), kFewThreads + 32, smem, s>>>(a);
+  if (int e = launched("wgrad_few_kernel")) return e;
+  if (a.p.blocks == 1) return 0;
+  const int sums = a.V * a.C;
+  wgrad_few_join_kernel<<<(sums + 31) / 32, 1024, 0, s>>>(a.partial, static_cast<int>(a.p.blocks), sums, a.scale, a.dw,
+                                                          a.dw_dtype);
+  return launched("wgrad_few_join_kernel");
+}
+
+template <typename T, typename I, int VEC>
+int few_launch_ids(const FewArgs& a, cudaStream_t s) {
+  // a predicate and VEC additions per token and row: a kernel for the counts of the networks here, and the most
+  if (a.V <= 4) return few_launch_tokens<T, I, VEC, 4>(a, s);
+  if (a.V == 5) return few_launch_tokens<T, I, VEC, 5>(a, s);
+  return few_launch_tokens<T, I, VEC, kFewTokens>(a, s);
+}
+
+template <typename T, int VEC>
+int few_launch_vec(const FewArgs& a, cudaStream_t s) {
+  return a.id_bytes == 8 ? few_launch_ids<T, int64_t, VEC>(a, s) : few_launch_ids<T, int32_t, VEC>(a, s);
+}
+
+template <typename T>
+int few_launch(const FewArgs& a, cudaStream_t s) {
+  switch (a.p.vec) {
+    case 1: return few_launch_vec<T, 1>(a, s);
+    case 2: return few_launch_vec<T, 2>(a, s);
+    case 4: return few_launch_vec<T, 4>(a, s);
+    default:
+      if constexpr (sizeof(T) == 2) return few_launch_vec<T, 8>(a, s);
+      return fail(BPC_ERR_ARG, "no such vector width");
+  }
+}
+
 int embed_check(const void* ids, int32_t id_bytes, int64_t n, int32_t V, int32_t C, int64_t stride, int32_t in_dtype,
                 int32_t out_dtype) {
   if (n < 0 || n > 0x7fffffffLL || V < 1 || V > 0x7ffffffe || C < 1 || C > (1 << 20))
@@ -477,7 +787,7 @@ extern "C" int bpc_embed_lookup(const void* ids, int32_t id_bytes, const void* w
 
 extern "C" size_t bpc_embed_wgrad_workspace_size(int64_t n, int32_t V, int32_t C) {
   if (n < 1 || n > 0x7fffffffLL || V < 1 || V > 0x7ffffffe || C < 1 || C > (1 << 20)) return 0;
-  return wgrad_plan(n, V, C).bytes;
+  return V <= kFewTokens ? few_bytes(n, V, C) : wgrad_plan(n, V, C).bytes;
 }
 
 extern "C" int bpc_embed_wgrad(const void* gy, const void* ids, int32_t id_bytes, void* dw, void* workspace,
@@ -494,8 +804,29 @@ extern "C" int bpc_embed_wgrad(const void* gy, const void* ids, int32_t id_bytes
   if (!gy || !ids || !workspace) return fail(BPC_ERR_ARG, "null buffer");
   if (reinterpret_cast<uintptr_t>(gy) % dtype_size(gy_dtype)) return fail(BPC_ERR_ARG, "gy must be aligned to its type");
   if (reinterpret_cast<uintptr_t>(workspace) & 15) return fail(BPC_ERR_ARG, "the workspace must be 16-byte aligned");
+  if (workspace_bytes < bpc_embed_wgrad_workspace_size(n, V, C))
+    return fail(BPC_ERR_SPACE, "embedding gradient workspace too small");
+  if (V <= kFewTokens) {
+    FewArgs a;
+    a.p = few_plan(gy, dw, n, C, gy_stride, dtype_size(gy_dtype));
+    a.gy = gy;
+    a.ids = ids;
+    a.id_bytes = id_bytes;
+    a.n = n;
+    a.ldg = gy_stride;
+    a.V = V;
+    a.C = C;
+    a.scale = scale;
+    a.dw = dw;
+    a.dw_dtype = dw_dtype;
+    a.partial = static_cast<float*>(workspace);
+    a.status = op_status_ptr();
+    if (!a.status) return fail(BPC_ERR_LAUNCH, "cudaGetSymbolAddress(op status) failed");
+    if (gy_dtype == BPC_DTYPE_F32) return few_launch<float>(a, s);
+    if (gy_dtype == BPC_DTYPE_BF16) return few_launch<__nv_bfloat16>(a, s);
+    return few_launch<__half>(a, s);
+  }
   const WgradPlan p = wgrad_plan(n, V, C);
-  if (workspace_bytes < p.bytes) return fail(BPC_ERR_SPACE, "embedding gradient workspace too small");
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   int* key[2] = {reinterpret_cast<int*>(ws + p.key[0]), reinterpret_cast<int*>(ws + p.key[1])};
   int* perm[2] = {reinterpret_cast<int*>(ws + p.perm[0]), reinterpret_cast<int*>(ws + p.perm[1])};
