@@ -3,12 +3,14 @@
 //   norm = sqrt(sum_t sum_i g_t[i]^2);   out_t[i] = g_t[i] min(1, max_norm / (norm + 1e-6))
 //
 // The list travels in the launch's parameters (no copy to the device, so a captured call replays as it is).  Every
-// tensor is cut into chunks of kChunk elements and the chunks of the list are dealt to the blocks in equal runs, so a
+// tensor is cut into chunks of 16 KB and the chunks of the list are dealt to the blocks in equal runs, so a
 // list of many small tensors and one of few large ones load the GPU alike.  Squares and sums are fp64: a square of any
 // finite fp32 value neither overflows nor vanishes, and the sum's order is fixed (no atomics).
 #include <algorithm>
 #include <cmath>
+#include <cstring>
 #include <string>
+#include <type_traits>
 #include <vector>
 
 #include <cuda_fp16.h>
@@ -22,22 +24,20 @@ namespace bpc {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kChunk = 4096;              // elements
-constexpr int kListMax = 1000;            // tensors per launch: 32 bytes each, within the 32,764 bytes of parameters
+constexpr int kChunkBytes = 16384;        // of the input: kUnroll 16-byte loads per thread
+constexpr int kListMax = 1000;            // tensors per launch: 24 bytes each, within the 32,764 bytes of parameters
 constexpr int kBlocksPerSm = 8;
+constexpr int kUnroll = 4;
 
-struct Entry {
-  const void* in;
-  void* out;
-  int64_t numel;
-  int32_t first_chunk;                    // chunks of the list before this tensor
-  int16_t in_dtype, out_dtype;
-};
-
-template <int N>
+// A launch's tensors, of one type (and one output type): a kernel that branched over nine pairs of types spilled its
+// registers.  Tensor t has chunks [first[t], first[t + 1]), the last of last[t] elements.
+template <int N, bool OUT>
 struct List {
   int32_t n, chunks;
-  Entry e[N];
+  const void* in[N];
+  void* out[OUT ? N : 1];
+  int32_t first[N + 1];
+  uint32_t last[N];
 };
 
 __device__ __forceinline__ float load_f32(const float* p) { return *p; }
@@ -52,16 +52,28 @@ struct alignas(sizeof(T) * VEC) Pack {
   T v[VEC];
 };
 
-// the last entry whose chunks begin at or before chunk k
-template <int N>
-__device__ __forceinline__ int find_entry(const List<N>& list, int k) {
+// the tensor of chunk k
+template <typename L>
+__device__ __forceinline__ int find_tensor(const L& list, int k) {
   int lo = 0, hi = list.n - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (list.e[mid].first_chunk <= k) lo = mid;
+    if (list.first[mid] <= k) lo = mid;
     else hi = mid - 1;
   }
   return lo;
+}
+
+// chunk k of tensor t: its first element and its length
+struct Chunk {
+  int64_t at;
+  int len;
+};
+template <typename T, typename L>
+__device__ __forceinline__ Chunk chunk_of(const L& list, int t, int k) {
+  constexpr int kWhole = kChunkBytes / sizeof(T);
+  return {static_cast<int64_t>(k - list.first[t]) * kWhole,
+          k + 1 == list.first[t + 1] ? static_cast<int>(list.last[t]) : kWhole};
 }
 
 __device__ __forceinline__ double warp_sum(double v) {
@@ -99,14 +111,20 @@ __device__ __forceinline__ double chunk_squares(const T* __restrict__ p, int len
     const double x = load_f32(p + threadIdx.x);
     s = x * x;
   }
-  const Pack<T, VEC>* v = reinterpret_cast<const Pack<T, VEC>*>(p + peel);
-#pragma unroll 4
-  for (int i = threadIdx.x; i < nv; i += kThreads) {
-    const Pack<T, VEC> x = v[i];
+  const uint4* v = reinterpret_cast<const uint4*>(p + peel);
+  for (int i = threadIdx.x; i < nv; i += kThreads * kUnroll) {
+    uint4 w[kUnroll];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      const double d = load_f32(&x.v[e]);
-      s = fma(d, d, s);
+    for (int u = 0; u < kUnroll; ++u) w[u] = i + u * kThreads < nv ? __ldg(v + i + u * kThreads) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      Pack<T, VEC> x;
+      memcpy(&x, &w[u], 16);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const double d = load_f32(&x.v[e]);
+        s = fma(d, d, s);
+      }
     }
   }
   const int t = peel + nv * VEC + threadIdx.x;
@@ -117,21 +135,18 @@ __device__ __forceinline__ double chunk_squares(const T* __restrict__ p, int len
   return s;
 }
 
-template <int N>
-__global__ void __launch_bounds__(kThreads) norm_partial_kernel(const __grid_constant__ List<N> list, int per_block,
-                                                                double* __restrict__ partial) {
+template <typename T, int N>
+__global__ void __launch_bounds__(kThreads) norm_partial_kernel(const __grid_constant__ List<N, false> list,
+                                                                int per_block, double* __restrict__ partial) {
   __shared__ double red[kThreads / 32];
+  pdl_launch_dependents();
   const int k0 = blockIdx.x * per_block, k1 = min(list.chunks, k0 + per_block);
   double s = 0.0;
-  int t = k0 < k1 ? find_entry(list, k0) : 0;
+  int t = find_tensor(list, k0);
   for (int k = k0; k < k1; ++k) {
-    while (t + 1 < list.n && list.e[t + 1].first_chunk <= k) ++t;
-    const Entry& e = list.e[t];
-    const int64_t off = static_cast<int64_t>(k - e.first_chunk) * kChunk;
-    const int len = static_cast<int>(min(static_cast<int64_t>(kChunk), e.numel - off));
-    if (e.in_dtype == BPC_DTYPE_F32) s += chunk_squares(static_cast<const float*>(e.in) + off, len);
-    else if (e.in_dtype == BPC_DTYPE_BF16) s += chunk_squares(static_cast<const __nv_bfloat16*>(e.in) + off, len);
-    else s += chunk_squares(static_cast<const __half*>(e.in) + off, len);
+    while (list.first[t + 1] <= k) ++t;
+    const Chunk c = chunk_of<T>(list, t, k);
+    s += chunk_squares(static_cast<const T*>(list.in[t]) + c.at, c.len);
   }
   s = block_sum(s, red);
   if (threadIdx.x == 0) partial[blockIdx.x] = s;
@@ -147,74 +162,145 @@ __device__ __forceinline__ double total_squares(const double* __restrict__ parti
 __global__ void __launch_bounds__(kThreads) norm_finish_kernel(const double* __restrict__ partial, int partials,
                                                                float* __restrict__ norm) {
   __shared__ double red[kThreads / 32];
+  pdl_wait();
   const double s = total_squares(partial, partials, red);
   if (threadIdx.x == 0) *norm = static_cast<float>(sqrt(s));
 }
 
-template <typename T, typename U>
-__device__ __forceinline__ void chunk_scale(const T* p, U* q, int len, double coef) {
-  constexpr int VEC = 16 / sizeof(T);
-  const float c = static_cast<float>(coef);
-  // a factor below fp32's normal range (a norm beyond 1e37) would lose bits: multiply in fp64 then
-  const bool tiny = coef < 1.1754944e-38;
-  auto scaled = [&](float x) { return tiny ? static_cast<float>(x * coef) : x * c; };
-  const int peel = peel_of(p, len);
-  const int nv = (len - peel) / VEC;
-  if (static_cast<int>(threadIdx.x) < peel) store_f32(q + threadIdx.x, scaled(load_f32(p + threadIdx.x)));
-  const Pack<T, VEC>* v = reinterpret_cast<const Pack<T, VEC>*>(p + peel);
-  U* o = q + peel;
-  constexpr int OVEC = sizeof(U) * VEC > 16 ? 16 / sizeof(U) : VEC;       // elements per store
-  const bool wide = reinterpret_cast<uintptr_t>(o) % (sizeof(U) * OVEC) == 0;
-#pragma unroll 4
-  for (int i = threadIdx.x; i < nv; i += kThreads) {
-    const Pack<T, VEC> x = v[i];
-    Pack<U, VEC> y;
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) store_f32(&y.v[e], scaled(load_f32(&x.v[e])));
-    if (wide) {
-#pragma unroll
-      for (int e = 0; e < VEC; e += OVEC)
-        *reinterpret_cast<Pack<U, OVEC>*>(o + static_cast<int64_t>(i) * VEC + e) =
-            *reinterpret_cast<const Pack<U, OVEC>*>(&y.v[e]);
+// A thread's piece is 16 bytes of the wider of the two types: its store is one access, and a warp's stores are one run.
+__device__ __forceinline__ float2 halves(uint32_t h, const __nv_bfloat16*) {
+  return make_float2(__uint_as_float(h << 16), __uint_as_float(h & 0xffff0000u));
+}
+__device__ __forceinline__ float2 halves(uint32_t h, const __half*) {
+  return __half22float2(__halves2half2(__ushort_as_half(h & 0xffff), __ushort_as_half(h >> 16)));
+}
+__device__ __forceinline__ uint32_t pair(float lo, float hi, const __nv_bfloat16*) {
+  const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
+  return static_cast<uint32_t>(__bfloat16_as_ushort(p.x)) | static_cast<uint32_t>(__bfloat16_as_ushort(p.y)) << 16;
+}
+__device__ __forceinline__ uint32_t pair(float lo, float hi, const __half*) {
+  const __half2 p = __floats2half2_rn(lo, hi);
+  return static_cast<uint32_t>(__half_as_ushort(__low2half(p))) | static_cast<uint32_t>(__half_as_ushort(__high2half(p))) << 16;
+}
+template <typename T, int VEC>
+struct Piece {
+  static constexpr int kWords = sizeof(T) * VEC / 4;       // 2 or 4
+  uint32_t w[kWords];
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (kWords == 4) {
+      const uint4 x = *reinterpret_cast<const uint4*>(p);
+      w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
     } else {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) o[static_cast<int64_t>(i) * VEC + e] = y.v[e];
+      const uint2 x = *reinterpret_cast<const uint2*>(p);
+      w[0] = x.x, w[1] = x.y;
     }
   }
+  __device__ __forceinline__ void load_elements(const T* p) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) w[e] = reinterpret_cast<const uint32_t*>(p)[e];
+    } else {
+      const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+      for (int e = 0; e < VEC; e += 2) w[e / 2] = h[e] | static_cast<uint32_t>(h[e + 1]) << 16;
+    }
+  }
+  __device__ __forceinline__ void store(T* p) const {      // streaming: nothing here reads it again
+    if constexpr (kWords == 4) __stcs(reinterpret_cast<uint4*>(p), make_uint4(w[0], w[1], w[2], w[3]));
+    else __stcs(reinterpret_cast<uint2*>(p), make_uint2(w[0], w[1]));
+  }
+  __device__ __forceinline__ void get(float (&f)[VEC]) const {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) f[e] = __uint_as_float(w[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; e += 2) {
+        const float2 v = halves(w[e / 2], static_cast<const T*>(nullptr));
+        f[e] = v.x, f[e + 1] = v.y;
+      }
+    }
+  }
+  __device__ __forceinline__ void set(const float (&f)[VEC]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) w[e] = __float_as_uint(f[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; e += 2) w[e / 2] = pair(f[e], f[e + 1], static_cast<const T*>(nullptr));
+    }
+  }
+};
+
+template <typename T, typename U>
+__device__ __forceinline__ void chunk_scale(const T* p, U* q, int len, float by) {
+  constexpr int VEC = 16 / (sizeof(T) > sizeof(U) ? sizeof(T) : sizeof(U));
+  const int off = static_cast<int>(((0 - reinterpret_cast<uintptr_t>(q)) & (sizeof(U) * VEC - 1)) / sizeof(U));
+  const int peel = off < len ? off : len;                  // elements before the first whole piece of the output
+  const int nv = (len - peel) / VEC;
+  const T* v = p + peel;
+  U* o = q + peel;
+  // an input that is not aligned where the output is (views of buckets at other offsets) is read by elements
+  const bool aligned = reinterpret_cast<uintptr_t>(v) % (sizeof(T) * VEC) == 0;
+  for (int i = threadIdx.x; i < nv; i += kThreads * kUnroll) {
+    Piece<T, VEC> x[kUnroll];             // every load of the batch before its first store (q may be p)
+    if (aligned) {
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (i + u * kThreads < nv) x[u].load(v + (i + u * kThreads) * VEC);
+    } else {
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (i + u * kThreads < nv) x[u].load_elements(v + (i + u * kThreads) * VEC);
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      if (i + u * kThreads < nv) {
+        float f[VEC];
+        x[u].get(f);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) f[e] *= by;
+        Piece<U, VEC> y;
+        y.set(f);
+        y.store(o + (i + u * kThreads) * VEC);
+      }
+    }
+  }
+  // the elements beside the pieces; none of them lies in a piece, so the order does not matter
+  if (static_cast<int>(threadIdx.x) < peel) store_f32(q + threadIdx.x, by * load_f32(p + threadIdx.x));
   const int t = peel + nv * VEC + threadIdx.x;
-  if (t < len) store_f32(q + t, scaled(load_f32(p + t)));
+  if (t < len) store_f32(q + t, by * load_f32(p + t));
 }
 
-template <typename T>
-__device__ __forceinline__ void chunk_scale_to(const T* p, void* out, int dtype, int64_t off, int len, double coef) {
-  if (dtype == BPC_DTYPE_F32) chunk_scale(p + off, static_cast<float*>(out) + off, len, coef);
-  else if (dtype == BPC_DTYPE_BF16) chunk_scale(p + off, static_cast<__nv_bfloat16*>(out) + off, len, coef);
-  else chunk_scale(p + off, static_cast<__half*>(out) + off, len, coef);
+// A factor below fp32's normal range (a norm beyond 1e37) would lose bits in fp32: fp64 products, an element at a time.
+template <typename T, typename U>
+__device__ __noinline__ void chunk_scale_tiny(const T* p, U* q, int len, double by) {
+  for (int i = threadIdx.x; i < len; i += kThreads) store_f32(q + i, static_cast<float>(load_f32(p + i) * by));
 }
 
-template <int N>
-__global__ void __launch_bounds__(kThreads) clip_scale_kernel(const __grid_constant__ List<N> list, int per_block,
+// The chunks in the reverse of norm_partial_kernel's order: what that read last is still in L2.
+template <typename T, typename U, int N>
+__global__ void __launch_bounds__(kThreads) clip_scale_kernel(const __grid_constant__ List<N, true> list, int per_block,
                                                               const double* __restrict__ partial, int partials,
                                                               double max_norm, float* __restrict__ norm) {
   __shared__ double red[kThreads / 32];
+  const int k0 = blockIdx.x * per_block, k1 = min(list.chunks, k0 + per_block);
+  int t = find_tensor(list, k1 - 1);
+  pdl_wait();
   const double total = sqrt(total_squares(partial, partials, red));
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = static_cast<float>(total);
-  double coef = max_norm / (total + 1e-6);
-  if (coef > 1.0) coef = 1.0;             // a NaN stays
-  const int k0 = blockIdx.x * per_block, k1 = min(list.chunks, k0 + per_block);
-  int t = k0 < k1 ? find_entry(list, k0) : 0;
-  for (int k = k0; k < k1; ++k) {
-    while (t + 1 < list.n && list.e[t + 1].first_chunk <= k) ++t;
-    const Entry& e = list.e[t];
-    if (coef == 1.0 && e.in == e.out) continue;           // in place and within the limit: nothing changes
-    const int64_t off = static_cast<int64_t>(k - e.first_chunk) * kChunk;
-    const int len = static_cast<int>(min(static_cast<int64_t>(kChunk), e.numel - off));
-    if (e.in_dtype == BPC_DTYPE_F32)
-      chunk_scale_to(static_cast<const float*>(e.in), e.out, e.out_dtype, off, len, coef);
-    else if (e.in_dtype == BPC_DTYPE_BF16)
-      chunk_scale_to(static_cast<const __nv_bfloat16*>(e.in), e.out, e.out_dtype, off, len, coef);
-    else
-      chunk_scale_to(static_cast<const __half*>(e.in), e.out, e.out_dtype, off, len, coef);
+  double factor = max_norm / (total + 1e-6);
+  if (factor > 1.0) factor = 1.0;         // a NaN stays
+  const float by = static_cast<float>(factor);
+  const bool tiny = factor < 1.1754944e-38;
+  for (int k = k1 - 1; k >= k0; --k) {
+    while (list.first[t] > k) --t;
+    if (factor == 1.0 && list.in[t] == list.out[t]) continue;         // in place and within the limit: nothing changes
+    const Chunk c = chunk_of<T>(list, t, k);
+    const T* p = static_cast<const T*>(list.in[t]) + c.at;
+    U* q = static_cast<U*>(list.out[t]) + c.at;
+    if (tiny) chunk_scale_tiny(p, q, c.len, factor);
+    else chunk_scale(p, q, c.len, by);
   }
 }
 
@@ -226,44 +312,69 @@ int launched(const char* what) {
 }
 
 int max_blocks() { return kBlocksPerSm * num_sms(); }
-int launches_of(int32_t n) { return (n + kListMax - 1) / kListMax; }
 
-// One launch's share of the list: tensors [t0, t1)
-struct Part {
-  int t0, t1, chunks, per_block, blocks;
+// the most launches of a list: three groups by type, each cut into lists of kListMax tensors
+int launches_of(int32_t n) { return n / kListMax + 3; }
+
+int64_t chunks_of(int64_t numel, int32_t dtype) {
+  const int whole = kChunkBytes / size_of(dtype);
+  return (numel + whole - 1) / whole;
+}
+
+struct Tensors {
+  const void* const* in;
+  void* const* out;              // null: the norm alone
+  const int64_t* numel;
+  const int32_t *dtype, *out_dtype;
+  int32_t n;
 };
 
-std::vector<Part> parts_of(const int64_t* numel, int32_t n) {
+// One launch: tensors of one type (and output type), by their places in the list
+struct Part {
+  std::vector<int32_t> at;
+  int32_t dtype, out_dtype;
+  int chunks, per_block, blocks;
+};
+
+std::vector<Part> parts_of(const Tensors& l, bool by_output) {
   std::vector<Part> parts;
-  for (int t0 = 0; t0 < n; t0 += kListMax) {
-    Part p{t0, std::min(n, t0 + kListMax), 0, 1, 0};
-    int64_t chunks = 0;
-    for (int t = p.t0; t < p.t1; ++t) chunks += (numel[t] + kChunk - 1) / kChunk;
-    p.chunks = static_cast<int>(chunks);
+  int open[3][3];                // the group's part that still takes tensors, or -1
+  for (auto& row : open)
+    for (int& k : row) k = -1;
+  for (int32_t t = 0; t < l.n; ++t) {
+    if (l.numel[t] == 0) continue;
+    const int32_t to = by_output ? l.out_dtype[t] : l.dtype[t];
+    int& k = open[l.dtype[t]][to];
+    if (k < 0 || parts[k].at.size() == kListMax) {
+      k = static_cast<int>(parts.size());
+      parts.push_back({{}, l.dtype[t], to, 0, 0, 0});
+      parts[k].at.reserve(std::min<int32_t>(kListMax, l.n - t));
+    }
+    parts[k].at.push_back(t);
+    parts[k].chunks += static_cast<int>(chunks_of(l.numel[t], l.dtype[t]));
+  }
+  for (Part& p : parts) {
     p.per_block = std::max(1, (p.chunks + max_blocks() - 1) / max_blocks());
     p.blocks = (p.chunks + p.per_block - 1) / p.per_block;
-    parts.push_back(p);
   }
   return parts;
 }
 
-template <int N>
-void fill(List<N>* list, const Part& p, const void* const* in, void* const* out, const int64_t* numel,
-          const int32_t* in_dtype, const int32_t* out_dtype) {
-  list->n = 0;
-  list->chunks = p.chunks;
-  int chunk = 0;
-  for (int t = p.t0; t < p.t1; ++t) {
-    if (numel[t] == 0) continue;
-    Entry& e = list->e[list->n++];
-    e.in = in[t];
-    e.out = out ? out[t] : nullptr;
-    e.numel = numel[t];
-    e.first_chunk = chunk;
-    e.in_dtype = static_cast<int16_t>(in_dtype[t]);
-    e.out_dtype = static_cast<int16_t>(out_dtype ? out_dtype[t] : in_dtype[t]);
-    chunk += static_cast<int>((numel[t] + kChunk - 1) / kChunk);
+template <int N, bool OUT>
+void fill(List<N, OUT>* list, const Part& p, const Tensors& l) {
+  int n = 0, chunk = 0;
+  for (const int32_t t : p.at) {
+    const int64_t chunks = chunks_of(l.numel[t], p.dtype);
+    list->in[n] = l.in[t];
+    if (OUT) list->out[n] = l.out[t];
+    list->first[n] = chunk;
+    list->last[n] = static_cast<uint32_t>(l.numel[t] - (chunks - 1) * (kChunkBytes / size_of(p.dtype)));
+    chunk += static_cast<int>(chunks);
+    ++n;
   }
+  list->first[n] = chunk;
+  list->n = n;
+  list->chunks = chunk;
 }
 
 int check_list(const void* const* in, const int64_t* numel, const int32_t* dtype, int32_t n, const char* what) {
@@ -275,7 +386,7 @@ int check_list(const void* const* in, const int64_t* numel, const int32_t* dtype
     if (!size) return fail(BPC_ERR_ARG, std::string(what) + ": dtype must be f32, bf16 or f16");
     if (numel[t] && !in[t]) return fail(BPC_ERR_ARG, std::string(what) + ": null tensor");
     if (reinterpret_cast<uintptr_t>(in[t]) % size) return fail(BPC_ERR_ARG, std::string(what) + ": tensor not aligned to its type");
-    chunks += (numel[t] + kChunk - 1) / kChunk;
+    chunks += chunks_of(numel[t], dtype[t]);
     if (chunks > 0x3fffffff) return fail(BPC_ERR_ARG, std::string(what) + ": too many elements");
   }
   return 0;
@@ -314,36 +425,39 @@ int check_overlap(const void* const* in, void* const* out, const int64_t* numel,
   return 0;
 }
 
-template <int N>
-int launch_partial(const Part& p, const void* const* in, const int64_t* numel, const int32_t* dtype, double* partial,
-                   cudaStream_t s) {
-  List<N> list;
-  fill(&list, p, in, nullptr, numel, dtype, nullptr);
-  norm_partial_kernel<N><<<p.blocks, kThreads, 0, s>>>(list, p.per_block, partial);
-  return launched("norm_partial_kernel");
+// Calls f with the smallest list size that holds n tensors (a launch copies its whole parameter block), or a type.
+template <typename F>
+int with_list(size_t n, F f) {
+  if (n <= 24) return f(std::integral_constant<int, 24>());
+  if (n <= 100) return f(std::integral_constant<int, 100>());
+  if (n <= 320) return f(std::integral_constant<int, 320>());
+  return f(std::integral_constant<int, kListMax>());
 }
-
-template <int N>
-int launch_scale(const Part& p, const void* const* in, void* const* out, const int64_t* numel, const int32_t* in_dtype,
-                 const int32_t* out_dtype, const double* partial, int partials, double max_norm, float* norm,
-                 cudaStream_t s) {
-  List<N> list;
-  fill(&list, p, in, out, numel, in_dtype, out_dtype);
-  clip_scale_kernel<N><<<p.blocks, kThreads, 0, s>>>(list, p.per_block, partial, partials, max_norm, norm);
-  return launched("clip_scale_kernel");
+template <typename T>
+struct Type {
+  typedef T type;
+};
+template <typename F>
+int with_type(int32_t dtype, F f) {
+  if (dtype == BPC_DTYPE_F32) return f(Type<float>());
+  if (dtype == BPC_DTYPE_BF16) return f(Type<__nv_bfloat16>());
+  return f(Type<__half>());
 }
 
 // The partial sums of every launch; *partials counts them
-int run_partials(const std::vector<Part>& parts, const void* const* in, const int64_t* numel, const int32_t* dtype,
-                 double* partial, int* partials, cudaStream_t s) {
+int run_partials(const Tensors& l, double* partial, int* partials, cudaStream_t s) {
   *partials = 0;
-  for (const Part& p : parts) {
-    if (!p.blocks) continue;
-    const int n = p.t1 - p.t0;
+  for (const Part& p : parts_of(l, false)) {
     double* at = partial + *partials;
-    const int e = n <= 32 ? launch_partial<32>(p, in, numel, dtype, at, s)
-                          : n <= 200 ? launch_partial<200>(p, in, numel, dtype, at, s)
-                                     : launch_partial<kListMax>(p, in, numel, dtype, at, s);
+    const int e = with_type(p.dtype, [&](auto type) {
+      return with_list(p.at.size(), [&](auto size) {
+        constexpr int N = decltype(size)::value;
+        List<N, false> list;
+        fill(&list, p, l);
+        norm_partial_kernel<typename decltype(type)::type, N><<<p.blocks, kThreads, 0, s>>>(list, p.per_block, at);
+        return launched("norm_partial_kernel");
+      });
+    });
     if (e) return e;
     *partials += p.blocks;
   }
@@ -351,8 +465,32 @@ int run_partials(const std::vector<Part>& parts, const void* const* in, const in
 }
 
 int finish(const double* partial, int partials, float* norm, cudaStream_t s) {
-  norm_finish_kernel<<<1, kThreads, 0, s>>>(partial, partials, norm);
-  return launched("norm_finish_kernel");
+  void* args[] = {&partial, &partials, &norm};
+  return launch_pdl(reinterpret_cast<const void*>(&norm_finish_kernel), dim3(1), dim3(kThreads), 0, s, args, 1,
+                    "norm_finish_kernel");
+}
+
+// The first launch may start before the norm's last kernel ends (it waits for it before it reads the sums); a later one
+// waits for one that has waited.
+int run_scale(const Tensors& l, const double* partial, int partials, double max_norm, float* norm, cudaStream_t s) {
+  for (const Part& p : parts_of(l, true)) {
+    const int e = with_type(p.dtype, [&](auto type) {
+      return with_type(p.out_dtype, [&](auto out_type) {
+        return with_list(p.at.size(), [&](auto size) {
+          constexpr int N = decltype(size)::value;
+          List<N, true> list;
+          fill(&list, p, l);
+          int per_block = p.per_block;
+          void* args[] = {&list, &per_block, &partial, &partials, &max_norm, &norm};
+          return launch_pdl(reinterpret_cast<const void*>(
+                                &clip_scale_kernel<typename decltype(type)::type, typename decltype(out_type)::type, N>),
+                            dim3(p.blocks), dim3(kThreads), 0, s, args, 1, "clip_scale_kernel");
+        });
+      });
+    });
+    if (e) return e;
+  }
+  return 0;
 }
 
 int check_common(const void* const* tensors, const int64_t* numel, const int32_t* dtype, int32_t n, float* norm,
@@ -373,7 +511,7 @@ using namespace bpc;
 
 extern "C" size_t bpc_grad_norm_workspace_size(int32_t n) {
   if (n < 0 || n > (1 << 20)) return 0;
-  return sizeof(double) * static_cast<size_t>(max_blocks()) * std::max(1, launches_of(n));
+  return sizeof(double) * static_cast<size_t>(max_blocks()) * launches_of(n);
 }
 
 extern "C" int bpc_grad_norm(const void* const* tensors, const int64_t* numel, const int32_t* dtype, int32_t n,
@@ -383,7 +521,7 @@ extern "C" int bpc_grad_norm(const void* const* tensors, const int64_t* numel, c
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     double* partial = static_cast<double*>(workspace);
     int partials = 0;
-    if (int e = run_partials(parts_of(numel, n), tensors, numel, dtype, partial, &partials, s)) return e;
+    if (int e = run_partials({tensors, nullptr, numel, dtype, nullptr, n}, partial, &partials, s)) return e;
     return finish(partial, partials, norm, s);
   } catch (const std::exception& e) {      // a host array that cannot be allocated
     return fail(BPC_ERR_ARG, e.what());
@@ -402,18 +540,10 @@ extern "C" int bpc_clip_grads(const void* const* tensors, void* const* out, cons
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     double* partial = static_cast<double*>(workspace);
     int partials = 0;
-    const std::vector<Part> parts = parts_of(numel, n);
-    if (int e = run_partials(parts, tensors, numel, dtype, partial, &partials, s)) return e;
+    const Tensors l{tensors, out, numel, dtype, out_dtype, n};
+    if (int e = run_partials(l, partial, &partials, s)) return e;
     if (!partials) return finish(partial, 0, norm, s);
-    for (const Part& p : parts) {
-      if (!p.blocks) continue;
-      const int k = p.t1 - p.t0;
-      const int e = k <= 32 ? launch_scale<32>(p, tensors, out, numel, dtype, out_dtype, partial, partials, max_norm, norm, s)
-                    : k <= 200 ? launch_scale<200>(p, tensors, out, numel, dtype, out_dtype, partial, partials, max_norm, norm, s)
-                               : launch_scale<kListMax>(p, tensors, out, numel, dtype, out_dtype, partial, partials, max_norm, norm, s);
-      if (e) return e;
-    }
-    return 0;
+    return run_scale(l, partial, partials, max_norm, norm, s);
   } catch (const std::exception& e) {
     return fail(BPC_ERR_ARG, e.what());
   }
