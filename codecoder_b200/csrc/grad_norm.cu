@@ -3,9 +3,9 @@
 //   norm = sqrt(sum_t sum_i g_t[i]^2);   out_t[i] = g_t[i] min(1, max_norm / (norm + 1e-6))
 //
 // The list travels in the launch's parameters (no copy to the device, so a captured call replays as it is).  Every
-// tensor is cut into chunks of 16 KB and the chunks of the list are dealt to the blocks in equal runs, so a
-// list of many small tensors and one of few large ones load the GPU alike.  Squares and sums are fp64: a square of any
-// finite fp32 value neither overflows nor vanishes, and the sum's order is fixed (no atomics).
+// tensor is cut into chunks of 16 KB, dealt to the blocks in turn, so a list of many small tensors and one of few large
+// ones load the GPU alike.  Squares and sums are fp64: a square of any finite fp32 value neither overflows nor vanishes,
+// and the sum's order is fixed (no atomics).
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -26,7 +26,8 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kChunkBytes = 16384;        // of the input: kUnroll 16-byte loads per thread
 constexpr int kListMax = 1000;            // tensors per launch: 24 bytes each, within the 32,764 bytes of parameters
-constexpr int kBlocksPerSm = 8;
+constexpr int kBlocksPerSm = 8;           // of the norm's kernel, at full occupancy
+constexpr int kScaleBlocksPerSm = 6;
 constexpr int kUnroll = 4;
 
 // A launch's tensors, of one type (and one output type): a kernel that branched over nine pairs of types spilled its
@@ -52,10 +53,9 @@ struct alignas(sizeof(T) * VEC) Pack {
   T v[VEC];
 };
 
-// the tensor of chunk k
+// the tensor of chunk k, which is one of lo .. hi
 template <typename L>
-__device__ __forceinline__ int find_tensor(const L& list, int k) {
-  int lo = 0, hi = list.n - 1;
+__device__ __forceinline__ int find_tensor(const L& list, int k, int lo, int hi) {
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
     if (list.first[mid] <= k) lo = mid;
@@ -137,14 +137,13 @@ __device__ __forceinline__ double chunk_squares(const T* __restrict__ p, int len
 
 template <typename T, int N>
 __global__ void __launch_bounds__(kThreads) norm_partial_kernel(const __grid_constant__ List<N, false> list,
-                                                                int per_block, double* __restrict__ partial) {
+                                                                double* __restrict__ partial) {
   __shared__ double red[kThreads / 32];
   pdl_launch_dependents();
-  const int k0 = blockIdx.x * per_block, k1 = min(list.chunks, k0 + per_block);
   double s = 0.0;
-  int t = find_tensor(list, k0);
-  for (int k = k0; k < k1; ++k) {
-    while (list.first[t + 1] <= k) ++t;
+  int t = find_tensor(list, blockIdx.x, 0, list.n - 1);
+  for (int k = blockIdx.x; k < list.chunks; k += gridDim.x) {
+    if (list.first[t + 1] <= k) t = find_tensor(list, k, t + 1, list.n - 1);
     const Chunk c = chunk_of<T>(list, t, k);
     s += chunk_squares(static_cast<const T*>(list.in[t]) + c.at, c.len);
   }
@@ -206,8 +205,8 @@ struct Piece {
     }
   }
   __device__ __forceinline__ void store(T* p) const {      // streaming: nothing here reads it again
-    if constexpr (kWords == 4) __stcs(reinterpret_cast<uint4*>(p), make_uint4(w[0], w[1], w[2], w[3]));
-    else __stcs(reinterpret_cast<uint2*>(p), make_uint2(w[0], w[1]));
+    if constexpr (kWords == 4) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    else *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
   }
   __device__ __forceinline__ void get(float (&f)[VEC]) const {
     if constexpr (sizeof(T) == 4) {
@@ -280,12 +279,12 @@ __device__ __noinline__ void chunk_scale_tiny(const T* p, U* q, int len, double 
 
 // The chunks in the reverse of norm_partial_kernel's order: what that read last is still in L2.
 template <typename T, typename U, int N>
-__global__ void __launch_bounds__(kThreads) clip_scale_kernel(const __grid_constant__ List<N, true> list, int per_block,
+__global__ void __launch_bounds__(kThreads, kScaleBlocksPerSm) clip_scale_kernel(const __grid_constant__ List<N, true> list,
                                                               const double* __restrict__ partial, int partials,
                                                               double max_norm, float* __restrict__ norm) {
   __shared__ double red[kThreads / 32];
-  const int k0 = blockIdx.x * per_block, k1 = min(list.chunks, k0 + per_block);
-  int t = find_tensor(list, k1 - 1);
+  const int last = list.chunks - 1 - blockIdx.x;
+  int t = find_tensor(list, last, 0, list.n - 1);
   pdl_wait();
   const double total = sqrt(total_squares(partial, partials, red));
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = static_cast<float>(total);
@@ -293,8 +292,8 @@ __global__ void __launch_bounds__(kThreads) clip_scale_kernel(const __grid_const
   if (factor > 1.0) factor = 1.0;         // a NaN stays
   const float by = static_cast<float>(factor);
   const bool tiny = factor < 1.1754944e-38;
-  for (int k = k1 - 1; k >= k0; --k) {
-    while (list.first[t] > k) --t;
+  for (int k = last; k >= 0; k -= gridDim.x) {
+    if (list.first[t] > k) t = find_tensor(list, k, 0, t - 1);
     if (factor == 1.0 && list.in[t] == list.out[t]) continue;         // in place and within the limit: nothing changes
     const Chunk c = chunk_of<T>(list, t, k);
     const T* p = static_cast<const T*>(list.in[t]) + c.at;
@@ -333,7 +332,7 @@ struct Tensors {
 struct Part {
   std::vector<int32_t> at;
   int32_t dtype, out_dtype;
-  int chunks, per_block, blocks;
+  int chunks, blocks;
 };
 
 std::vector<Part> parts_of(const Tensors& l, bool by_output) {
@@ -347,16 +346,14 @@ std::vector<Part> parts_of(const Tensors& l, bool by_output) {
     int& k = open[l.dtype[t]][to];
     if (k < 0 || parts[k].at.size() == kListMax) {
       k = static_cast<int>(parts.size());
-      parts.push_back({{}, l.dtype[t], to, 0, 0, 0});
+      parts.push_back({{}, l.dtype[t], to, 0, 0});
       parts[k].at.reserve(std::min<int32_t>(kListMax, l.n - t));
     }
     parts[k].at.push_back(t);
     parts[k].chunks += static_cast<int>(chunks_of(l.numel[t], l.dtype[t]));
   }
-  for (Part& p : parts) {
-    p.per_block = std::max(1, (p.chunks + max_blocks() - 1) / max_blocks());
-    p.blocks = (p.chunks + p.per_block - 1) / p.per_block;
-  }
+  const int most = by_output ? kScaleBlocksPerSm * num_sms() : max_blocks();
+  for (Part& p : parts) p.blocks = std::min(p.chunks, most);
   return parts;
 }
 
@@ -454,7 +451,7 @@ int run_partials(const Tensors& l, double* partial, int* partials, cudaStream_t 
         constexpr int N = decltype(size)::value;
         List<N, false> list;
         fill(&list, p, l);
-        norm_partial_kernel<typename decltype(type)::type, N><<<p.blocks, kThreads, 0, s>>>(list, p.per_block, at);
+        norm_partial_kernel<typename decltype(type)::type, N><<<p.blocks, kThreads, 0, s>>>(list, at);
         return launched("norm_partial_kernel");
       });
     });
@@ -480,8 +477,7 @@ int run_scale(const Tensors& l, const double* partial, int partials, double max_
           constexpr int N = decltype(size)::value;
           List<N, true> list;
           fill(&list, p, l);
-          int per_block = p.per_block;
-          void* args[] = {&list, &per_block, &partial, &partials, &max_norm, &norm};
+          void* args[] = {&list, &partial, &partials, &max_norm, &norm};
           return launch_pdl(reinterpret_cast<const void*>(
                                 &clip_scale_kernel<typename decltype(type)::type, typename decltype(out_type)::type, N>),
                             dim3(p.blocks), dim3(kThreads), 0, s, args, 1, "clip_scale_kernel");
