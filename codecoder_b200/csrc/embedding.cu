@@ -78,58 +78,178 @@ __global__ void __launch_bounds__(256) embed_lookup_kernel(const I* __restrict__
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// Stable radix sort of the positions by token, kDigitBits bits a pass: per-tile digit counts, one scan per digit over
-// the tiles, then each tile places its keys.  Positions whose id is outside [0, V) get key V: they sort to the end.
+// Stable radix sort of the positions by token into pairs {token, position}, 8 bits a pass.  Positions whose id is outside
+// [0, V) get token V: they sort to the end.
 constexpr int kDigitBits = 8;
 constexpr int kBins = 1 << kDigitBits;
-constexpr int kSortThreads = 256;
-constexpr int kSortWarps = kSortThreads / 32;
-constexpr int kSortRounds = 16;                           // keys per thread
-constexpr int kSortTile = kSortThreads * kSortRounds;
 
 template <typename I>
 __device__ __forceinline__ int token_key(I id, int V) {
   return id >= 0 && static_cast<int64_t>(id) < V ? static_cast<int>(id) : V;
 }
 
-// src: the ids (first pass) or the previous pass's keys, which are in [0, V] already
+__device__ __forceinline__ int warp_inclusive(int s, int lane) {
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int o = __shfl_up_sync(0xffffffffu, s, d);
+    if (lane >= d) s += o;
+  }
+  return s;
+}
+
+// The ranks of a warp's ROUNDS x 32 consecutive keys among its earlier ones of the same digit; cnt (kBins, the warp's own,
+// zero before) counts its digits.  A negative key is none.
+template <int ROUNDS, typename N>
+__device__ __forceinline__ void warp_ranks(const int (&key)[ROUNDS], int (&rank)[ROUNDS], int shift, N* cnt, int lane) {
+#pragma unroll
+  for (int r = 0; r < ROUNDS; ++r) {
+    const int digit = key[r] < 0 ? kBins : (key[r] >> shift) & (kBins - 1);
+    const unsigned same = __match_any_sync(0xffffffffu, digit);
+    const int before = key[r] < 0 ? 0 : cnt[digit];
+    rank[r] = before + __popc(same & ((1u << lane) - 1));
+    __syncwarp();
+    if (key[r] >= 0 && lane == __ffs(same) - 1) cnt[digit] = static_cast<N>(before + __popc(same));
+    __syncwarp();
+  }
+}
+
+// Up to kClusterKeys positions: one cluster of 8 CTAs runs every pass in one launch (separate launches of three kernels a
+// pass took 66 us for 32,768 positions, most of it latency).  The CTAs exchange their digit counts through distributed
+// shared memory and the pairs through L2.
+constexpr int kClusterCtas = 8;
+constexpr int kClusterThreads = 1024;
+constexpr int kClusterKeys = kClusterCtas * kClusterThreads * 8;
+
+__device__ __forceinline__ void st_cluster(uint32_t addr, int v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+
+template <typename I, int ROUNDS>
+__global__ void __launch_bounds__(kClusterThreads) sort_cluster_kernel(const I* __restrict__ ids, int n, int V, int passes,
+                                                                       int2* __restrict__ a, int2* __restrict__ b,
+                                                                       int* __restrict__ zero) {
+  __shared__ uint16_t cnt[kClusterThreads / 32][kBins];
+  __shared__ int hist[2][kClusterCtas][kBins];             // every CTA's counts of this pass; two, so that a pass may
+  __shared__ int warp_sum[kBins / 32];                     // write while a slower CTA still reads the one before
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int cta = static_cast<int>(cluster_ctarank());
+  const int first = (cta * kClusterThreads + warp * 32) * ROUNDS + lane;
+  pdl_launch_dependents();
+  if (cta == 0 && tid == 0) *zero = 0;
+  cluster_arrive_release();                                // every CTA runs before another writes its shared memory
+  cluster_wait_acquire();
+  for (int pass = 0; pass < passes; ++pass) {
+    int2* const to = pass & 1 ? b : a;
+    const int2* const from = pass & 1 ? a : b;
+    const int shift = pass * kDigitBits;
+    int key[ROUNDS], pos[ROUNDS], rank[ROUNDS];
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+      const int i = first + r * 32;
+      key[r] = -1;
+      pos[r] = i;
+      if (i < n) {
+        if (pass == 0) {
+          key[r] = token_key(ids[i], V);
+        } else {
+          const int2 p = __ldcg(from + i);                 // written by the other CTAs: from L2
+          key[r] = p.x;
+          pos[r] = p.y;
+        }
+      }
+    }
+    for (int k = tid; k < kClusterThreads / 32 * kBins; k += kClusterThreads) (&cnt[0][0])[k] = 0;
+    __syncthreads();
+    warp_ranks(key, rank, shift, cnt[warp], lane);
+    __syncthreads();
+    if (tid < kBins) {                                     // this CTA's counts, and each warp's first place among them
+      int at = 0;
+#pragma unroll 8
+      for (int w = 0; w < kClusterThreads / 32; ++w) {
+        const int c = cnt[w][tid];
+        cnt[w][tid] = static_cast<uint16_t>(at);
+        at += c;
+      }
+      for (int k = 0; k < kClusterCtas; ++k) st_cluster(map_to_cta(smem_u32(&hist[pass & 1][cta][tid]), k), at);
+    }
+    cluster_arrive_release();
+    cluster_wait_acquire();
+    int total = 0, before = 0, s = 0;
+    if (tid < kBins) {
+#pragma unroll
+      for (int k = 0; k < kClusterCtas; ++k) {
+        const int c = hist[pass & 1][k][tid];
+        if (k < cta) before += c;
+        total += c;
+      }
+      s = warp_inclusive(total, lane);
+      if (lane == 31) warp_sum[warp] = s;
+    }
+    __syncthreads();
+    if (tid < kBins) {
+      int at = s - total + before;
+      for (int w = 0; w < warp; ++w) at += warp_sum[w];
+      hist[pass & 1][cta][tid] = at;                       // only this CTA reads its own row from here on
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+      if (key[r] >= 0) {
+        const int digit = (key[r] >> shift) & (kBins - 1);
+        to[hist[pass & 1][cta][digit] + cnt[warp][digit] + rank[r]] = make_int2(key[r], pos[r]);
+      }
+    }
+    cluster_arrive_release();                              // the pairs are written, and every count read
+    cluster_wait_acquire();
+  }
+}
+
+// More positions: per-tile digit counts, one scan per digit over the tiles, then each tile places its keys.
+constexpr int kSortThreads = 256;
+constexpr int kSortWarps = kSortThreads / 32;
+constexpr int kSortRounds = 8;                            // keys per thread
+constexpr int kSortTile = kSortThreads * kSortRounds;
+
+// src: the ids (first pass) or the previous pass's pairs
+__device__ __forceinline__ int key_of(const int2* src, int64_t i, int) { return src[i].x; }
 template <typename I>
-__global__ void __launch_bounds__(kSortThreads) sort_count_kernel(const I* __restrict__ src, int64_t n, int V, int shift,
+__device__ __forceinline__ int key_of(const I* src, int64_t i, int V) { return token_key(src[i], V); }
+
+template <typename S>
+__global__ void __launch_bounds__(kSortThreads) sort_count_kernel(const S* __restrict__ src, int64_t n, int V, int shift,
                                                                   int* __restrict__ counts, int tiles) {
   __shared__ int cnt[kBins];
   for (int b = threadIdx.x; b < kBins; b += kSortThreads) cnt[b] = 0;
   __syncthreads();
-  const int64_t base = static_cast<int64_t>(blockIdx.x) * kSortTile;
+  const int64_t base = static_cast<int64_t>(blockIdx.x) * kSortTile + threadIdx.x;
+  int key[kSortRounds];
 #pragma unroll
   for (int r = 0; r < kSortRounds; ++r) {
-    const int64_t i = base + r * kSortThreads + threadIdx.x;
-    const bool ok = i < n;
-    const unsigned act = __ballot_sync(0xffffffffu, ok);
-    if (ok) {
-      const int digit = (token_key(src[i], V) >> shift) & (kBins - 1);
-      const unsigned same = __match_any_sync(act, digit);
-      if ((threadIdx.x & 31) == __ffs(same) - 1) atomicAdd(&cnt[digit], __popc(same));
-    }
+    const int64_t i = base + r * kSortThreads;
+    key[r] = i < n ? key_of(src, i, V) : -1;
+  }
+#pragma unroll
+  for (int r = 0; r < kSortRounds; ++r) {
+    const int digit = key[r] < 0 ? kBins : (key[r] >> shift) & (kBins - 1);
+    const unsigned same = __match_any_sync(0xffffffffu, digit);
+    if (key[r] >= 0 && (threadIdx.x & 31) == __ffs(same) - 1) atomicAdd(&cnt[digit], __popc(same));
   }
   __syncthreads();
   for (int b = threadIdx.x; b < kBins; b += kSortThreads) counts[static_cast<int64_t>(b) * tiles + blockIdx.x] = cnt[b];
 }
 
 // One block per digit: its counts over the tiles become exclusive sums; totals[digit] their sum.
-__global__ void __launch_bounds__(256) sort_scan_kernel(int* __restrict__ counts, int* __restrict__ totals, int tiles) {
+__global__ void __launch_bounds__(256) sort_scan_kernel(int* __restrict__ counts, int* __restrict__ totals, int tiles,
+                                                        int* __restrict__ zero) {
   __shared__ int warp_sum[8];
   int* row = counts + static_cast<int64_t>(blockIdx.x) * tiles;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *zero = 0;
   int carry = 0;
   for (int t0 = 0; t0 < tiles; t0 += 256) {
     const int t = t0 + threadIdx.x;
     const int v = t < tiles ? row[t] : 0;
-    int s = v;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int o = __shfl_up_sync(0xffffffffu, s, d);
-      if (lane >= d) s += o;
-    }
+    const int s = warp_inclusive(v, lane);
     if (lane == 31) warp_sum[warp] = s;
     __syncthreads();
     int before = carry, all = 0;
@@ -146,52 +266,36 @@ __global__ void __launch_bounds__(256) sort_scan_kernel(int* __restrict__ counts
 }
 
 // Places a tile's keys.  Each warp takes a run of kSortRounds x 32 consecutive keys in order, so ranks by (warp, round,
-// lane) keep the order of equal digits.  perm_in null: the first pass (position i itself).
+// lane) keep the order of equal digits.
+__device__ __forceinline__ int position_of(const int2* src, int64_t i) { return src[i].y; }
 template <typename I>
-__global__ void __launch_bounds__(kSortThreads) sort_place_kernel(const I* __restrict__ src,
-                                                                  const int* __restrict__ perm_in, int64_t n, int V,
-                                                                  int shift, const int* __restrict__ offsets,
+__device__ __forceinline__ int position_of(const I*, int64_t i) { return static_cast<int>(i); }
+
+template <typename S>
+__global__ void __launch_bounds__(kSortThreads) sort_place_kernel(const S* __restrict__ src, int64_t n, int V, int shift,
+                                                                  const int* __restrict__ offsets,
                                                                   const int* __restrict__ totals, int tiles,
-                                                                  int* __restrict__ key_out, int* __restrict__ perm_out) {
+                                                                  int2* __restrict__ out) {
   __shared__ int cnt[kSortWarps][kBins];
   __shared__ int warp_sum[kSortWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (int b = threadIdx.x; b < kSortWarps * kBins; b += kSortThreads) (&cnt[0][0])[b] = 0;
-  __syncthreads();
   const int64_t base = static_cast<int64_t>(blockIdx.x) * kSortTile + warp * (kSortRounds * 32) + lane;
   int key[kSortRounds], rank[kSortRounds];
 #pragma unroll
   for (int r = 0; r < kSortRounds; ++r) {
     const int64_t i = base + r * 32;
-    key[r] = i < n ? token_key(src[i], V) : -1;
+    key[r] = i < n ? key_of(src, i, V) : -1;
   }
-#pragma unroll
-  for (int r = 0; r < kSortRounds; ++r) {
-    const bool ok = key[r] >= 0;
-    const unsigned act = __ballot_sync(0xffffffffu, ok);
-    rank[r] = 0;
-    if (ok) {
-      const int digit = (key[r] >> shift) & (kBins - 1);
-      const unsigned same = __match_any_sync(act, digit);
-      const int before = cnt[warp][digit];
-      rank[r] = before + __popc(same & ((1u << lane) - 1));
-      __syncwarp(act);
-      if (lane == __ffs(same) - 1) cnt[warp][digit] = before + __popc(same);
-    }
-    __syncwarp();
-  }
+  __syncthreads();
+  warp_ranks(key, rank, shift, cnt[warp], lane);
   __syncthreads();
   {
     // first place of each digit: the digits below it, then this digit's earlier tiles, then its earlier warps
     static_assert(kBins == kSortThreads, "one thread per digit");
     const int b = threadIdx.x;
     const int v = totals[b];
-    int s = v;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int o = __shfl_up_sync(0xffffffffu, s, d);
-      if (lane >= d) s += o;
-    }
+    const int s = warp_inclusive(v, lane);
     if (lane == 31) warp_sum[warp] = s;
     __syncthreads();
     int at = s - v + offsets[static_cast<int64_t>(b) * tiles + blockIdx.x];
@@ -206,12 +310,8 @@ __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(const I* __res
   __syncthreads();
 #pragma unroll
   for (int r = 0; r < kSortRounds; ++r) {
-    if (key[r] >= 0) {
-      const int64_t i = base + r * 32;
-      const int at = cnt[warp][(key[r] >> shift) & (kBins - 1)] + rank[r];
-      key_out[at] = key[r];
-      perm_out[at] = perm_in ? perm_in[i] : static_cast<int>(i);
-    }
+    if (key[r] >= 0)
+      out[cnt[warp][(key[r] >> shift) & (kBins - 1)] + rank[r]] = make_int2(key[r], position_of(src, base + r * 32));
   }
 }
 
@@ -220,10 +320,9 @@ __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(const I* __res
 // token), cut into equal runs of `items` steps, one per worker, so that a token with millions of rows and a million
 // tokens without any both spread evenly; every row of dW is written once, the empty ones as zeros.  A token whose rows
 // cross workers: each worker but the one at its end leaves a partial sum in tail[], the last one leaves its own in
-// head[], and wgrad_join_kernel adds them in order.
+// head[] and its number in heads[], and wgrad_join_kernel adds them in order.
 struct MergeArgs {
-  const int* key;      // (n,) sorted
-  const int* perm;     // (n,) the rows in that order
+  const int2* pair;    // (n,) {token, row}, sorted by token
   int64_t n, items, workers;
   int V, C, G;         // G lanes per worker
   int64_t ldg;
@@ -232,17 +331,21 @@ struct MergeArgs {
   int dw_dtype;
   float* head;         // (workers, C)
   float* tail;
-  int* head_token;     // (workers,) the token of head[], or -1
+  int* heads;          // [0]: how many; [1 ..]: the workers with a head, in no order
 };
 
-// tokens finished within the first d steps of the path
-__device__ __forceinline__ int64_t path_search(const int* __restrict__ key, int64_t n, int V, int64_t d) {
-  int64_t lo = d > n ? d - n : 0, hi = d < V ? d : V;      // lo holds: every row consumed
+// The tokens finished within the first d steps of the path, by the G lanes of a worker together: each step of the search
+// probes G places.
+__device__ __forceinline__ int64_t path_search(const MergeArgs& a, int64_t d, int l, unsigned mask, int shift) {
+  int64_t lo = d > a.n ? d - a.n : 0, hi = d < a.V ? d : a.V;            // lo holds: every row consumed
   while (lo < hi) {
-    const int64_t mid = (lo + hi + 1) >> 1;
-    // token mid - 1 is finished before step d iff the next row belongs to a later one
-    if (d - mid >= n || key[d - mid] >= mid) lo = mid;
-    else hi = mid - 1;
+    const int64_t step = (hi - lo + a.G) / (a.G + 1), at = lo + (l + 1) * step;
+    // token at - 1 is finished before step d iff the next row belongs to a later one
+    const bool done = at <= hi && (d - at >= a.n || a.pair[d - at].x >= at);
+    const int c = __popc(__ballot_sync(mask, done) & mask);
+    const int64_t top = lo + (c + 1) * step - 1;
+    lo += c * step;
+    if (c < a.G && top < hi) hi = top;                     // below the first probe that failed
   }
   return lo;
 }
@@ -271,85 +374,164 @@ __device__ __forceinline__ void store_row(void* dw, int dtype, int64_t at, const
   }
 }
 
-template <typename T, int VEC>
-__global__ void __launch_bounds__(256) wgrad_merge_kernel(const T* __restrict__ gy, MergeArgs a) {
-  constexpr int kRows = 8;                                // rows whose loads are in flight per worker
-  const int per_block = 256 / a.G;
-  const int64_t w = blockIdx.x * static_cast<int64_t>(per_block) + threadIdx.x / a.G;
-  const int c = (blockIdx.y * a.G + threadIdx.x % a.G) * VEC;
+// S pieces of VEC channels per lane, 32 VEC channels apart
+template <typename T, int VEC, int S>
+__global__ void __launch_bounds__(256) wgrad_merge_kernel(const T* __restrict__ gy, const __grid_constant__ MergeArgs a) {
+  constexpr int kRows = S == 1 ? 8 : 4;                   // rows whose loads are in flight per worker
+  typedef Pack<T, VEC> Piece;
+  __shared__ int64_t starts[257];
+  const int l = threadIdx.x % a.G, mine = threadIdx.x / a.G, per_block = 256 / a.G;
+  const int64_t w = blockIdx.x * static_cast<int64_t>(per_block) + mine;
+  const int64_t end = a.V + a.n, d0 = min(end, w * a.items), d1 = min(end, d0 + a.items);
+  const int shift = (threadIdx.x & 31) / a.G * a.G;
+  const unsigned mask = (a.G == 32 ? 0xffffffffu : (1u << a.G) - 1) << shift;
+  pdl_launch_dependents();
+  pdl_wait();
+  {
+    const int64_t i = path_search(a, d0, l, mask, shift);
+    if (l == 0) starts[mine] = i;
+    if (mine == per_block - 1) {
+      const int64_t e = path_search(a, d1, l, mask, shift);
+      if (l == 0) starts[per_block] = e;
+    }
+  }
+  __syncthreads();
   if (w >= a.workers) return;
-  const bool on = c < a.C;
-  const int64_t end = a.V + a.n;
-  const int64_t d0 = min(end, w * a.items), d1 = min(end, d0 + a.items);
-  const int64_t i0 = path_search(a.key, a.n, a.V, d0), i1 = path_search(a.key, a.n, a.V, d1);
+  const int64_t i0 = starts[mine], i1 = starts[mine + 1];
   const int64_t j0 = d0 - i0, j1 = d1 - i1;
-  bool open = j0 > 0 && i0 < a.V && a.key[j0 - 1] == i0;   // token i0 began in an earlier worker
-  if (on && c == 0) a.head_token[w] = open && i1 > i0 ? static_cast<int>(i0) : -1;
-  float acc[VEC];
+  int c[S];
+  bool on[S];
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
-  int64_t tok = i0;
-  auto flush = [&]() {
-    if (on) {
-      if (open) {
+  for (int q = 0; q < S; ++q) {
+    c[q] = ((blockIdx.y * S + q) * a.G + l) * VEC;
+    on[q] = c[q] < a.C;
+  }
+  bool open = j0 > 0 && i0 < a.V && a.pair[j0 - 1].x == i0;               // token i0 began in an earlier worker
+  if (open && i1 > i0 && l == 0 && blockIdx.y == 0) a.heads[1 + atomicAdd(a.heads, 1)] = static_cast<int>(w);
+  float acc[S][VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) a.head[w * a.C + c + e] = acc[e];
-      } else {
-        store_row<VEC>(a.dw, a.dw_dtype, tok * a.C + c, acc, a.scale);
+  for (int q = 0; q < S; ++q)
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) acc[q][e] = 0.f;
+  int tok = static_cast<int>(i0);
+  const auto flush = [&]() {
+#pragma unroll
+    for (int q = 0; q < S; ++q) {
+      if (on[q]) {
+        if (open) store_row<VEC>(a.head, BPC_DTYPE_F32, w * a.C + c[q], acc[q], 1.f);
+        else store_row<VEC>(a.dw, a.dw_dtype, static_cast<int64_t>(tok) * a.C + c[q], acc[q], a.scale);
       }
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) acc[q][e] = 0.f;
     }
     open = false;
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
     ++tok;
   };
+  const auto pairs = [&](int64_t j, int2 (&p)[kRows]) {
+#pragma unroll
+    for (int u = 0; u < kRows; ++u) p[u] = j + u < j1 ? a.pair[j + u] : make_int2(a.V, 0);
+  };
+  int2 next[kRows];
+  pairs(j0, next);
   for (int64_t j = j0; j < j1; j += kRows) {
-    int k[kRows];
-    Pack<T, VEC> x[kRows];
+    int2 p[kRows];
+    Piece x[kRows][S];
 #pragma unroll
     for (int u = 0; u < kRows; ++u) {
-      k[u] = a.V;
-      if (j + u < j1) {
-        k[u] = a.key[j + u];
-        if (on && k[u] < a.V) x[u] = *reinterpret_cast<const Pack<T, VEC>*>(gy + a.perm[j + u] * a.ldg + c);
+      p[u] = next[u];
+      if (p[u].x < a.V) {                                  // V: a position without a token, or past the end
+#pragma unroll
+        for (int q = 0; q < S; ++q)
+          if (on[q]) x[u][q] = load_pack<Piece>(gy + p[u].y * a.ldg + c[q]);
       }
     }
+    pairs(j + kRows, next);
 #pragma unroll
     for (int u = 0; u < kRows; ++u) {
-      if (k[u] < a.V) {                                    // key V: a position without a token, or past the end
-        while (tok < k[u]) flush();
-        if (on) {
+      if (p[u].x < a.V) {
+        while (tok < p[u].x) flush();
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) acc[e] += to_f32(x[u].v[e]);
-        }
+        for (int q = 0; q < S; ++q)
+          if (on[q])
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) acc[q][e] += to_f32(x[u][q].v[e]);
       }
     }
   }
   while (tok < i1) flush();
-  if (on && i1 < a.V && j1 > 0 && a.key[j1 - 1] == i1) {
+  if (i1 < a.V && j1 > 0 && a.pair[j1 - 1].x == i1) {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) a.tail[w * a.C + c + e] = acc[e];
+    for (int q = 0; q < S; ++q)
+      if (on[q]) store_row<VEC>(a.tail, BPC_DTYPE_F32, w * a.C + c[q], acc[q], 1.f);
   }
 }
 
-// One block per worker that ended a token begun before it: the tails of the workers since the token's first row, in
-// order, then its own head.
-__global__ void __launch_bounds__(256) wgrad_join_kernel(MergeArgs a) {
-  const int64_t w = blockIdx.x;
-  const int t = a.head_token[w];
-  if (t < 0) return;
-  int64_t lo = 0, hi = a.n;                                // first row of token t
-  while (lo < hi) {
-    const int64_t mid = (lo + hi) >> 1;
-    if (a.key[mid] < t) lo = mid + 1;
-    else hi = mid;
-  }
-  const int64_t first = (lo + t) / a.items;
-  for (int c = threadIdx.x; c < a.C; c += 256) {
-    float s = 0.f;
-    for (int64_t v = first; v < w; ++v) s += a.tail[v * a.C + c];
-    s += a.head[w * a.C + c];
-    store_row<1>(a.dw, a.dw_dtype, static_cast<int64_t>(t) * a.C + c, &s, a.scale);
+// A warp per token that crosses workers and 128 channels: the tails of the workers since its first row, then the last
+// one's head, in fp64.  One with more than kLongJoin tails is left to the block's warps together, each a fixed share.
+constexpr int kLongJoin = 64;
+constexpr int kJoinWarps = 32;
+
+__global__ void __launch_bounds__(kJoinWarps * 32) wgrad_join_kernel(MergeArgs a) {
+  __shared__ double red[kJoinWarps][32];
+  __shared__ int64_t task_worker[kJoinWarps], task_first[kJoinWarps], task_token[kJoinWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int c_from = blockIdx.y * 128, c_to = min(a.C, c_from + 128);
+  pdl_wait();
+  a.G = 32;
+  const int count = a.heads[0];
+  for (int base = blockIdx.x * kJoinWarps; base < count; base += gridDim.x * kJoinWarps) {
+    int64_t w = -1, first = 0, t = 0;
+    if (base + warp < count) {
+      w = a.heads[1 + base + warp];
+      t = path_search(a, w * a.items, lane, 0xffffffffu, 0);              // the token that its first step continues
+      int64_t lo = 0, hi = a.n;                            // the first row of token t is in [lo, hi]
+      while (lo < hi) {
+        const int64_t step = (hi - lo + 32) / 33, at = lo + (lane + 1) * step;
+        const bool below = at <= hi && a.pair[at - 1].x < t;
+        const int c = __popc(__ballot_sync(0xffffffffu, below));
+        const int64_t top = lo + (c + 1) * step - 1;
+        lo += c * step;
+        if (c < 32 && top < hi) hi = top;
+      }
+      first = (lo + t) / a.items;
+      if (w - first <= kLongJoin) {
+        for (int c = c_from + lane; c < c_to; c += 32) {
+          double s = 0.0;
+#pragma unroll 8
+          for (int64_t v = first; v < w; ++v) s += a.tail[v * a.C + c];
+          const float f = static_cast<float>(s + a.head[w * a.C + c]);
+          store_row<1>(a.dw, a.dw_dtype, t * a.C + c, &f, a.scale);
+        }
+        w = -1;
+      }
+    }
+    if (lane == 0) {
+      task_worker[warp] = w;
+      task_first[warp] = first;
+      task_token[warp] = t;
+    }
+    __syncthreads();
+    for (int k = 0; k < kJoinWarps; ++k) {
+      const int64_t v1 = task_worker[k];
+      if (v1 < 0) continue;
+      for (int c0 = c_from; c0 < c_to; c0 += 32) {
+        const int c = c0 + lane;
+        double s = 0.0;
+        if (c < c_to) {
+#pragma unroll 8
+          for (int64_t v = task_first[k] + warp; v < v1; v += kJoinWarps) s += a.tail[v * a.C + c];
+        }
+        red[warp][lane] = s;
+        __syncthreads();
+        if (warp == 0 && c < c_to) {
+          for (int q = 1; q < kJoinWarps; ++q) s += red[q][lane];
+          const float f = static_cast<float>(s + a.head[v1 * a.C + c]);
+          store_row<1>(a.dw, a.dw_dtype, task_token[k] * a.C + c, &f, a.scale);
+        }
+        __syncthreads();
+      }
+    }
+    __syncthreads();
   }
 }
 
@@ -569,11 +751,11 @@ __global__ void __launch_bounds__(1024) wgrad_few_join_kernel(const float* __res
 
 int dtype_size(int32_t dtype) { return dtype == BPC_DTYPE_F32 ? 4 : dtype == BPC_DTYPE_BF16 || dtype == BPC_DTYPE_F16 ? 2 : 0; }
 
-// Workspace layout of the gradient
+// Workspace layout of the gradient by sorted tokens
 struct WgradPlan {
   int passes, tiles, G;
   int64_t items, workers;
-  size_t key[2], perm[2], counts, totals, head, tail, head_token, bytes;
+  size_t pair[2], counts, totals, head, tail, heads, bytes;
 };
 
 // Few tokens: how a block reads its rows, by alignment and row length.
@@ -620,11 +802,11 @@ size_t few_bytes(int64_t n, int32_t V, int32_t C) {
 WgradPlan wgrad_plan(int64_t n, int32_t V, int32_t C) {
   WgradPlan p;
   int bits = 1;
-  while (bits < 32 && (static_cast<int64_t>(1) << bits) <= V) ++bits;      // keys are in [0, V]
+  while (bits < 32 && (static_cast<int64_t>(1) << bits) <= V) ++bits;      // tokens are in [0, V]
   p.passes = (bits + kDigitBits - 1) / kDigitBits;
   p.tiles = static_cast<int>((n + kSortTile - 1) / kSortTile);
   p.G = 1;
-  while (p.G < 32 && p.G * 8 < C) p.G *= 2;
+  while (p.G < 32 && p.G * 4 < C) p.G *= 2;
   // about 16 warps of workers per SM, of at least 32 steps
   const int64_t target = static_cast<int64_t>(num_sms()) * 16 * (32 / p.G);
   p.items = std::max<int64_t>(32, (V + n + target - 1) / target);
@@ -635,15 +817,12 @@ WgradPlan wgrad_plan(int64_t n, int32_t V, int32_t C) {
     at += (bytes + 255) & ~static_cast<size_t>(255);
     return r;
   };
-  for (int k = 0; k < 2; ++k) {
-    p.key[k] = take(sizeof(int) * n);
-    p.perm[k] = take(sizeof(int) * n);
-  }
+  for (int k = 0; k < 2; ++k) p.pair[k] = take(sizeof(int2) * n);
   p.counts = take(sizeof(int) * kBins * static_cast<size_t>(p.tiles));
   p.totals = take(sizeof(int) * kBins);
   p.head = take(sizeof(float) * p.workers * C);
   p.tail = take(sizeof(float) * p.workers * C);
-  p.head_token = take(sizeof(int) * p.workers);
+  p.heads = take(sizeof(int) * (p.workers + 1));
   p.bytes = at;
   return p;
 }
@@ -687,33 +866,84 @@ int lookup_by_w(const void* ids, const void* w, void* y, int64_t n, int V, int C
   return lookup_by_y<I, __half>(ids, w, y, n, V, C, ldw, scale, y_dtype, s);
 }
 
-template <typename I>
-int sort_pass(const I* src, const int* perm_in, int64_t n, int V, int shift, int tiles, int* counts, int* totals,
-              int* key_out, int* perm_out, cudaStream_t s) {
-  sort_count_kernel<I><<<tiles, kSortThreads, 0, s>>>(src, n, V, shift, counts, tiles);
+template <typename S>
+int sort_pass(const S* src, int64_t n, int V, int shift, int tiles, int* counts, int* totals, int2* out, int* zero,
+              cudaStream_t s) {
+  sort_count_kernel<S><<<tiles, kSortThreads, 0, s>>>(src, n, V, shift, counts, tiles);
   if (int e = launched("sort_count_kernel")) return e;
-  sort_scan_kernel<<<kBins, 256, 0, s>>>(counts, totals, tiles);
+  sort_scan_kernel<<<kBins, 256, 0, s>>>(counts, totals, tiles, zero);
   if (int e = launched("sort_scan_kernel")) return e;
-  sort_place_kernel<I><<<tiles, kSortThreads, 0, s>>>(src, perm_in, n, V, shift, counts, totals, tiles, key_out,
-                                                      perm_out);
+  sort_place_kernel<S><<<tiles, kSortThreads, 0, s>>>(src, n, V, shift, counts, totals, tiles, out);
   return launched("sort_place_kernel");
 }
 
-template <typename T>
-int merge_launch(const void* gy, MergeArgs a, cudaStream_t s) {
-  constexpr int kVec = 16 / sizeof(T);
-  const bool wide = a.C % kVec == 0 && a.ldg % kVec == 0 && reinterpret_cast<uintptr_t>(gy) % 16 == 0 &&
-                    reinterpret_cast<uintptr_t>(a.dw) % 16 == 0;
-  const int vec = wide ? kVec : 1;
+template <typename I, int ROUNDS>
+int sort_cluster_rounds(const I* ids, int n, int V, int passes, int2* a, int2* b, int* zero, cudaStream_t s) {
+  cudaLaunchConfig_t lc = {};
+  lc.gridDim = dim3(kClusterCtas);
+  lc.blockDim = dim3(kClusterThreads);
+  lc.stream = s;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = kClusterCtas;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  lc.attrs = &attr;
+  lc.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&lc, sort_cluster_kernel<I, ROUNDS>, ids, n, V, passes, a, b, zero);
+  return e == cudaSuccess ? 0 : fail(BPC_ERR_LAUNCH, std::string("sort_cluster_kernel launch: ") + cudaGetErrorString(e));
+}
+
+template <typename I>
+int sort_cluster(const I* ids, int n, int V, int passes, int2* a, int2* b, int* zero, cudaStream_t s) {
+  constexpr int kRound = kClusterCtas * kClusterThreads;
+  if (n <= kRound) return sort_cluster_rounds<I, 1>(ids, n, V, passes, a, b, zero, s);
+  if (n <= 2 * kRound) return sort_cluster_rounds<I, 2>(ids, n, V, passes, a, b, zero, s);
+  if (n <= 4 * kRound) return sort_cluster_rounds<I, 4>(ids, n, V, passes, a, b, zero, s);
+  return sort_cluster_rounds<I, 8>(ids, n, V, passes, a, b, zero, s);
+}
+
+template <typename I>
+int sort_ids(const I* ids, int64_t n, int V, const WgradPlan& p, int2* const (&pair)[2], int* counts, int* totals,
+             int* zero, cudaStream_t s) {
+  if (n <= kClusterKeys) return sort_cluster(ids, static_cast<int>(n), V, p.passes, pair[0], pair[1], zero, s);
+  if (int e = sort_pass(ids, n, V, 0, p.tiles, counts, totals, pair[0], zero, s)) return e;
+  for (int k = 1; k < p.passes; ++k)
+    if (int e = sort_pass(static_cast<const int2*>(pair[(k - 1) & 1]), n, V, k * kDigitBits, p.tiles, counts, totals,
+                          pair[k & 1], zero, s))
+      return e;
+  return 0;
+}
+
+template <typename T, int VEC, int S>
+int merge_launch_pieces(const T* gy, MergeArgs a, cudaStream_t s) {
   const int64_t blocks = (a.workers + 256 / a.G - 1) / (256 / a.G);
-  const dim3 grid(static_cast<unsigned>(blocks), (a.C + a.G * vec - 1) / (a.G * vec));
-  if (wide)
-    wgrad_merge_kernel<T, kVec><<<grid, 256, 0, s>>>(static_cast<const T*>(gy), a);
-  else
-    wgrad_merge_kernel<T, 1><<<grid, 256, 0, s>>>(static_cast<const T*>(gy), a);
-  if (int e = launched("wgrad_merge_kernel")) return e;
-  wgrad_join_kernel<<<static_cast<unsigned>(a.workers), 256, 0, s>>>(a);
-  return launched("wgrad_join_kernel");
+  const dim3 grid(static_cast<unsigned>(blocks), (a.C + a.G * VEC * S - 1) / (a.G * VEC * S));
+  void* args[] = {&gy, &a};
+  if (int e = launch_pdl(reinterpret_cast<const void*>(&wgrad_merge_kernel<T, VEC, S>), grid, dim3(256), 0, s, args, 1,
+                         "wgrad_merge_kernel"))
+    return e;
+  void* join_args[] = {&a};
+  const int64_t join = std::min<int64_t>((a.workers + kJoinWarps - 1) / kJoinWarps, num_sms());
+  return launch_pdl(reinterpret_cast<const void*>(&wgrad_join_kernel), dim3(static_cast<unsigned>(join), (a.C + 127) / 128),
+                    dim3(kJoinWarps * 32), 0, s, join_args, 1, "wgrad_join_kernel");
+}
+
+template <typename T, int VEC>
+int merge_launch_vec(const T* gy, const MergeArgs& a, cudaStream_t s) {
+  return a.C > 32 * VEC ? merge_launch_pieces<T, VEC, 2>(gy, a, s) : merge_launch_pieces<T, VEC, 1>(gy, a, s);
+}
+
+template <typename T>
+int merge_launch(const void* gy, const MergeArgs& a, cudaStream_t s) {
+  const auto fits = [&](int vec) {
+    return a.C % vec == 0 && a.ldg % vec == 0 && reinterpret_cast<uintptr_t>(gy) % (vec * sizeof(T)) == 0 &&
+           reinterpret_cast<uintptr_t>(a.dw) % (vec * dtype_size(a.dw_dtype)) == 0;
+  };
+  const T* g = static_cast<const T*>(gy);
+  // 16 bytes of the wider of gy and the fp32 sums that head and tail hold
+  if (fits(4)) return merge_launch_vec<T, 4>(g, a, s);
+  if (fits(2)) return merge_launch_vec<T, 2>(g, a, s);
+  return merge_launch_vec<T, 1>(g, a, s);
 }
 
 template <typename T, typename I, int VEC, int NV>
@@ -828,24 +1058,15 @@ extern "C" int bpc_embed_wgrad(const void* gy, const void* ids, int32_t id_bytes
   }
   const WgradPlan p = wgrad_plan(n, V, C);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  int* key[2] = {reinterpret_cast<int*>(ws + p.key[0]), reinterpret_cast<int*>(ws + p.key[1])};
-  int* perm[2] = {reinterpret_cast<int*>(ws + p.perm[0]), reinterpret_cast<int*>(ws + p.perm[1])};
+  int2* const pair[2] = {reinterpret_cast<int2*>(ws + p.pair[0]), reinterpret_cast<int2*>(ws + p.pair[1])};
   int* counts = reinterpret_cast<int*>(ws + p.counts);
   int* totals = reinterpret_cast<int*>(ws + p.totals);
-  for (int k = 0; k < p.passes; ++k) {
-    int e;
-    if (k == 0 && id_bytes == 8)
-      e = sort_pass(static_cast<const int64_t*>(ids), nullptr, n, V, 0, p.tiles, counts, totals, key[0], perm[0], s);
-    else if (k == 0)
-      e = sort_pass(static_cast<const int32_t*>(ids), nullptr, n, V, 0, p.tiles, counts, totals, key[0], perm[0], s);
-    else
-      e = sort_pass(static_cast<const int*>(key[(k - 1) & 1]), perm[(k - 1) & 1], n, V, k * kDigitBits, p.tiles, counts,
-                    totals, key[k & 1], perm[k & 1], s);
-    if (e) return e;
-  }
+  int* heads = reinterpret_cast<int*>(ws + p.heads);
+  const int e = id_bytes == 8 ? sort_ids(static_cast<const int64_t*>(ids), n, V, p, pair, counts, totals, heads, s)
+                              : sort_ids(static_cast<const int32_t*>(ids), n, V, p, pair, counts, totals, heads, s);
+  if (e) return e;
   MergeArgs a;
-  a.key = key[(p.passes - 1) & 1];
-  a.perm = perm[(p.passes - 1) & 1];
+  a.pair = pair[(p.passes - 1) & 1];
   a.n = n;
   a.items = p.items;
   a.workers = p.workers;
@@ -858,7 +1079,7 @@ extern "C" int bpc_embed_wgrad(const void* gy, const void* ids, int32_t id_bytes
   a.dw_dtype = dw_dtype;
   a.head = reinterpret_cast<float*>(ws + p.head);
   a.tail = reinterpret_cast<float*>(ws + p.tail);
-  a.head_token = reinterpret_cast<int*>(ws + p.head_token);
+  a.heads = heads;
   if (gy_dtype == BPC_DTYPE_F32) return merge_launch<float>(gy, a, s);
   if (gy_dtype == BPC_DTYPE_BF16) return merge_launch<__nv_bfloat16>(gy, a, s);
   return merge_launch<__half>(gy, a, s);
