@@ -97,14 +97,26 @@ __device__ __forceinline__ int warp_inclusive(int s, int lane) {
   return s;
 }
 
+// the lanes whose digit is this lane's, from one ballot per bit (a key of none: any lanes)
+__device__ __forceinline__ unsigned same_digit(int digit) {
+  unsigned same = 0xffffffffu;
+#pragma unroll
+  for (int b = 0; b < kDigitBits; ++b) {
+    const bool set = digit >> b & 1;
+    const unsigned m = __ballot_sync(0xffffffffu, set);
+    same &= set ? m : ~m;
+  }
+  return same;
+}
+
 // The ranks of a warp's ROUNDS x 32 consecutive keys among its earlier ones of the same digit; cnt (kBins, the warp's own,
 // zero before) counts its digits.  A negative key is none.
 template <int ROUNDS, typename N>
 __device__ __forceinline__ void warp_ranks(const int (&key)[ROUNDS], int (&rank)[ROUNDS], int shift, N* cnt, int lane) {
 #pragma unroll
   for (int r = 0; r < ROUNDS; ++r) {
-    const int digit = key[r] < 0 ? kBins : (key[r] >> shift) & (kBins - 1);
-    const unsigned same = __match_any_sync(0xffffffffu, digit);
+    const int digit = (key[r] >> shift) & (kBins - 1);
+    const unsigned same = same_digit(digit) & __ballot_sync(0xffffffffu, key[r] >= 0);
     const int before = key[r] < 0 ? 0 : cnt[digit];
     rank[r] = before + __popc(same & ((1u << lane) - 1));
     __syncwarp();
@@ -230,8 +242,8 @@ __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(const S* __res
   }
 #pragma unroll
   for (int r = 0; r < kSortRounds; ++r) {
-    const int digit = key[r] < 0 ? kBins : (key[r] >> shift) & (kBins - 1);
-    const unsigned same = __match_any_sync(0xffffffffu, digit);
+    const int digit = (key[r] >> shift) & (kBins - 1);
+    const unsigned same = same_digit(digit) & __ballot_sync(0xffffffffu, key[r] >= 0);
     if (key[r] >= 0 && (threadIdx.x & 31) == __ffs(same) - 1) atomicAdd(&cnt[digit], __popc(same));
   }
   __syncthreads();
@@ -331,7 +343,7 @@ struct MergeArgs {
   int dw_dtype;
   float* head;         // (workers, C)
   float* tail;
-  int* heads;          // [0]: how many; [1 ..]: the workers with a head, in no order
+  int2* heads;         // [0].x: how many; [1 ..]: {worker, token} with a head, in no order
 };
 
 // The tokens finished within the first d steps of the path, by the G lanes of a worker together: each step of the search
@@ -374,12 +386,27 @@ __device__ __forceinline__ void store_row(void* dw, int dtype, int64_t at, const
   }
 }
 
-// S pieces of VEC channels per lane, 32 VEC channels apart
+// Pieces of less than 4 bytes have no asynchronous copy.
+template <typename P>
+__device__ __forceinline__ void copy_ahead(P* smem, const void* global) {
+  if constexpr (sizeof(P) >= 4)
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(smem)), "l"(global), "n"(sizeof(P)) : "memory");
+  else
+    *smem = load_pack<P>(global);
+}
+
+// S pieces of VEC channels per lane, G VEC channels apart.  Every lane copies its pieces of the rows ahead into its own
+// slots of shared memory (and reads only those, so no barrier is needed): the loads in flight do not depend on the
+// registers, which held a block of eight rows to two per SM.
+constexpr int kMergeRows = 8;                             // rows whose loads are in flight per worker
+
 template <typename T, int VEC, int S>
 __global__ void __launch_bounds__(256) wgrad_merge_kernel(const T* __restrict__ gy, const __grid_constant__ MergeArgs a) {
-  constexpr int kRows = S == 1 ? 8 : 4;                   // rows whose loads are in flight per worker
   typedef Pack<T, VEC> Piece;
+  extern __shared__ uint4 merge_smem[];                    // pieces (kMergeRows, S, 256), then tokens (kMergeRows, 256)
   __shared__ int64_t starts[257];
+  Piece* const slots = reinterpret_cast<Piece*>(merge_smem) + threadIdx.x;
+  int* const tokens = reinterpret_cast<int*>(reinterpret_cast<Piece*>(merge_smem) + kMergeRows * S * 256) + threadIdx.x;
   const int l = threadIdx.x % a.G, mine = threadIdx.x / a.G, per_block = 256 / a.G;
   const int64_t w = blockIdx.x * static_cast<int64_t>(per_block) + mine;
   const int64_t end = a.V + a.n, d0 = min(end, w * a.items), d1 = min(end, d0 + a.items);
@@ -397,29 +424,24 @@ __global__ void __launch_bounds__(256) wgrad_merge_kernel(const T* __restrict__ 
   }
   __syncthreads();
   if (w >= a.workers) return;
-  const int64_t i0 = starts[mine], i1 = starts[mine + 1];
-  const int64_t j0 = d0 - i0, j1 = d1 - i1;
-  int c[S];
-  bool on[S];
-#pragma unroll
-  for (int q = 0; q < S; ++q) {
-    c[q] = ((blockIdx.y * S + q) * a.G + l) * VEC;
-    on[q] = c[q] < a.C;
-  }
+  const int i0 = static_cast<int>(starts[mine]), i1 = static_cast<int>(starts[mine + 1]);
+  const int j0 = static_cast<int>(d0 - i0), j1 = static_cast<int>(d1 - i1);
+  const int c = (blockIdx.y * S * a.G + l) * VEC, apart = a.G * VEC;     // piece q: channels c + q apart ..
   bool open = j0 > 0 && i0 < a.V && a.pair[j0 - 1].x == i0;               // token i0 began in an earlier worker
-  if (open && i1 > i0 && l == 0 && blockIdx.y == 0) a.heads[1 + atomicAdd(a.heads, 1)] = static_cast<int>(w);
+  if (open && i1 > i0 && l == 0 && blockIdx.y == 0)
+    a.heads[1 + atomicAdd(&a.heads[0].x, 1)] = make_int2(static_cast<int>(w), i0);
   float acc[S][VEC];
 #pragma unroll
   for (int q = 0; q < S; ++q)
 #pragma unroll
     for (int e = 0; e < VEC; ++e) acc[q][e] = 0.f;
-  int tok = static_cast<int>(i0);
+  int tok = i0;
   const auto flush = [&]() {
 #pragma unroll
     for (int q = 0; q < S; ++q) {
-      if (on[q]) {
-        if (open) store_row<VEC>(a.head, BPC_DTYPE_F32, w * a.C + c[q], acc[q], 1.f);
-        else store_row<VEC>(a.dw, a.dw_dtype, static_cast<int64_t>(tok) * a.C + c[q], acc[q], a.scale);
+      if (c + q * apart < a.C) {
+        if (open) store_row<VEC>(a.head, BPC_DTYPE_F32, w * a.C + c + q * apart, acc[q], 1.f);
+        else store_row<VEC>(a.dw, a.dw_dtype, static_cast<int64_t>(tok) * a.C + c + q * apart, acc[q], a.scale);
       }
 #pragma unroll
       for (int e = 0; e < VEC; ++e) acc[q][e] = 0.f;
@@ -427,63 +449,94 @@ __global__ void __launch_bounds__(256) wgrad_merge_kernel(const T* __restrict__ 
     open = false;
     ++tok;
   };
-  const auto pairs = [&](int64_t j, int2 (&p)[kRows]) {
+  // row j into slot u; the pair of the row after it is read one call ahead
+  int2 ahead = j0 < j1 ? a.pair[j0] : make_int2(a.V, 0);
+  int next = j0;
+  const auto copy_row = [&](int u) {
+    if (next < j1) {
+      const int2 p = ahead;
+      ++next;
+      if (next < j1) ahead = a.pair[next];
+      tokens[u * 256] = p.x;
+      if (p.x < a.V) {                                     // V: a position without a token
+        const T* row = gy + p.y * a.ldg + c;
 #pragma unroll
-    for (int u = 0; u < kRows; ++u) p[u] = j + u < j1 ? a.pair[j + u] : make_int2(a.V, 0);
+        for (int q = 0; q < S; ++q)
+          if (c + q * apart < a.C) copy_ahead(slots + (u * S + q) * 256, row + q * apart);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  int2 next[kRows];
-  pairs(j0, next);
-  for (int64_t j = j0; j < j1; j += kRows) {
-    int2 p[kRows];
-    Piece x[kRows][S];
 #pragma unroll
-    for (int u = 0; u < kRows; ++u) {
-      p[u] = next[u];
-      if (p[u].x < a.V) {                                  // V: a position without a token, or past the end
+  for (int u = 0; u < kMergeRows - 1; ++u) copy_row(u);
+  int u = 0;
+  for (int j = j0; j < j1; ++j) {
+    copy_row(u == 0 ? kMergeRows - 1 : u - 1);             // into the slot that the step before read
+    asm volatile("cp.async.wait_group %0;" ::"n"(kMergeRows - 1) : "memory");
+    const int t = tokens[u * 256];
+    if (t >= a.V) break;                                   // they are the last ones
+    while (tok < t) flush();
 #pragma unroll
-        for (int q = 0; q < S; ++q)
-          if (on[q]) x[u][q] = load_pack<Piece>(gy + p[u].y * a.ldg + c[q]);
+    for (int q = 0; q < S; ++q) {
+      if (c + q * apart < a.C) {
+        const Piece x = load_pack<Piece>(slots + (u * S + q) * 256);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) acc[q][e] += to_f32(x.v[e]);
       }
     }
-    pairs(j + kRows, next);
-#pragma unroll
-    for (int u = 0; u < kRows; ++u) {
-      if (p[u].x < a.V) {
-        while (tok < p[u].x) flush();
-#pragma unroll
-        for (int q = 0; q < S; ++q)
-          if (on[q])
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) acc[q][e] += to_f32(x[u][q].v[e]);
-      }
-    }
+    u = u == kMergeRows - 1 ? 0 : u + 1;
   }
   while (tok < i1) flush();
   if (i1 < a.V && j1 > 0 && a.pair[j1 - 1].x == i1) {
 #pragma unroll
     for (int q = 0; q < S; ++q)
-      if (on[q]) store_row<VEC>(a.tail, BPC_DTYPE_F32, w * a.C + c[q], acc[q], 1.f);
+      if (c + q * apart < a.C) store_row<VEC>(a.tail, BPC_DTYPE_F32, w * a.C + c + q * apart, acc[q], 1.f);
   }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 // A warp per token that crosses workers and 128 channels: the tails of the workers since its first row, then the last
 // one's head, in fp64.  One with more than kLongJoin tails is left to the block's warps together, each a fixed share.
-constexpr int kLongJoin = 64;
-constexpr int kJoinWarps = 32;
+constexpr int kLongJoin = 128;
+constexpr int kJoinWarps = 8;
+constexpr int kJoinChannels = 128;
 
-__global__ void __launch_bounds__(kJoinWarps * 32) wgrad_join_kernel(MergeArgs a) {
-  __shared__ double red[kJoinWarps][32];
+template <int VEC>
+__global__ void __launch_bounds__(kJoinWarps * 32) wgrad_join_kernel(const __grid_constant__ MergeArgs a) {
+  __shared__ double red[kJoinWarps][32 * VEC];
   __shared__ int64_t task_worker[kJoinWarps], task_first[kJoinWarps], task_token[kJoinWarps];
+  typedef Pack<float, VEC> Piece;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int c_from = blockIdx.y * 128, c_to = min(a.C, c_from + 128);
+  const int c_from = blockIdx.y * kJoinChannels, c_to = min(a.C, c_from + kJoinChannels);
   pdl_wait();
-  a.G = 32;
-  const int count = a.heads[0];
+  // s += tails v0, v0 + by .. below v1, at this lane's channels
+  const auto add_tails = [&](double (&s)[VEC], int64_t v0, int64_t v1, int by, int c) {
+    for (int64_t v = v0; v < v1; v += 8 * by) {
+      Piece x[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (v + u * by < v1) x[u] = load_pack<Piece>(a.tail + (v + u * by) * a.C + c);
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (v + u * by < v1)
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) s[e] += x[u].v[e];
+    }
+  };
+  const auto finish = [&](const double (&s)[VEC], int64_t w, int64_t t, int c) {
+    const Piece h = load_pack<Piece>(a.head + w * a.C + c);
+    float f[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) f[e] = static_cast<float>(s[e] + h.v[e]);
+    store_row<VEC>(a.dw, a.dw_dtype, t * a.C + c, f, a.scale);
+  };
+  const int count = a.heads[0].x;
   for (int base = blockIdx.x * kJoinWarps; base < count; base += gridDim.x * kJoinWarps) {
     int64_t w = -1, first = 0, t = 0;
     if (base + warp < count) {
-      w = a.heads[1 + base + warp];
-      t = path_search(a, w * a.items, lane, 0xffffffffu, 0);              // the token that its first step continues
+      const int2 head = a.heads[1 + base + warp];
+      w = head.x;
+      t = head.y;
       int64_t lo = 0, hi = a.n;                            // the first row of token t is in [lo, hi]
       while (lo < hi) {
         const int64_t step = (hi - lo + 32) / 33, at = lo + (lane + 1) * step;
@@ -495,12 +548,10 @@ __global__ void __launch_bounds__(kJoinWarps * 32) wgrad_join_kernel(MergeArgs a
       }
       first = (lo + t) / a.items;
       if (w - first <= kLongJoin) {
-        for (int c = c_from + lane; c < c_to; c += 32) {
-          double s = 0.0;
-#pragma unroll 8
-          for (int64_t v = first; v < w; ++v) s += a.tail[v * a.C + c];
-          const float f = static_cast<float>(s + a.head[w * a.C + c]);
-          store_row<1>(a.dw, a.dw_dtype, t * a.C + c, &f, a.scale);
+        for (int c = c_from + lane * VEC; c < c_to; c += 32 * VEC) {
+          double s[VEC] = {};
+          add_tails(s, first, w, 1, c);
+          finish(s, w, t, c);
         }
         w = -1;
       }
@@ -514,19 +565,18 @@ __global__ void __launch_bounds__(kJoinWarps * 32) wgrad_join_kernel(MergeArgs a
     for (int k = 0; k < kJoinWarps; ++k) {
       const int64_t v1 = task_worker[k];
       if (v1 < 0) continue;
-      for (int c0 = c_from; c0 < c_to; c0 += 32) {
-        const int c = c0 + lane;
-        double s = 0.0;
-        if (c < c_to) {
-#pragma unroll 8
-          for (int64_t v = task_first[k] + warp; v < v1; v += kJoinWarps) s += a.tail[v * a.C + c];
-        }
-        red[warp][lane] = s;
+      for (int c0 = c_from; c0 < c_to; c0 += 32 * VEC) {
+        const int c = c0 + lane * VEC;
+        double s[VEC] = {};
+        if (c < c_to) add_tails(s, task_first[k] + warp, v1, kJoinWarps, c);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) red[warp][lane * VEC + e] = s[e];
         __syncthreads();
         if (warp == 0 && c < c_to) {
-          for (int q = 1; q < kJoinWarps; ++q) s += red[q][lane];
-          const float f = static_cast<float>(s + a.head[v1 * a.C + c]);
-          store_row<1>(a.dw, a.dw_dtype, task_token[k] * a.C + c, &f, a.scale);
+          for (int q = 1; q < kJoinWarps; ++q)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) s[e] += red[q][lane * VEC + e];
+          finish(s, v1, task_token[k], c);
         }
         __syncthreads();
       }
@@ -807,9 +857,9 @@ WgradPlan wgrad_plan(int64_t n, int32_t V, int32_t C) {
   p.tiles = static_cast<int>((n + kSortTile - 1) / kSortTile);
   p.G = 1;
   while (p.G < 32 && p.G * 4 < C) p.G *= 2;
-  // about 16 warps of workers per SM, of at least 32 steps
-  const int64_t target = static_cast<int64_t>(num_sms()) * 16 * (32 / p.G);
-  p.items = std::max<int64_t>(32, (V + n + target - 1) / target);
+  // about 32 warps per SM over the workers and the slices of 256 channels, at least 16 steps a worker
+  const int64_t target = std::max<int64_t>(1, static_cast<int64_t>(num_sms()) * 32 * (32 / p.G) / ((C + 255) / 256));
+  p.items = std::max<int64_t>(16, (V + n + target - 1) / target);
   p.workers = (V + n + p.items - 1) / p.items;
   size_t at = 0;
   auto take = [&](size_t bytes) {
@@ -822,7 +872,7 @@ WgradPlan wgrad_plan(int64_t n, int32_t V, int32_t C) {
   p.totals = take(sizeof(int) * kBins);
   p.head = take(sizeof(float) * p.workers * C);
   p.tail = take(sizeof(float) * p.workers * C);
-  p.heads = take(sizeof(int) * (p.workers + 1));
+  p.heads = take(sizeof(int2) * (p.workers + 1));
   p.bytes = at;
   return p;
 }
@@ -919,12 +969,14 @@ int merge_launch_pieces(const T* gy, MergeArgs a, cudaStream_t s) {
   const int64_t blocks = (a.workers + 256 / a.G - 1) / (256 / a.G);
   const dim3 grid(static_cast<unsigned>(blocks), (a.C + a.G * VEC * S - 1) / (a.G * VEC * S));
   void* args[] = {&gy, &a};
-  if (int e = launch_pdl(reinterpret_cast<const void*>(&wgrad_merge_kernel<T, VEC, S>), grid, dim3(256), 0, s, args, 1,
-                         "wgrad_merge_kernel"))
-    return e;
+  const void* fn = reinterpret_cast<const void*>(&wgrad_merge_kernel<T, VEC, S>);
+  constexpr int kSmem = kMergeRows * 256 * (S * VEC * static_cast<int>(sizeof(T)) + static_cast<int>(sizeof(int)));
+  if (int e = allow_smem(fn, kSmem)) return e;
+  if (int e = launch_pdl(fn, grid, dim3(256), kSmem, s, args, 1, "wgrad_merge_kernel")) return e;
   void* join_args[] = {&a};
-  const int64_t join = std::min<int64_t>((a.workers + kJoinWarps - 1) / kJoinWarps, num_sms());
-  return launch_pdl(reinterpret_cast<const void*>(&wgrad_join_kernel), dim3(static_cast<unsigned>(join), (a.C + 127) / 128),
+  const int64_t join = std::min<int64_t>((a.workers + kJoinWarps - 1) / kJoinWarps, 4 * num_sms());
+  return launch_pdl(reinterpret_cast<const void*>(&wgrad_join_kernel<VEC>),
+                    dim3(static_cast<unsigned>(join), (a.C + kJoinChannels - 1) / kJoinChannels),
                     dim3(kJoinWarps * 32), 0, s, join_args, 1, "wgrad_join_kernel");
 }
 
@@ -1061,9 +1113,10 @@ extern "C" int bpc_embed_wgrad(const void* gy, const void* ids, int32_t id_bytes
   int2* const pair[2] = {reinterpret_cast<int2*>(ws + p.pair[0]), reinterpret_cast<int2*>(ws + p.pair[1])};
   int* counts = reinterpret_cast<int*>(ws + p.counts);
   int* totals = reinterpret_cast<int*>(ws + p.totals);
-  int* heads = reinterpret_cast<int*>(ws + p.heads);
-  const int e = id_bytes == 8 ? sort_ids(static_cast<const int64_t*>(ids), n, V, p, pair, counts, totals, heads, s)
-                              : sort_ids(static_cast<const int32_t*>(ids), n, V, p, pair, counts, totals, heads, s);
+  int2* heads = reinterpret_cast<int2*>(ws + p.heads);
+  int* zero = reinterpret_cast<int*>(heads);
+  const int e = id_bytes == 8 ? sort_ids(static_cast<const int64_t*>(ids), n, V, p, pair, counts, totals, zero, s)
+                              : sort_ids(static_cast<const int32_t*>(ids), n, V, p, pair, counts, totals, zero, s);
   if (e) return e;
   MergeArgs a;
   a.pair = pair[(p.passes - 1) & 1];
