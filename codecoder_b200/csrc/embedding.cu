@@ -53,27 +53,42 @@ __device__ __forceinline__ P load_pack(const void* p) {
   return x;
 }
 
+template <typename P>
+__device__ __forceinline__ void store_pack(void* p, const P& x) {
+  typename Word<sizeof(P)>::type w;
+  memcpy(&w, &x, sizeof(P));
+  *static_cast<typename Word<sizeof(P)>::type*>(p) = w;
+}
+
 // ---------------------------------------------------------------------------------------------------------------
-// lookup: one thread per VEC channels of a row
+// lookup: the threads lie along a row's pieces of VEC channels and several rows, kLookupRows rows per thread in flight
+// (one at a time left the stores waiting for the ids' and the table's latency: 5.0 TB/s at 258,048 rows of 512 fp32).
+constexpr int kLookupRows = 4;
+
 template <typename I, typename TW, typename TY, int VEC>
 __global__ void __launch_bounds__(256) embed_lookup_kernel(const I* __restrict__ ids, const TW* __restrict__ w,
-                                                           TY* __restrict__ y, int64_t units, int V, int CV,
-                                                           int64_t ldw, float scale) {
-  for (int64_t u = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; u < units;
-       u += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    const int64_t row = u / CV;
-    const int c = static_cast<int>(u - row * CV) * VEC;
-    const int64_t id = ids[row];
-    Pack<TY, VEC> o;
-    if (id >= 0 && id < V) {
-      const Pack<TW, VEC> x = *reinterpret_cast<const Pack<TW, VEC>*>(w + id * ldw + c);
+                                                           TY* __restrict__ y, int64_t n, int V, int C, int pieces,
+                                                           int rows_at_once, int64_t ldw, float scale) {
+  const int tx = threadIdx.x % pieces, ty = threadIdx.x / pieces;
+  const int c = (blockIdx.y * pieces + tx) * VEC;
+  if (ty >= rows_at_once || c >= C) return;
+  const int64_t batch = static_cast<int64_t>(rows_at_once) * kLookupRows;
+  for (int64_t r = blockIdx.x * batch + ty; r < n; r += gridDim.x * batch) {
+    int64_t id[kLookupRows];
+    Pack<TW, VEC> x[kLookupRows];
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) o.v[e] = from_f32<TY>(scale * to_f32(x.v[e]));
-    } else {
+    for (int u = 0; u < kLookupRows; ++u) id[u] = r + u * rows_at_once < n ? static_cast<int64_t>(ids[r + u * rows_at_once]) : -1;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) o.v[e] = from_f32<TY>(0.f);
+    for (int u = 0; u < kLookupRows; ++u)
+      if (id[u] >= 0 && id[u] < V) x[u] = load_pack<Pack<TW, VEC>>(w + id[u] * ldw + c);
+#pragma unroll
+    for (int u = 0; u < kLookupRows; ++u) {
+      const bool in = id[u] >= 0 && id[u] < V;
+      Pack<TY, VEC> o;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) o.v[e] = from_f32<TY>(in ? scale * to_f32(x[u].v[e]) : 0.f);
+      if (r + u * rows_at_once < n) store_pack(y + (r + u * rows_at_once) * C + c, o);
     }
-    *reinterpret_cast<Pack<TY, VEC>*>(y + u * VEC) = o;
   }
 }
 
@@ -126,8 +141,8 @@ __device__ __forceinline__ void warp_ranks(const int (&key)[ROUNDS], int (&rank)
 }
 
 // Up to kClusterKeys positions: one cluster of 8 CTAs runs every pass in one launch (separate launches of three kernels a
-// pass took 66 us for 32,768 positions, most of it latency).  The CTAs exchange their digit counts through distributed
-// shared memory and the pairs through L2.
+// pass took 66 us for 32,768 positions, most of it latency).  The CTAs exchange digit counts and pairs through
+// distributed shared memory: each holds a run of ROUNDS x 1024 places.
 constexpr int kClusterCtas = 8;
 constexpr int kClusterThreads = 1024;
 constexpr int kClusterKeys = kClusterCtas * kClusterThreads * 8;
@@ -135,42 +150,44 @@ constexpr int kClusterKeys = kClusterCtas * kClusterThreads * 8;
 __device__ __forceinline__ void st_cluster(uint32_t addr, int v) {
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
+__device__ __forceinline__ void st_cluster(uint32_t addr, int x, int y) {
+  asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(addr), "r"(x), "r"(y) : "memory");
+}
 
 template <typename I, int ROUNDS>
 __global__ void __launch_bounds__(kClusterThreads) sort_cluster_kernel(const I* __restrict__ ids, int n, int V, int passes,
-                                                                       int2* __restrict__ a, int2* __restrict__ b,
-                                                                       int* __restrict__ zero) {
+                                                                       int2* __restrict__ out, int* __restrict__ zero) {
+  extern __shared__ int2 places[];                         // (ROUNDS x 1024) this CTA's run
   __shared__ uint16_t cnt[kClusterThreads / 32][kBins];
   __shared__ int hist[2][kClusterCtas][kBins];             // every CTA's counts of this pass; two, so that a pass may
   __shared__ int warp_sum[kBins / 32];                     // write while a slower CTA still reads the one before
+  constexpr int kRun = ROUNDS * kClusterThreads;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int cta = static_cast<int>(cluster_ctarank());
-  const int first = (cta * kClusterThreads + warp * 32) * ROUNDS + lane;
+  const int first = warp * 32 * ROUNDS + lane;             // of this thread's places in the run
   pdl_launch_dependents();
   if (cta == 0 && tid == 0) *zero = 0;
   cluster_arrive_release();                                // every CTA runs before another writes its shared memory
   cluster_wait_acquire();
   for (int pass = 0; pass < passes; ++pass) {
-    int2* const to = pass & 1 ? b : a;
-    const int2* const from = pass & 1 ? a : b;
     const int shift = pass * kDigitBits;
     int key[ROUNDS], pos[ROUNDS], rank[ROUNDS];
 #pragma unroll
     for (int r = 0; r < ROUNDS; ++r) {
-      const int i = first + r * 32;
+      const int i = cta * kRun + first + r * 32;
       key[r] = -1;
       pos[r] = i;
       if (i < n) {
         if (pass == 0) {
           key[r] = token_key(ids[i], V);
         } else {
-          const int2 p = __ldcg(from + i);                 // written by the other CTAs: from L2
+          const int2 p = places[first + r * 32];
           key[r] = p.x;
           pos[r] = p.y;
         }
       }
     }
-    for (int k = tid; k < kClusterThreads / 32 * kBins; k += kClusterThreads) (&cnt[0][0])[k] = 0;
+    for (int k = tid; k < kClusterThreads / 32 * kBins / 2; k += kClusterThreads) reinterpret_cast<int*>(cnt)[k] = 0;
     __syncthreads();
     warp_ranks(key, rank, shift, cnt[warp], lane);
     __syncthreads();
@@ -184,7 +201,7 @@ __global__ void __launch_bounds__(kClusterThreads) sort_cluster_kernel(const I* 
       }
       for (int k = 0; k < kClusterCtas; ++k) st_cluster(map_to_cta(smem_u32(&hist[pass & 1][cta][tid]), k), at);
     }
-    cluster_arrive_release();
+    cluster_arrive_release();                              // counts written, and every run read
     cluster_wait_acquire();
     int total = 0, before = 0, s = 0;
     if (tid < kBins) {
@@ -204,15 +221,22 @@ __global__ void __launch_bounds__(kClusterThreads) sort_cluster_kernel(const I* 
       hist[pass & 1][cta][tid] = at;                       // only this CTA reads its own row from here on
     }
     __syncthreads();
+    const uint32_t base = smem_u32(places);
 #pragma unroll
     for (int r = 0; r < ROUNDS; ++r) {
       if (key[r] >= 0) {
         const int digit = (key[r] >> shift) & (kBins - 1);
-        to[hist[pass & 1][cta][digit] + cnt[warp][digit] + rank[r]] = make_int2(key[r], pos[r]);
+        const int to = hist[pass & 1][cta][digit] + cnt[warp][digit] + rank[r];
+        st_cluster(map_to_cta(base + to % kRun * 8, to / kRun), key[r], pos[r]);
       }
     }
-    cluster_arrive_release();                              // the pairs are written, and every count read
+    cluster_arrive_release();                              // the pairs are in their places
     cluster_wait_acquire();
+  }
+#pragma unroll
+  for (int r = 0; r < ROUNDS; ++r) {
+    const int i = tid + r * kClusterThreads;
+    if (cta * kRun + i < n) out[cta * kRun + i] = places[i];
   }
 }
 
@@ -386,13 +410,10 @@ __device__ __forceinline__ void store_row(void* dw, int dtype, int64_t at, const
   }
 }
 
-// Pieces of less than 4 bytes have no asynchronous copy.
-template <typename P>
-__device__ __forceinline__ void copy_ahead(P* smem, const void* global) {
-  if constexpr (sizeof(P) >= 4)
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(smem)), "l"(global), "n"(sizeof(P)) : "memory");
-  else
-    *smem = load_pack<P>(global);
+// The asynchronous copy of a piece.  The shortest is 4 bytes: of a 2-byte piece the aligned word around it.
+template <int BYTES>
+__device__ __forceinline__ void copy_ahead(void* smem, const void* global) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(smem)), "l"(global), "n"(BYTES) : "memory");
 }
 
 // S pieces of VEC channels per lane, G VEC channels apart.  Every lane copies its pieces of the rows ahead into its own
@@ -403,10 +424,12 @@ constexpr int kMergeRows = 8;                             // rows whose loads ar
 template <typename T, int VEC, int S>
 __global__ void __launch_bounds__(256) wgrad_merge_kernel(const T* __restrict__ gy, const __grid_constant__ MergeArgs a) {
   typedef Pack<T, VEC> Piece;
-  extern __shared__ uint4 merge_smem[];                    // pieces (kMergeRows, S, 256), then tokens (kMergeRows, 256)
+  constexpr int kSlot = sizeof(Piece) < 4 ? 4 : sizeof(Piece);
+  extern __shared__ uint4 merge_smem[];                    // slots (kMergeRows, S, 256), then tokens (kMergeRows, 256)
   __shared__ int64_t starts[257];
-  Piece* const slots = reinterpret_cast<Piece*>(merge_smem) + threadIdx.x;
-  int* const tokens = reinterpret_cast<int*>(reinterpret_cast<Piece*>(merge_smem) + kMergeRows * S * 256) + threadIdx.x;
+  char* const slots = reinterpret_cast<char*>(merge_smem) + threadIdx.x * kSlot;
+  int* const tokens = reinterpret_cast<int*>(reinterpret_cast<char*>(merge_smem) + kMergeRows * S * 256 * kSlot) + threadIdx.x;
+  uint32_t odd = 0;                                        // 2-byte pieces: bit u S + q, whether it is its word's upper half
   const int l = threadIdx.x % a.G, mine = threadIdx.x / a.G, per_block = 256 / a.G;
   const int64_t w = blockIdx.x * static_cast<int64_t>(per_block) + mine;
   const int64_t end = a.V + a.n, d0 = min(end, w * a.items), d1 = min(end, d0 + a.items);
@@ -462,7 +485,16 @@ __global__ void __launch_bounds__(256) wgrad_merge_kernel(const T* __restrict__ 
         const T* row = gy + p.y * a.ldg + c;
 #pragma unroll
         for (int q = 0; q < S; ++q)
-          if (c + q * apart < a.C) copy_ahead(slots + (u * S + q) * 256, row + q * apart);
+          if (c + q * apart < a.C) {
+            if constexpr (sizeof(Piece) >= 4) {
+              copy_ahead<kSlot>(slots + (u * S + q) * 256 * kSlot, row + q * apart);
+            } else {
+              const uintptr_t at = reinterpret_cast<uintptr_t>(row + q * apart);
+              const uint32_t bit = 1u << (u * S + q);
+              odd = at & 2 ? odd | bit : odd & ~bit;
+              copy_ahead<4>(slots + (u * S + q) * 256 * kSlot, reinterpret_cast<const void*>(at & ~static_cast<uintptr_t>(3)));
+            }
+          }
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -479,7 +511,7 @@ __global__ void __launch_bounds__(256) wgrad_merge_kernel(const T* __restrict__ 
 #pragma unroll
     for (int q = 0; q < S; ++q) {
       if (c + q * apart < a.C) {
-        const Piece x = load_pack<Piece>(slots + (u * S + q) * 256);
+        const Piece x = load_pack<Piece>(slots + (u * S + q) * 256 * kSlot + (sizeof(Piece) < 4 ? odd >> (u * S + q) << 1 & 2 : 0));
 #pragma unroll
         for (int e = 0; e < VEC; ++e) acc[q][e] += to_f32(x.v[e]);
       }
@@ -495,14 +527,14 @@ __global__ void __launch_bounds__(256) wgrad_merge_kernel(const T* __restrict__ 
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-// A warp per token that crosses workers and 128 channels: the tails of the workers since its first row, then the last
+// A warp per token that crosses workers and kJoinChannels channels: the tails of the workers since its first row, then the last
 // one's head, in fp64.  One with more than kLongJoin tails is left to the block's warps together, each a fixed share.
-constexpr int kLongJoin = 128;
+constexpr int kLongJoin = 8;
 constexpr int kJoinWarps = 8;
-constexpr int kJoinChannels = 128;
+constexpr int kJoinChannels = 256;
 
 template <int VEC>
-__global__ void __launch_bounds__(kJoinWarps * 32) wgrad_join_kernel(const __grid_constant__ MergeArgs a) {
+__global__ void __launch_bounds__(kJoinWarps * 32, 3) wgrad_join_kernel(const __grid_constant__ MergeArgs a) {
   __shared__ double red[kJoinWarps][32 * VEC];
   __shared__ int64_t task_worker[kJoinWarps], task_first[kJoinWarps], task_token[kJoinWarps];
   typedef Pack<float, VEC> Piece;
@@ -888,15 +920,16 @@ int lookup_launch(const void* ids, const void* w, void* y, int64_t n, int V, int
   constexpr int kVec = 16 / (sizeof(TW) > sizeof(TY) ? sizeof(TW) : sizeof(TY));
   const bool wide = C % kVec == 0 && ldw % kVec == 0 && reinterpret_cast<uintptr_t>(w) % (kVec * sizeof(TW)) == 0 &&
                     reinterpret_cast<uintptr_t>(y) % (kVec * sizeof(TY)) == 0;
-  const int CV = wide ? C / kVec : C;
-  const int64_t units = n * CV;
-  const int grid = static_cast<int>(std::min<int64_t>((units + 255) / 256, static_cast<int64_t>(num_sms()) * 8));
-  if (wide)
-    embed_lookup_kernel<I, TW, TY, kVec><<<grid, 256, 0, s>>>(static_cast<const I*>(ids), static_cast<const TW*>(w),
-                                                              static_cast<TY*>(y), units, V, CV, ldw, scale);
-  else
-    embed_lookup_kernel<I, TW, TY, 1><<<grid, 256, 0, s>>>(static_cast<const I*>(ids), static_cast<const TW*>(w),
-                                                           static_cast<TY*>(y), units, V, CV, ldw, scale);
+  const int units = wide ? C / kVec : C;
+  const int slices = (units + 255) / 256, pieces = (units + slices - 1) / slices, rows_at_once = 256 / pieces;
+  const int64_t blocks = (n + rows_at_once * kLookupRows - 1) / (rows_at_once * kLookupRows);
+  const dim3 grid(static_cast<unsigned>(std::min<int64_t>(blocks, static_cast<int64_t>(num_sms()) * 16)), slices);
+  const auto run = [&](auto kernel) {
+    kernel<<<grid, 256, 0, s>>>(static_cast<const I*>(ids), static_cast<const TW*>(w), static_cast<TY*>(y), n, V, C, pieces,
+                                rows_at_once, ldw, scale);
+  };
+  if (wide) run(embed_lookup_kernel<I, TW, TY, kVec>);
+  else run(embed_lookup_kernel<I, TW, TY, 1>);
   return launched("embed_lookup_kernel");
 }
 
@@ -928,10 +961,14 @@ int sort_pass(const S* src, int64_t n, int V, int shift, int tiles, int* counts,
 }
 
 template <typename I, int ROUNDS>
-int sort_cluster_rounds(const I* ids, int n, int V, int passes, int2* a, int2* b, int* zero, cudaStream_t s) {
+int sort_cluster_rounds(const I* ids, int n, int V, int passes, int2* out, int* zero, cudaStream_t s) {
+  const auto fn = sort_cluster_kernel<I, ROUNDS>;
+  const int smem = ROUNDS * kClusterThreads * static_cast<int>(sizeof(int2));
+  if (int e = allow_smem(reinterpret_cast<const void*>(fn), smem)) return e;
   cudaLaunchConfig_t lc = {};
   lc.gridDim = dim3(kClusterCtas);
   lc.blockDim = dim3(kClusterThreads);
+  lc.dynamicSmemBytes = smem;
   lc.stream = s;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
@@ -939,28 +976,30 @@ int sort_cluster_rounds(const I* ids, int n, int V, int passes, int2* a, int2* b
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   lc.attrs = &attr;
   lc.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&lc, sort_cluster_kernel<I, ROUNDS>, ids, n, V, passes, a, b, zero);
+  const cudaError_t e = cudaLaunchKernelEx(&lc, fn, ids, n, V, passes, out, zero);
   return e == cudaSuccess ? 0 : fail(BPC_ERR_LAUNCH, std::string("sort_cluster_kernel launch: ") + cudaGetErrorString(e));
 }
 
 template <typename I>
-int sort_cluster(const I* ids, int n, int V, int passes, int2* a, int2* b, int* zero, cudaStream_t s) {
+int sort_cluster(const I* ids, int n, int V, int passes, int2* out, int* zero, cudaStream_t s) {
   constexpr int kRound = kClusterCtas * kClusterThreads;
-  if (n <= kRound) return sort_cluster_rounds<I, 1>(ids, n, V, passes, a, b, zero, s);
-  if (n <= 2 * kRound) return sort_cluster_rounds<I, 2>(ids, n, V, passes, a, b, zero, s);
-  if (n <= 4 * kRound) return sort_cluster_rounds<I, 4>(ids, n, V, passes, a, b, zero, s);
-  return sort_cluster_rounds<I, 8>(ids, n, V, passes, a, b, zero, s);
+  if (n <= kRound) return sort_cluster_rounds<I, 1>(ids, n, V, passes, out, zero, s);
+  if (n <= 2 * kRound) return sort_cluster_rounds<I, 2>(ids, n, V, passes, out, zero, s);
+  if (n <= 4 * kRound) return sort_cluster_rounds<I, 4>(ids, n, V, passes, out, zero, s);
+  return sort_cluster_rounds<I, 8>(ids, n, V, passes, out, zero, s);
 }
 
+// *sorted: where the pairs are
 template <typename I>
 int sort_ids(const I* ids, int64_t n, int V, const WgradPlan& p, int2* const (&pair)[2], int* counts, int* totals,
-             int* zero, cudaStream_t s) {
-  if (n <= kClusterKeys) return sort_cluster(ids, static_cast<int>(n), V, p.passes, pair[0], pair[1], zero, s);
+             int* zero, const int2** sorted, cudaStream_t s) {
+  *sorted = pair[0];
+  if (n <= kClusterKeys) return sort_cluster(ids, static_cast<int>(n), V, p.passes, pair[0], zero, s);
   if (int e = sort_pass(ids, n, V, 0, p.tiles, counts, totals, pair[0], zero, s)) return e;
-  for (int k = 1; k < p.passes; ++k)
-    if (int e = sort_pass(static_cast<const int2*>(pair[(k - 1) & 1]), n, V, k * kDigitBits, p.tiles, counts, totals,
-                          pair[k & 1], zero, s))
-      return e;
+  for (int k = 1; k < p.passes; ++k) {
+    if (int e = sort_pass(*sorted, n, V, k * kDigitBits, p.tiles, counts, totals, pair[k & 1], zero, s)) return e;
+    *sorted = pair[k & 1];
+  }
   return 0;
 }
 
@@ -970,7 +1009,7 @@ int merge_launch_pieces(const T* gy, MergeArgs a, cudaStream_t s) {
   const dim3 grid(static_cast<unsigned>(blocks), (a.C + a.G * VEC * S - 1) / (a.G * VEC * S));
   void* args[] = {&gy, &a};
   const void* fn = reinterpret_cast<const void*>(&wgrad_merge_kernel<T, VEC, S>);
-  constexpr int kSmem = kMergeRows * 256 * (S * VEC * static_cast<int>(sizeof(T)) + static_cast<int>(sizeof(int)));
+  constexpr int kSmem = kMergeRows * 256 * (S * std::max(4, VEC * static_cast<int>(sizeof(T))) + static_cast<int>(sizeof(int)));
   if (int e = allow_smem(fn, kSmem)) return e;
   if (int e = launch_pdl(fn, grid, dim3(256), kSmem, s, args, 1, "wgrad_merge_kernel")) return e;
   void* join_args[] = {&a};
@@ -1115,11 +1154,12 @@ extern "C" int bpc_embed_wgrad(const void* gy, const void* ids, int32_t id_bytes
   int* totals = reinterpret_cast<int*>(ws + p.totals);
   int2* heads = reinterpret_cast<int2*>(ws + p.heads);
   int* zero = reinterpret_cast<int*>(heads);
-  const int e = id_bytes == 8 ? sort_ids(static_cast<const int64_t*>(ids), n, V, p, pair, counts, totals, zero, s)
-                              : sort_ids(static_cast<const int32_t*>(ids), n, V, p, pair, counts, totals, zero, s);
-  if (e) return e;
   MergeArgs a;
-  a.pair = pair[(p.passes - 1) & 1];
+  const int e =
+      id_bytes == 8
+          ? sort_ids(static_cast<const int64_t*>(ids), n, V, p, pair, counts, totals, zero, &a.pair, s)
+          : sort_ids(static_cast<const int32_t*>(ids), n, V, p, pair, counts, totals, zero, &a.pair, s);
+  if (e) return e;
   a.n = n;
   a.items = p.items;
   a.workers = p.workers;
