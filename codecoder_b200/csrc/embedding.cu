@@ -372,16 +372,16 @@ struct MergeArgs {
 
 // The tokens finished within the first d steps of the path, by the G lanes of a worker together: each step of the search
 // probes G places.
-__device__ __forceinline__ int64_t path_search(const MergeArgs& a, int64_t d, int l, unsigned mask, int shift) {
+__device__ __forceinline__ int64_t path_search(const MergeArgs& a, int64_t d, int G, int l, unsigned mask, int shift) {
   int64_t lo = d > a.n ? d - a.n : 0, hi = d < a.V ? d : a.V;            // lo holds: every row consumed
   while (lo < hi) {
-    const int64_t step = (hi - lo + a.G) / (a.G + 1), at = lo + (l + 1) * step;
+    const int64_t step = (hi - lo + G) / (G + 1), at = lo + (l + 1) * step;
     // token at - 1 is finished before step d iff the next row belongs to a later one
     const bool done = at <= hi && (d - at >= a.n || a.pair[d - at].x >= at);
     const int c = __popc(__ballot_sync(mask, done) & mask);
     const int64_t top = lo + (c + 1) * step - 1;
     lo += c * step;
-    if (c < a.G && top < hi) hi = top;                     // below the first probe that failed
+    if (c < G && top < hi) hi = top;                     // below the first probe that failed
   }
   return lo;
 }
@@ -410,38 +410,54 @@ __device__ __forceinline__ void store_row(void* dw, int dtype, int64_t at, const
   }
 }
 
+__host__ __device__ constexpr int merge_rows(int pieces) { return pieces == 4 ? 4 : 8; }
+
 // The asynchronous copy of a piece.  The shortest is 4 bytes: of a 2-byte piece the aligned word around it.
 template <int BYTES>
 __device__ __forceinline__ void copy_ahead(void* smem, const void* global) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(smem)), "l"(global), "n"(BYTES) : "memory");
 }
 
-// S pieces of VEC channels per lane, G VEC channels apart.  Every lane copies its pieces of the rows ahead into its own
-// slots of shared memory (and reads only those, so no barrier is needed): the loads in flight do not depend on the
-// registers, which held a block of eight rows to two per SM.
-constexpr int kMergeRows = 8;                             // rows whose loads are in flight per worker
+// zeros for the rows [from, to) of dW, at this lane's pieces (first: their place in row 0)
+template <typename W, int S>
+__device__ __forceinline__ void zero_rows(void* first, int64_t row_bytes, int from, int to, int apart_bytes, int pieces) {
+  char* p = static_cast<char*>(first) + from * row_bytes;
+  W zero;
+  memset(&zero, 0, sizeof(W));
+  for (int t = from; t < to; ++t, p += row_bytes) {
+#pragma unroll
+    for (int q = 0; q < S; ++q)
+      if (q < pieces) *reinterpret_cast<W*>(p + q * apart_bytes) = zero;
+  }
+}
 
+// S pieces of VEC channels per lane, G VEC channels apart (G = 32 lanes where S > 1).  Every lane copies its pieces of the
+// rows ahead into its own slots of shared memory (and reads only those, so no barrier is needed): the loads in flight do
+// not depend on the registers, which held a block of eight rows to two per SM.  More pieces per lane share a step's
+// bookkeeping, which bounded two pieces (88 instructions a step at 50,021 tokens x 1,024).
 template <typename T, int VEC, int S>
 __global__ void __launch_bounds__(256) wgrad_merge_kernel(const T* __restrict__ gy, const __grid_constant__ MergeArgs a) {
   typedef Pack<T, VEC> Piece;
+  constexpr int kRows = merge_rows(S);                    // rows whose loads are in flight per worker
   constexpr int kSlot = sizeof(Piece) < 4 ? 4 : sizeof(Piece);
-  extern __shared__ uint4 merge_smem[];                    // slots (kMergeRows, S, 256), then tokens (kMergeRows, 256)
+  extern __shared__ uint4 merge_smem[];                    // slots (kRows, S, 256), then tokens (kRows, 256)
   __shared__ int64_t starts[257];
   char* const slots = reinterpret_cast<char*>(merge_smem) + threadIdx.x * kSlot;
-  int* const tokens = reinterpret_cast<int*>(reinterpret_cast<char*>(merge_smem) + kMergeRows * S * 256 * kSlot) + threadIdx.x;
+  int* const tokens = reinterpret_cast<int*>(reinterpret_cast<char*>(merge_smem) + kRows * S * 256 * kSlot) + threadIdx.x;
   uint32_t odd = 0;                                        // 2-byte pieces: bit u S + q, whether it is its word's upper half
-  const int l = threadIdx.x % a.G, mine = threadIdx.x / a.G, per_block = 256 / a.G;
+  const int G = S > 1 ? 32 : a.G;
+  const int l = threadIdx.x % G, mine = threadIdx.x / G, per_block = 256 / G;
   const int64_t w = blockIdx.x * static_cast<int64_t>(per_block) + mine;
   const int64_t end = a.V + a.n, d0 = min(end, w * a.items), d1 = min(end, d0 + a.items);
-  const int shift = (threadIdx.x & 31) / a.G * a.G;
-  const unsigned mask = (a.G == 32 ? 0xffffffffu : (1u << a.G) - 1) << shift;
+  const int shift = (threadIdx.x & 31) / G * G;
+  const unsigned mask = (G == 32 ? 0xffffffffu : (1u << G) - 1) << shift;
   pdl_launch_dependents();
   pdl_wait();
   {
-    const int64_t i = path_search(a, d0, l, mask, shift);
+    const int64_t i = path_search(a, d0, G, l, mask, shift);
     if (l == 0) starts[mine] = i;
     if (mine == per_block - 1) {
-      const int64_t e = path_search(a, d1, l, mask, shift);
+      const int64_t e = path_search(a, d1, G, l, mask, shift);
       if (l == 0) starts[per_block] = e;
     }
   }
@@ -449,7 +465,8 @@ __global__ void __launch_bounds__(256) wgrad_merge_kernel(const T* __restrict__ 
   if (w >= a.workers) return;
   const int i0 = static_cast<int>(starts[mine]), i1 = static_cast<int>(starts[mine + 1]);
   const int j0 = static_cast<int>(d0 - i0), j1 = static_cast<int>(d1 - i1);
-  const int c = (blockIdx.y * S * a.G + l) * VEC, apart = a.G * VEC;     // piece q: channels c + q apart ..
+  const int c = (blockIdx.y * S * G + l) * VEC, apart = G * VEC;          // piece q: channels c + q apart ..
+  const int pieces = c < a.C ? min(S, (a.C - c + apart - 1) / apart) : 0;
   bool open = j0 > 0 && i0 < a.V && a.pair[j0 - 1].x == i0;               // token i0 began in an earlier worker
   if (open && i1 > i0 && l == 0 && blockIdx.y == 0)
     a.heads[1 + atomicAdd(&a.heads[0].x, 1)] = make_int2(static_cast<int>(w), i0);
@@ -459,10 +476,11 @@ __global__ void __launch_bounds__(256) wgrad_merge_kernel(const T* __restrict__ 
 #pragma unroll
     for (int e = 0; e < VEC; ++e) acc[q][e] = 0.f;
   int tok = i0;
-  const auto flush = [&]() {
+  // ends the tokens up to t: the open one's sum, then the ones without a row
+  const auto end_tokens = [&](int t) {
 #pragma unroll
     for (int q = 0; q < S; ++q) {
-      if (c + q * apart < a.C) {
+      if (q < pieces) {
         if (open) store_row<VEC>(a.head, BPC_DTYPE_F32, w * a.C + c + q * apart, acc[q], 1.f);
         else store_row<VEC>(a.dw, a.dw_dtype, static_cast<int64_t>(tok) * a.C + c + q * apart, acc[q], a.scale);
       }
@@ -470,11 +488,16 @@ __global__ void __launch_bounds__(256) wgrad_merge_kernel(const T* __restrict__ 
       for (int e = 0; e < VEC; ++e) acc[q][e] = 0.f;
     }
     open = false;
-    ++tok;
+    if (a.dw_dtype == BPC_DTYPE_F32)
+      zero_rows<typename Word<4 * VEC>::type, S>(static_cast<float*>(a.dw) + c, 4ll * a.C, tok + 1, t, 4 * apart, pieces);
+    else
+      zero_rows<typename Word<2 * VEC>::type, S>(static_cast<uint16_t*>(a.dw) + c, 2ll * a.C, tok + 1, t, 2 * apart, pieces);
+    tok = t;
   };
   // row j into slot u; the pair of the row after it is read one call ahead
   int2 ahead = j0 < j1 ? a.pair[j0] : make_int2(a.V, 0);
   int next = j0;
+  const T* const lane_gy = gy + c;
   const auto copy_row = [&](int u) {
     if (next < j1) {
       const int2 p = ahead;
@@ -482,10 +505,10 @@ __global__ void __launch_bounds__(256) wgrad_merge_kernel(const T* __restrict__ 
       if (next < j1) ahead = a.pair[next];
       tokens[u * 256] = p.x;
       if (p.x < a.V) {                                     // V: a position without a token
-        const T* row = gy + p.y * a.ldg + c;
+        const T* row = lane_gy + p.y * a.ldg;
 #pragma unroll
         for (int q = 0; q < S; ++q)
-          if (c + q * apart < a.C) {
+          if (q < pieces) {
             if constexpr (sizeof(Piece) >= 4) {
               copy_ahead<kSlot>(slots + (u * S + q) * 256 * kSlot, row + q * apart);
             } else {
@@ -500,29 +523,29 @@ __global__ void __launch_bounds__(256) wgrad_merge_kernel(const T* __restrict__ 
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 #pragma unroll
-  for (int u = 0; u < kMergeRows - 1; ++u) copy_row(u);
+  for (int u = 0; u < kRows - 1; ++u) copy_row(u);
   int u = 0;
   for (int j = j0; j < j1; ++j) {
-    copy_row(u == 0 ? kMergeRows - 1 : u - 1);             // into the slot that the step before read
-    asm volatile("cp.async.wait_group %0;" ::"n"(kMergeRows - 1) : "memory");
+    copy_row(u == 0 ? kRows - 1 : u - 1);                  // into the slot that the step before read
+    asm volatile("cp.async.wait_group %0;" ::"n"(kRows - 1) : "memory");
     const int t = tokens[u * 256];
     if (t >= a.V) break;                                   // they are the last ones
-    while (tok < t) flush();
+    if (tok < t) end_tokens(t);
 #pragma unroll
     for (int q = 0; q < S; ++q) {
-      if (c + q * apart < a.C) {
+      if (q < pieces) {
         const Piece x = load_pack<Piece>(slots + (u * S + q) * 256 * kSlot + (sizeof(Piece) < 4 ? odd >> (u * S + q) << 1 & 2 : 0));
 #pragma unroll
         for (int e = 0; e < VEC; ++e) acc[q][e] += to_f32(x.v[e]);
       }
     }
-    u = u == kMergeRows - 1 ? 0 : u + 1;
+    u = u == kRows - 1 ? 0 : u + 1;
   }
-  while (tok < i1) flush();
+  if (tok < i1) end_tokens(i1);
   if (i1 < a.V && j1 > 0 && a.pair[j1 - 1].x == i1) {
 #pragma unroll
     for (int q = 0; q < S; ++q)
-      if (c + q * apart < a.C) store_row<VEC>(a.tail, BPC_DTYPE_F32, w * a.C + c + q * apart, acc[q], 1.f);
+      if (q < pieces) store_row<VEC>(a.tail, BPC_DTYPE_F32, w * a.C + c + q * apart, acc[q], 1.f);
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
@@ -889,8 +912,8 @@ WgradPlan wgrad_plan(int64_t n, int32_t V, int32_t C) {
   p.tiles = static_cast<int>((n + kSortTile - 1) / kSortTile);
   p.G = 1;
   while (p.G < 32 && p.G * 4 < C) p.G *= 2;
-  // about 32 warps per SM over the workers and the slices of 256 channels, at least 16 steps a worker
-  const int64_t target = std::max<int64_t>(1, static_cast<int64_t>(num_sms()) * 32 * (32 / p.G) / ((C + 255) / 256));
+  // about 32 warps per SM over the workers and the slices of 512 channels, at least 16 steps a worker
+  const int64_t target = std::max<int64_t>(1, static_cast<int64_t>(num_sms()) * 32 * (32 / p.G) / ((C + 511) / 512));
   p.items = std::max<int64_t>(16, (V + n + target - 1) / target);
   p.workers = (V + n + p.items - 1) / p.items;
   size_t at = 0;
@@ -1005,11 +1028,12 @@ int sort_ids(const I* ids, int64_t n, int V, const WgradPlan& p, int2* const (&p
 
 template <typename T, int VEC, int S>
 int merge_launch_pieces(const T* gy, MergeArgs a, cudaStream_t s) {
+  if (S > 1) a.G = 32;
   const int64_t blocks = (a.workers + 256 / a.G - 1) / (256 / a.G);
   const dim3 grid(static_cast<unsigned>(blocks), (a.C + a.G * VEC * S - 1) / (a.G * VEC * S));
   void* args[] = {&gy, &a};
   const void* fn = reinterpret_cast<const void*>(&wgrad_merge_kernel<T, VEC, S>);
-  constexpr int kSmem = kMergeRows * 256 * (S * std::max(4, VEC * static_cast<int>(sizeof(T))) + static_cast<int>(sizeof(int)));
+  constexpr int kSmem = merge_rows(S) * 256 * (S * std::max(4, VEC * static_cast<int>(sizeof(T))) + static_cast<int>(sizeof(int)));
   if (int e = allow_smem(fn, kSmem)) return e;
   if (int e = launch_pdl(fn, grid, dim3(256), kSmem, s, args, 1, "wgrad_merge_kernel")) return e;
   void* join_args[] = {&a};
@@ -1021,6 +1045,7 @@ int merge_launch_pieces(const T* gy, MergeArgs a, cudaStream_t s) {
 
 template <typename T, int VEC>
 int merge_launch_vec(const T* gy, const MergeArgs& a, cudaStream_t s) {
+  if (a.C > 64 * VEC) return merge_launch_pieces<T, VEC, 4>(gy, a, s);
   return a.C > 32 * VEC ? merge_launch_pieces<T, VEC, 2>(gy, a, s) : merge_launch_pieces<T, VEC, 1>(gy, a, s);
 }
 
