@@ -156,17 +156,18 @@ __device__ __forceinline__ void st_cluster(uint32_t addr, int x, int y) {
 
 template <typename I, int ROUNDS>
 __global__ void __launch_bounds__(kClusterThreads) sort_cluster_kernel(const I* __restrict__ ids, int n, int V, int passes,
-                                                                       int2* __restrict__ out, int* __restrict__ zero) {
-  extern __shared__ int2 places[];                         // (ROUNDS x 1024) this CTA's run
+                                                                       int2* __restrict__ out) {
+  extern __shared__ int2 places[];                         // (ROUNDS x 1024) this CTA's run, and again by this pass's digit
   __shared__ uint16_t cnt[kClusterThreads / 32][kBins];
   __shared__ int hist[2][kClusterCtas][kBins];             // every CTA's counts of this pass; two, so that a pass may
-  __shared__ int warp_sum[kBins / 32];                     // write while a slower CTA still reads the one before
+  __shared__ int own_first[kBins];                         // write while a slower CTA still reads the one before
+  __shared__ int warp_sum[2][kBins / 32];
   constexpr int kRun = ROUNDS * kClusterThreads;
+  int2* const ordered = places + kRun;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int cta = static_cast<int>(cluster_ctarank());
   const int first = warp * 32 * ROUNDS + lane;             // of this thread's places in the run
   pdl_launch_dependents();
-  if (cta == 0 && tid == 0) *zero = 0;
   cluster_arrive_release();                                // every CTA runs before another writes its shared memory
   cluster_wait_acquire();
   for (int pass = 0; pass < passes; ++pass) {
@@ -203,31 +204,52 @@ __global__ void __launch_bounds__(kClusterThreads) sort_cluster_kernel(const I* 
     }
     cluster_arrive_release();                              // counts written, and every run read
     cluster_wait_acquire();
-    int total = 0, before = 0, s = 0;
+    // each digit's first place in this CTA's own order, and among all the CTAs' pairs
+    int total = 0, before = 0, own = 0, s = 0, s_own = 0;
     if (tid < kBins) {
 #pragma unroll
       for (int k = 0; k < kClusterCtas; ++k) {
         const int c = hist[pass & 1][k][tid];
         if (k < cta) before += c;
+        if (k == cta) own = c;
         total += c;
       }
       s = warp_inclusive(total, lane);
-      if (lane == 31) warp_sum[warp] = s;
+      s_own = warp_inclusive(own, lane);
+      if (lane == 31) {
+        warp_sum[0][warp] = s;
+        warp_sum[1][warp] = s_own;
+      }
     }
     __syncthreads();
     if (tid < kBins) {
-      int at = s - total + before;
-      for (int w = 0; w < warp; ++w) at += warp_sum[w];
-      hist[pass & 1][cta][tid] = at;                       // only this CTA reads its own row from here on
+      int at = s - total + before, at_own = s_own - own;
+      for (int w = 0; w < warp; ++w) {
+        at += warp_sum[0][w];
+        at_own += warp_sum[1][w];
+      }
+      own_first[tid] = at_own;
+      hist[pass & 1][cta][tid] = at - at_own;              // only this CTA reads its own row from here on
     }
     __syncthreads();
-    const uint32_t base = smem_u32(places);
+    // in its own order first, so that the stores to other CTAs run along theirs
 #pragma unroll
     for (int r = 0; r < ROUNDS; ++r) {
       if (key[r] >= 0) {
         const int digit = (key[r] >> shift) & (kBins - 1);
-        const int to = hist[pass & 1][cta][digit] + cnt[warp][digit] + rank[r];
-        st_cluster(map_to_cta(base + to % kRun * 8, to / kRun), key[r], pos[r]);
+        ordered[own_first[digit] + cnt[warp][digit] + rank[r]] = make_int2(key[r], pos[r]);
+      }
+    }
+    __syncthreads();
+    const uint32_t base = smem_u32(places);
+    const int here = min(kRun, n - cta * kRun);
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+      const int i = tid + r * kClusterThreads;
+      if (i < here) {
+        const int2 p = ordered[i];
+        const int to = i + hist[pass & 1][cta][(p.x >> shift) & (kBins - 1)];
+        st_cluster(map_to_cta(base + to % kRun * 8, to / kRun), p.x, p.y);
       }
     }
     cluster_arrive_release();                              // the pairs are in their places
@@ -275,12 +297,10 @@ __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(const S* __res
 }
 
 // One block per digit: its counts over the tiles become exclusive sums; totals[digit] their sum.
-__global__ void __launch_bounds__(256) sort_scan_kernel(int* __restrict__ counts, int* __restrict__ totals, int tiles,
-                                                        int* __restrict__ zero) {
+__global__ void __launch_bounds__(256) sort_scan_kernel(int* __restrict__ counts, int* __restrict__ totals, int tiles) {
   __shared__ int warp_sum[8];
   int* row = counts + static_cast<int64_t>(blockIdx.x) * tiles;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (blockIdx.x == 0 && threadIdx.x == 0) *zero = 0;
   int carry = 0;
   for (int t0 = 0; t0 < tiles; t0 += 256) {
     const int t = t0 + threadIdx.x;
@@ -355,8 +375,8 @@ __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(const S* __res
 // The segmented sum.  V row ends and n sorted rows form one path of V + n steps (a row end follows the last row of its
 // token), cut into equal runs of `items` steps, one per worker, so that a token with millions of rows and a million
 // tokens without any both spread evenly; every row of dW is written once, the empty ones as zeros.  A token whose rows
-// cross workers: each worker but the one at its end leaves a partial sum in tail[], the last one leaves its own in
-// head[] and its number in heads[], and wgrad_join_kernel adds them in order.
+// cross workers: each worker but the one at its end leaves a partial sum in tail[], the last one its own in head[], and
+// wgrad_join_kernel adds them in order.
 struct MergeArgs {
   const int2* pair;    // (n,) {token, row}, sorted by token
   int64_t n, items, workers;
@@ -367,7 +387,7 @@ struct MergeArgs {
   int dw_dtype;
   float* head;         // (workers, C)
   float* tail;
-  int2* heads;         // [0].x: how many; [1 ..]: {worker, token} with a head, in no order
+  int2* ends;          // (workers,) {the token of head[] or -1, whether the token of tail[] begins in the worker}
 };
 
 // The tokens finished within the first d steps of the path, by the G lanes of a worker together: each step of the search
@@ -468,8 +488,7 @@ __global__ void __launch_bounds__(256) wgrad_merge_kernel(const T* __restrict__ 
   const int c = (blockIdx.y * S * G + l) * VEC, apart = G * VEC;          // piece q: channels c + q apart ..
   const int pieces = c < a.C ? min(S, (a.C - c + apart - 1) / apart) : 0;
   bool open = j0 > 0 && i0 < a.V && a.pair[j0 - 1].x == i0;               // token i0 began in an earlier worker
-  if (open && i1 > i0 && l == 0 && blockIdx.y == 0)
-    a.heads[1 + atomicAdd(&a.heads[0].x, 1)] = make_int2(static_cast<int>(w), i0);
+  if (l == 0 && blockIdx.y == 0) a.ends[w] = make_int2(open && i1 > i0 ? i0 : -1, i1 > i0 || !open);
   float acc[S][VEC];
 #pragma unroll
   for (int q = 0; q < S; ++q)
@@ -585,23 +604,30 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 3) wgrad_join_kernel(const __
     for (int e = 0; e < VEC; ++e) f[e] = static_cast<float>(s[e] + h.v[e]);
     store_row<VEC>(a.dw, a.dw_dtype, t * a.C + c, f, a.scale);
   };
-  const int count = a.heads[0].x;
-  for (int base = blockIdx.x * kJoinWarps; base < count; base += gridDim.x * kJoinWarps) {
-    int64_t w = -1, first = 0, t = 0;
-    if (base + warp < count) {
-      const int2 head = a.heads[1 + base + warp];
-      w = head.x;
-      t = head.y;
-      int64_t lo = 0, hi = a.n;                            // the first row of token t is in [lo, hi]
-      while (lo < hi) {
-        const int64_t step = (hi - lo + 32) / 33, at = lo + (lane + 1) * step;
-        const bool below = at <= hi && a.pair[at - 1].x < t;
-        const int c = __popc(__ballot_sync(0xffffffffu, below));
-        const int64_t top = lo + (c + 1) * step - 1;
-        lo += c * step;
-        if (c < 32 && top < hi) hi = top;
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * kJoinWarps; base < a.workers;
+       base += static_cast<int64_t>(gridDim.x) * kJoinWarps) {
+    int64_t w = base + warp, first = 0, t = w < a.workers ? a.ends[w].x : -1;
+    // the nearest worker before w whose tail's token begins in it, 128 at a time; that token is t where t is one
+    for (int64_t top = w - 1; w < a.workers && top >= 0; top -= 128) {
+      unsigned begins[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int64_t v = top - 32 * u - lane;
+        begins[u] = __ballot_sync(0xffffffffu, v < 0 || a.ends[v].y);
       }
-      first = (lo + t) / a.items;
+      if (t < 0) break;
+      int at = 128;
+#pragma unroll
+      for (int u = 3; u >= 0; --u)
+        if (begins[u]) at = 32 * u + __ffs(begins[u]) - 1;
+      if (at < 128) {
+        first = top - at;
+        break;
+      }
+    }
+    if (t < 0) {
+      w = -1;
+    } else {
       if (w - first <= kLongJoin) {
         for (int c = c_from + lane * VEC; c < c_to; c += 32 * VEC) {
           double s[VEC] = {};
@@ -860,7 +886,7 @@ int dtype_size(int32_t dtype) { return dtype == BPC_DTYPE_F32 ? 4 : dtype == BPC
 struct WgradPlan {
   int passes, tiles, G;
   int64_t items, workers;
-  size_t pair[2], counts, totals, head, tail, heads, bytes;
+  size_t pair[2], counts, totals, head, tail, ends, bytes;
 };
 
 // Few tokens: how a block reads its rows, by alignment and row length.
@@ -927,7 +953,7 @@ WgradPlan wgrad_plan(int64_t n, int32_t V, int32_t C) {
   p.totals = take(sizeof(int) * kBins);
   p.head = take(sizeof(float) * p.workers * C);
   p.tail = take(sizeof(float) * p.workers * C);
-  p.heads = take(sizeof(int2) * (p.workers + 1));
+  p.ends = take(sizeof(int2) * p.workers);
   p.bytes = at;
   return p;
 }
@@ -973,20 +999,19 @@ int lookup_by_w(const void* ids, const void* w, void* y, int64_t n, int V, int C
 }
 
 template <typename S>
-int sort_pass(const S* src, int64_t n, int V, int shift, int tiles, int* counts, int* totals, int2* out, int* zero,
-              cudaStream_t s) {
+int sort_pass(const S* src, int64_t n, int V, int shift, int tiles, int* counts, int* totals, int2* out, cudaStream_t s) {
   sort_count_kernel<S><<<tiles, kSortThreads, 0, s>>>(src, n, V, shift, counts, tiles);
   if (int e = launched("sort_count_kernel")) return e;
-  sort_scan_kernel<<<kBins, 256, 0, s>>>(counts, totals, tiles, zero);
+  sort_scan_kernel<<<kBins, 256, 0, s>>>(counts, totals, tiles);
   if (int e = launched("sort_scan_kernel")) return e;
   sort_place_kernel<S><<<tiles, kSortThreads, 0, s>>>(src, n, V, shift, counts, totals, tiles, out);
   return launched("sort_place_kernel");
 }
 
 template <typename I, int ROUNDS>
-int sort_cluster_rounds(const I* ids, int n, int V, int passes, int2* out, int* zero, cudaStream_t s) {
+int sort_cluster_rounds(const I* ids, int n, int V, int passes, int2* out, cudaStream_t s) {
   const auto fn = sort_cluster_kernel<I, ROUNDS>;
-  const int smem = ROUNDS * kClusterThreads * static_cast<int>(sizeof(int2));
+  const int smem = 2 * ROUNDS * kClusterThreads * static_cast<int>(sizeof(int2));
   if (int e = allow_smem(reinterpret_cast<const void*>(fn), smem)) return e;
   cudaLaunchConfig_t lc = {};
   lc.gridDim = dim3(kClusterCtas);
@@ -999,28 +1024,28 @@ int sort_cluster_rounds(const I* ids, int n, int V, int passes, int2* out, int* 
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   lc.attrs = &attr;
   lc.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&lc, fn, ids, n, V, passes, out, zero);
+  const cudaError_t e = cudaLaunchKernelEx(&lc, fn, ids, n, V, passes, out);
   return e == cudaSuccess ? 0 : fail(BPC_ERR_LAUNCH, std::string("sort_cluster_kernel launch: ") + cudaGetErrorString(e));
 }
 
 template <typename I>
-int sort_cluster(const I* ids, int n, int V, int passes, int2* out, int* zero, cudaStream_t s) {
+int sort_cluster(const I* ids, int n, int V, int passes, int2* out, cudaStream_t s) {
   constexpr int kRound = kClusterCtas * kClusterThreads;
-  if (n <= kRound) return sort_cluster_rounds<I, 1>(ids, n, V, passes, out, zero, s);
-  if (n <= 2 * kRound) return sort_cluster_rounds<I, 2>(ids, n, V, passes, out, zero, s);
-  if (n <= 4 * kRound) return sort_cluster_rounds<I, 4>(ids, n, V, passes, out, zero, s);
-  return sort_cluster_rounds<I, 8>(ids, n, V, passes, out, zero, s);
+  if (n <= kRound) return sort_cluster_rounds<I, 1>(ids, n, V, passes, out, s);
+  if (n <= 2 * kRound) return sort_cluster_rounds<I, 2>(ids, n, V, passes, out, s);
+  if (n <= 4 * kRound) return sort_cluster_rounds<I, 4>(ids, n, V, passes, out, s);
+  return sort_cluster_rounds<I, 8>(ids, n, V, passes, out, s);
 }
 
 // *sorted: where the pairs are
 template <typename I>
 int sort_ids(const I* ids, int64_t n, int V, const WgradPlan& p, int2* const (&pair)[2], int* counts, int* totals,
-             int* zero, const int2** sorted, cudaStream_t s) {
+             const int2** sorted, cudaStream_t s) {
   *sorted = pair[0];
-  if (n <= kClusterKeys) return sort_cluster(ids, static_cast<int>(n), V, p.passes, pair[0], zero, s);
-  if (int e = sort_pass(ids, n, V, 0, p.tiles, counts, totals, pair[0], zero, s)) return e;
+  if (n <= kClusterKeys) return sort_cluster(ids, static_cast<int>(n), V, p.passes, pair[0], s);
+  if (int e = sort_pass(ids, n, V, 0, p.tiles, counts, totals, pair[0], s)) return e;
   for (int k = 1; k < p.passes; ++k) {
-    if (int e = sort_pass(*sorted, n, V, k * kDigitBits, p.tiles, counts, totals, pair[k & 1], zero, s)) return e;
+    if (int e = sort_pass(*sorted, n, V, k * kDigitBits, p.tiles, counts, totals, pair[k & 1], s)) return e;
     *sorted = pair[k & 1];
   }
   return 0;
@@ -1037,7 +1062,7 @@ int merge_launch_pieces(const T* gy, MergeArgs a, cudaStream_t s) {
   if (int e = allow_smem(fn, kSmem)) return e;
   if (int e = launch_pdl(fn, grid, dim3(256), kSmem, s, args, 1, "wgrad_merge_kernel")) return e;
   void* join_args[] = {&a};
-  const int64_t join = std::min<int64_t>((a.workers + kJoinWarps - 1) / kJoinWarps, 4 * num_sms());
+  const int64_t join = std::min<int64_t>((a.workers + kJoinWarps - 1) / kJoinWarps, 8 * num_sms());
   return launch_pdl(reinterpret_cast<const void*>(&wgrad_join_kernel<VEC>),
                     dim3(static_cast<unsigned>(join), (a.C + kJoinChannels - 1) / kJoinChannels),
                     dim3(kJoinWarps * 32), 0, s, join_args, 1, "wgrad_join_kernel");
@@ -1177,13 +1202,11 @@ extern "C" int bpc_embed_wgrad(const void* gy, const void* ids, int32_t id_bytes
   int2* const pair[2] = {reinterpret_cast<int2*>(ws + p.pair[0]), reinterpret_cast<int2*>(ws + p.pair[1])};
   int* counts = reinterpret_cast<int*>(ws + p.counts);
   int* totals = reinterpret_cast<int*>(ws + p.totals);
-  int2* heads = reinterpret_cast<int2*>(ws + p.heads);
-  int* zero = reinterpret_cast<int*>(heads);
   MergeArgs a;
   const int e =
       id_bytes == 8
-          ? sort_ids(static_cast<const int64_t*>(ids), n, V, p, pair, counts, totals, zero, &a.pair, s)
-          : sort_ids(static_cast<const int32_t*>(ids), n, V, p, pair, counts, totals, zero, &a.pair, s);
+          ? sort_ids(static_cast<const int64_t*>(ids), n, V, p, pair, counts, totals, &a.pair, s)
+          : sort_ids(static_cast<const int32_t*>(ids), n, V, p, pair, counts, totals, &a.pair, s);
   if (e) return e;
   a.n = n;
   a.items = p.items;
@@ -1197,7 +1220,7 @@ extern "C" int bpc_embed_wgrad(const void* gy, const void* ids, int32_t id_bytes
   a.dw_dtype = dw_dtype;
   a.head = reinterpret_cast<float*>(ws + p.head);
   a.tail = reinterpret_cast<float*>(ws + p.tail);
-  a.heads = heads;
+  a.ends = reinterpret_cast<int2*>(ws + p.ends);
   if (gy_dtype == BPC_DTYPE_F32) return merge_launch<float>(gy, a, s);
   if (gy_dtype == BPC_DTYPE_BF16) return merge_launch<__nv_bfloat16>(gy, a, s);
   return merge_launch<__half>(gy, a, s);
