@@ -140,27 +140,27 @@ __device__ __forceinline__ void warp_ranks(const int (&key)[ROUNDS], int (&rank)
   }
 }
 
-// Up to kClusterKeys positions: one cluster of 8 CTAs runs every pass in one launch (separate launches of three kernels a
-// pass took 66 us for 32,768 positions, most of it latency).  The CTAs exchange digit counts and pairs through
+// Up to kClusterKeys positions: one cluster of 8 or 16 CTAs runs every pass in one launch (separate launches of three
+// kernels a pass took 66 us for 32,768 positions, most of it latency).  The CTAs exchange digit counts and pairs through
 // distributed shared memory: each holds a run of ROUNDS x 1024 places.
-constexpr int kClusterCtas = 8;
 constexpr int kClusterThreads = 1024;
-constexpr int kClusterKeys = kClusterCtas * kClusterThreads * 8;
+constexpr int kClusterKeys = 16 * kClusterThreads * 4;
 
-__device__ __forceinline__ void st_cluster(uint32_t addr, int v) {
-  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+__device__ __forceinline__ void st_cluster(uint32_t addr, uint16_t v) {
+  asm volatile("st.shared::cluster.u16 [%0], %1;" ::"r"(addr), "h"(v) : "memory");
 }
 __device__ __forceinline__ void st_cluster(uint32_t addr, int x, int y) {
   asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(addr), "r"(x), "r"(y) : "memory");
 }
 
-template <typename I, int ROUNDS>
+template <typename I, int CTAS, int ROUNDS>
 __global__ void __launch_bounds__(kClusterThreads) sort_cluster_kernel(const I* __restrict__ ids, int n, int V, int passes,
                                                                        int2* __restrict__ out) {
   extern __shared__ int2 places[];                         // (ROUNDS x 1024) this CTA's run, and again by this pass's digit
   __shared__ uint16_t cnt[kClusterThreads / 32][kBins];
-  __shared__ int hist[2][kClusterCtas][kBins];             // every CTA's counts of this pass; two, so that a pass may
-  __shared__ int own_first[kBins];                         // write while a slower CTA still reads the one before
+  __shared__ uint16_t hist[2][CTAS][kBins];                // every CTA's counts of this pass; two, so that a pass may
+                                                           // write while a slower CTA still reads the one before
+  __shared__ int own_first[kBins], shift_to[kBins];
   __shared__ int warp_sum[2][kBins / 32];
   constexpr int kRun = ROUNDS * kClusterThreads;
   int2* const ordered = places + kRun;
@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(kClusterThreads) sort_cluster_kernel(const I* 
         cnt[w][tid] = static_cast<uint16_t>(at);
         at += c;
       }
-      for (int k = 0; k < kClusterCtas; ++k) st_cluster(map_to_cta(smem_u32(&hist[pass & 1][cta][tid]), k), at);
+      for (int k = 0; k < CTAS; ++k) st_cluster(map_to_cta(smem_u32(&hist[pass & 1][cta][tid]), k), static_cast<uint16_t>(at));
     }
     cluster_arrive_release();                              // counts written, and every run read
     cluster_wait_acquire();
@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(kClusterThreads) sort_cluster_kernel(const I* 
     int total = 0, before = 0, own = 0, s = 0, s_own = 0;
     if (tid < kBins) {
 #pragma unroll
-      for (int k = 0; k < kClusterCtas; ++k) {
+      for (int k = 0; k < CTAS; ++k) {
         const int c = hist[pass & 1][k][tid];
         if (k < cta) before += c;
         if (k == cta) own = c;
@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(kClusterThreads) sort_cluster_kernel(const I* 
         at_own += warp_sum[1][w];
       }
       own_first[tid] = at_own;
-      hist[pass & 1][cta][tid] = at - at_own;              // only this CTA reads its own row from here on
+      shift_to[tid] = at - at_own;
     }
     __syncthreads();
     // in its own order first, so that the stores to other CTAs run along theirs
@@ -248,7 +248,7 @@ __global__ void __launch_bounds__(kClusterThreads) sort_cluster_kernel(const I* 
       const int i = tid + r * kClusterThreads;
       if (i < here) {
         const int2 p = ordered[i];
-        const int to = i + hist[pass & 1][cta][(p.x >> shift) & (kBins - 1)];
+        const int to = i + shift_to[(p.x >> shift) & (kBins - 1)];
         st_cluster(map_to_cta(base + to % kRun * 8, to / kRun), p.x, p.y);
       }
     }
@@ -406,6 +406,27 @@ __device__ __forceinline__ int64_t path_search(const MergeArgs& a, int64_t d, in
   return lo;
 }
 
+// Where a worker starts: {tokens finished, rows consumed} after d steps, or, inside a token that ends within `items` rows,
+// after that token: the worker before takes the whole of it, so that only the longer tokens are ever cut.
+__device__ __forceinline__ int2 path_start(const MergeArgs& a, int64_t d, int G, int l, unsigned mask, int shift) {
+  const int64_t i = path_search(a, d, G, l, mask, shift), j = d - i;
+  if (i < a.V && j > 0 && a.pair[j - 1].x == i) {
+    int64_t lo = j, hi = a.n < j + a.items ? a.n : j + a.items;
+    if (hi == a.n || a.pair[hi].x != i) {
+      while (lo < hi) {                                    // rows up to lo are the token's
+        const int64_t step = (hi - lo + G) / (G + 1), at = lo + (l + 1) * step;
+        const bool in = at <= hi && a.pair[at - 1].x == i;
+        const int c = __popc(__ballot_sync(mask, in) & mask);
+        const int64_t top = lo + (c + 1) * step - 1;
+        lo += c * step;
+        if (c < G && top < hi) hi = top;
+      }
+      return make_int2(static_cast<int>(i + 1), static_cast<int>(lo));
+    }
+  }
+  return make_int2(static_cast<int>(i), static_cast<int>(j));
+}
+
 template <int VEC>
 __device__ __forceinline__ void store_row(void* dw, int dtype, int64_t at, const float* acc, float scale) {
   if (dtype == BPC_DTYPE_F32) {
@@ -430,7 +451,8 @@ __device__ __forceinline__ void store_row(void* dw, int dtype, int64_t at, const
   }
 }
 
-__host__ __device__ constexpr int merge_rows(int pieces) { return pieces == 4 ? 4 : 8; }
+// rows whose loads are in flight per worker, for the bytes of a lane's pieces
+__host__ __device__ constexpr int merge_rows(int bytes) { return bytes >= 32 ? 4 : 8; }
 
 // The asynchronous copy of a piece.  The shortest is 4 bytes: of a 2-byte piece the aligned word around it.
 template <int BYTES>
@@ -439,15 +461,23 @@ __device__ __forceinline__ void copy_ahead(void* smem, const void* global) {
 }
 
 // zeros for the rows [from, to) of dW, at this lane's pieces (first: their place in row 0)
-template <typename W, int S>
+template <int BYTES>
+struct Zeros {
+  static constexpr int kBytes = BYTES;
+};
+template <typename Z, int S>
 __device__ __forceinline__ void zero_rows(void* first, int64_t row_bytes, int from, int to, int apart_bytes, int pieces) {
+  constexpr int kWord = Z::kBytes < 16 ? Z::kBytes : 16;
+  typename Word<kWord>::type zero;
+  memset(&zero, 0, kWord);
   char* p = static_cast<char*>(first) + from * row_bytes;
-  W zero;
-  memset(&zero, 0, sizeof(W));
   for (int t = from; t < to; ++t, p += row_bytes) {
 #pragma unroll
     for (int q = 0; q < S; ++q)
-      if (q < pieces) *reinterpret_cast<W*>(p + q * apart_bytes) = zero;
+      if (q < pieces)
+#pragma unroll
+        for (int b = 0; b < Z::kBytes; b += kWord)
+          *reinterpret_cast<typename Word<kWord>::type*>(p + q * apart_bytes + b) = zero;
   }
 }
 
@@ -458,10 +488,10 @@ __device__ __forceinline__ void zero_rows(void* first, int64_t row_bytes, int fr
 template <typename T, int VEC, int S>
 __global__ void __launch_bounds__(256) wgrad_merge_kernel(const T* __restrict__ gy, const __grid_constant__ MergeArgs a) {
   typedef Pack<T, VEC> Piece;
-  constexpr int kRows = merge_rows(S);                    // rows whose loads are in flight per worker
   constexpr int kSlot = sizeof(Piece) < 4 ? 4 : sizeof(Piece);
+  constexpr int kRows = merge_rows(S * kSlot);
   extern __shared__ uint4 merge_smem[];                    // slots (kRows, S, 256), then tokens (kRows, 256)
-  __shared__ int64_t starts[257];
+  __shared__ int2 starts[257];
   char* const slots = reinterpret_cast<char*>(merge_smem) + threadIdx.x * kSlot;
   int* const tokens = reinterpret_cast<int*>(reinterpret_cast<char*>(merge_smem) + kRows * S * 256 * kSlot) + threadIdx.x;
   uint32_t odd = 0;                                        // 2-byte pieces: bit u S + q, whether it is its word's upper half
@@ -474,17 +504,16 @@ __global__ void __launch_bounds__(256) wgrad_merge_kernel(const T* __restrict__ 
   pdl_launch_dependents();
   pdl_wait();
   {
-    const int64_t i = path_search(a, d0, G, l, mask, shift);
-    if (l == 0) starts[mine] = i;
+    const int2 at = path_start(a, d0, G, l, mask, shift);
+    if (l == 0) starts[mine] = at;
     if (mine == per_block - 1) {
-      const int64_t e = path_search(a, d1, G, l, mask, shift);
+      const int2 e = path_start(a, d1, G, l, mask, shift);
       if (l == 0) starts[per_block] = e;
     }
   }
   __syncthreads();
   if (w >= a.workers) return;
-  const int i0 = static_cast<int>(starts[mine]), i1 = static_cast<int>(starts[mine + 1]);
-  const int j0 = static_cast<int>(d0 - i0), j1 = static_cast<int>(d1 - i1);
+  const int i0 = starts[mine].x, i1 = starts[mine + 1].x, j0 = starts[mine].y, j1 = starts[mine + 1].y;
   const int c = (blockIdx.y * S * G + l) * VEC, apart = G * VEC;          // piece q: channels c + q apart ..
   const int pieces = c < a.C ? min(S, (a.C - c + apart - 1) / apart) : 0;
   bool open = j0 > 0 && i0 < a.V && a.pair[j0 - 1].x == i0;               // token i0 began in an earlier worker
@@ -508,9 +537,9 @@ __global__ void __launch_bounds__(256) wgrad_merge_kernel(const T* __restrict__ 
     }
     open = false;
     if (a.dw_dtype == BPC_DTYPE_F32)
-      zero_rows<typename Word<4 * VEC>::type, S>(static_cast<float*>(a.dw) + c, 4ll * a.C, tok + 1, t, 4 * apart, pieces);
+      zero_rows<Zeros<4 * VEC>, S>(static_cast<float*>(a.dw) + c, 4ll * a.C, tok + 1, t, 4 * apart, pieces);
     else
-      zero_rows<typename Word<2 * VEC>::type, S>(static_cast<uint16_t*>(a.dw) + c, 2ll * a.C, tok + 1, t, 2 * apart, pieces);
+      zero_rows<Zeros<2 * VEC>, S>(static_cast<uint16_t*>(a.dw) + c, 2ll * a.C, tok + 1, t, 2 * apart, pieces);
     tok = t;
   };
   // row j into slot u; the pair of the row after it is read one call ahead
@@ -573,12 +602,14 @@ __global__ void __launch_bounds__(256) wgrad_merge_kernel(const T* __restrict__ 
 // one's head, in fp64.  One with more than kLongJoin tails is left to the block's warps together, each a fixed share.
 constexpr int kLongJoin = 8;
 constexpr int kJoinWarps = 8;
-constexpr int kJoinChannels = 256;
+constexpr int kJoinRun = 8;
+constexpr int kJoinChannels = 128;
 
 template <int VEC>
 __global__ void __launch_bounds__(kJoinWarps * 32, 3) wgrad_join_kernel(const __grid_constant__ MergeArgs a) {
   __shared__ double red[kJoinWarps][32 * VEC];
-  __shared__ int64_t task_worker[kJoinWarps], task_first[kJoinWarps], task_token[kJoinWarps];
+  __shared__ int64_t task_worker[kJoinWarps][kJoinRun], task_first[kJoinWarps][kJoinRun], task_token[kJoinWarps][kJoinRun];
+  __shared__ int tasks[kJoinWarps];
   typedef Pack<float, VEC> Piece;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int c_from = blockIdx.y * kJoinChannels, c_to = min(a.C, c_from + kJoinChannels);
@@ -604,52 +635,62 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 3) wgrad_join_kernel(const __
     for (int e = 0; e < VEC; ++e) f[e] = static_cast<float>(s[e] + h.v[e]);
     store_row<VEC>(a.dw, a.dw_dtype, t * a.C + c, f, a.scale);
   };
-  for (int64_t base = static_cast<int64_t>(blockIdx.x) * kJoinWarps; base < a.workers;
+  // a warp looks at kJoinRun workers at once; few of them end a token that was cut
+  constexpr int kRun = kJoinRun;
+  const int64_t runs = (a.workers + kRun - 1) / kRun;
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * kJoinWarps; base < runs;
        base += static_cast<int64_t>(gridDim.x) * kJoinWarps) {
-    int64_t w = base + warp, first = 0, t = w < a.workers ? a.ends[w].x : -1;
-    // the nearest worker before w whose tail's token begins in it, 128 at a time; that token is t where t is one
-    for (int64_t top = w - 1; w < a.workers && top >= 0; top -= 128) {
-      unsigned begins[4];
+    const int64_t mine = (base + warp) * kRun + lane;
+    const int token = lane < kRun && mine < a.workers ? a.ends[mine].x : -1;
+    unsigned cut = __ballot_sync(0xffffffffu, token >= 0);
+    int longs = 0;
+    while (cut) {
+      const int at_lane = __ffs(cut) - 1;
+      cut &= cut - 1;
+      const int64_t w = (base + warp) * kRun + at_lane, t = __shfl_sync(0xffffffffu, token, at_lane);
+      // the nearest worker before w whose tail's token begins in it, 128 at a time: the first of token t
+      int64_t first = 0;
+      for (int64_t top = w - 1; top >= 0; top -= 128) {
+        unsigned begins[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int64_t v = top - 32 * u - lane;
-        begins[u] = __ballot_sync(0xffffffffu, v < 0 || a.ends[v].y);
-      }
-      if (t < 0) break;
-      int at = 128;
+        for (int u = 0; u < 4; ++u) {
+          const int64_t v = top - 32 * u - lane;
+          begins[u] = __ballot_sync(0xffffffffu, v < 0 || a.ends[v].y);
+        }
+        int at = 128;
 #pragma unroll
-      for (int u = 3; u >= 0; --u)
-        if (begins[u]) at = 32 * u + __ffs(begins[u]) - 1;
-      if (at < 128) {
-        first = top - at;
-        break;
+        for (int u = 3; u >= 0; --u)
+          if (begins[u]) at = 32 * u + __ffs(begins[u]) - 1;
+        if (at < 128) {
+          first = top - at;
+          break;
+        }
       }
-    }
-    if (t < 0) {
-      w = -1;
-    } else {
       if (w - first <= kLongJoin) {
         for (int c = c_from + lane * VEC; c < c_to; c += 32 * VEC) {
           double s[VEC] = {};
           add_tails(s, first, w, 1, c);
           finish(s, w, t, c);
         }
-        w = -1;
+      } else {
+        if (lane == 0) {
+          task_worker[warp][longs] = w;
+          task_first[warp][longs] = first;
+          task_token[warp][longs] = t;
+        }
+        ++longs;
       }
     }
-    if (lane == 0) {
-      task_worker[warp] = w;
-      task_first[warp] = first;
-      task_token[warp] = t;
-    }
-    __syncthreads();
-    for (int k = 0; k < kJoinWarps; ++k) {
-      const int64_t v1 = task_worker[k];
-      if (v1 < 0) continue;
+    if (lane == 0) tasks[warp] = longs;
+    if (!__syncthreads_or(longs)) continue;
+    for (int k = 0; k < kJoinWarps * kRun; ++k) {
+      if (k % kRun >= tasks[k / kRun]) continue;
+      const int64_t v1 = task_worker[k / kRun][k % kRun], v0 = task_first[k / kRun][k % kRun];
+      const int64_t t = task_token[k / kRun][k % kRun];
       for (int c0 = c_from; c0 < c_to; c0 += 32 * VEC) {
         const int c = c0 + lane * VEC;
         double s[VEC] = {};
-        if (c < c_to) add_tails(s, task_first[k] + warp, v1, kJoinWarps, c);
+        if (c < c_to) add_tails(s, v0 + warp, v1, kJoinWarps, c);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) red[warp][lane * VEC + e] = s[e];
         __syncthreads();
@@ -657,7 +698,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 3) wgrad_join_kernel(const __
           for (int q = 1; q < kJoinWarps; ++q)
 #pragma unroll
             for (int e = 0; e < VEC; ++e) s[e] += red[q][lane * VEC + e];
-          finish(s, v1, task_token[k], c);
+          finish(s, v1, t, c);
         }
         __syncthreads();
       }
@@ -938,7 +979,8 @@ WgradPlan wgrad_plan(int64_t n, int32_t V, int32_t C) {
   p.tiles = static_cast<int>((n + kSortTile - 1) / kSortTile);
   p.G = 1;
   while (p.G < 32 && p.G * 4 < C) p.G *= 2;
-  // about 32 warps per SM over the workers and the slices of 512 channels, at least 16 steps a worker
+  // about 32 warps per SM over the workers and the slices of 512 channels, at least 16 steps a worker (a step is some
+  // hundred instructions of one warp in a row: 12 longer workers' warps per SM took half as long again)
   const int64_t target = std::max<int64_t>(1, static_cast<int64_t>(num_sms()) * 32 * (32 / p.G) / ((C + 511) / 512));
   p.items = std::max<int64_t>(16, (V + n + target - 1) / target);
   p.workers = (V + n + p.items - 1) / p.items;
@@ -1008,33 +1050,34 @@ int sort_pass(const S* src, int64_t n, int V, int shift, int tiles, int* counts,
   return launched("sort_place_kernel");
 }
 
-template <typename I, int ROUNDS>
+template <typename I, int CTAS, int ROUNDS>
 int sort_cluster_rounds(const I* ids, int n, int V, int passes, int2* out, cudaStream_t s) {
-  const auto fn = sort_cluster_kernel<I, ROUNDS>;
+  const auto fn = sort_cluster_kernel<I, CTAS, ROUNDS>;
   const int smem = 2 * ROUNDS * kClusterThreads * static_cast<int>(sizeof(int2));
   if (int e = allow_smem(reinterpret_cast<const void*>(fn), smem)) return e;
+  cudaError_t e = cudaSuccess;
+  if (CTAS > 8) e = cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   cudaLaunchConfig_t lc = {};
-  lc.gridDim = dim3(kClusterCtas);
+  lc.gridDim = dim3(CTAS);
   lc.blockDim = dim3(kClusterThreads);
   lc.dynamicSmemBytes = smem;
   lc.stream = s;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = kClusterCtas;
+  attr.val.clusterDim.x = CTAS;
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   lc.attrs = &attr;
   lc.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&lc, fn, ids, n, V, passes, out);
+  if (e == cudaSuccess) e = cudaLaunchKernelEx(&lc, fn, ids, n, V, passes, out);
   return e == cudaSuccess ? 0 : fail(BPC_ERR_LAUNCH, std::string("sort_cluster_kernel launch: ") + cudaGetErrorString(e));
 }
 
 template <typename I>
 int sort_cluster(const I* ids, int n, int V, int passes, int2* out, cudaStream_t s) {
-  constexpr int kRound = kClusterCtas * kClusterThreads;
-  if (n <= kRound) return sort_cluster_rounds<I, 1>(ids, n, V, passes, out, s);
-  if (n <= 2 * kRound) return sort_cluster_rounds<I, 2>(ids, n, V, passes, out, s);
-  if (n <= 4 * kRound) return sort_cluster_rounds<I, 4>(ids, n, V, passes, out, s);
-  return sort_cluster_rounds<I, 8>(ids, n, V, passes, out, s);
+  if (n <= 8 * kClusterThreads) return sort_cluster_rounds<I, 8, 1>(ids, n, V, passes, out, s);
+  if (n <= 16 * kClusterThreads) return sort_cluster_rounds<I, 16, 1>(ids, n, V, passes, out, s);
+  if (n <= 32 * kClusterThreads) return sort_cluster_rounds<I, 16, 2>(ids, n, V, passes, out, s);
+  return sort_cluster_rounds<I, 16, 4>(ids, n, V, passes, out, s);
 }
 
 // *sorted: where the pairs are
@@ -1054,23 +1097,27 @@ int sort_ids(const I* ids, int64_t n, int V, const WgradPlan& p, int2* const (&p
 template <typename T, int VEC, int S>
 int merge_launch_pieces(const T* gy, MergeArgs a, cudaStream_t s) {
   if (S > 1) a.G = 32;
+  while (S == 1 && a.G > 1 && a.G / 2 * VEC >= a.C) a.G /= 2;              // no more lanes than pieces
   const int64_t blocks = (a.workers + 256 / a.G - 1) / (256 / a.G);
   const dim3 grid(static_cast<unsigned>(blocks), (a.C + a.G * VEC * S - 1) / (a.G * VEC * S));
   void* args[] = {&gy, &a};
   const void* fn = reinterpret_cast<const void*>(&wgrad_merge_kernel<T, VEC, S>);
-  constexpr int kSmem = merge_rows(S) * 256 * (S * std::max(4, VEC * static_cast<int>(sizeof(T))) + static_cast<int>(sizeof(int)));
+  constexpr int kSlots = S * std::max(4, VEC * static_cast<int>(sizeof(T)));
+  constexpr int kSmem = merge_rows(kSlots) * 256 * (kSlots + static_cast<int>(sizeof(int)));
   if (int e = allow_smem(fn, kSmem)) return e;
   if (int e = launch_pdl(fn, grid, dim3(256), kSmem, s, args, 1, "wgrad_merge_kernel")) return e;
   void* join_args[] = {&a};
-  const int64_t join = std::min<int64_t>((a.workers + kJoinWarps - 1) / kJoinWarps, 8 * num_sms());
-  return launch_pdl(reinterpret_cast<const void*>(&wgrad_join_kernel<VEC>),
+  const int64_t join = std::min<int64_t>((a.workers + kJoinWarps * kJoinRun - 1) / (kJoinWarps * kJoinRun), 8 * num_sms());
+  return launch_pdl(reinterpret_cast<const void*>(&wgrad_join_kernel<(VEC < 4 ? VEC : 4)>),
                     dim3(static_cast<unsigned>(join), (a.C + kJoinChannels - 1) / kJoinChannels),
                     dim3(kJoinWarps * 32), 0, s, join_args, 1, "wgrad_join_kernel");
 }
 
 template <typename T, int VEC>
 int merge_launch_vec(const T* gy, const MergeArgs& a, cudaStream_t s) {
-  if (a.C > 64 * VEC) return merge_launch_pieces<T, VEC, 4>(gy, a, s);
+  if constexpr (VEC < 8) {                                 // at most 512 channels per worker
+    if (a.C > 64 * VEC) return merge_launch_pieces<T, VEC, 4>(gy, a, s);
+  }
   return a.C > 32 * VEC ? merge_launch_pieces<T, VEC, 2>(gy, a, s) : merge_launch_pieces<T, VEC, 1>(gy, a, s);
 }
 
@@ -1078,10 +1125,12 @@ template <typename T>
 int merge_launch(const void* gy, const MergeArgs& a, cudaStream_t s) {
   const auto fits = [&](int vec) {
     return a.C % vec == 0 && a.ldg % vec == 0 && reinterpret_cast<uintptr_t>(gy) % (vec * sizeof(T)) == 0 &&
-           reinterpret_cast<uintptr_t>(a.dw) % (vec * dtype_size(a.dw_dtype)) == 0;
+           reinterpret_cast<uintptr_t>(a.dw) % std::min(16, vec * dtype_size(a.dw_dtype)) == 0;
   };
   const T* g = static_cast<const T*>(gy);
-  // 16 bytes of the wider of gy and the fp32 sums that head and tail hold
+  if constexpr (sizeof(T) == 2) {
+    if (fits(8)) return merge_launch_vec<T, 8>(g, a, s);
+  }
   if (fits(4)) return merge_launch_vec<T, 4>(g, a, s);
   if (fits(2)) return merge_launch_vec<T, 2>(g, a, s);
   return merge_launch_vec<T, 1>(g, a, s);
