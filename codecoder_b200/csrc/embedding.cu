@@ -485,7 +485,8 @@ __device__ __forceinline__ void zero_rows(void* first, int64_t row_bytes, int fr
 // rows ahead into its own slots of shared memory (and reads only those, so no barrier is needed): the loads in flight do
 // not depend on the registers, which held a block of eight rows to two per SM.  More pieces per lane share a step's
 // bookkeeping, which bounded two pieces (88 instructions a step at 50,021 tokens x 1,024).
-template <typename T, int VEC, int S>
+// FULL: every lane has all S pieces.
+template <typename T, int VEC, int S, bool FULL>
 __global__ void __launch_bounds__(256) wgrad_merge_kernel(const T* __restrict__ gy, const __grid_constant__ MergeArgs a) {
   typedef Pack<T, VEC> Piece;
   constexpr int kSlot = sizeof(Piece) < 4 ? 4 : sizeof(Piece);
@@ -515,7 +516,7 @@ __global__ void __launch_bounds__(256) wgrad_merge_kernel(const T* __restrict__ 
   if (w >= a.workers) return;
   const int i0 = starts[mine].x, i1 = starts[mine + 1].x, j0 = starts[mine].y, j1 = starts[mine + 1].y;
   const int c = (blockIdx.y * S * G + l) * VEC, apart = G * VEC;          // piece q: channels c + q apart ..
-  const int pieces = c < a.C ? min(S, (a.C - c + apart - 1) / apart) : 0;
+  const int pieces = FULL ? S : c < a.C ? min(S, (a.C - c + apart - 1) / apart) : 0;
   bool open = j0 > 0 && i0 < a.V && a.pair[j0 - 1].x == i0;               // token i0 began in an earlier worker
   if (l == 0 && blockIdx.y == 0) a.ends[w] = make_int2(open && i1 > i0 ? i0 : -1, i1 > i0 || !open);
   float acc[S][VEC];
@@ -544,23 +545,22 @@ __global__ void __launch_bounds__(256) wgrad_merge_kernel(const T* __restrict__ 
   };
   // row j into slot u; the pair of the row after it is read one call ahead
   int2 ahead = j0 < j1 ? a.pair[j0] : make_int2(a.V, 0);
-  int next = j0;
-  const T* const lane_gy = gy + c;
-  const auto copy_row = [&](int u) {
-    if (next < j1) {
+  const char* const lane_gy = reinterpret_cast<const char*>(gy + c);
+  const int64_t row_bytes = a.ldg * static_cast<int64_t>(sizeof(T));
+  const auto copy_row = [&](int u, int j) {
+    if (j < j1) {
       const int2 p = ahead;
-      ++next;
-      if (next < j1) ahead = a.pair[next];
+      if (j + 1 < j1) ahead = a.pair[j + 1];
       tokens[u * 256] = p.x;
       if (p.x < a.V) {                                     // V: a position without a token
-        const T* row = lane_gy + p.y * a.ldg;
+        const char* row = lane_gy + p.y * row_bytes;
 #pragma unroll
         for (int q = 0; q < S; ++q)
           if (q < pieces) {
             if constexpr (sizeof(Piece) >= 4) {
-              copy_ahead<kSlot>(slots + (u * S + q) * 256 * kSlot, row + q * apart);
+              copy_ahead<kSlot>(slots + (u * S + q) * 256 * kSlot, row + q * apart * sizeof(T));
             } else {
-              const uintptr_t at = reinterpret_cast<uintptr_t>(row + q * apart);
+              const uintptr_t at = reinterpret_cast<uintptr_t>(row + q * apart * sizeof(T));
               const uint32_t bit = 1u << (u * S + q);
               odd = at & 2 ? odd | bit : odd & ~bit;
               copy_ahead<4>(slots + (u * S + q) * 256 * kSlot, reinterpret_cast<const void*>(at & ~static_cast<uintptr_t>(3)));
@@ -571,23 +571,29 @@ __global__ void __launch_bounds__(256) wgrad_merge_kernel(const T* __restrict__ 
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 #pragma unroll
-  for (int u = 0; u < kRows - 1; ++u) copy_row(u);
-  int u = 0;
-  for (int j = j0; j < j1; ++j) {
-    copy_row(u == 0 ? kRows - 1 : u - 1);                  // into the slot that the step before read
-    asm volatile("cp.async.wait_group %0;" ::"n"(kRows - 1) : "memory");
-    const int t = tokens[u * 256];
-    if (t >= a.V) break;                                   // they are the last ones
-    if (tok < t) end_tokens(t);
+  for (int u = 0; u < kRows - 1; ++u) copy_row(u, j0 + u);
+  bool more = true;
+  for (int j = j0; more && j < j1; j += kRows) {
 #pragma unroll
-    for (int q = 0; q < S; ++q) {
-      if (q < pieces) {
-        const Piece x = load_pack<Piece>(slots + (u * S + q) * 256 * kSlot + (sizeof(Piece) < 4 ? odd >> (u * S + q) << 1 & 2 : 0));
+    for (int u = 0; u < kRows; ++u) {
+      if (!more || j + u >= j1) break;
+      copy_row((u + kRows - 1) % kRows, j + u + kRows - 1);               // into the slot that the step before read
+      asm volatile("cp.async.wait_group %0;" ::"n"(kRows - 1) : "memory");
+      const int t = tokens[u * 256];
+      if (t >= a.V) {                                      // the ones without a token are the last
+        more = false;
+        break;
+      }
+      if (tok < t) end_tokens(t);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) acc[q][e] += to_f32(x.v[e]);
+      for (int q = 0; q < S; ++q) {
+        if (q < pieces) {
+          const Piece x = load_pack<Piece>(slots + (u * S + q) * 256 * kSlot + (sizeof(Piece) < 4 ? odd >> (u * S + q) << 1 & 2 : 0));
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) acc[q][e] += to_f32(x.v[e]);
+        }
       }
     }
-    u = u == kRows - 1 ? 0 : u + 1;
   }
   if (tok < i1) end_tokens(i1);
   if (i1 < a.V && j1 > 0 && a.pair[j1 - 1].x == i1) {
@@ -1094,14 +1100,14 @@ int sort_ids(const I* ids, int64_t n, int V, const WgradPlan& p, int2* const (&p
   return 0;
 }
 
-template <typename T, int VEC, int S>
+template <typename T, int VEC, int S, bool FULL>
 int merge_launch_pieces(const T* gy, MergeArgs a, cudaStream_t s) {
   if (S > 1) a.G = 32;
   while (S == 1 && a.G > 1 && a.G / 2 * VEC >= a.C) a.G /= 2;              // no more lanes than pieces
   const int64_t blocks = (a.workers + 256 / a.G - 1) / (256 / a.G);
   const dim3 grid(static_cast<unsigned>(blocks), (a.C + a.G * VEC * S - 1) / (a.G * VEC * S));
   void* args[] = {&gy, &a};
-  const void* fn = reinterpret_cast<const void*>(&wgrad_merge_kernel<T, VEC, S>);
+  const void* fn = reinterpret_cast<const void*>(&wgrad_merge_kernel<T, VEC, S, FULL>);
   constexpr int kSlots = S * std::max(4, VEC * static_cast<int>(sizeof(T)));
   constexpr int kSmem = merge_rows(kSlots) * 256 * (kSlots + static_cast<int>(sizeof(int)));
   if (int e = allow_smem(fn, kSmem)) return e;
@@ -1113,12 +1119,18 @@ int merge_launch_pieces(const T* gy, MergeArgs a, cudaStream_t s) {
                     dim3(kJoinWarps * 32), 0, s, join_args, 1, "wgrad_join_kernel");
 }
 
+template <typename T, int VEC, int S>
+int merge_launch_full(const T* gy, const MergeArgs& a, cudaStream_t s) {
+  if (S > 1 && a.C % (32 * VEC * S) == 0) return merge_launch_pieces<T, VEC, S, true>(gy, a, s);
+  return merge_launch_pieces<T, VEC, S, false>(gy, a, s);
+}
+
 template <typename T, int VEC>
 int merge_launch_vec(const T* gy, const MergeArgs& a, cudaStream_t s) {
   if constexpr (VEC < 8) {                                 // at most 512 channels per worker
-    if (a.C > 64 * VEC) return merge_launch_pieces<T, VEC, 4>(gy, a, s);
+    if (a.C > 64 * VEC) return merge_launch_full<T, VEC, 4>(gy, a, s);
   }
-  return a.C > 32 * VEC ? merge_launch_pieces<T, VEC, 2>(gy, a, s) : merge_launch_pieces<T, VEC, 1>(gy, a, s);
+  return a.C > 32 * VEC ? merge_launch_full<T, VEC, 2>(gy, a, s) : merge_launch_full<T, VEC, 1>(gy, a, s);
 }
 
 template <typename T>
