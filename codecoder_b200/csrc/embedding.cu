@@ -485,7 +485,7 @@ __device__ __forceinline__ void zero_rows(void* first, int64_t row_bytes, int fr
 // rows ahead into its own slots of shared memory (and reads only those, so no barrier is needed): the loads in flight do
 // not depend on the registers, which held a block of eight rows to two per SM.  More pieces per lane share a step's
 // bookkeeping, which bounded two pieces (88 instructions a step at 50,021 tokens x 1,024).
-// FULL: every lane has all S pieces.
+// FULL: every lane has all S pieces, and dW begins on 16 bytes.
 template <typename T, int VEC, int S, bool FULL>
 __global__ void __launch_bounds__(256) wgrad_merge_kernel(const T* __restrict__ gy, const __grid_constant__ MergeArgs a) {
   typedef Pack<T, VEC> Piece;
@@ -537,7 +537,14 @@ __global__ void __launch_bounds__(256) wgrad_merge_kernel(const T* __restrict__ 
       for (int e = 0; e < VEC; ++e) acc[q][e] = 0.f;
     }
     open = false;
-    if (a.dw_dtype == BPC_DTYPE_F32)
+    if (FULL && VEC * S >= 4 && a.dw_dtype == BPC_DTYPE_F32) {
+      // a warp's pieces of a row are one run of memory: 16 bytes a lane along it, whole sectors in every store
+      char* p = reinterpret_cast<char*>(static_cast<float*>(a.dw) + (tok + 1) * static_cast<int64_t>(a.C) +
+                                        blockIdx.y * S * 32 * VEC) + l * 16;
+      for (int v = tok + 1; v < t; ++v, p += 4ll * a.C)
+#pragma unroll
+        for (int b = 0; b < VEC * S / 4; ++b) *reinterpret_cast<uint4*>(p + b * 512) = make_uint4(0, 0, 0, 0);
+    } else if (a.dw_dtype == BPC_DTYPE_F32)
       zero_rows<Zeros<4 * VEC>, S>(static_cast<float*>(a.dw) + c, 4ll * a.C, tok + 1, t, 4 * apart, pieces);
     else
       zero_rows<Zeros<2 * VEC>, S>(static_cast<uint16_t*>(a.dw) + c, 2ll * a.C, tok + 1, t, 2 * apart, pieces);
@@ -881,6 +888,7 @@ __global__ void __launch_bounds__(kFewThreads + 32) wgrad_few_kernel(const __gri
     if (v < a.V)
 #pragma unroll
       for (int e = 0; e < VEC; ++e) sums[(v * VEC + e) * kFewThreads + tid] = s[v][e];
+  pdl_launch_dependents();
   asm volatile("bar.sync 1, %0;" ::"n"(kFewThreads) : "memory");            // the eight warps that add
   for (int i = tid; i < a.V * p.pieces; i += kFewThreads) {
     const int v = i / p.pieces, xx = i - v * p.pieces;
@@ -908,6 +916,7 @@ __global__ void __launch_bounds__(1024) wgrad_few_join_kernel(const float* __res
                                                               float scale, void* dw, int dw_dtype) {
   __shared__ double red[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  pdl_wait();
   const int i = blockIdx.x * 32 + lane;
   double s = 0.0;
   if (i < n) {
@@ -1121,7 +1130,8 @@ int merge_launch_pieces(const T* gy, MergeArgs a, cudaStream_t s) {
 
 template <typename T, int VEC, int S>
 int merge_launch_full(const T* gy, const MergeArgs& a, cudaStream_t s) {
-  if (S > 1 && a.C % (32 * VEC * S) == 0) return merge_launch_pieces<T, VEC, S, true>(gy, a, s);
+  if (S > 1 && a.C % (32 * VEC * S) == 0 && reinterpret_cast<uintptr_t>(a.dw) % 16 == 0)
+    return merge_launch_pieces<T, VEC, S, true>(gy, a, s);
   return merge_launch_pieces<T, VEC, S, false>(gy, a, s);
 }
 
@@ -1156,10 +1166,13 @@ int few_launch_tokens(const FewArgs& a, cudaStream_t s) {
   fn<<<dim3(static_cast<unsigned>(a.p.blocks), a.p.slices), kFewThreads + 32, smem, s>>>(a);
   if (int e = launched("wgrad_few_kernel")) return e;
   if (a.p.blocks == 1) return 0;
-  const int sums = a.V * a.C;
-  wgrad_few_join_kernel<<<(sums + 31) / 32, 1024, 0, s>>>(a.partial, static_cast<int>(a.p.blocks), sums, a.scale, a.dw,
-                                                          a.dw_dtype);
-  return launched("wgrad_few_join_kernel");
+  int sums = a.V * a.C, blocks = static_cast<int>(a.p.blocks), dw_dtype = a.dw_dtype;
+  const float* partial = a.partial;
+  float scale = a.scale;
+  void* dw = a.dw;
+  void* args[] = {&partial, &blocks, &sums, &scale, &dw, &dw_dtype};
+  return launch_pdl(reinterpret_cast<const void*>(&wgrad_few_join_kernel), dim3((sums + 31) / 32), dim3(1024), 0, s, args, 1,
+                    "wgrad_few_join_kernel");
 }
 
 template <typename T, typename I, int VEC>

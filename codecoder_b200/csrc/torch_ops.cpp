@@ -137,6 +137,14 @@ Tensor embed_wgrad(const Tensor& gy_in, const Tensor& ids_in, int64_t n_tokens, 
   return dw;
 }
 
+// The tensors of a Python list, borrowed from it (the GIL is held meanwhile): a vector of tensors would count every
+// reference up and down.
+const Tensor& tensor_at(const py::list& list, size_t k, const char* what) {
+  PyObject* o = PyList_GET_ITEM(list.ptr(), static_cast<Py_ssize_t>(k));
+  TORCH_CHECK_TYPE(THPVariable_Check(o), what, " takes a list of tensors, got ", Py_TYPE(o)->tp_name);
+  return THPVariable_Unpack(o);
+}
+
 // Host arrays of a list of dense tensors on one GPU
 struct TensorArrays {
   std::vector<void*> at;
@@ -144,65 +152,74 @@ struct TensorArrays {
   std::vector<int32_t> dtype;
 };
 
-TensorArrays arrays_of(const std::vector<Tensor>& ts, const char* what) {
-  TORCH_CHECK_VALUE(!ts.empty(), what, " needs at least one tensor");
-  check_cuda(ts[0]);
+TensorArrays arrays_of(const py::list& list, const char* what) {
+  const size_t n = list.size();
+  TORCH_CHECK_VALUE(n > 0, what, " needs at least one tensor");
+  const Tensor& first = tensor_at(list, 0, what);
+  check_cuda(first);
+  const at::Device device = first.device();
   TensorArrays a;
-  a.at.reserve(ts.size());
-  a.numel.reserve(ts.size());
-  a.dtype.reserve(ts.size());
-  for (const Tensor& t : ts) {
-    TORCH_CHECK_VALUE(t.device() == ts[0].device(), what, ": tensors are on different devices");
-    TORCH_CHECK_TYPE(t.layout() == at::kStrided && dtype_code(t.scalar_type()) >= 0, what,
-                     " takes dense fp32, bf16 and fp16 tensors, got ", t.layout(), " ", t.scalar_type());
+  a.at.resize(n);
+  a.numel.resize(n);
+  a.dtype.resize(n);
+  for (size_t k = 0; k < n; ++k) {
+    const Tensor& t = tensor_at(list, k, what);
+    TORCH_CHECK_VALUE(t.device() == device, what, ": tensors are on different devices");
+    const int32_t code = dtype_code(t.scalar_type());
+    TORCH_CHECK_TYPE(t.layout() == at::kStrided && code >= 0, what, " takes dense fp32, bf16 and fp16 tensors, got ",
+                     t.layout(), " ", t.scalar_type());
     TORCH_CHECK_VALUE(t.is_non_overlapping_and_dense(), what,
                       ": a tensor with gaps or overlaps between its elements (strides ", t.strides(), ")");
-    a.at.push_back(t.data_ptr());
-    a.numel.push_back(t.numel());
-    a.dtype.push_back(dtype_code(t.scalar_type()));
+    a.at[k] = const_cast<void*>(t.const_data_ptr());
+    a.numel[k] = t.numel();
+    a.dtype[k] = code;
   }
   return a;
 }
 
-// One allocation of doubles: the kernels' partial sums
 Tensor norm_workspace(const Tensor& like, size_t n) {
   return empty({static_cast<int64_t>(entry.grad_norm_workspace_size(static_cast<int32_t>(n)))}, at::kByte, like);
 }
 
-Tensor grad_norm(const std::vector<Tensor>& ts) {
+Tensor grad_norm(const py::list& ts) {
   const TensorArrays a = arrays_of(ts, "grad_norm");
-  const c10::cuda::CUDAGuard guard(ts[0].device());
-  Tensor norm = empty({}, at::kFloat, ts[0]), ws = norm_workspace(ts[0], ts.size());
-  check(entry.grad_norm(a.at.data(), a.numel.data(), a.dtype.data(), static_cast<int32_t>(ts.size()),
-                        static_cast<float*>(norm.data_ptr()), ws.data_ptr(), ws.numel(), stream_of(ts[0])),
+  const Tensor& first = tensor_at(ts, 0, "grad_norm");
+  const c10::cuda::CUDAGuard guard(first.device());
+  Tensor norm = empty({}, at::kFloat, first), ws = norm_workspace(first, a.at.size());
+  check(entry.grad_norm(a.at.data(), a.numel.data(), a.dtype.data(), static_cast<int32_t>(a.at.size()),
+                        static_cast<float*>(norm.data_ptr()), ws.data_ptr(), ws.numel(), stream_of(first)),
         "bpc_grad_norm");
   return norm;
 }
 
-Tensor clip_grads(const std::vector<Tensor>& ts, double max_norm, const std::optional<std::vector<Tensor>>& out) {
+Tensor clip_grads(const py::list& ts, double max_norm, const std::optional<py::list>& out) {
   const TensorArrays a = arrays_of(ts, "clip_grads");
-  const std::vector<Tensor>& outs = out ? *out : ts;
+  const py::list& outs = out ? *out : ts;
+  const Tensor& first = tensor_at(ts, 0, "clip_grads");
   TensorArrays other;
   if (out) {
     TORCH_CHECK_VALUE(outs.size() == ts.size(), "clip_grads: out must hold one tensor of the same shape per gradient");
     other = arrays_of(outs, "clip_grads");
-    TORCH_CHECK_VALUE(outs[0].device() == ts[0].device(), "clip_grads: tensors are on different devices");
-    for (size_t k = 0; k < ts.size(); ++k) {
-      TORCH_CHECK_VALUE(outs[k].sizes() == ts[k].sizes(),
-                        "clip_grads: out must hold one tensor of the same shape per gradient");
-      TORCH_CHECK_VALUE((outs[k].is_contiguous() && ts[k].is_contiguous()) || outs[k].strides() == ts[k].strides(),
+    TORCH_CHECK_VALUE(tensor_at(outs, 0, "clip_grads").device() == first.device(),
+                      "clip_grads: tensors are on different devices");
+    for (size_t k = 0; k < a.at.size(); ++k) {
+      const Tensor &o = tensor_at(outs, k, "clip_grads"), &t = tensor_at(ts, k, "clip_grads");
+      TORCH_CHECK_VALUE(o.sizes() == t.sizes(), "clip_grads: out must hold one tensor of the same shape per gradient");
+      TORCH_CHECK_VALUE((o.is_contiguous() && t.is_contiguous()) || o.strides() == t.strides(),
                         "clip_grads: out must have the gradients' strides");
     }
   }
   const TensorArrays& b = out ? other : a;
-  const c10::cuda::CUDAGuard guard(ts[0].device());
-  Tensor norm = empty({}, at::kFloat, ts[0]), ws = norm_workspace(ts[0], ts.size());
+  const c10::cuda::CUDAGuard guard(first.device());
+  Tensor norm = empty({}, at::kFloat, first), ws = norm_workspace(first, a.at.size());
   check(entry.clip_grads(a.at.data(), b.at.data(), a.numel.data(), a.dtype.data(), b.dtype.data(),
-                         static_cast<int32_t>(ts.size()), max_norm, static_cast<float*>(norm.data_ptr()), ws.data_ptr(),
-                         ws.numel(), stream_of(ts[0])),
+                         static_cast<int32_t>(a.at.size()), max_norm, static_cast<float*>(norm.data_ptr()), ws.data_ptr(),
+                         ws.numel(), stream_of(first)),
         "bpc_clip_grads");
-  for (const Tensor& t : outs)                       // written behind autograd's back: count a new version
+  for (size_t k = 0; k < a.at.size(); ++k) {         // written behind autograd's back: count a new version
+    const Tensor& t = tensor_at(outs, k, "clip_grads");
     if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  }
   return norm;
 }
 
@@ -213,6 +230,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   const auto release = py::call_guard<py::gil_scoped_release>();
   m.def("embed_lookup", &embed_lookup, release);
   m.def("embed_wgrad", &embed_wgrad, release);
-  m.def("grad_norm", &grad_norm, release);
-  m.def("clip_grads", &clip_grads, release);
+  m.def("grad_norm", &grad_norm);
+  m.def("clip_grads", &clip_grads);
 }
