@@ -64,9 +64,10 @@ __device__ __forceinline__ void store_pack(void* p, const P& x) {
 // lookup: the threads lie along a row's pieces of VEC channels and several rows, kLookupRows rows per thread in flight
 // (one at a time left the stores waiting for the ids' and the table's latency: 5.0 TB/s at 258,048 rows of 512 fp32).
 constexpr int kLookupRows = 4;
+constexpr int kLookupBlocks = 4;                          // per SM
 
 template <typename I, typename TW, typename TY, int VEC>
-__global__ void __launch_bounds__(256) embed_lookup_kernel(const I* __restrict__ ids, const TW* __restrict__ w,
+__global__ void __launch_bounds__(256, kLookupBlocks) embed_lookup_kernel(const I* __restrict__ ids, const TW* __restrict__ w,
                                                            TY* __restrict__ y, int64_t n, int V, int C, int pieces,
                                                            int rows_at_once, int64_t ldw, float scale) {
   const int tx = threadIdx.x % pieces, ty = threadIdx.x / pieces;
@@ -613,7 +614,7 @@ __global__ void __launch_bounds__(256) wgrad_merge_kernel(const T* __restrict__ 
 
 // A warp per token that crosses workers and kJoinChannels channels: the tails of the workers since its first row, then the last
 // one's head, in fp64.  One with more than kLongJoin tails is left to the block's warps together, each a fixed share.
-constexpr int kLongJoin = 8;
+constexpr int kLongJoin = 64;
 constexpr int kJoinWarps = 8;
 constexpr int kJoinRun = 8;
 constexpr int kJoinChannels = 128;
@@ -1029,7 +1030,9 @@ int lookup_launch(const void* ids, const void* w, void* y, int64_t n, int V, int
   const int units = wide ? C / kVec : C;
   const int slices = (units + 255) / 256, pieces = (units + slices - 1) / slices, rows_at_once = 256 / pieces;
   const int64_t blocks = (n + rows_at_once * kLookupRows - 1) / (rows_at_once * kLookupRows);
-  const dim3 grid(static_cast<unsigned>(std::min<int64_t>(blocks, static_cast<int64_t>(num_sms()) * 16)), slices);
+  // one wave of blocks with equal shares of the rows
+  const int64_t rounds = (blocks + num_sms() * kLookupBlocks - 1) / (num_sms() * kLookupBlocks);
+  const dim3 grid(static_cast<unsigned>((blocks + rounds - 1) / rounds), slices);
   const auto run = [&](auto kernel) {
     kernel<<<grid, 256, 0, s>>>(static_cast<const I*>(ids), static_cast<const TW*>(w), static_cast<TY*>(y), n, V, C, pieces,
                                 rows_at_once, ldw, scale);
