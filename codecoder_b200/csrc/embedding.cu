@@ -616,7 +616,7 @@ __global__ void __launch_bounds__(256) wgrad_merge_kernel(const T* __restrict__ 
 // one's head, in fp64.  One with more than kLongJoin tails is left to the block's warps together, each a fixed share.
 constexpr int kLongJoin = 64;
 constexpr int kJoinWarps = 8;
-constexpr int kJoinRun = 8;
+constexpr int kJoinRun = 4;
 constexpr int kJoinChannels = 128;
 
 template <int VEC>
