@@ -432,10 +432,15 @@ class CascadeNet(nn.Module):
     Eval on the GPU: the blocks on the B200 kernels (with C14-size blocks the embedded stream is never written: the
     stem and the first block's kernels read the embedding table by token, and the last block boundary writes
     SiLU(bn_out(h))); the read-out's pooling and scatter are plain dense GEMMs (cuBLAS) in bf16 as under the
-    reference's autocast, its MLP in fp32."""
+    reference's autocast, its MLP in fp32.
 
-    def __init__(self, geo, H, L, det_t, det_typ, det_site, logicals, res="branch"):
+    embedding: the stem's lookup embedding(tokens, weight) wherever the embedded stream is written (training, CPU, blocks
+    of other sizes); ops.embedding runs it and its weight gradient on the library's kernels (GPU only): the same
+    values, a gradient that repeats bit for bit."""
+
+    def __init__(self, geo, H, L, det_t, det_typ, det_site, logicals, res="branch", embedding=F.embedding):
         super().__init__()
+        self.embedding = embedding
         if H % 4:
             raise ValueError("H must be a multiple of 4")
         self.H, self.L = H, L
@@ -487,7 +492,7 @@ class CascadeNet(nn.Module):
 
     def forward(self, det: torch.Tensor) -> torch.Tensor:
         if self.training or not det.is_cuda:
-            h = self.embed(self.tokens(det))
+            h = self.embedding(self.tokens(det), self.embed.weight)
             for b in self.blocks:
                 h = b(h)
             return self.readout(F.silu(self.bn_out(h.reshape(-1, self.H)).view(h.shape)))
@@ -498,6 +503,6 @@ class CascadeNet(nn.Module):
             tokens = (det.to(torch.uint8).contiguous(), *self._tables, self.embed.weight.float().contiguous())
             _, x = CascadeStack.forward_blocks(self.blocks, None, final=_fold_bn(self.bn_out), tokens=tokens)
         else:
-            h = self.embed(self.tokens(det))
+            h = self.embedding(self.tokens(det), self.embed.weight)
             _, x = CascadeStack.forward_blocks(self.blocks, h.float().contiguous(), final=_fold_bn(self.bn_out))
         return self.readout(x, torch.bfloat16)

@@ -31,11 +31,14 @@ from .params import N_TOKENS
 class PreDecoderNet(nn.Module):
     """geo: geometry.RotatedSurface; cfg: params.PreDecoderConfig; params: optional init_params-style dict (fp32
     numpy) to start from, else a seeded init with the same bounds.  `gmm` is the bipartite-conv op with the
-    reference's signature gmm(x, w, idx, inv) (default: the B200 op)."""
+    reference's signature gmm(x, w, idx, inv) (default: the B200 op); `embedding` the lookup embedding(ids, weight) of the
+    unfused network (ops.embedding: on the library's kernels, GPU only)."""
 
-    def __init__(self, geo, cfg, params: dict | None = None, gmm=gather_mm, seed: int = 0, fused: bool = True):
+    def __init__(self, geo, cfg, params: dict | None = None, gmm=gather_mm, seed: int = 0, fused: bool = True,
+                 embedding=F.embedding):
         super().__init__()
         self.fused = fused
+        self.embedding = embedding
         if cfg.K != geo.K or cfg.d != geo.d or cfg.rounds != geo.R:
             raise ValueError("configuration and geometry disagree")
         self.cfg, self.gmm = cfg, gmm
@@ -88,7 +91,7 @@ class PreDecoderNet(nn.Module):
 
     def _forward_unfused(self, det: torch.Tensor) -> torch.Tensor:
         tok = 2 * self.check_type + det.long()
-        hc = F.embedding(tok, self.embed)
+        hc = self.embedding(tok, self.embed)
         hd = None
         for l in range(self.cfg.layers):
             u = F.gelu(self.gmm(hc, self.w_c2d[l], self.c2d, self.inv_c2d), approximate="tanh")
@@ -124,10 +127,12 @@ class PreDecoderNet(nn.Module):
 class Trainer:
     """One process per GPU.  model: PreDecoderNet on `device`; with an initialised process group of world > 1 the
     model is wrapped in DDP (NCCL on GPUs, gloo on CPU).  graph=True (one GPU): step_graphed replays the whole step
-    from a CUDA graph (the optimiser then keeps its step count on the device)."""
+    from a CUDA graph (the optimiser then keeps its step count on the device).  clip_grad: the clipping with torch's
+    signature clip_grad(parameters, max_norm); ops.clip_grad_norm_ runs it on the library's kernels (GPU only): two
+    launches for the whole list, the norm in 64 bits."""
 
     def __init__(self, model: PreDecoderNet, lr: float = 1e-3, clip: float = 1.0, autocast: bool = True,
-                 graph: bool = False):
+                 graph: bool = False, clip_grad=torch.nn.utils.clip_grad_norm_):
         import torch.distributed as dist
         self.model = model
         self.device = next(model.parameters()).device
@@ -146,6 +151,7 @@ class Trainer:
             raise ValueError("graphed training steps run on one GPU (DDP's all-reduce is not captured)")
         self.opt = torch.optim.Adam(self.params, lr=lr, capturable=self.graphable)
         self.clip = clip
+        self.clip_grad = clip_grad
         self.autocast = autocast and self.device.type == "cuda"
         self._graph = None
 
@@ -160,7 +166,7 @@ class Trainer:
         with ctx:
             loss = self.net(det, err)            # logits and loss (fused on the GPU path)
         loss.backward()
-        torch.nn.utils.clip_grad_norm_(self.params, self.clip)
+        self.clip_grad(self.params, self.clip)
         self.opt.step()
         return loss.detach()
 
