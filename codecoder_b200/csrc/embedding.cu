@@ -461,25 +461,15 @@ __device__ __forceinline__ void copy_ahead(void* smem, const void* global) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(smem)), "l"(global), "n"(BYTES) : "memory");
 }
 
-// zeros for the rows [from, to) of dW, at this lane's pieces (first: their place in row 0)
-template <int BYTES>
-struct Zeros {
-  static constexpr int kBytes = BYTES;
-};
-template <typename Z, int S>
-__device__ __forceinline__ void zero_rows(void* first, int64_t row_bytes, int from, int to, int apart_bytes, int pieces) {
-  constexpr int kWord = Z::kBytes < 16 ? Z::kBytes : 16;
-  typename Word<kWord>::type zero;
-  memset(&zero, 0, kWord);
-  char* p = static_cast<char*>(first) + from * row_bytes;
-  for (int t = from; t < to; ++t, p += row_bytes) {
-#pragma unroll
-    for (int q = 0; q < S; ++q)
-      if (q < pieces)
-#pragma unroll
-        for (int b = 0; b < Z::kBytes; b += kWord)
-          *reinterpret_cast<typename Word<kWord>::type*>(p + q * apart_bytes + b) = zero;
-  }
+// zeros for a run of memory, by the G lanes of a worker: 16 bytes a lane between its unaligned ends (every type's size is
+// a multiple of 2 bytes, and so is the alignment of dW)
+__device__ __forceinline__ void zero_run(char* p, int64_t bytes, int l, int G) {
+  const int64_t front = (0 - reinterpret_cast<uintptr_t>(p)) & 15, head = front < bytes ? front : bytes;
+  for (int64_t b = 2 * l; b < head; b += 2 * G) *reinterpret_cast<uint16_t*>(p + b) = 0;
+  const int64_t whole = (bytes - head) / 16;
+  uint4* q = reinterpret_cast<uint4*>(p + head);
+  for (int64_t k = l; k < whole; k += G) q[k] = make_uint4(0, 0, 0, 0);
+  for (int64_t b = head + 16 * whole + 2 * l; b < bytes; b += 2 * G) *reinterpret_cast<uint16_t*>(p + b) = 0;
 }
 
 // S pieces of VEC channels per lane, G VEC channels apart (G = 32 lanes where S > 1).  Every lane copies its pieces of the
@@ -545,10 +535,10 @@ __global__ void __launch_bounds__(256) wgrad_merge_kernel(const T* __restrict__ 
       for (int v = tok + 1; v < t; ++v, p += 4ll * a.C)
 #pragma unroll
         for (int b = 0; b < VEC * S / 4; ++b) *reinterpret_cast<uint4*>(p + b * 512) = make_uint4(0, 0, 0, 0);
-    } else if (a.dw_dtype == BPC_DTYPE_F32)
-      zero_rows<Zeros<4 * VEC>, S>(static_cast<float*>(a.dw) + c, 4ll * a.C, tok + 1, t, 4 * apart, pieces);
-    else
-      zero_rows<Zeros<2 * VEC>, S>(static_cast<uint16_t*>(a.dw) + c, 2ll * a.C, tok + 1, t, 2 * apart, pieces);
+    } else if (blockIdx.y == 0 && tok + 1 < t) {           // whole rows, of every slice
+      const int64_t row_bytes = a.C * (a.dw_dtype == BPC_DTYPE_F32 ? 4ll : 2ll);
+      zero_run(static_cast<char*>(a.dw) + (tok + 1) * row_bytes, (t - tok - 1) * row_bytes, l, G);
+    }
     tok = t;
   };
   // row j into slot u; the pair of the row after it is read one call ahead
