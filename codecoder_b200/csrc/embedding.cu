@@ -971,6 +971,9 @@ struct WgradPlan {
   size_t pair[2], counts, totals, head, tail, ends, bytes;
 };
 
+// The most blocks along the rows; few_plan's slices are the fewest with eight channels a piece.
+int64_t few_most(int slices) { return std::max<int64_t>(1, kFewBlocksPerSm * static_cast<int64_t>(num_sms()) / slices); }
+
 // Few tokens: how a block reads its rows, by alignment and row length.
 FewPlan few_plan(const void* gy, const void* dw, int64_t n, int C, int64_t ldg, int size) {
   FewPlan p;
@@ -993,7 +996,7 @@ FewPlan few_plan(const void* gy, const void* dw, int64_t n, int C, int64_t ldg, 
   else p.mode = kFewDirect;
   // a whole number of stages per block, unless there are too few rows to fill the GPU that way; at least 8 rows, and a
   // multiple of 8, which begins on 16 bytes too
-  const int64_t most = std::max<int64_t>(1, kFewBlocksPerSm * num_sms() / p.slices);
+  const int64_t most = few_most(p.slices);
   int64_t per = (n + most - 1) / most;
   if (per >= 2 * p.batch) per = (per + p.batch - 1) / p.batch * p.batch;
   p.rows_per_block = (per + 7) / 8 * 8;
@@ -1007,9 +1010,9 @@ int few_smem(const FewPlan& p, int V) {
   return std::max(ring, V * kFewThreads * 4 * p.vec);
 }
 
-// the most blocks that few_plan cuts n rows into
 size_t few_bytes(int64_t n, int32_t V, int32_t C) {
-  return sizeof(float) * V * C * static_cast<size_t>(std::min<int64_t>((n + 7) / 8, kFewBlocksPerSm * static_cast<int64_t>(num_sms())));
+  const int slices = ((C + 7) / 8 + kFewThreads - 1) / kFewThreads;
+  return sizeof(float) * V * C * static_cast<size_t>(std::min((n + 7) / 8, few_most(slices)));
 }
 
 WgradPlan wgrad_plan(int64_t n, int32_t V, int32_t C) {

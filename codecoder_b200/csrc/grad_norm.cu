@@ -234,6 +234,7 @@ struct Piece {
 template <typename T, typename U>
 __device__ __forceinline__ void chunk_scale(const T* p, U* q, int len, float by) {
   constexpr int VEC = 16 / (sizeof(T) > sizeof(U) ? sizeof(T) : sizeof(U));
+  constexpr int kUnroll = sizeof(T) * VEC == 16 ? 4 : 8;   // the whole chunk's loads in flight
   const int off = static_cast<int>(((0 - reinterpret_cast<uintptr_t>(q)) & (sizeof(U) * VEC - 1)) / sizeof(U));
   const int peel = off < len ? off : len;                  // elements before the first whole piece of the output
   const int nv = (len - peel) / VEC;
@@ -291,7 +292,7 @@ __global__ void __launch_bounds__(kThreads, kScaleBlocksPerSm) clip_scale_kernel
   double factor = max_norm / (total + 1e-6);
   if (factor > 1.0) factor = 1.0;         // a NaN stays
   const float by = static_cast<float>(factor);
-  const bool tiny = factor < 1.1754944e-38;
+  const bool tiny = factor > 0.0 && factor < 1.1754944e-38;
   for (int k = last; k >= 0; k -= gridDim.x) {
     if (list.first[t] > k) t = find_tensor(list, k, 0, t - 1);
     if (factor == 1.0 && list.in[t] == list.out[t]) continue;         // in place and within the limit: nothing changes
