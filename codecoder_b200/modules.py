@@ -435,10 +435,10 @@ class CascadeNet(nn.Module):
     reference's autocast, its MLP in fp32.
 
     embedding: the stem's lookup embedding(tokens, weight) wherever the embedded stream is written (training, CPU, blocks
-    of other sizes); ops.embedding runs it and its weight gradient on the library's kernels (GPU only): the same
-    values, a gradient that repeats bit for bit."""
+    of other sizes); None: the `embed` module itself.  ops.embedding runs it and its weight gradient on the library's
+    kernels (GPU only): the same values, a gradient that repeats bit for bit."""
 
-    def __init__(self, geo, H, L, det_t, det_typ, det_site, logicals, res="branch", embedding=F.embedding):
+    def __init__(self, geo, H, L, det_t, det_typ, det_site, logicals, res="branch", embedding=None):
         super().__init__()
         self.embedding = embedding
         if H % 4:
@@ -482,6 +482,10 @@ class CascadeNet(nn.Module):
         det = F.pad(det.to(torch.uint8), (0, 1))
         return self.tbase + det[:, self.gidx].long()
 
+    def _embedded(self, det: torch.Tensor) -> torch.Tensor:
+        tok = self.tokens(det)
+        return self.embed(tok) if self.embedding is None else self.embedding(tok, self.embed.weight)
+
     def readout(self, x: torch.Tensor, dt: torch.dtype | None = None) -> torch.Tensor:
         """x = SiLU(bn_out(h)) (B, N, H) -> (B, k): the pooling and scatter GEMMs in dt (x's dtype by default), the
         observables' MLP (k rows per shot, a negligible share of the work) in fp32."""
@@ -492,7 +496,7 @@ class CascadeNet(nn.Module):
 
     def forward(self, det: torch.Tensor) -> torch.Tensor:
         if self.training or not det.is_cuda:
-            h = self.embedding(self.tokens(det), self.embed.weight)
+            h = self._embedded(det)
             for b in self.blocks:
                 h = b(h)
             return self.readout(F.silu(self.bn_out(h.reshape(-1, self.H)).view(h.shape)))
@@ -503,6 +507,6 @@ class CascadeNet(nn.Module):
             tokens = (det.to(torch.uint8).contiguous(), *self._tables, self.embed.weight.float().contiguous())
             _, x = CascadeStack.forward_blocks(self.blocks, None, final=_fold_bn(self.bn_out), tokens=tokens)
         else:
-            h = self.embedding(self.tokens(det), self.embed.weight)
+            h = self._embedded(det)
             _, x = CascadeStack.forward_blocks(self.blocks, h.float().contiguous(), final=_fold_bn(self.bn_out))
         return self.readout(x, torch.bfloat16)

@@ -127,12 +127,12 @@ class PreDecoderNet(nn.Module):
 class Trainer:
     """One process per GPU.  model: PreDecoderNet on `device`; with an initialised process group of world > 1 the
     model is wrapped in DDP (NCCL on GPUs, gloo on CPU).  graph=True (one GPU): step_graphed replays the whole step
-    from a CUDA graph (the optimiser then keeps its step count on the device).  clip_grad: the clipping with torch's
-    signature clip_grad(parameters, max_norm); ops.clip_grad_norm_ runs it on the library's kernels (GPU only): two
+    from a CUDA graph (the optimiser then keeps its step count on the device).  clip_grad: the clipping, with the
+    signature of torch.nn.utils.clip_grad_norm_ (the default); ops.clip_grad_norm_ runs it on the library's kernels (GPU only): two
     launches for the whole list, the norm in 64 bits."""
 
     def __init__(self, model: PreDecoderNet, lr: float = 1e-3, clip: float = 1.0, autocast: bool = True,
-                 graph: bool = False, clip_grad=torch.nn.utils.clip_grad_norm_):
+                 graph: bool = False, clip_grad=None):
         import torch.distributed as dist
         self.model = model
         self.device = next(model.parameters()).device
@@ -166,7 +166,7 @@ class Trainer:
         with ctx:
             loss = self.net(det, err)            # logits and loss (fused on the GPU path)
         loss.backward()
-        self.clip_grad(self.params, self.clip)
+        (self.clip_grad or torch.nn.utils.clip_grad_norm_)(self.params, self.clip)
         self.opt.step()
         return loss.detach()
 

@@ -42,7 +42,7 @@ def test_cascade_net_trains_on_the_embedding_op(golden_dir):
     net(det).square().sum().backward()
     check_wgrad(net.embed.weight.grad, seen["g"], seen["tok"], 5, 1.0, F32)
     # the same network, the default lookup: the same output
-    net.embedding = F.embedding
+    net.embedding = None
     a = net(det)
     net.embedding = ops.embedding
     assert torch.equal(a, net(det))
@@ -148,6 +148,41 @@ def test_few_tokens_over_many_stages_and_far_rows():
     w = gy                                                                    # and a table whose rows are that far apart
     assert torch.equal(ops.embed_lookup(torch.tensor([4, 0, 3, 9], device=DEV)[:3], w), w[[4, 0, 3]])
     assert ops.op_status() == 0
+
+
+def test_outputs_and_inputs_past_32_bits():
+    """More than 2^32 elements on either side: the last rows are as right as the first."""
+    g = torch.Generator(device=DEV).manual_seed(3)
+    w = torch.randn(7, 4001, device=DEV, generator=g).to(BF16)               # an odd width, and a wide one
+    for table in (w, w[:, :4000].contiguous()):
+        ids = torch.randint(-1, 8, (1100000,), device=DEV, generator=g)
+        y = ops.embed_lookup(ids, table)
+        assert y.numel() > 2**32
+        for part in (slice(0, 300), slice(-300, None), slice(1073000, 1074000)):
+            check_lookup(y[part], ids[part], table, 1.0, BF16)
+        del y
+    V, C, n = 1100000, 4000, 400                                              # 17.6 GB of gradient, nearly all zeros
+    ids = torch.randint(0, V, (n,), device=DEV, generator=g)
+    ids[0], ids[1] = V - 1, 0
+    gy = torch.randn(n, C, device=DEV, generator=g)
+    dw = ops.embed_wgrad(gy, ids, V)
+    used = ids.unique()
+    check_wgrad(dw[used], gy, torch.searchsorted(used, ids), len(used), 1.0, F32)
+    assert int(torch.count_nonzero(dw.view(torch.int32).view(-1)[:2**31])) + \
+        int(torch.count_nonzero(dw.view(torch.int32).view(-1)[2**31:])) <= len(used) * C
+    del dw
+    n, C = 47000000, 96                                                       # 4.5 G values: counts of ones are exact
+    gy = torch.ones(n, C, device=DEV, dtype=BF16)
+    ids = torch.randint(0, 4, (n,), device=DEV, generator=g, dtype=torch.int32)
+    for V, t in ((4, ids), (40, ids * 11)):
+        dw = ops.embed_wgrad(gy, t, V)
+        want = torch.bincount(t, minlength=V).double()[:, None]
+        assert bool(((dw.double() - want).abs() <= want * 2.0**-23).all())
+    assert ops.op_status() == 0
+    x = torch.ones(2**32 + 77, device=DEV, dtype=F16)                         # one tensor of more than 2^32 elements
+    assert abs(float(ops.grad_norm([x, x[:5]])) - (2**32 + 82) ** 0.5) <= 65537 * 2.0**-24
+    ops.clip_grads([x], 32768.0)
+    assert bool((x[-100:] == 0.5).all()) and bool((x[:100] == 0.5).all()) and bool((x[2**31 - 50:2**31 + 50] == 0.5).all())
 
 
 def test_two_streams_at_once():
