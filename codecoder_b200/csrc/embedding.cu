@@ -414,7 +414,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(const S* __res
 // tokens without any both spread evenly; every row of dW is written once, the empty ones as zeros.  A token whose rows
 // cross workers: each worker but the one at its end leaves a partial sum in tail[], the last one its own in head[], and
 // wgrad_join_kernel adds them in order.
-//   50,021 tokens, 32,768 rows of 1,024 bf16 into fp32: 86 us in all (floor 41), of which the sort 13, the merge about 58 (3.7
+//   50,021 tokens, 32,768 rows of 1,024 bf16 into fp32: 88 us in all (floor 41), of which the sort 13, the merge about 58 (3.7
 // TB/s, its bytes mostly the zeros of tokens without a row), the join 11.  65,536 rows of 512 over 4,096 tokens: sort 17,
 // merge 23, join 20.
 struct MergeArgs {
@@ -756,7 +756,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 3) wgrad_join_kernel(const __
 // flight depend neither on registers nor on the load units).  The threads of the other eight lie along a row's pieces
 // of VEC channels and several rows; each keeps one sum per token in registers and adds its piece under one predicate per
 // token.  A block adds its threads' sums in order, wgrad_few_join_kernel the blocks' in fp64.
-//   Bound by HBM: 10.8 M rows of 96 bf16 and four tokens take 350 us, 6.0 TB/s (0.92 of a measured copy), with the issue
+//   Bound by HBM: 10.8 M rows of 96 bf16 and four tokens take 350-356 us, 6.0 TB/s (0.91 of a measured copy), with the issue
 // slots 0.72 busy (4 tokens: some 70 instructions per 512 bytes).  Tried and slower at that size: sorting (2,144 us), sums in
 // shared memory indexed by token (609), cp.async rings per thread (427, bound by the load unit), rows listed by token by
 // the ninth warp (427) or by ballots of the adding warps (444).  Eight is the most tokens: groups of eight that read the
