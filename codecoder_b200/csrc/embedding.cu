@@ -544,7 +544,9 @@ __global__ void __launch_bounds__(256) wgrad_merge_kernel(const T* __restrict__ 
   }
   __syncthreads();
   if (w >= a.workers) return;
-  const int i0 = starts[mine].x, i1 = starts[mine + 1].x, j0 = starts[mine].y, j1 = starts[mine + 1].y;
+  const int i0 = starts[mine].x, i1 = starts[mine + 1].x;
+  // rows unsigned: the loop counts up to 2 kRows beyond the last one, and n may be 2^31 - 1
+  const uint32_t j0 = starts[mine].y, j1 = starts[mine + 1].y;
   const int c = (blockIdx.y * S * G + l) * VEC, apart = G * VEC;          // piece q: channels c + q apart ..
   const int pieces = FULL ? S : c < a.C ? min(S, (a.C - c + apart - 1) / apart) : 0;
   bool open = j0 > 0 && i0 < a.V && a.pair[j0 - 1].x == i0;               // token i0 began in an earlier worker
@@ -584,7 +586,7 @@ __global__ void __launch_bounds__(256) wgrad_merge_kernel(const T* __restrict__ 
   int2 ahead = j0 < j1 ? a.pair[j0] : make_int2(a.V, 0);
   const char* const lane_gy = reinterpret_cast<const char*>(gy + c);
   const int64_t row_bytes = a.ldg * static_cast<int64_t>(sizeof(T));
-  const auto copy_row = [&](int u, int j) {
+  const auto copy_row = [&](int u, uint32_t j) {
     if (j < j1) {
       const int2 p = ahead;
       if (j + 1 < j1) ahead = a.pair[j + 1];
@@ -610,7 +612,7 @@ __global__ void __launch_bounds__(256) wgrad_merge_kernel(const T* __restrict__ 
 #pragma unroll
   for (int u = 0; u < kRows - 1; ++u) copy_row(u, j0 + u);
   bool more = true;
-  for (int j = j0; more && j < j1; j += kRows) {
+  for (uint32_t j = j0; more && j < j1; j += kRows) {
 #pragma unroll
     for (int u = 0; u < kRows; ++u) {
       if (!more || j + u >= j1) break;
