@@ -13,6 +13,7 @@
 #include "bpc.h"
 #include "bpc_common.cuh"
 #include "bpc_internal.h"
+#include "ring_phase.h"
 
 namespace bpc {
 
@@ -842,9 +843,11 @@ __global__ void __launch_bounds__(kFewThreads + 32) wgrad_few_kernel(const __gri
   __syncthreads();
   if (warp == kFewThreads / 32) {
     const uint32_t ring = smem_u32(few_smem_base), row_bytes = width * sizeof(T);
+    int issued = 0;
     for (int k = 0; k < copied; ++k) {
       const int q = k % kFewStages;
-      if (k >= kFewStages && !mbar_wait(smem_u32(&empty[q]), (k / kFewStages - 1) & 1, gave_up, a.status, kFewTimeoutNs))
+      if (k >= kFewStages &&
+          !mbar_wait(smem_u32(&empty[q]), ring_parity(k - kFewStages, kFewStages), gave_up, a.status, kFewTimeoutNs))
         break;
       __syncwarp();
       const uint32_t dst = ring + q * batch * p.pitch, bar = smem_u32(&full[q]);
@@ -856,13 +859,15 @@ __global__ void __launch_bounds__(kFewThreads + 32) wgrad_few_kernel(const __gri
       } else {
         for (int r = lane; r < batch; r += 32) bulk_load(dst + r * p.pitch, src + r * a.ldg, row_bytes, bar);
       }
+      issued = k + 1;
     }
     __syncthreads();
     // after a wait that ran out: copies under way still write this block's memory, give them as long again
     if (abort && lane == 0) {
       volatile int never = 0;
-      for (int q = 0; q < kFewStages && q < copied; ++q)
-        mbar_wait(smem_u32(&full[q]), ((copied - 1 - q) / kFewStages) & 1, &never, nullptr, kFewTimeoutNs);
+      for (int q = 0; q < kFewStages && q < issued; ++q)
+        mbar_wait(smem_u32(&full[q]), ring_parity(ring_last_use(issued, q, kFewStages), kFewStages), &never, nullptr,
+                  kFewTimeoutNs);
     }
     __syncthreads();
     return;
