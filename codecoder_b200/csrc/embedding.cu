@@ -846,8 +846,10 @@ __global__ void __launch_bounds__(kFewThreads + 32) wgrad_few_kernel(const __gri
     int issued = 0;
     for (int k = 0; k < copied; ++k) {
       const int q = k % kFewStages;
+      // the warp leaves as a whole: a lane that gave up alone would leave the others at the barriers below
       if (k >= kFewStages &&
-          !mbar_wait(smem_u32(&empty[q]), ring_parity(k - kFewStages, kFewStages), gave_up, a.status, kFewTimeoutNs))
+          !__all_sync(0xffffffffu, mbar_wait(smem_u32(&empty[q]), ring_parity(k - kFewStages, kFewStages), gave_up,
+                                             a.status, kFewTimeoutNs)))
         break;
       __syncwarp();
       const uint32_t dst = ring + q * batch * p.pitch, bar = smem_u32(&full[q]);
@@ -898,7 +900,7 @@ __global__ void __launch_bounds__(kFewThreads + 32) wgrad_few_kernel(const __gri
   if (copied) tokens(0);
   uint32_t q = 0, parity = 0;
   for (int k = 0; k < copied; ++k) {
-    if (!mbar_wait(smem_u32(&full[q]), parity, gave_up, a.status, kFewTimeoutNs)) break;
+    const bool ok = mbar_wait(smem_u32(&full[q]), parity, gave_up, a.status, kFewTimeoutNs);
     const char* at = mine + q * stage_step;
 #pragma unroll
     for (int j = 0; j < kRows; j += kAhead) {
@@ -912,6 +914,7 @@ __global__ void __launch_bounds__(kFewThreads + 32) wgrad_few_kernel(const __gri
       }
     }
     idp += batch;
+    if (!__all_sync(0xffffffffu, ok)) break;               // as a warp: see above
     __syncwarp();
     if (lane == 0) mbar_arrive(smem_u32(&empty[q]));
     if (++q == kFewStages) {

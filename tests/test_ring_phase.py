@@ -40,3 +40,16 @@ def test_the_kernel_drains_what_it_issued():
     drain = src[src.index("after a wait that ran out"):]
     drain = drain[:drain.index("__syncthreads")]
     assert "ring_last_use(issued, q, kFewStages)" in drain and not re.search(r"\bcopied\b", drain)
+
+
+def test_a_warp_leaves_its_loop_as_a_whole():
+    """The kernel's waits: a vote decides for the warp (at once, or on the outcome kept until the end of the stage), or no
+    lane acts on the outcome."""
+    src = open(os.path.join(CSRC, "embedding.cu")).read()
+    waits = [m.start() for m in re.finditer(r"\bmbar_wait\(", src)]
+    assert len(waits) >= 3
+    for at in waits:
+        line = src[src.rindex("\n", 0, at) + 1:at]
+        kept = line.strip() == "const bool ok =" and len(re.findall(r"\bok\b", src[at:])) == 1 and \
+            "if (!__all_sync(0xffffffffu, ok)) break;" in src[at:]
+        assert line.endswith("__all_sync(0xffffffffu, ") or not line.strip() or kept, src[at - 80:at + 40]
