@@ -108,7 +108,7 @@ Tensor embed_lookup(const Tensor& ids_in, const Tensor& weight_in, double scale,
   if (y.numel() == 0) return y;
   TORCH_CHECK_VALUE(weight.size(0) <= 0x7ffffffe && weight.size(1) <= (1 << 20), "embed_lookup: weight is too large");
   const int64_t ld = row_stride(weight);
-  check(entry.embed_lookup(ids.data_ptr(), id_bytes, weight.data_ptr(), y.data_ptr(), ids.numel(),
+  check(entry.embed_lookup(ids.const_data_ptr(), id_bytes, weight.const_data_ptr(), y.data_ptr(), ids.numel(),
                            static_cast<int32_t>(weight.size(0)), static_cast<int32_t>(weight.size(1)), ld,
                            static_cast<float>(scale), dtype_code(weight.scalar_type()), dtype_code(out), stream_of(weight)),
         "bpc_embed_lookup");
@@ -131,7 +131,7 @@ Tensor embed_wgrad(const Tensor& gy_in, const Tensor& ids_in, int64_t n_tokens, 
   const int64_t ld = row_stride(gy);
   const int32_t V = static_cast<int32_t>(n_tokens), Ci = static_cast<int32_t>(C);
   Tensor ws = empty({static_cast<int64_t>(entry.embed_wgrad_workspace_size(n, V, Ci))}, at::kByte, gy);
-  check(entry.embed_wgrad(gy.data_ptr(), ids.data_ptr(), id_bytes, dw.data_ptr(), ws.data_ptr(), ws.numel(), n, V, Ci,
+  check(entry.embed_wgrad(gy.const_data_ptr(), ids.const_data_ptr(), id_bytes, dw.data_ptr(), ws.data_ptr(), ws.numel(), n, V, Ci,
                           ld, static_cast<float>(scale), dtype_code(gy.scalar_type()), dtype_code(dtype), stream_of(gy)),
         "bpc_embed_wgrad");
   return dw;
@@ -170,11 +170,19 @@ TensorArrays arrays_of(const py::list& list, const char* what) {
                      t.layout(), " ", t.scalar_type());
     TORCH_CHECK_VALUE(t.is_non_overlapping_and_dense(), what,
                       ": a tensor with gaps or overlaps between its elements (strides ", t.strides(), ")");
-    a.at[k] = const_cast<void*>(t.const_data_ptr());
     a.numel[k] = t.numel();
     a.dtype[k] = code;
   }
   return a;
+}
+
+// The addresses of tensors that are read, or written.  One that is to be written and shares its memory until then (copy on
+// write) gets its own here, so the written ones come first: what is read is then where it stays.
+void take_addresses(TensorArrays& a, const py::list& list, bool written) {
+  for (size_t k = 0; k < a.at.size(); ++k) {
+    const Tensor& t = THPVariable_Unpack(PyList_GET_ITEM(list.ptr(), static_cast<Py_ssize_t>(k)));
+    a.at[k] = written ? t.mutable_data_ptr() : const_cast<void*>(t.const_data_ptr());
+  }
 }
 
 Tensor norm_workspace(const Tensor& like, size_t n) {
@@ -182,9 +190,10 @@ Tensor norm_workspace(const Tensor& like, size_t n) {
 }
 
 Tensor grad_norm(const py::list& ts) {
-  const TensorArrays a = arrays_of(ts, "grad_norm");
+  TensorArrays a = arrays_of(ts, "grad_norm");
   const Tensor& first = tensor_at(ts, 0, "grad_norm");
   const c10::cuda::CUDAGuard guard(first.device());
+  take_addresses(a, ts, false);
   Tensor norm = empty({}, at::kFloat, first), ws = norm_workspace(first, a.at.size());
   check(entry.grad_norm(a.at.data(), a.numel.data(), a.dtype.data(), static_cast<int32_t>(a.at.size()),
                         static_cast<float*>(norm.data_ptr()), ws.data_ptr(), ws.numel(), stream_of(first)),
@@ -193,7 +202,7 @@ Tensor grad_norm(const py::list& ts) {
 }
 
 Tensor clip_grads(const py::list& ts, double max_norm, const std::optional<py::list>& out) {
-  const TensorArrays a = arrays_of(ts, "clip_grads");
+  TensorArrays a = arrays_of(ts, "clip_grads");
   const py::list& outs = out ? *out : ts;
   const Tensor& first = tensor_at(ts, 0, "clip_grads");
   TensorArrays other;
@@ -209,8 +218,10 @@ Tensor clip_grads(const py::list& ts, double max_norm, const std::optional<py::l
                         "clip_grads: out must have the gradients' strides");
     }
   }
-  const TensorArrays& b = out ? other : a;
+  TensorArrays& b = out ? other : a;
   const c10::cuda::CUDAGuard guard(first.device());
+  take_addresses(b, outs, true);
+  if (out) take_addresses(a, ts, false);
   Tensor norm = empty({}, at::kFloat, first), ws = norm_workspace(first, a.at.size());
   check(entry.clip_grads(a.at.data(), b.at.data(), a.numel.data(), a.dtype.data(), b.dtype.data(),
                          static_cast<int32_t>(a.at.size()), max_norm, static_cast<float*>(norm.data_ptr()), ws.data_ptr(),
