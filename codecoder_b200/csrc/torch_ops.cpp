@@ -101,7 +101,7 @@ Tensor embed_lookup(const Tensor& ids_in, const Tensor& weight_in, double scale,
   const int32_t id_bytes = check_embedding(ids_in, weight_in, out);
   TORCH_CHECK_VALUE(weight_in.dim() == 2, "embed_lookup: weight must be (V, C)");
   const c10::cuda::CUDAGuard guard(weight_in.device());
-  Tensor weight = weight_in, ids = ids_in.contiguous();
+  Tensor weight = weight_in.resolve_neg(), ids = ids_in.contiguous();      // resolve_neg: a lazily negated view is copied
   std::vector<int64_t> shape(ids.sizes().begin(), ids.sizes().end());
   shape.push_back(weight.size(1));
   Tensor y = empty(shape, out, weight);
@@ -127,7 +127,7 @@ Tensor embed_wgrad(const Tensor& gy_in, const Tensor& ids_in, int64_t n_tokens, 
   const c10::cuda::CUDAGuard guard(gy_in.device());
   Tensor dw = empty({n_tokens, C}, dtype, gy_in);
   if (C == 0) return dw;
-  Tensor ids = ids_in.contiguous(), gy = gy_in.reshape({n, C});
+  Tensor ids = ids_in.contiguous(), gy = gy_in.resolve_neg().reshape({n, C});
   const int64_t ld = row_stride(gy);
   const int32_t V = static_cast<int32_t>(n_tokens), Ci = static_cast<int32_t>(C);
   Tensor ws = empty({static_cast<int64_t>(entry.embed_wgrad_workspace_size(n, V, Ci))}, at::kByte, gy);
@@ -216,6 +216,7 @@ Tensor clip_grads(const py::list& ts, double max_norm, const std::optional<py::l
       TORCH_CHECK_VALUE(o.sizes() == t.sizes(), "clip_grads: out must hold one tensor of the same shape per gradient");
       TORCH_CHECK_VALUE((o.is_contiguous() && t.is_contiguous()) || o.strides() == t.strides(),
                         "clip_grads: out must have the gradients' strides");
+      TORCH_CHECK_VALUE(o.is_neg() == t.is_neg(), "clip_grads: a lazily negated view into one that is not, or the reverse");
     }
   }
   TensorArrays& b = out ? other : a;

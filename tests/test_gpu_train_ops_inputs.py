@@ -40,3 +40,27 @@ def test_reading_a_lazy_copy_makes_no_copy():
         want = f(w, ids, gy)
         assert torch.equal(f(*lazy), want)
         assert all(torch._C._is_cow_tensor(t) for t in lazy)
+
+
+def test_lazily_negated_views():
+    """The imaginary part of a conjugate is a view whose values are the negative of its memory."""
+    z = torch.randn(40, 1, device=DEV, dtype=torch.complex64).conj()
+    w = z.imag                                                  # one channel: no layout asks for a copy
+    ids = torch.randint(0, 40, (200,), device=DEV)
+    assert w.is_neg() and torch.equal(ops.embed_lookup(ids, w), w.resolve_neg()[ids])
+    gy = torch._neg_view(torch.randint(-3, 4, (200, 8), device=DEV).float())
+    for V in (5, 40):
+        want = torch.zeros(V, 8, device=DEV).index_add_(0, ids % V, gy.resolve_neg())
+        assert torch.equal(ops.embed_wgrad(gy, ids % V, V), want)
+    x = torch.randn(300, device=DEV)
+    keep, neg = x.clone(), torch._neg_view(x)
+    n = ops.grad_norm([neg])
+    assert torch.equal(n, ops.grad_norm([x]))
+    with pytest.raises(ValueError, match="negated"):
+        ops.clip_grads([neg], 0.5, out=[torch.empty_like(x)])
+    with pytest.raises(ValueError, match="negated"):
+        ops.clip_grads([keep], 0.5, out=[neg])
+    assert torch.equal(x, keep)
+    assert torch.equal(ops.clip_grads([neg], 0.5), n)           # in place: both sides of the view are scaled
+    coef = 0.5 / float(n)
+    assert float((neg - -keep * coef).abs().max()) < 1e-6 and float((x - keep * coef).abs().max()) < 1e-6
