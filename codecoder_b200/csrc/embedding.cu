@@ -6,7 +6,12 @@
 // The products and sums are fp32 and rounded once to the output's type.  The gradient is deterministic: the positions
 // are sorted stably by token (least-significant-digit radix sort), and the sorted rows are summed in that order.
 #include <algorithm>
+#include <cstdlib>
+#include <cstring>
+#include <map>
+#include <mutex>
 #include <string>
+#include <utility>
 
 #include <cuda_fp16.h>
 
@@ -1125,13 +1130,30 @@ int sort_pass(const S* src, int64_t n, int V, int shift, int tiles, int* counts,
   return launched("sort_place_kernel");
 }
 
+// Whether the kernel's cluster can be resident on the current device (a partition of a GPU may have no room for 16 CTAs);
+// asked once per device and kernel.
+bool cluster_fits(const void* fn, const cudaLaunchConfig_t& lc) {
+  static std::mutex mu;
+  static std::map<std::pair<int, const void*>, bool> known;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  std::lock_guard<std::mutex> lk(mu);
+  const auto it = known.find({dev, fn});
+  if (it != known.end()) return it->second;
+  int clusters = 0;
+  cudaError_t e = cudaSuccess;
+  if (lc.gridDim.x > 8) e = cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(&clusters, fn, &lc);
+  if (e != cudaSuccess) cudaGetLastError();
+  return known[{dev, fn}] = e == cudaSuccess && clusters > 0;
+}
+
+// *launched: whether the cluster can be resident here and was launched
 template <typename I, int CTAS, int ROUNDS>
-int sort_cluster_rounds(const I* ids, int n, int V, int passes, int2* out, cudaStream_t s) {
+int sort_cluster_rounds(const I* ids, int n, int V, int passes, int2* out, bool* launched, cudaStream_t s) {
   const auto fn = sort_cluster_kernel<I, CTAS, ROUNDS>;
   const int smem = 2 * ROUNDS * kClusterThreads * static_cast<int>(sizeof(int2));
   if (int e = allow_smem(reinterpret_cast<const void*>(fn), smem)) return e;
-  cudaError_t e = cudaSuccess;
-  if (CTAS > 8) e = cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   cudaLaunchConfig_t lc = {};
   lc.gridDim = dim3(CTAS);
   lc.blockDim = dim3(kClusterThreads);
@@ -1143,24 +1165,31 @@ int sort_cluster_rounds(const I* ids, int n, int V, int passes, int2* out, cudaS
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   lc.attrs = &attr;
   lc.numAttrs = 1;
-  if (e == cudaSuccess) e = cudaLaunchKernelEx(&lc, fn, ids, n, V, passes, out);
+  *launched = cluster_fits(reinterpret_cast<const void*>(fn), lc);
+  if (!*launched) return 0;
+  const cudaError_t e = cudaLaunchKernelEx(&lc, fn, ids, n, V, passes, out);
   return e == cudaSuccess ? 0 : fail(BPC_ERR_LAUNCH, std::string("sort_cluster_kernel launch: ") + cudaGetErrorString(e));
 }
 
 template <typename I>
-int sort_cluster(const I* ids, int n, int V, int passes, int2* out, cudaStream_t s) {
-  if (n <= 8 * kClusterThreads) return sort_cluster_rounds<I, 8, 1>(ids, n, V, passes, out, s);
-  if (n <= 16 * kClusterThreads) return sort_cluster_rounds<I, 16, 1>(ids, n, V, passes, out, s);
-  if (n <= 32 * kClusterThreads) return sort_cluster_rounds<I, 16, 2>(ids, n, V, passes, out, s);
-  return sort_cluster_rounds<I, 16, 4>(ids, n, V, passes, out, s);
+int sort_cluster(const I* ids, int n, int V, int passes, int2* out, bool* launched, cudaStream_t s) {
+  if (n <= 8 * kClusterThreads) return sort_cluster_rounds<I, 8, 1>(ids, n, V, passes, out, launched, s);
+  if (n <= 16 * kClusterThreads) return sort_cluster_rounds<I, 16, 1>(ids, n, V, passes, out, launched, s);
+  if (n <= 32 * kClusterThreads) return sort_cluster_rounds<I, 16, 2>(ids, n, V, passes, out, launched, s);
+  return sort_cluster_rounds<I, 16, 4>(ids, n, V, passes, out, launched, s);
 }
 
-// *sorted: where the pairs are
+// *sorted: where the pairs are.  BPC_EMBED_SORT=passes selects the launches per pass for every size (the same pairs).
 template <typename I>
 int sort_ids(const I* ids, int64_t n, int V, const WgradPlan& p, int2* const (&pair)[2], int* counts, int* totals,
              const int2** sorted, cudaStream_t s) {
   *sorted = pair[0];
-  if (n <= kClusterKeys) return sort_cluster(ids, static_cast<int>(n), V, p.passes, pair[0], s);
+  const char* how = std::getenv("BPC_EMBED_SORT");
+  if (n <= kClusterKeys && !(how && std::strcmp(how, "passes") == 0)) {
+    bool launched = false;
+    const int e = sort_cluster(ids, static_cast<int>(n), V, p.passes, pair[0], &launched, s);
+    if (e || launched) return e;
+  }
   if (int e = sort_pass(ids, n, V, 0, p.tiles, counts, totals, pair[0], s)) return e;
   for (int k = 1; k < p.passes; ++k) {
     if (int e = sort_pass(*sorted, n, V, k * kDigitBits, p.tiles, counts, totals, pair[k & 1], s)) return e;
