@@ -552,9 +552,10 @@ __global__ void __launch_bounds__(256) wgrad_merge_kernel(const T* __restrict__ 
   if (w >= a.workers) return;
   const int i0 = starts[mine].x, i1 = starts[mine + 1].x;
   const int j0 = starts[mine].y, j1 = starts[mine + 1].y;
-  const int2* const pair = a.pair + j0;                    // of this worker's rows
-  // their places are unsigned: the loop counts up to 2 kRows beyond the last one, and n may be 2^31 - 1
-  const uint32_t rows = j1 - j0;
+  // the rows from the loop's place on, and how many are left: a place counted up to 2 kRows beyond the last one would not
+  // fit 31 bits where n is 2^31 - 1
+  const int2* next = a.pair + j0;
+  int left = j1 - j0;
   const int c = (blockIdx.y * S * G + l) * VEC, apart = G * VEC;          // piece q: channels c + q apart ..
   const int pieces = FULL ? S : c < a.C ? min(S, (a.C - c + apart - 1) / apart) : 0;
   bool open = j0 > 0 && i0 < a.V && a.pair[j0 - 1].x == i0;               // token i0 began in an earlier worker
@@ -590,14 +591,14 @@ __global__ void __launch_bounds__(256) wgrad_merge_kernel(const T* __restrict__ 
     }
     tok = t;
   };
-  // the worker's row j into slot u; the pair of the row after it is read one call ahead
-  int2 ahead = rows ? pair[0] : make_int2(a.V, 0);
+  // row j from the loop's place on into slot u; the pair of the row after it is read one call ahead
+  int2 ahead = left > 0 ? next[0] : make_int2(a.V, 0);
   const char* const lane_gy = reinterpret_cast<const char*>(gy + c);
   const int64_t row_bytes = a.ldg * static_cast<int64_t>(sizeof(T));
-  const auto copy_row = [&](int u, uint32_t j) {
-    if (j < rows) {
+  const auto copy_row = [&](int u, int j) {
+    if (j < left) {
       const int2 p = ahead;
-      if (j + 1 < rows) ahead = pair[j + 1];
+      if (j + 1 < left) ahead = next[j + 1];
       tokens[u * 256] = p.x;
       if (p.x < a.V) {                                     // V: a position without a token
         const char* row = lane_gy + p.y * row_bytes;
@@ -620,11 +621,11 @@ __global__ void __launch_bounds__(256) wgrad_merge_kernel(const T* __restrict__ 
 #pragma unroll
   for (int u = 0; u < kRows - 1; ++u) copy_row(u, u);
   bool more = true;
-  for (uint32_t j = 0; more && j < rows; j += kRows) {
+  for (; more && left > 0; left -= kRows, next += kRows) {
 #pragma unroll
     for (int u = 0; u < kRows; ++u) {
-      if (!more || j + u >= rows) break;
-      copy_row((u + kRows - 1) % kRows, j + u + kRows - 1);               // into the slot that the step before read
+      if (!more || u >= left) break;
+      copy_row((u + kRows - 1) % kRows, u + kRows - 1);   // into the slot that the step before read
       asm volatile("cp.async.wait_group %0;" ::"n"(kRows - 1) : "memory");
       const int t = tokens[u * 256];
       if (t >= a.V) {                                      // the ones without a token are the last
