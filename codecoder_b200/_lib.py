@@ -122,7 +122,8 @@ def torch_ops():
     if _torch is None:
         path = os.path.join(_PKG, "_torch_ops.so")
         if not os.path.exists(path):
-            raise RuntimeError(f"{path} is missing: build it with `python -m codecoder_b200.build`")
+            raise RuntimeError(f"{path} is missing: build it with `python -m codecoder_b200.build`, which needs torch's "
+                               "C++ and CUDA headers")
         import importlib.util
 
         import torch  # noqa: F401  (its libraries must be loaded first)

@@ -57,6 +57,21 @@ def _run(cmd: list[str], what: str) -> str:
     return r.stderr
 
 
+def torch_ops_lack() -> str | None:
+    """What this machine lacks to compile csrc/torch_ops.cpp, or None."""
+    import sysconfig
+    try:
+        import torch
+    except ImportError:
+        return "torch cannot be imported"
+    root = os.path.dirname(os.path.abspath(torch.__file__))
+    for path in (os.path.join(root, "include", "c10", "cuda", "CUDAGuard.h"), os.path.join(root, "lib", "libc10_cuda.so"),
+                 os.path.join(sysconfig.get_paths()["include"], "Python.h")):
+        if not os.path.exists(path):
+            return f"{path} is missing"
+    return None
+
+
 def build_torch_ops() -> str:
     """Compile csrc/torch_ops.cpp against the headers and libraries of the installed torch: with g++, the compiler nvcc
     uses, whatever $CXX says (another one may bring its own C++ runtime into the process)."""
@@ -99,8 +114,14 @@ def build_lib(verbose: bool = False) -> str:
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
+    """Both libraries, where they are older than their sources; libbpc.so alone where there is no torch to compile against
+    (a C caller's machine: _lib.torch_ops() says then what is missing)."""
+    wanted = force or _older(TORCH_OUT, [TORCH_SRC, _header()])
+    lack = torch_ops_lack() if wanted else None
+    if lack:
+        sys.stderr.write(f"{os.path.basename(TORCH_OUT)} is not built: {lack}\n")
     with cf.ThreadPoolExecutor(max_workers=1) as ex:
-        host = ex.submit(build_torch_ops) if force or _older(TORCH_OUT, [TORCH_SRC, _header()]) else None
+        host = ex.submit(build_torch_ops) if wanted and not lack else None
         if force or _needs_build():
             build_lib(verbose)
         if host is not None:
