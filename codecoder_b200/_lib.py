@@ -127,6 +127,11 @@ def torch_ops():
         import importlib.util
 
         import torch  # noqa: F401  (its libraries must be loaded first)
+
+        from .build import stamp_of, torch_stamp
+        if stamp_of(path) != torch_stamp():
+            raise RuntimeError(f"{path} was built for {stamp_of(path)}, and this is {torch_stamp()}: run "
+                               "`python -m codecoder_b200.build`")
         spec = importlib.util.spec_from_file_location("_torch_ops", path)
         m = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(m)

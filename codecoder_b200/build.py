@@ -72,6 +72,26 @@ def torch_ops_lack() -> str | None:
     return None
 
 
+STAMP = b"torch_ops built for ["
+
+
+def torch_stamp() -> str:
+    """What a build of csrc/torch_ops.cpp depends on besides its sources: torch's C++ layout and Python's ABI."""
+    import sysconfig
+
+    import torch
+    return (f"torch {torch.__version__}, CUDA {torch.version.cuda}, C++11 ABI {int(torch._C._GLIBCXX_USE_CXX11_ABI)}, "
+            f"Python {sysconfig.get_config_var('SOABI')}")
+
+
+def stamp_of(path: str) -> str | None:
+    """The stamp that the built module carries, or None."""
+    with open(path, "rb") as f:
+        data = f.read()
+    at = data.find(STAMP)
+    return None if at < 0 else data[at + len(STAMP):data.index(b"]", at)].decode()
+
+
 def build_torch_ops() -> str:
     """Compile csrc/torch_ops.cpp against the headers and libraries of the installed torch: with g++, the compiler nvcc
     uses, whatever $CXX says (another one may bring its own C++ runtime into the process)."""
@@ -84,7 +104,7 @@ def build_torch_ops() -> str:
            os.path.join(REPO, "include")]
     tmp = TORCH_OUT + ".tmp"
     _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-          "-DTORCH_EXTENSION_NAME=_torch_ops", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+          "-DTORCH_EXTENSION_NAME=_torch_ops", f'-DBUILT_FOR="{torch_stamp()}"', f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
           *[f"-isystem{d}" for d in inc], TORCH_SRC, "-o", tmp, "-L", os.path.join(root, "lib"), "-lc10", "-lc10_cuda",
           "-ltorch_cpu", "-ltorch_python"], f"g++ on {TORCH_SRC}")
     os.replace(tmp, TORCH_OUT)
@@ -117,7 +137,9 @@ def build(force: bool = False, verbose: bool = False) -> str:
     """Both libraries, where they are older than their sources; libbpc.so alone where there is no torch to compile against
     (a C caller's machine: _lib.torch_ops() says then what is missing)."""
     wanted = force or _older(TORCH_OUT, [TORCH_SRC, _header()])
-    lack = torch_ops_lack() if wanted else None
+    lack = torch_ops_lack()
+    wanted = wanted or not lack and stamp_of(TORCH_OUT) != torch_stamp()
+    lack = lack if wanted else None
     if lack:
         sys.stderr.write(f"{os.path.basename(TORCH_OUT)} is not built: {lack}\n")
     with cf.ThreadPoolExecutor(max_workers=1) as ex:

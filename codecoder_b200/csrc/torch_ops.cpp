@@ -237,6 +237,9 @@ Tensor clip_grads(const py::list& ts, double max_norm, const std::optional<py::l
 
 }  // namespace
 
+// What the build reads back, to compile again for another torch or Python, and to refuse loading there until then
+__attribute__((used)) const char built_for[] = "torch_ops built for [" BUILT_FOR "]";
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("bind", &bind);
   const auto release = py::call_guard<py::gil_scoped_release>();

@@ -53,3 +53,35 @@ def test_the_torch_side_says_that_it_is_missing(monkeypatch, tmp_path):
     monkeypatch.setattr(_lib, "_PKG", str(tmp_path))
     with pytest.raises(RuntimeError, match="missing.*headers"):
         _lib.torch_ops()
+
+
+def test_another_torch_gets_another_build(elsewhere, monkeypatch):
+    calls, write, tmp_path = elsewhere
+    out = tmp_path / "_torch_ops.so"
+
+    def compile_():
+        calls.append("_torch_ops.so")
+        out.write_bytes(b"code" + build.STAMP + build.torch_stamp().encode() + b"]more code")
+    monkeypatch.setattr(build, "build_torch_ops", compile_)
+    build.build()
+    build.build()
+    assert sorted(calls) == ["_torch_ops.so", "libbpc.so"]      # the second call found both in order
+    import torch
+    monkeypatch.setattr(torch, "__version__", "9.9.9")
+    build.build()
+    assert calls.count("_torch_ops.so") == 2 and "torch 9.9.9" in build.stamp_of(str(out))
+    build.build()
+    assert calls.count("_torch_ops.so") == 2
+    out.write_bytes(b"a module from before the stamp")
+    build.build()
+    assert calls.count("_torch_ops.so") == 3
+
+
+def test_the_built_module_is_refused_under_another_torch(monkeypatch):
+    import torch
+    build.build()
+    assert build.stamp_of(build.TORCH_OUT) == build.torch_stamp()
+    monkeypatch.setattr(_lib, "_torch", None)
+    monkeypatch.setattr(torch, "__version__", "9.9.9")
+    with pytest.raises(RuntimeError, match="built for torch .*9.9.9"):
+        _lib.torch_ops()
