@@ -174,6 +174,20 @@ def test_refusals():
     check_norm(ops.grad_norm([x, x]), math.sqrt(2.0) * norm64([x]))       # the norm alone may read a tensor twice
 
 
+def test_refused_clips_change_nothing():
+    x = torch.randn(40, 50, device=DEV)
+    keep, out = x.clone(), torch.full((40, 50), 7.0, device=DEV)
+    for ts, limit, outs in (([x, x], 1.0, None), ([x, x[3]], 1.0, None), ([x], -1.0, None), ([x], float("nan"), None),
+                            ([x, x.double()], 1.0, None), ([x, x[:, :20]], 1.0, None), ([x], 1.0, [x[:, :1].expand(40, 50)]),
+                            ([x], 1.0, []), ([x], 1.0, [out.view(-1)]), ([x], 1.0, [torch.empty(50, 40, device=DEV).t()]),
+                            ([x, keep], 1.0, [out, out]), ([x, keep], 1.0, [keep, out])):
+        before = keep.clone()
+        with pytest.raises((ValueError, TypeError, RuntimeError)):
+            ops.clip_grads(ts, limit, out=outs)
+        torch.cuda.synchronize()
+        assert torch.equal(x, before) and torch.equal(keep, before) and bool((out == 7).all())
+
+
 def test_autograd_notices_clipping_in_place():
     w = torch.randn(10, device=DEV, requires_grad=True)
     x = torch.randn(10, device=DEV)

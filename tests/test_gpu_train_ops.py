@@ -63,6 +63,23 @@ def test_unfused_predecoder_net_takes_the_embedding_op():
     assert float((out[0][1] - out[1][1]).abs().max()) <= 2 * 769 * 2.0**-24 * 768 * float(out[0][1].abs().max())
 
 
+def test_unfused_predecoder_nets_embedding_gradient_is_its_streams_sum():
+    """The table's gradient against the sum by token of the stream's own gradient: at most 768 rows of one token."""
+    cfg = replace(CONFIGS["d5_fp32"], d=3, rounds=3, layers=2)
+    g = RotatedSurface(cfg.d, cfg.rounds)
+    det, err = sample_torch(g, 0.05, 32, 7, device=DEV)
+    seen = {}
+
+    def lookup(tok, weight):
+        h = ops.embedding(tok, weight)
+        h.register_hook(lambda gh: seen.update(tok=tok, g=gh.detach().clone()))
+        return h
+
+    net = PreDecoderNet(g, cfg, init_params(cfg, 5), embedding=lookup).to(DEV)
+    net(det, err).backward()
+    check_wgrad(net.embed.grad, seen["g"], seen["tok"], net.embed.shape[0], 1.0, F32)
+
+
 def test_trainer_clips_with_the_library():
     """Trainer(clip_grad=ops.clip_grad_norm_): eager and graphed steps give the same bits, and one step's update is that
     of torch's clipping to rounding (Adam's first step is lr times the gradient's sign where it is not tiny)."""
