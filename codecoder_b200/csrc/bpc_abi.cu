@@ -219,7 +219,8 @@ extern "C" int bpc_gather_mm_status(bpc_stream_t stream, int* status) {
   if (v != 0) {
     const int zero = 0;
     cudaMemcpy(p, &zero, sizeof(int), cudaMemcpyHostToDevice);
-    return fail(BPC_ERR_DEVICE, "a gather_mm kernel watchdog fired (status " + std::to_string(v) + ")");
+    return fail(BPC_ERR_DEVICE, "the watchdog of a gather_mm, Cascade block or embedding gradient kernel fired (status " +
+                                    std::to_string(v) + ")");
   }
   return 0;
 }

@@ -3,8 +3,10 @@
 //   lookup    y[i, :] = scale W[ids[i], :]                              (a zero row where ids[i] is outside [0, V))
 //   gradient  dW[v, :] = scale sum over i with ids[i] = v of gy[i, :]   (ids outside [0, V) contribute nothing)
 //
-// The products and sums are fp32 and rounded once to the output's type.  The gradient is deterministic: the positions
-// are sorted stably by token (least-significant-digit radix sort), and the sorted rows are summed in that order.
+// The products and sums are fp32 and rounded once to the output's type.  The gradient is deterministic.  More than 8 tokens:
+// the positions are sorted stably by token (least-significant-digit radix sort), and the sorted rows are summed in that
+// order.  Up to 8: every block has a fixed share of the rows, each thread adds its own in order, and the threads' and the
+// blocks' sums are added in a fixed order.
 #include <algorithm>
 #include <cstdlib>
 #include <cstring>
@@ -420,9 +422,9 @@ __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(const S* __res
 // tokens without any both spread evenly; every row of dW is written once, the empty ones as zeros.  A token whose rows
 // cross workers: each worker but the one at its end leaves a partial sum in tail[], the last one its own in head[], and
 // wgrad_join_kernel adds them in order.
-//   50,021 tokens, 32,768 rows of 1,024 bf16 into fp32: 88 us in all (floor 41), of which the sort 13, the merge about 58 (3.7
-// TB/s, its bytes mostly the zeros of tokens without a row), the join 11.  65,536 rows of 512 over 4,096 tokens: sort 17,
-// merge 23, join 20.
+//   50,021 tokens, 32,768 rows of 1,024 bf16 into fp32: 87 us in all (floor 41), of which the sort 13, the merge about 58 (269
+// MB, 4.6 TB/s, mostly the zeros of tokens without a row; 3.7 TB/s of it reach HBM), the join 11.  65,536 rows of 512 over
+// 4,096 tokens: sort 17, merge 23, join 20.
 struct MergeArgs {
   const int2* pair;    // (n,) {token, row}, sorted by token
   int64_t n, items, workers;
@@ -438,7 +440,7 @@ struct MergeArgs {
 
 // The tokens finished within the first d steps of the path, by the G lanes of a worker together: each step of the search
 // probes G places.
-__device__ __forceinline__ int64_t path_search(const MergeArgs& a, int64_t d, int G, int l, unsigned mask, int shift) {
+__device__ __forceinline__ int64_t path_search(const MergeArgs& a, int64_t d, int G, int l, unsigned mask) {
   int64_t lo = d > a.n ? d - a.n : 0, hi = d < a.V ? d : a.V;            // lo holds: every row consumed
   while (lo < hi) {
     const int64_t step = (hi - lo + G) / (G + 1), at = lo + (l + 1) * step;
@@ -454,8 +456,8 @@ __device__ __forceinline__ int64_t path_search(const MergeArgs& a, int64_t d, in
 
 // Where a worker starts: {tokens finished, rows consumed} after d steps, or, inside a token that ends within `items` rows,
 // after that token: the worker before takes the whole of it, so that only the longer tokens are ever cut.
-__device__ __forceinline__ int2 path_start(const MergeArgs& a, int64_t d, int G, int l, unsigned mask, int shift) {
-  const int64_t i = path_search(a, d, G, l, mask, shift), j = d - i;
+__device__ __forceinline__ int2 path_start(const MergeArgs& a, int64_t d, int G, int l, unsigned mask) {
+  const int64_t i = path_search(a, d, G, l, mask), j = d - i;
   if (i < a.V && j > 0 && a.pair[j - 1].x == i) {
     int64_t lo = j, hi = a.n < j + a.items ? a.n : j + a.items;
     if (hi == a.n || a.pair[hi].x != i) {
@@ -541,10 +543,10 @@ __global__ void __launch_bounds__(256) wgrad_merge_kernel(const T* __restrict__ 
   pdl_launch_dependents();
   pdl_wait();
   {
-    const int2 at = path_start(a, d0, G, l, mask, shift);
+    const int2 at = path_start(a, d0, G, l, mask);
     if (l == 0) starts[mine] = at;
     if (mine == per_block - 1) {
-      const int2 e = path_start(a, d1, G, l, mask, shift);
+      const int2 e = path_start(a, d1, G, l, mask);
       if (l == 0) starts[per_block] = e;
     }
   }
@@ -690,18 +692,17 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 3) wgrad_join_kernel(const __
     store_row<VEC>(a.dw, a.dw_dtype, t * a.C + c, f, a.scale);
   };
   // a warp looks at kJoinRun workers at once; few of them end a token that was cut
-  constexpr int kRun = kJoinRun;
-  const int64_t runs = (a.workers + kRun - 1) / kRun;
+  const int64_t runs = (a.workers + kJoinRun - 1) / kJoinRun;
   for (int64_t base = static_cast<int64_t>(blockIdx.x) * kJoinWarps; base < runs;
        base += static_cast<int64_t>(gridDim.x) * kJoinWarps) {
-    const int64_t mine = (base + warp) * kRun + lane;
-    const int token = lane < kRun && mine < a.workers ? a.ends[mine].x : -1;
+    const int64_t mine = (base + warp) * kJoinRun + lane;
+    const int token = lane < kJoinRun && mine < a.workers ? a.ends[mine].x : -1;
     unsigned cut = __ballot_sync(0xffffffffu, token >= 0);
     int longs = 0;
     while (cut) {
       const int at_lane = __ffs(cut) - 1;
       cut &= cut - 1;
-      const int64_t w = (base + warp) * kRun + at_lane, t = __shfl_sync(0xffffffffu, token, at_lane);
+      const int64_t w = (base + warp) * kJoinRun + at_lane, t = __shfl_sync(0xffffffffu, token, at_lane);
       // the nearest worker before w whose tail's token begins in it, 128 at a time: the first of token t
       int64_t first = 0;
       for (int64_t top = w - 1; top >= 0; top -= 128) {
@@ -737,10 +738,10 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 3) wgrad_join_kernel(const __
     }
     if (lane == 0) tasks[warp] = longs;
     if (!__syncthreads_or(longs)) continue;
-    for (int k = 0; k < kJoinWarps * kRun; ++k) {
-      if (k % kRun >= tasks[k / kRun]) continue;
-      const int64_t v1 = task_worker[k / kRun][k % kRun], v0 = task_first[k / kRun][k % kRun];
-      const int64_t t = task_token[k / kRun][k % kRun];
+    for (int k = 0; k < kJoinWarps * kJoinRun; ++k) {
+      const int from = k / kJoinRun, task = k % kJoinRun;
+      if (task >= tasks[from]) continue;
+      const int64_t v1 = task_worker[from][task], v0 = task_first[from][task], t = task_token[from][task];
       for (int c0 = c_from; c0 < c_to; c0 += 32 * VEC) {
         const int c = c0 + lane * VEC;
         double s[VEC] = {};
@@ -767,7 +768,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 3) wgrad_join_kernel(const __
 // flight depend neither on registers nor on the load units).  The threads of the other eight lie along a row's pieces
 // of VEC channels and several rows; each keeps one sum per token in registers and adds its piece under one predicate per
 // token.  A block adds its threads' sums in order, wgrad_few_join_kernel the blocks' in fp64.
-//   Bound by HBM: 10.8 M rows of 96 bf16 and four tokens take 350-356 us, 6.0 TB/s (0.91 of a measured copy), with the issue
+//   Bound by HBM: 10.8 M rows of 96 bf16 and four tokens take 354 us, 6.0 TB/s (0.91 of a measured copy), with the issue
 // slots 0.72 busy (4 tokens: some 70 instructions per 512 bytes).  Tried and slower at that size: sorting (2,144 us), sums in
 // shared memory indexed by token (609), cp.async rings per thread (427, bound by the load unit), rows listed by token by
 // the ninth warp (427) or by ballots of the adding warps (444).  Eight is the most tokens: groups of eight that read the
@@ -998,7 +999,9 @@ struct WgradPlan {
   size_t pair[2], counts, totals, head, tail, ends, bytes;
 };
 
-// The most blocks along the rows; few_plan's slices are the fewest with eight channels a piece.
+// The most blocks along the rows; few_plan's slices are the fewest with eight channels a piece.  Three blocks per SM is what
+// fits of the variants of up to 4 tokens (72 registers at most).  Of eight 16-bit channels a piece two fit at 5 tokens (79)
+// and at 6 to 8 (112), one of bf16 with int64 ids there (113): the grid is then one and a half waves, or three.
 int64_t few_most(int slices) { return std::max<int64_t>(1, kFewBlocksPerSm * static_cast<int64_t>(num_sms()) / slices); }
 
 // Few tokens: how a block reads its rows, by alignment and row length.
@@ -1051,8 +1054,9 @@ WgradPlan wgrad_plan(int64_t n, int32_t V, int32_t C) {
   p.G = 1;
   while (p.G < 32 && p.G * 4 < C) p.G *= 2;
   // about 32 warps per SM over the workers and the slices of 512 channels, at least 8 steps a worker (a step is some
-  // hundred instructions of one warp in a row: 12 longer workers' warps per SM took half as long again; 3,000 rows of 333 over
-  // 50 tokens: 24.6 us with 16 steps at least, 19.8 with 8)
+  // hundred instructions of one warp in a row: 12 longer workers' warps per SM took half as long again).  16 steps at least
+  // take longer where the rows spread over the tokens (3,000 rows of 333 over 50 tokens: 21.8 us of GPU time against 16.0)
+  // and 8 where half of them are one token's, whose parts one block joins (200,000 rows of 8 over 300 tokens: 350 against 200)
   const int64_t target = std::max<int64_t>(1, static_cast<int64_t>(num_sms()) * 32 * (32 / p.G) / ((C + 511) / 512));
   p.items = std::max<int64_t>(8, (V + n + target - 1) / target);
   p.workers = (V + n + p.items - 1) / p.items;

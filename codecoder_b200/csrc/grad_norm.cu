@@ -30,7 +30,7 @@ constexpr int kThreads = 256;
 constexpr int kChunkBytes = 16384;        // of the input: kUnroll 16-byte loads per thread
 constexpr int kListMax = 1000;            // tensors per launch: 24 bytes each, within the 32,764 bytes of parameters
 constexpr int kBlocksPerSm = 8;           // of the norm's kernel, at full occupancy
-constexpr int kScaleBlocksPerSm = 6;
+constexpr int kScaleBlocksPerSm = 6;      // 353 M bf16 values into fp32: 522 us with 6, 645 with 8 (40 registers), 571 with 4
 constexpr int kUnroll = 4;
 
 // A launch's tensors, of one type (and one output type): a kernel that branched over nine pairs of types spilled its
@@ -207,7 +207,7 @@ struct Piece {
       for (int e = 0; e < VEC; e += 2) w[e / 2] = h[e] | static_cast<uint32_t>(h[e + 1]) << 16;
     }
   }
-  __device__ __forceinline__ void store(T* p) const {      // streaming: nothing here reads it again
+  __device__ __forceinline__ void store(T* p) const {
     if constexpr (kWords == 4) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
     else *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
   }
@@ -426,7 +426,8 @@ int check_overlap(const void* const* in, void* const* out, const int64_t* numel,
   return 0;
 }
 
-// Calls f with the smallest list size that holds n tensors (a launch copies its whole parameter block), or a type.
+// Calls f with the smallest list size that holds n tensors, or a type.  A launch copies its whole parameter block: clipping 19
+// tensors takes 9.8 us a call with 24 places and 11.7 with 1,000, the norm of 300 takes 13.2 with 320 and 13.7.
 template <typename F>
 int with_list(size_t n, F f) {
   if (n <= 24) return f(std::integral_constant<int, 24>());

@@ -253,7 +253,8 @@ def gmm_wgrad(x: torch.Tensor, gy: torch.Tensor, idx: torch.Tensor) -> torch.Ten
 
 
 def op_status(device=None) -> int:
-    """Synchronise the current stream and read (and clear) the gather_mm kernels' watchdog word; raises if set."""
+    """Synchronise the current stream and read (and clear) the watchdog word of the op kernels with bounded waits (gather_mm,
+    the Cascade block boundary, embed_wgrad of up to 8 tokens); raises if set: a result since the last reading is not valid."""
     import ctypes
     s = ctypes.c_int(0)
     with torch.cuda.device(device if device is not None else torch.cuda.current_device()):
@@ -528,7 +529,7 @@ def embed_lookup(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
                  dtype: torch.dtype | None = None) -> torch.Tensor:
     """scale weight[ids] (C ABI bpc_embed_lookup): ids (...) int32 or int64, weight (V, C) fp32, bf16 or fp16 ->
     (..., C) in `dtype` (default: weight's), the product in fp32 and rounded once.  An id outside [0, V) reads a zero
-    row, as gmm's idx does: -1 marks a padded position."""
+    row, as gmm's idx does: -1 marks a padded position.  Not differentiable, whatever weight requires: see embedding."""
     return _lib.torch_ops().embed_lookup(ids, weight, scale, dtype)
 
 
@@ -536,7 +537,8 @@ def embed_wgrad(gy: torch.Tensor, ids: torch.Tensor, n_tokens: int, scale: float
                 dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """The weight gradient of embed_lookup (C ABI bpc_embed_wgrad): gy (..., C), ids (...) -> dW (n_tokens, C) in
     `dtype`, dW[v] = scale sum over ids == v of gy, summed in fp32 in a fixed order (deterministic) and rounded once.
-    Ids outside [0, n_tokens) contribute nothing; tokens that do not occur get zeros."""
+    Ids outside [0, n_tokens) contribute nothing; tokens that do not occur get zeros.  Up to 8 tokens run a kernel with
+    bounded waits: op_status reports one that ran out."""
     return _lib.torch_ops().embed_wgrad(gy, ids, n_tokens, scale, dtype)
 
 

@@ -144,10 +144,12 @@ BPC_API int bpc_embed_tokens_bwd(const uint8_t* det, const uint8_t* check_type, 
  *                     tokens without a row get zeros
  * ids (n) int32 or int64 (id_bytes 4 or 8); W (V, C) with rows w_stride elements apart, y (n, C); gy (n, C) with rows
  * gy_stride elements apart, dW (V, C).  Each of W, y, gy, dW is f32, bf16 or f16; products and sums are fp32, rounded
- * once.  The gradient sorts the positions by token and adds each token's rows in a fixed order (deterministic); its
+ * once.  The gradient adds each token's rows in a fixed order (deterministic): sorted by token, or for up to 8 tokens
+ * by fixed shares of the rows, in a kernel with bounded waits (bpc_gather_mm_status reports one that ran out).  Its
  * workspace holds the sorted positions and partial sums, bpc_embed_wgrad_workspace_size(n, V, C) bytes on the current
- * device, 16-byte aligned.  n < 2^31, V < 2^31 - 1, C <= 2^20; every buffer aligned to its type.  Up to 8 tokens are
- * summed without a sort, by a kernel with bounded waits; bpc_gather_mm_status reports one that ran out. */
+ * device, 16-byte aligned.  n < 2^31, V < 2^31 - 1, C <= 2^20; every buffer aligned to its type.  Rows of 16-bit gy that
+ * only 2 bytes align are read by the aligned 4-byte words around their elements: up to 2 bytes before or after gy's are
+ * read too, and not used. */
 BPC_API int bpc_embed_lookup(const void* ids, int32_t id_bytes, const void* w, void* y, int64_t n, int32_t V, int32_t C,
                              int64_t w_stride, float scale, int32_t w_dtype, int32_t y_dtype, bpc_stream_t stream);
 BPC_API size_t bpc_embed_wgrad_workspace_size(int64_t n, int32_t V, int32_t C);
@@ -228,9 +230,9 @@ BPC_API int bpc_gather_mm_wgrad(const void* x, const void* gy, const int32_t* id
 BPC_API size_t bpc_gather_mm_wgrad_workspace_size(int64_t B, int32_t NS, int32_t NT, int32_t K, int32_t Ci, int32_t Co,
                                                   int32_t dtype);
 
-/* Synchronises `stream`, reads and clears the current device's watchdog status word of the gather_mm entry points and
- * bpc_embed_wgrad (0 = every bounded wait completed).  Returns BPC_ERR_DEVICE when a tensor-core kernel gave up a wait, in
- * which case that launch's output is not valid. */
+/* Synchronises `stream`, reads and clears the current device's watchdog status word of the gather_mm entry points, the
+ * Cascade block boundary and bpc_embed_wgrad (0 = every bounded wait completed).  Returns BPC_ERR_DEVICE when a kernel gave
+ * up a wait, in which case that launch's output is not valid. */
 BPC_API int bpc_gather_mm_status(bpc_stream_t stream, int* status);
 
 /* ------------------------------------------------------------------------------------------------------------
