@@ -104,7 +104,8 @@ def build_torch_ops() -> str:
            os.path.join(REPO, "include")]
     tmp = TORCH_OUT + ".tmp"
     _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-          "-DTORCH_EXTENSION_NAME=_torch_ops", f'-DBUILT_FOR="{torch_stamp()}"', f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+          "-DTORCH_EXTENSION_NAME=_torch_ops", f'-DBUILT_FOR="{torch_stamp()}"',
+          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
           *[f"-isystem{d}" for d in inc], TORCH_SRC, "-o", tmp, "-L", os.path.join(root, "lib"), "-lc10", "-lc10_cuda",
           "-ltorch_cpu", "-ltorch_python"], f"g++ on {TORCH_SRC}")
     os.replace(tmp, TORCH_OUT)
@@ -136,11 +137,9 @@ def build_lib(verbose: bool = False) -> str:
 def build(force: bool = False, verbose: bool = False) -> str:
     """Both libraries, where they are older than their sources; libbpc.so alone where there is no torch to compile against
     (a C caller's machine: _lib.torch_ops() says then what is missing)."""
-    wanted = force or _older(TORCH_OUT, [TORCH_SRC, _header()])
     lack = torch_ops_lack()
-    wanted = wanted or not lack and stamp_of(TORCH_OUT) != torch_stamp()
-    lack = lack if wanted else None
-    if lack:
+    wanted = force or _older(TORCH_OUT, [TORCH_SRC, _header()]) or not lack and stamp_of(TORCH_OUT) != torch_stamp()
+    if wanted and lack:
         sys.stderr.write(f"{os.path.basename(TORCH_OUT)} is not built: {lack}\n")
     with cf.ThreadPoolExecutor(max_workers=1) as ex:
         host = ex.submit(build_torch_ops) if wanted and not lack else None

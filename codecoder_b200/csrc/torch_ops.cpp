@@ -131,8 +131,8 @@ Tensor embed_wgrad(const Tensor& gy_in, const Tensor& ids_in, int64_t n_tokens, 
   const int64_t ld = row_stride(gy);
   const int32_t V = static_cast<int32_t>(n_tokens), Ci = static_cast<int32_t>(C);
   Tensor ws = empty({static_cast<int64_t>(entry.embed_wgrad_workspace_size(n, V, Ci))}, at::kByte, gy);
-  check(entry.embed_wgrad(gy.const_data_ptr(), ids.const_data_ptr(), id_bytes, dw.data_ptr(), ws.data_ptr(), ws.numel(), n, V, Ci,
-                          ld, static_cast<float>(scale), dtype_code(gy.scalar_type()), dtype_code(dtype), stream_of(gy)),
+  check(entry.embed_wgrad(gy.const_data_ptr(), ids.const_data_ptr(), id_bytes, dw.data_ptr(), ws.data_ptr(), ws.numel(), n,
+                          V, Ci, ld, static_cast<float>(scale), dtype_code(gy.scalar_type()), dtype_code(dtype), stream_of(gy)),
         "bpc_embed_wgrad");
   return dw;
 }
