@@ -768,8 +768,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 3) wgrad_join_kernel(const __
 // flight depend neither on registers nor on the load units).  The threads of the other eight lie along a row's pieces
 // of VEC channels and several rows; each keeps one sum per token in registers and adds its piece under one predicate per
 // token.  A block adds its threads' sums in order, wgrad_few_join_kernel the blocks' in fp64.
-//   Bound by HBM: 10.8 M rows of 96 bf16 and four tokens take 354 us, 6.0 TB/s (0.91 of a measured copy), with the issue
-// slots 0.72 busy (4 tokens: some 70 instructions per 512 bytes).  Tried and slower at that size: sorting (2,144 us), sums in
+//   Bound by HBM: 10.8 M rows of 96 bf16 and four tokens take 354 us, 6.0 TB/s (0.91 of a measured copy; 324 us on
+// another B200), with the issue slots 0.72 busy (4 tokens: some 70 instructions per 512 bytes).  Tried and slower at that size: sorting (2,144 us), sums in
 // shared memory indexed by token (609), cp.async rings per thread (427, bound by the load unit), rows listed by token by
 // the ninth warp (427) or by ballots of the adding warps (444).  Eight is the most tokens: groups of eight that read the
 // rows again from L2 took 176 us against 127 sorted (20 tokens, 1 M rows of 64 bf16).
