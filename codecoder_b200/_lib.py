@@ -12,6 +12,9 @@ LIB_PATH = os.environ.get("BPC_LIB", os.path.join(_PKG, "libbpc.so"))
 BPC_DTYPE_F32 = 0
 BPC_DTYPE_BF16 = 1
 BPC_DTYPE_F16 = 2
+BPC_ACT_NONE = 0
+BPC_ACT_SILU = 1
+BPC_ACT_GELU = 2
 BPC_EPILOGUE_STORE = 0
 BPC_EPILOGUE_AFFINE_SILU = 1
 BPC_EPILOGUE_ADD = 2
@@ -60,6 +63,19 @@ SIGNATURES = {
     "bpc_embed_wgrad_workspace_size": (ctypes.c_size_t, [c_i64, c_i32, c_i32]),
     "bpc_embed_wgrad": (ctypes.c_int, [c_vp, c_vp, c_i32, c_vp, c_vp, ctypes.c_size_t, c_i64, c_i32, c_i32, c_i64,
                                        ctypes.c_float, c_i32, c_i32, c_vp]),
+    "bpc_group_norm_workspace_size": (ctypes.c_size_t, [c_i64, c_i64, c_i32, c_i32, c_i32]),
+    "bpc_group_norm_fwd": (ctypes.c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i32, c_i32, c_i64, c_i64,
+                                          ctypes.c_float, c_i32, c_i32, c_i32, c_vp, ctypes.c_size_t, c_vp]),
+    "bpc_group_norm_bwd": (ctypes.c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i32, c_i32,
+                                          c_i64, c_i64, c_i64, c_i64, c_i32, c_i32, c_i32, c_vp, ctypes.c_size_t, c_vp]),
+    "bpc_linear_attention_workspace_size": (ctypes.c_size_t, [c_i64, c_i64, c_i32, c_i32, c_i32, c_i32, c_i32]),
+    "bpc_linear_attention_fwd": (ctypes.c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i32, c_i64, c_i64, c_i32,
+                                                c_i32, c_i32, c_vp, ctypes.c_float, c_i32, c_vp, ctypes.c_size_t, c_vp]),
+    "bpc_linear_attention_bwd": (ctypes.c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i32, c_vp, c_vp, c_vp,
+                                                c_vp, c_i64, c_i64, c_i32, c_i32, c_i32, c_vp, ctypes.c_float, c_i32, c_vp,
+                                                ctypes.c_size_t, c_vp]),
+    "bpc_linear_attention_step": (ctypes.c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i32, c_i32, c_i32, c_vp,
+                                                 ctypes.c_float, c_i32, c_vp]),
     "bpc_grad_norm_workspace_size": (ctypes.c_size_t, [c_i32]),
     "bpc_grad_norm": (ctypes.c_int, [c_vp, c_vp, c_vp, c_i32, c_vp, c_vp, ctypes.c_size_t, c_vp]),
     "bpc_clip_grads": (ctypes.c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_i32, ctypes.c_double, c_vp, c_vp,

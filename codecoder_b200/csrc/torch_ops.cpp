@@ -1,4 +1,4 @@
-// Host side of the embedding and gradient-norm operators: argument checks, outputs, workspaces and the calls of
+// Host side of the embedding, gradient-norm, group-norm and linear-attention operators: argument checks, outputs, workspaces and the calls of
 // libbpc.so's C entry points, as a Python module on torch tensors.  In C++ because these calls are short: reading a
 // list of 176 gradients through Python costs about 0.4 us per tensor, more than the kernels take; here 0.02 us.
 // The module does not link to libbpc.so: _lib.py hands it the entry points of the library it loaded.
@@ -23,6 +23,13 @@ struct Entry {
   decltype(&bpc_embed_lookup) embed_lookup = nullptr;
   decltype(&bpc_embed_wgrad) embed_wgrad = nullptr;
   decltype(&bpc_embed_wgrad_workspace_size) embed_wgrad_workspace_size = nullptr;
+  decltype(&bpc_group_norm_fwd) group_norm_fwd = nullptr;
+  decltype(&bpc_group_norm_bwd) group_norm_bwd = nullptr;
+  decltype(&bpc_group_norm_workspace_size) group_norm_workspace_size = nullptr;
+  decltype(&bpc_linear_attention_fwd) linear_attention_fwd = nullptr;
+  decltype(&bpc_linear_attention_bwd) linear_attention_bwd = nullptr;
+  decltype(&bpc_linear_attention_step) linear_attention_step = nullptr;
+  decltype(&bpc_linear_attention_workspace_size) linear_attention_workspace_size = nullptr;
   decltype(&bpc_grad_norm) grad_norm = nullptr;
   decltype(&bpc_clip_grads) clip_grads = nullptr;
   decltype(&bpc_grad_norm_workspace_size) grad_norm_workspace_size = nullptr;
@@ -39,6 +46,13 @@ void bind(const py::dict& table) {
   take(entry.embed_lookup, table, "bpc_embed_lookup");
   take(entry.embed_wgrad, table, "bpc_embed_wgrad");
   take(entry.embed_wgrad_workspace_size, table, "bpc_embed_wgrad_workspace_size");
+  take(entry.group_norm_fwd, table, "bpc_group_norm_fwd");
+  take(entry.group_norm_bwd, table, "bpc_group_norm_bwd");
+  take(entry.group_norm_workspace_size, table, "bpc_group_norm_workspace_size");
+  take(entry.linear_attention_fwd, table, "bpc_linear_attention_fwd");
+  take(entry.linear_attention_bwd, table, "bpc_linear_attention_bwd");
+  take(entry.linear_attention_step, table, "bpc_linear_attention_step");
+  take(entry.linear_attention_workspace_size, table, "bpc_linear_attention_workspace_size");
   take(entry.grad_norm, table, "bpc_grad_norm");
   take(entry.clip_grads, table, "bpc_clip_grads");
   take(entry.grad_norm_workspace_size, table, "bpc_grad_norm_workspace_size");
@@ -235,6 +249,245 @@ Tensor clip_grads(const py::list& ts, double max_norm, const std::optional<py::l
   return norm;
 }
 
+// x (B, ..., C) as (B, N, C) with contiguous channels; copies only where the layout asks for it
+Tensor samples_of(const Tensor& x_in) {
+  Tensor x = x_in.resolve_neg();
+  const int64_t C = x.size(-1), N = x.numel() / (x.size(0) * C);
+  x = x.reshape({x.size(0), N, C});
+  return C > 1 && x.stride(2) != 1 ? x.contiguous() : x;
+}
+
+void check_norm(const Tensor& x, int64_t groups, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias,
+                at::ScalarType out) {
+  check_cuda(x);
+  const at::ScalarType in = x.scalar_type();
+  TORCH_CHECK_TYPE(dtype_code(in) >= 0 && dtype_code(out) >= 0 && (in == out || in == at::kFloat),
+                   "group_norm takes fp32, bf16 and fp16 features, and narrows fp32 ones only, got ", in, " -> ", out);
+  TORCH_CHECK_VALUE(x.dim() >= 2, "group_norm: x must be (samples, ..., channels)");
+  const int64_t C = x.size(-1);
+  TORCH_CHECK_VALUE(C >= 1 && C <= (1 << 20) && groups >= 1 && C % groups == 0,
+                    "group_norm: the channels (1 to 2^20) must divide into the groups, got ", C, " and ", groups);
+  for (const auto& p : {weight, bias})
+    if (p) {
+      check_pair(x, *p);
+      TORCH_CHECK_VALUE(p->dim() == 1 && p->size(0) == C, "group_norm: weight and bias must be (channels)");
+      TORCH_CHECK_TYPE(at::isFloatingType(p->scalar_type()), "group_norm: weight and bias must be floating point");
+    }
+}
+
+// A per-channel vector as contiguous fp32; an undefined tensor where there is none
+Tensor channel_vector(const std::optional<Tensor>& p) {
+  return p ? p->to(at::kFloat).resolve_neg().contiguous() : Tensor();
+}
+const float* f32_or_null(const Tensor& t) { return t.defined() ? static_cast<const float*>(t.const_data_ptr()) : nullptr; }
+
+Tensor norm_workspace(const Tensor& x, int64_t groups, bool backward) {
+  return empty({static_cast<int64_t>(entry.group_norm_workspace_size(x.size(0), x.size(1), static_cast<int32_t>(x.size(2)),
+                                                                     static_cast<int32_t>(groups), backward))},
+               at::kByte, x);
+}
+
+// y, and where `stats` is set the groups' mean and rstd (samples, groups)
+std::tuple<Tensor, Tensor, Tensor> group_norm_fwd(const Tensor& x_in, int64_t groups, const std::optional<Tensor>& weight,
+                                                  const std::optional<Tensor>& bias, double eps, int64_t activation,
+                                                  std::optional<at::ScalarType> dtype, bool stats) {
+  at::NoGradGuard no_grad;
+  const at::ScalarType out = dtype.value_or(x_in.scalar_type());
+  check_norm(x_in, groups, weight, bias, out);
+  const c10::cuda::CUDAGuard guard(x_in.device());
+  Tensor y = empty(x_in.sizes(), out, x_in), mean, rstd;
+  if (stats) mean = empty({x_in.size(0), groups}, at::kFloat, x_in), rstd = at::empty_like(mean);
+  if (y.numel() == 0) return {y, mean, rstd};
+  Tensor x = samples_of(x_in), w = channel_vector(weight), b = channel_vector(bias), ws = norm_workspace(x, groups, false);
+  check(entry.group_norm_fwd(x.const_data_ptr(), y.data_ptr(), stats ? static_cast<float*>(mean.data_ptr()) : nullptr,
+                             stats ? static_cast<float*>(rstd.data_ptr()) : nullptr, f32_or_null(w), f32_or_null(b),
+                             x.size(0), x.size(1), static_cast<int32_t>(x.size(2)), static_cast<int32_t>(groups),
+                             x.stride(0), x.stride(1), static_cast<float>(eps), static_cast<int32_t>(activation),
+                             dtype_code(x.scalar_type()), dtype_code(out), ws.data_ptr(), ws.numel(), stream_of(x)),
+        "bpc_group_norm_fwd");
+  return {y, mean, rstd};
+}
+
+// dx, dw, db; undefined where `want` says that one is not asked for
+std::tuple<Tensor, Tensor, Tensor> group_norm_bwd(const Tensor& gy_in, const Tensor& x_in, const Tensor& mean,
+                                                  const Tensor& rstd, int64_t groups, const std::optional<Tensor>& weight,
+                                                  const std::optional<Tensor>& bias, int64_t activation, bool want_dx,
+                                                  bool want_dw, bool want_db) {
+  at::NoGradGuard no_grad;
+  check_pair(x_in, gy_in);
+  check_norm(x_in, groups, weight, bias, gy_in.scalar_type());
+  TORCH_CHECK_VALUE(gy_in.sizes() == x_in.sizes(), "group_norm: gy must have x's shape");
+  const c10::cuda::CUDAGuard guard(x_in.device());
+  const int64_t C = x_in.size(-1);
+  Tensor dx, dw, db;
+  if (want_dx) dx = empty(x_in.sizes(), x_in.scalar_type(), x_in);
+  if (want_dw) dw = empty({C}, at::kFloat, x_in);
+  if (want_db) db = empty({C}, at::kFloat, x_in);
+  if (x_in.numel() == 0) {
+    if (want_dw) dw.zero_();
+    if (want_db) db.zero_();
+    return {dx, dw, db};
+  }
+  Tensor x = samples_of(x_in), gy = samples_of(gy_in), w = channel_vector(weight), b = channel_vector(bias);
+  Tensor ws = norm_workspace(x, groups, true);
+  check(entry.group_norm_bwd(gy.const_data_ptr(), x.const_data_ptr(), f32_or_null(mean), f32_or_null(rstd), f32_or_null(w),
+                             f32_or_null(b), want_dx ? dx.data_ptr() : nullptr,
+                             want_dw ? static_cast<float*>(dw.data_ptr()) : nullptr,
+                             want_db ? static_cast<float*>(db.data_ptr()) : nullptr, x.size(0), x.size(1),
+                             static_cast<int32_t>(C), static_cast<int32_t>(groups), gy.stride(0), gy.stride(1), x.stride(0),
+                             x.stride(1), static_cast<int32_t>(activation), dtype_code(x.scalar_type()),
+                             dtype_code(gy.scalar_type()), ws.data_ptr(), ws.numel(), stream_of(x)),
+        "bpc_group_norm_bwd");
+  return {dx, dw, db};
+}
+
+// Head rows with contiguous elements
+Tensor head_rows(const Tensor& t_in) {
+  Tensor t = t_in.resolve_neg();
+  return t.size(-1) > 1 && t.stride(-1) != 1 ? t.contiguous() : t;
+}
+
+int32_t check_heads(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, int64_t dims, const char* what) {
+  check_cuda(q);
+  for (const Tensor* t : {&k, &v, &log_decay}) check_pair(q, *t);
+  const int32_t code = dtype_code(q.scalar_type());
+  TORCH_CHECK_TYPE((code == BPC_DTYPE_F32 || code == BPC_DTYPE_BF16) && k.scalar_type() == q.scalar_type() &&
+                       v.scalar_type() == q.scalar_type(),
+                   what, " takes fp32 or bf16 q, k and v of one type, got ", q.scalar_type(), ", ", k.scalar_type(), ", ",
+                   v.scalar_type());
+  TORCH_CHECK_TYPE(log_decay.scalar_type() == at::kFloat, what, ": log_decay must be fp32, got ", log_decay.scalar_type());
+  TORCH_CHECK_VALUE(q.dim() == dims && k.sizes() == q.sizes() && v.dim() == dims &&
+                        v.sizes().slice(0, dims - 1) == q.sizes().slice(0, dims - 1),
+                    what, ": q and k of one shape, v the same but for the head size (", dims, " dimensions), got ", q.sizes(),
+                    ", ", k.sizes(), " and ", v.sizes());
+  TORCH_CHECK_VALUE(q.size(-1) >= 1 && q.size(-1) <= 128 && v.size(-1) >= 1 && v.size(-1) <= 128, what,
+                    ": head sizes must be 1 to 128, got ", q.size(-1), " and ", v.size(-1));
+  TORCH_CHECK_VALUE(log_decay.dim() == 1 && log_decay.size(0) == q.size(-2), what, ": log_decay must be (heads)");
+  return code;
+}
+
+// A (batch, heads, dk, dv) fp32 state as a contiguous, 16-byte aligned tensor
+Tensor check_state(const Tensor& s, const Tensor& q, const Tensor& v, const char* what) {
+  check_pair(q, s);
+  TORCH_CHECK_TYPE(s.scalar_type() == at::kFloat, what, ": states are fp32, got ", s.scalar_type());
+  TORCH_CHECK_VALUE(s.sizes() == at::IntArrayRef({q.size(0), q.size(-2), q.size(-1), v.size(-1)}), what,
+                    ": a state must be (batch, heads, dk, dv), got ", s.sizes());
+  Tensor t = s.resolve_neg().contiguous();
+  return reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 ? t.clone() : t;
+}
+
+Tensor check_lengths(const std::optional<Tensor>& lengths, const Tensor& q, const char* what) {
+  if (!lengths) return Tensor();
+  check_pair(q, *lengths);
+  TORCH_CHECK_TYPE(lengths->scalar_type() == at::kInt || lengths->scalar_type() == at::kLong, what,
+                   ": lengths must be int32 or int64, got ", lengths->scalar_type());
+  TORCH_CHECK_VALUE(lengths->dim() == 1 && lengths->size(0) == q.size(0), what, ": lengths must be (batch)");
+  return lengths->contiguous();
+}
+int32_t length_bytes(const Tensor& t) { return t.defined() ? static_cast<int32_t>(t.element_size()) : 0; }
+const void* data_or_null(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
+
+void strides_of(const Tensor& t, int64_t*& at) {
+  for (int64_t d = 0; d + 1 < t.dim(); ++d) *at++ = t.stride(d);
+}
+
+Tensor attention_workspace(const Tensor& q, const Tensor& v, int32_t code, bool backward) {
+  return empty({static_cast<int64_t>(entry.linear_attention_workspace_size(
+                   q.size(0), q.size(1), static_cast<int32_t>(q.size(2)), static_cast<int32_t>(q.size(3)),
+                   static_cast<int32_t>(v.size(3)), code, backward))},
+               at::kByte, q);
+}
+
+// o, and where `want_state` is set the state after each sequence's last position
+std::tuple<Tensor, Tensor> linear_attention_fwd(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in,
+                                                const Tensor& log_decay, double scale, const std::optional<Tensor>& state_in,
+                                                const std::optional<Tensor>& lengths_in, bool want_state) {
+  at::NoGradGuard no_grad;
+  const char* what = "linear_attention";
+  const int32_t code = check_heads(q_in, k_in, v_in, log_decay, 4, what);
+  const c10::cuda::CUDAGuard guard(q_in.device());
+  Tensor state = state_in ? check_state(*state_in, q_in, v_in, what) : Tensor(), lengths = check_lengths(lengths_in, q_in, what);
+  Tensor q = head_rows(q_in), k = head_rows(k_in), v = head_rows(v_in), decay = log_decay.resolve_neg().contiguous();
+  Tensor o = empty(v.sizes(), v.scalar_type(), v), new_state;
+  if (want_state) new_state = empty({q.size(0), q.size(2), q.size(3), v.size(3)}, at::kFloat, q);
+  if (q.size(0) == 0 || q.size(2) == 0) return {o, new_state};
+  Tensor ws = attention_workspace(q, v, code, false);
+  int64_t strides[9], *at = strides;
+  for (const Tensor* t : {&q, &k, &v}) strides_of(*t, at);
+  check(entry.linear_attention_fwd(q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), o.data_ptr(),
+                                   f32_or_null(decay), f32_or_null(state),
+                                   want_state ? static_cast<float*>(new_state.data_ptr()) : nullptr, data_or_null(lengths),
+                                   length_bytes(lengths), q.size(0), q.size(1), static_cast<int32_t>(q.size(2)),
+                                   static_cast<int32_t>(q.size(3)), static_cast<int32_t>(v.size(3)), strides,
+                                   static_cast<float>(scale), code, ws.data_ptr(), ws.numel(), stream_of(q)),
+        "bpc_linear_attention_fwd");
+  return {o, new_state};
+}
+
+// dq, dk, dv, and where `want_dstate` is set the gradient of the first state
+std::tuple<Tensor, Tensor, Tensor, Tensor> linear_attention_bwd(
+    const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const Tensor& go_in, const Tensor& log_decay, double scale,
+    const std::optional<Tensor>& state_in, const std::optional<Tensor>& grad_state_in, const std::optional<Tensor>& lengths_in,
+    bool want_dstate) {
+  at::NoGradGuard no_grad;
+  const char* what = "linear_attention";
+  const int32_t code = check_heads(q_in, k_in, v_in, log_decay, 4, what);
+  check_pair(q_in, go_in);
+  TORCH_CHECK_VALUE(go_in.sizes() == v_in.sizes() && go_in.scalar_type() == v_in.scalar_type(),
+                    "linear_attention: go must be like v");
+  const c10::cuda::CUDAGuard guard(q_in.device());
+  Tensor state = state_in ? check_state(*state_in, q_in, v_in, what) : Tensor();
+  Tensor grad_state = grad_state_in ? check_state(*grad_state_in, q_in, v_in, what) : Tensor();
+  Tensor lengths = check_lengths(lengths_in, q_in, what), decay = log_decay.resolve_neg().contiguous();
+  Tensor q = head_rows(q_in), k = head_rows(k_in), v = head_rows(v_in), go = head_rows(go_in);
+  Tensor dq = empty(q.sizes(), q.scalar_type(), q), dk = at::empty_like(dq), dv = empty(v.sizes(), v.scalar_type(), v), dstate;
+  if (want_dstate) dstate = empty({q.size(0), q.size(2), q.size(3), v.size(3)}, at::kFloat, q);
+  if (q.size(0) == 0 || q.size(2) == 0) return {dq, dk, dv, dstate};
+  Tensor ws = attention_workspace(q, v, code, true);
+  int64_t strides[12], *at = strides;
+  for (const Tensor* t : {&q, &k, &v, &go}) strides_of(*t, at);
+  check(entry.linear_attention_bwd(q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), go.const_data_ptr(),
+                                   f32_or_null(decay), f32_or_null(state), f32_or_null(grad_state), data_or_null(lengths),
+                                   length_bytes(lengths), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                                   want_dstate ? static_cast<float*>(dstate.data_ptr()) : nullptr, q.size(0), q.size(1),
+                                   static_cast<int32_t>(q.size(2)), static_cast<int32_t>(q.size(3)),
+                                   static_cast<int32_t>(v.size(3)), strides, static_cast<float>(scale), code, ws.data_ptr(),
+                                   ws.numel(), stream_of(q)),
+        "bpc_linear_attention_bwd");
+  return {dq, dk, dv, dstate};
+}
+
+// o; new_state (the state itself where none is given) is written
+Tensor linear_attention_step(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const Tensor& log_decay,
+                             const Tensor& state, double scale, const std::optional<Tensor>& new_state) {
+  at::NoGradGuard no_grad;
+  const char* what = "linear_attention_step";
+  const int32_t code = check_heads(q_in, k_in, v_in, log_decay, 3, what);
+  const Tensor& to = new_state ? *new_state : state;
+  for (const Tensor* s : {&state, &to}) {
+    check_pair(q_in, *s);
+    TORCH_CHECK_TYPE(s->scalar_type() == at::kFloat, what, ": states are fp32, got ", s->scalar_type());
+    TORCH_CHECK_VALUE(s->sizes() == at::IntArrayRef({q_in.size(0), q_in.size(1), q_in.size(2), v_in.size(2)}), what,
+                      ": a state must be (batch, heads, dk, dv), got ", s->sizes());
+    TORCH_CHECK_VALUE(s->is_contiguous() && !s->is_neg(), what, ": states must be contiguous");
+    TORCH_CHECK_VALUE(!s->requires_grad(), what, ": a state that requires a gradient (it is updated without one)");
+  }
+  const c10::cuda::CUDAGuard guard(q_in.device());
+  Tensor q = head_rows(q_in), k = head_rows(k_in), v = head_rows(v_in), decay = log_decay.resolve_neg().contiguous();
+  Tensor o = empty(v.sizes(), v.scalar_type(), v);
+  if (o.numel() == 0) return o;
+  int64_t strides[6], *at = strides;
+  for (const Tensor* t : {&q, &k, &v}) strides_of(*t, at);
+  float* written = static_cast<float*>(to.mutable_data_ptr());      // first: a state that shares its memory until written moves
+  check(entry.linear_attention_step(q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), o.data_ptr(),
+                                    f32_or_null(decay), f32_or_null(state), written, q.size(0),
+                                    static_cast<int32_t>(q.size(1)), static_cast<int32_t>(q.size(2)),
+                                    static_cast<int32_t>(v.size(2)), strides, static_cast<float>(scale), code, stream_of(q)),
+        "bpc_linear_attention_step");
+  if (!to.is_inference()) to.unsafeGetTensorImpl()->bump_version();       // written behind autograd's back
+  return o;
+}
+
 }  // namespace
 
 // What the build reads back, to compile again for another torch or Python, and to refuse loading there until then
@@ -245,6 +498,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   const auto release = py::call_guard<py::gil_scoped_release>();
   m.def("embed_lookup", &embed_lookup, release);
   m.def("embed_wgrad", &embed_wgrad, release);
+  m.def("group_norm_fwd", &group_norm_fwd, release);
+  m.def("group_norm_bwd", &group_norm_bwd, release);
+  m.def("linear_attention_fwd", &linear_attention_fwd, release);
+  m.def("linear_attention_bwd", &linear_attention_bwd, release);
+  m.def("linear_attention_step", &linear_attention_step, release);
   m.def("grad_norm", &grad_norm);
   m.def("clip_grads", &clip_grads);
 }

@@ -12,7 +12,9 @@ the rows, partial sums added in a fixed order), as the reference's is.
 
 Around the op, for training: embed_lookup / embed_wgrad / embedding (token embeddings of any size, as nn.Embedding is
 used by cascade_net.py:279-285) and grad_norm / clip_grads / clip_grad_norm_ (the gradient clipping of
-cascade_train.py:292-320).
+cascade_train.py:292-320).  Layers beside the op: group_norm (per-sample normalisation with an activation, where the
+reference has BatchNorm + SiLU, cascade_net.py:195-210) and linear_attention / linear_attention_step (a memory over rounds,
+for whole experiments and one round at a time).
 """
 from __future__ import annotations
 
@@ -592,6 +594,99 @@ def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
     if not grads:
         return torch.zeros(())
     return clip_grads(grads, max_norm)
+
+
+ACTIVATIONS = {"none": _lib.BPC_ACT_NONE, "silu": _lib.BPC_ACT_SILU, "gelu": _lib.BPC_ACT_GELU}
+
+
+class GroupNormB200(torch.autograd.Function):
+    """group_norm with its gradients (C ABI bpc_group_norm_fwd / _bwd); differentiable once."""
+
+    @staticmethod
+    def forward(ctx, x, groups, weight, bias, eps, act, dtype):
+        y, mean, rstd = _lib.torch_ops().group_norm_fwd(x, groups, weight, bias, eps, act, dtype, True)
+        ctx.save_for_backward(x, mean, rstd, weight, bias)
+        ctx.set_materialize_grads(False)
+        ctx.groups, ctx.act = groups, act
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gy):
+        if gy is None:
+            return (None,) * 7
+        x, mean, rstd, weight, bias = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx, dw, db = _lib.torch_ops().group_norm_bwd(gy, x, mean, rstd, ctx.groups, weight, bias, ctx.act, need[0], need[2],
+                                                     need[3])
+        return (dx, None, dw.to(weight.dtype) if need[2] else None, db.to(bias.dtype) if need[3] else None, None, None, None)
+
+
+def group_norm(x: torch.Tensor, groups: int, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+               eps: float = 1e-5, activation: str = "none", dtype: torch.dtype | None = None) -> torch.Tensor:
+    """act(weight (x - mean) / sqrt(var + eps) + bias) over channels-last features (C ABI bpc_group_norm_fwd / _bwd):
+    x (B, ..., C) fp32, bf16 or fp16; mean and variance over a sample's positions and the C / groups channels of a group;
+    weight, bias (C) or None; activation "none", "silu" or "gelu" (the tanh form) -> x's shape in `dtype` (default: x's; fp32
+    features may be narrowed).  Statistics in fp32, the result rounded once.  The gradients of x, weight and bias are
+    deterministic; differentiable once."""
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"group_norm: activation must be one of {', '.join(ACTIVATIONS)}, got {activation!r}")
+    act = ACTIVATIONS[activation]
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+        return GroupNormB200.apply(x, groups, weight, bias, eps, act, dtype)
+    return _lib.torch_ops().group_norm_fwd(x, groups, weight, bias, eps, act, dtype, False)[0]
+
+
+class LinearAttentionB200(torch.autograd.Function):
+    """linear_attention with its gradients (C ABI bpc_linear_attention_fwd / _bwd); differentiable once."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, log_decay, scale, state, lengths, return_state):
+        o, new_state = _lib.torch_ops().linear_attention_fwd(q, k, v, log_decay, scale, state, lengths, return_state)
+        ctx.save_for_backward(q, k, v, log_decay, state, lengths)
+        ctx.set_materialize_grads(False)
+        ctx.scale = scale
+        return (o, new_state) if return_state else o
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, go, grad_state=None):
+        if go is None and grad_state is None:
+            return (None,) * 8
+        q, k, v, log_decay, state, lengths = ctx.saved_tensors
+        if go is None:
+            go = torch.zeros_like(v)
+        dq, dk, dv, dstate = _lib.torch_ops().linear_attention_bwd(q, k, v, go, log_decay, ctx.scale, state, grad_state,
+                                                                   lengths, ctx.needs_input_grad[5])
+        return dq, dk, dv, None, None, dstate, None, None
+
+
+def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, scale: float | None = None,
+                     state: torch.Tensor | None = None, lengths: torch.Tensor | None = None, return_state: bool = False):
+    """Linear attention with a decay for each head over whole sequences (C ABI bpc_linear_attention_fwd / _bwd):
+      S_t = a_h S_(t-1) + k_t v_t^T,  o_t = scale q_t S_t,  a_h = exp(log_decay_h)
+    q, k (B, T, H, dk), v (B, T, H, dv) fp32 or bf16, any strides (head sizes 1 to 128); log_decay (H) fp32, not
+    differentiable; scale: dk^-0.5 by default; state (B, H, dk, dv) fp32: S before the first position (default: zero);
+    lengths (B) int32 or int64: positions at or behind a sequence's length are not read, and zero in the result -> o
+    (B, T, H, dv) in the inputs' type, and with return_state the state after each sequence's last position, which
+    linear_attention_step (or a next call) goes on from.  States and sums are fp32; the gradients of q, k, v and state are
+    deterministic; differentiable once."""
+    if log_decay.requires_grad:
+        raise ValueError("linear_attention: log_decay takes no gradient (detach it)")
+    scale = q.shape[-1] ** -0.5 if scale is None else scale
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, state)):
+        return LinearAttentionB200.apply(q, k, v, log_decay, scale, state, lengths, return_state)
+    o, new_state = _lib.torch_ops().linear_attention_fwd(q, k, v, log_decay, scale, state, lengths, return_state)
+    return (o, new_state) if return_state else o
+
+
+def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, state: torch.Tensor,
+                          scale: float | None = None, new_state: torch.Tensor | None = None) -> torch.Tensor:
+    """One position of linear_attention (C ABI bpc_linear_attention_step): q, k (B, H, dk), v (B, H, dv), state
+    (B, H, dk, dv) fp32 contiguous -> o (B, H, dv); the state is updated in place, or written to `new_state`, which must not
+    overlap it.  Not differentiable, whatever the inputs require."""
+    scale = q.shape[-1] ** -0.5 if scale is None else scale
+    return _lib.torch_ops().linear_attention_step(q, k, v, log_decay, state, scale, new_state)
 
 
 def head_bce(hd, W, b, labels):

@@ -33,7 +33,7 @@ enum {
   BPC_ERR_SPACE = 6     /* the workspace is smaller than bpc_predecoder_workspace_size() */
 };
 
-/* BPC_DTYPE_F16: the embedding lookup, its gradient and the gradient norm only. */
+/* BPC_DTYPE_F16: the embedding lookup, its gradient, the gradient norm and the group norm only. */
 enum { BPC_DTYPE_F32 = 0, BPC_DTYPE_BF16 = 1, BPC_DTYPE_F16 = 2 };
 
 /* Library version, (major << 16) | minor. */
@@ -156,6 +156,60 @@ BPC_API size_t bpc_embed_wgrad_workspace_size(int64_t n, int32_t V, int32_t C);
 BPC_API int bpc_embed_wgrad(const void* gy, const void* ids, int32_t id_bytes, void* dw, void* workspace,
                             size_t workspace_bytes, int64_t n, int32_t V, int32_t C, int64_t gy_stride, float scale,
                             int32_t gy_dtype, int32_t dw_dtype, bpc_stream_t stream);
+
+/* Group normalisation with an activation over channels-last features, and its gradients (the per-sample counterpart of
+ * the BatchNorm + SiLU in front of the Cascade block's layers, cascade_net.py:195-210,236-259):
+ *   x (B, N, C), group g = channels [g C / G, (g + 1) C / G); mean and variance (of the population) over the N C / G values
+ *   of a sample and group;  xh = (x - mean) / sqrt(var + eps);  z = weight_c xh + bias_c;  y = act(z)
+ *   act: BPC_ACT_NONE z; BPC_ACT_SILU z / (1 + e^-z); BPC_ACT_GELU z / (1 + e^-2u), u = sqrt(2 / pi) (z + 0.044715 z^3)
+ *   backward: dx, dw, db of sum(gy * y)
+ * x: samples x_sample_stride and rows x_row_stride elements apart, channels contiguous, f32, bf16 or f16; y (B, N, C)
+ * contiguous, x's type or, for f32 x, a narrower one; mean, rstd (B, G) fp32: written by the forward pass (either may be
+ * NULL), read by the backward pass; weight, bias (C) fp32 or NULL (1, 0).  gy: y's type, any strides as x; dx (B, N, C)
+ * contiguous, x's type; dw, db (C) fp32; NULL where a gradient is not wanted.  Statistics and sums are fp32 or wider, in
+ * a fixed order (deterministic), each result rounded once.  C <= 2^20; every buffer aligned to its type.  workspace:
+ * bpc_group_norm_workspace_size() bytes on the current device, 16-byte aligned. */
+enum { BPC_ACT_NONE = 0, BPC_ACT_SILU = 1, BPC_ACT_GELU = 2 };
+BPC_API size_t bpc_group_norm_workspace_size(int64_t B, int64_t N, int32_t C, int32_t G, int32_t backward);
+BPC_API int bpc_group_norm_fwd(const void* x, void* y, float* mean, float* rstd, const float* weight, const float* bias,
+                               int64_t B, int64_t N, int32_t C, int32_t G, int64_t x_sample_stride, int64_t x_row_stride,
+                               float eps, int32_t activation, int32_t x_dtype, int32_t y_dtype, void* workspace,
+                               size_t workspace_bytes, bpc_stream_t stream);
+BPC_API int bpc_group_norm_bwd(const void* gy, const void* x, const float* mean, const float* rstd, const float* weight,
+                               const float* bias, void* dx, float* dw, float* db, int64_t B, int64_t N, int32_t C, int32_t G,
+                               int64_t gy_sample_stride, int64_t gy_row_stride, int64_t x_sample_stride,
+                               int64_t x_row_stride, int32_t activation, int32_t x_dtype, int32_t y_dtype, void* workspace,
+                               size_t workspace_bytes, bpc_stream_t stream);
+
+/* Linear attention with a decay for each head: a memory over the rounds of an experiment (no reference counterpart: the
+ * reference's networks see a fixed window of rounds).
+ *   S_t = a_h S_(t-1) + k_t v_t^T;  o_t = scale q_t S_t;  a_h = exp(log_decay_h),  t = 0 .. length_b - 1
+ *   bpc_linear_attention_fwd   whole sequences: o, and the state after the last position (new_state, or NULL)
+ *   bpc_linear_attention_bwd   dq, dk, dv (and dstate, or NULL) of sum(go * o) + sum(grad_state * new_state)
+ *   bpc_linear_attention_step  one position: new_state = a state + k v^T, o = scale q new_state
+ * q, k (B, T, H, dk), v, go (B, T, H, dv): f32 or bf16, head rows contiguous, strides: a host array of (batch, position,
+ * head) element strides for q, k, v (and go) in turn, 0 where broadcast; for the step q, k (B, H, dk), v (B, H, dv) and
+ * (batch, head) strides.  o, dv like v, dq, dk like q, contiguous, of the inputs' type.  log_decay (H) fp32, -infinity
+ * forgets everything; no gradient of it is formed.  state, new_state, grad_state, dstate (B, H, dk, dv) fp32, 16-byte
+ * aligned (4-byte for the step); a NULL state or grad_state is zero.  lengths (B) int32 or int64 (length_bytes 4 or 8) or NULL (T each): positions
+ * at or behind a sequence's length are not read, and zero in o, dq, dk and dv.  1 <= dk, dv <= 128, B H < 2^31.  States,
+ * products and sums are fp32, in a fixed order (deterministic).  new_state may be the state itself, else they do not
+ * overlap.  workspace: bpc_linear_attention_workspace_size() bytes on the current device, 16-byte aligned. */
+BPC_API size_t bpc_linear_attention_workspace_size(int64_t B, int64_t T, int32_t H, int32_t dk, int32_t dv, int32_t dtype,
+                                                   int32_t backward);
+BPC_API int bpc_linear_attention_fwd(const void* q, const void* k, const void* v, void* o, const float* log_decay,
+                                     const float* state, float* new_state, const void* lengths, int32_t length_bytes,
+                                     int64_t B, int64_t T, int32_t H, int32_t dk, int32_t dv, const int64_t* strides,
+                                     float scale, int32_t dtype, void* workspace, size_t workspace_bytes,
+                                     bpc_stream_t stream);
+BPC_API int bpc_linear_attention_bwd(const void* q, const void* k, const void* v, const void* go, const float* log_decay,
+                                     const float* state, const float* grad_state, const void* lengths,
+                                     int32_t length_bytes, void* dq, void* dk_out, void* dv_out, float* dstate, int64_t B,
+                                     int64_t T, int32_t H, int32_t dk, int32_t dv, const int64_t* strides, float scale,
+                                     int32_t dtype, void* workspace, size_t workspace_bytes, bpc_stream_t stream);
+BPC_API int bpc_linear_attention_step(const void* q, const void* k, const void* v, void* o, const float* log_decay,
+                                      const float* state, float* new_state, int64_t B, int32_t H, int32_t dk, int32_t dv,
+                                      const int64_t* strides, float scale, int32_t dtype, bpc_stream_t stream);
 
 /* The 2-norm over every element of a list of n tensors, and clipping the list by it (the gradient clipping of the
  * reference's training step, cascade_train.py:292-320):
