@@ -3,12 +3,17 @@
 //
 //   S_t = a S_(t-1) + k_t v_t^T,   o_t = scale q_t S_t   (a = exp(log_decay_h) per head, S (dk, dv), q, k, v rows)
 //
-// Forward and every gradient are one scan over rows a_t, b_t, c_t and a state X:
+// Forward and every gradient are one scan over rows a_t, b_t, c_t and a state X (da, dc):
 //   S = X + in b_t c_t^T;   out_t = out_scale a_t S;   X = a S
 //   forward  a, b, c = q, k, v     X = a S_0             out_scale = scale      the last S is the new state
 //   dq       a, b, c = go, v, k    X = a S_0^T           out_scale = scale
 //   dk       a, b, c = v, go, q    X = gS^T, in = scale  backwards in time      (gS: the gradient of the new state)
 //   dv       a, b, c = k, q, go    X = gS, in = scale    backwards in time      a times the last S is dS_0
+// A step of the scan takes 32 positions (a chunk) as products of matrices.  With pos the position in the chunk in the
+// scan's order, 0 .. r - 1 of r:
+//   out_i = out_scale (sum_(pos j <= pos i) in a^(pos i - pos j) (a_i . b_j) c_j + a^(pos i) a_i X)
+//   X     = a^r X + sum_j in a^(r - pos j) b_j c_j^T
+#include <algorithm>
 #include <cmath>
 #include <string>
 
@@ -22,6 +27,8 @@ namespace {
 
 constexpr int kThreads = 128;
 constexpr int kMaxDim = 128;
+constexpr int kChunk = 32;
+constexpr int kShort = 16;        // positions that short_kernel takes
 
 __device__ __forceinline__ float load_f32(const float* p) { return *p; }
 __device__ __forceinline__ float load_f32(const __nv_bfloat16* p) { return __bfloat162float(*p); }
@@ -40,60 +47,865 @@ struct Scan {
   const float* log_decay;
   const float* first;           // X before its decay: (B, H, da, dc), or (B, H, dc, da) where first_t
   float* last;                  // (B, H, da, dc), or null
+  float* parts;                 // the segments' states: (B H, segments - 1, DP DP) in the order of the warps' registers
   const void* lengths;
   int length_bytes;
-  int64_t B, T;
-  int H, da, dc;
+  int T, H, da, dc;
+  int segments, segment;        // rows per segment, a multiple of kChunk
+  uint32_t items;               // B H segments
   float in_scale, out_scale;
-  bool reverse, first_t;
+  bool reverse, first_t, vec, out_vec;
 };
 
-__device__ __forceinline__ int64_t length_of(const void* lengths, int bytes, int64_t b, int64_t T) {
+__device__ __forceinline__ int length_of(const void* lengths, int bytes, uint32_t b, int T) {
   if (!lengths) return T;
   const int64_t n = bytes == 8 ? static_cast<const int64_t*>(lengths)[b] : static_cast<const int32_t*>(lengths)[b];
-  return n < 0 ? 0 : n > T ? T : n;
+  return n < 0 ? 0 : n > T ? T : static_cast<int>(n);
 }
 
-// One block per sequence and head, a thread per column of the state, which stays in shared memory.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) scan_kernel(const Scan p) {
-  extern __shared__ float S[];                          // (da, kThreads)
-  __shared__ float ra[kMaxDim], rb[kMaxDim];
-  const int64_t at = blockIdx.x, b = at / p.H;
-  const int h = static_cast<int>(at % p.H), j = threadIdx.x;
-  const int64_t n = length_of(p.lengths, p.length_bytes, b, p.T);
-  const float a = expf(p.log_decay[h]);
-  T* out = static_cast<T*>(p.out) + (b * p.T * p.H + h) * p.dc;
-  const int64_t row = static_cast<int64_t>(p.H) * p.dc;
-  const float* first = p.first ? p.first + at * p.da * p.dc : nullptr;
-  const float lead = p.reverse || n == 0 ? 1.0f : a;
-  for (int i = 0; i < p.da; ++i)
-    S[i * kThreads + j] = first && j < p.dc ? lead * first[p.first_t ? j * p.da + i : i * p.dc + j] : 0.0f;
-  for (int64_t k = 0; k < n; ++k) {
-    const int64_t t = p.reverse ? n - 1 - k : k;
-    __syncthreads();
-    if (j < p.da) {
-      ra[j] = load_f32(static_cast<const T*>(p.a.at) + b * p.a.b + t * p.a.t + h * p.a.h + j);
-      rb[j] = load_f32(static_cast<const T*>(p.b.at) + b * p.b.b + t * p.b.t + h * p.b.h + j);
+// a^n of log2 a, 1 for n = 0 whatever a is (log_decay may be -infinity), 0 for n < 0 (a pair out of order)
+__device__ __forceinline__ float log2_decay(const float* log_decay, int h) { return log_decay[h] * 1.4426950408889634f; }
+__device__ __forceinline__ float power(float log2_a, int n) {
+  float v;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(v) : "f"(log2_a * static_cast<float>(n)));
+  return n > 0 ? v : n == 0 ? 1.0f : 0.0f;
+}
+
+// ---- fragments -------------------------------------------------------------------------------------------------
+// mma.sync m16n8k16 (bf16) and m16n8k8 (tf32), fp32 accumulators.  Lane 4 g + t holds of the result rows g, g + 8 and
+// columns 2 t, 2 t + 1.  The tf32 products number their k so that lane t's two values are columns 2 t and 2 t + 1 of
+// the row-major operand: then an accumulator is an operand of the next product as it stands, and a bf16 operand is one of
+// a tf32 product by taking its halves apart.
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldmatrix(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(at)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix_trans(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(at)
+               : "memory");
+}
+__device__ __forceinline__ float lds(uint32_t at) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 lds2(uint32_t at) {
+  float2 v;
+  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t pack(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ float low(uint32_t p) { return __uint_as_float(p << 16); }
+__device__ __forceinline__ float high(uint32_t p) { return __uint_as_float(p & 0xffff0000u); }
+
+// x to the nearest tf32 (11 significant bits), with bits behind them that a product does not read
+__device__ __forceinline__ uint32_t tf32(float x) { return __float_as_uint(x) + 0x1000u; }
+// x = hi + lo in tf32, but for 2^-23 of x
+struct Split {
+  uint32_t hi, lo;
+  __device__ __forceinline__ explicit Split(float x) {
+    hi = tf32(x) & 0xffffe000u;
+    lo = tf32(x - __uint_as_float(hi));
+  }
+  Split() = default;
+};
+// d += a b in fp32's precision: three tf32 products leave out the product of the two small parts
+__device__ __forceinline__ void mma_f32(float (&d)[4], const Split (&a)[4], const Split& b0, const Split& b1) {
+  const uint32_t hi[4] = {a[0].hi, a[1].hi, a[2].hi, a[3].hi}, lo[4] = {a[0].lo, a[1].lo, a[2].lo, a[3].lo};
+  mma_tf32(d, lo, b0.hi, b1.hi);
+  mma_tf32(d, hi, b0.lo, b1.lo);
+  mma_tf32(d, hi, b0.hi, b1.hi);
+}
+
+// ---- tiles -----------------------------------------------------------------------------------------------------
+// 32 rows of DP elements in shared memory.  bf16: 16-byte pieces XORed with the row, so that ldmatrix reads without bank
+// conflicts; fp32: rows padded by 16 bytes, so that a lane's reads of four rows and eight columns do.
+template <typename T, int DP>
+struct Tile {
+  static constexpr bool kF32 = sizeof(T) == 4;
+  static constexpr int kCols = DP == 16 || DP == 128 ? 16 : 32;      // of c, per warp: a state of at most 64 values a lane
+  static constexpr int kWarps = DP / kCols;                          // of a group, which takes an item
+  static constexpr int kThreads = kWarps < 4 ? 128 : 32 * kWarps;
+  static constexpr int kGroups = kThreads / 32 / kWarps;
+  static constexpr int kMT = kCols / 16;
+  static constexpr int kNT = DP / 8;                                 // 8-column pieces of a, b
+  static constexpr int kRegs = kMT * kNT * 4;
+  static constexpr int kPitch = kF32 ? (DP + 4) * 4 : DP * 2;
+  static constexpr int kBytes = kChunk * kPitch;
+  static constexpr int kPiece = 16 / sizeof(T);
+  static constexpr int kPieces = DP / kPiece;                        // per row
+  static constexpr int kStages = kF32 ? 2 : 3;
+  static constexpr int kOutBytes = kF32 ? 0 : 16 * kCols * 2;        // a warp's rows on their way out
+  static constexpr int kSmem = kGroups * kStages * 3 * kBytes + kGroups * kWarps * kOutBytes;
+  __device__ static __forceinline__ uint32_t at(int row, int piece) {
+    if constexpr (kF32) return row * kPitch + piece * 16;
+    else return row * kPitch + ((piece ^ (DP == 16 ? row >> 2 & 1 : DP == 32 ? row >> 1 & 3 : row & 7)) << 4);
+  }
+};
+
+__device__ __forceinline__ void cp_async(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Rows [0, rows) of `src` (row stride in elements) into a tile, zeros behind them and behind dim; by one group of warps
+template <typename T, int DP>
+__device__ __forceinline__ void load_tile(uint32_t tile, const T* src, int64_t stride, int rows, int dim, bool vec, int lane) {
+  using L = Tile<T, DP>;
+  constexpr int kLanes = 32 * L::kWarps;
+  if (vec) {
+#pragma unroll
+    for (int k = 0; k < kChunk * L::kPieces / kLanes; ++k) {
+      const int e = k * kLanes + lane, row = e / L::kPieces, piece = e % L::kPieces;
+      const bool there = row < rows && piece * L::kPiece < dim;
+      cp_async(tile + L::at(row, piece), there ? src + row * stride + piece * L::kPiece : src, there ? 16 : 0);
     }
-    __syncthreads();
-    if (j < p.dc) {
-      const float c = p.in_scale * load_f32(static_cast<const T*>(p.c.at) + b * p.c.b + t * p.c.t + h * p.c.h + j);
-      const float keep = k ? a : 1.0f;
-      float o = 0.0f;
-      for (int i = 0; i < p.da; ++i) {
-        const float s = fmaf(rb[i], c, keep * S[i * kThreads + j]);
-        S[i * kThreads + j] = s;
-        o = fmaf(ra[i], s, o);
-      }
-      store_f32(out + t * row + j, p.out_scale * o);
+  } else {
+    for (int e = lane; e < kChunk * DP; e += kLanes) {
+      const int row = e / DP, col = e % DP;
+      const T v = row < rows && col < dim ? src[row * stride + col] : T(0.0f);
+      const uint32_t dst = tile + L::at(row, col / L::kPiece) + col % L::kPiece * sizeof(T);
+      if constexpr (L::kF32) asm volatile("st.shared.f32 [%0], %1;" ::"r"(dst), "f"(v) : "memory");
+      else asm volatile("st.shared.u16 [%0], %1;" ::"r"(dst), "h"(__bfloat16_as_ushort(v)) : "memory");
     }
   }
-  if (j < p.dc) {
-    for (int64_t t = n; t < p.T; ++t) store_f32(out + t * row + j, 0.0f);
-    if (p.last)
-      for (int i = 0; i < p.da; ++i)
-        p.last[(at * p.da + i) * p.dc + j] = (p.reverse && n ? a : 1.0f) * S[i * kThreads + j];
+}
+
+// ---- a chunk ---------------------------------------------------------------------------------------------------
+// A chunk is worked on in halves of 16 rows, in the scan's order: half 0 is the rows 0 - 15 forwards, 16 - 31 backwards (where
+// the chunk has more than 16 rows).  A lane's weights: of pairs of positions whose 8-row pieces are D = 0 .. 3 apart in
+// the scan's order (columns 2 t, 2 t + 1 of them); of the state for rows g, g + 8 of a half; of c's rows 2 t, 2 t + 1, 2 t + 8,
+// 2 t + 9 of a half in the state's update; of the state there.
+struct Weights {
+  float pair[4][2], row[2][2], update[2][4], keep;
+  int halves, flip;             // flip: half 0 is rows 16 - 31
+
+  // r: the chunk's rows; until: the position as of which the state is wanted, r or (as of the last one) r - 1
+  __device__ __forceinline__ void of_pairs(float log2_a, float in, bool reverse) {
+    const int lane = threadIdx.x & 31, e0 = (lane >> 2) - 2 * (lane & 3);
+#pragma unroll
+    for (int D = 0; D < 4; ++D)
+#pragma unroll
+      for (int z = 0; z < 2; ++z) pair[D][z] = in * power(log2_a, 8 * D + (reverse ? z - e0 : e0 - z));
+  }
+  __device__ __forceinline__ void of_rows(float log2_a, float in, bool reverse, int r, int until) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    halves = r > 16 ? 2 : 1;
+    flip = reverse && halves == 2;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int row0 = (flip ? 1 - h : h) * 16;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) row[h][k] = power(log2_a, reverse ? r - 1 - (row0 + g + 8 * k) : row0 + g + 8 * k);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int j = row0 + 2 * t + (k & 1) + (k >> 1) * 8;
+        update[h][k] = in * power(log2_a, until - (reverse ? r - 1 - j : j));
+      }
+    }
+    keep = power(log2_a, until);
+  }
+  __device__ __forceinline__ float of(int i_half, int j_half, int i, int j, int z, bool reverse) const {
+    const int D = 2 * (i_half - j_half) + (reverse ? j - i : i - j);
+    return D < 0 ? 0.0f : pair[D][z];
+  }
+};
+
+template <typename T, int DP>
+struct Warp {
+  using L = Tile<T, DP>;
+  static constexpr int kMT = L::kMT, kNT = L::kNT;
+  float X[kMT][kNT][4];         // X^T: rows = this warp's columns of c, columns = those of a, b
+
+  // O (16 positions x this warp's columns of c, for each half), and X after the chunk.  SPLIT: bf16 parts of the weighted c.
+  template <bool OUT, int SPLIT>
+  __device__ __forceinline__ void chunk(uint32_t sa, uint32_t sb, uint32_t sc, int slice, const Weights& w, bool reverse,
+                                        bool use_x, bool update, float (&O)[2][2 * kMT][4]) {
+    if constexpr (L::kF32) chunk_f32<OUT>(sa, sb, sc, slice, w, reverse, use_x, update, O);
+    else chunk_bf16<OUT, SPLIT>(sa, sb, sc, slice, w, reverse, use_x, update, O);
+  }
+
+  // What is fp32 and an operand of a bf16 product (the weighted a b^T, X, the weighted c) goes in as two bf16 parts, off by
+  // at most 2^-18 of itself; one part would round as coarsely as the result.  Where a state is handed out, c as three.
+  template <bool OUT, int SPLIT>
+  __device__ __forceinline__ void chunk_bf16(uint32_t sa, uint32_t sb, uint32_t sc, int slice, const Weights& w, bool reverse,
+                                             bool use_x, bool update, float (&O)[2][2 * kMT][4]) {
+    constexpr int kKS = DP / 16;
+    const int lane = threadIdx.x & 31;
+    // addresses of a lane's row in four 8 x 8 pieces: row lane % 16 and column piece lane / 16, or (b as the second
+    // operand of a b^T) row lane % 8 + 8 (lane / 16) and column piece lane / 8 % 2; the next 16 columns are an XOR by 32
+    const uint32_t by_row = L::at(lane & 15, lane >> 4), by_piece = L::at((lane & 7) + (lane >> 4) * 8, lane >> 3 & 1);
+    const uint32_t half[2] = {w.flip ? 16u * L::kPitch : 0u, w.flip ? 0u : 16u * L::kPitch};
+    const bool two = w.halves == 2;
+    uint32_t c[2][kMT][4];
+    {
+      const uint32_t c0 = L::at(lane & 15, slice * (L::kCols / 8) + (lane >> 4));
+#pragma unroll
+      for (int m = 0; m < kMT; ++m) ldmatrix_trans(c[0][m], sc + half[0] + (c0 ^ (m << 5)));
+      if (two) {
+#pragma unroll
+        for (int m = 0; m < kMT; ++m) ldmatrix_trans(c[1][m], sc + half[1] + (c0 ^ (m << 5)));
+      }
+    }
+    if constexpr (OUT) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int n = 0; n < 2 * kMT; ++n) O[h][n][0] = O[h][n][1] = O[h][n][2] = O[h][n][3] = 0.0f;
+      float P[3][2][4] = {};                       // halves (0, 0), (1, 0), (1, 1)
+#pragma unroll
+      for (int k = 0; k < kKS; ++k) {
+        uint32_t a[2][4], b[4];
+        ldmatrix(a[0], sa + half[0] + (by_row ^ (k << 5)));
+        ldmatrix(b, sb + half[0] + (by_piece ^ (k << 5)));
+        mma_bf16(P[0][0], a[0], b[0], b[1]);
+        mma_bf16(P[0][1], a[0], b[2], b[3]);
+        if (two) {
+          ldmatrix(a[1], sa + half[1] + (by_row ^ (k << 5)));
+          mma_bf16(P[1][0], a[1], b[0], b[1]);
+          mma_bf16(P[1][1], a[1], b[2], b[3]);
+          ldmatrix(b, sb + half[1] + (by_piece ^ (k << 5)));
+          mma_bf16(P[2][0], a[1], b[0], b[1]);
+          mma_bf16(P[2][1], a[1], b[2], b[3]);
+        }
+        if (use_x) {
+#pragma unroll
+          for (int n = 0; n < 2 * kMT; ++n) {
+            uint32_t hi[2], lo[2];
+#pragma unroll
+            for (int z = 0; z < 2; ++z) {
+              const float x0 = X[n / 2][2 * k + z][2 * (n % 2)], x1 = X[n / 2][2 * k + z][2 * (n % 2) + 1];
+              hi[z] = pack(x0, x1);
+              lo[z] = pack(x0 - low(hi[z]), x1 - high(hi[z]));
+            }
+            mma_bf16(O[0][n], a[0], lo[0], lo[1]);
+            mma_bf16(O[0][n], a[0], hi[0], hi[1]);
+            if (two) {
+              mma_bf16(O[1][n], a[1], lo[0], lo[1]);
+              mma_bf16(O[1][n], a[1], hi[0], hi[1]);
+            }
+          }
+        }
+      }
+      if (use_x) weigh_rows(w, O);
+#pragma unroll
+      for (int block = 0; block < 3; ++block) {
+        const int i_half = block > 0, j_half = block > 1;
+        if (block == 0 || two) {
+          uint32_t hi[4], lo[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {            // (rows g, columns of piece 0), (g + 8, 0), (g, 1), (g + 8, 1)
+            const int r = e & 1, n = e >> 1;
+            const float p0 = weighed(P[block][n][2 * r], w.of(i_half, j_half, r, n, 0, reverse));
+            const float p1 = weighed(P[block][n][2 * r + 1], w.of(i_half, j_half, r, n, 1, reverse));
+            hi[e] = pack(p0, p1);
+            lo[e] = pack(p0 - low(hi[e]), p1 - high(hi[e]));
+          }
+#pragma unroll
+          for (int n = 0; n < 2 * kMT; ++n) {
+            const uint32_t b0 = c[j_half][n / 2][2 * (n % 2)], b1 = c[j_half][n / 2][2 * (n % 2) + 1];
+            mma_bf16(O[i_half][n], lo, b0, b1);
+            mma_bf16(O[i_half][n], hi, b0, b1);
+          }
+        }
+      }
+    }
+    if (update) {
+      uint32_t wc[2][SPLIT][kMT][4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (h == 0 || two) {
+#pragma unroll
+          for (int m = 0; m < kMT; ++m)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {          // c's pieces: (positions 0-7, columns 0-7), (8-15, 0-7), (0-7, 8-15), (8-15, 8-15)
+              const int to = (e & 1) * 2 + (e >> 1);         // their places in the transposed first operand
+              float x0 = low(c[h][m][e]) * w.update[h][2 * (e & 1)], x1 = high(c[h][m][e]) * w.update[h][2 * (e & 1) + 1];
+#pragma unroll
+              for (int s = 0; s < SPLIT; ++s) {
+                wc[h][s][m][to] = pack(x0, x1);
+                x0 -= low(wc[h][s][m][to]), x1 -= high(wc[h][s][m][to]);
+              }
+            }
+        }
+#pragma unroll
+      for (int k = 0; k < kKS; ++k) {
+        uint32_t b[2][4];
+        ldmatrix_trans(b[0], sb + half[0] + (by_row ^ (k << 5)));
+        if (two) ldmatrix_trans(b[1], sb + half[1] + (by_row ^ (k << 5)));
+#pragma unroll
+        for (int m = 0; m < kMT; ++m)
+#pragma unroll
+          for (int z = 0; z < 2; ++z) {
+            float u[4] = {};
+#pragma unroll
+            for (int s = SPLIT - 1; s >= 0; --s) mma_bf16(u, wc[0][s][m], b[0][2 * z], b[0][2 * z + 1]);
+            if (two) {
+#pragma unroll
+              for (int s = SPLIT - 1; s >= 0; --s) mma_bf16(u, wc[1][s][m], b[1][2 * z], b[1][2 * z + 1]);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) X[m][2 * k + z][e] = fmaf(w.keep, X[m][2 * k + z][e], u[e]);
+          }
+      }
+    }
+  }
+
+  // a pair out of order is dropped, not multiplied by zero
+  __device__ static __forceinline__ float weighed(float p, float w) { return w == 0.0f ? 0.0f : p * w; }
+
+  __device__ static __forceinline__ void weigh_rows(const Weights& w, float (&O)[2][2 * kMT][4]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int n = 0; n < 2 * kMT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) O[h][n][e] *= w.row[h][e >> 1];
+  }
+
+  template <bool OUT>
+  __device__ __forceinline__ void chunk_f32(uint32_t sa, uint32_t sb, uint32_t sc, int slice, const Weights& w, bool reverse,
+                                            bool use_x, bool update, float (&O)[2][2 * kMT][4]) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const uint32_t half[2] = {w.flip ? 16u * L::kPitch : 0u, w.flip ? 0u : 16u * L::kPitch};
+    const bool two = w.halves == 2;
+    const uint32_t pair_at = g * L::kPitch + t * 8;              // (row g, columns 2 t, 2 t + 1)
+    const uint32_t cross_at = 2 * t * L::kPitch + g * 4;         // (rows 2 t and the next, column g)
+    const uint32_t c0 = sc + cross_at + slice * (L::kCols * 4);
+    if constexpr (OUT) {
+      float P[3][2][4] = {};                       // halves (0, 0), (1, 0), (1, 1)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int n = 0; n < 2 * kMT; ++n) O[h][n][0] = O[h][n][1] = O[h][n][2] = O[h][n][3] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kNT; ++k) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          if (h == 0 || two) {
+            const float2 a0 = lds2(sa + half[h] + pair_at + k * 32), a1 = lds2(sa + half[h] + pair_at + 8 * L::kPitch + k * 32);
+            const Split a[4] = {Split(a0.x), Split(a1.x), Split(a0.y), Split(a1.y)};
+#pragma unroll
+            for (int j = 0; j <= h; ++j)
+#pragma unroll
+              for (int n = 0; n < 2; ++n) {
+                const float2 b = lds2(sb + half[j] + pair_at + n * 8 * L::kPitch + k * 32);
+                mma_f32(P[h + j][n], a, Split(b.x), Split(b.y));
+              }
+            if (use_x) {
+#pragma unroll
+              for (int n = 0; n < 2 * kMT; ++n)
+                mma_f32(O[h][n], a, Split(X[n / 2][k][2 * (n % 2)]), Split(X[n / 2][k][2 * (n % 2) + 1]));
+            }
+          }
+      }
+      if (use_x) weigh_rows(w, O);
+#pragma unroll
+      for (int block = 0; block < 3; ++block) {
+        const int i_half = block > 0, j_half = block > 1;
+        if (block == 0 || two) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {            // 8 positions j at a time
+            Split p[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)            // (g, 2 t), (g + 8, 2 t), (g, 2 t + 1), (g + 8, 2 t + 1)
+              p[e] = Split(weighed(P[block][k][2 * (e & 1) + (e >> 1)], w.of(i_half, j_half, e & 1, k, e >> 1, reverse)));
+            const uint32_t at = c0 + half[j_half] + k * 8 * L::kPitch;
+#pragma unroll
+            for (int n = 0; n < 2 * kMT; ++n)
+              mma_f32(O[i_half][n], p, Split(lds(at + n * 32)), Split(lds(at + L::kPitch + n * 32)));
+          }
+        }
+      }
+    }
+    if (update) {
+#pragma unroll
+      for (int m = 0; m < kMT; ++m) {
+        float u[kNT][4] = {};
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          if (h == 0 || two) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const uint32_t rows = half[h] + k * 8 * L::kPitch;
+              Split wc[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e)          // (column g, 2 t), (g + 8, 2 t), (g, 2 t + 1), (g + 8, 2 t + 1)
+                wc[e] = Split(w.update[h][2 * k + (e >> 1)] * lds(c0 + rows + (e >> 1) * L::kPitch + (2 * m + (e & 1)) * 32));
+#pragma unroll
+              for (int n = 0; n < kNT; ++n)
+                mma_f32(u[n], wc, Split(lds(sb + rows + cross_at + n * 32)), Split(lds(sb + rows + cross_at + L::kPitch + n * 32)));
+            }
+          }
+#pragma unroll
+        for (int n = 0; n < kNT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) X[m][n][e] = fmaf(w.keep, X[m][n][e], u[n][e]);
+      }
+    }
+  }
+
+  // f(value of X at (row of c's columns, column of a's), index) over a lane's values
+  template <typename F>
+  __device__ __forceinline__ void each(int slice, F f) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int m = 0; m < kMT; ++m)
+#pragma unroll
+      for (int n = 0; n < kNT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          f(X[m][n][e], n * 8 + 2 * (lane & 3) + (e & 1), slice * L::kCols + m * 16 + (lane >> 2) + (e >> 1) * 8, (m * kNT + n) * 4 + e);
+  }
+};
+
+// ---- an item: a sequence's head, or one segment of it ------------------------------------------------------------
+struct Item {
+  uint32_t b;
+  int h, segment, n;            // n: the sequence's length
+  int row0, rows;               // its first row, its valid rows
+  int steps;                    // chunks with valid rows, one at least
+  __device__ __forceinline__ Item(const Scan& p, uint32_t at) {
+    const uint32_t rest = at / p.H;
+    h = static_cast<int>(at - rest * p.H);
+    b = p.segments > 1 ? rest / p.segments : rest;
+    segment = p.segments > 1 ? static_cast<int>(rest - b * p.segments) : 0;
+    n = length_of(p.lengths, p.length_bytes, b, p.T);
+    row0 = segment * p.segment;
+    const int left = n - row0;
+    rows = left < 0 ? 0 : left > p.segment ? p.segment : left;
+    steps = rows ? (rows + kChunk - 1) / kChunk : 1;
+  }
+  __device__ __forceinline__ int chunk(bool reverse, int step) const { return reverse ? steps - 1 - step : step; }
+  __device__ __forceinline__ int valid(int c) const { return rows - c * kChunk < kChunk ? rows - c * kChunk : kChunk; }
+};
+
+template <typename T>
+__device__ __forceinline__ const T* row_of(const Rows& r, const Item& it, int row) {
+  return static_cast<const T*>(r.at) + it.b * r.b + row * r.t + it.h * r.h;
+}
+
+// 16 rows of a warp's output columns, zeros from row `rows` on; rows behind `until` stay
+template <typename T, int DP>
+__device__ __forceinline__ void store_rows(T* out, int64_t stride, const float (&O)[2 * Tile<T, DP>::kMT][4], int slice, int rows,
+                                           int until, int dc, float scale, bool vec, uint32_t stage) {
+  using L = Tile<T, DP>;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  constexpr int kCols = L::kCols;
+  out += slice * kCols;
+  dc -= slice * kCols;
+  if (!vec) {
+#pragma unroll
+    for (int n = 0; n < 2 * L::kMT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int row = g + (e >> 1) * 8, col = n * 8 + 2 * t + (e & 1);
+        if (row < until && col < dc) store_f32(out + row * stride + col, row < rows ? scale * O[n][e] : 0.0f);
+      }
+  } else if constexpr (L::kF32) {
+#pragma unroll
+    for (int n = 0; n < 2 * L::kMT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int row = g + e * 8, col = n * 8 + 2 * t;
+        if (row < until && col < dc)
+          *reinterpret_cast<float2*>(out + row * stride + col) =
+              row < rows ? make_float2(scale * O[n][2 * e], scale * O[n][2 * e + 1]) : make_float2(0.0f, 0.0f);
+      }
+  } else {
+    // through shared memory: whole rows of 64 (32) bytes, of which a quad alone has 16
+    __syncwarp();
+#pragma unroll
+    for (int n = 0; n < 2 * L::kMT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int row = g + e * 8;
+        const uint32_t v = row < rows ? pack(scale * O[n][2 * e], scale * O[n][2 * e + 1]) : 0u;
+        asm volatile("st.shared.u32 [%0], %1;" ::"r"(stage + row * kCols * 2 + ((n ^ (row >> 1 & (2 * L::kMT - 1))) << 4) + t * 4), "r"(v)
+                     : "memory");
+      }
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < L::kMT; ++k) {
+      const int e = k * 32 + lane, row = e / (2 * L::kMT), n = e % (2 * L::kMT);
+      uint4 v;
+      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                   : "r"(stage + row * kCols * 2 + ((n ^ (row >> 1 & (2 * L::kMT - 1))) << 4))
+                   : "memory");
+      if (row < until && n * 8 < dc) *reinterpret_cast<uint4*>(out + row * stride + n * 8) = v;
+    }
+  }
+}
+
+// Rows [from, to) of a warp's output columns become zero
+template <typename T, int DP>
+__device__ __forceinline__ void zero_rows(T* out, int64_t stride, int slice, int from, int to, int dc) {
+  const int lane = threadIdx.x & 31, first = slice * Tile<T, DP>::kCols;
+  if (lane >= min(dc - first, Tile<T, DP>::kCols)) return;
+  for (int row = from; row < to; ++row) store_f32(out + row * stride + first + lane, 0.0f);
+}
+
+// A group of warps takes an item at a time, chunk by chunk, each warp some columns of c; the state stays in the warps'
+// registers.  The tiles of the next chunks, of the next items too, are on their way meanwhile.
+// OUT false: the states that the segments leave behind alone.
+template <typename T, int DP, bool OUT, int SPLIT>
+__global__ void __launch_bounds__(Tile<T, DP>::kThreads) scan_kernel(const __grid_constant__ Scan p) {
+  using L = Tile<T, DP>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  constexpr int kS = L::kStages;
+  const int warp = threadIdx.x >> 5, group = warp / L::kWarps, slice = warp % L::kWarps;
+  const int lane_in_group = threadIdx.x - group * (32 * L::kWarps), lane = threadIdx.x & 31;
+  const uint32_t base = smem_u32(smem) + group * (kS * 3 * L::kBytes);
+  const uint32_t stage_out = smem_u32(smem) + L::kGroups * (kS * 3 * L::kBytes) + warp * L::kOutBytes;
+  const uint32_t first_item = blockIdx.x * L::kGroups + group, stride = gridDim.x * L::kGroups;
+  auto sync = [&] {
+    if constexpr (L::kWarps == 1) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(32 * L::kWarps) : "memory");
+  };
+
+  uint32_t ahead_at = first_item;                  // the loads' item and step
+  int ahead_step = 0, ahead_slot = 0;
+  Item ahead(p, ahead_at < p.items ? ahead_at : 0);
+  auto load = [&] {
+    if (ahead_at < p.items) {
+      const int c = ahead.chunk(p.reverse, ahead_step), row = ahead.row0 + c * kChunk, r = ahead.valid(c);
+      const uint32_t tile = base + ahead_slot * (3 * L::kBytes);
+      if constexpr (OUT) load_tile<T, DP>(tile, row_of<T>(p.a, ahead, row), p.a.t, r, p.da, p.vec, lane_in_group);
+      load_tile<T, DP>(tile + L::kBytes, row_of<T>(p.b, ahead, row), p.b.t, r, p.da, p.vec, lane_in_group);
+      load_tile<T, DP>(tile + 2 * L::kBytes, row_of<T>(p.c, ahead, row), p.c.t, r, p.dc, p.vec, lane_in_group);
+      if (++ahead_step == ahead.steps) {
+        ahead_step = 0;
+        ahead_at += stride;
+        if (ahead_at < p.items) ahead = Item(p, ahead_at);
+      }
+    }
+    ahead_slot = ahead_slot + 1 == kS ? 0 : ahead_slot + 1;
+    cp_commit();
+  };
+#pragma unroll
+  for (int s = 0; s < kS - 1; ++s) load();
+
+  Warp<T, DP> state;
+  int slot = 0;
+  for (uint32_t at = first_item; at < p.items; at += stride) {
+    const Item it(p, at);
+    const int64_t bh = static_cast<int64_t>(it.b) * p.H + it.h;
+    const float log2_a = log2_decay(p.log_decay, it.h);
+    // where the scan enters and leaves the sequence
+    const int end_segment = (it.n ? it.n - 1 : 0) / p.segment;
+    const bool enters = it.segment == (p.reverse ? end_segment : 0), leaves = it.segment == (p.reverse ? 0 : end_segment);
+    const bool beyond = it.segment > end_segment;
+    bool use_x = false;
+    if (enters && p.first) {
+      const float lead = p.reverse || it.n == 0 ? 1.0f : power(log2_a, 1);
+      const float* f = p.first + bh * p.da * p.dc;
+      state.each(slice, [&](float& x, int i, int j, int) {
+        x = i < p.da && j < p.dc ? lead * f[p.first_t ? j * p.da + i : i * p.dc + j] : 0.0f;
+      });
+      use_x = true;
+    } else if (OUT && !enters && !beyond) {
+      const int s = p.reverse ? it.segment : it.segment - 1;
+      const float* f = p.parts + (bh * (p.segments - 1) + s) * (DP * DP) + slice * (L::kRegs * 32) + lane;
+      state.each(slice, [&](float& x, int, int, int k) { x = f[k * 32]; });
+      use_x = true;
+    } else {
+      state.each(slice, [&](float& x, int, int, int) { x = 0.0f; });
+    }
+    const bool keeps = OUT ? leaves && p.last : true;
+    Weights w;
+    if constexpr (OUT) w.of_pairs(log2_a, p.in_scale, p.reverse);
+    int weights_r = -1, weights_until = -1;
+    const int64_t out_stride = static_cast<int64_t>(p.H) * p.dc;
+    T* out = static_cast<T*>(p.out) + (static_cast<int64_t>(it.b) * p.T * p.H + it.h) * p.dc;
+    for (int step = 0; step < it.steps; ++step) {
+      const int c = it.chunk(p.reverse, step), row = it.row0 + c * kChunk, r = it.valid(c);
+      const bool final = step + 1 == it.steps;
+      // forwards the state that is handed out is as of the last position, without the decay into the next
+      const int until = OUT && final && keeps && !p.reverse ? (r ? r - 1 : 0) : r;
+      if (r != weights_r || until != weights_until) {
+        w.of_rows(log2_a, p.in_scale, p.reverse, r, until);
+        weights_r = r, weights_until = until;
+      }
+      cp_wait<kS - 2>();
+      sync();
+      load();
+      const uint32_t tile = base + slot * (3 * L::kBytes);
+      slot = slot + 1 == kS ? 0 : slot + 1;
+      float O[2][2 * L::kMT][4];
+      state.template chunk<OUT, SPLIT>(tile, tile + L::kBytes, tile + 2 * L::kBytes, slice, w, p.reverse, use_x,
+                                       !final || keeps, O);
+      if constexpr (OUT) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int from = (w.flip ? 1 - h : h) * 16;
+          if (h < w.halves)
+            store_rows<T, DP>(out + (row + from) * out_stride, out_stride, O[h], slice, r - from, p.T - row - from, p.dc,
+                              p.out_scale, p.out_vec, stage_out);
+        }
+        if (w.halves == 1) zero_rows<T, DP>(out, out_stride, slice, row + 16, min(p.T, row + kChunk), p.dc);
+      }
+      use_x = true;
+    }
+    if constexpr (OUT) {
+      zero_rows<T, DP>(out, out_stride, slice, it.row0 + it.steps * kChunk, min(p.T, it.row0 + p.segment), p.dc);
+      if (keeps) {
+        float* f = p.last + bh * p.da * p.dc;
+        state.each(slice, [&](float& x, int i, int j, int) {
+          if (i < p.da && j < p.dc) f[i * p.dc + j] = x;
+        });
+      }
+    } else if (it.segment != (p.reverse ? 0 : p.segments - 1)) {
+      const int s = p.reverse ? it.segment - 1 : it.segment;
+      float* f = p.parts + (bh * (p.segments - 1) + s) * (DP * DP) + slice * (L::kRegs * 32) + lane;
+      state.each(slice, [&](float& x, int, int, int k) { f[k * 32] = x; });
+    }
+  }
+}
+
+// The states that the segments leave behind, alone, become those that their next ones start from: a thread per value of
+// a state, along the segments.
+template <int DP>
+__global__ void __launch_bounds__(256) join_kernel(const Scan p) {
+  const int per = DP * DP / 256;
+  const uint32_t bh = blockIdx.x / per;
+  const int b = bh / p.H, n = length_of(p.lengths, p.length_bytes, b, p.T);
+  const float log2_a = log2_decay(p.log_decay, bh - b * p.H);
+  float* f = p.parts + static_cast<int64_t>(bh) * (p.segments - 1) * (DP * DP) + blockIdx.x % per * 256 + threadIdx.x;
+  float x = 0.0f;
+  constexpr int kAhead = 8;
+  for (int s0 = 0; s0 < p.segments - 1; s0 += kAhead) {
+    float v[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int s = p.reverse ? p.segments - 2 - s0 - u : s0 + u;
+      v[u] = s0 + u < p.segments - 1 ? f[static_cast<int64_t>(s) * (DP * DP)] : 0.0f;
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (s0 + u < p.segments - 1) {
+        const int s = p.reverse ? p.segments - 2 - s0 - u : s0 + u;
+        const int left = n - (p.reverse ? s + 1 : s) * p.segment;
+        x = fmaf(power(log2_a, left < 0 ? 0 : left > p.segment ? p.segment : left), x, v[u]);
+        f[static_cast<int64_t>(s) * (DP * DP)] = x;
+      }
+    }
+  }
+}
+
+// ---- short sequences ---------------------------------------------------------------------------------------------
+// Up to 16 positions and no state: out_i = scale sum_(j <= i) a^(i - j) (a_i . b_j) c_j (j >= i for dk and dv), one warp
+// per sequence and head, in registers.  A lane loads 16-byte pieces of rows g and g + 8.  The sum over a's columns may
+// number them as it likes, so a piece's words are operands as they lie; c's 8 x 8 pieces are transposed by the tensor
+// unit's move; and a result's columns come out where c's pieces had them, so that a lane stores the pieces it would load.
+// The forward pass reads three and writes one tensor, the backward pass reads four and writes three: no state, and nothing
+// twice.
+struct Short {
+  Rows q, k, v, go;
+  void *o, *dq, *dk, *dv;       // o, or the gradients
+  const float* log_decay;
+  const void* lengths;
+  int length_bytes, T, H, dim_k, dim_v;
+  float scale;
+  uint32_t items, step_b, step_h;     // B H; a grid's warps as sequences and heads
+};
+
+template <typename T, int DP>
+struct Piece {
+  static constexpr bool kF32 = sizeof(T) == 4;
+  static constexpr int kWords = DP * static_cast<int>(sizeof(T)) / 16;      // of a lane, per row
+  static constexpr int kWide = kWords < 4 ? kWords : 4;                    // of a load
+  static constexpr int kElements = kWide * 4 / static_cast<int>(sizeof(T));
+  uint32_t r[2][kWords];
+  // column of a lane's first element of load k
+  __device__ static __forceinline__ int column(int k) { return k * 4 * kElements + (threadIdx.x & 3) * kElements; }
+
+  __device__ __forceinline__ void load(const T* row, int64_t stride, int rows, int dim) {
+    const int g = (threadIdx.x & 31) >> 2;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int k = 0; k < kWords / kWide; ++k) {
+        const bool there = g + 8 * h < rows && column(k) < dim;
+        const T* at = row + (g + 8 * h) * stride + column(k);
+        if constexpr (kWide == 4) {
+          const uint4 v = there ? __ldg(reinterpret_cast<const uint4*>(at)) : make_uint4(0, 0, 0, 0);
+          r[h][4 * k] = v.x, r[h][4 * k + 1] = v.y, r[h][4 * k + 2] = v.z, r[h][4 * k + 3] = v.w;
+        } else {
+          const uint2 v = there ? __ldg(reinterpret_cast<const uint2*>(at)) : make_uint2(0, 0);
+          r[h][2 * k] = v.x, r[h][2 * k + 1] = v.y;
+        }
+      }
+  }
+  __device__ __forceinline__ void store(T* row, int64_t stride, int until, int dim) const {
+    const int g = (threadIdx.x & 31) >> 2;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int k = 0; k < kWords / kWide; ++k) {
+        T* at = row + (g + 8 * h) * stride + column(k);
+        if (g + 8 * h < until && column(k) < dim) {
+          if constexpr (kWide == 4) *reinterpret_cast<uint4*>(at) = make_uint4(r[h][4 * k], r[h][4 * k + 1], r[h][4 * k + 2], r[h][4 * k + 3]);
+          else *reinterpret_cast<uint2*>(at) = make_uint2(r[h][2 * k], r[h][2 * k + 1]);
+        }
+      }
+  }
+};
+
+__device__ __forceinline__ uint32_t transpose(uint32_t piece) {      // an 8 x 8 piece of 16-bit elements
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(piece));
+  return r;
+}
+
+// weights of (i, j): w[0], w[1] for i and j in the same half of the positions, w[2], w[3] for the later half's with the
+// earlier one's
+struct PairWeights {
+  float w[4];
+  __device__ __forceinline__ PairWeights(float log2_a, bool reverse, float scale) {
+    const int lane = threadIdx.x & 31, e0 = (lane >> 2) - 2 * (lane & 3);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = scale * power(log2_a, (reverse ? (k & 1) - e0 : e0 - (k & 1)) + (k >> 1) * 8);
+  }
+};
+
+template <typename T, int DP>
+__device__ __forceinline__ Piece<T, DP> attend(const Piece<T, DP>& a, const Piece<T, DP>& b, const Piece<T, DP>& c,
+                                               const PairWeights& w, bool reverse, int rows) {
+  using P_ = Piece<T, DP>;
+  const int g = (threadIdx.x & 31) >> 2;
+  float P[2][4] = {};
+  Piece<T, DP> out;
+  if constexpr (P_::kF32) {
+#pragma unroll
+    for (int k = 0; k < P_::kWords / 2; ++k) {
+      const Split x[4] = {Split(__uint_as_float(a.r[0][2 * k])), Split(__uint_as_float(a.r[1][2 * k])),
+                          Split(__uint_as_float(a.r[0][2 * k + 1])), Split(__uint_as_float(a.r[1][2 * k + 1]))};
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+        mma_f32(P[n], x, Split(__uint_as_float(b.r[n][2 * k])), Split(__uint_as_float(b.r[n][2 * k + 1])));
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < P_::kWords / 2; ++k) {
+      const uint32_t x[4] = {a.r[0][2 * k], a.r[1][2 * k], a.r[0][2 * k + 1], a.r[1][2 * k + 1]};
+#pragma unroll
+      for (int n = 0; n < 2; ++n) mma_bf16(P[n], x, b.r[n][2 * k], b.r[n][2 * k + 1]);
+    }
+  }
+  // [n][row half][column]: masked products are dropped, not multiplied by zero
+#pragma unroll
+  for (int n = 0; n < 2; ++n)
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int z = 0; z < 2; ++z) {
+        const bool never = reverse ? h > n : n > h;
+        const float wt = w.w[h == n ? z : 2 + z];
+        float& x = P[n][2 * h + z];
+        x = never || wt == 0.0f ? 0.0f : x * wt;
+      }
+  const bool keep0 = g < rows, keep1 = g + 8 < rows;
+  if constexpr (P_::kF32) {
+    Split p[2][4];
+#pragma unroll
+    for (int n = 0; n < 2; ++n) p[n][0] = Split(P[n][0]), p[n][1] = Split(P[n][2]), p[n][2] = Split(P[n][1]), p[n][3] = Split(P[n][3]);
+#pragma unroll
+    for (int q = 0; q < P_::kWords / 2; ++q) {
+      float O[4] = {};
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        // 32-bit elements as two pieces of 16-bit ones
+        const uint32_t x0 = c.r[n][2 * q], x1 = c.r[n][2 * q + 1];
+        const uint32_t lo = transpose(__byte_perm(x0, x1, 0x5410)), hi = transpose(__byte_perm(x0, x1, 0x7632));
+        mma_f32(O, p[n], Split(__uint_as_float(__byte_perm(lo, hi, 0x5410))), Split(__uint_as_float(__byte_perm(lo, hi, 0x7632))));
+      }
+      out.r[0][2 * q] = keep0 ? __float_as_uint(O[0]) : 0u, out.r[0][2 * q + 1] = keep0 ? __float_as_uint(O[1]) : 0u;
+      out.r[1][2 * q] = keep1 ? __float_as_uint(O[2]) : 0u, out.r[1][2 * q + 1] = keep1 ? __float_as_uint(O[3]) : 0u;
+    }
+  } else {
+    // the weighted products as two bf16 parts: one would round as coarsely as the result
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float p0 = P[e >> 1][2 * (e & 1)], p1 = P[e >> 1][2 * (e & 1) + 1];
+      hi[e] = pack(p0, p1);
+      lo[e] = pack(p0 - low(hi[e]), p1 - high(hi[e]));
+    }
+#pragma unroll
+    for (int q = 0; q < P_::kWords; ++q) {
+      float O[4] = {};
+      const uint32_t b0 = transpose(c.r[0][q]), b1 = transpose(c.r[1][q]);
+      mma_bf16(O, lo, b0, b1);
+      mma_bf16(O, hi, b0, b1);
+      out.r[0][q] = keep0 ? pack(O[0], O[1]) : 0u;
+      out.r[1][q] = keep1 ? pack(O[2], O[3]) : 0u;
+    }
+  }
+  return out;
+}
+
+template <typename T, int DP, bool BWD>
+__global__ void __launch_bounds__(kThreads) short_kernel(const __grid_constant__ Short p) {
+  const uint32_t first = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5), stride = gridDim.x * (kThreads / 32);
+  uint32_t b = first / p.H, h = first - b * p.H;
+  Piece<T, DP> q, k, v, go;
+  int rows = 0;
+  auto load = [&] {
+    rows = length_of(p.lengths, p.length_bytes, b, p.T);
+    auto at = [&](const Rows& r) { return static_cast<const T*>(r.at) + b * r.b + h * r.h; };
+    q.load(at(p.q), p.q.t, rows, p.dim_k);
+    k.load(at(p.k), p.k.t, rows, p.dim_k);
+    v.load(at(p.v), p.v.t, rows, p.dim_v);
+    if constexpr (BWD) go.load(at(p.go), p.go.t, rows, p.dim_v);
+  };
+  if (first < p.items) load();
+  for (uint32_t at = first; at < p.items;) {
+    const Piece<T, DP> q0 = q, k0 = k, v0 = v, go0 = go;
+    const uint32_t b0 = b, h0 = h;
+    const int rows0 = rows;
+    const float log2_a = log2_decay(p.log_decay, h);
+    // the next item's rows are on their way while this one's are used
+    b += p.step_b, h += p.step_h;
+    if (h >= static_cast<uint32_t>(p.H)) h -= p.H, ++b;
+    at += stride;
+    if (at < at - stride) at = p.items;            // past 2^32
+    if (at < p.items) load();
+    const int64_t row = (static_cast<int64_t>(b0) * p.T * p.H + h0);
+    const int64_t sk = static_cast<int64_t>(p.H) * p.dim_k, sv = static_cast<int64_t>(p.H) * p.dim_v;
+    const PairWeights forward(log2_a, false, p.scale);
+    if constexpr (!BWD) {
+      attend<T, DP>(q0, k0, v0, forward, false, rows0).store(static_cast<T*>(p.o) + row * p.dim_v, sv, p.T, p.dim_v);
+    } else {
+      attend<T, DP>(go0, v0, k0, forward, false, rows0).store(static_cast<T*>(p.dq) + row * p.dim_k, sk, p.T, p.dim_k);
+      const PairWeights back(log2_a, true, p.scale);
+      attend<T, DP>(v0, go0, q0, back, true, rows0).store(static_cast<T*>(p.dk) + row * p.dim_k, sk, p.T, p.dim_k);
+      attend<T, DP>(k0, q0, go0, back, true, rows0).store(static_cast<T*>(p.dv) + row * p.dim_v, sv, p.T, p.dim_v);
+    }
   }
 }
 
@@ -127,22 +939,157 @@ int size_of(int32_t dtype) { return dtype == BPC_DTYPE_F32 ? 4 : dtype == BPC_DT
 
 bool aligned(const void* p, int size) { return reinterpret_cast<uintptr_t>(p) % size == 0; }
 
-int run_scan(const Scan& p, int32_t dtype, cudaStream_t s) {
-  const int smem = p.da * kThreads * static_cast<int>(sizeof(float));
-  const void* fn = dtype == BPC_DTYPE_F32 ? reinterpret_cast<const void*>(&scan_kernel<float>)
-                                          : reinterpret_cast<const void*>(&scan_kernel<__nv_bfloat16>);
+// f(the padded head size as a type's value)
+template <typename F>
+auto with_dim(int dim, F f) {
+  if (dim <= 16) return f(std::integral_constant<int, 16>());
+  if (dim <= 32) return f(std::integral_constant<int, 32>());
+  if (dim <= 64) return f(std::integral_constant<int, 64>());
+  return f(std::integral_constant<int, 128>());
+}
+template <typename T>
+struct Type {
+  typedef T type;
+};
+template <typename F>
+auto with_type(int32_t dtype, F f) {
+  if (dtype == BPC_DTYPE_F32) return f(Type<float>());
+  return f(Type<__nv_bfloat16>());
+}
+
+int padded(int dim) {
+  return with_dim(dim, [](auto d) { return decltype(d)::value; });
+}
+
+// Blocks of scan_kernel that are resident per SM
+template <typename T, int DP, bool OUT, int SPLIT>
+int scan_blocks(int* blocks) {
+  const void* fn = reinterpret_cast<const void*>(&scan_kernel<T, DP, OUT, SPLIT>);
+  constexpr int smem = Tile<T, DP>::kSmem;
   if (int e = allow_smem(fn, smem)) return e;
-  const unsigned grid = static_cast<unsigned>(p.B * p.H);
-  if (dtype == BPC_DTYPE_F32) scan_kernel<float><<<grid, kThreads, smem, s>>>(p);
-  else scan_kernel<__nv_bfloat16><<<grid, kThreads, smem, s>>>(p);
+  static int resident = 0;      // the same on every device that this library runs on
+  if (!resident) {
+    int n = 0;
+    const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, fn, Tile<T, DP>::kThreads, smem);
+    if (e != cudaSuccess || n < 1) return fail(BPC_ERR_LAUNCH, std::string("linear_attention occupancy: ") + cudaGetErrorString(e));
+    resident = n;
+  }
+  *blocks = resident;
+  return 0;
+}
+
+template <typename T, int DP, bool OUT, int SPLIT>
+int launch_scan(const Scan& p, cudaStream_t s) {
+  int blocks = 0;
+  if (int e = scan_blocks<T, DP, OUT, SPLIT>(&blocks)) return e;
+  using L = Tile<T, DP>;
+  constexpr int groups = L::kGroups;
+  const unsigned grid = std::min<unsigned>((p.items + groups - 1) / groups, blocks * num_sms());
+  scan_kernel<T, DP, OUT, SPLIT><<<grid, L::kThreads, L::kSmem, s>>>(p);
   return launched("linear_attention");
+}
+
+// Into how many segments a sequence is cut: one where the heads alone keep the GPU busy
+int segments_of(int64_t BH, int64_t T, int dim) {
+  const int64_t groups = static_cast<int64_t>(num_sms()) * 8 / std::max(1, padded(dim) / 32);
+  if (BH >= groups || T <= 512) return 1;
+  return static_cast<int>(std::max<int64_t>(1, std::min((groups + BH - 1) / BH, T / 256)));
+}
+
+int64_t parts_bytes(int64_t BH, int64_t T, int dim) {
+  const int64_t D = padded(dim);
+  return BH * (segments_of(BH, T, dim) - 1) * D * D * static_cast<int64_t>(sizeof(float));
+}
+
+int run_scan(Scan p, int64_t B, int32_t dtype, float* workspace, cudaStream_t s) {
+  const int dim = std::max(p.da, p.dc);
+  const int64_t BH = B * p.H;
+  const int want = segments_of(BH, p.T, dim);
+  p.segment = std::max(kChunk, ((p.T + want - 1) / want + kChunk - 1) / kChunk * kChunk);
+  p.segments = std::max(1, (p.T + p.segment - 1) / p.segment);
+  p.items = static_cast<uint32_t>(BH * p.segments);
+  p.parts = workspace;
+  return with_type(dtype, [&](auto type) {
+    return with_dim(dim, [&](auto d) {
+      typedef typename decltype(type)::type T;
+      constexpr int DP = decltype(d)::value;
+      // the state handed out is fp32: it needs every bit of the weighted rows; a bf16 result alone does with 16
+      constexpr int kFew = sizeof(T) == 4 ? 3 : 2;
+      if (p.segments > 1) {
+        if (int e = p.last ? launch_scan<T, DP, false, 3>(p, s) : launch_scan<T, DP, false, kFew>(p, s)) return e;
+        join_kernel<DP><<<static_cast<unsigned>(BH * (DP * DP / 256)), 256, 0, s>>>(p);
+        if (int e = launched("linear_attention")) return e;
+      }
+      return p.last ? launch_scan<T, DP, true, 3>(p, s) : launch_scan<T, DP, true, kFew>(p, s);
+    });
+  });
+}
+
+// Blocks of a kernel without dynamic shared memory that are resident per SM
+int blocks_of(const void* fn, int* cached, int* blocks) {
+  if (!*cached) {
+    int n = 0;
+    const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, fn, kThreads, 0);
+    if (e != cudaSuccess || n < 1) return fail(BPC_ERR_LAUNCH, std::string("linear_attention occupancy: ") + cudaGetErrorString(e));
+    *cached = n;
+  }
+  *blocks = *cached;
+  return 0;
+}
+
+template <typename T, int DP, bool BWD>
+int launch_short(Short p, cudaStream_t s) {
+  static int cached = 0;
+  int blocks = 0;
+  if (int e = blocks_of(reinterpret_cast<const void*>(&short_kernel<T, DP, BWD>), &cached, &blocks)) return e;
+  const uint32_t warps = kThreads / 32;
+  const unsigned grid = std::min<unsigned>((p.items + warps - 1) / warps, blocks * num_sms());
+  p.step_b = grid * warps / p.H, p.step_h = grid * warps % p.H;
+  short_kernel<T, DP, BWD><<<grid, kThreads, 0, s>>>(p);
+  return launched("linear_attention");
+}
+
+template <bool BWD>
+int run_short(const Short& p, int32_t dtype, cudaStream_t s) {
+  return with_type(dtype, [&](auto type) {
+    typedef typename decltype(type)::type T;
+    const int dim = std::max(p.dim_k, p.dim_v);
+    if (dim <= 16) return launch_short<T, 16, BWD>(p, s);
+    if constexpr (sizeof(T) == 2)
+      if (dim > 32) return launch_short<T, 64, BWD>(p, s);
+    return launch_short<T, 32, BWD>(p, s);
+  });
+}
+
+// Head sizes that short_kernel holds in registers
+int short_dim(int size) { return size == 4 ? 32 : 64; }
+
+// 16-byte copies need rows of whole 16-byte pieces on 16-byte boundaries
+bool copies_whole(const Rows& r, int dim, int size) {
+  return aligned(r.at, 16) && dim * size % 16 == 0 && r.b * size % 16 == 0 && r.t * size % 16 == 0 && r.h * size % 16 == 0;
+}
+
+Scan make_scan(const Rows& a, const Rows& b, const Rows& c, void* out, const float* log_decay, const float* first, bool first_t,
+               float* last, const void* lengths, int length_bytes, int64_t T, int H, int da, int dc, float in, float scale,
+               bool reverse, int size) {
+  Scan p = {};
+  p.a = a, p.b = b, p.c = c;
+  p.out = out;
+  p.log_decay = log_decay;
+  p.first = first, p.first_t = first_t, p.last = last;
+  p.lengths = lengths, p.length_bytes = length_bytes;
+  p.T = static_cast<int>(T), p.H = H, p.da = da, p.dc = dc;
+  p.in_scale = in, p.out_scale = scale, p.reverse = reverse;
+  p.vec = T > 0 && copies_whole(a, da, size) && copies_whole(b, da, size) && copies_whole(c, dc, size);
+  p.out_vec = aligned(out, 16) && dc * size % (size == 4 ? 8 : 16) == 0;
+  return p;
 }
 
 int check_common(const std::string& what, int64_t B, int64_t T, int32_t H, int32_t dk, int32_t dv, const void* lengths,
                  int32_t length_bytes, const int64_t* strides, int n_strides, float scale, int32_t dtype,
                  const float* log_decay) {
   auto bad = [&](const char* m) { return fail(BPC_ERR_ARG, what + ": " + m); };
-  if (B < 0 || T < 0 || H < 0 || T > (static_cast<int64_t>(1) << 31)) return bad("batch, length and heads must not be negative, length <= 2^31");
+  if (B < 0 || T < 0 || H < 0 || T > (1 << 30)) return bad("batch, length and heads must not be negative, length <= 2^30");
   if (H && B > 0x7fffffff / H) return bad("batch x heads must be below 2^31");
   if (dk < 1 || dk > kMaxDim || dv < 1 || dv > kMaxDim) return bad("head sizes must be 1 to 128");
   if (!size_of(dtype)) return bad("dtype must be f32 or bf16");
@@ -167,7 +1114,7 @@ using namespace bpc;
 extern "C" size_t bpc_linear_attention_workspace_size(int64_t B, int64_t T, int32_t H, int32_t dk, int32_t dv,
                                                       int32_t dtype, int32_t backward) {
   if (B < 1 || T < 0 || H < 1 || dk < 1 || dk > kMaxDim || dv < 1 || dv > kMaxDim || !size_of(dtype)) return 0;
-  return 16;
+  return static_cast<size_t>(std::max<int64_t>(16, parts_bytes(B * H, T, std::max(dk, dv))));
 }
 
 extern "C" int bpc_linear_attention_fwd(const void* q, const void* k, const void* v, void* o, const float* log_decay,
@@ -185,9 +1132,16 @@ extern "C" int bpc_linear_attention_fwd(const void* q, const void* k, const void
     return fail(BPC_ERR_ARG, "linear_attention: buffer not aligned to its type (states and workspace: 16 bytes)");
   if (workspace_bytes < bpc_linear_attention_workspace_size(B, T, H, dk, dv, dtype, 0))
     return fail(BPC_ERR_SPACE, "linear_attention: workspace too small");
-  const Scan p{rows_of(q, strides), rows_of(k, strides + 3), rows_of(v, strides + 6), o, log_decay, state, new_state, lengths,
-               length_bytes, B, T, H, dk, dv, 1.0f, scale, false, false};
-  return run_scan(p, dtype, reinterpret_cast<cudaStream_t>(stream));
+  const Rows rq = rows_of(q, strides), rk = rows_of(k, strides + 3), rv = rows_of(v, strides + 6);
+  if (T && T <= kShort && !state && !new_state && std::max(dk, dv) <= short_dim(size) && copies_whole(rq, dk, size) &&
+      copies_whole(rk, dk, size) && copies_whole(rv, dv, size) && aligned(o, 16)) {
+    const Short p{rq, rk, rv, {}, o, nullptr, nullptr, nullptr, log_decay, lengths, length_bytes, static_cast<int>(T), H, dk, dv,
+                  scale, static_cast<uint32_t>(B * H), 0, 0};
+    return run_short<false>(p, dtype, reinterpret_cast<cudaStream_t>(stream));
+  }
+  const Scan p = make_scan(rq, rk, rv, o, log_decay, state, false,
+                           new_state, lengths, length_bytes, T, H, dk, dv, 1.0f, scale, false, size);
+  return run_scan(p, B, dtype, static_cast<float*>(workspace), reinterpret_cast<cudaStream_t>(stream));
 }
 
 extern "C" int bpc_linear_attention_bwd(const void* q, const void* k, const void* v, const void* go, const float* log_decay,
@@ -209,14 +1163,25 @@ extern "C" int bpc_linear_attention_bwd(const void* q, const void* k, const void
     return fail(BPC_ERR_SPACE, "linear_attention backward: workspace too small");
   const Rows rq = rows_of(q, strides), rk = rows_of(k, strides + 3), rv = rows_of(v, strides + 6), rg = rows_of(go, strides + 9);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (T) {
-    const Scan pq{rg, rv, rk, dq, log_decay, state, nullptr, lengths, length_bytes, B, T, H, dv, dk, 1.0f, scale, false, true};
-    if (int e = run_scan(pq, dtype, s)) return e;
-    const Scan pk{rv, rg, rq, dk_out, log_decay, grad_state, nullptr, lengths, length_bytes, B, T, H, dv, dk, scale, 1.0f, true, true};
-    if (int e = run_scan(pk, dtype, s)) return e;
+  if (T && T <= kShort && !state && !grad_state && !dstate && std::max(dk, dv) <= short_dim(size) && copies_whole(rq, dk, size) &&
+      copies_whole(rk, dk, size) && copies_whole(rv, dv, size) && copies_whole(rg, dv, size) && aligned(dq, 16) &&
+      aligned(dk_out, 16) && aligned(dv_out, 16)) {
+    const Short p{rq, rk, rv, rg, nullptr, dq, dk_out, dv_out, log_decay, lengths, length_bytes, static_cast<int>(T), H, dk, dv,
+                  scale, static_cast<uint32_t>(B * H), 0, 0};
+    return run_short<true>(p, dtype, s);
   }
-  const Scan pv{rk, rq, rg, dv_out, log_decay, grad_state, dstate, lengths, length_bytes, B, T, H, dk, dv, scale, 1.0f, true, false};
-  return run_scan(pv, dtype, s);
+  float* ws = static_cast<float*>(workspace);
+  if (T) {
+    const Scan pq = make_scan(rg, rv, rk, dq, log_decay, state, true, nullptr, lengths, length_bytes, T, H, dv, dk, 1.0f, scale,
+                              false, size);
+    if (int e = run_scan(pq, B, dtype, ws, s)) return e;
+    const Scan pk = make_scan(rv, rg, rq, dk_out, log_decay, grad_state, true, nullptr, lengths, length_bytes, T, H, dv, dk,
+                              scale, 1.0f, true, size);
+    if (int e = run_scan(pk, B, dtype, ws, s)) return e;
+  }
+  const Scan pv = make_scan(rk, rq, rg, dv_out, log_decay, grad_state, false, dstate, lengths, length_bytes, T, H, dk, dv, scale,
+                            1.0f, true, size);
+  return run_scan(pv, B, dtype, ws, s);
 }
 
 extern "C" int bpc_linear_attention_step(const void* q, const void* k, const void* v, void* o, const float* log_decay,

@@ -2,9 +2,14 @@
 definition in 64 bits.
 
 Tolerances, u = 2^-24.  Every output is a sum of products weighed by powers of the decay: with every factor replaced by its
-magnitude the same sum gives mag.  Sums, weights (a power a^n is off by at most (n + 2) u of itself, and |n a^n| is what the
-sum holds of it) and the state's n updates each round once, so an element is off by at most (D + 4 T + 16) u mag, D the
-head size (each product of two split operands leaves out at most u of itself), and by the rounding to its type.  That is a
+magnitude the same sum gives mag.  The sums over D elements of a head and over T positions, and the state's updates, each
+round once; a power a^n is off by (n + 4) u of itself: together at most (D + 4 T) u mag.  fp32 products are made of
+operands in two tf32 parts of 11 bits: what the second part rounds away is 2^-23 of the operand, twice, and the product
+of the second parts, left out, 2^-22: 8 u a product, and an element is a product of products, of the state with the rows
+and of the rows that made it: 3 of them, and 8 u for the powers' and the scale's: 48 u mag at most with the sums' ends.
+For bf16 inputs, products of the inputs are exact; an fp32 factor (the weighted pair, the state, the weighted row in it) goes
+in as two bf16 parts, off by (2^-9)^2 = 64 u of itself, at most two such factors in a term of a bf16 result: 128 u mag.
+A state handed out has its rows in three parts.  Then the rounding to the type: half a step.  That is a
 bound for the worst case.  Against a loss of bits the root mean square is tested too, over results of a thousand values and
 more (n = (sum v^2)^2 / sum v^4 counts them): roundings to the type are spread evenly over half a step either way, so
 their squares are a third of its square on average, with a deviation of 0.3 / sqrt(n), of which six are allowed; a single
@@ -74,7 +79,7 @@ def definition(q, k, v, g, scale, s0, n, go=None, gs=None, mag=False):
 
 def check(got, want, mag, dtype, T, D, what):
     assert got.dtype == dtype and got.shape == want.shape, what
-    e = (D + 4 * T + 16) * U * mag
+    e = (D + 4 * T + 48 + (128 if dtype == BF16 else 0)) * U * mag
     tol = e + (want.abs() + e) * HALF[dtype] + 1e-36
     err = (got.double() - want).abs()
     assert bool((err <= tol).all()), (what, float((err / tol).max()))
