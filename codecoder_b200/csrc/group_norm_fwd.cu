@@ -1,0 +1,366 @@
+// Group normalisation with an activation over channels-last features: the forward pass.
+//
+//   x (B, N, C), group g = channels [g C / G, (g + 1) C / G):  mean, var over the N C / G values of a sample and group
+//   xh = (x - mean) rstd, rstd = 1 / sqrt(var + eps);   z = w_c xh + b_c;   y = act(z) = z s(u(z))
+//     act: none (s = 1), SiLU (u = z), GELU in its tanh form (u = 2 sqrt(2 / pi) (z + 0.044715 z^3)), s the logistic
+//     function
+//
+// One read of x and one write of y where a sample's slab fits the registers of a block or a cluster; the variance is the
+// mean of the squared differences from the mean, never a difference of squares, and the parts of several blocks join as
+// var n = sum (var_i n_i + n_i (mean_i - mean)^2).
+#include "group_norm.cuh"
+
+namespace bpc {
+namespace gn {
+namespace {
+
+namespace cg_ = cooperative_groups;
+
+constexpr int kK = kForwardRows;
+
+// Units: a sample's group per `lanes` lanes, SLOTS vectors each; a thread's slots are the same places of every sample.
+template <typename T, typename U, int ACT, int VEC, int SLOTS>
+__global__ void __launch_bounds__(kMaxThreads) units_kernel(const T* __restrict__ x, U* __restrict__ y, float* mean_out,
+                                                            float* rstd_out, const float* __restrict__ w,
+                                                            const float* __restrict__ bias, const Shape s, const Plan p, float eps) {
+  constexpr int kAhead = SLOTS == 1 ? 4 : 1;       // samples at a time
+  const int cg = s.C / s.G, across = cg / VEC, n = static_cast<int>(s.N) * cg;
+  const int unit = threadIdx.x / p.lanes, l = threadIdx.x % p.lanes;
+  const int g = unit % s.G, r = unit / s.G;
+  const bool there = r < p.rows;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * p.rows;
+  int64_t in[SLOTS];
+  int out[SLOTS];
+  bool has[SLOTS];
+  float wv[SLOTS][VEC], bv[SLOTS][VEC];
+#pragma unroll
+  for (int k = 0; k < SLOTS; ++k) {
+    const int e = k * p.lanes + l, row = e / across, c = g * cg + e % across * VEC;
+    has[k] = there && row < s.N;
+    in[k] = row * s.x_row + c;
+    out[k] = row * s.C + c;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      wv[k][i] = has[k] && w ? w[c + i] : 1.0f;
+      bv[k][i] = has[k] && bias ? bias[c + i] : 0.0f;
+    }
+  }
+  const float per = 1.0f / static_cast<float>(n);
+  for (int64_t b0 = static_cast<int64_t>(blockIdx.x) * p.rows + r; b0 - r < s.B; b0 += kAhead * step) {
+    Pack<T, VEC> v[kAhead][SLOTS];
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a)
+#pragma unroll
+      for (int k = 0; k < SLOTS; ++k)
+        if (has[k] && b0 + a * step < s.B) v[a][k] = *reinterpret_cast<const Pack<T, VEC>*>(x + (b0 + a * step) * s.x_sample + in[k]);
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) {
+      const int64_t b = b0 + a * step;
+      const bool live = b < s.B;
+      float sum = 0.0f;
+#pragma unroll
+      for (int k = 0; k < SLOTS; ++k)
+        if (has[k] && live) {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) sum += v[a][k].get(i);
+        }
+      for (int d = p.lanes >> 1; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      const float mean = sum * per;
+      float sq = 0.0f;
+#pragma unroll
+      for (int k = 0; k < SLOTS; ++k)
+        if (has[k] && live) {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            const float d = v[a][k].get(i) - mean;
+            sq = fmaf(d, d, sq);
+          }
+        }
+      for (int d = p.lanes >> 1; d; d >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, d);
+      const float rstd = 1.0f / sqrtf(sq * per + eps);
+      if (l == 0 && there && live && mean_out) {
+        mean_out[b * s.G + g] = mean;
+        rstd_out[b * s.G + g] = rstd;
+      }
+#pragma unroll
+      for (int k = 0; k < SLOTS; ++k)
+        if (has[k] && live) {
+          Pack<U, VEC> o;
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) o.set(i, activate<ACT>(fmaf(wv[k][i], (v[a][k].get(i) - mean) * rstd, bv[k][i])));
+          *reinterpret_cast<Pack<U, VEC>*>(y + b * s.N * s.C + out[k]) = o;
+        }
+    }
+  }
+}
+
+enum Mode { kFused, kStats, kApply };
+
+// Tiles: a block's chunk of a slab in registers.  parts: (B, chunks, G) pairs of mean and summed squared differences
+// between the two kernels of samples that no cluster holds.
+template <typename T, typename U, int ACT, int VEC, int MODE>
+__global__ void __launch_bounds__(kMaxThreads) tiles_kernel(const T* __restrict__ x, U* __restrict__ y, float* mean_out,
+                                                            float* rstd_out, const float* __restrict__ w,
+                                                            const float* __restrict__ bias, const Shape s, const Plan p, float eps,
+                                                            float2* parts) {
+  __shared__ float part[kMaxThreads];
+  __shared__ float sums[kMaxThreads], squares[kMaxThreads];
+  __shared__ float2 mine[kMaxThreads];             // a group's mean and squares here, and (in place) in the whole sample
+  const int cg = s.C / s.G, across = cg / VEC, groups = p.slab / cg;
+  const int v = threadIdx.x % p.V, r = threadIdx.x / p.V, lanes = blockDim.x / p.V;
+  const int64_t works = s.B * p.slabs * p.chunks;
+  for (int64_t at = blockIdx.x; at < works; at += gridDim.x) {
+    // what the statistics' kernel read last is read first
+    const int64_t work = MODE == kApply ? works - 1 - at : at;
+    const int chunk = static_cast<int>(work % p.chunks);
+    const int64_t rest = work / p.chunks, b = rest / p.slabs;
+    const int slab = static_cast<int>(rest % p.slabs), c = slab * p.slab + v * VEC, j = v / across;
+    const int row0 = chunk * p.chunk_rows, rows = min(p.chunk_rows, static_cast<int>(s.N) - row0);
+    const bool there = r < lanes && c < s.C;
+    Pack<T, VEC> d[kK];
+    const T* from = x + b * s.x_sample + (row0 + r) * s.x_row + c;
+#pragma unroll
+    for (int k = 0; k < kK; ++k)
+      if (there && r + k * lanes < rows) d[k] = *reinterpret_cast<const Pack<T, VEC>*>(from + k * lanes * s.x_row);
+    float mean, rstd;
+    if constexpr (MODE != kApply) {
+      float sum = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kK; ++k)
+        if (there && r + k * lanes < rows) {
+          float t = 0.0f;
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) t += d[k].get(i);
+          sum += t;
+        }
+      group_sums(sum, p.V, lanes, across, groups, part, sums);
+      const float n = static_cast<float>(rows) * static_cast<float>(cg);
+      mean = j < groups ? sums[j] / n : 0.0f;
+      float sq = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kK; ++k)
+        if (there && r + k * lanes < rows) {
+          float t = 0.0f;
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            const float e = d[k].get(i) - mean;
+            t = fmaf(e, e, t);
+          }
+          sq += t;
+        }
+      group_sums(sq, p.V, lanes, across, groups, part, squares);
+      if (MODE == kFused && p.chunks == 1) {
+        rstd = j < groups ? 1.0f / sqrtf(squares[j] / n + eps) : 0.0f;
+        if (there && r == 0 && v % across == 0 && mean_out) {
+          mean_out[b * s.G + slab * groups + j] = mean;
+          rstd_out[b * s.G + slab * groups + j] = rstd;
+        }
+      } else if (MODE == kStats) {
+        if (there && r == 0 && v % across == 0) parts[(b * p.chunks + chunk) * s.G + slab * groups + j] = make_float2(mean, squares[j]);
+        __syncthreads();
+        continue;
+      } else {
+        for (int k = threadIdx.x; k < groups; k += blockDim.x) mine[k] = make_float2(sums[k] / n, squares[k]);
+        cg_::cluster_group cluster = cg_::this_cluster();
+        cluster.sync();
+        for (int k = threadIdx.x; k < groups; k += blockDim.x) {
+          float2 theirs[kCluster];
+          float total = 0.0f;
+          for (int q = 0; q < p.chunks; ++q) {
+            theirs[q] = cluster.map_shared_rank(mine, q)[k];
+            total = fmaf(theirs[q].x, static_cast<float>(min(p.chunk_rows, static_cast<int>(s.N) - q * p.chunk_rows)), total);
+          }
+          const float m = total / static_cast<float>(s.N);
+          float all = 0.0f;
+          for (int q = 0; q < p.chunks; ++q) {
+            const float e = theirs[q].x - m, rows_q = static_cast<float>(min(p.chunk_rows, static_cast<int>(s.N) - q * p.chunk_rows));
+            all += fmaf(e * e, rows_q * static_cast<float>(cg), theirs[q].y);
+          }
+          sums[k] = m;
+          squares[k] = 1.0f / sqrtf(all / (static_cast<float>(s.N) * static_cast<float>(cg)) + eps);
+          if (chunk == 0 && mean_out && slab * groups + k < s.G) {
+            mean_out[b * s.G + slab * groups + k] = m;
+            rstd_out[b * s.G + slab * groups + k] = squares[k];
+          }
+        }
+        cluster.sync();                            // every block has read the others' parts
+        mean = j < groups ? sums[j] : 0.0f;
+        rstd = j < groups ? squares[j] : 0.0f;
+      }
+    } else {
+      const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+      for (int k = warp; k < groups && slab * groups + k < s.G; k += warps) {
+        const float2* f = parts + b * p.chunks * s.G + slab * groups + k;
+        float total = 0.0f;
+        for (int q = lane; q < p.chunks; q += 32)
+          total = fmaf(f[static_cast<int64_t>(q) * s.G].x, static_cast<float>(min(p.chunk_rows, static_cast<int>(s.N) - q * p.chunk_rows)), total);
+#pragma unroll
+        for (int m = 16; m; m >>= 1) total += __shfl_xor_sync(0xffffffffu, total, m);
+        const float m = total / static_cast<float>(s.N);
+        float all = 0.0f;
+        for (int q = lane; q < p.chunks; q += 32) {
+          const float2 t = f[static_cast<int64_t>(q) * s.G];
+          const float e = t.x - m;
+          all += fmaf(e * e, static_cast<float>(min(p.chunk_rows, static_cast<int>(s.N) - q * p.chunk_rows)) * static_cast<float>(cg), t.y);
+        }
+#pragma unroll
+        for (int q = 16; q; q >>= 1) all += __shfl_xor_sync(0xffffffffu, all, q);
+        if (lane == 0) {
+          sums[k] = m;
+          squares[k] = 1.0f / sqrtf(all / (static_cast<float>(s.N) * static_cast<float>(cg)) + eps);
+          if (chunk == 0 && mean_out) {
+            mean_out[b * s.G + slab * groups + k] = m;
+            rstd_out[b * s.G + slab * groups + k] = squares[k];
+          }
+        }
+      }
+      __syncthreads();
+      mean = j < groups ? sums[j] : 0.0f;
+      rstd = j < groups ? squares[j] : 0.0f;
+    }
+    if constexpr (MODE != kStats) {
+      float wv[VEC], bv[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        wv[i] = there && w ? __ldg(w + c + i) : 1.0f;
+        bv[i] = there && bias ? __ldg(bias + c + i) : 0.0f;
+      }
+      U* to = y + (b * s.N + row0 + r) * s.C + c;
+#pragma unroll
+      for (int k = 0; k < kK; ++k)
+        if (there && r + k * lanes < rows) {
+          Pack<U, VEC> o;
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) o.set(i, activate<ACT>(fmaf(wv[i], (d[k].get(i) - mean) * rstd, bv[i])));
+          *reinterpret_cast<Pack<U, VEC>*>(to + static_cast<int64_t>(k) * lanes * s.C) = o;
+        }
+      __syncthreads();                             // sums and squares are this work's until here
+    }
+  }
+}
+
+// the sum over the block, in every thread; red: 8 floats
+__device__ __forceinline__ float block_sum(float v, float* red) {
+#pragma unroll
+  for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  float s = 0.0f;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) s += red[w];
+  __syncthreads();
+  return s;
+}
+
+// Wide groups: a block per sample and group, in three passes
+template <typename T, typename U, int ACT>
+__global__ void __launch_bounds__(256) wide_kernel(const T* __restrict__ x, U* __restrict__ y, float* mean_out, float* rstd_out,
+                                                   const float* __restrict__ w, const float* __restrict__ bias, const Shape s,
+                                                   float eps) {
+  __shared__ float red[8];
+  const int cg = s.C / s.G;
+  const int64_t n = s.N * cg;
+  for (int64_t at = blockIdx.x; at < s.B * s.G; at += gridDim.x) {
+    const int64_t b = at / s.G;
+    const int c0 = static_cast<int>(at % s.G) * cg;
+    const T* xs = x + b * s.x_sample + c0;
+    float sum = 0.0f;
+    for (int64_t i = threadIdx.x; i < n; i += 256) sum += load_f32(xs + i / cg * s.x_row + i % cg);
+    const float mean = block_sum(sum, red) / static_cast<float>(n);
+    float sq = 0.0f;
+    for (int64_t i = threadIdx.x; i < n; i += 256) {
+      const float d = load_f32(xs + i / cg * s.x_row + i % cg) - mean;
+      sq = fmaf(d, d, sq);
+    }
+    const float rstd = 1.0f / sqrtf(block_sum(sq, red) / static_cast<float>(n) + eps);
+    if (threadIdx.x == 0 && mean_out) mean_out[at] = mean, rstd_out[at] = rstd;
+    for (int64_t i = threadIdx.x; i < n; i += 256) {
+      const int c = c0 + static_cast<int>(i % cg);
+      const int64_t r = i / cg;
+      const float xh = (load_f32(x + b * s.x_sample + r * s.x_row + c) - mean) * rstd;
+      store_f32(y + (b * s.N + r) * s.C + c, activate<ACT>(fmaf(w ? w[c] : 1.0f, xh, bias ? bias[c] : 0.0f)));
+    }
+  }
+}
+
+Plan plan_of(const Shape& s, int size, bool aligned) { return make_plan(s, size, kK, num_sms(), aligned); }
+
+}  // namespace
+
+size_t forward_workspace(const Shape& s, int size) {
+  size_t bytes = 16;
+  for (bool aligned : {false, true}) {
+    const Plan p = plan_of(s, size, aligned);
+    if (p.kind == kTiles && !p.fused) bytes = std::max(bytes, sizeof(float2) * static_cast<size_t>(s.B) * p.chunks * s.G);
+  }
+  return bytes;
+}
+
+namespace {
+
+template <typename T, typename U, int ACT, int VEC>
+int run(const T* x, U* y, float* mean, float* rstd, const float* w, const float* bias, const Shape& s, const Plan& p, float eps,
+        void* ws, cudaStream_t st) {
+  const char* what = "group_norm";
+  if (p.kind == kUnits) {
+    const int ahead = p.slots == 1 ? 4 : 1;
+    const int64_t blocks = (s.B + static_cast<int64_t>(p.rows) * ahead - 1) / (static_cast<int64_t>(p.rows) * ahead);
+    const unsigned grid = static_cast<unsigned>(std::min<int64_t>(blocks, num_sms() * (2048 / p.threads)));
+    if (p.slots == 1) units_kernel<T, U, ACT, VEC, 1><<<grid, p.threads, 0, st>>>(x, y, mean, rstd, w, bias, s, p, eps);
+    else units_kernel<T, U, ACT, VEC, 4><<<grid, p.threads, 0, st>>>(x, y, mean, rstd, w, bias, s, p, eps);
+    return launched(what);
+  }
+  const int64_t works = s.B * p.slabs * p.chunks, most = static_cast<int64_t>(1) << 30;
+  unsigned grid = static_cast<unsigned>(std::min(works, most / p.chunks * p.chunks));
+  float2* parts = static_cast<float2*>(ws);
+  Shape shape = s;
+  Plan plan = p;
+  void* args[] = {&x, &y, &mean, &rstd, &w, &bias, &shape, &plan, &eps, &parts};
+  if (p.fused) return launch(reinterpret_cast<const void*>(&tiles_kernel<T, U, ACT, VEC, kFused>), grid, p.threads, p.chunks, st, args, what);
+  if (int e = launch(reinterpret_cast<const void*>(&tiles_kernel<T, U, BPC_ACT_NONE, VEC, kStats>), grid, p.threads, 1, st, args, what)) return e;
+  return launch(reinterpret_cast<const void*>(&tiles_kernel<T, U, ACT, VEC, kApply>), grid, p.threads, 1, st, args, what);
+}
+
+}  // namespace
+}  // namespace gn
+}  // namespace bpc
+
+using namespace bpc;
+using namespace bpc::gn;
+
+extern "C" int bpc_group_norm_fwd(const void* x, void* y, float* mean, float* rstd, const float* weight, const float* bias,
+                                  int64_t B, int64_t N, int32_t C, int32_t G, int64_t x_sample_stride,
+                                  int64_t x_row_stride, float eps, int32_t activation, int32_t x_dtype, int32_t y_dtype,
+                                  void* workspace, size_t workspace_bytes, bpc_stream_t stream) {
+  const Shape s{B, N, C, G, x_sample_stride, x_row_stride, 0, 0};
+  const char* what = "group_norm";
+  if (int e = check_shape(s, activation, x_dtype, y_dtype, what)) return e;
+  if (!(eps >= 0.0f) || std::isinf(eps)) return fail(BPC_ERR_ARG, "group_norm: eps must be finite and not negative");
+  if (!mean != !rstd) return fail(BPC_ERR_ARG, "group_norm: give both mean and rstd, or neither");
+  if (B == 0 || N == 0) return 0;
+  if (!x || !y || !workspace) return fail(BPC_ERR_ARG, "group_norm: null buffer");
+  const int size = size_of(x_dtype);
+  if (!aligned(x, size) || !aligned(y, size_of(y_dtype)) || !aligned(mean, 4) || !aligned(rstd, 4) || !aligned(weight, 4) ||
+      !aligned(bias, 4) || !aligned(workspace, 16))
+    return fail(BPC_ERR_ARG, "group_norm: buffer not aligned to its type (workspace: 16 bytes)");
+  if (workspace_bytes < bpc_group_norm_workspace_size(B, N, C, G, x_dtype, 0)) return fail(BPC_ERR_SPACE, "group_norm: workspace too small");
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const bool whole = aligned(x, 16) && aligned(y, 16) && x_sample_stride * size % 16 == 0 && x_row_stride * size % 16 == 0;
+  const Plan p = plan_of(s, size, whole);
+  return with_types(x_dtype, y_dtype, [&](auto xt, auto yt) {
+    return with_act(activation, [&](auto act) {
+      typedef typename decltype(xt)::type T;
+      typedef typename decltype(yt)::type U;
+      constexpr int ACT = decltype(act)::value;
+      const T* from = static_cast<const T*>(x);
+      U* to = static_cast<U*>(y);
+      if (p.kind == kWide) {
+        const unsigned grid = static_cast<unsigned>(std::min<int64_t>(B * G, 8 * num_sms()));
+        wide_kernel<T, U, ACT><<<grid, 256, 0, st>>>(from, to, mean, rstd, weight, bias, s, eps);
+        return launched(what);
+      }
+      if (p.vec == 1) return run<T, U, ACT, 1>(from, to, mean, rstd, weight, bias, s, p, eps, workspace, st);
+      return run<T, U, ACT, 16 / sizeof(T)>(from, to, mean, rstd, weight, bias, s, p, eps, workspace, st);
+    });
+  });
+}

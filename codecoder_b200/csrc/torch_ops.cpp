@@ -283,7 +283,7 @@ const float* f32_or_null(const Tensor& t) { return t.defined() ? static_cast<con
 
 Tensor norm_workspace(const Tensor& x, int64_t groups, bool backward) {
   return empty({static_cast<int64_t>(entry.group_norm_workspace_size(x.size(0), x.size(1), static_cast<int32_t>(x.size(2)),
-                                                                     static_cast<int32_t>(groups), backward))},
+                                                                     static_cast<int32_t>(groups), dtype_code(x.scalar_type()), backward))},
                at::kByte, x);
 }
 

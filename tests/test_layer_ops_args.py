@@ -44,12 +44,14 @@ def test_group_norm_refusals(lib):
     refused(call(f, ok, rs=-8), "strides")
     refused(call(f, ok, eps=-1e-5), "eps")
     refused(call(f, ok, eps=float("nan")), "eps")
+    refused(call(f, ok, mean=16), "both")
+    ok.update(mean=16, rstd=16)
     for name, at in (("x", 18), ("y", 17), ("mean", 18), ("rstd", 18), ("w", 18), ("b", 18), ("ws", 8)):
         refused(call(f, ok, **{name: at}), "aligned")
     refused(call(f, ok, wsb=0), "workspace", code=6)
     assert call(f, ok, B=0, x=None, y=None) == 0 and call(f, ok, N=0, x=None, y=None) == 0
     size = lib.bpc_group_norm_workspace_size
-    assert size(0, 3, 8, 2, 0) == 0 and size(2, 3, 8, 3, 0) == 0
+    assert size(0, 3, 8, 2, F32, 0) == 0 and size(2, 3, 8, 3, F32, 0) == 0 and size(2, 3, 8, 2, 9, 0) == 0
 
 
 def test_group_norm_backward_refusals(lib):
