@@ -24,35 +24,98 @@ __device__ __forceinline__ void store_f32(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store_f32(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 __device__ __forceinline__ void store_f32(__half* p, float v) { *p = __float2half_rn(v); }
 
+// VEC elements of an access.  Arithmetic is on pairs of them in fp32 (f2_* of bpc_common.cuh: half the instructions); a single
+// element has a pair with a zero beside it.
 template <typename T, int VEC>
 struct alignas(sizeof(T) * VEC) Pack {
+  static constexpr int kPairs = (VEC + 1) / 2;
   T v[VEC];
-  __device__ __forceinline__ float get(int e) const { return load_f32(&v[e]); }
-  __device__ __forceinline__ void set(int e, float f) { store_f32(&v[e], f); }
+  __device__ __forceinline__ uint64_t pair(int k) const {
+    if constexpr (VEC == 1) return f2_pack(load_f32(&v[0]), 0.0f);
+    else return f2_pack(load_f32(&v[2 * k]), load_f32(&v[2 * k + 1]));
+  }
+  __device__ __forceinline__ void set(int k, uint64_t x) {
+    if constexpr (VEC == 1) {
+      store_f32(&v[0], f2_lo(x));
+    } else if constexpr (sizeof(T) == 4) {
+      v[2 * k] = f2_lo(x), v[2 * k + 1] = f2_hi(x);
+    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      *reinterpret_cast<__nv_bfloat162*>(&v[2 * k]) = __floats2bfloat162_rn(f2_lo(x), f2_hi(x));
+    } else {
+      *reinterpret_cast<__half2*>(&v[2 * k]) = __floats2half2_rn(f2_lo(x), f2_hi(x));
+    }
+  }
 };
+template <int VEC>
+__device__ __forceinline__ float both(uint64_t x) {
+  return VEC == 1 ? f2_lo(x) : f2_lo(x) + f2_hi(x);
+}
+__device__ __forceinline__ uint64_t f2_of(float x) { return f2_pack(x, x); }
+
+// per-channel parameters of a vector from channel c on, `other` where there are none
+template <int VEC>
+__device__ __forceinline__ void channels(const float* p, int c, bool there, float other, uint64_t (&out)[(VEC + 1) / 2]) {
+#pragma unroll
+  for (int k = 0; k < (VEC + 1) / 2; ++k) {
+    const float lo = there && p ? __ldg(p + c + 2 * k) : other;
+    out[k] = f2_pack(lo, VEC == 1 ? 0.0f : there && p ? __ldg(p + c + (VEC == 1 ? 0 : 2 * k + 1)) : other);
+  }
+}
 
 // s(u) = 1 / (1 + e^-u); relative errors of a few 2^-24 and |u| 2^-23, whatever u is
-__device__ __forceinline__ float logistic(float u) { return __fdividef(1.0f, 1.0f + __expf(-u)); }
+__device__ __forceinline__ uint64_t logistic(uint64_t u) {
+  const uint64_t t = f2_mul(u, f2_of(-1.4426950408889634f));
+  float e0, e1;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(f2_lo(t)));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(f2_hi(t)));
+  const uint64_t d = f2_add(f2_pack(e0, e1), f2_of(1.0f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(f2_lo(d)));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(f2_hi(d)));
+  return f2_pack(e0, e1);
+}
 
-// act(z) = z s(u), act'(z) = s + z s (1 - s) u'
+// act(z) = z s(u(z)) and act'(z) = s (1 + z u' (1 - s))
 constexpr float kGelu = 1.5957691216057308f;      // 2 sqrt(2 / pi)
+constexpr float kGelu3 = 0.044715f * kGelu;
 template <int ACT>
-__device__ __forceinline__ float activate(float z) {
+__device__ __forceinline__ uint64_t activate(uint64_t z) {
   if constexpr (ACT == BPC_ACT_NONE) return z;
-  else if constexpr (ACT == BPC_ACT_SILU) return z * logistic(z);
-  else return z * logistic(kGelu * z * fmaf(0.044715f * z, z, 1.0f));
+  else if constexpr (ACT == BPC_ACT_SILU) return f2_mul(z, logistic(z));
+  else return f2_mul(z, logistic(f2_mul(z, f2_fma(f2_mul(z, z), f2_of(kGelu3), f2_of(kGelu)))));
 }
 template <int ACT>
-__device__ __forceinline__ float slope(float z) {
-  if constexpr (ACT == BPC_ACT_NONE) {
-    return 1.0f;
-  } else if constexpr (ACT == BPC_ACT_SILU) {
-    const float s = logistic(z);
-    return fmaf(z * s, 1.0f - s, s);
+__device__ __forceinline__ uint64_t slope(uint64_t z) {
+  if constexpr (ACT == BPC_ACT_NONE) return f2_of(1.0f);
+  uint64_t s, zu = z;
+  if constexpr (ACT == BPC_ACT_SILU) {
+    s = logistic(z);
   } else {
-    const float s = logistic(kGelu * z * fmaf(0.044715f * z, z, 1.0f));
-    return fmaf(z * s * (1.0f - s), kGelu * fmaf(3.0f * 0.044715f * z, z, 1.0f), s);
+    const uint64_t zz = f2_mul(z, z);
+    s = logistic(f2_mul(z, f2_fma(zz, f2_of(kGelu3), f2_of(kGelu))));
+    zu = f2_mul(z, f2_fma(zz, f2_of(3.0f * kGelu3), f2_of(kGelu)));
   }
+  return f2_mul(s, f2_fma(zu, f2_fma(s, f2_of(-1.0f), f2_of(1.0f)), f2_of(1.0f)));
+}
+// the wide kernels' single values
+template <int ACT>
+__device__ __forceinline__ float activate1(float z) {
+  return f2_lo(activate<ACT>(f2_pack(z, 0.0f)));
+}
+template <int ACT>
+__device__ __forceinline__ float slope1(float z) {
+  return f2_lo(slope<ACT>(f2_pack(z, 0.0f)));
+}
+
+// sum / n with per = 1 / n rounded: the quotient of a product and its remainder, exact where the quotient is a number of fp32
+__device__ __forceinline__ float over(float sum, float n, float per) {
+  const float q = sum * per;
+  return fmaf(fmaf(-q, n, sum), per, q);
+}
+
+// 1 / sqrt(v) to within 2^-23: the approximation and one step of Newton's, but at the ends, where that has no value
+__device__ __forceinline__ float inverse_sqrt(float v) {
+  const float r = rsqrtf(v), n = r * fmaf(-0.5f * v * r, r, 1.5f);
+  return v > 1e-30f && v < 1e30f ? n : 1.0f / sqrtf(v);
 }
 
 struct Shape {
@@ -70,6 +133,8 @@ struct Shape {
 //   wide   groups too wide for a row of threads: a block per sample and group in loops
 enum Kind { kUnits, kTiles, kWide };
 constexpr int kCluster = 8;
+constexpr int kRows = 8;             // of a thread's registers
+constexpr int kTileVec = 4;          // elements of a tile's access, whatever their type: eight rows of eight would not stay in registers
 struct Plan {
   Kind kind;
   int vec;                        // elements per access
@@ -80,76 +145,167 @@ struct Plan {
   int threads;
 };
 
-constexpr int kMaxThreads = 512;
+constexpr int kUnitThreads = 512;    // at most
+constexpr int kTileThreads = 256;
 
-// rows a thread holds; whole-width accesses need everything on 16-byte boundaries (`aligned`)
-inline Plan make_plan(const Shape& s, int size, int k_rows, int sms, bool aligned) {
+// full: elements of a whole access of units, taken where the pointers and strides allow it (`aligned`) and the groups hold whole
+// ones; of tiles kTileVec
+inline Plan make_plan(const Shape& s, int size, int full, int sms, bool aligned) {
   Plan p = {};
-  const int cg = s.C / s.G, full = 16 / size;
+  const int cg = s.C / s.G;
   p.vec = aligned && cg % full == 0 ? full : 1;
-  const int across = cg / p.vec;
+  int across = cg / p.vec;
   // small samples, of which a block per sample and slab would have little: 32-byte pieces of rows at least, or whole rows
   const int64_t vectors = s.N * across;
   if (vectors <= 128 && (s.N == 1 || cg * size >= 32)) {
     p.lanes = 1;
     while (p.lanes < 32 && p.lanes < vectors) p.lanes *= 2;
     p.slots = vectors <= p.lanes ? 1 : 4;
-    if (static_cast<int64_t>(p.lanes) * s.G <= kMaxThreads) {
+    if (static_cast<int64_t>(p.lanes) * s.G <= kUnitThreads) {
       p.kind = kUnits;
       p.rows = std::max(1, 256 / (p.lanes * s.G));
       p.threads = (p.lanes * s.G * p.rows + 31) / 32 * 32;
       return p;
     }
   }
-  if (across > kMaxThreads) {
+  p.vec = aligned && cg % kTileVec == 0 ? kTileVec : 1;
+  across = cg / p.vec;
+  if (across > kTileThreads) {
     p.kind = kWide;
     p.threads = 256;
     return p;
   }
   p.kind = kTiles;
-  // slabs of 64-byte rows or one group, whichever is wider
-  const int groups = std::min(s.G, std::max(1, std::min((64 / size + cg - 1) / cg, kMaxThreads / across)));
-  p.slab = groups * cg;
-  p.slabs = (s.G + groups - 1) / groups;
-  p.V = p.slab / p.vec;
-  int lanes = std::max(1, 256 / p.V);
-  if (s.N > static_cast<int64_t>(lanes) * k_rows) lanes = std::max(1, kMaxThreads / p.V);
-  // few blocks: more chunks, down to a row per thread
-  const int64_t blocks = s.B * p.slabs;
-  int64_t chunks = (s.N + static_cast<int64_t>(lanes) * k_rows - 1) / (static_cast<int64_t>(lanes) * k_rows);
-  if (chunks <= kCluster) {
-    while (chunks < kCluster && blocks * chunks * 2 <= sms && s.N >= lanes * chunks * 2) chunks *= 2;
-    chunks = std::min<int64_t>(chunks, kCluster);
+  // slabs of 64-byte rows or one group, whichever is wider; of 32-byte rows where they keep the sample in a cluster
+  for (int bytes = 64; bytes >= 32; bytes /= 2) {
+    const int groups = std::min(s.G, std::max(1, std::min((bytes / size + cg - 1) / cg, kTileThreads / across)));
+    p.slab = groups * cg;
+    p.slabs = (s.G + groups - 1) / groups;
+    p.V = p.slab / p.vec;
+    const int lanes = kTileThreads / p.V;
+    int64_t chunks = (s.N + static_cast<int64_t>(lanes) * kRows - 1) / (static_cast<int64_t>(lanes) * kRows);
+    // few blocks: more chunks, down to two rows per thread
+    while (chunks * 2 <= kCluster && s.B * p.slabs * chunks * 2 <= sms && s.N >= lanes * chunks * 4) chunks *= 2;
+    p.fused = chunks <= kCluster;
+    p.chunk_rows = static_cast<int>((s.N + chunks - 1) / chunks);
+    p.chunks = static_cast<int>((s.N + p.chunk_rows - 1) / p.chunk_rows);
+    p.threads = (std::min(lanes, p.chunk_rows) * p.V + 31) / 32 * 32;
+    if (p.fused) break;
   }
-  p.fused = chunks <= kCluster;
-  p.chunk_rows = static_cast<int>((s.N + chunks - 1) / chunks);
-  p.chunks = static_cast<int>((s.N + p.chunk_rows - 1) / p.chunk_rows);
-  p.threads = (std::min(lanes, p.chunk_rows) * p.V + 31) / 32 * 32;
   return p;
 }
 
-// Sums over the threads of each group of a slab: thread (row r, vector v) has v, groups of `across` vectors; the sums of
-// group j come out in out[j].  part: a float per thread.
-__device__ __forceinline__ void group_sums(float value, int V, int rows, int across, int groups, float* part, float* out) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  int entries = rows;
-  if (V <= 32 && (V & (V - 1)) == 0) {
-    for (int d = 16; d >= V; d >>= 1) value += __shfl_xor_sync(0xffffffffu, value, d);
-    if (lane < V) part[warp * V + lane] = value;
-    entries = warps;
-  } else if (threadIdx.x < rows * V) {
-    part[threadIdx.x] = value;
-  }
-  __syncthreads();
-  for (int j = warp; j < groups; j += warps) {
-    float sum = 0.0f;
-    for (int i = lane; i < entries * across; i += 32) sum += part[i / across * V + j * across + i % across];
+// The sums of N values over the threads of the calling thread's group of a slab, in each of them: thread (row r, vector v) has
+// vector v of V, groups of `across` vectors.  part: N floats per tile thread, free again after the next barrier but one.
+template <int N>
+__device__ __forceinline__ void group_sums(float (&value)[N], int V, int rows, int across, int v, float* part) {
+  constexpr int kWarps = kTileThreads / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, j = v / across;
+  if (V <= 32 && (V & (V - 1)) == 0) {             // so is across: a warp's lanes of a group join by shuffles
+    const int joins = ~(V - 1) | (across - 1);     // the bits of the lane that its group does not say
 #pragma unroll
-    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    if (lane == 0) out[j] = sum;
+    for (int d = 16; d; d >>= 1)
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const float t = __shfl_xor_sync(0xffffffffu, value[k], d);
+        value[k] += d & joins ? t : 0.0f;
+      }
+    // [value][group][warp]
+    if (lane < V && lane % across == 0) {
+#pragma unroll
+      for (int k = 0; k < N; ++k) part[k * kTileThreads + lane / across * kWarps + warp] = value[k];
+    }
+    __syncthreads();
+    const int warps = blockDim.x >> 5;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const float* f = part + k * kTileThreads + j * kWarps;
+      float4 a = *reinterpret_cast<const float4*>(f), b = *reinterpret_cast<const float4*>(f + 4);
+      if (warps < kWarps) {
+        a = make_float4(a.x, warps > 1 ? a.y : 0.0f, warps > 2 ? a.z : 0.0f, warps > 3 ? a.w : 0.0f);
+        b = make_float4(warps > 4 ? b.x : 0.0f, warps > 5 ? b.y : 0.0f, warps > 6 ? b.z : 0.0f, 0.0f);
+      }
+      value[k] = ((a.x + a.y) + (a.z + a.w)) + ((b.x + b.y) + (b.z + b.w));
+    }
+    return;
+  }
+  if (threadIdx.x < rows * V) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) part[k * kTileThreads + threadIdx.x] = value[k];
   }
   __syncthreads();
+  // a warp per group; the sums go where its first thread's values were, when all of them are read
+  for (int g = warp; g < V / across; g += blockDim.x >> 5) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      float* f = part + k * kTileThreads + g * across;
+      float sum = 0.0f;
+      for (int i = lane; i < rows * across; i += 32) sum += f[i / across * V + i % across];
+#pragma unroll
+      for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      if (lane == 0) f[0] = sum;                   // read by this warp alone until here
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < N; ++k) value[k] = part[k * kTileThreads + j * across];
 }
+
+// f(a constant true or false): whether all of a thread's rows are there, so that most threads need not ask for each
+template <typename F>
+__device__ __forceinline__ void with_rows(bool all, F f) {
+  if (all) f(std::true_type());
+  else f(std::false_type());
+}
+
+__device__ __forceinline__ void cp_async(void* dst, const void* src, std::integral_constant<int, 16>) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async(void* dst, const void* src, std::integral_constant<int, 8>) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void cp_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// A thread's rows of the next piece of work on their way through shared memory, K vectors of its own (no barrier): fetch
+// starts the copies, take waits for them.  Single elements are read when taken.
+template <typename T, int VEC, int K>
+struct Ahead {
+  static constexpr bool kStaged = VEC > 1;
+  static constexpr int kBytes = kStaged ? K * static_cast<int>(sizeof(T)) * VEC : 0;      // per thread
+  using P = Pack<T, VEC>;
+  P* at;
+  const T* from;
+  int64_t step;
+  int n;
+  __device__ __forceinline__ explicit Ahead(uint8_t* smem) : at(reinterpret_cast<P*>(smem) + threadIdx.x), from(nullptr), step(0), n(0) {}
+  // n of K vectors, `step` elements apart
+  __device__ __forceinline__ void fetch(const T* src, int64_t step_, int n_) {
+    from = src, step = step_, n = n_;
+    if constexpr (kStaged) {
+      with_rows(n == K, [&](auto all) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          if (decltype(all)::value || k < n) cp_async(at + k * kTileThreads, src, std::integral_constant<int, static_cast<int>(sizeof(P))>());
+          src += step;
+        }
+      });
+    }
+  }
+  __device__ __forceinline__ void take(P (&d)[K]) const {
+    if constexpr (kStaged) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) d[k] = at[k * kTileThreads];      // without meaning behind n
+    } else {
+      const T* src = from;
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        if (k < n) d[k] = *reinterpret_cast<const P*>(src);
+        src += step;
+      }
+    }
+  }
+};
 
 inline int launched(const char* what) {
   const cudaError_t e = cudaGetLastError();
@@ -157,10 +313,13 @@ inline int launched(const char* what) {
 }
 
 // One launch, as clusters of `cluster` blocks
-inline int launch(const void* fn, unsigned grid, int threads, int cluster, cudaStream_t s, void** args, const char* what) {
+inline int launch(const void* fn, dim3 grid, int threads, int cluster, int smem, cudaStream_t s, void** args, const char* what) {
+  if (smem > 32 * 1024)          // beside a few KB of static memory
+    if (int e = allow_smem(fn, smem)) return e;
   cudaLaunchConfig_t lc = {};
-  lc.gridDim = dim3(grid);
+  lc.gridDim = grid;
   lc.blockDim = dim3(threads);
+  lc.dynamicSmemBytes = smem;
   lc.stream = s;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -170,6 +329,13 @@ inline int launch(const void* fn, unsigned grid, int threads, int cluster, cudaS
   lc.numAttrs = cluster > 1 ? 1 : 0;
   const cudaError_t e = cudaLaunchKernelExC(&lc, fn, args);
   return e == cudaSuccess ? 0 : fail(BPC_ERR_LAUNCH, std::string(what) + " launch: " + cudaGetErrorString(e));
+}
+
+// Blocks of x, y: every slab and chunk, and the samples that a slab's blocks walk at once; `per_sm` blocks of 256 threads
+inline dim3 tiles_grid(const Shape& s, const Plan& p, int per_sm, int sms) {
+  const int64_t across = static_cast<int64_t>(p.slabs) * p.chunks;
+  const int64_t resident = static_cast<int64_t>(sms) * std::max(1, per_sm * 256 / p.threads);
+  return dim3(static_cast<unsigned>(across), static_cast<unsigned>(std::min<int64_t>({s.B, 65535, std::max<int64_t>(1, resident / across)})));
 }
 
 inline int size_of(int32_t dtype) { return dtype == BPC_DTYPE_F32 ? 4 : dtype == BPC_DTYPE_BF16 || dtype == BPC_DTYPE_F16 ? 2 : 0; }
@@ -215,11 +381,6 @@ inline int check_shape(const Shape& s, int32_t act, int32_t x_dtype, int32_t y_d
     return bad("strides outside [0, 2^40]");
   return 0;
 }
-
-// Rows of a thread's registers: 16 bytes of x each.  The backward pass keeps gz in fp32 beside x: half as many of 16-bit
-// features.
-constexpr int kForwardRows = 8;
-inline int backward_rows(int size) { return size == 4 ? 8 : 4; }
 
 }  // namespace gn
 }  // namespace bpc

@@ -15,17 +15,22 @@ namespace {
 
 namespace cg_ = cooperative_groups;
 
+constexpr int kVec = kTileVec;      // of units too: the sums, the weights and gz are in the registers beside the features
+
 // The channels' sums of a block: thread (row r, vector v) has VEC channels from c on, `rows` rows of threads; into
 // parts[block][2][C]
 template <int VEC>
-__device__ __forceinline__ void channel_sums(const float (&a)[VEC], const float (&d)[VEC], int v, int V, int r, int rows, int c, int C,
-                                             bool there, float* buffer, float* parts) {
+__device__ __forceinline__ void channel_sums(const uint64_t (&a)[(VEC + 1) / 2], const uint64_t (&d)[(VEC + 1) / 2], int v, int V, int r,
+                                             int rows, int c, int C, bool there, float* buffer, float* parts) {
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     __syncthreads();
     if (there) {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) buffer[(r * V + v) * VEC + i] = which ? d[i] : a[i];
+      for (int i = 0; i < VEC; ++i) {
+        const uint64_t x = which ? d[i / 2] : a[i / 2];
+        buffer[(r * V + v) * VEC + i] = i % 2 ? f2_hi(x) : f2_lo(x);
+      }
     }
     __syncthreads();
     if (there && r == 0) {
@@ -41,7 +46,7 @@ __device__ __forceinline__ void channel_sums(const float (&a)[VEC], const float 
 
 // Units: a sample's group per `lanes` lanes, SLOTS vectors each; a thread's slots are the same places of every sample.
 template <typename T, typename U, int ACT, int VEC, int SLOTS>
-__global__ void __launch_bounds__(kMaxThreads) units_kernel(const U* __restrict__ gy, const T* __restrict__ x,
+__global__ void __launch_bounds__(kUnitThreads) units_kernel(const U* __restrict__ gy, const T* __restrict__ x,
                                                             const float* __restrict__ mean_in,
                                                             const float* __restrict__ rstd_in, const float* __restrict__ w,
                                                             const float* __restrict__ bias, T* __restrict__ dx, float* parts,
@@ -53,25 +58,26 @@ __global__ void __launch_bounds__(kMaxThreads) units_kernel(const U* __restrict_
   const int g = unit % s.G, r = unit / s.G;
   const bool there = r < p.rows;
   const int64_t step = static_cast<int64_t>(gridDim.x) * p.rows;
-  int64_t in_x[SLOTS], in_g[SLOTS];
+  constexpr int kP = Pack<T, VEC>::kPairs;
+  const T* in_x[SLOTS];
+  const U* in_g[SLOTS];
   int out[SLOTS];
   bool has[SLOTS];
-  float wv[SLOTS][VEC], bv[SLOTS][VEC], acc_a[SLOTS][VEC], acc_b[SLOTS][VEC];
+  uint64_t wv[SLOTS][kP], bv[SLOTS][kP], acc_a[SLOTS][kP], acc_b[SLOTS][kP];
 #pragma unroll
   for (int k = 0; k < SLOTS; ++k) {
     const int e = k * p.lanes + l, row = e / across, c = g * cg + e % across * VEC;
     has[k] = there && row < s.N;
-    in_x[k] = row * s.x_row + c;
-    in_g[k] = row * s.g_row + c;
+    in_x[k] = x + row * s.x_row + c;
+    in_g[k] = gy + row * s.g_row + c;
     out[k] = row * s.C + c;
+    channels<VEC>(w, c, has[k], 1.0f, wv[k]);
+    channels<VEC>(bias, c, has[k], 0.0f, bv[k]);
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      wv[k][i] = has[k] && w ? w[c + i] : 1.0f;
-      bv[k][i] = has[k] && bias ? bias[c + i] : 0.0f;
-      acc_a[k][i] = acc_b[k][i] = 0.0f;
-    }
+    for (int i = 0; i < kP; ++i) acc_a[k][i] = acc_b[k][i] = 0;
   }
   const float per = 1.0f / static_cast<float>(n);
+  const int64_t o_sample = s.N * s.C;
   for (int64_t b0 = static_cast<int64_t>(blockIdx.x) * p.rows + r; b0 - r < s.B; b0 += kAhead * step) {
     Pack<T, VEC> vx[kAhead][SLOTS];
     Pack<U, VEC> vg[kAhead][SLOTS];
@@ -83,48 +89,50 @@ __global__ void __launch_bounds__(kMaxThreads) units_kernel(const U* __restrict_
       mean[a] = live ? mean_in[b * s.G + g] : 0.0f;
       rstd[a] = live ? rstd_in[b * s.G + g] : 0.0f;
 #pragma unroll
-      for (int k = 0; k < SLOTS; ++k)
+      for (int k = 0; k < SLOTS; ++k) {
         if (has[k] && live) {
-          vx[a][k] = *reinterpret_cast<const Pack<T, VEC>*>(x + b * s.x_sample + in_x[k]);
-          vg[a][k] = *reinterpret_cast<const Pack<U, VEC>*>(gy + b * s.g_sample + in_g[k]);
+          vx[a][k] = *reinterpret_cast<const Pack<T, VEC>*>(in_x[k] + b * s.x_sample);
+          vg[a][k] = *reinterpret_cast<const Pack<U, VEC>*>(in_g[k] + b * s.g_sample);
+        } else {
+          vx[a][k] = Pack<T, VEC>(), vg[a][k] = Pack<U, VEC>();      // zeros: nothing to any sum
         }
+      }
     }
 #pragma unroll
     for (int a = 0; a < kAhead; ++a) {
       const int64_t b = b0 + a * step;
       const bool live = b < s.B;
-      float gz[SLOTS][VEC], s1 = 0.0f, s2 = 0.0f;
+      const uint64_t scale = f2_of(rstd[a]), minus = f2_of(-mean[a]);
+      uint64_t gz[SLOTS][kP], s1 = 0, s2 = 0;
 #pragma unroll
       for (int k = 0; k < SLOTS; ++k)
-        if (has[k] && live) {
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            const float xh = (vx[a][k].get(i) - mean[a]) * rstd[a];
-            gz[k][i] = vg[a][k].get(i) * slope<ACT>(fmaf(wv[k][i], xh, bv[k][i]));
-            acc_a[k][i] += gz[k][i];
-            acc_b[k][i] = fmaf(gz[k][i], xh, acc_b[k][i]);
-            const float t = gz[k][i] * wv[k][i];
-            s1 += t;
-            s2 = fmaf(t, xh, s2);
-          }
+        for (int i = 0; i < kP; ++i) {
+          const uint64_t xh = f2_mul(f2_add(vx[a][k].pair(i), minus), scale);
+          gz[k][i] = f2_mul(vg[a][k].pair(i), slope<ACT>(f2_fma(wv[k][i], xh, bv[k][i])));
+          acc_a[k][i] = f2_add(acc_a[k][i], gz[k][i]);
+          acc_b[k][i] = f2_fma(gz[k][i], xh, acc_b[k][i]);
+          const uint64_t t = f2_mul(gz[k][i], wv[k][i]);
+          s1 = f2_add(s1, t);
+          s2 = f2_fma(t, xh, s2);
         }
+      float m1 = both<VEC>(s1), m2 = both<VEC>(s2);
       for (int d = p.lanes >> 1; d; d >>= 1) {
-        s1 += __shfl_xor_sync(0xffffffffu, s1, d);
-        s2 += __shfl_xor_sync(0xffffffffu, s2, d);
+        m1 += __shfl_xor_sync(0xffffffffu, m1, d);
+        m2 += __shfl_xor_sync(0xffffffffu, m2, d);
       }
-      s1 *= per, s2 *= per;
       if (dx) {
+        const uint64_t u1 = f2_of(-m1 * per), u2 = f2_of(-m2 * per);
 #pragma unroll
-        for (int k = 0; k < SLOTS; ++k)
-          if (has[k] && live) {
-            Pack<T, VEC> o;
+        for (int k = 0; k < SLOTS; ++k) {
+          Pack<T, VEC> o;
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-              const float xh = (vx[a][k].get(i) - mean[a]) * rstd[a];
-              o.set(i, rstd[a] * (gz[k][i] * wv[k][i] - fmaf(xh, s2, s1)));
-            }
-            *reinterpret_cast<Pack<T, VEC>*>(dx + b * s.N * s.C + out[k]) = o;
+          for (int i = 0; i < kP; ++i) {
+            const uint64_t xh = f2_mul(f2_add(vx[a][k].pair(i), minus), scale);
+            o.set(i, f2_mul(scale, f2_fma(gz[k][i], wv[k][i], f2_fma(xh, u2, u1))));
           }
+          if (has[k] && live) *reinterpret_cast<Pack<T, VEC>*>(dx + b * o_sample + out[k]) = o;
+        }
       }
     }
   }
@@ -140,7 +148,10 @@ __global__ void __launch_bounds__(kMaxThreads) units_kernel(const U* __restrict_
       if (has[k]) {
         const int e = k * p.lanes + l, at = (r * static_cast<int>(s.N) + e / across) * V + g * across + e % across;
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) buffer[at * VEC + i] = which ? acc_b[k][i] : acc_a[k][i];
+        for (int i = 0; i < VEC; ++i) {
+          const uint64_t t = which ? acc_b[k][i / 2] : acc_a[k][i / 2];
+          buffer[at * VEC + i] = i % 2 ? f2_hi(t) : f2_lo(t);
+        }
       }
     __syncthreads();
     for (int c = threadIdx.x; c < s.C; c += blockDim.x) {
@@ -153,104 +164,112 @@ __global__ void __launch_bounds__(kMaxThreads) units_kernel(const U* __restrict_
 
 enum Mode { kFused, kSums, kApply };
 
-// Tiles: a block's chunk of a slab in registers; blocks keep their slab (and chunk, where fused) and walk the samples.
-// between: (B, chunks, G) pairs s1, s2 between the two kernels of samples that no cluster holds.
+// Tiles: a block's chunk of a slab in registers, the next sample's on its way meanwhile; blocks keep their slab and chunk and
+// walk the samples.  between: (B, chunks, G) pairs s1, s2 between the two kernels of samples that no cluster holds.
 template <typename T, typename U, int ACT, int VEC, int MODE>
-__global__ void __launch_bounds__(kMaxThreads) tiles_kernel(const U* __restrict__ gy, const T* __restrict__ x,
+__global__ void __launch_bounds__(kTileThreads, 2) tiles_kernel(const U* __restrict__ gy, const T* __restrict__ x,
                                                             const float* __restrict__ mean_in,
                                                             const float* __restrict__ rstd_in, const float* __restrict__ w,
                                                             const float* __restrict__ bias, T* __restrict__ dx, float* parts,
                                                             const Shape s, const Plan p, float2* between) {
-  constexpr int kK = sizeof(T) == 4 ? 8 : 4;
-  __shared__ float part[kMaxThreads];
-  __shared__ float first[kMaxThreads], second[kMaxThreads];
-  __shared__ float2 mine[kMaxThreads];
-  __shared__ float buffer[kMaxThreads * VEC];
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ __align__(16) float part[2][2 * kTileThreads];
+  __shared__ float2 mine[kTileThreads];
   const int cg = s.C / s.G, across = cg / VEC, groups = p.slab / cg;
-  const int v = threadIdx.x % p.V, r = threadIdx.x / p.V, lanes = blockDim.x / p.V;
-  // fused: clusters of chunks, slab fastest; else blocks, slab fastest, walking samples and chunks
-  const int per_team = MODE == kFused ? p.chunks : 1;
-  const int team = blockIdx.x / per_team, slab = team % p.slabs, first_work = team / p.slabs;
-  const int teams = gridDim.x / per_team / p.slabs;
-  const int c = slab * p.slab + v * VEC, j = v / across, g = slab * groups + j;
-  const bool there = r < lanes && c < s.C;
-  float wv[VEC], bv[VEC], acc_a[VEC], acc_b[VEC];
+  const int v = threadIdx.x % p.V, r = threadIdx.x / p.V, lanes = blockDim.x / p.V, j = v / across;
+  // what the other kernel read last is read first
+  const int chunk0 = blockIdx.x % p.chunks, slab = blockIdx.x / p.chunks, chunk = MODE == kApply ? p.chunks - 1 - chunk0 : chunk0;
+  const int c = slab * p.slab + v * VEC, g = slab * groups + j;
+  const int row0 = chunk * p.chunk_rows, rows = min(p.chunk_rows, static_cast<int>(s.N) - row0);
+  const bool there = r < lanes && c < s.C, speaks = there && r == 0 && v % across == 0;
+  const int n = there && r < rows ? (rows - r + lanes - 1) / lanes : 0;        // this thread's rows
+  auto sample = [&](int64_t k) { return MODE == kApply ? s.B - 1 - k : k; };
+  const T* from = x + static_cast<int64_t>(row0 + r) * s.x_row + c;
+  const U* from_g = gy + static_cast<int64_t>(row0 + r) * s.g_row + c;
+  T* to = dx + static_cast<int64_t>(row0 + r) * s.C + c;
+  const int64_t x_step = lanes * s.x_row, g_step = lanes * s.g_row, o_step = static_cast<int64_t>(lanes) * s.C;
+  Ahead<T, VEC, kRows> ahead_x(smem);
+  Ahead<U, VEC, kRows> ahead_g(smem + Ahead<T, VEC, kRows>::kBytes * kTileThreads);
+  float mean_next = 0.0f, rstd_next = 0.0f;
+  auto fetch = [&](int64_t b) {
+    ahead_x.fetch(from + b * s.x_sample, x_step, n);
+    ahead_g.fetch(from_g + b * s.g_sample, g_step, n);
+    if (there) mean_next = mean_in[b * s.G + g], rstd_next = rstd_in[b * s.G + g];
+  };
+  fetch(sample(blockIdx.y));
+  constexpr int kP = Pack<T, VEC>::kPairs;
+  uint64_t wv[kP], bv[kP], acc_a[kP], acc_b[kP];
+  channels<VEC>(w, c, there, 1.0f, wv);
+  channels<VEC>(bias, c, there, 0.0f, bv);
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) {
-    wv[i] = there && w ? __ldg(w + c + i) : 1.0f;
-    bv[i] = there && bias ? __ldg(bias + c + i) : 0.0f;
-    acc_a[i] = acc_b[i] = 0.0f;
-  }
+  for (int i = 0; i < kP; ++i) acc_a[i] = acc_b[i] = 0;
   const float per = 1.0f / (static_cast<float>(s.N) * static_cast<float>(cg));
-  const int64_t works = MODE == kFused ? s.B : s.B * p.chunks;
-  for (int64_t at = first_work; at < works; at += teams) {
-    const int64_t work = MODE == kApply ? works - 1 - at : at;      // what the other kernel read last is read first
-    const int64_t b = MODE == kFused ? work : work / p.chunks;
-    const int chunk = static_cast<int>(MODE == kFused ? blockIdx.x % p.chunks : work % p.chunks);
-    const int row0 = chunk * p.chunk_rows, rows = min(p.chunk_rows, static_cast<int>(s.N) - row0);
-    const float mean = there ? mean_in[b * s.G + g] : 0.0f, rstd = there ? rstd_in[b * s.G + g] : 0.0f;
-    Pack<T, VEC> vx[kK];
-    float gz[kK][VEC];
+  int turn = 0;
+  for (int64_t at = blockIdx.y; at < s.B; at += gridDim.y) {
+    const int64_t b = sample(at);
+    const uint64_t scale = f2_of(rstd_next), minus = f2_of(-mean_next);
+    Pack<T, VEC> vx[kRows];
+    uint64_t gz[kRows][kP];
+    float sums[2] = {0.0f, 0.0f};
+    cp_wait_all();
+    ahead_x.take(vx);
     {
-      Pack<U, VEC> vg[kK];
-      const T* from = x + b * s.x_sample + (row0 + r) * s.x_row + c;
-      const U* from_g = gy + b * s.g_sample + (row0 + r) * s.g_row + c;
+      Pack<U, VEC> vg[kRows];
+      ahead_g.take(vg);
+      uint64_t a[kP], d[kP];
 #pragma unroll
-      for (int k = 0; k < kK; ++k)
-        if (there && r + k * lanes < rows) {
-          vx[k] = *reinterpret_cast<const Pack<T, VEC>*>(from + k * lanes * s.x_row);
-          vg[k] = *reinterpret_cast<const Pack<U, VEC>*>(from_g + k * lanes * s.g_row);
-        }
+      for (int i = 0; i < kP; ++i) a[i] = d[i] = 0;
+      with_rows(n == kRows, [&](auto all) {
 #pragma unroll
-      for (int k = 0; k < kK; ++k)
-        if (there && r + k * lanes < rows) {
+        for (int k = 0; k < kRows; ++k)
+          if (decltype(all)::value || k < n) {
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) gz[k][i] = vg[k].get(i);
-        }
-    }
-    float s1 = 0.0f, s2 = 0.0f;
-#pragma unroll
-    for (int k = 0; k < kK; ++k)
-      if (there && r + k * lanes < rows) {
-        float t1 = 0.0f, t2 = 0.0f;
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const float xh = (vx[k].get(i) - mean) * rstd;
-          gz[k][i] *= slope<ACT>(fmaf(wv[i], xh, bv[i]));
-          if (MODE != kApply) {
-            acc_a[i] += gz[k][i];
-            acc_b[i] = fmaf(gz[k][i], xh, acc_b[i]);
-            const float t = gz[k][i] * wv[i];
-            t1 += t;
-            t2 = fmaf(t, xh, t2);
+            for (int i = 0; i < kP; ++i) {
+              const uint64_t xh = f2_mul(f2_add(vx[k].pair(i), minus), scale);
+              gz[k][i] = f2_mul(vg[k].pair(i), slope<ACT>(f2_fma(wv[i], xh, bv[i])));
+              if (MODE != kApply) {
+                a[i] = f2_add(a[i], gz[k][i]);
+                d[i] = f2_fma(gz[k][i], xh, d[i]);
+              }
+            }
           }
+      });
+      if constexpr (MODE != kApply) {
+        // the channels' sums of this sample, weighed, are the group's
+        uint64_t t1 = 0, t2 = 0;
+#pragma unroll
+        for (int i = 0; i < kP; ++i) {
+          acc_a[i] = f2_add(acc_a[i], a[i]);
+          acc_b[i] = f2_add(acc_b[i], d[i]);
+          t1 = f2_fma(a[i], wv[i], t1);
+          t2 = f2_fma(d[i], wv[i], t2);
         }
-        s1 += t1, s2 += t2;
+        sums[0] = both<VEC>(t1), sums[1] = both<VEC>(t2);
       }
+    }
+    if (at + gridDim.y < s.B) fetch(sample(at + gridDim.y));
     if constexpr (MODE != kApply) {
-      group_sums(s1, p.V, lanes, across, groups, part, first);
-      group_sums(s2, p.V, lanes, across, groups, part, second);
+      // two buffers in turn: a sample has one barrier
+      group_sums(sums, p.V, lanes, across, v, part[turn]);
+      turn ^= 1;
       if (MODE == kSums) {
-        if (there && r == 0 && v % across == 0) between[(b * p.chunks + chunk) * s.G + g] = make_float2(first[j], second[j]);
-        __syncthreads();
+        if (speaks) between[(b * p.chunks + chunk) * s.G + g] = make_float2(sums[0], sums[1]);
         continue;
       }
       if (p.chunks > 1) {
-        for (int k = threadIdx.x; k < groups; k += blockDim.x) mine[k] = make_float2(first[k], second[k]);
+        if (speaks) mine[j] = make_float2(sums[0], sums[1]);
         cg_::cluster_group cluster = cg_::this_cluster();
         cluster.sync();
-        for (int k = threadIdx.x; k < groups; k += blockDim.x) {
-          float t1 = 0.0f, t2 = 0.0f;
-          for (int q = 0; q < p.chunks; ++q) {
-            const float2 t = cluster.map_shared_rank(mine, q)[k];
-            t1 += t.x, t2 += t.y;
-          }
-          first[k] = t1, second[k] = t2;
+        sums[0] = sums[1] = 0.0f;
+        for (int q = 0; q < p.chunks; ++q) {
+          const float2 t = cluster.map_shared_rank(mine, q)[j];
+          sums[0] += t.x, sums[1] += t.y;
         }
         cluster.sync();                            // every block has read the others' parts
       }
     } else {
       const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+      __syncthreads();
       for (int k = warp; k < groups && slab * groups + k < s.G; k += warps) {
         const float2* f = between + b * p.chunks * s.G + slab * groups + k;
         float t1 = 0.0f, t2 = 0.0f;
@@ -263,32 +282,38 @@ __global__ void __launch_bounds__(kMaxThreads) tiles_kernel(const U* __restrict_
           t1 += __shfl_xor_sync(0xffffffffu, t1, m);
           t2 += __shfl_xor_sync(0xffffffffu, t2, m);
         }
-        if (lane == 0) first[k] = t1, second[k] = t2;
+        if (lane == 0) mine[k] = make_float2(t1, t2);
       }
       __syncthreads();
+      sums[0] = mine[j].x, sums[1] = mine[j].y;
     }
     if constexpr (MODE != kSums) {
-      if (dx && there) {
-        const float m1 = first[j] * per, m2 = second[j] * per;
-        T* to = dx + (b * s.N + row0 + r) * s.C + c;
+      if (dx) {
+        const uint64_t u1 = f2_of(-sums[0] * per), u2 = f2_of(-sums[1] * per);
+        T* out = to + b * s.N * s.C;
+        with_rows(n == kRows, [&](auto all) {
 #pragma unroll
-        for (int k = 0; k < kK; ++k)
-          if (r + k * lanes < rows) {
-            Pack<T, VEC> o;
+          for (int k = 0; k < kRows; ++k) {
+            if (decltype(all)::value || k < n) {
+              Pack<T, VEC> o;
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-              const float xh = (vx[k].get(i) - mean) * rstd;
-              o.set(i, rstd * (gz[k][i] * wv[i] - fmaf(xh, m2, m1)));
+              for (int i = 0; i < kP; ++i) {
+                const uint64_t xh = f2_mul(f2_add(vx[k].pair(i), minus), scale);
+                o.set(i, f2_mul(scale, f2_fma(gz[k][i], wv[i], f2_fma(xh, u2, u1))));
+              }
+              *reinterpret_cast<Pack<T, VEC>*>(out) = o;
             }
-            *reinterpret_cast<Pack<T, VEC>*>(to + static_cast<int64_t>(k) * lanes * s.C) = o;
+            out += o_step;
           }
+        });
       }
-      __syncthreads();                             // first and second are this work's until here
     }
   }
   if (MODE != kApply && parts) {
-    const int64_t row = MODE == kFused ? static_cast<int64_t>(first_work) * p.chunks + blockIdx.x % p.chunks : first_work;
-    channel_sums<VEC>(acc_a, acc_b, v, p.V, r, lanes, c, s.C, there, buffer, parts + row * 2 * s.C);
+    // the copies have all been taken: their memory holds the channels' sums now (VEC floats a thread are no more than them)
+    float* buffer = reinterpret_cast<float*>(smem);
+    channel_sums<VEC>(acc_a, acc_b, v, p.V, r, lanes, c, s.C, there, buffer,
+                      parts + (static_cast<int64_t>(blockIdx.y) * p.chunks + chunk) * 2 * s.C);
   }
 }
 
@@ -343,7 +368,7 @@ __global__ void __launch_bounds__(256) wide_kernel(const U* __restrict__ gy, con
       const int64_t r = i / cg;
       const float wc = w ? w[c] : 1.0f;
       const float xh = (load_f32(x + b * s.x_sample + r * s.x_row + c) - mean) * rstd;
-      const float a = load_f32(gy + b * s.g_sample + r * s.g_row + c) * slope<ACT>(fmaf(wc, xh, bias ? bias[c] : 0.0f)) * wc;
+      const float a = load_f32(gy + b * s.g_sample + r * s.g_row + c) * slope1<ACT>(fmaf(wc, xh, bias ? bias[c] : 0.0f)) * wc;
       s1 += a;
       s2 = fmaf(a, xh, s2);
     }
@@ -354,7 +379,7 @@ __global__ void __launch_bounds__(256) wide_kernel(const U* __restrict__ gy, con
       const int64_t r = i / cg;
       const float wc = w ? w[c] : 1.0f;
       const float xh = (load_f32(x + b * s.x_sample + r * s.x_row + c) - mean) * rstd;
-      const float a = load_f32(gy + b * s.g_sample + r * s.g_row + c) * slope<ACT>(fmaf(wc, xh, bias ? bias[c] : 0.0f)) * wc;
+      const float a = load_f32(gy + b * s.g_sample + r * s.g_row + c) * slope1<ACT>(fmaf(wc, xh, bias ? bias[c] : 0.0f)) * wc;
       store_f32(dx + (b * s.N + r) * s.C + c, rstd * (a - fmaf(xh, s2, s1)));
     }
   }
@@ -374,7 +399,7 @@ __global__ void __launch_bounds__(256) wide_channels_kernel(const U* __restrict_
   for (int64_t i = blockIdx.y; i < s.B * s.N; i += gridDim.y) {
     const int64_t b = i / s.N, r = i % s.N;
     const float xh = (load_f32(x + b * s.x_sample + r * s.x_row + c) - mean_in[b * s.G + g]) * rstd_in[b * s.G + g];
-    const float gz = load_f32(gy + b * s.g_sample + r * s.g_row + c) * slope<ACT>(fmaf(wc, xh, bc));
+    const float gz = load_f32(gy + b * s.g_sample + r * s.g_row + c) * slope1<ACT>(fmaf(wc, xh, bc));
     a += gz;
     d += static_cast<double>(gz) * xh;
   }
@@ -382,16 +407,15 @@ __global__ void __launch_bounds__(256) wide_channels_kernel(const U* __restrict_
   parts[static_cast<int64_t>(blockIdx.y) * 2 * s.C + s.C + c] = static_cast<float>(d);
 }
 
-Plan plan_of(const Shape& s, int size, bool aligned) { return make_plan(s, size, backward_rows(size), num_sms(), aligned); }
+Plan plan_of(const Shape& s, int size, bool aligned) { return make_plan(s, size, kVec, num_sms(), aligned); }
 
-// Blocks that walk the samples: as many as are resident, two of 512 threads per SM at most
-int64_t walkers(const Shape& s, const Plan& p) {
-  const int64_t resident = static_cast<int64_t>(num_sms()) * std::max(1, std::min(4, 640 / p.threads));
-  if (p.kind == kUnits) return std::min(resident, (s.B + p.rows - 1) / p.rows);
+constexpr int kTilesPerSm = 2;
+
+// Parts of dw and db: one per block that walks the samples, per slab
+int64_t parts_of(const Shape& s, const Plan& p) {
+  if (p.kind == kUnits) return std::min<int64_t>(static_cast<int64_t>(num_sms()) * std::max(1, 1024 / p.threads), (s.B + p.rows - 1) / p.rows);
   if (p.kind == kWide) return std::min<int64_t>(s.B * s.N, 32);
-  // per slab: teams of a cluster, or blocks
-  const int64_t team = p.fused ? p.chunks : 1;
-  return std::max<int64_t>(1, std::min(p.fused ? s.B : s.B * p.chunks, resident / (p.slabs * team))) * team;
+  return static_cast<int64_t>(tiles_grid(s, p, kTilesPerSm, num_sms()).y) * p.chunks;
 }
 
 }  // namespace
@@ -400,7 +424,7 @@ size_t backward_workspace(const Shape& s, int size) {
   size_t bytes = 16;
   for (bool aligned : {false, true}) {
     const Plan p = plan_of(s, size, aligned);
-    size_t parts = sizeof(float) * 2 * static_cast<size_t>(s.C) * walkers(s, p);
+    size_t parts = sizeof(float) * 2 * static_cast<size_t>(s.C) * parts_of(s, p);
     parts = (parts + 15) / 16 * 16;
     if (p.kind == kTiles && !p.fused) parts += sizeof(float2) * static_cast<size_t>(s.B) * p.chunks * s.G;
     bytes = std::max(bytes, parts);
@@ -414,13 +438,13 @@ template <typename T, typename U, int ACT, int VEC>
 int run(const U* gy, const T* x, const float* mean, const float* rstd, const float* w, const float* bias, T* dx, bool want_parts,
         const Shape& s, const Plan& p, void* ws, cudaStream_t st) {
   const char* what = "group_norm backward";
-  const int64_t n = walkers(s, p);
+  const int64_t n = parts_of(s, p);
   float* parts = want_parts ? static_cast<float*>(ws) : nullptr;
   if (p.kind == kUnits) {
     const int smem = p.rows * static_cast<int>(s.N) * s.C * static_cast<int>(sizeof(float));
     const void* fn = p.slots == 1 ? reinterpret_cast<const void*>(&units_kernel<T, U, ACT, VEC, 1>)
                                   : reinterpret_cast<const void*>(&units_kernel<T, U, ACT, VEC, 4>);
-    if (smem > 48 * 1024)
+    if (smem > 32 * 1024)          // beside a few KB of static memory
       if (int e = allow_smem(fn, smem)) return e;
     const unsigned grid = static_cast<unsigned>(n);
     if (p.slots == 1) units_kernel<T, U, ACT, VEC, 1><<<grid, p.threads, smem, st>>>(gy, x, mean, rstd, w, bias, dx, parts, s, p);
@@ -431,11 +455,13 @@ int run(const U* gy, const T* x, const float* mean, const float* rstd, const flo
   Shape shape = s;
   Plan plan = p;
   void* args[] = {&gy, &x, &mean, &rstd, &w, &bias, &dx, &parts, &shape, &plan, &between};
-  const unsigned grid = static_cast<unsigned>(n * p.slabs);
-  if (p.fused) return launch(reinterpret_cast<const void*>(&tiles_kernel<T, U, ACT, VEC, kFused>), grid, p.threads, p.chunks, st, args, what);
-  if (int e = launch(reinterpret_cast<const void*>(&tiles_kernel<T, U, ACT, VEC, kSums>), grid, p.threads, 1, st, args, what)) return e;
+  const int smem = std::max(Ahead<T, VEC, kRows>::kBytes + Ahead<U, VEC, kRows>::kBytes, VEC * static_cast<int>(sizeof(float))) * kTileThreads;
+  const dim3 grid = tiles_grid(s, p, kTilesPerSm, num_sms());
+  if (p.fused)
+    return launch(reinterpret_cast<const void*>(&tiles_kernel<T, U, ACT, VEC, kFused>), grid, p.threads, p.chunks, smem, st, args, what);
+  if (int e = launch(reinterpret_cast<const void*>(&tiles_kernel<T, U, ACT, VEC, kSums>), grid, p.threads, 1, smem, st, args, what)) return e;
   if (!dx) return 0;
-  return launch(reinterpret_cast<const void*>(&tiles_kernel<T, U, ACT, VEC, kApply>), grid, p.threads, 1, st, args, what);
+  return launch(reinterpret_cast<const void*>(&tiles_kernel<T, U, ACT, VEC, kApply>), grid, p.threads, 1, smem, st, args, what);
 }
 
 }  // namespace
@@ -477,9 +503,11 @@ extern "C" int bpc_group_norm_bwd(const void* gy, const void* x, const float* me
   if (workspace_bytes < bpc_group_norm_workspace_size(B, N, C, G, x_dtype, 1))
     return fail(BPC_ERR_SPACE, "group_norm backward: workspace too small");
   if (!dx && !dw && !db) return 0;
-  // gy's accesses are as many elements as x's: 8 bytes of 16-bit gradients of fp32 features
-  const bool whole = aligned(x, 16) && aligned(dx, 16) && aligned(gy, 16) && x_sample_stride * size % 16 == 0 &&
-                     x_row_stride * size % 16 == 0 && gy_sample_stride * y_size % 16 == 0 && gy_row_stride * y_size % 16 == 0;
+  auto whole_of = [](const void* q, int64_t sample, int64_t row, int bytes) {
+    return aligned(q, kVec * bytes) && sample % kVec == 0 && row % kVec == 0;
+  };
+  const bool whole = whole_of(x, x_sample_stride, x_row_stride, size) && whole_of(dx, 0, 0, size) &&
+                     whole_of(gy, gy_sample_stride, gy_row_stride, y_size);
   const Plan p = plan_of(s, size, whole);
   const bool want = dw || db;
   const int e = with_types(x_dtype, y_dtype, [&](auto xt, auto yt) {
@@ -497,15 +525,15 @@ extern "C" int bpc_group_norm_bwd(const void* gy, const void* x, const float* me
           if (int e = launched(what)) return e;
         }
         if (!want) return 0;
-        const dim3 grid((C + 255) / 256, static_cast<unsigned>(walkers(s, p)));
+        const dim3 grid((C + 255) / 256, static_cast<unsigned>(parts_of(s, p)));
         wide_channels_kernel<T, U, ACT><<<grid, 256, 0, st>>>(g, from, mean, rstd, weight, bias, static_cast<float*>(workspace), s);
         return launched(what);
       }
       if (p.vec == 1) return run<T, U, ACT, 1>(g, from, mean, rstd, weight, bias, to, want, s, p, workspace, st);
-      return run<T, U, ACT, 16 / sizeof(T)>(g, from, mean, rstd, weight, bias, to, want, s, p, workspace, st);
+      return run<T, U, ACT, kVec>(g, from, mean, rstd, weight, bias, to, want, s, p, workspace, st);
     });
   });
   if (e || !want) return e;
-  join_kernel<<<(2 * C + 31) / 32, 256, 0, st>>>(static_cast<const float*>(workspace), walkers(s, p), C, dw, db);
+  join_kernel<<<(2 * C + 31) / 32, 256, 0, st>>>(static_cast<const float*>(workspace), parts_of(s, p), C, dw, db);
   return launched(what);
 }

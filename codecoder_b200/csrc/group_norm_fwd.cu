@@ -16,11 +16,9 @@ namespace {
 
 namespace cg_ = cooperative_groups;
 
-constexpr int kK = kForwardRows;
-
 // Units: a sample's group per `lanes` lanes, SLOTS vectors each; a thread's slots are the same places of every sample.
 template <typename T, typename U, int ACT, int VEC, int SLOTS>
-__global__ void __launch_bounds__(kMaxThreads) units_kernel(const T* __restrict__ x, U* __restrict__ y, float* mean_out,
+__global__ void __launch_bounds__(kUnitThreads) units_kernel(const T* __restrict__ x, U* __restrict__ y, float* mean_out,
                                                             float* rstd_out, const float* __restrict__ w,
                                                             const float* __restrict__ bias, const Shape s, const Plan p, float eps) {
   constexpr int kAhead = SLOTS == 1 ? 4 : 1;       // samples at a time
@@ -29,171 +27,175 @@ __global__ void __launch_bounds__(kMaxThreads) units_kernel(const T* __restrict_
   const int g = unit % s.G, r = unit / s.G;
   const bool there = r < p.rows;
   const int64_t step = static_cast<int64_t>(gridDim.x) * p.rows;
-  int64_t in[SLOTS];
+  constexpr int kP = Pack<T, VEC>::kPairs;
+  const T* in[SLOTS];
   int out[SLOTS];
   bool has[SLOTS];
-  float wv[SLOTS][VEC], bv[SLOTS][VEC];
+  uint64_t wv[SLOTS][kP], bv[SLOTS][kP];
 #pragma unroll
   for (int k = 0; k < SLOTS; ++k) {
     const int e = k * p.lanes + l, row = e / across, c = g * cg + e % across * VEC;
     has[k] = there && row < s.N;
-    in[k] = row * s.x_row + c;
+    in[k] = x + row * s.x_row + c;
     out[k] = row * s.C + c;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      wv[k][i] = has[k] && w ? w[c + i] : 1.0f;
-      bv[k][i] = has[k] && bias ? bias[c + i] : 0.0f;
-    }
+    channels<VEC>(w, c, has[k], 1.0f, wv[k]);
+    channels<VEC>(bias, c, has[k], 0.0f, bv[k]);
   }
   const float per = 1.0f / static_cast<float>(n);
+  const int64_t y_sample = s.N * s.C;
   for (int64_t b0 = static_cast<int64_t>(blockIdx.x) * p.rows + r; b0 - r < s.B; b0 += kAhead * step) {
     Pack<T, VEC> v[kAhead][SLOTS];
 #pragma unroll
     for (int a = 0; a < kAhead; ++a)
 #pragma unroll
       for (int k = 0; k < SLOTS; ++k)
-        if (has[k] && b0 + a * step < s.B) v[a][k] = *reinterpret_cast<const Pack<T, VEC>*>(x + (b0 + a * step) * s.x_sample + in[k]);
+        if (has[k] && b0 + a * step < s.B) v[a][k] = *reinterpret_cast<const Pack<T, VEC>*>(in[k] + (b0 + a * step) * s.x_sample);
 #pragma unroll
     for (int a = 0; a < kAhead; ++a) {
       const int64_t b = b0 + a * step;
       const bool live = b < s.B;
       float sum = 0.0f;
 #pragma unroll
-      for (int k = 0; k < SLOTS; ++k)
-        if (has[k] && live) {
+      for (int k = 0; k < SLOTS; ++k) {
+        uint64_t t = v[a][k].pair(0);
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) sum += v[a][k].get(i);
-        }
+        for (int i = 1; i < kP; ++i) t = f2_add(t, v[a][k].pair(i));
+        sum += has[k] ? both<VEC>(t) : 0.0f;
+      }
       for (int d = p.lanes >> 1; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-      const float mean = sum * per;
+      const float mean = over(sum, static_cast<float>(n), per);
       float sq = 0.0f;
 #pragma unroll
-      for (int k = 0; k < SLOTS; ++k)
-        if (has[k] && live) {
+      for (int k = 0; k < SLOTS; ++k) {
+        uint64_t t = 0;
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            const float d = v[a][k].get(i) - mean;
-            sq = fmaf(d, d, sq);
-          }
+        for (int i = 0; i < kP; ++i) {
+          const uint64_t d = f2_add(v[a][k].pair(i), f2_of(-mean));
+          t = f2_fma(d, d, t);
         }
+        sq += has[k] ? both<VEC>(t) : 0.0f;
+      }
       for (int d = p.lanes >> 1; d; d >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, d);
-      const float rstd = 1.0f / sqrtf(sq * per + eps);
+      const float rstd = inverse_sqrt(fmaf(sq, per, eps));
       if (l == 0 && there && live && mean_out) {
         mean_out[b * s.G + g] = mean;
         rstd_out[b * s.G + g] = rstd;
       }
 #pragma unroll
-      for (int k = 0; k < SLOTS; ++k)
-        if (has[k] && live) {
-          Pack<U, VEC> o;
+      for (int k = 0; k < SLOTS; ++k) {
+        Pack<U, VEC> o;
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) o.set(i, activate<ACT>(fmaf(wv[k][i], (v[a][k].get(i) - mean) * rstd, bv[k][i])));
-          *reinterpret_cast<Pack<U, VEC>*>(y + b * s.N * s.C + out[k]) = o;
+        for (int i = 0; i < kP; ++i) {
+          const uint64_t scale = f2_mul(wv[k][i], f2_of(rstd));
+          o.set(i, activate<ACT>(f2_fma(f2_add(v[a][k].pair(i), f2_of(-mean)), scale, bv[k][i])));
         }
+        if (has[k] && live) *reinterpret_cast<Pack<U, VEC>*>(y + b * y_sample + out[k]) = o;
+      }
     }
   }
 }
 
 enum Mode { kFused, kStats, kApply };
 
-// Tiles: a block's chunk of a slab in registers.  parts: (B, chunks, G) pairs of mean and summed squared differences
-// between the two kernels of samples that no cluster holds.
+// Tiles: a block's chunk of a slab in registers, the next sample's on its way meanwhile.  parts: (B, chunks, G) pairs of mean
+// and summed squared differences between the two kernels of samples that no cluster holds.
 template <typename T, typename U, int ACT, int VEC, int MODE>
-__global__ void __launch_bounds__(kMaxThreads) tiles_kernel(const T* __restrict__ x, U* __restrict__ y, float* mean_out,
-                                                            float* rstd_out, const float* __restrict__ w,
-                                                            const float* __restrict__ bias, const Shape s, const Plan p, float eps,
-                                                            float2* parts) {
-  __shared__ float part[kMaxThreads];
-  __shared__ float sums[kMaxThreads], squares[kMaxThreads];
-  __shared__ float2 mine[kMaxThreads];             // a group's mean and squares here, and (in place) in the whole sample
+__global__ void __launch_bounds__(kTileThreads, 3) tiles_kernel(const T* __restrict__ x, U* __restrict__ y, float* mean_out,
+                                                               float* rstd_out, const float* __restrict__ w,
+                                                               const float* __restrict__ bias, const Shape s, const Plan p, float eps,
+                                                               float2* parts) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ __align__(16) float part[2][kTileThreads];
+  __shared__ float2 mine[kTileThreads];             // a group's mean and squares here
   const int cg = s.C / s.G, across = cg / VEC, groups = p.slab / cg;
-  const int v = threadIdx.x % p.V, r = threadIdx.x / p.V, lanes = blockDim.x / p.V;
-  const int64_t works = s.B * p.slabs * p.chunks;
-  for (int64_t at = blockIdx.x; at < works; at += gridDim.x) {
-    // what the statistics' kernel read last is read first
-    const int64_t work = MODE == kApply ? works - 1 - at : at;
-    const int chunk = static_cast<int>(work % p.chunks);
-    const int64_t rest = work / p.chunks, b = rest / p.slabs;
-    const int slab = static_cast<int>(rest % p.slabs), c = slab * p.slab + v * VEC, j = v / across;
-    const int row0 = chunk * p.chunk_rows, rows = min(p.chunk_rows, static_cast<int>(s.N) - row0);
-    const bool there = r < lanes && c < s.C;
-    Pack<T, VEC> d[kK];
-    const T* from = x + b * s.x_sample + (row0 + r) * s.x_row + c;
-#pragma unroll
-    for (int k = 0; k < kK; ++k)
-      if (there && r + k * lanes < rows) d[k] = *reinterpret_cast<const Pack<T, VEC>*>(from + k * lanes * s.x_row);
-    float mean, rstd;
+  const int v = threadIdx.x % p.V, r = threadIdx.x / p.V, lanes = blockDim.x / p.V, j = v / across;
+  // what the statistics' kernel read last is read first
+  const int chunk0 = blockIdx.x % p.chunks, slab = blockIdx.x / p.chunks, chunk = MODE == kApply ? p.chunks - 1 - chunk0 : chunk0;
+  const int c = slab * p.slab + v * VEC, g = slab * groups + j;
+  const int row0 = chunk * p.chunk_rows, rows = min(p.chunk_rows, static_cast<int>(s.N) - row0);
+  const bool there = r < lanes && c < s.C, speaks = there && r == 0 && v % across == 0;
+  const int n = there && r < rows ? (rows - r + lanes - 1) / lanes : 0;        // this thread's rows
+  auto sample = [&](int64_t k) { return MODE == kApply ? s.B - 1 - k : k; };
+  const T* from = x + static_cast<int64_t>(row0 + r) * s.x_row + c;
+  U* to = y + static_cast<int64_t>(row0 + r) * s.C + c;
+  const int64_t x_step = lanes * s.x_row, y_step = static_cast<int64_t>(lanes) * s.C;
+  Ahead<T, VEC, kRows> ahead(smem);
+  ahead.fetch(from + sample(blockIdx.y) * s.x_sample, x_step, n);
+  constexpr int kP = Pack<T, VEC>::kPairs;
+  uint64_t wv[kP], bv[kP];
+  channels<VEC>(w, c, there, 1.0f, wv);
+  channels<VEC>(bias, c, there, 0.0f, bv);
+  const float per = 1.0f / (static_cast<float>(s.N) * static_cast<float>(cg));
+  const float here = static_cast<float>(rows) * static_cast<float>(cg), per_here = 1.0f / here;
+  auto rows_of = [&](int q) { return static_cast<float>(min(p.chunk_rows, static_cast<int>(s.N) - q * p.chunk_rows)); };
+  for (int64_t at = blockIdx.y; at < s.B; at += gridDim.y) {
+    const int64_t b = sample(at);
+    Pack<T, VEC> d[kRows];
+    cp_wait_all();
+    ahead.take(d);
+    float mean, rstd, sum[1] = {0.0f}, sq[1] = {0.0f};
     if constexpr (MODE != kApply) {
-      float sum = 0.0f;
+      with_rows(n == kRows, [&](auto all) {
+        uint64_t t = 0;
 #pragma unroll
-      for (int k = 0; k < kK; ++k)
-        if (there && r + k * lanes < rows) {
-          float t = 0.0f;
+        for (int k = 0; k < kRows; ++k)
+          if (decltype(all)::value || k < n) {
+            uint64_t u = d[k].pair(0);
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) t += d[k].get(i);
-          sum += t;
-        }
-      group_sums(sum, p.V, lanes, across, groups, part, sums);
-      const float n = static_cast<float>(rows) * static_cast<float>(cg);
-      mean = j < groups ? sums[j] / n : 0.0f;
-      float sq = 0.0f;
-#pragma unroll
-      for (int k = 0; k < kK; ++k)
-        if (there && r + k * lanes < rows) {
-          float t = 0.0f;
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            const float e = d[k].get(i) - mean;
-            t = fmaf(e, e, t);
+            for (int i = 1; i < kP; ++i) u = f2_add(u, d[k].pair(i));
+            t = f2_add(t, u);
           }
-          sq += t;
-        }
-      group_sums(sq, p.V, lanes, across, groups, part, squares);
-      if (MODE == kFused && p.chunks == 1) {
-        rstd = j < groups ? 1.0f / sqrtf(squares[j] / n + eps) : 0.0f;
-        if (there && r == 0 && v % across == 0 && mean_out) {
-          mean_out[b * s.G + slab * groups + j] = mean;
-          rstd_out[b * s.G + slab * groups + j] = rstd;
-        }
-      } else if (MODE == kStats) {
-        if (there && r == 0 && v % across == 0) parts[(b * p.chunks + chunk) * s.G + slab * groups + j] = make_float2(mean, squares[j]);
-        __syncthreads();
+        sum[0] = both<VEC>(t);
+      });
+    }
+    if (at + gridDim.y < s.B) ahead.fetch(from + sample(at + gridDim.y) * s.x_sample, x_step, n);
+    if constexpr (MODE != kApply) {
+      group_sums(sum, p.V, lanes, across, v, part[0]);
+      mean = over(sum[0], here, per_here);
+      with_rows(n == kRows, [&](auto all) {
+        uint64_t t = 0;
+#pragma unroll
+        for (int k = 0; k < kRows; ++k)
+          if (decltype(all)::value || k < n) {
+            uint64_t u = 0;
+#pragma unroll
+            for (int i = 0; i < kP; ++i) {
+              const uint64_t e = f2_add(d[k].pair(i), f2_of(-mean));
+              u = f2_fma(e, e, u);
+            }
+            t = f2_add(t, u);
+          }
+        sq[0] = both<VEC>(t);
+      });
+      group_sums(sq, p.V, lanes, across, v, part[1]);
+      if (MODE == kStats) {
+        if (speaks) parts[(b * p.chunks + chunk) * s.G + g] = make_float2(mean, sq[0]);
         continue;
-      } else {
-        for (int k = threadIdx.x; k < groups; k += blockDim.x) mine[k] = make_float2(sums[k] / n, squares[k]);
+      }
+      if (p.chunks > 1) {
+        // the cluster's blocks have the other chunks
+        if (speaks) mine[j] = make_float2(mean, sq[0]);
         cg_::cluster_group cluster = cg_::this_cluster();
         cluster.sync();
-        for (int k = threadIdx.x; k < groups; k += blockDim.x) {
-          float2 theirs[kCluster];
-          float total = 0.0f;
-          for (int q = 0; q < p.chunks; ++q) {
-            theirs[q] = cluster.map_shared_rank(mine, q)[k];
-            total = fmaf(theirs[q].x, static_cast<float>(min(p.chunk_rows, static_cast<int>(s.N) - q * p.chunk_rows)), total);
-          }
-          const float m = total / static_cast<float>(s.N);
-          float all = 0.0f;
-          for (int q = 0; q < p.chunks; ++q) {
-            const float e = theirs[q].x - m, rows_q = static_cast<float>(min(p.chunk_rows, static_cast<int>(s.N) - q * p.chunk_rows));
-            all += fmaf(e * e, rows_q * static_cast<float>(cg), theirs[q].y);
-          }
-          sums[k] = m;
-          squares[k] = 1.0f / sqrtf(all / (static_cast<float>(s.N) * static_cast<float>(cg)) + eps);
-          if (chunk == 0 && mean_out && slab * groups + k < s.G) {
-            mean_out[b * s.G + slab * groups + k] = m;
-            rstd_out[b * s.G + slab * groups + k] = squares[k];
-          }
+        float total = 0.0f;
+        for (int q = 0; q < p.chunks; ++q) total = fmaf(cluster.map_shared_rank(mine, q)[j].x, rows_of(q), total);
+        mean = total / static_cast<float>(s.N);
+        sq[0] = 0.0f;
+        for (int q = 0; q < p.chunks; ++q) {
+          const float2 theirs = cluster.map_shared_rank(mine, q)[j];
+          const float e = theirs.x - mean;
+          sq[0] += fmaf(e * e, rows_of(q) * static_cast<float>(cg), theirs.y);
         }
         cluster.sync();                            // every block has read the others' parts
-        mean = j < groups ? sums[j] : 0.0f;
-        rstd = j < groups ? squares[j] : 0.0f;
       }
     } else {
+      // the chunks' parts, the group's threads in a row taking them in turn: 32 lanes of warp k for group k
       const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+      __syncthreads();
       for (int k = warp; k < groups && slab * groups + k < s.G; k += warps) {
         const float2* f = parts + b * p.chunks * s.G + slab * groups + k;
         float total = 0.0f;
-        for (int q = lane; q < p.chunks; q += 32)
-          total = fmaf(f[static_cast<int64_t>(q) * s.G].x, static_cast<float>(min(p.chunk_rows, static_cast<int>(s.N) - q * p.chunk_rows)), total);
+        for (int q = lane; q < p.chunks; q += 32) total = fmaf(f[static_cast<int64_t>(q) * s.G].x, rows_of(q), total);
 #pragma unroll
         for (int m = 16; m; m >>= 1) total += __shfl_xor_sync(0xffffffffu, total, m);
         const float m = total / static_cast<float>(s.N);
@@ -201,40 +203,37 @@ __global__ void __launch_bounds__(kMaxThreads) tiles_kernel(const T* __restrict_
         for (int q = lane; q < p.chunks; q += 32) {
           const float2 t = f[static_cast<int64_t>(q) * s.G];
           const float e = t.x - m;
-          all += fmaf(e * e, static_cast<float>(min(p.chunk_rows, static_cast<int>(s.N) - q * p.chunk_rows)) * static_cast<float>(cg), t.y);
+          all += fmaf(e * e, rows_of(q) * static_cast<float>(cg), t.y);
         }
 #pragma unroll
         for (int q = 16; q; q >>= 1) all += __shfl_xor_sync(0xffffffffu, all, q);
-        if (lane == 0) {
-          sums[k] = m;
-          squares[k] = 1.0f / sqrtf(all / (static_cast<float>(s.N) * static_cast<float>(cg)) + eps);
-          if (chunk == 0 && mean_out) {
-            mean_out[b * s.G + slab * groups + k] = m;
-            rstd_out[b * s.G + slab * groups + k] = squares[k];
-          }
-        }
+        if (lane == 0) mine[k] = make_float2(m, all);
       }
       __syncthreads();
-      mean = j < groups ? sums[j] : 0.0f;
-      rstd = j < groups ? squares[j] : 0.0f;
+      mean = mine[j].x, sq[0] = mine[j].y;
     }
     if constexpr (MODE != kStats) {
-      float wv[VEC], bv[VEC];
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        wv[i] = there && w ? __ldg(w + c + i) : 1.0f;
-        bv[i] = there && bias ? __ldg(bias + c + i) : 0.0f;
+      rstd = inverse_sqrt(fmaf(sq[0], per, eps));
+      if (speaks && chunk == 0 && mean_out) {
+        mean_out[b * s.G + g] = mean;
+        rstd_out[b * s.G + g] = rstd;
       }
-      U* to = y + (b * s.N + row0 + r) * s.C + c;
+      U* out = to + b * s.N * s.C;
+      uint64_t scale[kP];
 #pragma unroll
-      for (int k = 0; k < kK; ++k)
-        if (there && r + k * lanes < rows) {
-          Pack<U, VEC> o;
+      for (int i = 0; i < kP; ++i) scale[i] = f2_mul(wv[i], f2_of(rstd));
+      with_rows(n == kRows, [&](auto all) {
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) o.set(i, activate<ACT>(fmaf(wv[i], (d[k].get(i) - mean) * rstd, bv[i])));
-          *reinterpret_cast<Pack<U, VEC>*>(to + static_cast<int64_t>(k) * lanes * s.C) = o;
+        for (int k = 0; k < kRows; ++k) {
+          if (decltype(all)::value || k < n) {
+            Pack<U, VEC> o;
+#pragma unroll
+            for (int i = 0; i < kP; ++i) o.set(i, activate<ACT>(f2_fma(f2_add(d[k].pair(i), f2_of(-mean)), scale[i], bv[i])));
+            *reinterpret_cast<Pack<U, VEC>*>(out) = o;
+          }
+          out += y_step;
         }
-      __syncthreads();                             // sums and squares are this work's until here
+      });
     }
   }
 }
@@ -278,12 +277,12 @@ __global__ void __launch_bounds__(256) wide_kernel(const T* __restrict__ x, U* _
       const int c = c0 + static_cast<int>(i % cg);
       const int64_t r = i / cg;
       const float xh = (load_f32(x + b * s.x_sample + r * s.x_row + c) - mean) * rstd;
-      store_f32(y + (b * s.N + r) * s.C + c, activate<ACT>(fmaf(w ? w[c] : 1.0f, xh, bias ? bias[c] : 0.0f)));
+      store_f32(y + (b * s.N + r) * s.C + c, activate1<ACT>(fmaf(w ? w[c] : 1.0f, xh, bias ? bias[c] : 0.0f)));
     }
   }
 }
 
-Plan plan_of(const Shape& s, int size, bool aligned) { return make_plan(s, size, kK, num_sms(), aligned); }
+Plan plan_of(const Shape& s, int size, bool aligned) { return make_plan(s, size, 16 / size, num_sms(), aligned); }
 
 }  // namespace
 
@@ -299,26 +298,31 @@ size_t forward_workspace(const Shape& s, int size) {
 namespace {
 
 template <typename T, typename U, int ACT, int VEC>
-int run(const T* x, U* y, float* mean, float* rstd, const float* w, const float* bias, const Shape& s, const Plan& p, float eps,
-        void* ws, cudaStream_t st) {
+int run_units(const T* x, U* y, float* mean, float* rstd, const float* w, const float* bias, const Shape& s, const Plan& p, float eps,
+              cudaStream_t st) {
+  const int ahead = p.slots == 1 ? 4 : 1;
+  const int64_t blocks = (s.B + static_cast<int64_t>(p.rows) * ahead - 1) / (static_cast<int64_t>(p.rows) * ahead);
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(blocks, num_sms() * (2048 / p.threads)));
+  if (p.slots == 1) units_kernel<T, U, ACT, VEC, 1><<<grid, p.threads, 0, st>>>(x, y, mean, rstd, w, bias, s, p, eps);
+  else units_kernel<T, U, ACT, VEC, 4><<<grid, p.threads, 0, st>>>(x, y, mean, rstd, w, bias, s, p, eps);
+  return launched("group_norm");
+}
+
+template <typename T, typename U, int ACT, int VEC>
+int run_tiles(const T* x, U* y, float* mean, float* rstd, const float* w, const float* bias, const Shape& s, const Plan& p, float eps,
+              void* ws, cudaStream_t st) {
   const char* what = "group_norm";
-  if (p.kind == kUnits) {
-    const int ahead = p.slots == 1 ? 4 : 1;
-    const int64_t blocks = (s.B + static_cast<int64_t>(p.rows) * ahead - 1) / (static_cast<int64_t>(p.rows) * ahead);
-    const unsigned grid = static_cast<unsigned>(std::min<int64_t>(blocks, num_sms() * (2048 / p.threads)));
-    if (p.slots == 1) units_kernel<T, U, ACT, VEC, 1><<<grid, p.threads, 0, st>>>(x, y, mean, rstd, w, bias, s, p, eps);
-    else units_kernel<T, U, ACT, VEC, 4><<<grid, p.threads, 0, st>>>(x, y, mean, rstd, w, bias, s, p, eps);
-    return launched(what);
-  }
-  const int64_t works = s.B * p.slabs * p.chunks, most = static_cast<int64_t>(1) << 30;
-  unsigned grid = static_cast<unsigned>(std::min(works, most / p.chunks * p.chunks));
   float2* parts = static_cast<float2*>(ws);
   Shape shape = s;
   Plan plan = p;
   void* args[] = {&x, &y, &mean, &rstd, &w, &bias, &shape, &plan, &eps, &parts};
-  if (p.fused) return launch(reinterpret_cast<const void*>(&tiles_kernel<T, U, ACT, VEC, kFused>), grid, p.threads, p.chunks, st, args, what);
-  if (int e = launch(reinterpret_cast<const void*>(&tiles_kernel<T, U, BPC_ACT_NONE, VEC, kStats>), grid, p.threads, 1, st, args, what)) return e;
-  return launch(reinterpret_cast<const void*>(&tiles_kernel<T, U, ACT, VEC, kApply>), grid, p.threads, 1, st, args, what);
+  const dim3 grid = tiles_grid(s, p, 3, num_sms());
+  const int smem = Ahead<T, VEC, kRows>::kBytes * kTileThreads;
+  if (p.fused)
+    return launch(reinterpret_cast<const void*>(&tiles_kernel<T, U, ACT, VEC, kFused>), grid, p.threads, p.chunks, smem, st, args, what);
+  if (int e = launch(reinterpret_cast<const void*>(&tiles_kernel<T, U, BPC_ACT_NONE, VEC, kStats>), grid, p.threads, 1, smem, st, args, what))
+    return e;
+  return launch(reinterpret_cast<const void*>(&tiles_kernel<T, U, ACT, VEC, kApply>), grid, p.threads, 1, smem, st, args, what);
 }
 
 }  // namespace
@@ -359,8 +363,12 @@ extern "C" int bpc_group_norm_fwd(const void* x, void* y, float* mean, float* rs
         wide_kernel<T, U, ACT><<<grid, 256, 0, st>>>(from, to, mean, rstd, weight, bias, s, eps);
         return launched(what);
       }
-      if (p.vec == 1) return run<T, U, ACT, 1>(from, to, mean, rstd, weight, bias, s, p, eps, workspace, st);
-      return run<T, U, ACT, 16 / sizeof(T)>(from, to, mean, rstd, weight, bias, s, p, eps, workspace, st);
+      if (p.kind == kUnits) {
+        if (p.vec == 1) return run_units<T, U, ACT, 1>(from, to, mean, rstd, weight, bias, s, p, eps, st);
+        return run_units<T, U, ACT, 16 / sizeof(T)>(from, to, mean, rstd, weight, bias, s, p, eps, st);
+      }
+      if (p.vec == 1) return run_tiles<T, U, ACT, 1>(from, to, mean, rstd, weight, bias, s, p, eps, workspace, st);
+      return run_tiles<T, U, ACT, kTileVec>(from, to, mean, rstd, weight, bias, s, p, eps, workspace, st);
     });
   });
 }
