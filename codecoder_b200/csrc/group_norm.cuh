@@ -158,9 +158,10 @@ inline Plan make_plan(const Shape& s, int size, int full, int sms, bool aligned)
   // small samples, of which a block per sample and slab would have little: 32-byte pieces of rows at least, or whole rows
   const int64_t vectors = s.N * across;
   if (vectors <= 128 && (s.N == 1 || cg * size >= 32)) {
+    // two vectors a lane where there are two: the sums' joins and the addresses are half of the rest
+    p.slots = vectors == 1 ? 1 : vectors <= 64 ? 2 : 4;
     p.lanes = 1;
-    while (p.lanes < 32 && p.lanes < vectors) p.lanes *= 2;
-    p.slots = vectors <= p.lanes ? 1 : 4;
+    while (p.lanes * p.slots < vectors) p.lanes *= 2;
     if (static_cast<int64_t>(p.lanes) * s.G <= kUnitThreads) {
       p.kind = kUnits;
       p.rows = std::max(1, 256 / (p.lanes * s.G));

@@ -44,95 +44,97 @@ __device__ __forceinline__ void channel_sums(const uint64_t (&a)[(VEC + 1) / 2],
   }
 }
 
-// Units: a sample's group per `lanes` lanes, SLOTS vectors each; a thread's slots are the same places of every sample.
+// Units: a sample's group per `lanes` lanes, SLOTS vectors each; a thread's slots are the same places of every sample, and
+// the next sample's are on their way while one is worked on.
 template <typename T, typename U, int ACT, int VEC, int SLOTS>
 __global__ void __launch_bounds__(kUnitThreads) units_kernel(const U* __restrict__ gy, const T* __restrict__ x,
-                                                            const float* __restrict__ mean_in,
-                                                            const float* __restrict__ rstd_in, const float* __restrict__ w,
-                                                            const float* __restrict__ bias, T* __restrict__ dx, float* parts,
-                                                            const Shape s, const Plan p) {
-  constexpr int kAhead = SLOTS == 1 ? 2 : 1;       // samples at a time
+                                                             const float* __restrict__ mean_in,
+                                                             const float* __restrict__ rstd_in, const float* __restrict__ w,
+                                                             const float* __restrict__ bias, T* __restrict__ dx, float* parts,
+                                                             const Shape s, const Plan p) {
+  constexpr int kP = Pack<T, VEC>::kPairs;
   extern __shared__ float buffer[];
-  const int cg = s.C / s.G, across = cg / VEC, n = static_cast<int>(s.N) * cg;
+  const int cg = s.C / s.G, across = cg / VEC;
   const int unit = threadIdx.x / p.lanes, l = threadIdx.x % p.lanes;
   const int g = unit % s.G, r = unit / s.G;
   const bool there = r < p.rows;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * p.rows;
-  constexpr int kP = Pack<T, VEC>::kPairs;
-  const T* in_x[SLOTS];
-  const U* in_g[SLOTS];
-  int out[SLOTS];
+  const int64_t step = static_cast<int64_t>(gridDim.x) * p.rows, b0 = static_cast<int64_t>(blockIdx.x) * p.rows;
+  const int rounds = static_cast<int>((s.B - b0 + step - 1) / step);                          // of the block
+  const int mine = there && b0 + r < s.B ? static_cast<int>((s.B - b0 - r + step - 1) / step) : 0;
+  const T* from[SLOTS];
+  const U* from_g[SLOTS];
+  T* to[SLOTS];
   bool has[SLOTS];
   uint64_t wv[SLOTS][kP], bv[SLOTS][kP], acc_a[SLOTS][kP], acc_b[SLOTS][kP];
+  Pack<T, VEC> next[SLOTS];
+  Pack<U, VEC> next_g[SLOTS];
+  float mean_next = 0.0f, rstd_next = 0.0f;
+  int64_t stat = (b0 + r) * s.G + g;
 #pragma unroll
   for (int k = 0; k < SLOTS; ++k) {
     const int e = k * p.lanes + l, row = e / across, c = g * cg + e % across * VEC;
     has[k] = there && row < s.N;
-    in_x[k] = x + row * s.x_row + c;
-    in_g[k] = gy + row * s.g_row + c;
-    out[k] = row * s.C + c;
+    from[k] = x + (b0 + r) * s.x_sample + row * s.x_row + c;
+    from_g[k] = gy + (b0 + r) * s.g_sample + row * s.g_row + c;
+    to[k] = dx + ((b0 + r) * s.N + row) * s.C + c;
     channels<VEC>(w, c, has[k], 1.0f, wv[k]);
     channels<VEC>(bias, c, has[k], 0.0f, bv[k]);
 #pragma unroll
     for (int i = 0; i < kP; ++i) acc_a[k][i] = acc_b[k][i] = 0;
   }
-  const float per = 1.0f / static_cast<float>(n);
-  const int64_t o_sample = s.N * s.C;
-  for (int64_t b0 = static_cast<int64_t>(blockIdx.x) * p.rows + r; b0 - r < s.B; b0 += kAhead * step) {
-    Pack<T, VEC> vx[kAhead][SLOTS];
-    Pack<U, VEC> vg[kAhead][SLOTS];
-    float mean[kAhead], rstd[kAhead];
+  auto load = [&](bool live) {
+    if (live) mean_next = mean_in[stat], rstd_next = rstd_in[stat];
 #pragma unroll
-    for (int a = 0; a < kAhead; ++a) {
-      const int64_t b = b0 + a * step;
-      const bool live = there && b < s.B;
-      mean[a] = live ? mean_in[b * s.G + g] : 0.0f;
-      rstd[a] = live ? rstd_in[b * s.G + g] : 0.0f;
-#pragma unroll
-      for (int k = 0; k < SLOTS; ++k) {
-        if (has[k] && live) {
-          vx[a][k] = *reinterpret_cast<const Pack<T, VEC>*>(in_x[k] + b * s.x_sample);
-          vg[a][k] = *reinterpret_cast<const Pack<U, VEC>*>(in_g[k] + b * s.g_sample);
-        } else {
-          vx[a][k] = Pack<T, VEC>(), vg[a][k] = Pack<U, VEC>();      // zeros: nothing to any sum
-        }
+    for (int k = 0; k < SLOTS; ++k) {
+      next[k] = Pack<T, VEC>(), next_g[k] = Pack<U, VEC>();        // zeros: nothing to any sum
+      if (has[k] && live) {
+        next[k] = *reinterpret_cast<const Pack<T, VEC>*>(from[k]);
+        next_g[k] = *reinterpret_cast<const Pack<U, VEC>*>(from_g[k]);
       }
     }
+  };
+  load(mine > 0);
+  const float per = 1.0f / (static_cast<float>(s.N) * static_cast<float>(cg));
+  const int64_t x_step = step * s.x_sample, g_step = step * s.g_sample, o_step = step * s.N * s.C;
+  for (int round = 0; round < rounds; ++round) {
+    const uint64_t scale = f2_of(rstd_next), minus = f2_of(-mean_next);
+    uint64_t xh[SLOTS][kP], gz[SLOTS][kP], s1 = 0, s2 = 0;
 #pragma unroll
-    for (int a = 0; a < kAhead; ++a) {
-      const int64_t b = b0 + a * step;
-      const bool live = b < s.B;
-      const uint64_t scale = f2_of(rstd[a]), minus = f2_of(-mean[a]);
-      uint64_t gz[SLOTS][kP], s1 = 0, s2 = 0;
+    for (int k = 0; k < SLOTS; ++k) {
 #pragma unroll
-      for (int k = 0; k < SLOTS; ++k)
-#pragma unroll
-        for (int i = 0; i < kP; ++i) {
-          const uint64_t xh = f2_mul(f2_add(vx[a][k].pair(i), minus), scale);
-          gz[k][i] = f2_mul(vg[a][k].pair(i), slope<ACT>(f2_fma(wv[k][i], xh, bv[k][i])));
-          acc_a[k][i] = f2_add(acc_a[k][i], gz[k][i]);
-          acc_b[k][i] = f2_fma(gz[k][i], xh, acc_b[k][i]);
-          const uint64_t t = f2_mul(gz[k][i], wv[k][i]);
-          s1 = f2_add(s1, t);
-          s2 = f2_fma(t, xh, s2);
-        }
-      float m1 = both<VEC>(s1), m2 = both<VEC>(s2);
-      for (int d = p.lanes >> 1; d; d >>= 1) {
-        m1 += __shfl_xor_sync(0xffffffffu, m1, d);
-        m2 += __shfl_xor_sync(0xffffffffu, m2, d);
+      for (int i = 0; i < kP; ++i) {
+        xh[k][i] = f2_mul(f2_add(next[k].pair(i), minus), scale);
+        gz[k][i] = next_g[k].pair(i);
       }
-      if (dx) {
-        const uint64_t u1 = f2_of(-m1 * per), u2 = f2_of(-m2 * per);
+      from[k] += x_step, from_g[k] += g_step;
+    }
+    stat += step * s.G;
+    load(round + 1 < mine);
 #pragma unroll
-        for (int k = 0; k < SLOTS; ++k) {
-          Pack<T, VEC> o;
+    for (int k = 0; k < SLOTS; ++k)
 #pragma unroll
-          for (int i = 0; i < kP; ++i) {
-            const uint64_t xh = f2_mul(f2_add(vx[a][k].pair(i), minus), scale);
-            o.set(i, f2_mul(scale, f2_fma(gz[k][i], wv[k][i], f2_fma(xh, u2, u1))));
-          }
-          if (has[k] && live) *reinterpret_cast<Pack<T, VEC>*>(dx + b * o_sample + out[k]) = o;
-        }
+      for (int i = 0; i < kP; ++i) {
+        gz[k][i] = f2_mul(gz[k][i], slope<ACT>(f2_fma(wv[k][i], xh[k][i], bv[k][i])));
+        acc_a[k][i] = f2_add(acc_a[k][i], gz[k][i]);
+        acc_b[k][i] = f2_fma(gz[k][i], xh[k][i], acc_b[k][i]);
+        gz[k][i] = f2_mul(gz[k][i], wv[k][i]);
+        s1 = f2_add(s1, gz[k][i]);
+        s2 = f2_fma(gz[k][i], xh[k][i], s2);
+      }
+    float m1 = both<VEC>(s1), m2 = both<VEC>(s2);
+    for (int m = p.lanes >> 1; m; m >>= 1) {
+      m1 += __shfl_xor_sync(0xffffffffu, m1, m);
+      m2 += __shfl_xor_sync(0xffffffffu, m2, m);
+    }
+    if (dx) {
+      const uint64_t u1 = f2_of(-m1 * per), u2 = f2_of(-m2 * per);
+#pragma unroll
+      for (int k = 0; k < SLOTS; ++k) {
+        Pack<T, VEC> o;
+#pragma unroll
+        for (int i = 0; i < kP; ++i) o.set(i, f2_mul(scale, f2_add(gz[k][i], f2_fma(xh[k][i], u2, u1))));
+        if (has[k] && round < mine) *reinterpret_cast<Pack<T, VEC>*>(to[k]) = o;
+        to[k] += o_step;
       }
     }
   }
@@ -413,7 +415,11 @@ constexpr int kTilesPerSm = 2;
 
 // Parts of dw and db: one per block that walks the samples, per slab
 int64_t parts_of(const Shape& s, const Plan& p) {
-  if (p.kind == kUnits) return std::min<int64_t>(static_cast<int64_t>(num_sms()) * std::max(1, 1024 / p.threads), (s.B + p.rows - 1) / p.rows);
+  if (p.kind == kUnits) {
+    // rounds are counted in 32 bits
+    const int64_t blocks = (s.B + p.rows - 1) / p.rows;
+    return std::min(blocks, std::max(static_cast<int64_t>(num_sms()) * std::max(1, 1024 / p.threads), blocks >> 30));
+  }
   if (p.kind == kWide) return std::min<int64_t>(s.B * s.N, 32);
   return static_cast<int64_t>(tiles_grid(s, p, kTilesPerSm, num_sms()).y) * p.chunks;
 }
@@ -442,14 +448,13 @@ int run(const U* gy, const T* x, const float* mean, const float* rstd, const flo
   float* parts = want_parts ? static_cast<float*>(ws) : nullptr;
   if (p.kind == kUnits) {
     const int smem = p.rows * static_cast<int>(s.N) * s.C * static_cast<int>(sizeof(float));
-    const void* fn = p.slots == 1 ? reinterpret_cast<const void*>(&units_kernel<T, U, ACT, VEC, 1>)
-                                  : reinterpret_cast<const void*>(&units_kernel<T, U, ACT, VEC, 4>);
-    if (smem > 32 * 1024)          // beside a few KB of static memory
-      if (int e = allow_smem(fn, smem)) return e;
-    const unsigned grid = static_cast<unsigned>(n);
-    if (p.slots == 1) units_kernel<T, U, ACT, VEC, 1><<<grid, p.threads, smem, st>>>(gy, x, mean, rstd, w, bias, dx, parts, s, p);
-    else units_kernel<T, U, ACT, VEC, 4><<<grid, p.threads, smem, st>>>(gy, x, mean, rstd, w, bias, dx, parts, s, p);
-    return launched(what);
+    const void* fn = p.slots == 1   ? reinterpret_cast<const void*>(&units_kernel<T, U, ACT, VEC, 1>)
+                     : p.slots == 2 ? reinterpret_cast<const void*>(&units_kernel<T, U, ACT, VEC, 2>)
+                                    : reinterpret_cast<const void*>(&units_kernel<T, U, ACT, VEC, 4>);
+    Shape shape = s;
+    Plan plan = p;
+    void* args[] = {&gy, &x, &mean, &rstd, &w, &bias, &dx, &parts, &shape, &plan};
+    return launch(fn, dim3(static_cast<unsigned>(n)), p.threads, 1, smem, st, args, what);
   }
   float2* between = reinterpret_cast<float2*>(static_cast<char*>(ws) + (sizeof(float) * 2 * s.C * n + 15) / 16 * 16);
   Shape shape = s;

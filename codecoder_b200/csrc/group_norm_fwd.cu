@@ -16,81 +16,78 @@ namespace {
 
 namespace cg_ = cooperative_groups;
 
-// Units: a sample's group per `lanes` lanes, SLOTS vectors each; a thread's slots are the same places of every sample.
+// Units: a sample's group per `lanes` lanes, SLOTS vectors each; a thread's slots are the same places of every sample, and
+// the next sample's are on their way while one is worked on.
 template <typename T, typename U, int ACT, int VEC, int SLOTS>
 __global__ void __launch_bounds__(kUnitThreads) units_kernel(const T* __restrict__ x, U* __restrict__ y, float* mean_out,
-                                                            float* rstd_out, const float* __restrict__ w,
-                                                            const float* __restrict__ bias, const Shape s, const Plan p, float eps) {
-  constexpr int kAhead = SLOTS == 1 ? 4 : 1;       // samples at a time
-  const int cg = s.C / s.G, across = cg / VEC, n = static_cast<int>(s.N) * cg;
+                                                             float* rstd_out, const float* __restrict__ w,
+                                                             const float* __restrict__ bias, const Shape s, const Plan p, float eps) {
+  constexpr int kP = Pack<T, VEC>::kPairs;
+  const int cg = s.C / s.G, across = cg / VEC;
   const int unit = threadIdx.x / p.lanes, l = threadIdx.x % p.lanes;
   const int g = unit % s.G, r = unit / s.G;
   const bool there = r < p.rows;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * p.rows;
-  constexpr int kP = Pack<T, VEC>::kPairs;
-  const T* in[SLOTS];
-  int out[SLOTS];
+  const int64_t step = static_cast<int64_t>(gridDim.x) * p.rows, b0 = static_cast<int64_t>(blockIdx.x) * p.rows;
+  const int rounds = static_cast<int>((s.B - b0 + step - 1) / step);                          // of the block
+  const int mine = there && b0 + r < s.B ? static_cast<int>((s.B - b0 - r + step - 1) / step) : 0;
+  const T* from[SLOTS];
+  U* to[SLOTS];
   bool has[SLOTS];
   uint64_t wv[SLOTS][kP], bv[SLOTS][kP];
+  Pack<T, VEC> next[SLOTS];
 #pragma unroll
   for (int k = 0; k < SLOTS; ++k) {
     const int e = k * p.lanes + l, row = e / across, c = g * cg + e % across * VEC;
     has[k] = there && row < s.N;
-    in[k] = x + row * s.x_row + c;
-    out[k] = row * s.C + c;
+    from[k] = x + (b0 + r) * s.x_sample + row * s.x_row + c;
+    to[k] = y + ((b0 + r) * s.N + row) * s.C + c;
     channels<VEC>(w, c, has[k], 1.0f, wv[k]);
     channels<VEC>(bias, c, has[k], 0.0f, bv[k]);
+    next[k] = Pack<T, VEC>();
+    if (has[k] && mine > 0) next[k] = *reinterpret_cast<const Pack<T, VEC>*>(from[k]);
   }
-  const float per = 1.0f / static_cast<float>(n);
-  const int64_t y_sample = s.N * s.C;
-  for (int64_t b0 = static_cast<int64_t>(blockIdx.x) * p.rows + r; b0 - r < s.B; b0 += kAhead * step) {
-    Pack<T, VEC> v[kAhead][SLOTS];
+  const float n = static_cast<float>(s.N) * static_cast<float>(cg), per = 1.0f / n;
+  const int64_t x_step = step * s.x_sample, y_step = step * s.N * s.C;
+  int64_t stat = (b0 + r) * s.G + g;
+  for (int round = 0; round < rounds; ++round) {
+    uint64_t d[SLOTS][kP], t = 0;
 #pragma unroll
-    for (int a = 0; a < kAhead; ++a)
+    for (int k = 0; k < SLOTS; ++k) {
 #pragma unroll
-      for (int k = 0; k < SLOTS; ++k)
-        if (has[k] && b0 + a * step < s.B) v[a][k] = *reinterpret_cast<const Pack<T, VEC>*>(in[k] + (b0 + a * step) * s.x_sample);
+      for (int i = 0; i < kP; ++i) d[k][i] = next[k].pair(i);
 #pragma unroll
-    for (int a = 0; a < kAhead; ++a) {
-      const int64_t b = b0 + a * step;
-      const bool live = b < s.B;
-      float sum = 0.0f;
+      for (int i = 0; i < kP; ++i) t = f2_add(t, d[k][i]);
+      from[k] += x_step;
+      if (has[k] && round + 1 < mine) next[k] = *reinterpret_cast<const Pack<T, VEC>*>(from[k]);
+    }
+    float sum = both<VEC>(t);
+    for (int m = p.lanes >> 1; m; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+    const float mean = over(sum, n, per);
+    const uint64_t minus = f2_of(-mean);
+    t = 0;
 #pragma unroll
-      for (int k = 0; k < SLOTS; ++k) {
-        uint64_t t = v[a][k].pair(0);
+    for (int k = 0; k < SLOTS; ++k) {
+      uint64_t u = 0;
 #pragma unroll
-        for (int i = 1; i < kP; ++i) t = f2_add(t, v[a][k].pair(i));
-        sum += has[k] ? both<VEC>(t) : 0.0f;
+      for (int i = 0; i < kP; ++i) {
+        d[k][i] = f2_add(d[k][i], minus);
+        u = f2_fma(d[k][i], d[k][i], u);
       }
-      for (int d = p.lanes >> 1; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-      const float mean = over(sum, static_cast<float>(n), per);
-      float sq = 0.0f;
+      if (has[k]) t = f2_add(t, u);
+    }
+    float sq = both<VEC>(t);
+    for (int m = p.lanes >> 1; m; m >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, m);
+    const float rstd = inverse_sqrt(fmaf(sq, per, eps));
+    if (mean_out && l == 0 && round < mine) mean_out[stat] = mean, rstd_out[stat] = rstd;
+    stat += step * s.G;
+    const uint64_t scale = f2_of(rstd);
 #pragma unroll
-      for (int k = 0; k < SLOTS; ++k) {
-        uint64_t t = 0;
+    for (int k = 0; k < SLOTS; ++k) {
+      Pack<U, VEC> o;
 #pragma unroll
-        for (int i = 0; i < kP; ++i) {
-          const uint64_t d = f2_add(v[a][k].pair(i), f2_of(-mean));
-          t = f2_fma(d, d, t);
-        }
-        sq += has[k] ? both<VEC>(t) : 0.0f;
-      }
-      for (int d = p.lanes >> 1; d; d >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, d);
-      const float rstd = inverse_sqrt(fmaf(sq, per, eps));
-      if (l == 0 && there && live && mean_out) {
-        mean_out[b * s.G + g] = mean;
-        rstd_out[b * s.G + g] = rstd;
-      }
-#pragma unroll
-      for (int k = 0; k < SLOTS; ++k) {
-        Pack<U, VEC> o;
-#pragma unroll
-        for (int i = 0; i < kP; ++i) {
-          const uint64_t scale = f2_mul(wv[k][i], f2_of(rstd));
-          o.set(i, activate<ACT>(f2_fma(f2_add(v[a][k].pair(i), f2_of(-mean)), scale, bv[k][i])));
-        }
-        if (has[k] && live) *reinterpret_cast<Pack<U, VEC>*>(y + b * y_sample + out[k]) = o;
-      }
+      for (int i = 0; i < kP; ++i) o.set(i, activate<ACT>(f2_fma(f2_mul(d[k][i], scale), wv[k][i], bv[k][i])));
+      if (has[k] && round < mine) *reinterpret_cast<Pack<U, VEC>*>(to[k]) = o;
+      to[k] += y_step;
     }
   }
 }
@@ -300,10 +297,11 @@ namespace {
 template <typename T, typename U, int ACT, int VEC>
 int run_units(const T* x, U* y, float* mean, float* rstd, const float* w, const float* bias, const Shape& s, const Plan& p, float eps,
               cudaStream_t st) {
-  const int ahead = p.slots == 1 ? 4 : 1;
-  const int64_t blocks = (s.B + static_cast<int64_t>(p.rows) * ahead - 1) / (static_cast<int64_t>(p.rows) * ahead);
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(blocks, num_sms() * (2048 / p.threads)));
+  // rounds are counted in 32 bits: more blocks for more than 2^31 of them (of which the first ones' memory would be full)
+  const int64_t blocks = (s.B + p.rows - 1) / p.rows, resident = num_sms() * static_cast<int64_t>(std::max(1, 1024 / p.threads));
+  const unsigned grid = static_cast<unsigned>(std::min(blocks, std::max(resident, blocks >> 30)));
   if (p.slots == 1) units_kernel<T, U, ACT, VEC, 1><<<grid, p.threads, 0, st>>>(x, y, mean, rstd, w, bias, s, p, eps);
+  else if (p.slots == 2) units_kernel<T, U, ACT, VEC, 2><<<grid, p.threads, 0, st>>>(x, y, mean, rstd, w, bias, s, p, eps);
   else units_kernel<T, U, ACT, VEC, 4><<<grid, p.threads, 0, st>>>(x, y, mean, rstd, w, bias, s, p, eps);
   return launched("group_norm");
 }
