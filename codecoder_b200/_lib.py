@@ -64,9 +64,9 @@ SIGNATURES = {
     "bpc_embed_wgrad": (ctypes.c_int, [c_vp, c_vp, c_i32, c_vp, c_vp, ctypes.c_size_t, c_i64, c_i32, c_i32, c_i64,
                                        ctypes.c_float, c_i32, c_i32, c_vp]),
     "bpc_group_norm_workspace_size": (ctypes.c_size_t, [c_i64, c_i64, c_i32, c_i32, c_i32, c_i32]),
-    "bpc_group_norm_fwd": (ctypes.c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i32, c_i32, c_i64, c_i64,
+    "bpc_group_norm_fwd": (ctypes.c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i32, c_i32, c_i64, c_i64,
                                           ctypes.c_float, c_i32, c_i32, c_i32, c_vp, ctypes.c_size_t, c_vp]),
-    "bpc_group_norm_bwd": (ctypes.c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i32, c_i32,
+    "bpc_group_norm_bwd": (ctypes.c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i32, c_i32,
                                           c_i64, c_i64, c_i64, c_i64, c_i32, c_i32, c_i32, c_vp, ctypes.c_size_t, c_vp]),
     "bpc_linear_attention_workspace_size": (ctypes.c_size_t, [c_i64, c_i64, c_i32, c_i32, c_i32, c_i32, c_i32]),
     "bpc_linear_attention_fwd": (ctypes.c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i32, c_i64, c_i64, c_i32,

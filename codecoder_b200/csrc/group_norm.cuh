@@ -147,22 +147,24 @@ struct Plan {
 
 constexpr int kUnitThreads = 512;    // at most
 constexpr int kTileThreads = 256;
+constexpr int kDepth = 4;            // samples of units on their way or worked on
 
-// full: elements of a whole access of units, taken where the pointers and strides allow it (`aligned`) and the groups hold whole
-// ones; of tiles kTileVec
-inline Plan make_plan(const Shape& s, int size, int full, int sms, bool aligned) {
+// Whole accesses are taken where the pointers and strides allow it (`aligned`) and the groups hold whole ones: of kTileVec
+// elements in tiles, in units of `full`, SLOTS of them a lane: two where there are two forwards, as the joins and the addresses are
+// half of the rest; one backwards, where the sums of gradients fill the registers, and of kTileVec where one is not enough.
+inline Plan make_plan(const Shape& s, int size, int sms, bool aligned, bool backward) {
   Plan p = {};
   const int cg = s.C / s.G;
-  p.vec = aligned && cg % full == 0 ? full : 1;
-  int across = cg / p.vec;
+  int full = 16 / size;
   // small samples, of which a block per sample and slab would have little: 32-byte pieces of rows at least, or whole rows
-  const int64_t vectors = s.N * across;
-  if (vectors <= 128 && (s.N == 1 || cg * size >= 32)) {
-    // two vectors a lane where there are two: the sums' joins and the addresses are half of the rest
-    p.slots = vectors == 1 ? 1 : vectors <= 64 ? 2 : 4;
+  if (s.N * cg <= 128 * full && (s.N == 1 || cg * size >= 32)) {
+    if (backward && s.N * cg > 32 * full) full = kTileVec;
+    p.vec = aligned && cg % full == 0 ? full : 1;
+    const int vectors = static_cast<int>(s.N) * (cg / p.vec);
+    p.slots = vectors > 64 ? 4 : vectors > (backward ? 32 : 1) ? 2 : 1;
     p.lanes = 1;
     while (p.lanes * p.slots < vectors) p.lanes *= 2;
-    if (static_cast<int64_t>(p.lanes) * s.G <= kUnitThreads) {
+    if (p.lanes <= 32 && p.lanes * s.G <= kUnitThreads) {
       p.kind = kUnits;
       p.rows = std::max(1, 256 / (p.lanes * s.G));
       p.threads = (p.lanes * s.G * p.rows + 31) / 32 * 32;
@@ -170,7 +172,7 @@ inline Plan make_plan(const Shape& s, int size, int full, int sms, bool aligned)
     }
   }
   p.vec = aligned && cg % kTileVec == 0 ? kTileVec : 1;
-  across = cg / p.vec;
+  const int across = cg / p.vec;
   if (across > kTileThreads) {
     p.kind = kWide;
     p.threads = 256;
@@ -265,8 +267,30 @@ __device__ __forceinline__ void cp_async(void* dst, const void* src, std::integr
 __device__ __forceinline__ void cp_async(void* dst, const void* src, std::integral_constant<int, 8>) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
 }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void cp_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// Vectors of the next kDepth - 1 samples on their way through shared memory, each read by the thread that fetched it: no
+// barrier, and no registers (one sample ahead in those kept too little under way).  A stage holds what the block's threads
+// fetch of a sample each; copies cannot take single elements of 2 bytes, which are read when used.
+template <typename T, int VEC>
+struct Copied {
+  using P = Pack<T, VEC>;
+  static constexpr bool kCopies = sizeof(P) >= 4;
+  static constexpr int kBytes = kCopies ? static_cast<int>(sizeof(P)) : 0;
+  __device__ static __forceinline__ void fetch(uint32_t at, const T* src) {
+    if constexpr (kBytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(src) : "memory");
+    else if constexpr (kBytes > 0) asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(at), "l"(src), "n"(kBytes) : "memory");
+  }
+  __device__ static __forceinline__ P take(const uint8_t* smem, uint32_t at, const T* src) {
+    if constexpr (kCopies) return *reinterpret_cast<const P*>(smem + at);
+    else return *reinterpret_cast<const P*>(src);
+  }
+};
 
 // A thread's rows of the next piece of work on their way through shared memory, K vectors of its own (no barrier): fetch
 // starts the copies, take waits for them.  Single elements are read when taken.

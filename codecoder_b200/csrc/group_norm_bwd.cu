@@ -15,8 +15,6 @@ namespace {
 
 namespace cg_ = cooperative_groups;
 
-constexpr int kVec = kTileVec;      // of units too: the sums, the weights and gz are in the registers beside the features
-
 // The channels' sums of a block: thread (row r, vector v) has VEC channels from c on, `rows` rows of threads; into
 // parts[block][2][C]
 template <int VEC>
@@ -45,15 +43,14 @@ __device__ __forceinline__ void channel_sums(const uint64_t (&a)[(VEC + 1) / 2],
 }
 
 // Units: a sample's group per `lanes` lanes, SLOTS vectors each; a thread's slots are the same places of every sample, and
-// the next sample's are on their way while one is worked on.
+// the next samples' are on their way while one is worked on.
 template <typename T, typename U, int ACT, int VEC, int SLOTS>
 __global__ void __launch_bounds__(kUnitThreads) units_kernel(const U* __restrict__ gy, const T* __restrict__ x,
-                                                             const float* __restrict__ mean_in,
-                                                             const float* __restrict__ rstd_in, const float* __restrict__ w,
-                                                             const float* __restrict__ bias, T* __restrict__ dx, float* parts,
+                                                             const float2* __restrict__ stats,
+                                                             const float* __restrict__ w, const float* __restrict__ bias, T* __restrict__ dx, float* parts,
                                                              const Shape s, const Plan p) {
   constexpr int kP = Pack<T, VEC>::kPairs;
-  extern __shared__ float buffer[];
+  extern __shared__ __align__(16) uint8_t smem[];
   const int cg = s.C / s.G, across = cg / VEC;
   const int unit = threadIdx.x / p.lanes, l = threadIdx.x % p.lanes;
   const int g = unit % s.G, r = unit / s.G;
@@ -66,10 +63,6 @@ __global__ void __launch_bounds__(kUnitThreads) units_kernel(const U* __restrict
   T* to[SLOTS];
   bool has[SLOTS];
   uint64_t wv[SLOTS][kP], bv[SLOTS][kP], acc_a[SLOTS][kP], acc_b[SLOTS][kP];
-  Pack<T, VEC> next[SLOTS];
-  Pack<U, VEC> next_g[SLOTS];
-  float mean_next = 0.0f, rstd_next = 0.0f;
-  int64_t stat = (b0 + r) * s.G + g;
 #pragma unroll
   for (int k = 0; k < SLOTS; ++k) {
     const int e = k * p.lanes + l, row = e / across, c = g * cg + e % across * VEC;
@@ -82,34 +75,62 @@ __global__ void __launch_bounds__(kUnitThreads) units_kernel(const U* __restrict
 #pragma unroll
     for (int i = 0; i < kP; ++i) acc_a[k][i] = acc_b[k][i] = 0;
   }
-  auto load = [&](bool live) {
-    if (live) mean_next = mean_in[stat], rstd_next = rstd_in[stat];
-#pragma unroll
-    for (int k = 0; k < SLOTS; ++k) {
-      next[k] = Pack<T, VEC>(), next_g[k] = Pack<U, VEC>();        // zeros: nothing to any sum
-      if (has[k] && live) {
-        next[k] = *reinterpret_cast<const Pack<T, VEC>*>(from[k]);
-        next_g[k] = *reinterpret_cast<const Pack<U, VEC>*>(from_g[k]);
-      }
-    }
-  };
-  load(mine > 0);
   const float per = 1.0f / (static_cast<float>(s.N) * static_cast<float>(cg));
   const int64_t x_step = step * s.x_sample, g_step = step * s.g_sample, o_step = step * s.N * s.C;
+  // a stage: the block's vectors of x, those of gy, the statistics; a thread's places in it, and the stages of the sample
+  // fetched and of the one worked on
+  using X = Copied<T, VEC>;
+  using Y = Copied<U, VEC>;
+  const uint32_t x_bytes = blockDim.x * X::kBytes, g_bytes = blockDim.x * Y::kBytes;
+  const uint32_t at_x = threadIdx.x * X::kBytes, at_g = SLOTS * x_bytes + threadIdx.x * Y::kBytes;
+  const uint32_t at_stat = SLOTS * (x_bytes + g_bytes) + threadIdx.x * 8, stage_bytes = SLOTS * (x_bytes + g_bytes) + blockDim.x * 8;
+  const uint32_t base = smem_u32(smem);
+  uint32_t fetched = 0, used = 0;
+  int64_t ahead_x = 0, ahead_g = 0, off_x = 0, off_g = 0;
+  const float2* stat = stats + (b0 + r) * s.G + g;
+  auto fetch = [&](int round) {
+    if (round < mine) {
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(base + fetched + at_stat), "l"(stat) : "memory");
+#pragma unroll
+      for (int k = 0; k < SLOTS; ++k)
+        if (has[k]) {
+          X::fetch(base + fetched + at_x + k * x_bytes, from[k] + ahead_x);
+          Y::fetch(base + fetched + at_g + k * g_bytes, from_g[k] + ahead_g);
+        }
+    }
+    ahead_x += x_step, ahead_g += g_step, stat += step * s.G;
+    fetched = fetched == (kDepth - 1) * stage_bytes ? 0 : fetched + stage_bytes;
+    cp_commit();
+  };
+#pragma unroll
+  for (int round = 0; round < kDepth - 1; ++round) fetch(round);
   for (int round = 0; round < rounds; ++round) {
-    const uint64_t scale = f2_of(rstd_next), minus = f2_of(-mean_next);
+    fetch(round + kDepth - 1);
+    cp_wait<kDepth - 1>();
+    const bool live = round < mine;
+    float mean = 0.0f, rstd = 0.0f;
+    if (live) {
+      const float2 f = *reinterpret_cast<const float2*>(smem + used + at_stat);
+      mean = f.x, rstd = f.y;
+    }
+    const uint64_t scale = f2_of(rstd), minus = f2_of(-mean);
     uint64_t xh[SLOTS][kP], gz[SLOTS][kP], s1 = 0, s2 = 0;
 #pragma unroll
     for (int k = 0; k < SLOTS; ++k) {
+      Pack<T, VEC> vx = Pack<T, VEC>();            // zeros: nothing to any sum
+      Pack<U, VEC> vg = Pack<U, VEC>();
+      if (has[k] && live) {
+        vx = X::take(smem, used + at_x + k * x_bytes, from[k] + off_x);
+        vg = Y::take(smem, used + at_g + k * g_bytes, from_g[k] + off_g);
+      }
 #pragma unroll
       for (int i = 0; i < kP; ++i) {
-        xh[k][i] = f2_mul(f2_add(next[k].pair(i), minus), scale);
-        gz[k][i] = next_g[k].pair(i);
+        xh[k][i] = f2_mul(f2_add(vx.pair(i), minus), scale);
+        gz[k][i] = vg.pair(i);
       }
-      from[k] += x_step, from_g[k] += g_step;
     }
-    stat += step * s.G;
-    load(round + 1 < mine);
+    off_x += x_step, off_g += g_step;
+    used = used == (kDepth - 1) * stage_bytes ? 0 : used + stage_bytes;
 #pragma unroll
     for (int k = 0; k < SLOTS; ++k)
 #pragma unroll
@@ -133,14 +154,15 @@ __global__ void __launch_bounds__(kUnitThreads) units_kernel(const U* __restrict
         Pack<T, VEC> o;
 #pragma unroll
         for (int i = 0; i < kP; ++i) o.set(i, f2_mul(scale, f2_add(gz[k][i], f2_fma(xh[k][i], u2, u1))));
-        if (has[k] && round < mine) *reinterpret_cast<Pack<T, VEC>*>(to[k]) = o;
+        if (has[k] && live) *reinterpret_cast<Pack<T, VEC>*>(to[k]) = o;
         to[k] += o_step;
       }
     }
   }
   if (!parts) return;
-  // the rows of a sample share channels: a row of the buffer for each of them and each of the block's samples
+  // every copy has been taken: its memory holds the channels' sums now.  The rows of a sample share channels: a row of the buffer for each of them and each of the block's samples
   parts += static_cast<int64_t>(blockIdx.x) * 2 * s.C;
+  float* buffer = reinterpret_cast<float*>(smem);
   const int V = s.G * across, rows = p.rows * static_cast<int>(s.N);
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
@@ -170,9 +192,8 @@ enum Mode { kFused, kSums, kApply };
 // walk the samples.  between: (B, chunks, G) pairs s1, s2 between the two kernels of samples that no cluster holds.
 template <typename T, typename U, int ACT, int VEC, int MODE>
 __global__ void __launch_bounds__(kTileThreads, 2) tiles_kernel(const U* __restrict__ gy, const T* __restrict__ x,
-                                                            const float* __restrict__ mean_in,
-                                                            const float* __restrict__ rstd_in, const float* __restrict__ w,
-                                                            const float* __restrict__ bias, T* __restrict__ dx, float* parts,
+                                                            const float2* __restrict__ stats,
+                                                            const float* __restrict__ w, const float* __restrict__ bias, T* __restrict__ dx, float* parts,
                                                             const Shape s, const Plan p, float2* between) {
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ __align__(16) float part[2][2 * kTileThreads];
@@ -192,11 +213,11 @@ __global__ void __launch_bounds__(kTileThreads, 2) tiles_kernel(const U* __restr
   const int64_t x_step = lanes * s.x_row, g_step = lanes * s.g_row, o_step = static_cast<int64_t>(lanes) * s.C;
   Ahead<T, VEC, kRows> ahead_x(smem);
   Ahead<U, VEC, kRows> ahead_g(smem + Ahead<T, VEC, kRows>::kBytes * kTileThreads);
-  float mean_next = 0.0f, rstd_next = 0.0f;
+  float2 next = make_float2(0.0f, 0.0f);
   auto fetch = [&](int64_t b) {
     ahead_x.fetch(from + b * s.x_sample, x_step, n);
     ahead_g.fetch(from_g + b * s.g_sample, g_step, n);
-    if (there) mean_next = mean_in[b * s.G + g], rstd_next = rstd_in[b * s.G + g];
+    if (there) next = stats[b * s.G + g];
   };
   fetch(sample(blockIdx.y));
   constexpr int kP = Pack<T, VEC>::kPairs;
@@ -209,7 +230,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) tiles_kernel(const U* __restr
   int turn = 0;
   for (int64_t at = blockIdx.y; at < s.B; at += gridDim.y) {
     const int64_t b = sample(at);
-    const uint64_t scale = f2_of(rstd_next), minus = f2_of(-mean_next);
+    const uint64_t scale = f2_of(next.y), minus = f2_of(-next.x);
     Pack<T, VEC> vx[kRows];
     uint64_t gz[kRows][kP];
     float sums[2] = {0.0f, 0.0f};
@@ -354,16 +375,15 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
 
 // Wide groups: a block per sample and group, in two passes
 template <typename T, typename U, int ACT>
-__global__ void __launch_bounds__(256) wide_kernel(const U* __restrict__ gy, const T* __restrict__ x, const float* __restrict__ mean_in,
-                                                   const float* __restrict__ rstd_in, const float* __restrict__ w,
-                                                   const float* __restrict__ bias, T* __restrict__ dx, const Shape s) {
+__global__ void __launch_bounds__(256) wide_kernel(const U* __restrict__ gy, const T* __restrict__ x, const float2* __restrict__ stats,
+                                                   const float* __restrict__ w, const float* __restrict__ bias, T* __restrict__ dx, const Shape s) {
   __shared__ float red[8];
   const int cg = s.C / s.G;
   const int64_t n = s.N * cg;
   for (int64_t at = blockIdx.x; at < s.B * s.G; at += gridDim.x) {
     const int64_t b = at / s.G;
     const int c0 = static_cast<int>(at % s.G) * cg;
-    const float mean = mean_in[at], rstd = rstd_in[at];
+    const float mean = stats[at].x, rstd = stats[at].y;
     float s1 = 0.0f, s2 = 0.0f;
     for (int64_t i = threadIdx.x; i < n; i += 256) {
       const int c = c0 + static_cast<int>(i % cg);
@@ -390,9 +410,8 @@ __global__ void __launch_bounds__(256) wide_kernel(const U* __restrict__ gy, con
 // Wide groups: a thread per channel walks a share of the rows, into the parts that join_kernel adds
 template <typename T, typename U, int ACT>
 __global__ void __launch_bounds__(256) wide_channels_kernel(const U* __restrict__ gy, const T* __restrict__ x,
-                                                            const float* __restrict__ mean_in,
-                                                            const float* __restrict__ rstd_in, const float* __restrict__ w,
-                                                            const float* __restrict__ bias, float* __restrict__ parts, const Shape s) {
+                                                            const float2* __restrict__ stats,
+                                                            const float* __restrict__ w, const float* __restrict__ bias, float* __restrict__ parts, const Shape s) {
   const int c = blockIdx.x * 256 + threadIdx.x;
   if (c >= s.C) return;
   const int g = c / (s.C / s.G);
@@ -400,7 +419,8 @@ __global__ void __launch_bounds__(256) wide_channels_kernel(const U* __restrict_
   double a = 0.0, d = 0.0;
   for (int64_t i = blockIdx.y; i < s.B * s.N; i += gridDim.y) {
     const int64_t b = i / s.N, r = i % s.N;
-    const float xh = (load_f32(x + b * s.x_sample + r * s.x_row + c) - mean_in[b * s.G + g]) * rstd_in[b * s.G + g];
+    const float2 f = stats[b * s.G + g];
+    const float xh = (load_f32(x + b * s.x_sample + r * s.x_row + c) - f.x) * f.y;
     const float gz = load_f32(gy + b * s.g_sample + r * s.g_row + c) * slope1<ACT>(fmaf(wc, xh, bc));
     a += gz;
     d += static_cast<double>(gz) * xh;
@@ -409,7 +429,7 @@ __global__ void __launch_bounds__(256) wide_channels_kernel(const U* __restrict_
   parts[static_cast<int64_t>(blockIdx.y) * 2 * s.C + s.C + c] = static_cast<float>(d);
 }
 
-Plan plan_of(const Shape& s, int size, bool aligned) { return make_plan(s, size, kVec, num_sms(), aligned); }
+Plan plan_of(const Shape& s, int size, bool aligned) { return make_plan(s, size, num_sms(), aligned, true); }
 
 constexpr int kTilesPerSm = 2;
 
@@ -440,26 +460,27 @@ size_t backward_workspace(const Shape& s, int size) {
 
 namespace {
 
+template <typename T, typename U, int ACT, int VEC, int SLOTS>
+int run_units(const U* gy, const T* x, const float2* stats, const float* w, const float* bias, T* dx, float* parts, const Shape& s,
+              const Plan& p, cudaStream_t st) {
+  const int copies = kDepth * ((Copied<T, VEC>::kBytes + Copied<U, VEC>::kBytes) * SLOTS + 8);      // of a thread
+  const int smem = std::max(copies * p.threads, p.rows * static_cast<int>(s.N) * s.C * static_cast<int>(sizeof(float)));
+  Shape shape = s;
+  Plan plan = p;
+  void* args[] = {&gy, &x, &stats, &w, &bias, &dx, &parts, &shape, &plan};
+  return launch(reinterpret_cast<const void*>(&units_kernel<T, U, ACT, VEC, SLOTS>), dim3(static_cast<unsigned>(parts_of(s, p))), p.threads,
+                1, smem, st, args, "group_norm backward");
+}
+
 template <typename T, typename U, int ACT, int VEC>
-int run(const U* gy, const T* x, const float* mean, const float* rstd, const float* w, const float* bias, T* dx, bool want_parts,
-        const Shape& s, const Plan& p, void* ws, cudaStream_t st) {
+int run_tiles(const U* gy, const T* x, const float2* stats, const float* w, const float* bias, T* dx, float* parts, const Shape& s,
+              const Plan& p, void* ws, cudaStream_t st) {
   const char* what = "group_norm backward";
   const int64_t n = parts_of(s, p);
-  float* parts = want_parts ? static_cast<float*>(ws) : nullptr;
-  if (p.kind == kUnits) {
-    const int smem = p.rows * static_cast<int>(s.N) * s.C * static_cast<int>(sizeof(float));
-    const void* fn = p.slots == 1   ? reinterpret_cast<const void*>(&units_kernel<T, U, ACT, VEC, 1>)
-                     : p.slots == 2 ? reinterpret_cast<const void*>(&units_kernel<T, U, ACT, VEC, 2>)
-                                    : reinterpret_cast<const void*>(&units_kernel<T, U, ACT, VEC, 4>);
-    Shape shape = s;
-    Plan plan = p;
-    void* args[] = {&gy, &x, &mean, &rstd, &w, &bias, &dx, &parts, &shape, &plan};
-    return launch(fn, dim3(static_cast<unsigned>(n)), p.threads, 1, smem, st, args, what);
-  }
   float2* between = reinterpret_cast<float2*>(static_cast<char*>(ws) + (sizeof(float) * 2 * s.C * n + 15) / 16 * 16);
   Shape shape = s;
   Plan plan = p;
-  void* args[] = {&gy, &x, &mean, &rstd, &w, &bias, &dx, &parts, &shape, &plan, &between};
+  void* args[] = {&gy, &x, &stats, &w, &bias, &dx, &parts, &shape, &plan, &between};
   const int smem = std::max(Ahead<T, VEC, kRows>::kBytes + Ahead<U, VEC, kRows>::kBytes, VEC * static_cast<int>(sizeof(float))) * kTileThreads;
   const dim3 grid = tiles_grid(s, p, kTilesPerSm, num_sms());
   if (p.fused)
@@ -485,8 +506,8 @@ extern "C" size_t bpc_group_norm_workspace_size(int64_t B, int64_t N, int32_t C,
   return backward ? backward_workspace(s, size_of(x_dtype)) : forward_workspace(s, size_of(x_dtype));
 }
 
-extern "C" int bpc_group_norm_bwd(const void* gy, const void* x, const float* mean, const float* rstd, const float* weight,
-                                  const float* bias, void* dx, float* dw, float* db, int64_t B, int64_t N, int32_t C,
+extern "C" int bpc_group_norm_bwd(const void* gy, const void* x, const float* stats, const float* weight, const float* bias,
+                                  void* dx, float* dw, float* db, int64_t B, int64_t N, int32_t C,
                                   int32_t G, int64_t gy_sample_stride, int64_t gy_row_stride, int64_t x_sample_stride,
                                   int64_t x_row_stride, int32_t activation, int32_t x_dtype, int32_t y_dtype,
                                   void* workspace, size_t workspace_bytes, bpc_stream_t stream) {
@@ -500,16 +521,18 @@ extern "C" int bpc_group_norm_bwd(const void* gy, const void* x, const float* me
     if (db && cudaMemsetAsync(db, 0, sizeof(float) * C, st) != cudaSuccess) return launched(what);
     return 0;
   }
-  if (!gy || !x || !mean || !rstd || !workspace) return fail(BPC_ERR_ARG, "group_norm backward: null buffer");
+  if (!gy || !x || !stats || !workspace) return fail(BPC_ERR_ARG, "group_norm backward: null buffer");
   const int size = size_of(x_dtype), y_size = size_of(y_dtype);
-  if (!aligned(x, size) || !aligned(dx, size) || !aligned(gy, y_size) || !aligned(mean, 4) || !aligned(rstd, 4) ||
+  if (!aligned(x, size) || !aligned(dx, size) || !aligned(gy, y_size) || !aligned(stats, 8) ||
       !aligned(weight, 4) || !aligned(bias, 4) || !aligned(workspace, 16))
-    return fail(BPC_ERR_ARG, "group_norm backward: buffer not aligned to its type (workspace: 16 bytes)");
+    return fail(BPC_ERR_ARG, "group_norm backward: buffer not aligned to its type (stats: 8 bytes, workspace: 16)");
   if (workspace_bytes < bpc_group_norm_workspace_size(B, N, C, G, x_dtype, 1))
     return fail(BPC_ERR_SPACE, "group_norm backward: workspace too small");
   if (!dx && !dw && !db) return 0;
-  auto whole_of = [](const void* q, int64_t sample, int64_t row, int bytes) {
-    return aligned(q, kVec * bytes) && sample % kVec == 0 && row % kVec == 0;
+  // accesses are of as many elements of gy as of x
+  const int64_t full = 16 / size;
+  auto whole_of = [&](const void* q, int64_t sample, int64_t row, int bytes) {
+    return aligned(q, static_cast<int>(full) * bytes) && sample % full == 0 && row % full == 0;
   };
   const bool whole = whole_of(x, x_sample_stride, x_row_stride, size) && whole_of(dx, 0, 0, size) &&
                      whole_of(gy, gy_sample_stride, gy_row_stride, y_size);
@@ -523,19 +546,33 @@ extern "C" int bpc_group_norm_bwd(const void* gy, const void* x, const float* me
       const U* g = static_cast<const U*>(gy);
       const T* from = static_cast<const T*>(x);
       T* to = static_cast<T*>(dx);
+      const float2* pairs = reinterpret_cast<const float2*>(stats);
       if (p.kind == kWide) {
         if (dx) {
           const unsigned grid = static_cast<unsigned>(std::min<int64_t>(B * G, 8 * num_sms()));
-          wide_kernel<T, U, ACT><<<grid, 256, 0, st>>>(g, from, mean, rstd, weight, bias, to, s);
+          wide_kernel<T, U, ACT><<<grid, 256, 0, st>>>(g, from, pairs, weight, bias, to, s);
           if (int e = launched(what)) return e;
         }
         if (!want) return 0;
         const dim3 grid((C + 255) / 256, static_cast<unsigned>(parts_of(s, p)));
-        wide_channels_kernel<T, U, ACT><<<grid, 256, 0, st>>>(g, from, mean, rstd, weight, bias, static_cast<float*>(workspace), s);
+        wide_channels_kernel<T, U, ACT><<<grid, 256, 0, st>>>(g, from, pairs, weight, bias, static_cast<float*>(workspace), s);
         return launched(what);
       }
-      if (p.vec == 1) return run<T, U, ACT, 1>(g, from, mean, rstd, weight, bias, to, want, s, p, workspace, st);
-      return run<T, U, ACT, kVec>(g, from, mean, rstd, weight, bias, to, want, s, p, workspace, st);
+      float* parts = want ? static_cast<float*>(workspace) : nullptr;
+      if (p.kind == kUnits) {
+        auto units = [&](auto vec, auto slots) {
+          return run_units<T, U, ACT, decltype(vec)::value, decltype(slots)::value>(g, from, pairs, weight, bias, to, parts, s, p, st);
+        };
+        std::integral_constant<int, 1> one;
+        std::integral_constant<int, 2> two;
+        std::integral_constant<int, 4> four;
+        if constexpr (sizeof(T) == 2)
+          if (p.vec == 8) return units(std::integral_constant<int, 8>(), one);
+        if (p.vec == 4) return p.slots == 1 ? units(four, one) : p.slots == 2 ? units(four, two) : units(four, four);
+        return p.slots == 1 ? units(one, one) : p.slots == 2 ? units(one, two) : units(one, four);
+      }
+      if (p.vec == 1) return run_tiles<T, U, ACT, 1>(g, from, pairs, weight, bias, to, parts, s, p, workspace, st);
+      return run_tiles<T, U, ACT, kTileVec>(g, from, pairs, weight, bias, to, parts, s, p, workspace, st);
     });
   });
   if (e || !want) return e;

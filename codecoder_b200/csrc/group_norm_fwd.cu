@@ -17,11 +17,10 @@ namespace {
 namespace cg_ = cooperative_groups;
 
 // Units: a sample's group per `lanes` lanes, SLOTS vectors each; a thread's slots are the same places of every sample, and
-// the next sample's are on their way while one is worked on.
+// the next samples' are on their way while one is worked on.
 template <typename T, typename U, int ACT, int VEC, int SLOTS>
-__global__ void __launch_bounds__(kUnitThreads) units_kernel(const T* __restrict__ x, U* __restrict__ y, float* mean_out,
-                                                             float* rstd_out, const float* __restrict__ w,
-                                                             const float* __restrict__ bias, const Shape s, const Plan p, float eps) {
+__global__ void __launch_bounds__(kUnitThreads) units_kernel(const T* __restrict__ x, U* __restrict__ y, float2* stats,
+                                                             const float* __restrict__ w, const float* __restrict__ bias, const Shape s, const Plan p, float eps) {
   constexpr int kP = Pack<T, VEC>::kPairs;
   const int cg = s.C / s.G, across = cg / VEC;
   const int unit = threadIdx.x / p.lanes, l = threadIdx.x % p.lanes;
@@ -34,7 +33,8 @@ __global__ void __launch_bounds__(kUnitThreads) units_kernel(const T* __restrict
   U* to[SLOTS];
   bool has[SLOTS];
   uint64_t wv[SLOTS][kP], bv[SLOTS][kP];
-  Pack<T, VEC> next[SLOTS];
+  using In = Copied<T, VEC>;
+  extern __shared__ __align__(16) uint8_t smem[];
 #pragma unroll
   for (int k = 0; k < SLOTS; ++k) {
     const int e = k * p.lanes + l, row = e / across, c = g * cg + e % across * VEC;
@@ -43,23 +43,42 @@ __global__ void __launch_bounds__(kUnitThreads) units_kernel(const T* __restrict
     to[k] = y + ((b0 + r) * s.N + row) * s.C + c;
     channels<VEC>(w, c, has[k], 1.0f, wv[k]);
     channels<VEC>(bias, c, has[k], 0.0f, bv[k]);
-    next[k] = Pack<T, VEC>();
-    if (has[k] && mine > 0) next[k] = *reinterpret_cast<const Pack<T, VEC>*>(from[k]);
   }
   const float n = static_cast<float>(s.N) * static_cast<float>(cg), per = 1.0f / n;
   const int64_t x_step = step * s.x_sample, y_step = step * s.N * s.C;
-  int64_t stat = (b0 + r) * s.G + g;
+  float2* stat = stats + (b0 + r) * s.G + g;
+  // a thread's places in a stage, and the stages of the sample fetched and of the one worked on
+  const uint32_t mine_at = threadIdx.x * In::kBytes, slot_bytes = blockDim.x * In::kBytes, stage_bytes = SLOTS * slot_bytes;
+  const uint32_t base = smem_u32(smem) + mine_at;
+  uint32_t fetched = 0, used = 0;
+  int64_t ahead = 0, offset = 0;
+  auto fetch = [&](int round) {
+    if (round < mine) {
+#pragma unroll
+      for (int k = 0; k < SLOTS; ++k)
+        if (has[k]) In::fetch(base + fetched + k * slot_bytes, from[k] + ahead);
+    }
+    ahead += x_step;
+    fetched = fetched == (kDepth - 1) * stage_bytes ? 0 : fetched + stage_bytes;
+    cp_commit();
+  };
+#pragma unroll
+  for (int round = 0; round < kDepth - 1; ++round) fetch(round);
   for (int round = 0; round < rounds; ++round) {
     uint64_t d[SLOTS][kP], t = 0;
+    fetch(round + kDepth - 1);
+    cp_wait<kDepth - 1>();
 #pragma unroll
     for (int k = 0; k < SLOTS; ++k) {
+      Pack<T, VEC> v = Pack<T, VEC>();
+      if (has[k] && round < mine) v = In::take(smem, mine_at + used + k * slot_bytes, from[k] + offset);
 #pragma unroll
-      for (int i = 0; i < kP; ++i) d[k][i] = next[k].pair(i);
+      for (int i = 0; i < kP; ++i) d[k][i] = v.pair(i);
 #pragma unroll
       for (int i = 0; i < kP; ++i) t = f2_add(t, d[k][i]);
-      from[k] += x_step;
-      if (has[k] && round + 1 < mine) next[k] = *reinterpret_cast<const Pack<T, VEC>*>(from[k]);
     }
+    used = used == (kDepth - 1) * stage_bytes ? 0 : used + stage_bytes;
+    offset += x_step;
     float sum = both<VEC>(t);
     for (int m = p.lanes >> 1; m; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
     const float mean = over(sum, n, per);
@@ -78,7 +97,7 @@ __global__ void __launch_bounds__(kUnitThreads) units_kernel(const T* __restrict
     float sq = both<VEC>(t);
     for (int m = p.lanes >> 1; m; m >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, m);
     const float rstd = inverse_sqrt(fmaf(sq, per, eps));
-    if (mean_out && l == 0 && round < mine) mean_out[stat] = mean, rstd_out[stat] = rstd;
+    if (stats && l == 0 && round < mine) *stat = make_float2(mean, rstd);
     stat += step * s.G;
     const uint64_t scale = f2_of(rstd);
 #pragma unroll
@@ -97,9 +116,8 @@ enum Mode { kFused, kStats, kApply };
 // Tiles: a block's chunk of a slab in registers, the next sample's on its way meanwhile.  parts: (B, chunks, G) pairs of mean
 // and summed squared differences between the two kernels of samples that no cluster holds.
 template <typename T, typename U, int ACT, int VEC, int MODE>
-__global__ void __launch_bounds__(kTileThreads, 3) tiles_kernel(const T* __restrict__ x, U* __restrict__ y, float* mean_out,
-                                                               float* rstd_out, const float* __restrict__ w,
-                                                               const float* __restrict__ bias, const Shape s, const Plan p, float eps,
+__global__ void __launch_bounds__(kTileThreads, 3) tiles_kernel(const T* __restrict__ x, U* __restrict__ y, float2* stats,
+                                                               const float* __restrict__ w, const float* __restrict__ bias, const Shape s, const Plan p, float eps,
                                                                float2* parts) {
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ __align__(16) float part[2][kTileThreads];
@@ -211,10 +229,7 @@ __global__ void __launch_bounds__(kTileThreads, 3) tiles_kernel(const T* __restr
     }
     if constexpr (MODE != kStats) {
       rstd = inverse_sqrt(fmaf(sq[0], per, eps));
-      if (speaks && chunk == 0 && mean_out) {
-        mean_out[b * s.G + g] = mean;
-        rstd_out[b * s.G + g] = rstd;
-      }
+      if (speaks && chunk == 0 && stats) stats[b * s.G + g] = make_float2(mean, rstd);
       U* out = to + b * s.N * s.C;
       uint64_t scale[kP];
 #pragma unroll
@@ -250,7 +265,7 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
 
 // Wide groups: a block per sample and group, in three passes
 template <typename T, typename U, int ACT>
-__global__ void __launch_bounds__(256) wide_kernel(const T* __restrict__ x, U* __restrict__ y, float* mean_out, float* rstd_out,
+__global__ void __launch_bounds__(256) wide_kernel(const T* __restrict__ x, U* __restrict__ y, float2* stats,
                                                    const float* __restrict__ w, const float* __restrict__ bias, const Shape s,
                                                    float eps) {
   __shared__ float red[8];
@@ -269,7 +284,7 @@ __global__ void __launch_bounds__(256) wide_kernel(const T* __restrict__ x, U* _
       sq = fmaf(d, d, sq);
     }
     const float rstd = 1.0f / sqrtf(block_sum(sq, red) / static_cast<float>(n) + eps);
-    if (threadIdx.x == 0 && mean_out) mean_out[at] = mean, rstd_out[at] = rstd;
+    if (threadIdx.x == 0 && stats) stats[at] = make_float2(mean, rstd);
     for (int64_t i = threadIdx.x; i < n; i += 256) {
       const int c = c0 + static_cast<int>(i % cg);
       const int64_t r = i / cg;
@@ -279,7 +294,7 @@ __global__ void __launch_bounds__(256) wide_kernel(const T* __restrict__ x, U* _
   }
 }
 
-Plan plan_of(const Shape& s, int size, bool aligned) { return make_plan(s, size, 16 / size, num_sms(), aligned); }
+Plan plan_of(const Shape& s, int size, bool aligned) { return make_plan(s, size, num_sms(), aligned, false); }
 
 }  // namespace
 
@@ -295,25 +310,28 @@ size_t forward_workspace(const Shape& s, int size) {
 namespace {
 
 template <typename T, typename U, int ACT, int VEC>
-int run_units(const T* x, U* y, float* mean, float* rstd, const float* w, const float* bias, const Shape& s, const Plan& p, float eps,
+int run_units(const T* x, U* y, float2* stats, const float* w, const float* bias, const Shape& s, const Plan& p, float eps,
               cudaStream_t st) {
   // rounds are counted in 32 bits: more blocks for more than 2^31 of them (of which the first ones' memory would be full)
   const int64_t blocks = (s.B + p.rows - 1) / p.rows, resident = num_sms() * static_cast<int64_t>(std::max(1, 1024 / p.threads));
   const unsigned grid = static_cast<unsigned>(std::min(blocks, std::max(resident, blocks >> 30)));
-  if (p.slots == 1) units_kernel<T, U, ACT, VEC, 1><<<grid, p.threads, 0, st>>>(x, y, mean, rstd, w, bias, s, p, eps);
-  else if (p.slots == 2) units_kernel<T, U, ACT, VEC, 2><<<grid, p.threads, 0, st>>>(x, y, mean, rstd, w, bias, s, p, eps);
-  else units_kernel<T, U, ACT, VEC, 4><<<grid, p.threads, 0, st>>>(x, y, mean, rstd, w, bias, s, p, eps);
-  return launched("group_norm");
+  Shape shape = s;
+  Plan plan = p;
+  void* args[] = {&x, &y, &stats, &w, &bias, &shape, &plan, &eps};
+  const void* fn = p.slots == 1   ? reinterpret_cast<const void*>(&units_kernel<T, U, ACT, VEC, 1>)
+                   : p.slots == 2 ? reinterpret_cast<const void*>(&units_kernel<T, U, ACT, VEC, 2>)
+                                  : reinterpret_cast<const void*>(&units_kernel<T, U, ACT, VEC, 4>);
+  return launch(fn, dim3(grid), p.threads, 1, kDepth * Copied<T, VEC>::kBytes * p.slots * p.threads, st, args, "group_norm");
 }
 
 template <typename T, typename U, int ACT, int VEC>
-int run_tiles(const T* x, U* y, float* mean, float* rstd, const float* w, const float* bias, const Shape& s, const Plan& p, float eps,
+int run_tiles(const T* x, U* y, float2* stats, const float* w, const float* bias, const Shape& s, const Plan& p, float eps,
               void* ws, cudaStream_t st) {
   const char* what = "group_norm";
   float2* parts = static_cast<float2*>(ws);
   Shape shape = s;
   Plan plan = p;
-  void* args[] = {&x, &y, &mean, &rstd, &w, &bias, &shape, &plan, &eps, &parts};
+  void* args[] = {&x, &y, &stats, &w, &bias, &shape, &plan, &eps, &parts};
   const dim3 grid = tiles_grid(s, p, 3, num_sms());
   const int smem = Ahead<T, VEC, kRows>::kBytes * kTileThreads;
   if (p.fused)
@@ -330,7 +348,7 @@ int run_tiles(const T* x, U* y, float* mean, float* rstd, const float* w, const 
 using namespace bpc;
 using namespace bpc::gn;
 
-extern "C" int bpc_group_norm_fwd(const void* x, void* y, float* mean, float* rstd, const float* weight, const float* bias,
+extern "C" int bpc_group_norm_fwd(const void* x, void* y, float* stats, const float* weight, const float* bias,
                                   int64_t B, int64_t N, int32_t C, int32_t G, int64_t x_sample_stride,
                                   int64_t x_row_stride, float eps, int32_t activation, int32_t x_dtype, int32_t y_dtype,
                                   void* workspace, size_t workspace_bytes, bpc_stream_t stream) {
@@ -338,13 +356,12 @@ extern "C" int bpc_group_norm_fwd(const void* x, void* y, float* mean, float* rs
   const char* what = "group_norm";
   if (int e = check_shape(s, activation, x_dtype, y_dtype, what)) return e;
   if (!(eps >= 0.0f) || std::isinf(eps)) return fail(BPC_ERR_ARG, "group_norm: eps must be finite and not negative");
-  if (!mean != !rstd) return fail(BPC_ERR_ARG, "group_norm: give both mean and rstd, or neither");
   if (B == 0 || N == 0) return 0;
   if (!x || !y || !workspace) return fail(BPC_ERR_ARG, "group_norm: null buffer");
   const int size = size_of(x_dtype);
-  if (!aligned(x, size) || !aligned(y, size_of(y_dtype)) || !aligned(mean, 4) || !aligned(rstd, 4) || !aligned(weight, 4) ||
-      !aligned(bias, 4) || !aligned(workspace, 16))
-    return fail(BPC_ERR_ARG, "group_norm: buffer not aligned to its type (workspace: 16 bytes)");
+  if (!aligned(x, size) || !aligned(y, size_of(y_dtype)) || !aligned(stats, 8) || !aligned(weight, 4) || !aligned(bias, 4) ||
+      !aligned(workspace, 16))
+    return fail(BPC_ERR_ARG, "group_norm: buffer not aligned to its type (stats: 8 bytes, workspace: 16)");
   if (workspace_bytes < bpc_group_norm_workspace_size(B, N, C, G, x_dtype, 0)) return fail(BPC_ERR_SPACE, "group_norm: workspace too small");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const bool whole = aligned(x, 16) && aligned(y, 16) && x_sample_stride * size % 16 == 0 && x_row_stride * size % 16 == 0;
@@ -356,17 +373,18 @@ extern "C" int bpc_group_norm_fwd(const void* x, void* y, float* mean, float* rs
       constexpr int ACT = decltype(act)::value;
       const T* from = static_cast<const T*>(x);
       U* to = static_cast<U*>(y);
+      float2* pairs = reinterpret_cast<float2*>(stats);
       if (p.kind == kWide) {
         const unsigned grid = static_cast<unsigned>(std::min<int64_t>(B * G, 8 * num_sms()));
-        wide_kernel<T, U, ACT><<<grid, 256, 0, st>>>(from, to, mean, rstd, weight, bias, s, eps);
+        wide_kernel<T, U, ACT><<<grid, 256, 0, st>>>(from, to, pairs, weight, bias, s, eps);
         return launched(what);
       }
       if (p.kind == kUnits) {
-        if (p.vec == 1) return run_units<T, U, ACT, 1>(from, to, mean, rstd, weight, bias, s, p, eps, st);
-        return run_units<T, U, ACT, 16 / sizeof(T)>(from, to, mean, rstd, weight, bias, s, p, eps, st);
+        if (p.vec == 1) return run_units<T, U, ACT, 1>(from, to, pairs, weight, bias, s, p, eps, st);
+        return run_units<T, U, ACT, 16 / sizeof(T)>(from, to, pairs, weight, bias, s, p, eps, st);
       }
-      if (p.vec == 1) return run_tiles<T, U, ACT, 1>(from, to, mean, rstd, weight, bias, s, p, eps, workspace, st);
-      return run_tiles<T, U, ACT, kTileVec>(from, to, mean, rstd, weight, bias, s, p, eps, workspace, st);
+      if (p.vec == 1) return run_tiles<T, U, ACT, 1>(from, to, pairs, weight, bias, s, p, eps, workspace, st);
+      return run_tiles<T, U, ACT, kTileVec>(from, to, pairs, weight, bias, s, p, eps, workspace, st);
     });
   });
 }

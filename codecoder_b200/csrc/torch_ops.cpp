@@ -287,30 +287,30 @@ Tensor norm_workspace(const Tensor& x, int64_t groups, bool backward) {
                at::kByte, x);
 }
 
-// y, and where `stats` is set the groups' mean and rstd (samples, groups)
-std::tuple<Tensor, Tensor, Tensor> group_norm_fwd(const Tensor& x_in, int64_t groups, const std::optional<Tensor>& weight,
+// y, and where `want_stats` is set the groups' statistics (samples, groups, 2)
+std::tuple<Tensor, Tensor> group_norm_fwd(const Tensor& x_in, int64_t groups, const std::optional<Tensor>& weight,
                                                   const std::optional<Tensor>& bias, double eps, int64_t activation,
-                                                  std::optional<at::ScalarType> dtype, bool stats) {
+                                                  std::optional<at::ScalarType> dtype, bool want_stats) {
   at::NoGradGuard no_grad;
   const at::ScalarType out = dtype.value_or(x_in.scalar_type());
   check_norm(x_in, groups, weight, bias, out);
   const c10::cuda::CUDAGuard guard(x_in.device());
-  Tensor y = empty(x_in.sizes(), out, x_in), mean, rstd;
-  if (stats) mean = empty({x_in.size(0), groups}, at::kFloat, x_in), rstd = at::empty_like(mean);
-  if (y.numel() == 0) return {y, mean, rstd};
+  Tensor y = empty(x_in.sizes(), out, x_in), stats;
+  if (want_stats) stats = empty({x_in.size(0), groups, 2}, at::kFloat, x_in);
+  if (y.numel() == 0) return {y, stats};
   Tensor x = samples_of(x_in), w = channel_vector(weight), b = channel_vector(bias), ws = norm_workspace(x, groups, false);
-  check(entry.group_norm_fwd(x.const_data_ptr(), y.data_ptr(), stats ? static_cast<float*>(mean.data_ptr()) : nullptr,
-                             stats ? static_cast<float*>(rstd.data_ptr()) : nullptr, f32_or_null(w), f32_or_null(b),
-                             x.size(0), x.size(1), static_cast<int32_t>(x.size(2)), static_cast<int32_t>(groups),
-                             x.stride(0), x.stride(1), static_cast<float>(eps), static_cast<int32_t>(activation),
-                             dtype_code(x.scalar_type()), dtype_code(out), ws.data_ptr(), ws.numel(), stream_of(x)),
+  check(entry.group_norm_fwd(x.const_data_ptr(), y.data_ptr(), want_stats ? static_cast<float*>(stats.data_ptr()) : nullptr,
+                             f32_or_null(w), f32_or_null(b), x.size(0), x.size(1), static_cast<int32_t>(x.size(2)),
+                             static_cast<int32_t>(groups), x.stride(0), x.stride(1), static_cast<float>(eps),
+                             static_cast<int32_t>(activation), dtype_code(x.scalar_type()), dtype_code(out), ws.data_ptr(),
+                             ws.numel(), stream_of(x)),
         "bpc_group_norm_fwd");
-  return {y, mean, rstd};
+  return {y, stats};
 }
 
 // dx, dw, db; undefined where `want` says that one is not asked for
-std::tuple<Tensor, Tensor, Tensor> group_norm_bwd(const Tensor& gy_in, const Tensor& x_in, const Tensor& mean,
-                                                  const Tensor& rstd, int64_t groups, const std::optional<Tensor>& weight,
+std::tuple<Tensor, Tensor, Tensor> group_norm_bwd(const Tensor& gy_in, const Tensor& x_in, const Tensor& stats,
+                                                  int64_t groups, const std::optional<Tensor>& weight,
                                                   const std::optional<Tensor>& bias, int64_t activation, bool want_dx,
                                                   bool want_dw, bool want_db) {
   at::NoGradGuard no_grad;
@@ -330,8 +330,8 @@ std::tuple<Tensor, Tensor, Tensor> group_norm_bwd(const Tensor& gy_in, const Ten
   }
   Tensor x = samples_of(x_in), gy = samples_of(gy_in), w = channel_vector(weight), b = channel_vector(bias);
   Tensor ws = norm_workspace(x, groups, true);
-  check(entry.group_norm_bwd(gy.const_data_ptr(), x.const_data_ptr(), f32_or_null(mean), f32_or_null(rstd), f32_or_null(w),
-                             f32_or_null(b), want_dx ? dx.data_ptr() : nullptr,
+  check(entry.group_norm_bwd(gy.const_data_ptr(), x.const_data_ptr(), f32_or_null(stats), f32_or_null(w), f32_or_null(b),
+                             want_dx ? dx.data_ptr() : nullptr,
                              want_dw ? static_cast<float*>(dw.data_ptr()) : nullptr,
                              want_db ? static_cast<float*>(db.data_ptr()) : nullptr, x.size(0), x.size(1),
                              static_cast<int32_t>(C), static_cast<int32_t>(groups), gy.stride(0), gy.stride(1), x.stride(0),

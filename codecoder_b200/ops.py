@@ -604,8 +604,8 @@ class GroupNormB200(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, groups, weight, bias, eps, act, dtype):
-        y, mean, rstd = _lib.torch_ops().group_norm_fwd(x, groups, weight, bias, eps, act, dtype, True)
-        ctx.save_for_backward(x, mean, rstd, weight, bias)
+        y, stats = _lib.torch_ops().group_norm_fwd(x, groups, weight, bias, eps, act, dtype, True)
+        ctx.save_for_backward(x, stats, weight, bias)
         ctx.set_materialize_grads(False)
         ctx.groups, ctx.act = groups, act
         return y
@@ -615,10 +615,9 @@ class GroupNormB200(torch.autograd.Function):
     def backward(ctx, gy):
         if gy is None:
             return (None,) * 7
-        x, mean, rstd, weight, bias = ctx.saved_tensors
+        x, stats, weight, bias = ctx.saved_tensors
         need = ctx.needs_input_grad
-        dx, dw, db = _lib.torch_ops().group_norm_bwd(gy, x, mean, rstd, ctx.groups, weight, bias, ctx.act, need[0], need[2],
-                                                     need[3])
+        dx, dw, db = _lib.torch_ops().group_norm_bwd(gy, x, stats, ctx.groups, weight, bias, ctx.act, need[0], need[2], need[3])
         return (dx, None, dw.to(weight.dtype) if need[2] else None, db.to(bias.dtype) if need[3] else None, None, None, None)
 
 

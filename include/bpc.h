@@ -164,19 +164,19 @@ BPC_API int bpc_embed_wgrad(const void* gy, const void* ids, int32_t id_bytes, v
  *   act: BPC_ACT_NONE z; BPC_ACT_SILU z / (1 + e^-z); BPC_ACT_GELU z / (1 + e^-2u), u = sqrt(2 / pi) (z + 0.044715 z^3)
  *   backward: dx, dw, db of sum(gy * y)
  * x: samples x_sample_stride and rows x_row_stride elements apart, channels contiguous, f32, bf16 or f16; y (B, N, C)
- * contiguous, x's type or, for f32 x, a narrower one; mean, rstd (B, G) fp32: written by the forward pass (or both
- * NULL), read by the backward pass; weight, bias (C) fp32 or NULL (1, 0).  gy: y's type, any strides as x; dx (B, N, C)
+ * contiguous, x's type or, for f32 x, a narrower one; stats (B, G, 2) fp32, 8-byte aligned: each group's mean
+ * and 1 / sqrt(var + eps), written by the forward pass (or NULL), read by the backward pass; weight, bias (C) fp32 or NULL (1, 0).  gy: y's type, any strides as x; dx (B, N, C)
  * contiguous, x's type; dw, db (C) fp32; NULL where a gradient is not wanted.  Statistics and sums are fp32 or wider, in
  * a fixed order (deterministic), each result rounded once.  N <= 2^30, C <= 2^20; every buffer aligned to its type.
  * workspace: bpc_group_norm_workspace_size() bytes on the current device, 16-byte aligned. */
 enum { BPC_ACT_NONE = 0, BPC_ACT_SILU = 1, BPC_ACT_GELU = 2 };
 BPC_API size_t bpc_group_norm_workspace_size(int64_t B, int64_t N, int32_t C, int32_t G, int32_t x_dtype, int32_t backward);
-BPC_API int bpc_group_norm_fwd(const void* x, void* y, float* mean, float* rstd, const float* weight, const float* bias,
+BPC_API int bpc_group_norm_fwd(const void* x, void* y, float* stats, const float* weight, const float* bias,
                                int64_t B, int64_t N, int32_t C, int32_t G, int64_t x_sample_stride, int64_t x_row_stride,
                                float eps, int32_t activation, int32_t x_dtype, int32_t y_dtype, void* workspace,
                                size_t workspace_bytes, bpc_stream_t stream);
-BPC_API int bpc_group_norm_bwd(const void* gy, const void* x, const float* mean, const float* rstd, const float* weight,
-                               const float* bias, void* dx, float* dw, float* db, int64_t B, int64_t N, int32_t C, int32_t G,
+BPC_API int bpc_group_norm_bwd(const void* gy, const void* x, const float* stats, const float* weight, const float* bias,
+                               void* dx, float* dw, float* db, int64_t B, int64_t N, int32_t C, int32_t G,
                                int64_t gy_sample_stride, int64_t gy_row_stride, int64_t x_sample_stride,
                                int64_t x_row_stride, int32_t activation, int32_t x_dtype, int32_t y_dtype, void* workspace,
                                size_t workspace_bytes, bpc_stream_t stream);

@@ -27,7 +27,7 @@ def call(f, args, **changes):
 
 def test_group_norm_refusals(lib):
     f = lib.bpc_group_norm_fwd
-    ok = dict(x=16, y=16, mean=None, rstd=None, w=None, b=None, B=2, N=3, C=8, G=2, ss=24, rs=8, eps=1e-5, act=1, xt=F32,
+    ok = dict(x=16, y=16, stats=None, w=None, b=None, B=2, N=3, C=8, G=2, ss=24, rs=8, eps=1e-5, act=1, xt=F32,
               yt=BF16, ws=16, wsb=1 << 40, st=None)
     for name in ("x", "y", "ws"):
         refused(call(f, ok, **{name: None}), "null")
@@ -44,9 +44,7 @@ def test_group_norm_refusals(lib):
     refused(call(f, ok, rs=-8), "strides")
     refused(call(f, ok, eps=-1e-5), "eps")
     refused(call(f, ok, eps=float("nan")), "eps")
-    refused(call(f, ok, mean=16), "both")
-    ok.update(mean=16, rstd=16)
-    for name, at in (("x", 18), ("y", 17), ("mean", 18), ("rstd", 18), ("w", 18), ("b", 18), ("ws", 8)):
+    for name, at in (("x", 18), ("y", 17), ("stats", 20), ("w", 18), ("b", 18), ("ws", 8)):
         refused(call(f, ok, **{name: at}), "aligned")
     refused(call(f, ok, wsb=0), "workspace", code=6)
     assert call(f, ok, B=0, x=None, y=None) == 0 and call(f, ok, N=0, x=None, y=None) == 0
@@ -56,15 +54,15 @@ def test_group_norm_refusals(lib):
 
 def test_group_norm_backward_refusals(lib):
     f = lib.bpc_group_norm_bwd
-    ok = dict(gy=16, x=16, mean=16, rstd=16, w=None, b=None, dx=16, dw=16, db=16, B=2, N=3, C=8, G=2, gs=24, gr=8, xs=24, xr=8,
+    ok = dict(gy=16, x=16, stats=16, w=None, b=None, dx=16, dw=16, db=16, B=2, N=3, C=8, G=2, gs=24, gr=8, xs=24, xr=8,
               act=1, xt=F32, yt=BF16, ws=16, wsb=1 << 40, st=None)
-    for name in ("gy", "x", "mean", "rstd", "ws"):
+    for name in ("gy", "x", "stats", "ws"):
         refused(call(f, ok, **{name: None}), "null")
     refused(call(f, ok, G=5), "divide")
     refused(call(f, ok, gr=-1), "strides")
     refused(call(f, ok, act=-1), "activation")
     refused(call(f, ok, xt=F16, yt=BF16), "dtype")
-    for name, at in (("gy", 17), ("x", 18), ("dx", 18), ("mean", 18), ("rstd", 18), ("w", 18), ("b", 18), ("dw", 18), ("db", 18),
+    for name, at in (("gy", 17), ("x", 18), ("dx", 18), ("stats", 20), ("w", 18), ("b", 18), ("dw", 18), ("db", 18),
                      ("ws", 8)):
         refused(call(f, ok, **{name: at}), "aligned")
     refused(call(f, ok, wsb=0), "workspace", code=6)
