@@ -24,27 +24,40 @@ __device__ __forceinline__ void store_f32(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store_f32(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 __device__ __forceinline__ void store_f32(__half* p, float v) { *p = __float2half_rn(v); }
 
-// VEC elements of an access.  Arithmetic is on pairs of them in fp32 (f2_* of bpc_common.cuh: half the instructions); a single
-// element has a pair with a zero beside it.
+// VEC elements of an access, as 32-bit words.  Arithmetic is on pairs of them in fp32 (f2_* of bpc_common.cuh: half the
+// instructions); a single element has a pair with a zero beside it.
 template <typename T, int VEC>
 struct alignas(sizeof(T) * VEC) Pack {
-  static constexpr int kPairs = (VEC + 1) / 2;
-  T v[VEC];
+  static constexpr int kPairs = VEC / 2;
+  static constexpr bool kF32 = sizeof(T) == 4;
+  uint32_t w[VEC * sizeof(T) / 4];
   __device__ __forceinline__ uint64_t pair(int k) const {
-    if constexpr (VEC == 1) return f2_pack(load_f32(&v[0]), 0.0f);
-    else return f2_pack(load_f32(&v[2 * k]), load_f32(&v[2 * k + 1]));
-  }
-  __device__ __forceinline__ void set(int k, uint64_t x) {
-    if constexpr (VEC == 1) {
-      store_f32(&v[0], f2_lo(x));
-    } else if constexpr (sizeof(T) == 4) {
-      v[2 * k] = f2_lo(x), v[2 * k + 1] = f2_hi(x);
+    if constexpr (kF32) {
+      return f2_pack(__uint_as_float(w[2 * k]), __uint_as_float(w[2 * k + 1]));
     } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-      *reinterpret_cast<__nv_bfloat162*>(&v[2 * k]) = __floats2bfloat162_rn(f2_lo(x), f2_hi(x));
+      return bf2_to_f2(w[k]);
     } else {
-      *reinterpret_cast<__half2*>(&v[2 * k]) = __floats2half2_rn(f2_lo(x), f2_hi(x));
+      const float2 f = __half22float2(__halves2half2(__ushort_as_half(w[k] & 0xffff), __ushort_as_half(w[k] >> 16)));
+      return f2_pack(f.x, f.y);
     }
   }
+  __device__ __forceinline__ void set(int k, uint64_t x) {
+    if constexpr (kF32) {
+      w[2 * k] = __float_as_uint(f2_lo(x)), w[2 * k + 1] = __float_as_uint(f2_hi(x));
+    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      w[k] = f2_to_bf2(x);
+    } else {
+      const __half2 h = __floats2half2_rn(f2_lo(x), f2_hi(x));
+      w[k] = static_cast<uint32_t>(__half_as_ushort(__low2half(h))) | static_cast<uint32_t>(__half_as_ushort(__high2half(h))) << 16;
+    }
+  }
+};
+template <typename T>
+struct alignas(sizeof(T)) Pack<T, 1> {
+  static constexpr int kPairs = 1;
+  T v;
+  __device__ __forceinline__ uint64_t pair(int) const { return f2_pack(load_f32(&v), 0.0f); }
+  __device__ __forceinline__ void set(int, uint64_t x) { store_f32(&v, f2_lo(x)); }
 };
 template <int VEC>
 __device__ __forceinline__ float both(uint64_t x) {
@@ -110,6 +123,14 @@ __device__ __forceinline__ float slope1(float z) {
 __device__ __forceinline__ float over(float sum, float n, float per) {
   const float q = sum * per;
   return fmaf(fmaf(-q, n, sum), per, q);
+}
+
+// the sum over `lanes` neighbouring lanes, in each of them; the steps written out: a loop of them costs as much again
+__device__ __forceinline__ float lanes_sum(float v, int lanes) {
+#pragma unroll
+  for (int m = 1; m < 32; m *= 2)
+    if (lanes > m) v += __shfl_xor_sync(0xffffffffu, v, m);
+  return v;
 }
 
 // 1 / sqrt(v) to within 2^-23: the approximation and one step of Newton's, but at the ends, where that has no value

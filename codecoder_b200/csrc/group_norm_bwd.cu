@@ -142,11 +142,7 @@ __global__ void __launch_bounds__(kUnitThreads) units_kernel(const U* __restrict
         s1 = f2_add(s1, gz[k][i]);
         s2 = f2_fma(gz[k][i], xh[k][i], s2);
       }
-    float m1 = both<VEC>(s1), m2 = both<VEC>(s2);
-    for (int m = p.lanes >> 1; m; m >>= 1) {
-      m1 += __shfl_xor_sync(0xffffffffu, m1, m);
-      m2 += __shfl_xor_sync(0xffffffffu, m2, m);
-    }
+    const float m1 = lanes_sum(both<VEC>(s1), p.lanes), m2 = lanes_sum(both<VEC>(s2), p.lanes);
     if (dx) {
       const uint64_t u1 = f2_of(-m1 * per), u2 = f2_of(-m2 * per);
 #pragma unroll

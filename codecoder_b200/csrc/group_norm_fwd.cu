@@ -79,9 +79,7 @@ __global__ void __launch_bounds__(kUnitThreads) units_kernel(const T* __restrict
     }
     used = used == (kDepth - 1) * stage_bytes ? 0 : used + stage_bytes;
     offset += x_step;
-    float sum = both<VEC>(t);
-    for (int m = p.lanes >> 1; m; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
-    const float mean = over(sum, n, per);
+    const float mean = over(lanes_sum(both<VEC>(t), p.lanes), n, per);
     const uint64_t minus = f2_of(-mean);
     t = 0;
 #pragma unroll
@@ -94,9 +92,7 @@ __global__ void __launch_bounds__(kUnitThreads) units_kernel(const T* __restrict
       }
       if (has[k]) t = f2_add(t, u);
     }
-    float sq = both<VEC>(t);
-    for (int m = p.lanes >> 1; m; m >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, m);
-    const float rstd = inverse_sqrt(fmaf(sq, per, eps));
+    const float rstd = inverse_sqrt(fmaf(lanes_sum(both<VEC>(t), p.lanes), per, eps));
     if (stats && l == 0 && round < mine) *stat = make_float2(mean, rstd);
     stat += step * s.G;
     const uint64_t scale = f2_of(rstd);

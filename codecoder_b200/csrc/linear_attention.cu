@@ -909,25 +909,102 @@ __global__ void __launch_bounds__(kThreads) short_kernel(const __grid_constant__
   }
 }
 
-// One block per sequence and head: the state updated and read once.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) step_kernel(const T* __restrict__ q, const T* __restrict__ k,
-                                                        const T* __restrict__ v, T* __restrict__ o,
-                                                        const float* __restrict__ log_decay, const float* state,
-                                                        float* new_state, int H, int dk, int dv, int64_t qb, int64_t qh,
-                                                        int64_t kb, int64_t kh, int64_t vb, int64_t vh, float scale) {
-  const int64_t at = blockIdx.x, b = at / H;
-  const int h = static_cast<int>(at % H), j = threadIdx.x;
-  if (j >= dv) return;
-  const float a = expf(log_decay[h]), c = load_f32(v + b * vb + h * vh + j);
-  float sum = 0.0f;
-  for (int i = 0; i < dk; ++i) {
-    const int64_t e = (at * dk + i) * dv + j;
-    const float s = fmaf(load_f32(k + b * kb + h * kh + i), c, a * state[e]);
-    new_state[e] = s;
-    sum = fmaf(load_f32(q + b * qb + h * qh + i), s, sum);
+// ---- one position --------------------------------------------------------------------------------------------------
+// The state updated and read once: memory alone bounds it.  WARPS warps per sequence and head, each some rows of the state; LV
+// lanes of four columns across a row, so that a lane has 16-byte pieces of kUnroll rows under way.
+struct Step {
+  const void *q, *k, *v;
+  void* o;
+  const float *log_decay, *state;
+  float* new_state;
+  uint32_t items;               // B H
+  int H, dk, dv;
+  int64_t qb, qh, kb, kh, vb, vh;
+  float scale;
+};
+
+template <typename T, int LV, int WARPS>
+__global__ void __launch_bounds__(kThreads) step_kernel(const __grid_constant__ Step p) {
+  constexpr int kUnroll = 8, kAcross = 32 / LV;      // rows at a time
+  __shared__ float4 sums[WARPS > 1 ? kThreads : 1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % WARPS;
+  const uint32_t at = blockIdx.x * (kThreads / 32 / WARPS) + warp / WARPS;
+  const bool there = at < p.items;
+  const uint32_t b = there ? at / p.H : 0;
+  const int h = there ? static_cast<int>(at - b * p.H) : 0;
+  const int col = lane % LV * 4, share = (p.dk + WARPS - 1) / WARPS;
+  const int row0 = part * share + lane / LV, end = min(p.dk, (part + 1) * share);
+  const bool has = there && col < p.dv;
+  const T* q = static_cast<const T*>(p.q) + b * p.qb + h * p.qh;
+  const T* k = static_cast<const T*>(p.k) + b * p.kb + h * p.kh;
+  const T* v = static_cast<const T*>(p.v) + b * p.vb + h * p.vh + col;
+  const float a = expf(p.log_decay[h]);
+  float4 c = make_float4(0.0f, 0.0f, 0.0f, 0.0f), o = c;
+  if (has) c = make_float4(load_f32(v), load_f32(v + 1), load_f32(v + 2), load_f32(v + 3));
+  const int64_t base = static_cast<int64_t>(at) * p.dk * p.dv + col;
+  for (int r0 = row0; r0 - lane / LV < end; r0 += kUnroll * kAcross) {
+    float4 s[kUnroll];
+    float kr[kUnroll], qr[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int row = r0 + u * kAcross;
+      if (has && row < end) {
+        s[u] = *reinterpret_cast<const float4*>(p.state + base + row * p.dv);
+        kr[u] = load_f32(k + row), qr[u] = load_f32(q + row);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int row = r0 + u * kAcross;
+      if (has && row < end) {
+        s[u].x = fmaf(kr[u], c.x, a * s[u].x), s[u].y = fmaf(kr[u], c.y, a * s[u].y);
+        s[u].z = fmaf(kr[u], c.z, a * s[u].z), s[u].w = fmaf(kr[u], c.w, a * s[u].w);
+        *reinterpret_cast<float4*>(p.new_state + base + row * p.dv) = s[u];
+        o.x = fmaf(qr[u], s[u].x, o.x), o.y = fmaf(qr[u], s[u].y, o.y);
+        o.z = fmaf(qr[u], s[u].z, o.z), o.w = fmaf(qr[u], s[u].w, o.w);
+      }
+    }
   }
-  store_f32(o + at * dv + j, scale * sum);
+#pragma unroll
+  for (int m = LV; m < 32; m *= 2) {
+    o.x += __shfl_xor_sync(0xffffffffu, o.x, m), o.y += __shfl_xor_sync(0xffffffffu, o.y, m);
+    o.z += __shfl_xor_sync(0xffffffffu, o.z, m), o.w += __shfl_xor_sync(0xffffffffu, o.w, m);
+  }
+  if constexpr (WARPS > 1) {
+    sums[threadIdx.x] = o;
+    __syncthreads();
+    if (part == 0) {
+#pragma unroll
+      for (int w = 1; w < WARPS; ++w) {
+        const float4 t = sums[threadIdx.x + 32 * w];
+        o.x += t.x, o.y += t.y, o.z += t.z, o.w += t.w;
+      }
+    }
+  }
+  if (has && part == 0 && lane < LV) {
+    T* out = static_cast<T*>(p.o) + static_cast<int64_t>(at) * p.dv + col;
+    store_f32(out, p.scale * o.x), store_f32(out + 1, p.scale * o.y), store_f32(out + 2, p.scale * o.z), store_f32(out + 3, p.scale * o.w);
+  }
+}
+
+// The same for states whose rows are no whole 16-byte pieces: a block per sequence and head, a thread per column
+template <typename T>
+__global__ void __launch_bounds__(kThreads) step_columns_kernel(const __grid_constant__ Step p) {
+  const uint32_t at = blockIdx.x, b = at / p.H;
+  const int h = static_cast<int>(at - b * p.H), j = threadIdx.x;
+  if (j >= p.dv) return;
+  const T* q = static_cast<const T*>(p.q) + b * p.qb + h * p.qh;
+  const T* k = static_cast<const T*>(p.k) + b * p.kb + h * p.kh;
+  const float a = expf(p.log_decay[h]), c = load_f32(static_cast<const T*>(p.v) + b * p.vb + h * p.vh + j);
+  float sum = 0.0f;
+#pragma unroll 4
+  for (int i = 0; i < p.dk; ++i) {
+    const int64_t e = (static_cast<int64_t>(at) * p.dk + i) * p.dv + j;
+    const float s = fmaf(load_f32(k + i), c, a * p.state[e]);
+    p.new_state[e] = s;
+    sum = fmaf(load_f32(q + i), s, sum);
+  }
+  store_f32(static_cast<T*>(p.o) + static_cast<int64_t>(at) * p.dv + j, p.scale * sum);
 }
 
 int launched(const char* what) {
@@ -1199,16 +1276,25 @@ extern "C" int bpc_linear_attention_step(const void* q, const void* k, const voi
   if (at != to && at < to + bytes && to < at + bytes)
     return fail(BPC_ERR_ARG, "linear_attention_step: new_state overlaps state (give the same buffer to update it in place)");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const unsigned grid = static_cast<unsigned>(B * H);
-  if (dtype == BPC_DTYPE_F32)
-    step_kernel<float><<<grid, kThreads, 0, s>>>(static_cast<const float*>(q), static_cast<const float*>(k),
-                                                 static_cast<const float*>(v), static_cast<float*>(o), log_decay, state, new_state,
-                                                 H, dk, dv, strides[0], strides[1], strides[2], strides[3], strides[4], strides[5],
-                                                 scale);
-  else
-    step_kernel<__nv_bfloat16><<<grid, kThreads, 0, s>>>(
-        static_cast<const __nv_bfloat16*>(q), static_cast<const __nv_bfloat16*>(k), static_cast<const __nv_bfloat16*>(v),
-        static_cast<__nv_bfloat16*>(o), log_decay, state, new_state, H, dk, dv, strides[0], strides[1], strides[2], strides[3],
-        strides[4], strides[5], scale);
+  const Step p{q, k, v, o, log_decay, state, new_state, static_cast<uint32_t>(B * H), H, dk, dv,
+               strides[0], strides[1], strides[2], strides[3], strides[4], strides[5], scale};
+  with_type(dtype, [&](auto type) {
+    typedef typename decltype(type)::type T;
+    if (dv % 4 || !aligned(state, 16) || !aligned(new_state, 16)) {
+      step_columns_kernel<T><<<p.items, kThreads, 0, s>>>(p);
+      return 0;
+    }
+    // states of more than 4 KB by four warps: 64 x 64 and 128 x 128 have as much under way per state as 32 x 32
+    auto run = [&](auto lanes) {
+      constexpr int LV = decltype(lanes)::value;
+      if (dk * dv > 1024) step_kernel<T, LV, 4><<<p.items, kThreads, 0, s>>>(p);
+      else step_kernel<T, LV, 1><<<(p.items + 3) / 4, kThreads, 0, s>>>(p);
+    };
+    if (dv <= 16) run(std::integral_constant<int, 4>());
+    else if (dv <= 32) run(std::integral_constant<int, 8>());
+    else if (dv <= 64) run(std::integral_constant<int, 16>());
+    else run(std::integral_constant<int, 32>());
+    return 0;
+  });
   return launched(what);
 }
