@@ -47,14 +47,14 @@ struct Scan {
   const float* log_decay;
   const float* first;           // X before its decay: (B, H, da, dc), or (B, H, dc, da) where first_t
   float* last;                  // (B, H, da, dc), or null
-  float* parts;                 // the segments' states: (B H, segments - 1, DP DP) in the order of the warps' registers
+  float* parts;                 // the segments' states: (B H, segments - 1, da, dc)
   const void* lengths;
   int length_bytes;
   int T, H, da, dc;
   int segments, segment;        // rows per segment, a multiple of kChunk
   uint32_t items;               // B H segments
   float in_scale, out_scale;
-  bool reverse, first_t, vec, out_vec;
+  bool first_t, parts_t, vec, out_vec;      // _t: (dc, da)
 };
 
 __device__ __forceinline__ int length_of(const void* lengths, int bytes, uint32_t b, int T) {
@@ -77,14 +77,12 @@ __device__ __forceinline__ float power(float log2_a, int n) {
 // the row-major operand: then an accumulator is an operand of the next product as it stands, and a bf16 operand is one of
 // a tf32 product by taking its halves apart.
 __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -143,7 +141,7 @@ __device__ __forceinline__ void mma_f32(float (&d)[4], const Split (&a)[4], cons
 template <typename T, int DP>
 struct Tile {
   static constexpr bool kF32 = sizeof(T) == 4;
-  static constexpr int kCols = DP == 16 || DP == 128 ? 16 : 32;      // of c, per warp: a state of at most 64 values a lane
+  static constexpr int kCols = DP == 32 ? 32 : 16;                   // of c, per warp: a state of at most 64 values a lane
   static constexpr int kWarps = DP / kCols;                          // of a group, which takes an item
   static constexpr int kThreads = kWarps < 4 ? 128 : 32 * kWarps;
   static constexpr int kGroups = kThreads / 32 / kWarps;
@@ -154,9 +152,10 @@ struct Tile {
   static constexpr int kBytes = kChunk * kPitch;
   static constexpr int kPiece = 16 / sizeof(T);
   static constexpr int kPieces = DP / kPiece;                        // per row
-  static constexpr int kStages = kF32 ? 2 : 3;
+  static constexpr int kStages = kF32 || DP == 32 ? 2 : 3;
   static constexpr int kOutBytes = kF32 ? 0 : 16 * kCols * 2;        // a warp's rows on their way out
   static constexpr int kSmem = kGroups * kStages * 3 * kBytes + kGroups * kWarps * kOutBytes;
+  static constexpr int kBlocks = kWarps == 8 ? 1 : kSmem > 74 * 1024 || DP == 32 ? 2 : 3;      // per SM: registers and shared memory
   __device__ static __forceinline__ uint32_t at(int row, int piece) {
     if constexpr (kF32) return row * kPitch + piece * 16;
     else return row * kPitch + ((piece ^ (DP == 16 ? row >> 2 & 1 : DP == 32 ? row >> 1 & 3 : row & 7)) << 4);
@@ -176,13 +175,17 @@ __device__ __forceinline__ void cp_wait() {
 template <typename T, int DP>
 __device__ __forceinline__ void load_tile(uint32_t tile, const T* src, int64_t stride, int rows, int dim, bool vec, int lane) {
   using L = Tile<T, DP>;
-  constexpr int kLanes = 32 * L::kWarps;
+  constexpr int kLanes = 32 * L::kWarps, kPasses = kChunk * L::kPieces / kLanes, kStep = kLanes / L::kPieces;      // rows per pass
   if (vec) {
+    static_assert(kLanes % L::kPieces == 0, "a lane keeps its piece of a row");
+    const int row = lane / L::kPieces, piece = lane % L::kPieces;
+    const T* at = src + row * stride + piece * L::kPiece;
+    const bool inside = piece * L::kPiece < dim;
 #pragma unroll
-    for (int k = 0; k < kChunk * L::kPieces / kLanes; ++k) {
-      const int e = k * kLanes + lane, row = e / L::kPieces, piece = e % L::kPieces;
-      const bool there = row < rows && piece * L::kPiece < dim;
-      cp_async(tile + L::at(row, piece), there ? src + row * stride + piece * L::kPiece : src, there ? 16 : 0);
+    for (int k = 0; k < kPasses; ++k) {
+      const bool there = inside && row + k * kStep < rows;
+      cp_async(tile + L::at(row + k * kStep, piece), there ? at : src, there ? 16 : 0);
+      at += kStep * stride;
     }
   } else {
     for (int e = lane; e < kChunk * DP; e += kLanes) {
@@ -200,67 +203,81 @@ __device__ __forceinline__ void load_tile(uint32_t tile, const T* src, int64_t s
 // the chunk has more than 16 rows).  A lane's weights: of pairs of positions whose 8-row pieces are D = 0 .. 3 apart in
 // the scan's order (columns 2 t, 2 t + 1 of them); of the state for rows g, g + 8 of a half; of c's rows 2 t, 2 t + 1, 2 t + 8,
 // 2 t + 9 of a half in the state's update; of the state there.
+template <bool REV>
 struct Weights {
   float pair[4][2], row[2][2], update[2][4], keep;
+  bool in_order[2];             // D = 0: the columns 2 t, 2 t + 1 that do not come after the row
   int halves, flip;             // flip: half 0 is rows 16 - 31
 
   // r: the chunk's rows; until: the position as of which the state is wanted, r or (as of the last one) r - 1
-  __device__ __forceinline__ void of_pairs(float log2_a, float in, bool reverse) {
+  __device__ __forceinline__ void of_pairs(float log2_a, float in) {
     const int lane = threadIdx.x & 31, e0 = (lane >> 2) - 2 * (lane & 3);
 #pragma unroll
     for (int D = 0; D < 4; ++D)
 #pragma unroll
-      for (int z = 0; z < 2; ++z) pair[D][z] = in * power(log2_a, 8 * D + (reverse ? z - e0 : e0 - z));
+      for (int z = 0; z < 2; ++z) pair[D][z] = in * power(log2_a, 8 * D + (REV ? z - e0 : e0 - z));
+#pragma unroll
+    for (int z = 0; z < 2; ++z) in_order[z] = (REV ? z - e0 : e0 - z) >= 0;
   }
-  __device__ __forceinline__ void of_rows(float log2_a, float in, bool reverse, int r, int until) {
+  __device__ __forceinline__ void of_rows(float log2_a, float in, int r, int until) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     halves = r > 16 ? 2 : 1;
-    flip = reverse && halves == 2;
+    flip = REV && halves == 2;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int row0 = (flip ? 1 - h : h) * 16;
 #pragma unroll
-      for (int k = 0; k < 2; ++k) row[h][k] = power(log2_a, reverse ? r - 1 - (row0 + g + 8 * k) : row0 + g + 8 * k);
+      for (int k = 0; k < 2; ++k) row[h][k] = power(log2_a, REV ? r - 1 - (row0 + g + 8 * k) : row0 + g + 8 * k);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int j = row0 + 2 * t + (k & 1) + (k >> 1) * 8;
-        update[h][k] = in * power(log2_a, until - (reverse ? r - 1 - j : j));
+        update[h][k] = in * power(log2_a, until - (REV ? r - 1 - j : j));
       }
     }
     keep = power(log2_a, until);
   }
-  __device__ __forceinline__ float of(int i_half, int j_half, int i, int j, int z, bool reverse) const {
-    const int D = 2 * (i_half - j_half) + (reverse ? j - i : i - j);
-    return D < 0 ? 0.0f : pair[D][z];
+  // the product of a pair in 8-row pieces i and j of their halves, column z: weighed, and dropped (not multiplied by zero)
+  // where j comes after i
+  __device__ __forceinline__ float weigh(float p, int i_half, int j_half, int i, int j, int z) const {
+    const int D = 2 * (i_half - j_half) + (REV ? j - i : i - j);
+    return D < 0 || (D == 0 && !in_order[z]) ? 0.0f : p * pair[D < 0 ? 0 : D][z];
   }
 };
 
-template <typename T, int DP>
+template <typename T, int DP, bool REV>
 struct Warp {
   using L = Tile<T, DP>;
   static constexpr int kMT = L::kMT, kNT = L::kNT;
   float X[kMT][kNT][4];         // X^T: rows = this warp's columns of c, columns = those of a, b
 
   // O (16 positions x this warp's columns of c, for each half), and X after the chunk.  SPLIT: bf16 parts of the weighted c.
+  // FULL: more than 16 rows, a state and an update, as nearly all chunks of long sequences; their many branches cost as much
+  // again as the products.
   template <bool OUT, int SPLIT>
-  __device__ __forceinline__ void chunk(uint32_t sa, uint32_t sb, uint32_t sc, int slice, const Weights& w, bool reverse,
-                                        bool use_x, bool update, float (&O)[2][2 * kMT][4]) {
-    if constexpr (L::kF32) chunk_f32<OUT>(sa, sb, sc, slice, w, reverse, use_x, update, O);
-    else chunk_bf16<OUT, SPLIT>(sa, sb, sc, slice, w, reverse, use_x, update, O);
+  __device__ __forceinline__ void chunk(uint32_t sa, uint32_t sb, uint32_t sc, int slice, const Weights<REV>& w, bool use_x,
+                                        bool update, float (&O)[2][2 * kMT][4]) {
+    if (w.halves == 2 && use_x && update) chunk_of<true, OUT, SPLIT>(sa, sb, sc, slice, w, true, true, O);
+    else chunk_of<false, OUT, SPLIT>(sa, sb, sc, slice, w, use_x, update, O);
+  }
+  template <bool FULL, bool OUT, int SPLIT>
+  __device__ __forceinline__ void chunk_of(uint32_t sa, uint32_t sb, uint32_t sc, int slice, const Weights<REV>& w, bool use_x,
+                                           bool update, float (&O)[2][2 * kMT][4]) {
+    if constexpr (L::kF32) chunk_f32<FULL, OUT>(sa, sb, sc, slice, w, use_x, update, O);
+    else chunk_bf16<FULL, OUT, SPLIT>(sa, sb, sc, slice, w, use_x, update, O);
   }
 
   // What is fp32 and an operand of a bf16 product (the weighted a b^T, X, the weighted c) goes in as two bf16 parts, off by
   // at most 2^-18 of itself; one part would round as coarsely as the result.  Where a state is handed out, c as three.
-  template <bool OUT, int SPLIT>
-  __device__ __forceinline__ void chunk_bf16(uint32_t sa, uint32_t sb, uint32_t sc, int slice, const Weights& w, bool reverse,
-                                             bool use_x, bool update, float (&O)[2][2 * kMT][4]) {
+  template <bool FULL, bool OUT, int SPLIT>
+  __device__ __forceinline__ void chunk_bf16(uint32_t sa, uint32_t sb, uint32_t sc, int slice, const Weights<REV>& w, bool use_x,
+                                             bool update, float (&O)[2][2 * kMT][4]) {
     constexpr int kKS = DP / 16;
     const int lane = threadIdx.x & 31;
     // addresses of a lane's row in four 8 x 8 pieces: row lane % 16 and column piece lane / 16, or (b as the second
     // operand of a b^T) row lane % 8 + 8 (lane / 16) and column piece lane / 8 % 2; the next 16 columns are an XOR by 32
     const uint32_t by_row = L::at(lane & 15, lane >> 4), by_piece = L::at((lane & 7) + (lane >> 4) * 8, lane >> 3 & 1);
     const uint32_t half[2] = {w.flip ? 16u * L::kPitch : 0u, w.flip ? 0u : 16u * L::kPitch};
-    const bool two = w.halves == 2;
+    const bool two = FULL || w.halves == 2;
     uint32_t c[2][kMT][4];
     {
       const uint32_t c0 = L::at(lane & 15, slice * (L::kCols / 8) + (lane >> 4));
@@ -292,7 +309,7 @@ struct Warp {
           mma_bf16(P[2][0], a[1], b[0], b[1]);
           mma_bf16(P[2][1], a[1], b[2], b[3]);
         }
-        if (use_x) {
+        if (FULL || use_x) {
 #pragma unroll
           for (int n = 0; n < 2 * kMT; ++n) {
             uint32_t hi[2], lo[2];
@@ -311,7 +328,7 @@ struct Warp {
           }
         }
       }
-      if (use_x) weigh_rows(w, O);
+      if (FULL || use_x) weigh_rows(w, O);
 #pragma unroll
       for (int block = 0; block < 3; ++block) {
         const int i_half = block > 0, j_half = block > 1;
@@ -320,8 +337,8 @@ struct Warp {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {            // (rows g, columns of piece 0), (g + 8, 0), (g, 1), (g + 8, 1)
             const int r = e & 1, n = e >> 1;
-            const float p0 = weighed(P[block][n][2 * r], w.of(i_half, j_half, r, n, 0, reverse));
-            const float p1 = weighed(P[block][n][2 * r + 1], w.of(i_half, j_half, r, n, 1, reverse));
+            const float p0 = w.weigh(P[block][n][2 * r], i_half, j_half, r, n, 0);
+            const float p1 = w.weigh(P[block][n][2 * r + 1], i_half, j_half, r, n, 1);
             hi[e] = pack(p0, p1);
             lo[e] = pack(p0 - low(hi[e]), p1 - high(hi[e]));
           }
@@ -334,7 +351,7 @@ struct Warp {
         }
       }
     }
-    if (update) {
+    if (FULL || update) {
       uint32_t wc[2][SPLIT][kMT][4];
 #pragma unroll
       for (int h = 0; h < 2; ++h)
@@ -375,10 +392,7 @@ struct Warp {
     }
   }
 
-  // a pair out of order is dropped, not multiplied by zero
-  __device__ static __forceinline__ float weighed(float p, float w) { return w == 0.0f ? 0.0f : p * w; }
-
-  __device__ static __forceinline__ void weigh_rows(const Weights& w, float (&O)[2][2 * kMT][4]) {
+  __device__ static __forceinline__ void weigh_rows(const Weights<REV>& w, float (&O)[2][2 * kMT][4]) {
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -387,12 +401,12 @@ struct Warp {
         for (int e = 0; e < 4; ++e) O[h][n][e] *= w.row[h][e >> 1];
   }
 
-  template <bool OUT>
-  __device__ __forceinline__ void chunk_f32(uint32_t sa, uint32_t sb, uint32_t sc, int slice, const Weights& w, bool reverse,
-                                            bool use_x, bool update, float (&O)[2][2 * kMT][4]) {
+  template <bool FULL, bool OUT>
+  __device__ __forceinline__ void chunk_f32(uint32_t sa, uint32_t sb, uint32_t sc, int slice, const Weights<REV>& w, bool use_x,
+                                            bool update, float (&O)[2][2 * kMT][4]) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const uint32_t half[2] = {w.flip ? 16u * L::kPitch : 0u, w.flip ? 0u : 16u * L::kPitch};
-    const bool two = w.halves == 2;
+    const bool two = FULL || w.halves == 2;
     const uint32_t pair_at = g * L::kPitch + t * 8;              // (row g, columns 2 t, 2 t + 1)
     const uint32_t cross_at = 2 * t * L::kPitch + g * 4;         // (rows 2 t and the next, column g)
     const uint32_t c0 = sc + cross_at + slice * (L::kCols * 4);
@@ -416,14 +430,14 @@ struct Warp {
                 const float2 b = lds2(sb + half[j] + pair_at + n * 8 * L::kPitch + k * 32);
                 mma_f32(P[h + j][n], a, Split(b.x), Split(b.y));
               }
-            if (use_x) {
+            if (FULL || use_x) {
 #pragma unroll
               for (int n = 0; n < 2 * kMT; ++n)
                 mma_f32(O[h][n], a, Split(X[n / 2][k][2 * (n % 2)]), Split(X[n / 2][k][2 * (n % 2) + 1]));
             }
           }
       }
-      if (use_x) weigh_rows(w, O);
+      if (FULL || use_x) weigh_rows(w, O);
 #pragma unroll
       for (int block = 0; block < 3; ++block) {
         const int i_half = block > 0, j_half = block > 1;
@@ -433,7 +447,7 @@ struct Warp {
             Split p[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e)            // (g, 2 t), (g + 8, 2 t), (g, 2 t + 1), (g + 8, 2 t + 1)
-              p[e] = Split(weighed(P[block][k][2 * (e & 1) + (e >> 1)], w.of(i_half, j_half, e & 1, k, e >> 1, reverse)));
+              p[e] = Split(w.weigh(P[block][k][2 * (e & 1) + (e >> 1)], i_half, j_half, e & 1, k, e >> 1));
             const uint32_t at = c0 + half[j_half] + k * 8 * L::kPitch;
 #pragma unroll
             for (int n = 0; n < 2 * kMT; ++n)
@@ -442,7 +456,7 @@ struct Warp {
         }
       }
     }
-    if (update) {
+    if (FULL || update) {
 #pragma unroll
       for (int m = 0; m < kMT; ++m) {
         float u[kNT][4] = {};
@@ -469,7 +483,7 @@ struct Warp {
     }
   }
 
-  // f(value of X at (row of c's columns, column of a's), index) over a lane's values
+  // f(value of X, column of a, column of c) over a lane's values
   template <typename F>
   __device__ __forceinline__ void each(int slice, F f) {
     const int lane = threadIdx.x & 31;
@@ -479,7 +493,7 @@ struct Warp {
       for (int n = 0; n < kNT; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          f(X[m][n][e], n * 8 + 2 * (lane & 3) + (e & 1), slice * L::kCols + m * 16 + (lane >> 2) + (e >> 1) * 8, (m * kNT + n) * 4 + e);
+          f(X[m][n][e], n * 8 + 2 * (lane & 3) + (e & 1), slice * L::kCols + m * 16 + (lane >> 2) + (e >> 1) * 8);
   }
 };
 
@@ -500,7 +514,6 @@ struct Item {
     rows = left < 0 ? 0 : left > p.segment ? p.segment : left;
     steps = rows ? (rows + kChunk - 1) / kChunk : 1;
   }
-  __device__ __forceinline__ int chunk(bool reverse, int step) const { return reverse ? steps - 1 - step : step; }
   __device__ __forceinline__ int valid(int c) const { return rows - c * kChunk < kChunk ? rows - c * kChunk : kChunk; }
 };
 
@@ -571,15 +584,15 @@ __device__ __forceinline__ void zero_rows(T* out, int64_t stride, int slice, int
 }
 
 // A group of warps takes an item at a time, chunk by chunk, each warp some columns of c; the state stays in the warps'
-// registers.  The tiles of the next chunks, of the next items too, are on their way meanwhile.
+// registers.  The tiles of the next chunks, of the next items too, are on their way meanwhile.  REV: backwards in time.
 // OUT false: the states that the segments leave behind alone.
-template <typename T, int DP, bool OUT, int SPLIT>
-__global__ void __launch_bounds__(Tile<T, DP>::kThreads) scan_kernel(const __grid_constant__ Scan p) {
+template <typename T, int DP, bool REV, bool OUT, int SPLIT>
+__global__ void __launch_bounds__(Tile<T, DP>::kThreads, Tile<T, DP>::kBlocks) scan_kernel(const __grid_constant__ Scan p) {
   using L = Tile<T, DP>;
   extern __shared__ __align__(128) uint8_t smem[];
   constexpr int kS = L::kStages;
   const int warp = threadIdx.x >> 5, group = warp / L::kWarps, slice = warp % L::kWarps;
-  const int lane_in_group = threadIdx.x - group * (32 * L::kWarps), lane = threadIdx.x & 31;
+  const int lane_in_group = threadIdx.x - group * (32 * L::kWarps);
   const uint32_t base = smem_u32(smem) + group * (kS * 3 * L::kBytes);
   const uint32_t stage_out = smem_u32(smem) + L::kGroups * (kS * 3 * L::kBytes) + warp * L::kOutBytes;
   const uint32_t first_item = blockIdx.x * L::kGroups + group, stride = gridDim.x * L::kGroups;
@@ -588,77 +601,83 @@ __global__ void __launch_bounds__(Tile<T, DP>::kThreads) scan_kernel(const __gri
     else asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(32 * L::kWarps) : "memory");
   };
 
-  uint32_t ahead_at = first_item;                  // the loads' item and step
-  int ahead_step = 0, ahead_slot = 0;
-  Item ahead(p, ahead_at < p.items ? ahead_at : 0);
+  // the loads' item, its chunk's rows and its steps left
+  uint32_t ahead_at = first_item, ahead_tile = base;
+  const T *ahead_a = nullptr, *ahead_b = nullptr, *ahead_c = nullptr;
+  int ahead_left = 0, ahead_r = 0;
+  const int64_t by = REV ? -kChunk : kChunk;
+  auto start = [&] {
+    const Item it(p, ahead_at);
+    ahead_left = it.steps;
+    const int c = REV ? it.steps - 1 : 0, row = it.row0 + c * kChunk;
+    ahead_r = it.rows - (REV ? c * kChunk : 0);      // backwards the first chunk may be short, forwards the last
+    ahead_a = row_of<T>(p.a, it, row), ahead_b = row_of<T>(p.b, it, row), ahead_c = row_of<T>(p.c, it, row);
+  };
+  if (ahead_at < p.items) start();
   auto load = [&] {
     if (ahead_at < p.items) {
-      const int c = ahead.chunk(p.reverse, ahead_step), row = ahead.row0 + c * kChunk, r = ahead.valid(c);
-      const uint32_t tile = base + ahead_slot * (3 * L::kBytes);
-      if constexpr (OUT) load_tile<T, DP>(tile, row_of<T>(p.a, ahead, row), p.a.t, r, p.da, p.vec, lane_in_group);
-      load_tile<T, DP>(tile + L::kBytes, row_of<T>(p.b, ahead, row), p.b.t, r, p.da, p.vec, lane_in_group);
-      load_tile<T, DP>(tile + 2 * L::kBytes, row_of<T>(p.c, ahead, row), p.c.t, r, p.dc, p.vec, lane_in_group);
-      if (++ahead_step == ahead.steps) {
-        ahead_step = 0;
+      const int r = min(ahead_r, kChunk);
+      if constexpr (OUT) load_tile<T, DP>(ahead_tile, ahead_a, p.a.t, r, p.da, p.vec, lane_in_group);
+      load_tile<T, DP>(ahead_tile + L::kBytes, ahead_b, p.b.t, r, p.da, p.vec, lane_in_group);
+      load_tile<T, DP>(ahead_tile + 2 * L::kBytes, ahead_c, p.c.t, r, p.dc, p.vec, lane_in_group);
+      ahead_a += by * p.a.t, ahead_b += by * p.b.t, ahead_c += by * p.c.t;
+      ahead_r = REV ? kChunk : ahead_r - kChunk;
+      if (--ahead_left == 0) {
         ahead_at += stride;
-        if (ahead_at < p.items) ahead = Item(p, ahead_at);
+        if (ahead_at < p.items) start();
       }
     }
-    ahead_slot = ahead_slot + 1 == kS ? 0 : ahead_slot + 1;
+    ahead_tile = ahead_tile == base + (kS - 1) * (3 * L::kBytes) ? base : ahead_tile + 3 * L::kBytes;
     cp_commit();
   };
 #pragma unroll
   for (int s = 0; s < kS - 1; ++s) load();
 
-  Warp<T, DP> state;
-  int slot = 0;
+  Warp<T, DP, REV> state;
+  uint32_t tile = base;
   for (uint32_t at = first_item; at < p.items; at += stride) {
     const Item it(p, at);
     const int64_t bh = static_cast<int64_t>(it.b) * p.H + it.h;
     const float log2_a = log2_decay(p.log_decay, it.h);
     // where the scan enters and leaves the sequence
     const int end_segment = (it.n ? it.n - 1 : 0) / p.segment;
-    const bool enters = it.segment == (p.reverse ? end_segment : 0), leaves = it.segment == (p.reverse ? 0 : end_segment);
+    const bool enters = it.segment == (REV ? end_segment : 0), leaves = it.segment == (REV ? 0 : end_segment);
     const bool beyond = it.segment > end_segment;
-    bool use_x = false;
-    if (enters && p.first) {
-      const float lead = p.reverse || it.n == 0 ? 1.0f : power(log2_a, 1);
-      const float* f = p.first + bh * p.da * p.dc;
-      state.each(slice, [&](float& x, int i, int j, int) {
-        x = i < p.da && j < p.dc ? lead * f[p.first_t ? j * p.da + i : i * p.dc + j] : 0.0f;
-      });
-      use_x = true;
-    } else if (OUT && !enters && !beyond) {
-      const int s = p.reverse ? it.segment : it.segment - 1;
-      const float* f = p.parts + (bh * (p.segments - 1) + s) * (DP * DP) + slice * (L::kRegs * 32) + lane;
-      state.each(slice, [&](float& x, int, int, int k) { x = f[k * 32]; });
-      use_x = true;
-    } else {
-      state.each(slice, [&](float& x, int, int, int) { x = 0.0f; });
+    const float* f = nullptr;                      // what X starts from
+    float lead = 1.0f;
+    bool turned = p.first_t;
+    if (enters) {
+      if (p.first) f = p.first + bh * p.da * p.dc;
+      if (!REV && it.n) lead = power(log2_a, 1);
+    } else if (OUT && !beyond) {
+      f = p.parts + (bh * (p.segments - 1) + (REV ? it.segment : it.segment - 1)) * (p.da * p.dc);
+      turned = p.parts_t;
     }
+    state.each(slice, [&](float& x, int i, int j) {
+      x = f && i < p.da && j < p.dc ? lead * f[turned ? j * p.da + i : i * p.dc + j] : 0.0f;
+    });
+    bool use_x = f != nullptr;
     const bool keeps = OUT ? leaves && p.last : true;
-    Weights w;
-    if constexpr (OUT) w.of_pairs(log2_a, p.in_scale, p.reverse);
+    Weights<REV> w;
+    if constexpr (OUT) w.of_pairs(log2_a, p.in_scale);
     int weights_r = -1, weights_until = -1;
     const int64_t out_stride = static_cast<int64_t>(p.H) * p.dc;
     T* out = static_cast<T*>(p.out) + (static_cast<int64_t>(it.b) * p.T * p.H + it.h) * p.dc;
     for (int step = 0; step < it.steps; ++step) {
-      const int c = it.chunk(p.reverse, step), row = it.row0 + c * kChunk, r = it.valid(c);
+      const int c = REV ? it.steps - 1 - step : step, row = it.row0 + c * kChunk, r = it.valid(c);
       const bool final = step + 1 == it.steps;
       // forwards the state that is handed out is as of the last position, without the decay into the next
-      const int until = OUT && final && keeps && !p.reverse ? (r ? r - 1 : 0) : r;
+      const int until = OUT && !REV && final && keeps ? (r ? r - 1 : 0) : r;
       if (r != weights_r || until != weights_until) {
-        w.of_rows(log2_a, p.in_scale, p.reverse, r, until);
+        w.of_rows(log2_a, p.in_scale, r, until);
         weights_r = r, weights_until = until;
       }
       cp_wait<kS - 2>();
       sync();
       load();
-      const uint32_t tile = base + slot * (3 * L::kBytes);
-      slot = slot + 1 == kS ? 0 : slot + 1;
       float O[2][2 * L::kMT][4];
-      state.template chunk<OUT, SPLIT>(tile, tile + L::kBytes, tile + 2 * L::kBytes, slice, w, p.reverse, use_x,
-                                       !final || keeps, O);
+      state.template chunk<OUT, SPLIT>(tile, tile + L::kBytes, tile + 2 * L::kBytes, slice, w, use_x, !final || keeps, O);
+      tile = tile == base + (kS - 1) * (3 * L::kBytes) ? base : tile + 3 * L::kBytes;
       if constexpr (OUT) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -674,44 +693,46 @@ __global__ void __launch_bounds__(Tile<T, DP>::kThreads) scan_kernel(const __gri
     if constexpr (OUT) {
       zero_rows<T, DP>(out, out_stride, slice, it.row0 + it.steps * kChunk, min(p.T, it.row0 + p.segment), p.dc);
       if (keeps) {
-        float* f = p.last + bh * p.da * p.dc;
-        state.each(slice, [&](float& x, int i, int j, int) {
-          if (i < p.da && j < p.dc) f[i * p.dc + j] = x;
+        float* to = p.last + bh * p.da * p.dc;
+        state.each(slice, [&](float& x, int i, int j) {
+          if (i < p.da && j < p.dc) to[i * p.dc + j] = x;
         });
       }
-    } else if (it.segment != (p.reverse ? 0 : p.segments - 1)) {
-      const int s = p.reverse ? it.segment - 1 : it.segment;
-      float* f = p.parts + (bh * (p.segments - 1) + s) * (DP * DP) + slice * (L::kRegs * 32) + lane;
-      state.each(slice, [&](float& x, int, int, int k) { f[k * 32] = x; });
+    } else if (it.segment != (REV ? 0 : p.segments - 1)) {
+      float* to = p.parts + (bh * (p.segments - 1) + (REV ? it.segment - 1 : it.segment)) * (p.da * p.dc);
+      state.each(slice, [&](float& x, int i, int j) {
+        if (i < p.da && j < p.dc) to[i * p.dc + j] = x;
+      });
     }
   }
 }
 
 // The states that the segments leave behind, alone, become those that their next ones start from: a thread per value of
 // a state, along the segments.
-template <int DP>
-__global__ void __launch_bounds__(256) join_kernel(const Scan p) {
-  const int per = DP * DP / 256;
+template <bool REV>
+__global__ void __launch_bounds__(256) join_kernel(const Scan p, int per) {      // blocks per state
   const uint32_t bh = blockIdx.x / per;
-  const int b = bh / p.H, n = length_of(p.lengths, p.length_bytes, b, p.T);
+  const int b = bh / p.H, n = length_of(p.lengths, p.length_bytes, b, p.T), D = p.da * p.dc;
+  const int e = blockIdx.x % per * 256 + threadIdx.x;
+  if (e >= D) return;
   const float log2_a = log2_decay(p.log_decay, bh - b * p.H);
-  float* f = p.parts + static_cast<int64_t>(bh) * (p.segments - 1) * (DP * DP) + blockIdx.x % per * 256 + threadIdx.x;
+  float* f = p.parts + static_cast<int64_t>(bh) * (p.segments - 1) * D + e;
   float x = 0.0f;
-  constexpr int kAhead = 8;
+  constexpr int kAhead = 32;
   for (int s0 = 0; s0 < p.segments - 1; s0 += kAhead) {
     float v[kAhead];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      const int s = p.reverse ? p.segments - 2 - s0 - u : s0 + u;
-      v[u] = s0 + u < p.segments - 1 ? f[static_cast<int64_t>(s) * (DP * DP)] : 0.0f;
+      const int s = REV ? p.segments - 2 - s0 - u : s0 + u;
+      v[u] = s0 + u < p.segments - 1 ? f[static_cast<int64_t>(s) * D] : 0.0f;
     }
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       if (s0 + u < p.segments - 1) {
-        const int s = p.reverse ? p.segments - 2 - s0 - u : s0 + u;
-        const int left = n - (p.reverse ? s + 1 : s) * p.segment;
+        const int s = REV ? p.segments - 2 - s0 - u : s0 + u;
+        const int left = n - (REV ? s + 1 : s) * p.segment;
         x = fmaf(power(log2_a, left < 0 ? 0 : left > p.segment ? p.segment : left), x, v[u]);
-        f[static_cast<int64_t>(s) * (DP * DP)] = x;
+        f[static_cast<int64_t>(s) * D] = x;
       }
     }
   }
@@ -778,7 +799,7 @@ struct Piece {
 
 __device__ __forceinline__ uint32_t transpose(uint32_t piece) {      // an 8 x 8 piece of 16-bit elements
   uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(piece));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(piece));
   return r;
 }
 
@@ -1038,50 +1059,40 @@ int padded(int dim) {
   return with_dim(dim, [](auto d) { return decltype(d)::value; });
 }
 
-// Blocks of scan_kernel that are resident per SM
-template <typename T, int DP, bool OUT, int SPLIT>
-int scan_blocks(int* blocks) {
-  const void* fn = reinterpret_cast<const void*>(&scan_kernel<T, DP, OUT, SPLIT>);
-  constexpr int smem = Tile<T, DP>::kSmem;
-  if (int e = allow_smem(fn, smem)) return e;
-  static int resident = 0;      // the same on every device that this library runs on
-  if (!resident) {
-    int n = 0;
-    const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, fn, Tile<T, DP>::kThreads, smem);
-    if (e != cudaSuccess || n < 1) return fail(BPC_ERR_LAUNCH, std::string("linear_attention occupancy: ") + cudaGetErrorString(e));
-    resident = n;
-  }
-  *blocks = resident;
-  return 0;
+// Groups of scan_kernel's warps that are resident
+int64_t resident_groups(int dim, int size) {
+  return static_cast<int64_t>(num_sms()) * with_dim(dim, [&](auto d) {
+    constexpr int DP = decltype(d)::value;
+    return size == 4 ? Tile<float, DP>::kBlocks * Tile<float, DP>::kGroups : Tile<__nv_bfloat16, DP>::kBlocks * Tile<__nv_bfloat16, DP>::kGroups;
+  });
 }
 
-template <typename T, int DP, bool OUT, int SPLIT>
+template <typename T, int DP, bool REV, bool OUT, int SPLIT>
 int launch_scan(const Scan& p, cudaStream_t s) {
-  int blocks = 0;
-  if (int e = scan_blocks<T, DP, OUT, SPLIT>(&blocks)) return e;
   using L = Tile<T, DP>;
-  constexpr int groups = L::kGroups;
-  const unsigned grid = std::min<unsigned>((p.items + groups - 1) / groups, blocks * num_sms());
-  scan_kernel<T, DP, OUT, SPLIT><<<grid, L::kThreads, L::kSmem, s>>>(p);
+  const void* fn = reinterpret_cast<const void*>(&scan_kernel<T, DP, REV, OUT, SPLIT>);
+  if (int e = allow_smem(fn, L::kSmem)) return e;
+  const unsigned grid = std::min<unsigned>((p.items + L::kGroups - 1) / L::kGroups, L::kBlocks * num_sms());
+  scan_kernel<T, DP, REV, OUT, SPLIT><<<grid, L::kThreads, L::kSmem, s>>>(p);
   return launched("linear_attention");
 }
 
-// Into how many segments a sequence is cut: one where the heads alone keep the GPU busy
-int segments_of(int64_t BH, int64_t T, int dim) {
-  const int64_t groups = static_cast<int64_t>(num_sms()) * 8 / std::max(1, padded(dim) / 32);
-  if (BH >= groups || T <= 512) return 1;
-  return static_cast<int>(std::max<int64_t>(1, std::min((groups + BH - 1) / BH, T / 256)));
+// Into how many segments a sequence is cut: one where the heads alone keep the GPU busy, else as many as fill it once, of 256
+// rows at least
+int segments_of(int64_t BH, int64_t T, int dim, int size) {
+  return static_cast<int>(std::max<int64_t>(1, std::min(resident_groups(dim, size) / std::max<int64_t>(1, BH), T / 256)));
 }
 
-int64_t parts_bytes(int64_t BH, int64_t T, int dim) {
-  const int64_t D = padded(dim);
-  return BH * (segments_of(BH, T, dim) - 1) * D * D * static_cast<int64_t>(sizeof(float));
+int64_t parts_bytes(int64_t BH, int64_t T, int da, int dc, int size) {
+  return BH * (segments_of(BH, T, std::max(da, dc), size) - 1) * da * dc * static_cast<int64_t>(sizeof(float));
 }
 
-int run_scan(Scan p, int64_t B, int32_t dtype, float* workspace, cudaStream_t s) {
+// have_parts: the workspace holds the segments' states already, those of the same scan or of the one with b and c exchanged
+template <bool REV>
+int run_scan(Scan p, int64_t B, int32_t dtype, float* workspace, bool have_parts, cudaStream_t s) {
   const int dim = std::max(p.da, p.dc);
   const int64_t BH = B * p.H;
-  const int want = segments_of(BH, p.T, dim);
+  const int want = segments_of(BH, p.T, dim, size_of(dtype));
   p.segment = std::max(kChunk, ((p.T + want - 1) / want + kChunk - 1) / kChunk * kChunk);
   p.segments = std::max(1, (p.T + p.segment - 1) / p.segment);
   p.items = static_cast<uint32_t>(BH * p.segments);
@@ -1092,12 +1103,13 @@ int run_scan(Scan p, int64_t B, int32_t dtype, float* workspace, cudaStream_t s)
       constexpr int DP = decltype(d)::value;
       // the state handed out is fp32: it needs every bit of the weighted rows; a bf16 result alone does with 16
       constexpr int kFew = sizeof(T) == 4 ? 3 : 2;
-      if (p.segments > 1) {
-        if (int e = p.last ? launch_scan<T, DP, false, 3>(p, s) : launch_scan<T, DP, false, kFew>(p, s)) return e;
-        join_kernel<DP><<<static_cast<unsigned>(BH * (DP * DP / 256)), 256, 0, s>>>(p);
+      if (p.segments > 1 && !have_parts) {
+        if (int e = p.last ? launch_scan<T, DP, REV, false, 3>(p, s) : launch_scan<T, DP, REV, false, kFew>(p, s)) return e;
+        const int per = (p.da * p.dc + 255) / 256;
+        join_kernel<REV><<<static_cast<unsigned>(BH * per), 256, 0, s>>>(p, per);
         if (int e = launched("linear_attention")) return e;
       }
-      return p.last ? launch_scan<T, DP, true, 3>(p, s) : launch_scan<T, DP, true, kFew>(p, s);
+      return p.last ? launch_scan<T, DP, REV, true, 3>(p, s) : launch_scan<T, DP, REV, true, kFew>(p, s);
     });
   });
 }
@@ -1147,8 +1159,7 @@ bool copies_whole(const Rows& r, int dim, int size) {
 }
 
 Scan make_scan(const Rows& a, const Rows& b, const Rows& c, void* out, const float* log_decay, const float* first, bool first_t,
-               float* last, const void* lengths, int length_bytes, int64_t T, int H, int da, int dc, float in, float scale,
-               bool reverse, int size) {
+               float* last, const void* lengths, int length_bytes, int64_t T, int H, int da, int dc, float in, float scale, int size) {
   Scan p = {};
   p.a = a, p.b = b, p.c = c;
   p.out = out;
@@ -1156,7 +1167,7 @@ Scan make_scan(const Rows& a, const Rows& b, const Rows& c, void* out, const flo
   p.first = first, p.first_t = first_t, p.last = last;
   p.lengths = lengths, p.length_bytes = length_bytes;
   p.T = static_cast<int>(T), p.H = H, p.da = da, p.dc = dc;
-  p.in_scale = in, p.out_scale = scale, p.reverse = reverse;
+  p.in_scale = in, p.out_scale = scale;
   p.vec = T > 0 && copies_whole(a, da, size) && copies_whole(b, da, size) && copies_whole(c, dc, size);
   p.out_vec = aligned(out, 16) && dc * size % (size == 4 ? 8 : 16) == 0;
   return p;
@@ -1191,7 +1202,7 @@ using namespace bpc;
 extern "C" size_t bpc_linear_attention_workspace_size(int64_t B, int64_t T, int32_t H, int32_t dk, int32_t dv,
                                                       int32_t dtype, int32_t backward) {
   if (B < 1 || T < 0 || H < 1 || dk < 1 || dk > kMaxDim || dv < 1 || dv > kMaxDim || !size_of(dtype)) return 0;
-  return static_cast<size_t>(std::max<int64_t>(16, parts_bytes(B * H, T, std::max(dk, dv))));
+  return static_cast<size_t>(std::max<int64_t>(16, parts_bytes(B * H, T, dk, dv, size_of(dtype))));
 }
 
 extern "C" int bpc_linear_attention_fwd(const void* q, const void* k, const void* v, void* o, const float* log_decay,
@@ -1217,8 +1228,8 @@ extern "C" int bpc_linear_attention_fwd(const void* q, const void* k, const void
     return run_short<false>(p, dtype, reinterpret_cast<cudaStream_t>(stream));
   }
   const Scan p = make_scan(rq, rk, rv, o, log_decay, state, false,
-                           new_state, lengths, length_bytes, T, H, dk, dv, 1.0f, scale, false, size);
-  return run_scan(p, B, dtype, static_cast<float*>(workspace), reinterpret_cast<cudaStream_t>(stream));
+                           new_state, lengths, length_bytes, T, H, dk, dv, 1.0f, scale, size);
+  return run_scan<false>(p, B, dtype, static_cast<float*>(workspace), false, reinterpret_cast<cudaStream_t>(stream));
 }
 
 extern "C" int bpc_linear_attention_bwd(const void* q, const void* k, const void* v, const void* go, const float* log_decay,
@@ -1249,16 +1260,16 @@ extern "C" int bpc_linear_attention_bwd(const void* q, const void* k, const void
   }
   float* ws = static_cast<float*>(workspace);
   if (T) {
-    const Scan pq = make_scan(rg, rv, rk, dq, log_decay, state, true, nullptr, lengths, length_bytes, T, H, dv, dk, 1.0f, scale,
-                              false, size);
-    if (int e = run_scan(pq, B, dtype, ws, s)) return e;
-    const Scan pk = make_scan(rv, rg, rq, dk_out, log_decay, grad_state, true, nullptr, lengths, length_bytes, T, H, dv, dk,
-                              scale, 1.0f, true, size);
-    if (int e = run_scan(pk, B, dtype, ws, s)) return e;
+    const Scan pq = make_scan(rg, rv, rk, dq, log_decay, state, true, nullptr, lengths, length_bytes, T, H, dv, dk, 1.0f, scale, size);
+    if (int e = run_scan<false>(pq, B, dtype, ws, false, s)) return e;
   }
-  const Scan pv = make_scan(rk, rq, rg, dv_out, log_decay, grad_state, false, dstate, lengths, length_bytes, T, H, dk, dv, scale,
-                            1.0f, true, size);
-  return run_scan(pv, B, dtype, ws, s);
+  const Scan pv = make_scan(rk, rq, rg, dv_out, log_decay, grad_state, false, dstate, lengths, length_bytes, T, H, dk, dv, scale, 1.0f, size);
+  if (int e = run_scan<true>(pv, B, dtype, ws, false, s)) return e;
+  if (!T) return 0;
+  // the same states the other way round
+  Scan pk = make_scan(rv, rg, rq, dk_out, log_decay, grad_state, true, nullptr, lengths, length_bytes, T, H, dv, dk, scale, 1.0f, size);
+  pk.parts_t = true;
+  return run_scan<true>(pk, B, dtype, ws, true, s);
 }
 
 extern "C" int bpc_linear_attention_step(const void* q, const void* k, const void* v, void* o, const float* log_decay,
