@@ -6,6 +6,10 @@ BipartiteConv(C, geo, impl) keeps the reference's constructor, parameter names (
 target type), registered tables (c2d{k}, inv_c2d{k}, d2c{k}, inv_d2c{k}) and forward (cascade_net.py:213-233).  It
 takes the reference's Geometry (BB codes, K = 12) or geometry.RotatedSurface (K = 8).
 
+GroupNorm is the per-shot normalisation with an activation that CascadeBlock and CascadeNet take in BatchNorm's place
+(norm="group"); RoundMemory carries information over the rounds of an experiment (train.PreDecoderNet(memory=heads)).  Both
+are on the library's kernels: GPU only.
+
 PreDecoder(geo, cfg, params) runs the whole rotated-surface pre-decoder (params.py) in one C-ABI call per batch:
 forward(det) -> (logits (B, N_d, 2) fp32, residual (B, N_c) uint8).
 """
@@ -20,7 +24,7 @@ import torch.nn.functional as F
 from torch import nn
 
 from . import _lib
-from .ops import gather_mm, residual_affine_silu
+from .ops import gather_mm, group_norm, linear_attention, linear_attention_step, residual_affine_silu
 
 
 class BipartiteConv(nn.Module):
@@ -235,6 +239,74 @@ def _fold_bn(bn: nn.BatchNorm1d):
     return scale, bn.bias.float() - bn.running_mean.float() * scale
 
 
+class GroupNorm(nn.Module):
+    """ops.group_norm as a module: weight and bias (C) over channels-last features (B, ..., C), statistics per sample and
+    group.  Under autocast the result has the autocast type (the layer behind it would cast it), statistics stay fp32."""
+
+    def __init__(self, C, groups, activation="none", eps=1e-5):
+        super().__init__()
+        if groups < 1 or C % groups:
+            raise ValueError(f"{C} channels do not divide into {groups} groups")
+        self.groups, self.activation, self.eps = groups, activation, eps
+        self.weight = nn.Parameter(torch.ones(C))
+        self.bias = nn.Parameter(torch.zeros(C))
+
+    def forward(self, x):
+        dtype = None
+        if x.dtype == torch.float32 and x.is_cuda and torch.is_autocast_enabled("cuda"):
+            dtype = torch.get_autocast_dtype("cuda")
+        return group_norm(x, self.groups, self.weight, self.bias, self.eps, self.activation, dtype)
+
+
+class RoundMemory(nn.Module):
+    """A memory over the rounds of an experiment: x (B, T, S, C) features of T rounds at S sites -> x + out(y) with
+        q, k, v = linear maps of x, `heads` heads of C / heads per site
+        S_t = a S_(t-1) + k_t v_t^T,  o_t = q_t S_t / sqrt(C / heads)      per site and head, over the rounds
+        y = SiLU(group norm of o, a group per head)
+    The heads forget at fixed rates, from half to 2^-6 of their memory a round.  `out` starts at zero: the layer is the
+    identity until it is trained.  forward takes whole experiments (lengths (B): rounds that each shot has, default all;
+    positions behind are passed through), step one round, going on from the state that forward returns or start() makes.
+    No reference counterpart: the reference's networks see a fixed window of rounds."""
+
+    def __init__(self, C, heads, sites, seed=0):
+        super().__init__()
+        if heads < 1 or C % heads or C // heads > 128:
+            raise ValueError(f"{C} channels do not divide into {heads} heads of at most 128")
+        self.C, self.heads, self.sites, self.D = C, heads, sites, C // heads
+        g = torch.Generator().manual_seed(seed)
+        for name in ("q", "k", "v"):
+            setattr(self, name, nn.Parameter((torch.rand(C, C, generator=g) * 2 - 1) / math.sqrt(C)))
+        self.out = nn.Parameter(torch.zeros(C, C))
+        self.norm = GroupNorm(C, heads, "silu")
+        decay = torch.log1p(-torch.exp2(-torch.linspace(1.0, 6.0, heads, dtype=torch.float64))).float()
+        self.register_buffer("log_decay", decay.repeat(sites), persistent=False)         # (sites, heads)
+
+    def _project(self, x, *lead):
+        return (F.linear(x, w).view(*lead, self.sites * self.heads, self.D) for w in (self.q, self.k, self.v))
+
+    def start(self, B):
+        """The state before the first round."""
+        return torch.zeros(B, self.sites * self.heads, self.D, self.D, device=self.log_decay.device)
+
+    def forward(self, x, lengths=None, state=None, return_state=False):
+        B, T = x.shape[:2]
+        q, k, v = self._project(x, B, T)
+        o = linear_attention(q, k, v, self.log_decay, state=state, lengths=lengths, return_state=return_state)
+        o, new_state = o if return_state else (o, None)
+        u = F.linear(self.norm(o.reshape(B * T * self.sites, self.C)), self.out).view(x.shape)
+        if lengths is not None:                 # the norm of nothing is its bias: rounds that are not there add nothing
+            there = torch.arange(T, device=x.device) < lengths[:, None]
+            u = torch.where(there[:, :, None, None], u, torch.zeros((), device=u.device, dtype=u.dtype))
+        return (x + u, new_state) if return_state else x + u
+
+    @torch.no_grad()
+    def step(self, x, state):
+        """One round: x (B, S, C); the state is updated in place."""
+        B = x.shape[0]
+        o = linear_attention_step(*self._project(x, B), self.log_decay, state)
+        return x + F.linear(self.norm(o.reshape(B * self.sites, self.C)), self.out).view(x.shape)
+
+
 class CascadeBlock(nn.Module):
     """The reference's bottleneck residual block (cascade_net.py:236-259) on the B200 op, with its parameter names
     (bn1, bn2, bn3, down, conv, up) so its state_dicts load unchanged:
@@ -246,12 +318,21 @@ class CascadeBlock(nn.Module):
         BN1 + SiLU: one elementwise pass;  down + BN2 + SiLU: the op with K = 1 (identity table) and the affine + SiLU
         epilogue;  conv: two launches, each covering both target types (stacked relation matrices, the targets are
         type-major);  BN3 + SiLU: the epilogue of the second;  up and the residual: one bf16 GEMM and one fp32 add.
-    The bottleneck activations are bf16 (the reference's bf16 autocast), the residual stream keeps h's dtype."""
+    The bottleneck activations are bf16 (the reference's bf16 autocast), the residual stream keeps h's dtype.
+    norm="group": a GroupNorm + SiLU of `groups` groups in place of each BatchNorm + SiLU (gn1, gn2, gn3; GPU only), whose
+    statistics are a shot's own: training and eval compute the same, and a shot's result does not depend on its batch.  It
+    runs the composition in both modes."""
 
-    def __init__(self, H, geo, L, res="branch", impl="b200"):
+    def __init__(self, H, geo, L, res="branch", impl="b200", norm="batch", groups=32):
         super().__init__()
         Hb = H // 4
-        self.bn1, self.bn2, self.bn3 = nn.BatchNorm1d(H), nn.BatchNorm1d(Hb), nn.BatchNorm1d(Hb)
+        if norm not in ("batch", "group"):
+            raise ValueError(f'norm must be "batch" or "group", got {norm!r}')
+        self.norm = norm
+        if norm == "batch":
+            self.bn1, self.bn2, self.bn3 = nn.BatchNorm1d(H), nn.BatchNorm1d(Hb), nn.BatchNorm1d(Hb)
+        else:
+            self.gn1, self.gn2, self.gn3 = (GroupNorm(c, groups, "silu") for c in (H, Hb, Hb))
         self.down = nn.Linear(H, Hb, bias=False)
         self.conv = BipartiteConv(Hb, geo, impl)
         self.up = nn.Linear(Hb, H, bias=False)
@@ -272,6 +353,8 @@ class CascadeBlock(nn.Module):
         return mod(x.reshape(-1, C)).view(x.shape)
 
     def branch(self, h):
+        if self.norm == "group":
+            return self.up(self.gn3(self.conv(self.gn2(self.down(self.gn1(h))))))
         u = self.down(F.silu(self._bn(self.bn1, h)))
         u = self.conv(F.silu(self._bn(self.bn2, u)))
         return self.up(F.silu(self._bn(self.bn3, u)))
@@ -313,7 +396,7 @@ class CascadeBlock(nn.Module):
         return residual_affine_silu(h, u, sh, su, a_n, b_n)
 
     def forward(self, h):
-        if not self.training and h.is_cuda and h.dtype == torch.float32:
+        if self.norm == "batch" and not self.training and h.is_cuda and h.dtype == torch.float32:
             if self._cache is None or self._cache["a1"].device != h.device:
                 self.prepare_inference()
             return self._fused(h)[0]
@@ -332,7 +415,7 @@ class CascadeStack(nn.Module):
         self.blocks = nn.ModuleList(blocks)
 
     def forward(self, h):
-        if self.training or not h.is_cuda or h.dtype != torch.float32:
+        if self.training or not h.is_cuda or h.dtype != torch.float32 or any(b.norm != "batch" for b in self.blocks):
             for b in self.blocks:
                 h = b(h)
             return h
@@ -436,9 +519,12 @@ class CascadeNet(nn.Module):
 
     embedding: the stem's lookup embedding(tokens, weight) wherever the embedded stream is written (training, CPU, blocks
     of other sizes); None: the `embed` module itself.  ops.embedding runs it and its weight gradient on the library's
-    kernels (GPU only): the same values, a gradient that repeats bit for bit."""
+    kernels (GPU only): the same values, a gradient that repeats bit for bit.
+    norm="group": GroupNorm + SiLU in place of every BatchNorm + SiLU (CascadeBlock; gn_out before the read-out), GPU only;
+    eval then runs the composition of training."""
 
-    def __init__(self, geo, H, L, det_t, det_typ, det_site, logicals, res="branch", embedding=None):
+    def __init__(self, geo, H, L, det_t, det_typ, det_site, logicals, res="branch", embedding=None, norm="batch",
+                 groups=32):
         super().__init__()
         self.embedding = embedding
         if H % 4:
@@ -457,8 +543,12 @@ class CascadeNet(nn.Module):
         self.register_buffer("gidx", torch.as_tensor(gidx), persistent=False)
         self.register_buffer("tbase", torch.as_tensor(tbase), persistent=False)
         self.embed = nn.Embedding(5, H)
-        self.blocks = nn.ModuleList([CascadeBlock(H, geo, L, res) for _ in range(L)])
-        self.bn_out = nn.BatchNorm1d(H)
+        self.blocks = nn.ModuleList([CascadeBlock(H, geo, L, res, norm=norm, groups=groups) for _ in range(L)])
+        self.norm = norm
+        if norm == "batch":
+            self.bn_out = nn.BatchNorm1d(H)
+        else:
+            self.gn_out = GroupNorm(H, groups, "silu")
         logicals = np.asarray(logicals, np.int64)
         self.k = k = len(logicals)
         self.support = [np.flatnonzero(r) for r in logicals]      # each observable's data qubits, d n2 + s
@@ -495,10 +585,12 @@ class CascadeNet(nn.Module):
         return self.mlp2(F.silu(self.mlp1(z))).squeeze(-1)
 
     def forward(self, det: torch.Tensor) -> torch.Tensor:
-        if self.training or not det.is_cuda:
+        if self.training or not det.is_cuda or self.norm == "group":
             h = self._embedded(det)
             for b in self.blocks:
                 h = b(h)
+            if self.norm == "group":
+                return self.readout(self.gn_out(h))
             return self.readout(F.silu(self.bn_out(h.reshape(-1, self.H)).view(h.shape)))
         if CascadeStack.boundary_path(self.blocks):
             # the stem's embedding is computed by the first block's kernels, never written

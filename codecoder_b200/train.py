@@ -24,6 +24,7 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
+from .modules import RoundMemory
 from .ops import bipartite_step, embed_tokens, gather_mm, head_bce, target_table
 from .params import N_TOKENS
 
@@ -32,10 +33,11 @@ class PreDecoderNet(nn.Module):
     """geo: geometry.RotatedSurface; cfg: params.PreDecoderConfig; params: optional init_params-style dict (fp32
     numpy) to start from, else a seeded init with the same bounds.  `gmm` is the bipartite-conv op with the
     reference's signature gmm(x, w, idx, inv) (default: the B200 op); `embedding` the lookup embedding(ids, weight) of the
-    unfused network (ops.embedding: on the library's kernels, GPU only)."""
+    unfused network (ops.embedding: on the library's kernels, GPU only); `memory` a number of heads: a modules.RoundMemory over
+    the rounds of the data stream in front of the head (GPU only; None: no memory, and the network of params.py)."""
 
     def __init__(self, geo, cfg, params: dict | None = None, gmm=gather_mm, seed: int = 0, fused: bool = True,
-                 embedding=F.embedding):
+                 embedding=F.embedding, memory: int | None = None):
         super().__init__()
         self.fused = fused
         self.embedding = embedding
@@ -72,6 +74,8 @@ class PreDecoderNet(nn.Module):
         self._fused_ok = (geo.d2c[0].shape[0] == geo.d2c[1].shape[0] and
                           np.array_equal(np.concatenate([np.flatnonzero(geo.check_type == 0),
                                                          np.flatnonzero(geo.check_type == 1)]), np.arange(geo.N_c)))
+        self.rounds = geo.R
+        self.memory = None if memory is None else RoundMemory(C, memory, geo.n_data_round, seed)
         # the logits read h_d after the last check -> data step: the last data -> check step does not reach the
         # loss, so its weights take no gradient (kept for the inference weight set)
         for c in range(2):
@@ -101,7 +105,14 @@ class PreDecoderNet(nn.Module):
             a = torch.cat([self.gmm(hd, self.w_d2c[2 * l + c], getattr(self, f"d2c{c}"), getattr(self, f"inv_d2c{c}"))
                            for c in range(2)], 1)
             hc = hc + F.gelu(a, approximate="tanh")
-        return F.linear(hd, self.head_w, self.head_b)
+        return F.linear(self._remembered(hd), self.head_w, self.head_b)
+
+    def _remembered(self, hd: torch.Tensor) -> torch.Tensor:
+        """h_d (B, N_d, C) through the memory: data nodes are round-major."""
+        if self.memory is None:
+            return hd
+        B, N, C = hd.shape
+        return self.memory(hd.view(B, self.rounds, N // self.rounds, C)).view(B, N, C)
 
     def _forward_fused(self, det: torch.Tensor, labels: torch.Tensor | None = None) -> torch.Tensor:
         """The same network under bf16 autocast through ops.bipartite_step: each step is the op's forward kernels
@@ -117,6 +128,7 @@ class PreDecoderNet(nn.Module):
             if l == self.cfg.layers - 1:
                 break
             hc, hc16 = bipartite_step(hd, hc, d2c, self.w_d2c[2 * l], self.w_d2c[2 * l + 1], carry=(carry, None, l))
+        hd = self._remembered(hd)
         if labels is not None and self.cfg.channels <= 128:
             # head and loss in one pass each way, the logits never materialised (ops.HeadBCEB200)
             return head_bce(hd, self.head_w, self.head_b, labels)
