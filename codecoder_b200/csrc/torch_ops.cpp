@@ -1,6 +1,6 @@
-// Host side of the embedding, gradient-norm, group-norm and linear-attention operators: argument checks, outputs, workspaces and the calls of
-// libbpc.so's C entry points, as a Python module on torch tensors.  In C++ because these calls are short: reading a
-// list of 176 gradients through Python costs about 0.4 us per tensor, more than the kernels take; here 0.02 us.
+// Host side of the embedding, gradient-norm, group-norm and linear-attention operators: argument checks, outputs, workspaces
+// and the calls of libbpc.so's C entry points, as a Python module on torch tensors.  In C++ because these calls are short:
+// reading a list of 176 gradients through Python costs about 0.4 us per tensor, more than the kernels take; here 0.02 us.
 // The module does not link to libbpc.so: _lib.py hands it the entry points of the library it loaded.
 #include <cstdint>
 #include <string>
@@ -8,6 +8,8 @@
 
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/utils/pybind.h>
 #include <torch/extension.h>
 
@@ -488,6 +490,97 @@ Tensor linear_attention_step(const Tensor& q_in, const Tensor& k_in, const Tenso
   return o;
 }
 
+// ---- autograd: in C++ too, a forward and backward pass of small tensors through Python costs some 40 us more ----------------
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// Gradients that are not differentiable themselves: where a graph of them is asked for, its use is an error
+variable_list once(variable_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
+  variable_list in;
+  for (const Tensor& t : grads) in.push_back(t.defined() ? t.detach().set_requires_grad(true) : t);
+  const auto error = std::make_shared<torch::autograd::DelayedError>(
+      "trying to differentiate twice a function that is differentiable once", static_cast<int64_t>(in.size()));
+  return (*error)(std::move(in));
+}
+
+bool wants_grad(const Tensor& t) { return t.requires_grad(); }
+bool wants_grad(const std::optional<Tensor>& t) { return t && t->requires_grad(); }
+
+std::optional<Tensor> if_defined(const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
+
+struct GroupNorm : torch::autograd::Function<GroupNorm> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, int64_t groups, const std::optional<Tensor>& weight,
+                        const std::optional<Tensor>& bias, double eps, int64_t activation, std::optional<at::ScalarType> dtype) {
+    auto [y, stats] = group_norm_fwd(x, groups, weight, bias, eps, activation, dtype, true);
+    ctx->save_for_backward({x, stats, weight.value_or(Tensor()), bias.value_or(Tensor())});
+    ctx->saved_data["groups"] = groups;
+    ctx->saved_data["activation"] = activation;
+    ctx->set_materialize_grads(false);
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list gy) {
+    variable_list out(7);
+    if (!gy[0].defined()) return out;
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor &weight = saved[2], &bias = saved[3];
+    size_t at = 0;                       // edges are counted over the tensors that were given
+    const bool dx = ctx->needs_input_grad(at++), dw = weight.defined() && ctx->needs_input_grad(at++);
+    const bool db = bias.defined() && ctx->needs_input_grad(at++);
+    auto [gx, gw, gb] = group_norm_bwd(gy[0], saved[0], saved[1], ctx->saved_data["groups"].toInt(), if_defined(weight),
+                                       if_defined(bias), ctx->saved_data["activation"].toInt(), dx, dw, db);
+    const variable_list g = once({gx, dw ? gw.to(weight.scalar_type()) : gw, db ? gb.to(bias.scalar_type()) : gb});
+    out[0] = g[0], out[2] = g[1], out[3] = g[2];
+    return out;
+  }
+};
+
+Tensor group_norm(const Tensor& x, int64_t groups, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias,
+                  double eps, int64_t activation, std::optional<at::ScalarType> dtype) {
+  if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(weight) || wants_grad(bias)))
+    return GroupNorm::apply(x, groups, weight, bias, eps, activation, dtype);
+  return std::get<0>(group_norm_fwd(x, groups, weight, bias, eps, activation, dtype, false));
+}
+
+struct LinearAttention : torch::autograd::Function<LinearAttention> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay,
+                               double scale, const std::optional<Tensor>& state, const std::optional<Tensor>& lengths,
+                               bool want_state) {
+    auto [o, new_state] = linear_attention_fwd(q, k, v, log_decay, scale, state, lengths, want_state);
+    ctx->save_for_backward({q, k, v, log_decay, state.value_or(Tensor()), lengths.value_or(Tensor())});
+    ctx->saved_data["scale"] = scale;
+    ctx->set_materialize_grads(false);
+    return want_state ? variable_list{o, new_state} : variable_list{o};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    variable_list out(8);
+    const Tensor grad_state = g.size() > 1 ? g[1] : Tensor();
+    if (!g[0].defined() && !grad_state.defined()) return out;
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &state = saved[4];
+    const Tensor go = g[0].defined() ? g[0] : at::zeros_like(v);
+    auto [dq, dk, dv, dstate] = linear_attention_bwd(q, k, v, go, saved[3], ctx->saved_data["scale"].toDouble(), if_defined(state),
+                                                     if_defined(grad_state), if_defined(saved[5]),
+                                                     state.defined() && ctx->needs_input_grad(4));
+    const variable_list grads = once({dq, dk, dv, dstate});
+    for (int i = 0; i < 3; ++i) out[i] = grads[i];
+    out[5] = grads[3];
+    return out;
+  }
+};
+
+// o, and with want_state the state after each sequence's last position
+std::tuple<Tensor, Tensor> linear_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, double scale,
+                                            const std::optional<Tensor>& state, const std::optional<Tensor>& lengths,
+                                            bool want_state) {
+  if (at::GradMode::is_enabled() && (wants_grad(q) || wants_grad(k) || wants_grad(v) || wants_grad(state))) {
+    const variable_list r = LinearAttention::apply(q, k, v, log_decay, scale, state, lengths, want_state);
+    return {r[0], want_state ? r[1] : Tensor()};
+  }
+  return linear_attention_fwd(q, k, v, log_decay, scale, state, lengths, want_state);
+}
+
 }  // namespace
 
 // What the build reads back, to compile again for another torch or Python, and to refuse loading there until then
@@ -498,10 +591,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   const auto release = py::call_guard<py::gil_scoped_release>();
   m.def("embed_lookup", &embed_lookup, release);
   m.def("embed_wgrad", &embed_wgrad, release);
-  m.def("group_norm_fwd", &group_norm_fwd, release);
-  m.def("group_norm_bwd", &group_norm_bwd, release);
-  m.def("linear_attention_fwd", &linear_attention_fwd, release);
-  m.def("linear_attention_bwd", &linear_attention_bwd, release);
+  m.def("group_norm", &group_norm, release);
+  m.def("linear_attention", &linear_attention, release);
   m.def("linear_attention_step", &linear_attention_step, release);
   m.def("grad_norm", &grad_norm);
   m.def("clip_grads", &clip_grads);

@@ -599,28 +599,6 @@ def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
 ACTIVATIONS = {"none": _lib.BPC_ACT_NONE, "silu": _lib.BPC_ACT_SILU, "gelu": _lib.BPC_ACT_GELU}
 
 
-class GroupNormB200(torch.autograd.Function):
-    """group_norm with its gradients (C ABI bpc_group_norm_fwd / _bwd); differentiable once."""
-
-    @staticmethod
-    def forward(ctx, x, groups, weight, bias, eps, act, dtype):
-        y, stats = _lib.torch_ops().group_norm_fwd(x, groups, weight, bias, eps, act, dtype, True)
-        ctx.save_for_backward(x, stats, weight, bias)
-        ctx.set_materialize_grads(False)
-        ctx.groups, ctx.act = groups, act
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, gy):
-        if gy is None:
-            return (None,) * 7
-        x, stats, weight, bias = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        dx, dw, db = _lib.torch_ops().group_norm_bwd(gy, x, stats, ctx.groups, weight, bias, ctx.act, need[0], need[2], need[3])
-        return (dx, None, dw.to(weight.dtype) if need[2] else None, db.to(bias.dtype) if need[3] else None, None, None, None)
-
-
 def group_norm(x: torch.Tensor, groups: int, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
                eps: float = 1e-5, activation: str = "none", dtype: torch.dtype | None = None) -> torch.Tensor:
     """act(weight (x - mean) / sqrt(var + eps) + bias) over channels-last features (C ABI bpc_group_norm_fwd / _bwd):
@@ -630,34 +608,7 @@ def group_norm(x: torch.Tensor, groups: int, weight: torch.Tensor | None = None,
     deterministic; differentiable once."""
     if activation not in ACTIVATIONS:
         raise ValueError(f"group_norm: activation must be one of {', '.join(ACTIVATIONS)}, got {activation!r}")
-    act = ACTIVATIONS[activation]
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
-        return GroupNormB200.apply(x, groups, weight, bias, eps, act, dtype)
-    return _lib.torch_ops().group_norm_fwd(x, groups, weight, bias, eps, act, dtype, False)[0]
-
-
-class LinearAttentionB200(torch.autograd.Function):
-    """linear_attention with its gradients (C ABI bpc_linear_attention_fwd / _bwd); differentiable once."""
-
-    @staticmethod
-    def forward(ctx, q, k, v, log_decay, scale, state, lengths, return_state):
-        o, new_state = _lib.torch_ops().linear_attention_fwd(q, k, v, log_decay, scale, state, lengths, return_state)
-        ctx.save_for_backward(q, k, v, log_decay, state, lengths)
-        ctx.set_materialize_grads(False)
-        ctx.scale = scale
-        return (o, new_state) if return_state else o
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, go, grad_state=None):
-        if go is None and grad_state is None:
-            return (None,) * 8
-        q, k, v, log_decay, state, lengths = ctx.saved_tensors
-        if go is None:
-            go = torch.zeros_like(v)
-        dq, dk, dv, dstate = _lib.torch_ops().linear_attention_bwd(q, k, v, go, log_decay, ctx.scale, state, grad_state,
-                                                                   lengths, ctx.needs_input_grad[5])
-        return dq, dk, dv, None, None, dstate, None, None
+    return _lib.torch_ops().group_norm(x, groups, weight, bias, eps, ACTIVATIONS[activation], dtype)
 
 
 def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, scale: float | None = None,
@@ -673,9 +624,7 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     if log_decay.requires_grad:
         raise ValueError("linear_attention: log_decay takes no gradient (detach it)")
     scale = q.shape[-1] ** -0.5 if scale is None else scale
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, state)):
-        return LinearAttentionB200.apply(q, k, v, log_decay, scale, state, lengths, return_state)
-    o, new_state = _lib.torch_ops().linear_attention_fwd(q, k, v, log_decay, scale, state, lengths, return_state)
+    o, new_state = _lib.torch_ops().linear_attention(q, k, v, log_decay, scale, state, lengths, return_state)
     return (o, new_state) if return_state else o
 
 
