@@ -57,6 +57,12 @@ struct Scan {
   bool first_t, parts_t, vec, out_vec;      // _t: (dc, da)
 };
 
+// One scan, or two in one launch (dk and dv): the items of the first, then those of the second
+struct Scans {
+  Scan s[2];
+  uint32_t each, total;
+};
+
 __device__ __forceinline__ int length_of(const void* lengths, int bytes, uint32_t b, int T) {
   if (!lengths) return T;
   const int64_t n = bytes == 8 ? static_cast<const int64_t*>(lengths)[b] : static_cast<const int32_t*>(lengths)[b];
@@ -587,7 +593,7 @@ __device__ __forceinline__ void zero_rows(T* out, int64_t stride, int slice, int
 // registers.  The tiles of the next chunks, of the next items too, are on their way meanwhile.  REV: backwards in time.
 // OUT false: the states that the segments leave behind alone.
 template <typename T, int DP, bool REV, bool OUT, int SPLIT>
-__global__ void __launch_bounds__(Tile<T, DP>::kThreads, Tile<T, DP>::kBlocks) scan_kernel(const __grid_constant__ Scan p) {
+__global__ void __launch_bounds__(Tile<T, DP>::kThreads, Tile<T, DP>::kBlocks) scan_kernel(const __grid_constant__ Scans all) {
   using L = Tile<T, DP>;
   extern __shared__ __align__(128) uint8_t smem[];
   constexpr int kS = L::kStages;
@@ -606,16 +612,22 @@ __global__ void __launch_bounds__(Tile<T, DP>::kThreads, Tile<T, DP>::kBlocks) s
   const T *ahead_a = nullptr, *ahead_b = nullptr, *ahead_c = nullptr;
   int ahead_left = 0, ahead_r = 0;
   const int64_t by = REV ? -kChunk : kChunk;
+  // two scans backwards only, as dk and dv: to ask which one it is costs the others a quarter (16,384 rounds 63 -> 80 us)
+  auto scan_of = [&](uint32_t at) { return &all.s[REV && OUT && at >= all.each ? 1 : 0]; };
+  const Scan* ahead_p = all.s;
   auto start = [&] {
-    const Item it(p, ahead_at);
+    ahead_p = scan_of(ahead_at);
+    const Scan& p = *ahead_p;
+    const Item it(p, ahead_at - (ahead_p == all.s ? 0 : all.each));
     ahead_left = it.steps;
     const int c = REV ? it.steps - 1 : 0, row = it.row0 + c * kChunk;
     ahead_r = it.rows - (REV ? c * kChunk : 0);      // backwards the first chunk may be short, forwards the last
     ahead_a = row_of<T>(p.a, it, row), ahead_b = row_of<T>(p.b, it, row), ahead_c = row_of<T>(p.c, it, row);
   };
-  if (ahead_at < p.items) start();
+  if (ahead_at < all.total) start();
   auto load = [&] {
-    if (ahead_at < p.items) {
+    if (ahead_at < all.total) {
+      const Scan& p = *ahead_p;
       const int r = min(ahead_r, kChunk);
       if constexpr (OUT) load_tile<T, DP>(ahead_tile, ahead_a, p.a.t, r, p.da, p.vec, lane_in_group);
       load_tile<T, DP>(ahead_tile + L::kBytes, ahead_b, p.b.t, r, p.da, p.vec, lane_in_group);
@@ -624,7 +636,7 @@ __global__ void __launch_bounds__(Tile<T, DP>::kThreads, Tile<T, DP>::kBlocks) s
       ahead_r = REV ? kChunk : ahead_r - kChunk;
       if (--ahead_left == 0) {
         ahead_at += stride;
-        if (ahead_at < p.items) start();
+        if (ahead_at < all.total) start();
       }
     }
     ahead_tile = ahead_tile == base + (kS - 1) * (3 * L::kBytes) ? base : ahead_tile + 3 * L::kBytes;
@@ -635,8 +647,9 @@ __global__ void __launch_bounds__(Tile<T, DP>::kThreads, Tile<T, DP>::kBlocks) s
 
   Warp<T, DP, REV> state;
   uint32_t tile = base;
-  for (uint32_t at = first_item; at < p.items; at += stride) {
-    const Item it(p, at);
+  for (uint32_t at = first_item; at < all.total; at += stride) {
+    const Scan& p = *scan_of(at);
+    const Item it(p, at - (&p == all.s ? 0 : all.each));
     const int64_t bh = static_cast<int64_t>(it.b) * p.H + it.h;
     const float log2_a = log2_decay(p.log_decay, it.h);
     // where the scan enters and leaves the sequence
@@ -1068,28 +1081,29 @@ int64_t resident_groups(int dim, int size) {
 }
 
 template <typename T, int DP, bool REV, bool OUT, int SPLIT>
-int launch_scan(const Scan& p, cudaStream_t s) {
+int launch_scan(const Scan& p, const Scan* second, cudaStream_t s) {
   using L = Tile<T, DP>;
   const void* fn = reinterpret_cast<const void*>(&scan_kernel<T, DP, REV, OUT, SPLIT>);
   if (int e = allow_smem(fn, L::kSmem)) return e;
-  const unsigned grid = std::min<unsigned>((p.items + L::kGroups - 1) / L::kGroups, L::kBlocks * num_sms());
-  scan_kernel<T, DP, REV, OUT, SPLIT><<<grid, L::kThreads, L::kSmem, s>>>(p);
+  const Scans all{{p, second ? *second : p}, p.items, second ? 2 * p.items : p.items};
+  const unsigned grid = std::min<unsigned>((all.total + L::kGroups - 1) / L::kGroups, L::kBlocks * num_sms());
+  scan_kernel<T, DP, REV, OUT, SPLIT><<<grid, L::kThreads, L::kSmem, s>>>(all);
   return launched("linear_attention");
 }
 
-// Into how many segments a sequence is cut: one where the heads alone keep the GPU busy, else as many as fill it once, of 256
-// rows at least
+// Into how many segments a sequence is cut: one where the heads alone keep the GPU busy, else as many as fill it once, of three
+// chunks at least: the states' pass before costs a third of a chunk's time each and two launches
 int segments_of(int64_t BH, int64_t T, int dim, int size) {
-  return static_cast<int>(std::max<int64_t>(1, std::min(resident_groups(dim, size) / std::max<int64_t>(1, BH), T / 256)));
+  return static_cast<int>(std::max<int64_t>(1, std::min(resident_groups(dim, size) / std::max<int64_t>(1, BH), T / (3 * kChunk))));
 }
 
 int64_t parts_bytes(int64_t BH, int64_t T, int da, int dc, int size) {
   return BH * (segments_of(BH, T, std::max(da, dc), size) - 1) * da * dc * static_cast<int64_t>(sizeof(float));
 }
 
-// have_parts: the workspace holds the segments' states already, those of the same scan or of the one with b and c exchanged
+// A scan, and `second` (or null) beside it: the one with b and c exchanged, which starts from the same states the other way round
 template <bool REV>
-int run_scan(Scan p, int64_t B, int32_t dtype, float* workspace, bool have_parts, cudaStream_t s) {
+int run_scan(Scan p, Scan* second, int64_t B, int32_t dtype, float* workspace, cudaStream_t s) {
   const int dim = std::max(p.da, p.dc);
   const int64_t BH = B * p.H;
   const int want = segments_of(BH, p.T, dim, size_of(dtype));
@@ -1097,19 +1111,23 @@ int run_scan(Scan p, int64_t B, int32_t dtype, float* workspace, bool have_parts
   p.segments = std::max(1, (p.T + p.segment - 1) / p.segment);
   p.items = static_cast<uint32_t>(BH * p.segments);
   p.parts = workspace;
+  if (second) {
+    second->segment = p.segment, second->segments = p.segments, second->items = p.items, second->parts = p.parts;
+    second->parts_t = true;
+  }
   return with_type(dtype, [&](auto type) {
     return with_dim(dim, [&](auto d) {
       typedef typename decltype(type)::type T;
       constexpr int DP = decltype(d)::value;
       // the state handed out is fp32: it needs every bit of the weighted rows; a bf16 result alone does with 16
       constexpr int kFew = sizeof(T) == 4 ? 3 : 2;
-      if (p.segments > 1 && !have_parts) {
-        if (int e = p.last ? launch_scan<T, DP, REV, false, 3>(p, s) : launch_scan<T, DP, REV, false, kFew>(p, s)) return e;
+      if (p.segments > 1) {
+        if (int e = p.last ? launch_scan<T, DP, REV, false, 3>(p, nullptr, s) : launch_scan<T, DP, REV, false, kFew>(p, nullptr, s)) return e;
         const int per = (p.da * p.dc + 255) / 256;
         join_kernel<REV><<<static_cast<unsigned>(BH * per), 256, 0, s>>>(p, per);
         if (int e = launched("linear_attention")) return e;
       }
-      return p.last ? launch_scan<T, DP, REV, true, 3>(p, s) : launch_scan<T, DP, REV, true, kFew>(p, s);
+      return p.last ? launch_scan<T, DP, REV, true, 3>(p, second, s) : launch_scan<T, DP, REV, true, kFew>(p, second, s);
     });
   });
 }
@@ -1229,7 +1247,7 @@ extern "C" int bpc_linear_attention_fwd(const void* q, const void* k, const void
   }
   const Scan p = make_scan(rq, rk, rv, o, log_decay, state, false,
                            new_state, lengths, length_bytes, T, H, dk, dv, 1.0f, scale, size);
-  return run_scan<false>(p, B, dtype, static_cast<float*>(workspace), false, reinterpret_cast<cudaStream_t>(stream));
+  return run_scan<false>(p, nullptr, B, dtype, static_cast<float*>(workspace), reinterpret_cast<cudaStream_t>(stream));
 }
 
 extern "C" int bpc_linear_attention_bwd(const void* q, const void* k, const void* v, const void* go, const float* log_decay,
@@ -1261,15 +1279,12 @@ extern "C" int bpc_linear_attention_bwd(const void* q, const void* k, const void
   float* ws = static_cast<float*>(workspace);
   if (T) {
     const Scan pq = make_scan(rg, rv, rk, dq, log_decay, state, true, nullptr, lengths, length_bytes, T, H, dv, dk, 1.0f, scale, size);
-    if (int e = run_scan<false>(pq, B, dtype, ws, false, s)) return e;
+    if (int e = run_scan<false>(pq, nullptr, B, dtype, ws, s)) return e;
   }
   const Scan pv = make_scan(rk, rq, rg, dv_out, log_decay, grad_state, false, dstate, lengths, length_bytes, T, H, dk, dv, scale, 1.0f, size);
-  if (int e = run_scan<true>(pv, B, dtype, ws, false, s)) return e;
-  if (!T) return 0;
-  // the same states the other way round
+  if (!T) return run_scan<true>(pv, nullptr, B, dtype, ws, s);
   Scan pk = make_scan(rv, rg, rq, dk_out, log_decay, grad_state, true, nullptr, lengths, length_bytes, T, H, dv, dk, scale, 1.0f, size);
-  pk.parts_t = true;
-  return run_scan<true>(pk, B, dtype, ws, true, s);
+  return run_scan<true>(pv, &pk, B, dtype, ws, s);
 }
 
 extern "C" int bpc_linear_attention_step(const void* q, const void* k, const void* v, void* o, const float* log_decay,
