@@ -71,8 +71,8 @@ SIGNATURES = {
     "bpc_linear_attention_workspace_size": (ctypes.c_size_t, [c_i64, c_i64, c_i32, c_i32, c_i32, c_i32, c_i32]),
     "bpc_linear_attention_fwd": (ctypes.c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i32, c_i64, c_i64, c_i32,
                                                 c_i32, c_i32, c_vp, ctypes.c_float, c_i32, c_vp, ctypes.c_size_t, c_vp]),
-    "bpc_linear_attention_bwd": (ctypes.c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i32, c_vp, c_vp, c_vp,
-                                                c_vp, c_i64, c_i64, c_i32, c_i32, c_i32, c_vp, ctypes.c_float, c_i32, c_vp,
+    "bpc_linear_attention_bwd": (ctypes.c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i32, c_vp, c_vp,
+                                                c_vp, c_vp, c_i64, c_i64, c_i32, c_i32, c_i32, c_vp, ctypes.c_float, c_i32, c_vp,
                                                 ctypes.c_size_t, c_vp]),
     "bpc_linear_attention_step": (ctypes.c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i32, c_i32, c_i32, c_vp,
                                                  ctypes.c_float, c_i32, c_vp]),

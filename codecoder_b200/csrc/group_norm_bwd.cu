@@ -336,22 +336,28 @@ __global__ void __launch_bounds__(kTileThreads, 2) tiles_kernel(const U* __restr
   }
 }
 
-// dw and db from the blocks' parts: a warp takes 32 neighbouring columns' parts w, w + 8, ..., the warps' sums join in order
-__global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ parts, int64_t n, int C, float* __restrict__ dw,
-                                                   float* __restrict__ db) {
-  __shared__ double sums[8][32];
+// dw and db from the blocks' parts: a warp takes 32 neighbouring columns' parts w, w + 32, ..., the warps' sums join in order
+__global__ void __launch_bounds__(1024) join_kernel(const float* __restrict__ parts, int64_t n, int C, float* __restrict__ dw,
+                                                    float* __restrict__ db) {
+  __shared__ double sums[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, column = blockIdx.x * 32 + lane;
   double sum = 0.0;
-  if (column < 2 * C)
-    for (int64_t k = warp; k < n; k += 8) sum += parts[k * 2 * C + column];
+  if (column < 2 * C) {
+#pragma unroll 8
+    for (int64_t k = warp; k < n; k += 32) sum += parts[k * 2 * C + column];
+  }
   sums[warp][lane] = sum;
   __syncthreads();
-  if (warp == 0 && column < 2 * C) {
-    for (int k = 1; k < 8; ++k) sum += sums[k][lane];
-    if (column < C) {
-      if (db) db[column] = static_cast<float>(sum);
+  // a warp per column
+  sum = sums[lane][warp];
+#pragma unroll
+  for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  const int mine = blockIdx.x * 32 + warp;
+  if (lane == 0 && mine < 2 * C) {
+    if (mine < C) {
+      if (db) db[mine] = static_cast<float>(sum);
     } else if (dw) {
-      dw[column - C] = static_cast<float>(sum);
+      dw[mine - C] = static_cast<float>(sum);
     }
   }
 }
@@ -572,6 +578,6 @@ extern "C" int bpc_group_norm_bwd(const void* gy, const void* x, const float* st
     });
   });
   if (e || !want) return e;
-  join_kernel<<<(2 * C + 31) / 32, 256, 0, st>>>(static_cast<const float*>(workspace), parts_of(s, p), C, dw, db);
+  join_kernel<<<(2 * C + 31) / 32, 1024, 0, st>>>(static_cast<const float*>(workspace), parts_of(s, p), C, dw, db);
   return launched(what);
 }

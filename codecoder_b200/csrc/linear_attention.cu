@@ -903,8 +903,12 @@ __device__ __forceinline__ Piece<T, DP> attend(const Piece<T, DP>& a, const Piec
   return out;
 }
 
+// Blocks per SM that the registers are cut for: bf16 backwards 342 us with 4, 363 with the 3 that it takes by itself
 template <typename T, int DP, bool BWD>
-__global__ void __launch_bounds__(kThreads) short_kernel(const __grid_constant__ Short p) {
+constexpr int kShortBlocks = sizeof(T) == 2 && DP <= 32 ? (BWD ? 4 : 6) : 1;
+
+template <typename T, int DP, bool BWD>
+__global__ void __launch_bounds__(kThreads, kShortBlocks<T, DP, BWD>) short_kernel(const __grid_constant__ Short p) {
   const uint32_t first = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5), stride = gridDim.x * (kThreads / 32);
   uint32_t b = first / p.H, h = first - b * p.H;
   Piece<T, DP> q, k, v, go;
@@ -1101,9 +1105,10 @@ int64_t parts_bytes(int64_t BH, int64_t T, int da, int dc, int size) {
   return BH * (segments_of(BH, T, std::max(da, dc), size) - 1) * da * dc * static_cast<int64_t>(sizeof(float));
 }
 
-// A scan, and `second` (or null) beside it: the one with b and c exchanged, which starts from the same states the other way round
+// A scan, and `second` (or null) beside it: the one with b and c exchanged, which starts from the same states the other way
+// round.  turned_parts: the segments' states of such a scan that has run before, or null.
 template <bool REV>
-int run_scan(Scan p, Scan* second, int64_t B, int32_t dtype, float* workspace, cudaStream_t s) {
+int run_scan(Scan p, Scan* second, int64_t B, int32_t dtype, float* workspace, const float* turned_parts, cudaStream_t s) {
   const int dim = std::max(p.da, p.dc);
   const int64_t BH = B * p.H;
   const int want = segments_of(BH, p.T, dim, size_of(dtype));
@@ -1111,6 +1116,7 @@ int run_scan(Scan p, Scan* second, int64_t B, int32_t dtype, float* workspace, c
   p.segments = std::max(1, (p.T + p.segment - 1) / p.segment);
   p.items = static_cast<uint32_t>(BH * p.segments);
   p.parts = workspace;
+  if (turned_parts) p.parts = const_cast<float*>(turned_parts), p.parts_t = true;
   if (second) {
     second->segment = p.segment, second->segments = p.segments, second->items = p.items, second->parts = p.parts;
     second->parts_t = true;
@@ -1121,7 +1127,7 @@ int run_scan(Scan p, Scan* second, int64_t B, int32_t dtype, float* workspace, c
       constexpr int DP = decltype(d)::value;
       // the state handed out is fp32: it needs every bit of the weighted rows; a bf16 result alone does with 16
       constexpr int kFew = sizeof(T) == 4 ? 3 : 2;
-      if (p.segments > 1) {
+      if (p.segments > 1 && !turned_parts) {
         if (int e = p.last ? launch_scan<T, DP, REV, false, 3>(p, nullptr, s) : launch_scan<T, DP, REV, false, kFew>(p, nullptr, s)) return e;
         const int per = (p.da * p.dc + 255) / 256;
         join_kernel<REV><<<static_cast<unsigned>(BH * per), 256, 0, s>>>(p, per);
@@ -1247,12 +1253,12 @@ extern "C" int bpc_linear_attention_fwd(const void* q, const void* k, const void
   }
   const Scan p = make_scan(rq, rk, rv, o, log_decay, state, false,
                            new_state, lengths, length_bytes, T, H, dk, dv, 1.0f, scale, size);
-  return run_scan<false>(p, nullptr, B, dtype, static_cast<float*>(workspace), reinterpret_cast<cudaStream_t>(stream));
+  return run_scan<false>(p, nullptr, B, dtype, static_cast<float*>(workspace), nullptr, reinterpret_cast<cudaStream_t>(stream));
 }
 
 extern "C" int bpc_linear_attention_bwd(const void* q, const void* k, const void* v, const void* go, const float* log_decay,
-                                        const float* state, const float* grad_state, const void* lengths,
-                                        int32_t length_bytes, void* dq, void* dk_out, void* dv_out, float* dstate, int64_t B,
+                                        const float* state, const float* grad_state, const void* fwd_workspace,
+                                        const void* lengths, int32_t length_bytes, void* dq, void* dk_out, void* dv_out, float* dstate, int64_t B,
                                         int64_t T, int32_t H, int32_t dk, int32_t dv, const int64_t* strides, float scale,
                                         int32_t dtype, void* workspace, size_t workspace_bytes, bpc_stream_t stream) {
   const char* what = "linear_attention backward";
@@ -1263,7 +1269,7 @@ extern "C" int bpc_linear_attention_bwd(const void* q, const void* k, const void
     return fail(BPC_ERR_ARG, "linear_attention backward: null buffer");
   for (const void* b : {q, k, v, go, static_cast<const void*>(dq), static_cast<const void*>(dk_out), static_cast<const void*>(dv_out)})
     if (!aligned(b, size)) return fail(BPC_ERR_ARG, "linear_attention backward: buffer not aligned to its type");
-  if (!aligned(state, 16) || !aligned(grad_state, 16) || !aligned(dstate, 16) || !aligned(workspace, 16))
+  if (!aligned(state, 16) || !aligned(grad_state, 16) || !aligned(dstate, 16) || !aligned(workspace, 16) || !aligned(fwd_workspace, 16))
     return fail(BPC_ERR_ARG, "linear_attention backward: buffer not aligned to its type (states and workspace: 16 bytes)");
   if (workspace_bytes < bpc_linear_attention_workspace_size(B, T, H, dk, dv, dtype, 1))
     return fail(BPC_ERR_SPACE, "linear_attention backward: workspace too small");
@@ -1279,12 +1285,12 @@ extern "C" int bpc_linear_attention_bwd(const void* q, const void* k, const void
   float* ws = static_cast<float*>(workspace);
   if (T) {
     const Scan pq = make_scan(rg, rv, rk, dq, log_decay, state, true, nullptr, lengths, length_bytes, T, H, dv, dk, 1.0f, scale, size);
-    if (int e = run_scan<false>(pq, nullptr, B, dtype, ws, s)) return e;
+    if (int e = run_scan<false>(pq, nullptr, B, dtype, ws, static_cast<const float*>(fwd_workspace), s)) return e;
   }
   const Scan pv = make_scan(rk, rq, rg, dv_out, log_decay, grad_state, false, dstate, lengths, length_bytes, T, H, dk, dv, scale, 1.0f, size);
-  if (!T) return run_scan<true>(pv, nullptr, B, dtype, ws, s);
+  if (!T) return run_scan<true>(pv, nullptr, B, dtype, ws, nullptr, s);
   Scan pk = make_scan(rv, rg, rq, dk_out, log_decay, grad_state, true, nullptr, lengths, length_bytes, T, H, dv, dk, scale, 1.0f, size);
-  return run_scan<true>(pv, &pk, B, dtype, ws, s);
+  return run_scan<true>(pv, &pk, B, dtype, ws, nullptr, s);
 }
 
 extern "C" int bpc_linear_attention_step(const void* q, const void* k, const void* v, void* o, const float* log_decay,

@@ -400,8 +400,8 @@ Tensor attention_workspace(const Tensor& q, const Tensor& v, int32_t code, bool 
                at::kByte, q);
 }
 
-// o, and where `want_state` is set the state after each sequence's last position
-std::tuple<Tensor, Tensor> linear_attention_fwd(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in,
+// o, where `want_state` is set the state after each sequence's last position, and the workspace
+std::tuple<Tensor, Tensor, Tensor> linear_attention_fwd(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in,
                                                 const Tensor& log_decay, double scale, const std::optional<Tensor>& state_in,
                                                 const std::optional<Tensor>& lengths_in, bool want_state) {
   at::NoGradGuard no_grad;
@@ -412,7 +412,7 @@ std::tuple<Tensor, Tensor> linear_attention_fwd(const Tensor& q_in, const Tensor
   Tensor q = head_rows(q_in), k = head_rows(k_in), v = head_rows(v_in), decay = log_decay.resolve_neg().contiguous();
   Tensor o = empty(v.sizes(), v.scalar_type(), v), new_state;
   if (want_state) new_state = empty({q.size(0), q.size(2), q.size(3), v.size(3)}, at::kFloat, q);
-  if (q.size(0) == 0 || q.size(2) == 0) return {o, new_state};
+  if (q.size(0) == 0 || q.size(2) == 0) return {o, new_state, Tensor()};
   Tensor ws = attention_workspace(q, v, code, false);
   int64_t strides[9], *at = strides;
   for (const Tensor* t : {&q, &k, &v}) strides_of(*t, at);
@@ -423,14 +423,14 @@ std::tuple<Tensor, Tensor> linear_attention_fwd(const Tensor& q_in, const Tensor
                                    static_cast<int32_t>(q.size(3)), static_cast<int32_t>(v.size(3)), strides,
                                    static_cast<float>(scale), code, ws.data_ptr(), ws.numel(), stream_of(q)),
         "bpc_linear_attention_fwd");
-  return {o, new_state};
+  return {o, new_state, ws};
 }
 
 // dq, dk, dv, and where `want_dstate` is set the gradient of the first state
 std::tuple<Tensor, Tensor, Tensor, Tensor> linear_attention_bwd(
     const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const Tensor& go_in, const Tensor& log_decay, double scale,
-    const std::optional<Tensor>& state_in, const std::optional<Tensor>& grad_state_in, const std::optional<Tensor>& lengths_in,
-    bool want_dstate) {
+    const std::optional<Tensor>& state_in, const std::optional<Tensor>& grad_state_in, const Tensor& fwd_workspace,
+    const std::optional<Tensor>& lengths_in, bool want_dstate) {
   at::NoGradGuard no_grad;
   const char* what = "linear_attention";
   const int32_t code = check_heads(q_in, k_in, v_in, log_decay, 4, what);
@@ -449,8 +449,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> linear_attention_bwd(
   int64_t strides[12], *at = strides;
   for (const Tensor* t : {&q, &k, &v, &go}) strides_of(*t, at);
   check(entry.linear_attention_bwd(q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), go.const_data_ptr(),
-                                   f32_or_null(decay), f32_or_null(state), f32_or_null(grad_state), data_or_null(lengths),
-                                   length_bytes(lengths), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                                   f32_or_null(decay), f32_or_null(state), f32_or_null(grad_state), data_or_null(fwd_workspace),
+                                   data_or_null(lengths), length_bytes(lengths), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                                    want_dstate ? static_cast<float*>(dstate.data_ptr()) : nullptr, q.size(0), q.size(1),
                                    static_cast<int32_t>(q.size(2)), static_cast<int32_t>(q.size(3)),
                                    static_cast<int32_t>(v.size(3)), strides, static_cast<float>(scale), code, ws.data_ptr(),
@@ -547,8 +547,8 @@ struct LinearAttention : torch::autograd::Function<LinearAttention> {
   static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay,
                                double scale, const std::optional<Tensor>& state, const std::optional<Tensor>& lengths,
                                bool want_state) {
-    auto [o, new_state] = linear_attention_fwd(q, k, v, log_decay, scale, state, lengths, want_state);
-    ctx->save_for_backward({q, k, v, log_decay, state.value_or(Tensor()), lengths.value_or(Tensor())});
+    auto [o, new_state, ws] = linear_attention_fwd(q, k, v, log_decay, scale, state, lengths, want_state);
+    ctx->save_for_backward({q, k, v, log_decay, state.value_or(Tensor()), lengths.value_or(Tensor()), ws});
     ctx->saved_data["scale"] = scale;
     ctx->set_materialize_grads(false);
     return want_state ? variable_list{o, new_state} : variable_list{o};
@@ -561,7 +561,7 @@ struct LinearAttention : torch::autograd::Function<LinearAttention> {
     const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &state = saved[4];
     const Tensor go = g[0].defined() ? g[0] : at::zeros_like(v);
     auto [dq, dk, dv, dstate] = linear_attention_bwd(q, k, v, go, saved[3], ctx->saved_data["scale"].toDouble(), if_defined(state),
-                                                     if_defined(grad_state), if_defined(saved[5]),
+                                                     if_defined(grad_state), saved[6], if_defined(saved[5]),
                                                      state.defined() && ctx->needs_input_grad(4));
     const variable_list grads = once({dq, dk, dv, dstate});
     for (int i = 0; i < 3; ++i) out[i] = grads[i];
@@ -578,7 +578,8 @@ std::tuple<Tensor, Tensor> linear_attention(const Tensor& q, const Tensor& k, co
     const variable_list r = LinearAttention::apply(q, k, v, log_decay, scale, state, lengths, want_state);
     return {r[0], want_state ? r[1] : Tensor()};
   }
-  return linear_attention_fwd(q, k, v, log_decay, scale, state, lengths, want_state);
+  auto [o, new_state, ws] = linear_attention_fwd(q, k, v, log_decay, scale, state, lengths, want_state);
+  return {o, new_state};
 }
 
 }  // namespace

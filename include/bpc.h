@@ -194,7 +194,9 @@ BPC_API int bpc_group_norm_bwd(const void* gy, const void* x, const float* stats
  * aligned (4-byte for the step); a NULL state or grad_state is zero.  lengths (B) int32 or int64 (length_bytes 4 or 8) or NULL (T each): positions
  * at or behind a sequence's length are not read, and zero in o, dq, dk and dv.  1 <= dk, dv <= 128, B H < 2^31.  States,
  * products and sums are fp32, in a fixed order (deterministic).  new_state may be the state itself, else they do not
- * overlap.  workspace: bpc_linear_attention_workspace_size() bytes on the current device, 16-byte aligned. */
+ * overlap.  workspace: bpc_linear_attention_workspace_size() bytes on the current device, 16-byte aligned; fwd_workspace: the
+ * workspace of bpc_linear_attention_fwd on the same inputs, as it was left (another than workspace), or NULL: what it holds is
+ * then formed again. */
 BPC_API size_t bpc_linear_attention_workspace_size(int64_t B, int64_t T, int32_t H, int32_t dk, int32_t dv, int32_t dtype,
                                                    int32_t backward);
 BPC_API int bpc_linear_attention_fwd(const void* q, const void* k, const void* v, void* o, const float* log_decay,
@@ -203,8 +205,8 @@ BPC_API int bpc_linear_attention_fwd(const void* q, const void* k, const void* v
                                      float scale, int32_t dtype, void* workspace, size_t workspace_bytes,
                                      bpc_stream_t stream);
 BPC_API int bpc_linear_attention_bwd(const void* q, const void* k, const void* v, const void* go, const float* log_decay,
-                                     const float* state, const float* grad_state, const void* lengths,
-                                     int32_t length_bytes, void* dq, void* dk_out, void* dv_out, float* dstate, int64_t B,
+                                     const float* state, const float* grad_state, const void* fwd_workspace,
+                                     const void* lengths, int32_t length_bytes, void* dq, void* dk_out, void* dv_out, float* dstate, int64_t B,
                                      int64_t T, int32_t H, int32_t dk, int32_t dv, const int64_t* strides, float scale,
                                      int32_t dtype, void* workspace, size_t workspace_bytes, bpc_stream_t stream);
 BPC_API int bpc_linear_attention_step(const void* q, const void* k, const void* v, void* o, const float* log_decay,

@@ -105,13 +105,13 @@ def test_linear_attention_refusals(lib):
 def test_linear_attention_backward_refusals(lib):
     f = lib.bpc_linear_attention_bwd
     keep, st = strides(*(24, 8, 4) * 4)
-    ok = dict(q=16, k=16, v=16, go=16, g=16, s=None, gs=None, n=None, nb=0, dq=16, dk_=16, dv_=16, ds=None, B=2, T=3, H=2, dk=4,
+    ok = dict(q=16, k=16, v=16, go=16, g=16, s=None, gs=None, fw=None, n=None, nb=0, dq=16, dk_=16, dv_=16, ds=None, B=2, T=3, H=2, dk=4,
               dv=4, strides=st, scale=1.0, dt=F32, ws=16, wsb=1 << 40, stream=None)
     for name in ("q", "k", "v", "go", "g", "dq", "dk_", "dv_", "ws", "strides"):
         refused(call(f, ok, **{name: None}), "null")
     for name in ("q", "k", "v", "go", "dq", "dk_", "dv_"):
         refused(call(f, ok, **{name: 18}), "aligned")
-    for name in ("s", "gs", "ds"):
+    for name in ("s", "gs", "ds", "fw"):
         refused(call(f, ok, **{name: 24}), "aligned")
     refused(call(f, ok, dk=200), "head sizes")
     refused(call(f, ok, wsb=0), "workspace", code=6)
