@@ -133,7 +133,7 @@ def lib() -> ctypes.CDLL:
 
 
 def torch_ops():
-    """The host side of the embedding and gradient-norm operators (csrc/torch_ops.cpp), bound to lib()'s entry points."""
+    """The host side of the embedding, norm and linear-attention operators (csrc/torch_ops.cpp), bound to lib()'s entry points."""
     global _torch
     if _torch is None:
         path = os.path.join(_PKG, "_torch_ops.so")

@@ -4,8 +4,8 @@
 
 Each csrc/*.cu is compiled by nvcc with -gencode arch=compute_100a,code=sm_100a into _build/, then linked into
 codecoder_b200/libbpc.so with the static CUDA runtime, so the library loads on a machine without a GPU (the driver is
-only opened on first use).  csrc/torch_ops.cpp, the host side of the embedding and gradient-norm operators on torch
-tensors, is compiled by g++ against the installed torch into codecoder_b200/_torch_ops.so."""
+only opened on first use).  csrc/torch_ops.cpp, the host side of the embedding, gradient-norm, group-norm and
+linear-attention operators on torch tensors, is compiled by g++ against the installed torch into codecoder_b200/_torch_ops.so."""
 from __future__ import annotations
 
 import concurrent.futures as cf

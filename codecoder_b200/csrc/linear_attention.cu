@@ -153,7 +153,6 @@ struct Tile {
   static constexpr int kGroups = kThreads / 32 / kWarps;
   static constexpr int kMT = kCols / 16;
   static constexpr int kNT = DP / 8;                                 // 8-column pieces of a, b
-  static constexpr int kRegs = kMT * kNT * 4;
   static constexpr int kPitch = kF32 ? (DP + 4) * 4 : DP * 2;
   static constexpr int kBytes = kChunk * kPitch;
   static constexpr int kPiece = 16 / sizeof(T);
@@ -590,7 +589,10 @@ __device__ __forceinline__ void zero_rows(T* out, int64_t stride, int slice, int
 }
 
 // A group of warps takes an item at a time, chunk by chunk, each warp some columns of c; the state stays in the warps'
-// registers.  The tiles of the next chunks, of the next items too, are on their way meanwhile.  REV: backwards in time.
+// registers.  Twelve warps an SM, whose dependent products and conversions bound it: 30,011 positions x 12 bf16 heads of 64
+// take 84 us (184 MB: 28 at the copy's rate), the tensor unit a quarter busy, 0.44 instructions a cycle and scheduler.  16
+// columns a warp and three blocks an SM against 32 and two: 115 us.  Chunks of 16 positions read and cut the state twice as often;
+// the state read as tf32 (11 bits) would save the cutting, and show in the result.  The tiles of the next chunks, of the next items too, are on their way meanwhile.  REV: backwards in time.
 // OUT false: the states that the segments leave behind alone.
 template <typename T, int DP, bool REV, bool OUT, int SPLIT>
 __global__ void __launch_bounds__(Tile<T, DP>::kThreads, Tile<T, DP>::kBlocks) scan_kernel(const __grid_constant__ Scans all) {
@@ -757,7 +759,10 @@ __global__ void __launch_bounds__(256) join_kernel(const Scan p, int per) {     
 // number them as it likes, so a piece's words are operands as they lie; c's 8 x 8 pieces are transposed by the tensor
 // unit's move; and a result's columns come out where c's pieces had them, so that a lane stores the pieces it would load.
 // The forward pass reads three and writes one tensor, the backward pass reads four and writes three: no state, and nothing
-// twice.
+// twice.  Up to 8 positions (HALVES 1) take half of the work: 25,600 heads of 5 fp32 positions 31 -> 20 us.
+//   bf16 heads of 32 are bound by memory: 371,712 of 11 positions 182 us forwards (5.8 TB/s of 1.05 GB), 343 backwards (5.3 of
+// 1.84).  Through shared memory and the long sequences' kernel, at 833 instructions a head against 240, they took 500 us a scan;
+// a state's worth of registers cost the occupancy that hides the loads.
 struct Short {
   Rows q, k, v, go;
   void *o, *dq, *dk, *dv;       // o, or the gradients
@@ -768,20 +773,20 @@ struct Short {
   uint32_t items, step_b, step_h;     // B H; a grid's warps as sequences and heads
 };
 
-template <typename T, int DP>
+template <typename T, int DP, int HALVES>
 struct Piece {
   static constexpr bool kF32 = sizeof(T) == 4;
   static constexpr int kWords = DP * static_cast<int>(sizeof(T)) / 16;      // of a lane, per row
   static constexpr int kWide = kWords < 4 ? kWords : 4;                    // of a load
   static constexpr int kElements = kWide * 4 / static_cast<int>(sizeof(T));
-  uint32_t r[2][kWords];
+  uint32_t r[HALVES][kWords];
   // column of a lane's first element of load k
   __device__ static __forceinline__ int column(int k) { return k * 4 * kElements + (threadIdx.x & 3) * kElements; }
 
   __device__ __forceinline__ void load(const T* row, int64_t stride, int rows, int dim) {
     const int g = (threadIdx.x & 31) >> 2;
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int h = 0; h < HALVES; ++h)
 #pragma unroll
       for (int k = 0; k < kWords / kWide; ++k) {
         const bool there = g + 8 * h < rows && column(k) < dim;
@@ -798,7 +803,7 @@ struct Piece {
   __device__ __forceinline__ void store(T* row, int64_t stride, int until, int dim) const {
     const int g = (threadIdx.x & 31) >> 2;
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int h = 0; h < HALVES; ++h)
 #pragma unroll
       for (int k = 0; k < kWords / kWide; ++k) {
         T* at = row + (g + 8 * h) * stride + column(k);
@@ -827,35 +832,37 @@ struct PairWeights {
   }
 };
 
-template <typename T, int DP>
-__device__ __forceinline__ Piece<T, DP> attend(const Piece<T, DP>& a, const Piece<T, DP>& b, const Piece<T, DP>& c,
-                                               const PairWeights& w, bool reverse, int rows) {
-  using P_ = Piece<T, DP>;
+template <typename T, int DP, int HALVES>
+__device__ __forceinline__ Piece<T, DP, HALVES> attend(const Piece<T, DP, HALVES>& a, const Piece<T, DP, HALVES>& b,
+                                                       const Piece<T, DP, HALVES>& c, const PairWeights& w, bool reverse, int rows) {
+  using P_ = Piece<T, DP, HALVES>;
+  constexpr int kLast = HALVES - 1;
+  auto second = [](uint32_t x) { return HALVES == 2 ? x : 0u; };      // of rows g + 8
   const int g = (threadIdx.x & 31) >> 2;
-  float P[2][4] = {};
-  Piece<T, DP> out;
+  float P[HALVES][4] = {};
+  P_ out;
   if constexpr (P_::kF32) {
 #pragma unroll
     for (int k = 0; k < P_::kWords / 2; ++k) {
-      const Split x[4] = {Split(__uint_as_float(a.r[0][2 * k])), Split(__uint_as_float(a.r[1][2 * k])),
-                          Split(__uint_as_float(a.r[0][2 * k + 1])), Split(__uint_as_float(a.r[1][2 * k + 1]))};
+      const Split x[4] = {Split(__uint_as_float(a.r[0][2 * k])), Split(__uint_as_float(second(a.r[kLast][2 * k]))),
+                          Split(__uint_as_float(a.r[0][2 * k + 1])), Split(__uint_as_float(second(a.r[kLast][2 * k + 1])))};
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int n = 0; n < HALVES; ++n)
         mma_f32(P[n], x, Split(__uint_as_float(b.r[n][2 * k])), Split(__uint_as_float(b.r[n][2 * k + 1])));
     }
   } else {
 #pragma unroll
     for (int k = 0; k < P_::kWords / 2; ++k) {
-      const uint32_t x[4] = {a.r[0][2 * k], a.r[1][2 * k], a.r[0][2 * k + 1], a.r[1][2 * k + 1]};
+      const uint32_t x[4] = {a.r[0][2 * k], second(a.r[kLast][2 * k]), a.r[0][2 * k + 1], second(a.r[kLast][2 * k + 1])};
 #pragma unroll
-      for (int n = 0; n < 2; ++n) mma_bf16(P[n], x, b.r[n][2 * k], b.r[n][2 * k + 1]);
+      for (int n = 0; n < HALVES; ++n) mma_bf16(P[n], x, b.r[n][2 * k], b.r[n][2 * k + 1]);
     }
   }
   // [n][row half][column]: masked products are dropped, not multiplied by zero
 #pragma unroll
-  for (int n = 0; n < 2; ++n)
+  for (int n = 0; n < HALVES; ++n)
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int h = 0; h < HALVES; ++h)
 #pragma unroll
       for (int z = 0; z < 2; ++z) {
         const bool never = reverse ? h > n : n > h;
@@ -865,53 +872,56 @@ __device__ __forceinline__ Piece<T, DP> attend(const Piece<T, DP>& a, const Piec
       }
   const bool keep0 = g < rows, keep1 = g + 8 < rows;
   if constexpr (P_::kF32) {
-    Split p[2][4];
+    Split p[HALVES][4];
 #pragma unroll
-    for (int n = 0; n < 2; ++n) p[n][0] = Split(P[n][0]), p[n][1] = Split(P[n][2]), p[n][2] = Split(P[n][1]), p[n][3] = Split(P[n][3]);
+    for (int n = 0; n < HALVES; ++n)
+      p[n][0] = Split(P[n][0]), p[n][1] = Split(HALVES == 2 ? P[n][2] : 0.0f), p[n][2] = Split(P[n][1]), p[n][3] = Split(HALVES == 2 ? P[n][3] : 0.0f);
 #pragma unroll
     for (int q = 0; q < P_::kWords / 2; ++q) {
       float O[4] = {};
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
+      for (int n = 0; n < HALVES; ++n) {
         // 32-bit elements as two pieces of 16-bit ones
         const uint32_t x0 = c.r[n][2 * q], x1 = c.r[n][2 * q + 1];
         const uint32_t lo = transpose(__byte_perm(x0, x1, 0x5410)), hi = transpose(__byte_perm(x0, x1, 0x7632));
         mma_f32(O, p[n], Split(__uint_as_float(__byte_perm(lo, hi, 0x5410))), Split(__uint_as_float(__byte_perm(lo, hi, 0x7632))));
       }
       out.r[0][2 * q] = keep0 ? __float_as_uint(O[0]) : 0u, out.r[0][2 * q + 1] = keep0 ? __float_as_uint(O[1]) : 0u;
-      out.r[1][2 * q] = keep1 ? __float_as_uint(O[2]) : 0u, out.r[1][2 * q + 1] = keep1 ? __float_as_uint(O[3]) : 0u;
+      if (HALVES == 2) out.r[kLast][2 * q] = keep1 ? __float_as_uint(O[2]) : 0u, out.r[kLast][2 * q + 1] = keep1 ? __float_as_uint(O[3]) : 0u;
     }
   } else {
     // the weighted products as two bf16 parts: one would round as coarsely as the result
     uint32_t hi[4], lo[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float p0 = P[e >> 1][2 * (e & 1)], p1 = P[e >> 1][2 * (e & 1) + 1];
+      const bool some = HALVES == 2 || e == 0;
+      const float p0 = some ? P[HALVES == 2 ? e >> 1 : 0][2 * (e & 1)] : 0.0f, p1 = some ? P[HALVES == 2 ? e >> 1 : 0][2 * (e & 1) + 1] : 0.0f;
       hi[e] = pack(p0, p1);
       lo[e] = pack(p0 - low(hi[e]), p1 - high(hi[e]));
     }
 #pragma unroll
     for (int q = 0; q < P_::kWords; ++q) {
       float O[4] = {};
-      const uint32_t b0 = transpose(c.r[0][q]), b1 = transpose(c.r[1][q]);
+      const uint32_t b0 = transpose(c.r[0][q]), b1 = HALVES == 2 ? transpose(c.r[kLast][q]) : 0u;
       mma_bf16(O, lo, b0, b1);
       mma_bf16(O, hi, b0, b1);
       out.r[0][q] = keep0 ? pack(O[0], O[1]) : 0u;
-      out.r[1][q] = keep1 ? pack(O[2], O[3]) : 0u;
+      if (HALVES == 2) out.r[kLast][q] = keep1 ? pack(O[2], O[3]) : 0u;
     }
   }
   return out;
 }
 
-// Blocks per SM that the registers are cut for: bf16 backwards 342 us with 4, 363 with the 3 that it takes by itself
+// Blocks per SM that the registers are cut for (0: the compiler's choice): bf16 backwards 343 us with 4, 365 with its 3; forwards its 6
+// take 180 us and a cut to the same 6 takes 190
 template <typename T, int DP, bool BWD>
-constexpr int kShortBlocks = sizeof(T) == 2 && DP <= 32 ? (BWD ? 4 : 6) : 1;
+constexpr int kShortBlocks = BWD && sizeof(T) == 2 && DP <= 32 ? 4 : 0;
 
-template <typename T, int DP, bool BWD>
+template <typename T, int DP, bool BWD, int HALVES>
 __global__ void __launch_bounds__(kThreads, kShortBlocks<T, DP, BWD>) short_kernel(const __grid_constant__ Short p) {
   const uint32_t first = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5), stride = gridDim.x * (kThreads / 32);
   uint32_t b = first / p.H, h = first - b * p.H;
-  Piece<T, DP> q, k, v, go;
+  Piece<T, DP, HALVES> q, k, v, go;
   int rows = 0;
   auto load = [&] {
     rows = length_of(p.lengths, p.length_bytes, b, p.T);
@@ -923,7 +933,7 @@ __global__ void __launch_bounds__(kThreads, kShortBlocks<T, DP, BWD>) short_kern
   };
   if (first < p.items) load();
   for (uint32_t at = first; at < p.items;) {
-    const Piece<T, DP> q0 = q, k0 = k, v0 = v, go0 = go;
+    const Piece<T, DP, HALVES> q0 = q, k0 = k, v0 = v, go0 = go;
     const uint32_t b0 = b, h0 = h;
     const int rows0 = rows;
     const float log2_a = log2_decay(p.log_decay, h);
@@ -937,18 +947,19 @@ __global__ void __launch_bounds__(kThreads, kShortBlocks<T, DP, BWD>) short_kern
     const int64_t sk = static_cast<int64_t>(p.H) * p.dim_k, sv = static_cast<int64_t>(p.H) * p.dim_v;
     const PairWeights forward(log2_a, false, p.scale);
     if constexpr (!BWD) {
-      attend<T, DP>(q0, k0, v0, forward, false, rows0).store(static_cast<T*>(p.o) + row * p.dim_v, sv, p.T, p.dim_v);
+      attend<T, DP, HALVES>(q0, k0, v0, forward, false, rows0).store(static_cast<T*>(p.o) + row * p.dim_v, sv, p.T, p.dim_v);
     } else {
-      attend<T, DP>(go0, v0, k0, forward, false, rows0).store(static_cast<T*>(p.dq) + row * p.dim_k, sk, p.T, p.dim_k);
+      attend<T, DP, HALVES>(go0, v0, k0, forward, false, rows0).store(static_cast<T*>(p.dq) + row * p.dim_k, sk, p.T, p.dim_k);
       const PairWeights back(log2_a, true, p.scale);
-      attend<T, DP>(v0, go0, q0, back, true, rows0).store(static_cast<T*>(p.dk) + row * p.dim_k, sk, p.T, p.dim_k);
-      attend<T, DP>(k0, q0, go0, back, true, rows0).store(static_cast<T*>(p.dv) + row * p.dim_v, sv, p.T, p.dim_v);
+      attend<T, DP, HALVES>(v0, go0, q0, back, true, rows0).store(static_cast<T*>(p.dk) + row * p.dim_k, sk, p.T, p.dim_k);
+      attend<T, DP, HALVES>(k0, q0, go0, back, true, rows0).store(static_cast<T*>(p.dv) + row * p.dim_v, sv, p.T, p.dim_v);
     }
   }
 }
 
 // ---- one position --------------------------------------------------------------------------------------------------
-// The state updated and read once: memory alone bounds it.  WARPS warps per sequence and head, each some rows of the state; LV
+// The state updated and read once: memory alone bounds it (64 x 676 heads of 32 x 32: 354 MB in 64 us, 5.7 TB/s; a block per head
+// and a thread per column took 178).  WARPS warps per sequence and head, each some rows of the state; LV
 // lanes of four columns across a row, so that a lane has 16-byte pieces of kUnroll rows under way.
 struct Step {
   const void *q, *k, *v;
@@ -1072,10 +1083,6 @@ auto with_type(int32_t dtype, F f) {
   return f(Type<__nv_bfloat16>());
 }
 
-int padded(int dim) {
-  return with_dim(dim, [](auto d) { return decltype(d)::value; });
-}
-
 // Groups of scan_kernel's warps that are resident
 int64_t resident_groups(int dim, int size) {
   return static_cast<int64_t>(num_sms()) * with_dim(dim, [&](auto d) {
@@ -1150,28 +1157,33 @@ int blocks_of(const void* fn, int* cached, int* blocks) {
   return 0;
 }
 
-template <typename T, int DP, bool BWD>
+template <typename T, int DP, bool BWD, int HALVES>
 int launch_short(Short p, cudaStream_t s) {
   static int cached = 0;
   int blocks = 0;
-  if (int e = blocks_of(reinterpret_cast<const void*>(&short_kernel<T, DP, BWD>), &cached, &blocks)) return e;
+  if (int e = blocks_of(reinterpret_cast<const void*>(&short_kernel<T, DP, BWD, HALVES>), &cached, &blocks)) return e;
   const uint32_t warps = kThreads / 32;
   const unsigned grid = std::min<unsigned>((p.items + warps - 1) / warps, blocks * num_sms());
   p.step_b = grid * warps / p.H, p.step_h = grid * warps % p.H;
-  short_kernel<T, DP, BWD><<<grid, kThreads, 0, s>>>(p);
+  short_kernel<T, DP, BWD, HALVES><<<grid, kThreads, 0, s>>>(p);
   return launched("linear_attention");
+}
+
+template <bool BWD, int HALVES>
+int run_short_of(const Short& p, int32_t dtype, cudaStream_t s) {
+  return with_type(dtype, [&](auto type) {
+    typedef typename decltype(type)::type T;
+    const int dim = std::max(p.dim_k, p.dim_v);
+    if (dim <= 16) return launch_short<T, 16, BWD, HALVES>(p, s);
+    if constexpr (sizeof(T) == 2)
+      if (dim > 32) return launch_short<T, 64, BWD, HALVES>(p, s);
+    return launch_short<T, 32, BWD, HALVES>(p, s);
+  });
 }
 
 template <bool BWD>
 int run_short(const Short& p, int32_t dtype, cudaStream_t s) {
-  return with_type(dtype, [&](auto type) {
-    typedef typename decltype(type)::type T;
-    const int dim = std::max(p.dim_k, p.dim_v);
-    if (dim <= 16) return launch_short<T, 16, BWD>(p, s);
-    if constexpr (sizeof(T) == 2)
-      if (dim > 32) return launch_short<T, 64, BWD>(p, s);
-    return launch_short<T, 32, BWD>(p, s);
-  });
+  return p.T <= 8 ? run_short_of<BWD, 1>(p, dtype, s) : run_short_of<BWD, 2>(p, dtype, s);
 }
 
 // Head sizes that short_kernel holds in registers
