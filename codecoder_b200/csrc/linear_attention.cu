@@ -1214,7 +1214,7 @@ int check_common(const std::string& what, int64_t B, int64_t T, int32_t H, int32
                  const float* log_decay) {
   auto bad = [&](const char* m) { return fail(BPC_ERR_ARG, what + ": " + m); };
   if (B < 0 || T < 0 || H < 0 || T > (1 << 30)) return bad("batch, length and heads must not be negative, length <= 2^30");
-  if (H && B > 0x7fffffff / H) return bad("batch x heads must be below 2^31");
+  if (H && B > 0x3fffffff / H) return bad("batch x heads must be below 2^30");      // items of two scans are counted in 32 bits
   if (dk < 1 || dk > kMaxDim || dv < 1 || dv > kMaxDim) return bad("head sizes must be 1 to 128");
   if (!size_of(dtype)) return bad("dtype must be f32 or bf16");
   if (!std::isfinite(scale)) return bad("scale must be finite");

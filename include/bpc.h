@@ -192,7 +192,7 @@ BPC_API int bpc_group_norm_bwd(const void* gy, const void* x, const float* stats
  * (batch, head) strides.  o, dv like v, dq, dk like q, contiguous, of the inputs' type.  log_decay (H) fp32, -infinity
  * forgets everything; no gradient of it is formed.  state, new_state, grad_state, dstate (B, H, dk, dv) fp32, 16-byte
  * aligned (4-byte for the step); a NULL state or grad_state is zero.  lengths (B) int32 or int64 (length_bytes 4 or 8) or NULL (T each): positions
- * at or behind a sequence's length are not read, and zero in o, dq, dk and dv.  1 <= dk, dv <= 128, B H < 2^31.  States,
+ * at or behind a sequence's length are not read, and zero in o, dq, dk and dv.  1 <= dk, dv <= 128, B H < 2^30, T <= 2^30.  States,
  * products and sums are fp32, in a fixed order (deterministic).  new_state may be the state itself, else they do not
  * overlap.  workspace: bpc_linear_attention_workspace_size() bytes on the current device, 16-byte aligned; fwd_workspace: the
  * workspace of bpc_linear_attention_fwd on the same inputs, as it was left (another than workspace), or NULL: what it holds is

@@ -151,6 +151,34 @@ def test_layouts(N):
     assert torch.equal(y, ops.group_norm(x[:, :, ::2].contiguous(), 4))
 
 
+@pytest.mark.parametrize("N,C,G", [(1, 96, 3), (40, 64, 4), (700, 16, 1)])
+def test_offsets_past_32_bits(N, C, G):
+    """Samples more than 2^31 elements apart (rows and gradients too)."""
+    def far(t):
+        wide = torch.empty(2**31 + 2**20 + N * C, device=DEV, dtype=t.dtype)
+        v = wide.as_strided(t.shape, (2**31 + 2**20, C, 1))
+        return v.copy_(t)
+    run(2, N, C, G, "silu", BF16, BF16, True, N, views=far)
+
+
+def test_a_bias_without_a_weight():
+    x, gy, w, b = make(9, 31, 24, F32, F32, True, 2)
+    x, b = x.requires_grad_(), b.requires_grad_()
+    dx, db = torch.autograd.grad(ops.group_norm(x, 3, None, b, EPS, "gelu"), (x, b), gy)
+    one = torch.ones(24, device=DEV)
+    want = definition(x.detach(), 3, one, b.detach(), EPS, "gelu", gy)
+    check(dx, want[1], F32, "dx")
+    check(db, want[3], F32, "db")
+
+
+def test_many_samples_and_many_groups():
+    run(70000, 2, 16, 2, "silu", BF16, BF16, True, 1)          # more samples than a grid has rows of blocks
+    run(66000, 40, 6, 2, "none", F32, F32, True, 2)
+    run(1, 3, 8192, 4096, "silu", F32, BF16, True, 3)
+    run(2, 1, 100000, 100000, "none", F32, F32, True, 4)
+    run(1, 5, 9000, 3, "gelu", BF16, BF16, True, 5)            # groups wider than a row of threads
+
+
 def test_empty_tensors():
     w = torch.ones(8, device=DEV, requires_grad=True)
     for shape in ((0, 5, 8), (3, 0, 8), (0, 8)):

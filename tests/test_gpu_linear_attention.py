@@ -129,6 +129,15 @@ def test_values_and_gradients_match_the_definition(shape, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("T", [2, 3, 7, 8, 9, 15, 16, 17, 32])
+def test_lengths_where_the_kernels_change(T, dtype):
+    for D in (8, 16, 24, 32, 40, 64):
+        run(make(3, T, 5, D, D, dtype, T + D))
+    run(make(3, T, 5, 24, 32, dtype, T, lengths=[T, T - 1, 1]))
+    run(make(2, T, 3, 64, 16, dtype, T, state=True))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("T,dk,dv", [(11, 32, 32), (40, 64, 64), (150, 24, 40), (300, 32, 32)])
 def test_lengths(T, dk, dv, dtype):
     lengths = [0, 1, T, T // 2, T - 1, T + 5, -3, min(16, T), min(17, T)]
@@ -166,23 +175,78 @@ def test_long_sequences(B, T, H, D, dtype):
     run(s)
 
 
-def test_offsets_past_32_bits():
-    """Rows more than 2^31 elements apart, and a sequence's positions too."""
+@pytest.mark.parametrize("with_state", [False, True])
+def test_offsets_past_32_bits(with_state):
+    """Rows more than 2^31 elements apart, and a sequence's positions too; without a state in registers, with one in chunks."""
     B, T, H, D = 2, 3, 2, 32
-    s = make(B, T, H, D, D, BF16, 3)
+    s = make(B, T, H, D, D, BF16, 3, with_state)
     far = {}
     for i, x in enumerate(("q", "k", "v", "go")):
         wide = torch.empty((B - 1) * 6 * 2**29 + (T - 1) * 2**30 + H * D, device=DEV, dtype=BF16)
         far[x] = wide.as_strided((B, T, H, D), (6 * 2**29, 2**30, D, 1))
         far[x].copy_(s[x])
-    ref = ops.linear_attention(s["q"], s["k"], s["v"], s["g"])
+    ref = ops.linear_attention(s["q"], s["k"], s["v"], s["g"], state=s["s0"])
     leaves = [far[x].requires_grad_() for x in "qkv"]
-    o = ops.linear_attention(*leaves, s["g"])
+    o = ops.linear_attention(*leaves, s["g"], state=s["s0"])
     assert torch.equal(o, ref)
     grads = torch.autograd.grad(o, leaves, far["go"])
     near = [s[x].requires_grad_() for x in "qkv"]
-    for p, q in zip(grads, torch.autograd.grad(ops.linear_attention(*near, s["g"]), near, s["go"])):
+    for p, q in zip(grads, torch.autograd.grad(ops.linear_attention(*near, s["g"], state=s["s0"]), near, s["go"])):
         assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_the_gradients_do_not_need_the_forwards_workspace(dtype):
+    """bpc_linear_attention_bwd with and without the workspace that the forward pass left, over several segments."""
+    from array import array
+
+    from codecoder_b200 import _lib
+    B, T, H, dk, dv = 2, 700, 2, 32, 24
+    s = make(B, T, H, dk, dv, dtype, 6, True)
+    s["n"] = torch.tensor([650, 90], device=DEV)
+    L, code = _lib.lib(), _lib.BPC_DTYPE_F32 if dtype == F32 else _lib.BPC_DTYPE_BF16
+    tensors = [s[x] for x in ("q", "k", "v", "go")]
+    strides = array("q", [st for t in tensors for st in t.stride()[:3]])
+    at = strides.buffer_info()[0]
+    fwd_ws, bwd_ws = (torch.empty(int(L.bpc_linear_attention_workspace_size(B, T, H, dk, dv, code, i)), device=DEV, dtype=torch.uint8)
+                      for i in range(2))
+    assert fwd_ws.numel() > 16                      # several segments
+    o, end = torch.empty_like(s["v"]), torch.empty_like(s["s0"])
+    stream = torch.cuda.current_stream().cuda_stream
+    p = lambda t: None if t is None else t.data_ptr()
+    _lib.check(L.bpc_linear_attention_fwd(p(s["q"]), p(s["k"]), p(s["v"]), p(o), p(s["g"]), p(s["s0"]), p(end), p(s["n"]), 8, B, T, H,
+                                          dk, dv, at, 0.5, code, p(fwd_ws), fwd_ws.numel(), stream), "fwd")
+    out = []
+    for ws in (fwd_ws, None):
+        g = [torch.empty_like(s[x]) for x in ("q", "k", "v", "s0")]
+        _lib.check(L.bpc_linear_attention_bwd(*(p(t) for t in tensors), p(s["g"]), p(s["s0"]), p(s["gs"]), p(ws), p(s["n"]), 8,
+                                              *(p(t) for t in g), B, T, H, dk, dv, at, 0.5, code, p(bwd_ws), bwd_ws.numel(), stream),
+                   "bwd")
+        out.append(g)
+    want = definition(*(s[x] for x in "qkv"), s["g"], 0.5, s["s0"], s["n"], s["go"], s["gs"])
+    mag = definition(*(s[x] for x in "qkv"), s["g"], 0.5, s["s0"], s["n"], s["go"], s["gs"], mag=True)
+    check(o, want[0], mag[0], dtype, T, 32, "o")
+    for g in out:
+        for name, t, i in zip(("q", "k", "v", "s0"), g, range(2, 6)):
+            check(t, want[i], mag[i], F32 if name == "s0" else dtype, T, 32, "d" + name)
+
+
+def test_two_streams_at_once():
+    """Calls on two streams, each with its own workspaces, do not disturb one another."""
+    cases = [make(2, 900, 2, 64, 64, BF16, i, True) for i in range(2)]
+    call = lambda s: ops.linear_attention(s["q"], s["k"], s["v"], s["g"], state=s["s0"], return_state=True)
+    want = [call(s) for s in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = [[], []]
+    for _ in range(5):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(call(cases[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for o, end in got[i]:
+            assert torch.equal(o, want[i][0]) and torch.equal(end, want[i][1])
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])

@@ -83,7 +83,8 @@ def test_linear_attention_refusals(lib):
         refused(call(f, ok, **{name: None}), "null")
     for name in ("B", "T", "H"):
         refused(call(f, ok, **{name: -1}), "negative")
-    refused(call(f, ok, B=1 << 20, H=1 << 12), "2^31")
+    refused(call(f, ok, B=1 << 20, H=1 << 10), "2^30")
+    refused(call(f, ok, T=(1 << 30) + 1), "2^30")
     for name in ("dk", "dv"):
         for d in (0, 129):
             refused(call(f, ok, **{name: d}), "head sizes")
