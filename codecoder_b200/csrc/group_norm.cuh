@@ -259,12 +259,17 @@ __device__ __forceinline__ void group_sums(float (&value)[N], int V, int rows, i
   }
   __syncthreads();
   // a warp per group; the sums go where its first thread's values were, when all of them are read
+  const int down = 32 / across, along = 32 % across;
   for (int g = warp; g < V / across; g += blockDim.x >> 5) {
 #pragma unroll
     for (int k = 0; k < N; ++k) {
       float* f = part + k * kTileThreads + g * across;
       float sum = 0.0f;
-      for (int i = lane; i < rows * across; i += 32) sum += f[i / across * V + i % across];
+      for (int row = lane / across, col = lane % across; row < rows;) {      // entries lane, lane + 32, ... of rows of `across`
+        sum += f[row * V + col];
+        row += down, col += along;
+        if (col >= across) col -= across, ++row;
+      }
 #pragma unroll
       for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
       if (lane == 0) f[0] = sum;                   // read by this warp alone until here

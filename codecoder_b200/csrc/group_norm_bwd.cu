@@ -88,19 +88,21 @@ __global__ void __launch_bounds__(kUnitThreads) units_kernel(const U* __restrict
   const uint32_t at_stat = SLOTS * (x_bytes + g_bytes) + threadIdx.x * 8, stage_bytes = SLOTS * (x_bytes + g_bytes) + blockDim.x * 8;
   const uint32_t base = smem_u32(smem);
   uint32_t fetched = 0, used = 0;
-  int64_t ahead_x = 0, ahead_g = 0, off_x = 0, off_g = 0;
   const float2* stat = stats + (b0 + r) * s.G + g;
+  const int64_t stat_step = step * s.G;
   auto fetch = [&](int round) {
     if (round < mine) {
       asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(base + fetched + at_stat), "l"(stat) : "memory");
 #pragma unroll
       for (int k = 0; k < SLOTS; ++k)
         if (has[k]) {
-          X::fetch(base + fetched + at_x + k * x_bytes, from[k] + ahead_x);
-          Y::fetch(base + fetched + at_g + k * g_bytes, from_g[k] + ahead_g);
+          X::fetch(base + fetched + at_x + k * x_bytes, from[k]);
+          Y::fetch(base + fetched + at_g + k * g_bytes, from_g[k]);
         }
     }
-    ahead_x += x_step, ahead_g += g_step, stat += step * s.G;
+#pragma unroll
+    for (int k = 0; k < SLOTS; ++k) from[k] += x_step, from_g[k] += g_step;
+    stat += stat_step;
     fetched = fetched == (kDepth - 1) * stage_bytes ? 0 : fetched + stage_bytes;
     cp_commit();
   };
@@ -110,20 +112,20 @@ __global__ void __launch_bounds__(kUnitThreads) units_kernel(const U* __restrict
     fetch(round + kDepth - 1);
     cp_wait<kDepth - 1>();
     const bool live = round < mine;
-    float mean = 0.0f, rstd = 0.0f;
-    if (live) {
-      const float2 f = *reinterpret_cast<const float2*>(smem + used + at_stat);
-      mean = f.x, rstd = f.y;
-    }
+    const float2 f = *reinterpret_cast<const float2*>(smem + used + at_stat);
+    const float mean = live ? f.x : 0.0f, rstd = live ? f.y : 0.0f;
     const uint64_t scale = f2_of(rstd), minus = f2_of(-mean);
     uint64_t xh[SLOTS][kP], gz[SLOTS][kP], s1 = 0, s2 = 0;
 #pragma unroll
     for (int k = 0; k < SLOTS; ++k) {
       Pack<T, VEC> vx = Pack<T, VEC>();            // zeros: nothing to any sum
       Pack<U, VEC> vg = Pack<U, VEC>();
-      if (has[k] && live) {
-        vx = X::take(smem, used + at_x + k * x_bytes, from[k] + off_x);
-        vg = Y::take(smem, used + at_g + k * g_bytes, from_g[k] + off_g);
+      if (X::kCopies && Y::kCopies) {              // what was not fetched is replaced, not asked for: nearly all is
+        vx = X::take(smem, used + at_x + k * x_bytes, nullptr), vg = Y::take(smem, used + at_g + k * g_bytes, nullptr);
+        if (!(has[k] && live)) vx = Pack<T, VEC>(), vg = Pack<U, VEC>();
+      } else if (has[k] && live) {                 // the pointers are kDepth samples ahead
+        vx = X::take(smem, used + at_x + k * x_bytes, from[k] - kDepth * x_step);
+        vg = Y::take(smem, used + at_g + k * g_bytes, from_g[k] - kDepth * g_step);
       }
 #pragma unroll
       for (int i = 0; i < kP; ++i) {
@@ -131,7 +133,6 @@ __global__ void __launch_bounds__(kUnitThreads) units_kernel(const U* __restrict
         gz[k][i] = vg.pair(i);
       }
     }
-    off_x += x_step, off_g += g_step;
     used = used == (kDepth - 1) * stage_bytes ? 0 : used + stage_bytes;
 #pragma unroll
     for (int k = 0; k < SLOTS; ++k)

@@ -646,6 +646,10 @@ __global__ void __launch_bounds__(Tile<T, DP>::kThreads, Tile<T, DP>::kBlocks) s
   };
 #pragma unroll
   for (int s = 0; s < kS - 1; ++s) load();
+  // the kernels of one call follow one another programmatically: the inputs were there before the first, the states are when
+  // the one before is done
+  if constexpr (!OUT) pdl_launch_dependents();
+  else pdl_wait();
 
   Warp<T, DP, REV> state;
   uint32_t tile = base;
@@ -729,6 +733,8 @@ __global__ void __launch_bounds__(256) join_kernel(const Scan p, int per) {     
   const uint32_t bh = blockIdx.x / per;
   const int b = bh / p.H, n = length_of(p.lengths, p.length_bytes, b, p.T), D = p.da * p.dc;
   const int e = blockIdx.x % per * 256 + threadIdx.x;
+  pdl_launch_dependents();
+  pdl_wait();
   if (e >= D) return;
   const float log2_a = log2_decay(p.log_decay, bh - b * p.H);
   float* f = p.parts + static_cast<int64_t>(bh) * (p.segments - 1) * D + e;
@@ -1092,12 +1098,16 @@ int64_t resident_groups(int dim, int size) {
 }
 
 template <typename T, int DP, bool REV, bool OUT, int SPLIT>
-int launch_scan(const Scan& p, const Scan* second, cudaStream_t s) {
+int launch_scan(const Scan& p, const Scan* second, bool follows, cudaStream_t s) {
   using L = Tile<T, DP>;
   const void* fn = reinterpret_cast<const void*>(&scan_kernel<T, DP, REV, OUT, SPLIT>);
   if (int e = allow_smem(fn, L::kSmem)) return e;
-  const Scans all{{p, second ? *second : p}, p.items, second ? 2 * p.items : p.items};
+  Scans all{{p, second ? *second : p}, p.items, second ? 2 * p.items : p.items};
   const unsigned grid = std::min<unsigned>((all.total + L::kGroups - 1) / L::kGroups, L::kBlocks * num_sms());
+  if (follows) {
+    void* args[] = {&all};
+    return launch_pdl(fn, dim3(grid), dim3(L::kThreads), L::kSmem, s, args, 1, "linear_attention");
+  }
   scan_kernel<T, DP, REV, OUT, SPLIT><<<grid, L::kThreads, L::kSmem, s>>>(all);
   return launched("linear_attention");
 }
@@ -1134,13 +1144,17 @@ int run_scan(Scan p, Scan* second, int64_t B, int32_t dtype, float* workspace, c
       constexpr int DP = decltype(d)::value;
       // the state handed out is fp32: it needs every bit of the weighted rows; a bf16 result alone does with 16
       constexpr int kFew = sizeof(T) == 4 ? 3 : 2;
-      if (p.segments > 1 && !turned_parts) {
-        if (int e = p.last ? launch_scan<T, DP, REV, false, 3>(p, nullptr, s) : launch_scan<T, DP, REV, false, kFew>(p, nullptr, s)) return e;
-        const int per = (p.da * p.dc + 255) / 256;
-        join_kernel<REV><<<static_cast<unsigned>(BH * per), 256, 0, s>>>(p, per);
-        if (int e = launched("linear_attention")) return e;
+      const bool parts = p.segments > 1 && !turned_parts;
+      if (parts) {
+        if (int e = p.last ? launch_scan<T, DP, REV, false, 3>(p, nullptr, false, s) : launch_scan<T, DP, REV, false, kFew>(p, nullptr, false, s))
+          return e;
+        int per = (p.da * p.dc + 255) / 256;
+        void* args[] = {&p, &per};
+        if (int e = launch_pdl(reinterpret_cast<const void*>(&join_kernel<REV>), dim3(static_cast<unsigned>(BH * per)), dim3(256), 0, s, args, 1,
+                               "linear_attention"))
+          return e;
       }
-      return p.last ? launch_scan<T, DP, REV, true, 3>(p, second, s) : launch_scan<T, DP, REV, true, kFew>(p, second, s);
+      return p.last ? launch_scan<T, DP, REV, true, 3>(p, second, parts, s) : launch_scan<T, DP, REV, true, kFew>(p, second, parts, s);
     });
   });
 }
