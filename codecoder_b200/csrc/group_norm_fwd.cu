@@ -52,18 +52,19 @@ __global__ void __launch_bounds__(kUnitThreads) units_kernel(const T* __restrict
   const float n = static_cast<float>(s.N) * static_cast<float>(cg), per = 1.0f / n;
   const int64_t x_step = step * s.x_sample, y_step = step * s.N * s.C;
   float2* stat = stats + (b0 + r) * s.G + g;
+  const int64_t stat_step = step * s.G;
   // a thread's places in a stage, and the stages of the sample fetched and of the one worked on
   const uint32_t mine_at = threadIdx.x * In::kBytes, slot_bytes = blockDim.x * In::kBytes, stage_bytes = SLOTS * slot_bytes;
   const uint32_t base = smem_u32(smem) + mine_at;
   uint32_t fetched = 0, used = 0;
-  int64_t ahead = 0, offset = 0;
   auto fetch = [&](int round) {
     if (round < mine) {
 #pragma unroll
       for (int k = 0; k < SLOTS; ++k)
-        if (has[k]) In::fetch(base + fetched + k * slot_bytes, from[k] + ahead);
+        if (has[k]) In::fetch(base + fetched + k * slot_bytes, from[k]);
     }
-    ahead += x_step;
+#pragma unroll
+    for (int k = 0; k < SLOTS; ++k) from[k] += x_step;
     fetched = fetched == (kDepth - 1) * stage_bytes ? 0 : fetched + stage_bytes;
     cp_commit();
   };
@@ -76,14 +77,18 @@ __global__ void __launch_bounds__(kUnitThreads) units_kernel(const T* __restrict
 #pragma unroll
     for (int k = 0; k < SLOTS; ++k) {
       Pack<T, VEC> v = Pack<T, VEC>();
-      if (has[k] && round < mine) v = In::take(smem, mine_at + used + k * slot_bytes, from[k] + offset);
+      if (In::kCopies) {                           // what was not fetched is replaced, not asked for: nearly all is
+        v = In::take(smem, mine_at + used + k * slot_bytes, nullptr);
+        if (!(has[k] && round < mine)) v = Pack<T, VEC>();
+      } else if (has[k] && round < mine) {         // the pointers are kDepth samples ahead
+        v = In::take(smem, 0, from[k] - kDepth * x_step);
+      }
 #pragma unroll
       for (int i = 0; i < kP; ++i) d[k][i] = v.pair(i);
 #pragma unroll
       for (int i = 0; i < kP; ++i) t = f2_add(t, d[k][i]);
     }
     used = used == (kDepth - 1) * stage_bytes ? 0 : used + stage_bytes;
-    offset += x_step;
     const float mean = over(lanes_sum(both<VEC>(t), p.lanes), n, per);
     const uint64_t minus = f2_of(-mean);
     t = 0;
@@ -99,7 +104,7 @@ __global__ void __launch_bounds__(kUnitThreads) units_kernel(const T* __restrict
     }
     const float rstd = inverse_sqrt(fmaf(lanes_sum(both<VEC>(t), p.lanes), per, eps));
     if (stats && l == 0 && round < mine) *stat = make_float2(mean, rstd);
-    stat += step * s.G;
+    stat += stat_step;
     const uint64_t scale = f2_of(rstd);
 #pragma unroll
     for (int k = 0; k < SLOTS; ++k) {
