@@ -7,8 +7,8 @@
 // One read of gy and x and one write of dx where a sample's slab fits the registers of a block or a cluster.  A thread
 // always has the same channels and walks the samples, so that dw and db are sums in registers until the end: a part per
 // block, joined in order in fp64 (deterministic, no atomics).
-//   512 x 504 x 512 fp32 with bf16 gradients: 289 us, 4.6 TB/s of 1.32 GB; 1.36 M samples of 96 bf16 channels: 233 us, 3.4 TB/s of
-// 785 MB, bound by instructions (39 a value, of which the activation's are 5).
+//   512 x 504 x 512 fp32 with bf16 gradients: 289 us, 4.6 TB/s of 1.32 GB; 1.36 M samples of 96 bf16 channels: 189 us, 4.2 TB/s of
+// 794 MB, bound by instructions (32 a value, of which the activation's are 5).
 #include "group_norm.cuh"
 
 namespace bpc {
@@ -49,7 +49,8 @@ __device__ __forceinline__ void channel_sums(const uint64_t (&a)[(VEC + 1) / 2],
 template <typename T, typename U, int ACT, int VEC, int SLOTS>
 __global__ void __launch_bounds__(kUnitThreads) units_kernel(const U* __restrict__ gy, const T* __restrict__ x,
                                                              const float2* __restrict__ stats,
-                                                             const float* __restrict__ w, const float* __restrict__ bias, T* __restrict__ dx, float* parts,
+                                                             const float* __restrict__ w, const float* __restrict__ bias, T* __restrict__ dx,
+                                                             float* parts,
                                                              const Shape s, const Plan p) {
   constexpr int kP = Pack<T, VEC>::kPairs;
   extern __shared__ __align__(16) uint8_t smem[];
@@ -159,7 +160,8 @@ __global__ void __launch_bounds__(kUnitThreads) units_kernel(const U* __restrict
     }
   }
   if (!parts) return;
-  // every copy has been taken: its memory holds the channels' sums now.  The rows of a sample share channels: a row of the buffer for each of them and each of the block's samples
+  // every copy has been taken: its memory holds the channels' sums now.  The rows of a sample share channels: a row of the
+  // buffer for each of them and each of the block's samples
   parts += static_cast<int64_t>(blockIdx.x) * 2 * s.C;
   float* buffer = reinterpret_cast<float*>(smem);
   const int V = s.G * across, rows = p.rows * static_cast<int>(s.N);
@@ -192,7 +194,8 @@ enum Mode { kFused, kSums, kApply };
 template <typename T, typename U, int ACT, int VEC, int MODE>
 __global__ void __launch_bounds__(kTileThreads, 2) tiles_kernel(const U* __restrict__ gy, const T* __restrict__ x,
                                                             const float2* __restrict__ stats,
-                                                            const float* __restrict__ w, const float* __restrict__ bias, T* __restrict__ dx, float* parts,
+                                                            const float* __restrict__ w, const float* __restrict__ bias, T* __restrict__ dx,
+                                                            float* parts,
                                                             const Shape s, const Plan p, float2* between) {
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ __align__(16) float part[2][2 * kTileThreads];
@@ -381,7 +384,8 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
 // Wide groups: a block per sample and group, in two passes
 template <typename T, typename U, int ACT>
 __global__ void __launch_bounds__(256) wide_kernel(const U* __restrict__ gy, const T* __restrict__ x, const float2* __restrict__ stats,
-                                                   const float* __restrict__ w, const float* __restrict__ bias, T* __restrict__ dx, const Shape s) {
+                                                   const float* __restrict__ w, const float* __restrict__ bias, T* __restrict__ dx,
+                                                   const Shape s) {
   __shared__ float red[8];
   const int cg = s.C / s.G;
   const int64_t n = s.N * cg;
@@ -416,7 +420,8 @@ __global__ void __launch_bounds__(256) wide_kernel(const U* __restrict__ gy, con
 template <typename T, typename U, int ACT>
 __global__ void __launch_bounds__(256) wide_channels_kernel(const U* __restrict__ gy, const T* __restrict__ x,
                                                             const float2* __restrict__ stats,
-                                                            const float* __restrict__ w, const float* __restrict__ bias, float* __restrict__ parts, const Shape s) {
+                                                            const float* __restrict__ w, const float* __restrict__ bias, float* __restrict__ parts,
+                                                            const Shape s) {
   const int c = blockIdx.x * 256 + threadIdx.x;
   if (c >= s.C) return;
   const int g = c / (s.C / s.G);

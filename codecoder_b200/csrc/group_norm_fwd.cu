@@ -9,7 +9,7 @@
 // mean of the squared differences from the mean, never a difference of squares, and the parts of several blocks join as
 // var n = sum (var_i n_i + n_i (mean_i - mean)^2).
 //   512 x 504 x 512 fp32 into bf16 with 32 groups and SiLU: 158 us, 5.0 TB/s of 793 MB; 1.36 M samples of 96 bf16 channels in 3
-// groups: 116 us, 4.5 TB/s.  Bound by instructions and the latency of the two joins of a sample as much as by memory: on
+// groups: 110 us, 4.8 TB/s.  Bound by instructions and the latency of the two joins of a sample as much as by memory: on
 // pairs of values, with the rows that are all there told apart from those that are not, a tile takes half of what it took (34 -> 16 M
 // instructions for 96 shots).  64 samples of 2,197 x 128 fp32 in one group each fit no cluster: 45 us with x read twice, the
 // second time mostly from L2.
@@ -25,7 +25,8 @@ namespace cg_ = cooperative_groups;
 // the next samples' are on their way while one is worked on.
 template <typename T, typename U, int ACT, int VEC, int SLOTS>
 __global__ void __launch_bounds__(kUnitThreads) units_kernel(const T* __restrict__ x, U* __restrict__ y, float2* stats,
-                                                             const float* __restrict__ w, const float* __restrict__ bias, const Shape s, const Plan p, float eps) {
+                                                             const float* __restrict__ w, const float* __restrict__ bias, const Shape s, const Plan p,
+                                                             float eps) {
   constexpr int kP = Pack<T, VEC>::kPairs;
   const int cg = s.C / s.G, across = cg / VEC;
   const int unit = threadIdx.x / p.lanes, l = threadIdx.x % p.lanes;
@@ -123,7 +124,8 @@ enum Mode { kFused, kStats, kApply };
 // and summed squared differences between the two kernels of samples that no cluster holds.
 template <typename T, typename U, int ACT, int VEC, int MODE>
 __global__ void __launch_bounds__(kTileThreads, 3) tiles_kernel(const T* __restrict__ x, U* __restrict__ y, float2* stats,
-                                                               const float* __restrict__ w, const float* __restrict__ bias, const Shape s, const Plan p, float eps,
+                                                               const float* __restrict__ w, const float* __restrict__ bias, const Shape s, const Plan p,
+                                                               float eps,
                                                                float2* parts) {
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ __align__(16) float part[2][kTileThreads];

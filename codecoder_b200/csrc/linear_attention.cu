@@ -590,9 +590,10 @@ __device__ __forceinline__ void zero_rows(T* out, int64_t stride, int slice, int
 
 // A group of warps takes an item at a time, chunk by chunk, each warp some columns of c; the state stays in the warps'
 // registers.  Twelve warps an SM, whose dependent products and conversions bound it: 30,011 positions x 12 bf16 heads of 64
-// take 84 us (184 MB: 28 at the copy's rate), the tensor unit a quarter busy, 0.44 instructions a cycle and scheduler.  16
-// columns a warp and three blocks an SM against 32 and two: 115 us.  Chunks of 16 positions read and cut the state twice as often;
-// the state read as tf32 (11 bits) would save the cutting, and show in the result.  The tiles of the next chunks, of the next items too, are on their way meanwhile.  REV: backwards in time.
+// take 85 us (184 MB: 28 at the copy's rate), the tensor unit 40 % busy, 0.48 instructions a cycle and scheduler.  16
+// columns a warp and three blocks an SM against 32 and two: 115 us.  Chunks of 16 positions read and cut the state twice as
+// often; the state read as tf32 (11 bits) would save the cutting, and show in the result.  The tiles of the next chunks, of
+// the next items too, are on their way meanwhile.  REV: backwards in time.
 // OUT false: the states that the segments leave behind alone.
 template <typename T, int DP, bool REV, bool OUT, int SPLIT>
 __global__ void __launch_bounds__(Tile<T, DP>::kThreads, Tile<T, DP>::kBlocks) scan_kernel(const __grid_constant__ Scans all) {
@@ -814,7 +815,8 @@ struct Piece {
       for (int k = 0; k < kWords / kWide; ++k) {
         T* at = row + (g + 8 * h) * stride + column(k);
         if (g + 8 * h < until && column(k) < dim) {
-          if constexpr (kWide == 4) *reinterpret_cast<uint4*>(at) = make_uint4(r[h][4 * k], r[h][4 * k + 1], r[h][4 * k + 2], r[h][4 * k + 3]);
+          if constexpr (kWide == 4)
+            *reinterpret_cast<uint4*>(at) = make_uint4(r[h][4 * k], r[h][4 * k + 1], r[h][4 * k + 2], r[h][4 * k + 3]);
           else *reinterpret_cast<uint2*>(at) = make_uint2(r[h][2 * k], r[h][2 * k + 1]);
         }
       }
@@ -880,8 +882,10 @@ __device__ __forceinline__ Piece<T, DP, HALVES> attend(const Piece<T, DP, HALVES
   if constexpr (P_::kF32) {
     Split p[HALVES][4];
 #pragma unroll
-    for (int n = 0; n < HALVES; ++n)
-      p[n][0] = Split(P[n][0]), p[n][1] = Split(HALVES == 2 ? P[n][2] : 0.0f), p[n][2] = Split(P[n][1]), p[n][3] = Split(HALVES == 2 ? P[n][3] : 0.0f);
+    for (int n = 0; n < HALVES; ++n) {
+      p[n][0] = Split(P[n][0]), p[n][1] = Split(HALVES == 2 ? P[n][2] : 0.0f);
+      p[n][2] = Split(P[n][1]), p[n][3] = Split(HALVES == 2 ? P[n][3] : 0.0f);
+    }
 #pragma unroll
     for (int q = 0; q < P_::kWords / 2; ++q) {
       float O[4] = {};
@@ -893,7 +897,8 @@ __device__ __forceinline__ Piece<T, DP, HALVES> attend(const Piece<T, DP, HALVES
         mma_f32(O, p[n], Split(__uint_as_float(__byte_perm(lo, hi, 0x5410))), Split(__uint_as_float(__byte_perm(lo, hi, 0x7632))));
       }
       out.r[0][2 * q] = keep0 ? __float_as_uint(O[0]) : 0u, out.r[0][2 * q + 1] = keep0 ? __float_as_uint(O[1]) : 0u;
-      if (HALVES == 2) out.r[kLast][2 * q] = keep1 ? __float_as_uint(O[2]) : 0u, out.r[kLast][2 * q + 1] = keep1 ? __float_as_uint(O[3]) : 0u;
+      if (HALVES == 2)
+        out.r[kLast][2 * q] = keep1 ? __float_as_uint(O[2]) : 0u, out.r[kLast][2 * q + 1] = keep1 ? __float_as_uint(O[3]) : 0u;
     }
   } else {
     // the weighted products as two bf16 parts: one would round as coarsely as the result

@@ -165,9 +165,10 @@ BPC_API int bpc_embed_wgrad(const void* gy, const void* ids, int32_t id_bytes, v
  *   backward: dx, dw, db of sum(gy * y)
  * x: samples x_sample_stride and rows x_row_stride elements apart, channels contiguous, f32, bf16 or f16; y (B, N, C)
  * contiguous, x's type or, for f32 x, a narrower one; stats (B, G, 2) fp32, 8-byte aligned: each group's mean
- * and 1 / sqrt(var + eps), written by the forward pass (or NULL), read by the backward pass; weight, bias (C) fp32 or NULL (1, 0).  gy: y's type, any strides as x; dx (B, N, C)
- * contiguous, x's type; dw, db (C) fp32; NULL where a gradient is not wanted.  Statistics and sums are fp32 or wider, in
- * a fixed order (deterministic), each result rounded once.  N <= 2^30, C <= 2^20; every buffer aligned to its type.
+ * and 1 / sqrt(var + eps), written by the forward pass (or NULL), read by the backward pass; weight, bias (C) fp32 or
+ * NULL (1, 0).  gy: y's type, any strides as x; dx (B, N, C) contiguous, x's type; dw, db (C) fp32; NULL where a gradient
+ * is not wanted.  Statistics and sums are fp32 or wider, in a fixed order (deterministic), each result rounded once.  N
+ * <= 2^30, C <= 2^20; every buffer aligned to its type.
  * workspace: bpc_group_norm_workspace_size() bytes on the current device, 16-byte aligned. */
 enum { BPC_ACT_NONE = 0, BPC_ACT_SILU = 1, BPC_ACT_GELU = 2 };
 BPC_API size_t bpc_group_norm_workspace_size(int64_t B, int64_t N, int32_t C, int32_t G, int32_t x_dtype, int32_t backward);
@@ -191,12 +192,12 @@ BPC_API int bpc_group_norm_bwd(const void* gy, const void* x, const float* stats
  * head) element strides for q, k, v (and go) in turn, 0 where broadcast; for the step q, k (B, H, dk), v (B, H, dv) and
  * (batch, head) strides.  o, dv like v, dq, dk like q, contiguous, of the inputs' type.  log_decay (H) fp32, -infinity
  * forgets everything; no gradient of it is formed.  state, new_state, grad_state, dstate (B, H, dk, dv) fp32, 16-byte
- * aligned (4-byte for the step); a NULL state or grad_state is zero.  lengths (B) int32 or int64 (length_bytes 4 or 8) or NULL (T each): positions
- * at or behind a sequence's length are not read, and zero in o, dq, dk and dv.  1 <= dk, dv <= 128, B H < 2^30, T <= 2^30.  States,
- * products and sums are fp32, in a fixed order (deterministic).  new_state may be the state itself, else they do not
- * overlap.  workspace: bpc_linear_attention_workspace_size() bytes on the current device, 16-byte aligned; fwd_workspace: the
- * workspace of bpc_linear_attention_fwd on the same inputs, as it was left (another than workspace), or NULL: what it holds is
- * then formed again. */
+ * aligned (4-byte for the step); a NULL state or grad_state is zero.  lengths (B) int32 or int64 (length_bytes 4 or 8) or
+ * NULL (T each): positions at or behind a sequence's length are not read, and zero in o, dq, dk and dv.  1 <= dk, dv <=
+ * 128, B H < 2^30, T <= 2^30.  States, products and sums are fp32, in a fixed order (deterministic).  new_state may be
+ * the state itself, else they do not overlap.  workspace: bpc_linear_attention_workspace_size() bytes on the current
+ * device, 16-byte aligned; fwd_workspace: the workspace of bpc_linear_attention_fwd on the same inputs, as it was left
+ * (another than workspace), or NULL: what it holds is then formed again. */
 BPC_API size_t bpc_linear_attention_workspace_size(int64_t B, int64_t T, int32_t H, int32_t dk, int32_t dv, int32_t dtype,
                                                    int32_t backward);
 BPC_API int bpc_linear_attention_fwd(const void* q, const void* k, const void* v, void* o, const float* log_decay,
