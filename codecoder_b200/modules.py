@@ -266,6 +266,7 @@ class RoundMemory(nn.Module):
     The heads forget at fixed rates, from half to 2^-6 of their memory a round.  `out` starts at zero: the layer is the
     identity until it is trained.  forward takes whole experiments (lengths (B): rounds that each shot has, default all;
     positions behind are passed through), step one round, going on from the state that forward returns or start() makes.
+    q, k and v are fp32 or bf16: the layer runs in either, or under bf16 autocast; the state is fp32.
     No reference counterpart: the reference's networks see a fixed window of rounds."""
 
     def __init__(self, C, heads, sites, seed=0):
@@ -278,8 +279,16 @@ class RoundMemory(nn.Module):
             setattr(self, name, nn.Parameter((torch.rand(C, C, generator=g) * 2 - 1) / math.sqrt(C)))
         self.out = nn.Parameter(torch.zeros(C, C))
         self.norm = GroupNorm(C, heads, "silu")
-        decay = torch.log1p(-torch.exp2(-torch.linspace(1.0, 6.0, heads, dtype=torch.float64))).float()
-        self.register_buffer("log_decay", decay.repeat(sites), persistent=False)         # (sites, heads)
+        self.register_buffer("log_decay", self._rates(), persistent=False)         # (sites, heads)
+
+    def _rates(self):
+        return torch.log1p(-torch.exp2(-torch.linspace(1.0, 6.0, self.heads, dtype=torch.float64))).float().repeat(self.sites)
+
+    def _apply(self, fn, recurse=True):
+        super()._apply(fn, recurse)
+        if self.log_decay.dtype != torch.float32:       # a layer cast to another type keeps its rates
+            self.log_decay = self._rates().to(self.log_decay.device)
+        return self
 
     def _project(self, x, *lead):
         return (F.linear(x, w).view(*lead, self.sites * self.heads, self.D) for w in (self.q, self.k, self.v))
@@ -360,7 +369,10 @@ class CascadeBlock(nn.Module):
         return self.up(F.silu(self._bn(self.bn3, u)))
 
     def prepare_inference(self):
-        """Fold the BatchNorms and cast the weights once (call again after changing weights or statistics)."""
+        """Fold the BatchNorms and cast the weights once (call again after changing weights or statistics).  Nothing to do
+        with norm="group"."""
+        if self.norm == "group":
+            return self
         with torch.no_grad():
             a1, b1 = _fold_bn(self.bn1)
             a2, b2 = _fold_bn(self.bn2)

@@ -619,7 +619,8 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     differentiable; scale: dk^-0.5 by default; state (B, H, dk, dv) fp32: S before the first position (default: zero);
     lengths (B) int32 or int64: positions at or behind a sequence's length are not read, and zero in the result -> o
     (B, T, H, dv) in the inputs' type, and with return_state the state after each sequence's last position, which
-    linear_attention_step (or a next call) goes on from.  States and sums are fp32; the gradients of q, k, v and state are
+    linear_attention_step (or a next call) goes on from.  States and sums are fp32; a value that is not finite may show in the
+    results of up to 31 positions before its own too.  The gradients of q, k, v and state are
     deterministic; differentiable once."""
     if log_decay.requires_grad:
         raise ValueError("linear_attention: log_decay takes no gradient (detach it)")

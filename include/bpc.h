@@ -197,7 +197,8 @@ BPC_API int bpc_group_norm_bwd(const void* gy, const void* x, const float* stats
  * 128, B H < 2^30, T <= 2^30.  States, products and sums are fp32, in a fixed order (deterministic).  new_state may be
  * the state itself, else they do not overlap.  workspace: bpc_linear_attention_workspace_size() bytes on the current
  * device, 16-byte aligned; fwd_workspace: the workspace of bpc_linear_attention_fwd on the same inputs, as it was left
- * (another than workspace), or NULL: what it holds is then formed again. */
+ * (another than workspace), or NULL: what it holds is then formed again.  A value that is not finite may show in the results
+ * of up to 31 positions on either side of its own, besides those that it belongs to. */
 BPC_API size_t bpc_linear_attention_workspace_size(int64_t B, int64_t T, int32_t H, int32_t dk, int32_t dv, int32_t dtype,
                                                    int32_t backward);
 BPC_API int bpc_linear_attention_fwd(const void* q, const void* k, const void* v, void* o, const float* log_decay,

@@ -106,6 +106,11 @@ def test_round_memory_matches_the_recurrence(C, heads, S, T):
 
 
 def test_round_memory_of_experiments_of_different_lengths():
+    """A shot among others and by itself: products of other shapes, whose sums are rounded in another order.  q, k and v
+    (about 0.6) are sums of 32 products, sqrt(32) 2^-24 0.6 = 2e-7 apart, so o = sum of 16 q S / 4 is about
+    sqrt(16) / 4 3 2e-7 0.6^2 = 2e-7 apart.  The norm divides that by sqrt(var + eps), in a first round whose q is nearly
+    orthogonal to its k by no more than sqrt(eps) = 1 / 316: 6e-5, and the map back (16 such values, weights 1 / sqrt(32))
+    makes 4.5e-5 of it, or 1.3e-5 of max |y| = 3.5.  fp32 arithmetic on the CPU in two orders: up to 7e-6 in 60 draws."""
     m = make_memory(32, 2, 5, 3)
     x = torch.randn(4, 12, 5, 32, device=DEV)
     n = torch.tensor([12, 0, 5, 1], device=DEV)
@@ -114,8 +119,32 @@ def test_round_memory_of_experiments_of_different_lengths():
         assert torch.equal(y[b, k:], x[b, k:])          # nothing there: passed through
         if k:
             z, s = m(x[b:b + 1, :k], return_state=True)
-            assert rel(y[b, :k], z[0]) < 1e-6 and rel(state[b], s[0]) < 1e-6
+            assert rel(y[b, :k], z[0]) < 2e-5 and rel(state[b], s[0]) < 1e-6
     assert bool((state[1] == 0).all())
+
+
+def test_a_memory_in_bf16_keeps_its_rates():
+    """The layer cast to bf16 is its own operators on its bf16 weights with the rates in fp32, bit for bit.  (Against the fp32
+    layer no tolerance holds: the norm divides by what is left of q k, whose rounding is relative to |q| |k|.)"""
+    from codecoder_b200 import ops
+    m = make_memory(64, 2, 9, 5)
+    x = torch.randn(2, 20, 9, 64, device=DEV)
+    rates = m.log_decay.clone()
+    m.bfloat16()
+    assert torch.equal(m.log_decay, rates) and m.log_decay.device == rates.device
+    xb = x.bfloat16()
+    y, state = m(xb, return_state=True)
+    q, k, v = (F.linear(xb, w).view(2, 20, 18, 32) for w in (m.q, m.k, m.v))
+    o, want = ops.linear_attention(q, k, v, rates, return_state=True)
+    n = ops.group_norm(o.view(-1, 64), 2, m.norm.weight, m.norm.bias, activation="silu")
+    assert y.dtype == torch.bfloat16 and torch.equal(y, xb + F.linear(n, m.out).view(x.shape)) and torch.equal(state, want)
+    steps = m.start(2)
+    for t in range(20):
+        m.step(x[:, t].bfloat16(), steps)
+    # k and v of products of other shapes: a rounding apart in places, 2^-7 of a term; the terms' sum is a few times the largest
+    assert rel(steps, state) < 10 * 2**-8
+    with pytest.raises(TypeError, match="fp32 or bf16"):
+        m.half()(x.half())
 
 
 def test_a_new_memory_is_the_identity():

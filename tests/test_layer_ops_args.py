@@ -149,3 +149,16 @@ def test_python_refusals():
         ops.linear_attention_step(q[:, 0], q[:, 0], q[:, 0], torch.zeros(2), torch.zeros(2, 2, 4, 4))
     with pytest.raises(ValueError, match="gradient"):
         ops.linear_attention(q, q, q, torch.zeros(2, requires_grad=True))
+
+
+def test_layers_cast_and_prepared():
+    from codecoder_b200.geometry import RotatedSurface
+    from codecoder_b200.modules import CascadeBlock, RoundMemory
+    m = RoundMemory(32, 2, 5)
+    rates = m.log_decay.clone()
+    assert m.bfloat16().log_decay.dtype == torch.float32 and torch.equal(m.log_decay, rates)
+    assert m.q.dtype == torch.bfloat16 and m.double().q.dtype == torch.float64 and torch.equal(m.log_decay, rates)
+    kept = m.log_decay
+    assert m.to("cpu").log_decay is kept
+    blk = CascadeBlock(64, RotatedSurface(3, 3), 1, norm="group", groups=8)
+    assert blk.prepare_inference() is blk
