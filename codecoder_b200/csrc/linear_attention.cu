@@ -122,14 +122,13 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {
 __device__ __forceinline__ float low(uint32_t p) { return __uint_as_float(p << 16); }
 __device__ __forceinline__ float high(uint32_t p) { return __uint_as_float(p & 0xffff0000u); }
 
-// x to the nearest tf32 (11 significant bits), with bits behind them that a product does not read
-__device__ __forceinline__ uint32_t tf32(float x) { return __float_as_uint(x) + 0x1000u; }
-// x = hi + lo in tf32, but for 2^-23 of x
+// x = hi + lo in tf32 (11 significant bits), but for 2^-23 of x: hi is x to the nearest, what is left has 12 bits, of which
+// a product reads 11.  A NaN may carry over into hi's sign (0x7fffffff makes -0): lo, which is x less that, is NaN then.
 struct Split {
   uint32_t hi, lo;
   __device__ __forceinline__ explicit Split(float x) {
-    hi = tf32(x) & 0xffffe000u;
-    lo = tf32(x - __uint_as_float(hi));
+    hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+    lo = __float_as_uint(x - __uint_as_float(hi));
   }
   Split() = default;
 };

@@ -433,3 +433,43 @@ def test_refusals():
     both = torch.zeros(3, 3, 16, 16, device=DEV)
     with pytest.raises(RuntimeError, match="overlaps"):
         step(q[:, 0], k[:, 0], v[:, 0], g, both[:2], new_state=both[1:])
+
+
+NAN_BITS = {F32: (0x7fc00000, 0x7fffffff, -1, 0x7f800001), BF16: (0x7fc0, 0x7fff, -1, 0x7f81)}
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("T,at", [(1, 0), (5, 2), (12, 11), (16, 0), (40, 35), (100, 50), (700, 400)])
+@pytest.mark.parametrize("where", ["q", "k", "v", "go", "s0"])
+def test_values_that_are_not_finite_show(dtype, T, at, where):
+    """NaN of any bits, and infinities, in one element: not finite where the definition is not, and finite 32 positions and
+    more before (for o) or behind (for gradients) wherever the definition is."""
+    ints = {F32: torch.int32, BF16: torch.int16}
+    for n, bits in enumerate((*NAN_BITS[dtype], None)):
+        s = make(2, T, 2, 24, 40, dtype, 7 * T + n, state=where == "s0")
+        x = s[where]
+        if bits is None:
+            bad = torch.tensor(float("inf"), device=DEV, dtype=x.dtype)
+        else:
+            bits = NAN_BITS[x.dtype][n]
+            bad = torch.tensor(bits, device=DEV, dtype=ints[x.dtype]).view(x.dtype)
+        if where == "s0":
+            x[1, 1, 3, 5] = bad
+        else:
+            x[1, at, 1, 3] = bad
+        want = definition(s["q"], s["k"], s["v"], s["g"], 24**-0.5, s["s0"], None, s["go"], s["gs"])
+        leaves = [s[i].detach().requires_grad_() for i in ("q", "k", "v", "s0") if s[i] is not None]
+        o, S = ops.linear_attention(*leaves[:3], s["g"], None, leaves[3] if where == "s0" else None, return_state=True)
+        outs, gouts = ([o, S], [s["go"], s["gs"]]) if where == "s0" else ([o], [s["go"]])
+        grads = torch.autograd.grad(outs, leaves, gouts)
+        alone = ops.linear_attention(s["q"], s["k"], s["v"], s["g"], None, s["s0"])
+        far = (torch.arange(T, device=DEV) - at).abs()[:, None, None] >= 32
+        for what, a, b in (("o", o, want[0]), ("alone", alone, want[0]), *zip(("dq", "dk", "dv"), grads, want[2:5])):
+            lost = a.isfinite() & ~b.isfinite()
+            assert not bool(lost.any()), (what, n, int(lost.sum()))
+            spread = ~a.isfinite() & b.isfinite() & far
+            assert not bool(spread.any()), (what, n, int(spread.sum()))
+        assert not bool((S.isfinite() & ~want[1].isfinite()).any()), ("state", n)
+        if where == "s0":
+            assert not bool((grads[3].isfinite() & ~want[5].isfinite()).any()), ("dstate", n)
+
