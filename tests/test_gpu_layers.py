@@ -2,8 +2,11 @@
 compositions in 64 bits.
 
 Tolerances: relative to max |ref|; 1e-4 for fp32 networks and 5e-2 for gradients under bf16 autocast, as the networks' other
-tests (every stored activation and gradient is rounded to bf16 along the way).  A layer alone in fp32: 1e-5, a few hundred
-roundings of 2^-24 in sums of random signs."""
+tests (every stored activation and gradient is rounded to bf16 along the way).  A layer alone in fp32, and the operators as
+they are used together: 1e-4 behind the norm, 1e-5 for states.  The norm divides a head's result by its own deviation, which
+in a first round is |q k| and may be nearly nothing: plain fp32 arithmetic is off by up to 1.3e-5 in the gradients of these
+layers, and 3e-7 of o's root mean square (a third of 2^-24 sqrt(T + D) times the products of a product, the operator's usual
+error in fp32), put into the 64-bit composition as noise, makes 1.4e-5 of the results and 5.3e-5 of the gradients."""
 import os
 from dataclasses import replace
 
@@ -85,24 +88,24 @@ def test_round_memory_matches_the_recurrence(C, heads, S, T):
     gy = torch.randn(3, T, S, C, generator=torch.Generator().manual_seed(T + 1))
     xd, xr = x.to(DEV).requires_grad_(), x.double().requires_grad_()
     y, yr = m(xd), ref(xr)
-    assert rel(y, yr) < 1e-5
+    assert rel(y, yr) < 1e-4
     y.backward(gy.to(DEV))
     yr.backward(gy.double())
-    assert rel(xd.grad, xr.grad) < 1e-5
+    assert rel(xd.grad, xr.grad) < 1e-4
     for n, p in m.named_parameters():
-        assert rel(p.grad, dict(ref.named_parameters())[n].grad) < 1e-5, n
+        assert rel(p.grad, dict(ref.named_parameters())[n].grad) < 1e-4, n
     # a whole experiment, or its rounds one by one
     state = m.start(3)
     for t in range(T):
         z = m.step(xd.detach()[:, t], state)
-        assert rel(z, y[:, t]) < 1e-5
+        assert rel(z, y[:, t]) < 1e-4
     _, end = m(xd.detach(), return_state=True)
     assert rel(state, end) < 1e-5
     # or in two parts, with what the first leaves behind
     if T > 5:
         a, mid = m(xd.detach()[:, :5], return_state=True)
         b = m(xd.detach()[:, 5:], state=mid)
-        assert rel(torch.cat([a, b], 1), y) < 1e-5
+        assert rel(torch.cat([a, b], 1), y) < 1e-4
 
 
 def test_round_memory_of_experiments_of_different_lengths():
@@ -299,9 +302,9 @@ def test_a_run_of_the_operators_as_they_are_used_together():
     y64 = F.silu(((x - mean) / (var + 1e-5).sqrt()).reshape(B * T, H * D) * w64)
     go, gw = torch.autograd.grad(y64, (leaf, w64), gy.double())
     want = definition(q.detach(), k.detach(), v.detach(), decay, D**-0.5, None, None, go)
-    assert rel(y, y64) < 1e-5 and rel(state, s64) < 1e-5 and rel(grads[3], gw) < 1e-5
+    assert rel(y, y64) < 1e-4 and rel(state, s64) < 1e-5 and rel(grads[3], gw) < 1e-4
     for a, b in zip(grads, want[2:5]):
-        assert rel(a, b) < 2e-5
+        assert rel(a, b) < 1e-4
     # the next round goes on from there
     nxt = [torch.randn(B, H, D, generator=g, device=DEV) for _ in range(3)]
     o1 = ops.linear_attention_step(*nxt, decay, state.detach())
