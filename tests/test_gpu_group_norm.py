@@ -205,6 +205,36 @@ def test_special_values_stay_in_their_group(N, C, G):
     assert bool((ops.group_norm(const, G) == 0).all())              # no variance: eps keeps it finite
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("N,C,G", [(1, 64, 4), (1, 45, 5), (50, 64, 4), (2000, 64, 4), (20000, 16, 4), (2, 4096, 2)])
+def test_gradients_of_special_values_stay_in_their_group(N, C, G, dtype):
+    """NaN (of the bits that arithmetic makes, and of others) and infinities in x or gy: not finite in all of their group's dx
+    and their channels' dw, and elsewhere as they were."""
+    x, gy, w, b = make(5, N, C, dtype, dtype, True, N + C)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    clean = torch.autograd.grad(ops.group_norm(x, G, w, b, EPS, "silu"), leaves, gy)
+    zero = torch.zeros((), device=DEV)
+    made = (zero / zero).to(dtype)                      # 0x7fffffff
+    cg = C // G
+    bad, bad_g = x.detach().clone(), gy.clone()
+    bad[1, N // 2, cg] = float("inf")
+    bad[2, 0, 0] = made
+    bad_g[3, N - 1, C - 1] = made
+    bad_g[4, 0, C - 1] = -float("inf")
+    bad.requires_grad_()
+    got = torch.autograd.grad(ops.group_norm(bad, G, w, b, EPS, "silu"), [bad, w, b], bad_g)
+    touched = torch.zeros(5, 1, C, dtype=torch.bool, device=DEV)
+    touched[1, :, cg:2 * cg] = touched[2, :, :cg] = touched[3:, :, C - cg:] = True
+    rest = ~touched.expand_as(x)
+    assert torch.equal(got[0][rest], clean[0][rest])
+    assert not bool(got[0][2, :, :cg].isfinite().any()) and not bool(got[0][3:, :, C - cg:].isfinite().any())
+    channels = ~touched.any(0)[0]
+    for a_, b_ in zip(got[1:], clean[1:]):
+        assert torch.equal(a_[channels], b_[channels])
+        assert not bool(a_[C - 1].isfinite())
+    assert not bool(got[1][:cg].isfinite().any())
+
+
 def test_gradients_match_differences():
     torch.manual_seed(5)
     for N, C, G, act in ((1, 12, 2, "silu"), (9, 10, 5, "gelu"), (700, 4, 2, "silu")):
