@@ -765,7 +765,7 @@ __global__ void __launch_bounds__(256) join_kernel(const Scan p, int per) {     
 // number them as it likes, so a piece's words are operands as they lie; c's 8 x 8 pieces are transposed by the tensor
 // unit's move; and a result's columns come out where c's pieces had them, so that a lane stores the pieces it would load.
 // The forward pass reads three and writes one tensor, the backward pass reads four and writes three: no state, and nothing
-// twice.  Up to 8 positions (HALVES 1) take half of the work: 25,600 heads of 5 fp32 positions 31 -> 20 us.
+// twice.  Up to 8 positions (HALVES 1) take half of the work: 25,600 heads of 5 fp32 positions 31 -> 20 us, 18 with splits of one addition less.
 //   bf16 heads of 32 are bound by memory: 371,712 of 11 positions 182 us forwards (5.8 TB/s of 1.05 GB), 343 backwards (5.3 of
 // 1.84).  Through shared memory and the long sequences' kernel, at 833 instructions a head against 240, they took 500 us a scan;
 // a state's worth of registers cost the occupancy that hides the loads.
