@@ -439,7 +439,7 @@ __global__ void __launch_bounds__(256) wide_channels_kernel(const U* __restrict_
   parts[static_cast<int64_t>(blockIdx.y) * 2 * s.C + s.C + c] = static_cast<float>(d);
 }
 
-Plan plan_of(const Shape& s, int size, bool aligned) { return make_plan(s, size, num_sms(), aligned, true); }
+Plan plan_of(const Shape& s, int size, int y_size, bool aligned) { return make_plan(s, size, y_size, num_sms(), aligned, true); }
 
 constexpr int kTilesPerSm = 2;
 
@@ -458,13 +458,14 @@ int64_t parts_of(const Shape& s, const Plan& p) {
 
 size_t backward_workspace(const Shape& s, int size) {
   size_t bytes = 16;
-  for (bool aligned : {false, true}) {
-    const Plan p = plan_of(s, size, aligned);
-    size_t parts = sizeof(float) * 2 * static_cast<size_t>(s.C) * parts_of(s, p);
-    parts = (parts + 15) / 16 * 16;
-    if (p.kind == kTiles && !p.fused) parts += sizeof(float2) * static_cast<size_t>(s.B) * p.chunks * s.G;
-    bytes = std::max(bytes, parts);
-  }
+  for (int y_size : {2, size})                     // the gradients' type may be narrower
+    for (bool aligned : {false, true}) {
+      const Plan p = plan_of(s, size, y_size, aligned);
+      size_t parts = sizeof(float) * 2 * static_cast<size_t>(s.C) * parts_of(s, p);
+      parts = (parts + 15) / 16 * 16;
+      if (p.kind == kTiles && !p.fused) parts += sizeof(float2) * static_cast<size_t>(s.B) * p.chunks * s.G;
+      bytes = std::max(bytes, parts);
+    }
   return bytes;
 }
 
@@ -473,8 +474,7 @@ namespace {
 template <typename T, typename U, int ACT, int VEC, int SLOTS>
 int run_units(const U* gy, const T* x, const float2* stats, const float* w, const float* bias, T* dx, float* parts, const Shape& s,
               const Plan& p, cudaStream_t st) {
-  const int copies = kDepth * ((Copied<T, VEC>::kBytes + Copied<U, VEC>::kBytes) * SLOTS + 8);      // of a thread
-  const int smem = std::max(copies * p.threads, p.rows * static_cast<int>(s.N) * s.C * static_cast<int>(sizeof(float)));
+  const int smem = units_smem(p, s, sizeof(T), sizeof(U), true);
   Shape shape = s;
   Plan plan = p;
   void* args[] = {&gy, &x, &stats, &w, &bias, &dx, &parts, &shape, &plan};
@@ -546,7 +546,7 @@ extern "C" int bpc_group_norm_bwd(const void* gy, const void* x, const float* st
   };
   const bool whole = whole_of(x, x_sample_stride, x_row_stride, size) && whole_of(dx, 0, 0, size) &&
                      whole_of(gy, gy_sample_stride, gy_row_stride, y_size);
-  const Plan p = plan_of(s, size, whole);
+  const Plan p = plan_of(s, size, y_size, whole);
   const bool want = dw || db;
   const int e = with_types(x_dtype, y_dtype, [&](auto xt, auto yt) {
     return with_act(activation, [&](auto act) {

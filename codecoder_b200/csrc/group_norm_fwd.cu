@@ -302,7 +302,7 @@ __global__ void __launch_bounds__(256) wide_kernel(const T* __restrict__ x, U* _
   }
 }
 
-Plan plan_of(const Shape& s, int size, bool aligned) { return make_plan(s, size, num_sms(), aligned, false); }
+Plan plan_of(const Shape& s, int size, bool aligned) { return make_plan(s, size, size, num_sms(), aligned, false); }
 
 }  // namespace
 
@@ -329,7 +329,7 @@ int run_units(const T* x, U* y, float2* stats, const float* w, const float* bias
   const void* fn = p.slots == 1   ? reinterpret_cast<const void*>(&units_kernel<T, U, ACT, VEC, 1>)
                    : p.slots == 2 ? reinterpret_cast<const void*>(&units_kernel<T, U, ACT, VEC, 2>)
                                   : reinterpret_cast<const void*>(&units_kernel<T, U, ACT, VEC, 4>);
-  return launch(fn, dim3(grid), p.threads, 1, kDepth * Copied<T, VEC>::kBytes * p.slots * p.threads, st, args, "group_norm");
+  return launch(fn, dim3(grid), p.threads, 1, units_smem(p, s, sizeof(T), sizeof(U), false), st, args, "group_norm");
 }
 
 template <typename T, typename U, int ACT, int VEC>
