@@ -108,6 +108,9 @@ int gmm_pair_tile_shots();
 // CUDA-core path: fp32 (f32 = true) or bf16 storage, fp32 accumulation.  Any Ci, Co % 4 == 0, Co <= 256.
 int gmm_fma_launch(const GmmProblem& p, bool f32, cudaStream_t stream);
 
+// A runtime call or launch that was refused: the error code, with no error left behind for the thread's next check.
+int refused(const std::string& what, cudaError_t e);
+
 int num_sms();
 // Opt a kernel in to `bytes` of dynamic shared memory on the current device (once per device and kernel).
 int allow_smem(const void* fn, int bytes);
@@ -115,6 +118,9 @@ int allow_smem(const void* fn, int bytes);
 // calls pdl_wait before it reads what earlier kernels wrote), optionally as clusters of cluster_x CTAs.
 int launch_pdl(const void* fn, dim3 grid, dim3 block, size_t smem, cudaStream_t stream, void** args, int cluster_x,
                const char* what);
+
+// A plain launch, as clusters of cluster_x CTAs; opts in to the shared memory.
+int launch_clusters(const void* fn, dim3 grid, dim3 block, int smem, cudaStream_t stream, void** args, int cluster_x, const char* what);
 
 // cuTensorMapEncodeTiled through the runtime's driver entry point (null when the driver lacks it).
 PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder();

@@ -501,7 +501,7 @@ int launch_boundary(const void* x3, const void* w_up, const float* h, const Toke
   void* args[] = {&mX3, &mWup, &mWdn, &mH, &mHo, &mY, &a};
   cudaError_t le = cudaLaunchKernel(fn, dim3(static_cast<unsigned>(grid)), dim3(kBThreads), args, kSmemBytes,
                                     reinterpret_cast<cudaStream_t>(stream));
-  if (le != cudaSuccess) return fail(BPC_ERR_LAUNCH, std::string("cascade_boundary_kernel launch: ") + cudaGetErrorString(le));
+  if (le != cudaSuccess) return refused("cascade_boundary_kernel launch", le);
   return 0;
 }
 

@@ -1173,7 +1173,7 @@ int sort_cluster_rounds(const I* ids, int n, int V, int passes, int2* out, bool*
   *launched = cluster_fits(reinterpret_cast<const void*>(fn), lc);
   if (!*launched) return 0;
   const cudaError_t e = cudaLaunchKernelEx(&lc, fn, ids, n, V, passes, out);
-  return e == cudaSuccess ? 0 : fail(BPC_ERR_LAUNCH, std::string("sort_cluster_kernel launch: ") + cudaGetErrorString(e));
+  return e == cudaSuccess ? 0 : refused("sort_cluster_kernel launch", e);
 }
 
 template <typename I>

@@ -734,7 +734,7 @@ int gmm_pair_launch(const GmmProblem& p, const GmmMaps& maps, const int32_t* typ
   lc.numAttrs = 1;
   void* args[] = {const_cast<CUtensorMap*>(&maps.x), const_cast<CUtensorMap*>(&maps.w), &a};
   cudaError_t le = cudaLaunchKernelExC(&lc, reinterpret_cast<const void*>(fn), args);
-  if (le != cudaSuccess) return fail(4, std::string("gmm_pair_kernel launch: ") + cudaGetErrorString(le));
+  if (le != cudaSuccess) return refused("gmm_pair_kernel launch", le);
   return 0;
 }
 

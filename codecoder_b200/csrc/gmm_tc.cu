@@ -26,11 +26,8 @@
 // Every wait is bounded (mbar_wait); a timeout sets the status word and the CTA drains and returns.
 #include <algorithm>
 #include <cstdio>
-#include <map>
 #include <mutex>
 #include <string>
-#include <set>
-#include <utility>
 
 #include <cudaTypedefs.h>
 
@@ -995,59 +992,6 @@ const void* wide_kernel_for(bool blocked, int epi, bool head, int Ci) {
 
 }  // namespace
 
-int allow_smem(const void* fn, int bytes) {
-  // the attribute is per device and kernel: remember the size set for each (device, kernel) pair and raise it when
-  // a launch needs more
-  static std::mutex mu;
-  static std::map<std::pair<int, const void*>, int> configured;
-  int dev = 0;
-  cudaGetDevice(&dev);
-  std::lock_guard<std::mutex> lk(mu);
-  auto it = configured.find({dev, fn});
-  if (it != configured.end() && it->second >= bytes) return 0;
-  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e != cudaSuccess) return fail(4, std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(e));
-  configured[{dev, fn}] = bytes;
-  return 0;
-}
-
-int launch_pdl(const void* fn, dim3 grid, dim3 block, size_t smem, cudaStream_t stream, void** args, int cluster_x,
-               const char* what) {
-  cudaLaunchConfig_t lc = {};
-  lc.gridDim = grid;
-  lc.blockDim = block;
-  lc.dynamicSmemBytes = smem;
-  lc.stream = stream;
-  cudaLaunchAttribute attr[2];
-  int n = 0;
-  attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[n].val.programmaticStreamSerializationAllowed = 1;
-  ++n;
-  if (cluster_x > 1) {
-    attr[n].id = cudaLaunchAttributeClusterDimension;
-    attr[n].val.clusterDim.x = static_cast<unsigned>(cluster_x);
-    attr[n].val.clusterDim.y = 1;
-    attr[n].val.clusterDim.z = 1;
-    ++n;
-  }
-  lc.attrs = attr;
-  lc.numAttrs = n;
-  cudaError_t e = cudaLaunchKernelExC(&lc, fn, args);
-  if (e != cudaSuccess) return fail(4, std::string(what) + " launch: " + cudaGetErrorString(e));
-  return 0;
-}
-
-int num_sms() {
-  static int n = 0;
-  if (n == 0) {
-    int dev = 0;
-    cudaGetDevice(&dev);
-    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-    if (n <= 0) n = 1;
-  }
-  return n;
-}
-
 int gmm_tc_check(const GmmProblem& p) {
   if (p.Ci < 64 || p.Ci % 8 != 0) return fail(2, "tcgen05 path needs C_in >= 64 and a multiple of 8");
   if (p.Co < 32 || p.Co > 256 || p.Co % 32 != 0) return fail(2, "tcgen05 path needs C_out in 32..256, multiple of 32");
@@ -1171,7 +1115,7 @@ int gmm_tc_launch(const GmmProblem& p, const GmmMaps& maps, int* status, uint64_
     void* args[] = {const_cast<CUtensorMap*>(&maps.x), const_cast<CUtensorMap*>(&maps.w), &a};
     cudaError_t le = cudaLaunchKernel(wf, dim3(static_cast<unsigned>(grid)),
                                       dim3(kThreads), args, static_cast<size_t>(wsmem), stream);
-    if (le != cudaSuccess) return fail(4, std::string("gmm_wide_kernel launch: ") + cudaGetErrorString(le));
+    if (le != cudaSuccess) return refused("gmm_wide_kernel launch", le);
     return 0;
   }
   const int smem = smem_bytes_for(p.Co, a.stages);
@@ -1182,7 +1126,7 @@ int gmm_tc_launch(const GmmProblem& p, const GmmMaps& maps, int* status, uint64_
   void* args[] = {const_cast<CUtensorMap*>(&maps.x), const_cast<CUtensorMap*>(&maps.w), &a};
   cudaError_t le = cudaLaunchKernel(reinterpret_cast<const void*>(fn), dim3(static_cast<unsigned>(grid)),
                                     dim3(kThreads), args, static_cast<size_t>(smem), stream);
-  if (le != cudaSuccess) return fail(4, std::string("gmm_tc_kernel launch: ") + cudaGetErrorString(le));
+  if (le != cudaSuccess) return refused("gmm_tc_kernel launch", le);
   return 0;
 }
 

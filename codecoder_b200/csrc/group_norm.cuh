@@ -284,25 +284,6 @@ inline int launched(const char* what) {
   return e == cudaSuccess ? 0 : fail(BPC_ERR_LAUNCH, std::string(what) + " launch: " + cudaGetErrorString(e));
 }
 
-// One launch, as clusters of `cluster` blocks
-inline int launch(const void* fn, dim3 grid, int threads, int cluster, int smem, cudaStream_t s, void** args, const char* what) {
-  if (smem > 32 * 1024)          // beside a few KB of static memory
-    if (int e = allow_smem(fn, smem)) return e;
-  cudaLaunchConfig_t lc = {};
-  lc.gridDim = grid;
-  lc.blockDim = dim3(threads);
-  lc.dynamicSmemBytes = smem;
-  lc.stream = s;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = cluster;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  lc.attrs = at;
-  lc.numAttrs = cluster > 1 ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelExC(&lc, fn, args);
-  return e == cudaSuccess ? 0 : fail(BPC_ERR_LAUNCH, std::string(what) + " launch: " + cudaGetErrorString(e));
-}
-
 // Blocks of x, y: every slab and chunk, and the samples that a slab's blocks walk at once; `per_sm` blocks of 256 threads
 inline dim3 tiles_grid(const Shape& s, const Plan& p, int per_sm, int sms) {
   const int64_t across = static_cast<int64_t>(p.slabs) * p.chunks;

@@ -478,8 +478,8 @@ int run_units(const U* gy, const T* x, const float2* stats, const float* w, cons
   Shape shape = s;
   Plan plan = p;
   void* args[] = {&gy, &x, &stats, &w, &bias, &dx, &parts, &shape, &plan};
-  return launch(reinterpret_cast<const void*>(&units_kernel<T, U, ACT, VEC, SLOTS>), dim3(static_cast<unsigned>(parts_of(s, p))), p.threads,
-                1, smem, st, args, "group_norm backward");
+  return launch_clusters(reinterpret_cast<const void*>(&units_kernel<T, U, ACT, VEC, SLOTS>), dim3(static_cast<unsigned>(parts_of(s, p))),
+                         dim3(p.threads), smem, st, args, 1, "group_norm backward");
 }
 
 template <typename T, typename U, int ACT, int VEC>
@@ -494,10 +494,10 @@ int run_tiles(const U* gy, const T* x, const float2* stats, const float* w, cons
   const int smem = std::max(Ahead<T, VEC, kRows>::kBytes + Ahead<U, VEC, kRows>::kBytes, VEC * static_cast<int>(sizeof(float))) * kTileThreads;
   const dim3 grid = tiles_grid(s, p, kTilesPerSm, num_sms());
   if (p.fused)
-    return launch(reinterpret_cast<const void*>(&tiles_kernel<T, U, ACT, VEC, kFused>), grid, p.threads, p.chunks, smem, st, args, what);
-  if (int e = launch(reinterpret_cast<const void*>(&tiles_kernel<T, U, ACT, VEC, kSums>), grid, p.threads, 1, smem, st, args, what)) return e;
+    return launch_clusters(reinterpret_cast<const void*>(&tiles_kernel<T, U, ACT, VEC, kFused>), grid, dim3(p.threads), smem, st, args, p.chunks, what);
+  if (int e = launch_clusters(reinterpret_cast<const void*>(&tiles_kernel<T, U, ACT, VEC, kSums>), grid, dim3(p.threads), smem, st, args, 1, what)) return e;
   if (!dx) return 0;
-  return launch(reinterpret_cast<const void*>(&tiles_kernel<T, U, ACT, VEC, kApply>), grid, p.threads, 1, smem, st, args, what);
+  return launch_clusters(reinterpret_cast<const void*>(&tiles_kernel<T, U, ACT, VEC, kApply>), grid, dim3(p.threads), smem, st, args, 1, what);
 }
 
 }  // namespace

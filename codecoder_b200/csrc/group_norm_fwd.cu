@@ -329,7 +329,7 @@ int run_units(const T* x, U* y, float2* stats, const float* w, const float* bias
   const void* fn = p.slots == 1   ? reinterpret_cast<const void*>(&units_kernel<T, U, ACT, VEC, 1>)
                    : p.slots == 2 ? reinterpret_cast<const void*>(&units_kernel<T, U, ACT, VEC, 2>)
                                   : reinterpret_cast<const void*>(&units_kernel<T, U, ACT, VEC, 4>);
-  return launch(fn, dim3(grid), p.threads, 1, units_smem(p, s, sizeof(T), sizeof(U), false), st, args, "group_norm");
+  return launch_clusters(fn, dim3(grid), dim3(p.threads), units_smem(p, s, sizeof(T), sizeof(U), false), st, args, 1, "group_norm");
 }
 
 template <typename T, typename U, int ACT, int VEC>
@@ -343,10 +343,10 @@ int run_tiles(const T* x, U* y, float2* stats, const float* w, const float* bias
   const dim3 grid = tiles_grid(s, p, 3, num_sms());
   const int smem = Ahead<T, VEC, kRows>::kBytes * kTileThreads;
   if (p.fused)
-    return launch(reinterpret_cast<const void*>(&tiles_kernel<T, U, ACT, VEC, kFused>), grid, p.threads, p.chunks, smem, st, args, what);
-  if (int e = launch(reinterpret_cast<const void*>(&tiles_kernel<T, U, BPC_ACT_NONE, VEC, kStats>), grid, p.threads, 1, smem, st, args, what))
+    return launch_clusters(reinterpret_cast<const void*>(&tiles_kernel<T, U, ACT, VEC, kFused>), grid, dim3(p.threads), smem, st, args, p.chunks, what);
+  if (int e = launch_clusters(reinterpret_cast<const void*>(&tiles_kernel<T, U, BPC_ACT_NONE, VEC, kStats>), grid, dim3(p.threads), smem, st, args, 1, what))
     return e;
-  return launch(reinterpret_cast<const void*>(&tiles_kernel<T, U, ACT, VEC, kApply>), grid, p.threads, 1, smem, st, args, what);
+  return launch_clusters(reinterpret_cast<const void*>(&tiles_kernel<T, U, ACT, VEC, kApply>), grid, dim3(p.threads), smem, st, args, 1, what);
 }
 
 }  // namespace

@@ -1168,7 +1168,7 @@ int blocks_of(const void* fn, int* cached, int* blocks) {
   if (!*cached) {
     int n = 0;
     const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, fn, kThreads, 0);
-    if (e != cudaSuccess || n < 1) return fail(BPC_ERR_LAUNCH, std::string("linear_attention occupancy: ") + cudaGetErrorString(e));
+    if (e != cudaSuccess || n < 1) return refused("linear_attention occupancy", e);
     *cached = n;
   }
   *blocks = *cached;

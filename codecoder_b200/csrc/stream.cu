@@ -1165,8 +1165,7 @@ int launch_one_cluster(bpc_stream* s, void** args) {
     return 1;
   }
   const cudaError_t le = cudaLaunchKernelExC(&lc, fn, args);
-  if (le != cudaSuccess)
-    return fail(BPC_ERR_LAUNCH, std::string("one-cluster stream kernel launch: ") + cudaGetErrorString(le));
+  if (le != cudaSuccess) return refused("one-cluster stream kernel launch", le);
   return 0;
 }
 
@@ -1225,10 +1224,9 @@ extern "C" int bpc_stream_start(bpc_stream* s) {
     if (cudaOccupancyMaxActiveClusters(&max_clusters, reinterpret_cast<const void*>(&stream_kernel), &lc) !=
             cudaSuccess ||
         max_clusters < kSClusters)
-      return fail(BPC_ERR_LAUNCH, std::string("stream kernel: 8 resident clusters not available (") +
-                                      cudaGetErrorString(le) + ")");
+      return refused("stream kernel: 8 resident clusters not available", le);
     le = cudaLaunchKernelExC(&lc, reinterpret_cast<const void*>(&stream_kernel), args);
-    if (le != cudaSuccess) return fail(BPC_ERR_LAUNCH, std::string("stream kernel launch: ") + cudaGetErrorString(le));
+    if (le != cudaSuccess) return refused("stream kernel launch", le);
   }
   s->running_layout = BPC_STREAM_CLUSTERS;
   return wait_ready(s);
