@@ -1245,6 +1245,12 @@ int check_common(const std::string& what, int64_t B, int64_t T, int32_t H, int32
   return 0;
 }
 
+// Whether two states of `count` values share memory
+bool overlap(const void* a, const void* b, int64_t count) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(a), to = reinterpret_cast<uintptr_t>(b), bytes = sizeof(float) * static_cast<uintptr_t>(count);
+  return a && b && at < to + bytes && to < at + bytes;
+}
+
 Rows rows_of(const void* p, const int64_t* s) { return {p, s[0], s[1], s[2]}; }
 
 }  // namespace
@@ -1272,6 +1278,8 @@ extern "C" int bpc_linear_attention_fwd(const void* q, const void* k, const void
   if (!aligned(q, size) || !aligned(k, size) || !aligned(v, size) || !aligned(o, size) || !aligned(state, 16) ||
       !aligned(new_state, 16) || !aligned(workspace, 16))
     return fail(BPC_ERR_ARG, "linear_attention: buffer not aligned to its type (states and workspace: 16 bytes)");
+  // a block may write a sequence's last state before another has read its first
+  if (overlap(state, new_state, B * H * dk * dv)) return fail(BPC_ERR_ARG, "linear_attention: new_state overlaps state");
   if (workspace_bytes < bpc_linear_attention_workspace_size(B, T, H, dk, dv, dtype, 0))
     return fail(BPC_ERR_SPACE, "linear_attention: workspace too small");
   const Rows rq = rows_of(q, strides), rk = rows_of(k, strides + 3), rv = rows_of(v, strides + 6);
@@ -1301,6 +1309,8 @@ extern "C" int bpc_linear_attention_bwd(const void* q, const void* k, const void
     if (!aligned(b, size)) return fail(BPC_ERR_ARG, "linear_attention backward: buffer not aligned to its type");
   if (!aligned(state, 16) || !aligned(grad_state, 16) || !aligned(dstate, 16) || !aligned(workspace, 16) || !aligned(fwd_workspace, 16))
     return fail(BPC_ERR_ARG, "linear_attention backward: buffer not aligned to its type (states and workspace: 16 bytes)");
+  if (overlap(grad_state, dstate, B * H * dk * dv) || overlap(state, dstate, B * H * dk * dv))
+    return fail(BPC_ERR_ARG, "linear_attention backward: dstate overlaps state or grad_state");
   if (workspace_bytes < bpc_linear_attention_workspace_size(B, T, H, dk, dv, dtype, 1))
     return fail(BPC_ERR_SPACE, "linear_attention backward: workspace too small");
   const Rows rq = rows_of(q, strides), rk = rows_of(k, strides + 3), rv = rows_of(v, strides + 6), rg = rows_of(go, strides + 9);
@@ -1333,9 +1343,7 @@ extern "C" int bpc_linear_attention_step(const void* q, const void* k, const voi
   if (!q || !k || !v || !o || !state || !new_state) return fail(BPC_ERR_ARG, "linear_attention_step: null buffer");
   if (!aligned(q, size) || !aligned(k, size) || !aligned(v, size) || !aligned(o, size) || !aligned(state, 4) || !aligned(new_state, 4))
     return fail(BPC_ERR_ARG, "linear_attention_step: buffer not aligned to its type");
-  const uintptr_t at = reinterpret_cast<uintptr_t>(state), to = reinterpret_cast<uintptr_t>(new_state);
-  const uintptr_t bytes = sizeof(float) * static_cast<uintptr_t>(B) * H * dk * dv;
-  if (at != to && at < to + bytes && to < at + bytes)
+  if (state != new_state && overlap(state, new_state, B * H * dk * dv))
     return fail(BPC_ERR_ARG, "linear_attention_step: new_state overlaps state (give the same buffer to update it in place)");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const Step p{q, k, v, o, log_decay, state, new_state, static_cast<uint32_t>(B * H), H, dk, dv,

@@ -169,7 +169,8 @@ BPC_API int bpc_embed_wgrad(const void* gy, const void* ids, int32_t id_bytes, v
  * NULL (1, 0).  gy: y's type, any strides as x; dx (B, N, C) contiguous, x's type; dw, db (C) fp32; NULL where a gradient
  * is not wanted.  Statistics and sums are fp32 or wider, in a fixed order (deterministic), each result rounded once.  N
  * <= 2^30, C <= 2^20; every buffer aligned to its type.
- * workspace: bpc_group_norm_workspace_size() bytes on the current device, 16-byte aligned. */
+ * No buffer that is written overlaps another.  workspace: bpc_group_norm_workspace_size() bytes on the current device, 16-byte
+ * aligned. */
 enum { BPC_ACT_NONE = 0, BPC_ACT_SILU = 1, BPC_ACT_GELU = 2 };
 BPC_API size_t bpc_group_norm_workspace_size(int64_t B, int64_t N, int32_t C, int32_t G, int32_t x_dtype, int32_t backward);
 BPC_API int bpc_group_norm_fwd(const void* x, void* y, float* stats, const float* weight, const float* bias,
@@ -194,11 +195,12 @@ BPC_API int bpc_group_norm_bwd(const void* gy, const void* x, const float* stats
  * forgets everything; no gradient of it is formed.  state, new_state, grad_state, dstate (B, H, dk, dv) fp32, 16-byte
  * aligned (4-byte for the step); a NULL state or grad_state is zero.  lengths (B) int32 or int64 (length_bytes 4 or 8) or
  * NULL (T each): positions at or behind a sequence's length are not read, and zero in o, dq, dk and dv.  1 <= dk, dv <=
- * 128, B H < 2^30, T <= 2^30.  States, products and sums are fp32, in a fixed order (deterministic).  new_state may be
- * the state itself, else they do not overlap.  workspace: bpc_linear_attention_workspace_size() bytes on the current
- * device, 16-byte aligned; fwd_workspace: the workspace of bpc_linear_attention_fwd on the same inputs, as it was left
- * (another than workspace), or NULL: what it holds is then formed again.  A value that is not finite may show in the results
- * of up to 31 positions on either side of its own, besides those that it belongs to. */
+ * 128, B H < 2^30, T <= 2^30.  States, products and sums are fp32, in a fixed order (deterministic).  No buffer that is
+ * written overlaps another, but the step's new_state may be the state itself; states that overlap otherwise are refused.
+ * workspace: bpc_linear_attention_workspace_size() bytes on the current device, 16-byte aligned; fwd_workspace: the workspace
+ * of bpc_linear_attention_fwd on the same inputs, as it was left (another than workspace), or NULL: what it holds is then
+ * formed again.  A value that is not finite may show in the results of up to 31 positions on either side of its own, besides
+ * those that it belongs to. */
 BPC_API size_t bpc_linear_attention_workspace_size(int64_t B, int64_t T, int32_t H, int32_t dk, int32_t dv, int32_t dtype,
                                                    int32_t backward);
 BPC_API int bpc_linear_attention_fwd(const void* q, const void* k, const void* v, void* o, const float* log_decay,
