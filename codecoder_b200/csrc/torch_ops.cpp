@@ -10,6 +10,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 #include <torch/extension.h>
 
@@ -251,6 +252,14 @@ Tensor clip_grads(const py::list& ts, double max_norm, const std::optional<py::l
   return norm;
 }
 
+// What would be lost without a word: the kernels have no forward-mode derivative, and a trace would keep their result as a
+// constant.  Undefined tensors carry nothing.
+void check_followed(const char* what, std::initializer_list<const Tensor*> inputs) {
+  for (const Tensor* t : inputs)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), what, " has no forward-mode derivative");
+  TORCH_CHECK(!torch::jit::tracer::isTracing(), what, " cannot be traced: its result would be a constant of the trace");
+}
+
 // x (B, ..., C) as (B, N, C) with contiguous channels; copies only where the layout asks for it
 Tensor samples_of(const Tensor& x_in) {
   Tensor x = x_in.resolve_neg();
@@ -464,6 +473,7 @@ Tensor linear_attention_step(const Tensor& q_in, const Tensor& k_in, const Tenso
                              const Tensor& state, double scale, const std::optional<Tensor>& new_state) {
   at::NoGradGuard no_grad;
   const char* what = "linear_attention_step";
+  check_followed(what, {&q_in, &k_in, &v_in, &log_decay, &state});
   const int32_t code = check_heads(q_in, k_in, v_in, log_decay, 3, what);
   const Tensor& to = new_state ? *new_state : state;
   for (const Tensor* s : {&state, &to}) {
@@ -538,6 +548,8 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
 
 Tensor group_norm(const Tensor& x, int64_t groups, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias,
                   double eps, int64_t activation, std::optional<at::ScalarType> dtype) {
+  const Tensor none;
+  check_followed("group_norm", {&x, weight ? &*weight : &none, bias ? &*bias : &none});
   if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(weight) || wants_grad(bias)))
     return GroupNorm::apply(x, groups, weight, bias, eps, activation, dtype);
   return std::get<0>(group_norm_fwd(x, groups, weight, bias, eps, activation, dtype, false));
@@ -574,6 +586,8 @@ struct LinearAttention : torch::autograd::Function<LinearAttention> {
 std::tuple<Tensor, Tensor> linear_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, double scale,
                                             const std::optional<Tensor>& state, const std::optional<Tensor>& lengths,
                                             bool want_state) {
+  const Tensor none;
+  check_followed("linear_attention", {&q, &k, &v, &log_decay, state ? &*state : &none});
   if (at::GradMode::is_enabled() && (wants_grad(q) || wants_grad(k) || wants_grad(v) || wants_grad(state))) {
     const variable_list r = LinearAttention::apply(q, k, v, log_decay, scale, state, lengths, want_state);
     return {r[0], want_state ? r[1] : Tensor()};

@@ -605,7 +605,7 @@ def group_norm(x: torch.Tensor, groups: int, weight: torch.Tensor | None = None,
     x (B, ..., C) fp32, bf16 or fp16; mean and variance over a sample's positions and the C / groups channels of a group;
     weight, bias (C) or None; activation "none", "silu" or "gelu" (the tanh form) -> x's shape in `dtype` (default: x's; fp32
     features may be narrowed).  Statistics in fp32, the result rounded once.  The gradients of x, weight and bias are
-    deterministic; differentiable once."""
+    deterministic; differentiable once, in reverse mode."""
     if activation not in ACTIVATIONS:
         raise ValueError(f"group_norm: activation must be one of {', '.join(ACTIVATIONS)}, got {activation!r}")
     return _lib.torch_ops().group_norm(x, groups, weight, bias, eps, ACTIVATIONS[activation], dtype)
@@ -621,7 +621,7 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     (B, T, H, dv) in the inputs' type, and with return_state the state after each sequence's last position, which
     linear_attention_step (or a next call) goes on from.  States and sums are fp32; a value that is not finite may show in the
     results of up to 31 positions before its own too.  The gradients of q, k, v and state are
-    deterministic; differentiable once."""
+    deterministic; differentiable once, in reverse mode."""
     if log_decay.requires_grad:
         raise ValueError("linear_attention: log_decay takes no gradient (detach it)")
     scale = q.shape[-1] ** -0.5 if scale is None else scale
