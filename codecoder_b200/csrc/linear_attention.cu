@@ -832,10 +832,13 @@ __device__ __forceinline__ uint32_t transpose(uint32_t piece) {      // an 8 x 8
 // earlier one's
 struct PairWeights {
   float w[4];
+  bool in_order[2];             // of the same half: the columns that do not come after the row
   __device__ __forceinline__ PairWeights(float log2_a, bool reverse, float scale) {
     const int lane = threadIdx.x & 31, e0 = (lane >> 2) - 2 * (lane & 3);
 #pragma unroll
     for (int k = 0; k < 4; ++k) w[k] = scale * power(log2_a, (reverse ? (k & 1) - e0 : e0 - (k & 1)) + (k >> 1) * 8);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) in_order[k] = (reverse ? k - e0 : e0 - k) >= 0;
   }
 };
 
@@ -865,17 +868,17 @@ __device__ __forceinline__ Piece<T, DP, HALVES> attend(const Piece<T, DP, HALVES
       for (int n = 0; n < HALVES; ++n) mma_bf16(P[n], x, b.r[n][2 * k], b.r[n][2 * k + 1]);
     }
   }
-  // [n][row half][column]: masked products are dropped, not multiplied by zero
+  // [n][row half][column]: products out of order are dropped, not multiplied by zero; others are multiplied whatever their
+  // weight is, for a NaN shows through a weight of zero too
 #pragma unroll
   for (int n = 0; n < HALVES; ++n)
 #pragma unroll
     for (int h = 0; h < HALVES; ++h)
 #pragma unroll
       for (int z = 0; z < 2; ++z) {
-        const bool never = reverse ? h > n : n > h;
-        const float wt = w.w[h == n ? z : 2 + z];
+        const bool ordered = h == n ? w.in_order[z] : reverse ? h < n : n < h;
         float& x = P[n][2 * h + z];
-        x = never || wt == 0.0f ? 0.0f : x * wt;
+        x = ordered ? x * w.w[h == n ? z : 2 + z] : 0.0f;
       }
   const bool keep0 = g < rows, keep1 = g + 8 < rows;
   if constexpr (P_::kF32) {
