@@ -299,13 +299,14 @@ class RoundMemory(nn.Module):
 
     def forward(self, x, lengths=None, state=None, return_state=False):
         B, T = x.shape[:2]
-        q, k, v = self._project(x, B, T)
+        there = None if lengths is None else (torch.arange(T, device=x.device) < lengths[:, None])[:, :, None, None]
+        # what stands behind a shot's rounds may be anything: it would reach the weights' gradients as zero times it
+        q, k, v = self._project(x if there is None else torch.where(there, x, 0), B, T)
         o = linear_attention(q, k, v, self.log_decay, state=state, lengths=lengths, return_state=return_state)
         o, new_state = o if return_state else (o, None)
         u = F.linear(self.norm(o.reshape(B * T * self.sites, self.C)), self.out).view(x.shape)
-        if lengths is not None:                 # the norm of nothing is its bias: rounds that are not there add nothing
-            there = torch.arange(T, device=x.device) < lengths[:, None]
-            u = torch.where(there[:, :, None, None], u, torch.zeros((), device=u.device, dtype=u.dtype))
+        if there is not None:                   # the norm of nothing is its bias: rounds that are not there add nothing
+            u = torch.where(there, u, 0)
         return (x + u, new_state) if return_state else x + u
 
     @torch.no_grad()
