@@ -616,13 +616,13 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     """Linear attention with a decay for each head over whole sequences (C ABI bpc_linear_attention_fwd / _bwd):
       S_t = a_h S_(t-1) + k_t v_t^T,  o_t = scale q_t S_t,  a_h = exp(log_decay_h)
     q, k (B, T, H, dk), v (B, T, H, dv) fp32 or bf16, any strides (head sizes 1 to 128); log_decay (H) fp32, not
-    differentiable; scale: dk^-0.5 by default; state (B, H, dk, dv) fp32: S before the first position (default: zero);
+    differentiable (refused if it requires a gradient, but under no_grad); scale: dk^-0.5 by default; state (B, H, dk, dv) fp32: S before the first position (default: zero);
     lengths (B) int32 or int64: positions at or behind a sequence's length are not read, and zero in the result -> o
     (B, T, H, dv) in the inputs' type, and with return_state the state after each sequence's last position, which
     linear_attention_step (or a next call) goes on from.  States and sums are fp32; a value that is not finite may show in the
     results of up to 31 positions before its own too.  The gradients of q, k, v and state are
     deterministic; differentiable once, in reverse mode."""
-    if log_decay.requires_grad:
+    if log_decay.requires_grad and torch.is_grad_enabled():
         raise ValueError("linear_attention: log_decay takes no gradient (detach it)")
     scale = q.shape[-1] ** -0.5 if scale is None else scale
     o, new_state = _lib.torch_ops().linear_attention(q, k, v, log_decay, scale, state, lengths, return_state)
