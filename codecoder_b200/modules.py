@@ -279,15 +279,14 @@ class RoundMemory(nn.Module):
             setattr(self, name, nn.Parameter((torch.rand(C, C, generator=g) * 2 - 1) / math.sqrt(C)))
         self.out = nn.Parameter(torch.zeros(C, C))
         self.norm = GroupNorm(C, heads, "silu")
-        self.register_buffer("log_decay", self._rates(), persistent=False)         # (sites, heads)
-
-    def _rates(self):
-        return torch.log1p(-torch.exp2(-torch.linspace(1.0, 6.0, self.heads, dtype=torch.float64))).float().repeat(self.sites)
+        rates = torch.log1p(-torch.exp2(-torch.linspace(1.0, 6.0, heads, dtype=torch.float64)))
+        self.register_buffer("log_decay", rates.float().repeat(sites), persistent=False)          # (sites, heads)
 
     def _apply(self, fn, recurse=True):
+        rates = self.log_decay
         super()._apply(fn, recurse)
-        if self.log_decay.dtype != torch.float32:       # a layer cast to another type keeps its rates
-            self.log_decay = self._rates().to(self.log_decay.device)
+        if self.log_decay.dtype != rates.dtype:         # a layer cast to another type keeps its rates as they are
+            self.log_decay = rates.to(self.log_decay.device)
         return self
 
     def _project(self, x, *lead):
