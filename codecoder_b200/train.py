@@ -218,12 +218,18 @@ class Trainer:
         return bool(fl[0].item()), bool(fl[1].item())
 
 
-def train_flops_per_shot(geo, cfg) -> float:
+def train_flops_per_shot(geo, cfg, memory: int | None = None) -> float:
     """Algorithmic FLOPs of one training shot: forward + input gradient + weight gradient of every bipartite step
     that reaches the loss (3 x 2 K C^2 per target node and step, all K slots counted; L check -> data steps and
-    L - 1 data -> check steps) plus the head."""
+    L - 1 data -> check steps) plus the head.  With `memory` heads of D = C / memory channels also those of the memory over R
+    rounds: four maps (3 x 2 C^2 per data node each), and the attention's four scans (forward, dq, dk, dv), per position and head
+    the products with the state (4 D^2) or with the positions before it (2 D (R + 1) on average), whichever are fewer."""
     C, K, L = cfg.channels, cfg.K, cfg.layers
-    return 3.0 * 2 * K * C * C * (L * geo.N_d + (L - 1) * geo.N_c) + 3.0 * 2 * 2 * C * geo.N_d
+    flops = 3.0 * 2 * K * C * C * (L * geo.N_d + (L - 1) * geo.N_c) + 3.0 * 2 * 2 * C * geo.N_d
+    if memory is not None:
+        D = C // memory
+        flops += geo.N_d * (4 * 3.0 * 2 * C * C + 4.0 * memory * min(4 * D * D, 2 * D * (geo.R + 1)))
+    return flops
 
 
 def bce_at_init(err_rate: float) -> float:
