@@ -368,43 +368,29 @@ __global__ void __launch_bounds__(1024) join_kernel(const float* __restrict__ pa
   }
 }
 
-// the sum over the block, in every thread; red: 8 floats
-__device__ __forceinline__ float block_sum(float v, float* red) {
-#pragma unroll
-  for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float s = 0.0f;
-#pragma unroll
-  for (int w = 0; w < 8; ++w) s += red[w];
-  __syncthreads();
-  return s;
-}
-
 // Wide groups: a block per sample and group, in two passes
 template <typename T, typename U, int ACT>
 __global__ void __launch_bounds__(256) wide_kernel(const U* __restrict__ gy, const T* __restrict__ x, const float2* __restrict__ stats,
                                                    const float* __restrict__ w, const float* __restrict__ bias, T* __restrict__ dx,
                                                    const Shape s) {
-  __shared__ float red[8];
+  __shared__ double red[8];
   const int cg = s.C / s.G;
   const int64_t n = s.N * cg;
   for (int64_t at = blockIdx.x; at < s.B * s.G; at += gridDim.x) {
     const int64_t b = at / s.G;
     const int c0 = static_cast<int>(at % s.G) * cg;
     const float mean = stats[at].x, rstd = stats[at].y;
-    float s1 = 0.0f, s2 = 0.0f;
+    double sum1 = 0.0, sum2 = 0.0;
     for (int64_t i = threadIdx.x; i < n; i += 256) {
       const int c = c0 + static_cast<int>(i % cg);
       const int64_t r = i / cg;
       const float wc = w ? w[c] : 1.0f;
       const float xh = (load_f32(x + b * s.x_sample + r * s.x_row + c) - mean) * rstd;
       const float a = load_f32(gy + b * s.g_sample + r * s.g_row + c) * slope1<ACT>(fmaf(wc, xh, bias ? bias[c] : 0.0f)) * wc;
-      s1 += a;
-      s2 = fmaf(a, xh, s2);
+      sum1 += a;
+      sum2 = fma(static_cast<double>(a), static_cast<double>(xh), sum2);
     }
-    s1 = block_sum(s1, red) / static_cast<float>(n);
-    s2 = block_sum(s2, red) / static_cast<float>(n);
+    const float s1 = block_mean(sum1, n, red), s2 = block_mean(sum2, n, red);
     for (int64_t i = threadIdx.x; i < n; i += 256) {
       const int c = c0 + static_cast<int>(i % cg);
       const int64_t r = i / cg;

@@ -258,40 +258,27 @@ __global__ void __launch_bounds__(kTileThreads, 3) tiles_kernel(const T* __restr
   }
 }
 
-// the sum over the block, in every thread; red: 8 floats
-__device__ __forceinline__ float block_sum(float v, float* red) {
-#pragma unroll
-  for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float s = 0.0f;
-#pragma unroll
-  for (int w = 0; w < 8; ++w) s += red[w];
-  __syncthreads();
-  return s;
-}
-
 // Wide groups: a block per sample and group, in three passes
 template <typename T, typename U, int ACT>
 __global__ void __launch_bounds__(256) wide_kernel(const T* __restrict__ x, U* __restrict__ y, float2* stats,
                                                    const float* __restrict__ w, const float* __restrict__ bias, const Shape s,
                                                    float eps) {
-  __shared__ float red[8];
+  __shared__ double red[8];
   const int cg = s.C / s.G;
   const int64_t n = s.N * cg;
   for (int64_t at = blockIdx.x; at < s.B * s.G; at += gridDim.x) {
     const int64_t b = at / s.G;
     const int c0 = static_cast<int>(at % s.G) * cg;
     const T* xs = x + b * s.x_sample + c0;
-    float sum = 0.0f;
+    double sum = 0.0;
     for (int64_t i = threadIdx.x; i < n; i += 256) sum += load_f32(xs + i / cg * s.x_row + i % cg);
-    const float mean = block_sum(sum, red) / static_cast<float>(n);
-    float sq = 0.0f;
+    const float mean = block_mean(sum, n, red);
+    double sq = 0.0;
     for (int64_t i = threadIdx.x; i < n; i += 256) {
-      const float d = load_f32(xs + i / cg * s.x_row + i % cg) - mean;
-      sq = fmaf(d, d, sq);
+      const double d = load_f32(xs + i / cg * s.x_row + i % cg) - mean;
+      sq = fma(d, d, sq);
     }
-    const float rstd = 1.0f / sqrtf(block_sum(sq, red) / static_cast<float>(n) + eps);
+    const float rstd = 1.0f / sqrtf(block_mean(sq, n, red) + eps);
     if (threadIdx.x == 0 && stats) stats[at] = make_float2(mean, rstd);
     for (int64_t i = threadIdx.x; i < n; i += 256) {
       const int c = c0 + static_cast<int>(i % cg);
