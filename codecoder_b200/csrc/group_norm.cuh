@@ -235,14 +235,14 @@ __device__ __forceinline__ void cp_wait() {
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void cp_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
-// Vectors of the next kDepth - 1 samples on their way through shared memory, each read by the thread that fetched it: no
+// Vectors of the next samples on their way through shared memory, each read by the thread that fetched it: no
 // barrier, and no registers (one sample ahead in those kept too little under way).  A stage holds what the block's threads
 // fetch of a sample each; copies cannot take single elements of 2 bytes, which are read when used.
 template <typename T, int VEC>
 struct Copied {
   using P = Pack<T, VEC>;
-  static constexpr bool kCopies = sizeof(P) >= 4;
-  static constexpr int kBytes = kCopies ? static_cast<int>(sizeof(P)) : 0;
+  static constexpr int kBytes = copied_bytes(sizeof(T), VEC);
+  static constexpr bool kCopies = kBytes > 0;
   __device__ static __forceinline__ void fetch(uint32_t at, const T* src) {
     if constexpr (kBytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(src) : "memory");
     else if constexpr (kBytes > 0) asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(at), "l"(src), "n"(kBytes) : "memory");

@@ -84,6 +84,7 @@ __global__ void __launch_bounds__(kUnitThreads) units_kernel(const U* __restrict
   // fetched and of the one worked on
   using X = Copied<T, VEC>;
   using Y = Copied<U, VEC>;
+  constexpr int kDepth = units_depth(units_bytes(X::kBytes, Y::kBytes, SLOTS, true));
   const uint32_t x_bytes = blockDim.x * X::kBytes, g_bytes = blockDim.x * Y::kBytes;
   const uint32_t at_x = threadIdx.x * X::kBytes, at_g = SLOTS * x_bytes + threadIdx.x * Y::kBytes;
   const uint32_t at_stat = SLOTS * (x_bytes + g_bytes) + threadIdx.x * 8, stage_bytes = SLOTS * (x_bytes + g_bytes) + blockDim.x * 8;
@@ -425,7 +426,7 @@ __global__ void __launch_bounds__(256) wide_channels_kernel(const U* __restrict_
   parts[static_cast<int64_t>(blockIdx.y) * 2 * s.C + s.C + c] = static_cast<float>(d);
 }
 
-Plan plan_of(const Shape& s, int size, int y_size, bool aligned) { return make_plan(s, size, y_size, num_sms(), aligned, true); }
+Plan plan_of(const Shape& s, int size, bool aligned) { return make_plan(s, size, num_sms(), aligned, true); }
 
 constexpr int kTilesPerSm = 2;
 
@@ -444,14 +445,13 @@ int64_t parts_of(const Shape& s, const Plan& p) {
 
 size_t backward_workspace(const Shape& s, int size) {
   size_t bytes = 16;
-  for (int y_size : {2, size})                     // the gradients' type may be narrower
-    for (bool aligned : {false, true}) {
-      const Plan p = plan_of(s, size, y_size, aligned);
-      size_t parts = sizeof(float) * 2 * static_cast<size_t>(s.C) * parts_of(s, p);
-      parts = (parts + 15) / 16 * 16;
-      if (p.kind == kTiles && !p.fused) parts += sizeof(float2) * static_cast<size_t>(s.B) * p.chunks * s.G;
-      bytes = std::max(bytes, parts);
-    }
+  for (bool aligned : {false, true}) {
+    const Plan p = plan_of(s, size, aligned);
+    size_t parts = sizeof(float) * 2 * static_cast<size_t>(s.C) * parts_of(s, p);
+    parts = (parts + 15) / 16 * 16;
+    if (p.kind == kTiles && !p.fused) parts += sizeof(float2) * static_cast<size_t>(s.B) * p.chunks * s.G;
+    bytes = std::max(bytes, parts);
+  }
   return bytes;
 }
 
@@ -532,7 +532,7 @@ extern "C" int bpc_group_norm_bwd(const void* gy, const void* x, const float* st
   };
   const bool whole = whole_of(x, x_sample_stride, x_row_stride, size) && whole_of(dx, 0, 0, size) &&
                      whole_of(gy, gy_sample_stride, gy_row_stride, y_size);
-  const Plan p = plan_of(s, size, y_size, whole);
+  const Plan p = plan_of(s, size, whole);
   const bool want = dw || db;
   const int e = with_types(x_dtype, y_dtype, [&](auto xt, auto yt) {
     return with_act(activation, [&](auto act) {

@@ -40,6 +40,7 @@ __global__ void __launch_bounds__(kUnitThreads) units_kernel(const T* __restrict
   bool has[SLOTS];
   uint64_t wv[SLOTS][kP], bv[SLOTS][kP];
   using In = Copied<T, VEC>;
+  constexpr int kDepth = units_depth(units_bytes(In::kBytes, 0, SLOTS, false));
   extern __shared__ __align__(16) uint8_t smem[];
 #pragma unroll
   for (int k = 0; k < SLOTS; ++k) {
@@ -289,7 +290,7 @@ __global__ void __launch_bounds__(256) wide_kernel(const T* __restrict__ x, U* _
   }
 }
 
-Plan plan_of(const Shape& s, int size, bool aligned) { return make_plan(s, size, size, num_sms(), aligned, false); }
+Plan plan_of(const Shape& s, int size, bool aligned) { return make_plan(s, size, num_sms(), aligned, false); }
 
 }  // namespace
 

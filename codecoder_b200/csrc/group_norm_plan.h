@@ -35,24 +35,28 @@ struct Plan {
 
 constexpr int kUnitThreads = 512;    // at most
 constexpr int kTileThreads = 256;
-constexpr int kDepth = 4;            // samples of units on their way or worked on
 
 // Dynamic shared memory of a block: one that a launch can have, and what a kernel takes.
 constexpr int kBlockSmem = 227 * 1024;
-// units: a ring of a thread's vectors that are on their way (single elements of 2 bytes are not copied), backwards with gy's and
-// the statistics beside them, and at the end a row of sums for each of the block's rows
+// units: samples that are on their way or worked on, of which a thread copies so many bytes each: four, or three where the largest
+// block has no room for four.  That is fp32 with fp32 gradients and four slots, 136 bytes: 278,528 or 208,896 for 512 threads.
+// Smaller blocks of it lose nothing by the same depth (65,536 x 512 in one group forward and backward 152 us with four, 144 with
+// three; 20,000 x 33 x 104 in 13 groups 408 and 366), and tiles would take 547 us for 4,096 x 8,192 in 16 groups: 156.
+constexpr int units_depth(int thread_bytes) { return 4 * thread_bytes * kUnitThreads <= kBlockSmem ? 4 : 3; }
+// a ring of them (single elements of 2 bytes are not copied), backwards with gy's and the statistics beside x's, and at the end a
+// row of sums for each of the block's rows
+constexpr int copied_bytes(int size, int vec) { return size * vec >= 4 ? size * vec : 0; }
+constexpr int units_bytes(int x_copied, int y_copied, int slots, bool backward) { return backward ? (x_copied + y_copied) * slots + 8 : x_copied * slots; }
 inline int units_smem(const Plan& p, const Shape& s, int size, int y_size, bool backward) {
-  auto copied = [&](int bytes) { return bytes * p.vec >= 4 ? bytes * p.vec : 0; };
-  const int thread = backward ? (copied(size) + copied(y_size)) * p.slots + 8 : copied(size) * p.slots;
-  const int ring = kDepth * thread * p.threads;
+  const int thread = units_bytes(copied_bytes(size, p.vec), copied_bytes(y_size, p.vec), p.slots, backward);
+  const int ring = units_depth(thread) * thread * p.threads;
   return backward ? std::max(ring, p.rows * static_cast<int>(s.N) * s.C * static_cast<int>(sizeof(float))) : ring;
 }
 
 // Whole accesses are taken where the pointers and strides allow it (`aligned`) and the groups hold whole ones: of kTileVec
 // elements in tiles, in units of `full`, SLOTS of them a lane: two where there are two forwards, as the joins and the addresses are
 // half of the rest; one backwards, where the sums of gradients fill the registers, and of kTileVec where one is not enough.
-// y_size: of y's elements, gy's backwards, whose copies must fit beside x's.
-inline Plan make_plan(const Shape& s, int size, int y_size, int sms, bool aligned, bool backward) {
+inline Plan make_plan(const Shape& s, int size, int sms, bool aligned, bool backward) {
   Plan p = {};
   const int cg = s.C / s.G;
   int full = 16 / size;
@@ -68,8 +72,7 @@ inline Plan make_plan(const Shape& s, int size, int y_size, int sms, bool aligne
       p.kind = kUnits;
       p.rows = std::max(1, 256 / (p.lanes * s.G));
       p.threads = (p.lanes * s.G * p.rows + 31) / 32 * 32;
-      // four slots of fp32 and fp32 gradients: 544 bytes a thread, too many for the 448 threads of 14 groups and more
-      if (units_smem(p, s, size, y_size, backward) <= kBlockSmem) return p;
+      return p;
     }
   }
   p.vec = aligned && cg % kTileVec == 0 ? kTileVec : 1;

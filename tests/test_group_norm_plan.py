@@ -22,15 +22,16 @@ int main() {
               for (bool backward : {false, true}) {
                 if (y_size > size) continue;
                 const Shape s{5, N, G * cg, G, static_cast<int64_t>(N) * G * cg, G * cg, static_cast<int64_t>(N) * G * cg, G * cg};
-                const Plan p = make_plan(s, size, y_size, 148, aligned, backward);
+                const Plan p = make_plan(s, size, 148, aligned, backward);
                 if (p.threads < 32 || p.threads % 32 || p.threads > (p.kind == kUnits ? kUnitThreads : kTileThreads))
                   return std::printf("threads %d: %d groups of %d, %d rows\n", p.threads, G, cg, N), 1;
                 if (p.kind != kUnits) continue;
                 ++units;
-                // counted here again: a stage of every vector that a thread copies, four deep
+                // counted here again: a stage of every vector that a thread copies, four deep or three
                 int thread = size * p.vec >= 4 ? size * p.vec * p.slots : 0;
                 if (backward) thread += (y_size * p.vec >= 4 ? y_size * p.vec * p.slots : 0) + 8;
-                int bytes = 4 * thread * p.threads;
+                const int depth = 4 * thread * 512 <= limit ? 4 : 3;
+                int bytes = depth * thread * p.threads;
                 if (backward && bytes < p.rows * N * G * cg * 4) bytes = p.rows * N * G * cg * 4;
                 if (units_smem(p, s, size, y_size, backward) != bytes)
                   return std::printf("bytes: %d groups of %d, %d rows\n", G, cg, N), 1;
