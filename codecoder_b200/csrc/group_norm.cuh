@@ -298,11 +298,12 @@ inline int launched(const char* what) {
   return e == cudaSuccess ? 0 : fail(BPC_ERR_LAUNCH, std::string(what) + " launch: " + cudaGetErrorString(e));
 }
 
-// Blocks of x, y: every slab and chunk, and the samples that a slab's blocks walk at once; `per_sm` blocks of 256 threads
-inline dim3 tiles_grid(const Shape& s, const Plan& p, int per_sm, int sms) {
+// Blocks of x, y: every slab and chunk, and the samples that a slab's blocks walk at once; `per_sm` blocks of 256 threads, and
+// more where one would walk more than `walk` samples
+inline dim3 tiles_grid(const Shape& s, const Plan& p, int per_sm, int sms, int64_t walk) {
   const int64_t across = static_cast<int64_t>(p.slabs) * p.chunks;
   const int64_t resident = static_cast<int64_t>(sms) * std::max(1, per_sm * 256 / p.threads);
-  return dim3(static_cast<unsigned>(across), static_cast<unsigned>(std::min<int64_t>({s.B, 65535, std::max<int64_t>(1, resident / across)})));
+  return dim3(static_cast<unsigned>(across), static_cast<unsigned>(std::min<int64_t>({s.B, 65535, std::max<int64_t>({1, resident / across, (s.B + walk - 1) / walk})})));
 }
 
 inline int size_of(int32_t dtype) { return dtype == BPC_DTYPE_F32 ? 4 : dtype == BPC_DTYPE_BF16 || dtype == BPC_DTYPE_F16 ? 2 : 0; }

@@ -429,16 +429,18 @@ __global__ void __launch_bounds__(256) wide_channels_kernel(const U* __restrict_
 Plan plan_of(const Shape& s, int size, bool aligned) { return make_plan(s, size, num_sms(), aligned, true); }
 
 constexpr int kTilesPerSm = 2;
+// Samples whose gradients a thread adds up in fp32 before they are joined in fp64.  Values that are all alike round the same way:
+// 3,333 times 0.1 is 560 roundings of 2^-24 off, 256 times 40.
+constexpr int64_t kWalk = 256;
 
 // Parts of dw and db: one per block that walks the samples, per slab
 int64_t parts_of(const Shape& s, const Plan& p) {
   if (p.kind == kUnits) {
-    // rounds are counted in 32 bits
     const int64_t blocks = (s.B + p.rows - 1) / p.rows;
-    return std::min(blocks, std::max(static_cast<int64_t>(num_sms()) * std::max(1, 1024 / p.threads), blocks >> 30));
+    return std::min(blocks, std::max(static_cast<int64_t>(num_sms()) * std::max(1, 1024 / p.threads), (blocks + kWalk - 1) / kWalk));
   }
   if (p.kind == kWide) return std::min<int64_t>(s.B * s.N, 32);
-  return static_cast<int64_t>(tiles_grid(s, p, kTilesPerSm, num_sms()).y) * p.chunks;
+  return static_cast<int64_t>(tiles_grid(s, p, kTilesPerSm, num_sms(), kWalk).y) * p.chunks;
 }
 
 }  // namespace
@@ -478,7 +480,7 @@ int run_tiles(const U* gy, const T* x, const float2* stats, const float* w, cons
   Plan plan = p;
   void* args[] = {&gy, &x, &stats, &w, &bias, &dx, &parts, &shape, &plan, &between};
   const int smem = std::max(Ahead<T, VEC, kRows>::kBytes + Ahead<U, VEC, kRows>::kBytes, VEC * static_cast<int>(sizeof(float))) * kTileThreads;
-  const dim3 grid = tiles_grid(s, p, kTilesPerSm, num_sms());
+  const dim3 grid = tiles_grid(s, p, kTilesPerSm, num_sms(), kWalk);
   if (p.fused)
     return launch_clusters(reinterpret_cast<const void*>(&tiles_kernel<T, U, ACT, VEC, kFused>), grid, dim3(p.threads), smem, st, args, p.chunks, what);
   if (int e = launch_clusters(reinterpret_cast<const void*>(&tiles_kernel<T, U, ACT, VEC, kSums>), grid, dim3(p.threads), smem, st, args, 1, what)) return e;

@@ -328,7 +328,7 @@ int run_tiles(const T* x, U* y, float2* stats, const float* w, const float* bias
   Shape shape = s;
   Plan plan = p;
   void* args[] = {&x, &y, &stats, &w, &bias, &shape, &plan, &eps, &parts};
-  const dim3 grid = tiles_grid(s, p, 3, num_sms());
+  const dim3 grid = tiles_grid(s, p, 3, num_sms(), s.B);
   const int smem = Ahead<T, VEC, kRows>::kBytes * kTileThreads;
   if (p.fused)
     return launch_clusters(reinterpret_cast<const void*>(&tiles_kernel<T, U, ACT, VEC, kFused>), grid, dim3(p.threads), smem, st, args, p.chunks, what);

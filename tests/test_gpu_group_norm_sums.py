@@ -47,3 +47,16 @@ def test_wide_groups_of_many_rows(shape, offset):
     e_dw = (gd.abs() * e_xh).sum((0, 1)) + U * (gd * xh).abs().sum((0, 1))
     assert bool(((dw.double().view(G, -1) - (gd * xh).sum((0, 1))).abs() <= e_dw).all())
     assert bool(((db.double().view(G, -1) - gd.sum((0, 1))).abs() <= U * gd.abs().sum((0, 1))).all())
+
+
+@pytest.mark.parametrize("B,C,G", [(60_000, 16_384, 32), (60_000, 8192, 4), (150_000_000, 4, 1)])
+def test_a_bias_gradient_over_many_samples(B, C, G):
+    """Gradients that are all alike, whose roundings do not cancel: a thread adds up 256 samples at most, 256 u, and what the
+    threads have joins in 64 bits, rounded to fp32 twice."""
+    x = torch.zeros(B, 1, C, device=DEV)
+    x[:, :, ::2] = 1.0
+    b = torch.zeros(C, device=DEV, requires_grad=True)
+    gy = torch.full((B, 1, C), 0.1, device=DEV)
+    db, = torch.autograd.grad(ops.group_norm(x, G, None, b), b, gy)
+    want = B * float(gy[0, 0, 0].double())
+    assert float((db.double() - want).abs().max()) <= 258 * U * want
