@@ -122,6 +122,9 @@ int launch_pdl(const void* fn, dim3 grid, dim3 block, size_t smem, cudaStream_t 
 // A plain launch, as clusters of cluster_x CTAs; opts in to the shared memory.
 int launch_clusters(const void* fn, dim3 grid, dim3 block, int smem, cudaStream_t stream, void** args, int cluster_x, const char* what);
 
+// Blocks per SM of a kernel without dynamic shared memory (asked once per device and kernel; calls may come from several threads).
+int resident_blocks(const void* fn, int threads, const char* what, int* blocks);
+
 // cuTensorMapEncodeTiled through the runtime's driver entry point (null when the driver lacks it).
 PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder();
 

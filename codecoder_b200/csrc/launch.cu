@@ -1,5 +1,6 @@
 // Kernel launches and their attributes on the host.  A call that is refused leaves no error behind: the next kernel's check reads
 // the last one of its thread.  Plain C++ but for its name.
+#include <atomic>
 #include <map>
 #include <mutex>
 #include <string>
@@ -73,13 +74,33 @@ int launch_clusters(const void* fn, dim3 grid, dim3 block, int smem, cudaStream_
   return e == cudaSuccess ? 0 : refused(std::string(what) + " launch", e);
 }
 
+int resident_blocks(const void* fn, int threads, const char* what, int* blocks) {
+  static std::mutex mu;
+  static std::map<std::pair<int, const void*>, int> known;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  std::lock_guard<std::mutex> lk(mu);
+  int& n = known[{dev, fn}];
+  if (n < 1) {
+    const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, fn, threads, 0);
+    if (e != cudaSuccess || n < 1) {
+      n = 0;
+      return refused(std::string(what) + " occupancy", e);
+    }
+  }
+  *blocks = n;
+  return 0;
+}
+
 int num_sms() {
-  static int n = 0;
+  static std::atomic<int> known{0};
+  int n = known.load(std::memory_order_relaxed);
   if (n == 0) {
     int dev = 0;
     cudaGetDevice(&dev);
     cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
     if (n <= 0) n = 1;
+    known.store(n, std::memory_order_relaxed);
   }
   return n;
 }

@@ -1166,23 +1166,11 @@ int run_scan(Scan p, Scan* second, int64_t B, int32_t dtype, float* workspace, c
   });
 }
 
-// Blocks of a kernel without dynamic shared memory that are resident per SM
-int blocks_of(const void* fn, int* cached, int* blocks) {
-  if (!*cached) {
-    int n = 0;
-    const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, fn, kThreads, 0);
-    if (e != cudaSuccess || n < 1) return refused("linear_attention occupancy", e);
-    *cached = n;
-  }
-  *blocks = *cached;
-  return 0;
-}
-
 template <typename T, int DP, bool BWD, int HALVES>
 int launch_short(Short p, cudaStream_t s) {
-  static int cached = 0;
   int blocks = 0;
-  if (int e = blocks_of(reinterpret_cast<const void*>(&short_kernel<T, DP, BWD, HALVES>), &cached, &blocks)) return e;
+  if (int e = resident_blocks(reinterpret_cast<const void*>(&short_kernel<T, DP, BWD, HALVES>), kThreads, "linear_attention", &blocks))
+    return e;
   const uint32_t warps = kThreads / 32;
   const unsigned grid = std::min<unsigned>((p.items + warps - 1) / warps, blocks * num_sms());
   p.step_b = grid * warps / p.H, p.step_h = grid * warps % p.H;

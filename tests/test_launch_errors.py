@@ -19,6 +19,7 @@ const char* cudaGetErrorString(cudaError_t) { return "refused"; }
 cudaError_t cudaGetDevice(int* d) { *d = 0; return cudaSuccess; }
 cudaError_t cudaDeviceGetAttribute(int* v, cudaDeviceAttr, int) { *v = 148; return cudaSuccess; }
 cudaError_t cudaFuncSetAttribute(const void*, cudaFuncAttribute, int) { ++attributes; return answer(cudaErrorInvalidValue); }
+cudaError_t cudaOccupancyMaxActiveBlocksPerMultiprocessor(int*, const void*, int, size_t) { return answer(cudaErrorInvalidValue); }
 cudaError_t cudaLaunchKernelExC(const cudaLaunchConfig_t*, const void*, void**) { ++launches; return answer(cudaErrorInvalidConfiguration); }
 }
 namespace bpc {
@@ -37,6 +38,9 @@ int main() {
   if (attributes != 2 || launches != 2) return std::printf("calls %d %d\n", attributes, launches), 1;
   launch_pdl(&kernel, dim3(1), dim3(32), 0, nullptr, nullptr, 1, "this");
   if (message != "this launch: refused" || last != cudaSuccess) return std::printf("left behind: %d\n", last), 1;
+  int blocks = 0;
+  if (resident_blocks(&kernel, 128, "these", &blocks) != BPC_ERR_LAUNCH || message != "these occupancy: refused" || last != cudaSuccess)
+    return std::printf("left behind: %d\n", last), 1;
   refuse = false;               // what was refused is not remembered as granted
   if (allow_smem(&kernel, 100000) || attributes != 3 || allow_smem(&kernel, 50000) || attributes != 3) return std::printf("granted\n"), 1;
   return launch_clusters(&kernel, dim3(1), dim3(32), 100000, nullptr, nullptr, 4, "that");
