@@ -953,8 +953,7 @@ __global__ void __launch_bounds__(kThreads, kShortBlocks<T, DP, BWD>) short_kern
     // the next item's rows are on their way while this one's are used
     b += p.step_b, h += p.step_h;
     if (h >= static_cast<uint32_t>(p.H)) h -= p.H, ++b;
-    at += stride;
-    if (at < at - stride) at = p.items;            // past 2^32
+    at += stride;                                  // below 2^31: B H is below 2^30
     if (at < p.items) load();
     const int64_t row = (static_cast<int64_t>(b0) * p.T * p.H + h0);
     const int64_t sk = static_cast<int64_t>(p.H) * p.dim_k, sv = static_cast<int64_t>(p.H) * p.dim_v;
