@@ -447,6 +447,8 @@ class CascadeStack(nn.Module):
         Blocks of H = 512 with a 128-channel bottleneck (the reference's C14 blocks) hand over in one launch per block
         boundary (bpc_cascade_boundary: up, residual, the next block's BN1 + SiLU, down and BN2 + SiLU); other sizes
         run the block-by-block fused path."""
+        if any(b.norm != "batch" for b in blocks):
+            raise ValueError('forward_blocks: blocks with norm="group" have no folded norms (call the stack)')
         dev = h.device if h is not None else tokens[3].device
         for b in blocks:
             if b._cache is None or b._cache["a1"].device != dev:

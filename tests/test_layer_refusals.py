@@ -1,0 +1,14 @@
+"""Calls of the layers and of linear attention that have no answer are refused with a reason.  Runs without a GPU."""
+import pytest
+import torch
+
+from codecoder_b200.geometry import RotatedSurface
+from codecoder_b200.modules import CascadeBlock, CascadeStack
+
+
+@pytest.mark.parametrize("H", [64, 512])
+def test_the_fused_path_refuses_blocks_with_group_norm(H):
+    blocks = [CascadeBlock(H, RotatedSurface(3, 3), 2, norm=n, groups=8) for n in ("batch", "group")]
+    h = torch.zeros(1, blocks[0].c2d_all.shape[0], H)
+    with pytest.raises(ValueError, match="group"):
+        CascadeStack.forward_blocks(blocks, h)
