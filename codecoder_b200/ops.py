@@ -611,6 +611,10 @@ def group_norm(x: torch.Tensor, groups: int, weight: torch.Tensor | None = None,
     return _lib.torch_ops().group_norm(x, groups, weight, bias, eps, ACTIVATIONS[activation], dtype)
 
 
+def _head_scale(q: torch.Tensor) -> float:
+    return max(1, q.shape[-1:].numel()) ** -0.5          # the entry points refuse what has no head size
+
+
 def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, scale: float | None = None,
                      state: torch.Tensor | None = None, lengths: torch.Tensor | None = None, return_state: bool = False):
     """Linear attention with a decay for each head over whole sequences (C ABI bpc_linear_attention_fwd / _bwd):
@@ -624,7 +628,7 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     deterministic; differentiable once, in reverse mode."""
     if log_decay.requires_grad and torch.is_grad_enabled():
         raise ValueError("linear_attention: log_decay takes no gradient (detach it)")
-    scale = q.shape[-1] ** -0.5 if scale is None else scale
+    scale = _head_scale(q) if scale is None else scale
     o, new_state = _lib.torch_ops().linear_attention(q, k, v, log_decay, scale, state, lengths, return_state)
     return (o, new_state) if return_state else o
 
@@ -634,7 +638,7 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
     """One position of linear_attention (C ABI bpc_linear_attention_step): q, k (B, H, dk), v (B, H, dv), state
     (B, H, dk, dv) fp32 contiguous -> o (B, H, dv); the state is updated in place, or written to `new_state`, which must not
     overlap it.  Not differentiable, whatever the inputs require."""
-    scale = q.shape[-1] ** -0.5 if scale is None else scale
+    scale = _head_scale(q) if scale is None else scale
     return _lib.torch_ops().linear_attention_step(q, k, v, log_decay, state, scale, new_state)
 
 
