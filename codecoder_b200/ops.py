@@ -604,7 +604,7 @@ def group_norm(x: torch.Tensor, groups: int, weight: torch.Tensor | None = None,
     """act(weight (x - mean) / sqrt(var + eps) + bias) over channels-last features (C ABI bpc_group_norm_fwd / _bwd):
     x (B, ..., C) fp32, bf16 or fp16; mean and variance over a sample's positions and the C / groups channels of a group;
     weight, bias (C) or None; activation "none", "silu" or "gelu" (the tanh form) -> x's shape in `dtype` (default: x's; fp32
-    features may be narrowed).  Statistics in fp32, the result rounded once.  The gradients of x, weight and bias are
+    features may be narrowed).  Statistics in fp32 or wider, the result rounded once.  The gradients of x, weight and bias are
     deterministic; differentiable once, in reverse mode."""
     if activation not in ACTIVATIONS:
         raise ValueError(f"group_norm: activation must be one of {', '.join(ACTIVATIONS)}, got {activation!r}")
@@ -620,12 +620,14 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     """Linear attention with a decay for each head over whole sequences (C ABI bpc_linear_attention_fwd / _bwd):
       S_t = a_h S_(t-1) + k_t v_t^T,  o_t = scale q_t S_t,  a_h = exp(log_decay_h)
     q, k (B, T, H, dk), v (B, T, H, dv) fp32 or bf16, any strides (head sizes 1 to 128); log_decay (H) fp32, not
-    differentiable (refused if it requires a gradient, but under no_grad); scale: dk^-0.5 by default; state (B, H, dk, dv) fp32: S before the first position (default: zero);
-    lengths (B) int32 or int64: positions at or behind a sequence's length are not read, and zero in the result -> o
-    (B, T, H, dv) in the inputs' type, and with return_state the state after each sequence's last position, which
-    linear_attention_step (or a next call) goes on from.  States and sums are fp32; a value that is not finite may show in the
-    results of up to 31 positions before its own too.  The gradients of q, k, v and state are
-    deterministic; differentiable once, in reverse mode."""
+    differentiable (refused if it requires a gradient, but under no_grad); scale: dk^-0.5 by default; state (B, H, dk, dv)
+    fp32: S before the first position (default: zero); lengths (B) int32 or int64: positions at or behind a sequence's length
+    are not read, and zero in the result -> o (B, T, H, dv) in the inputs' type, and with return_state the state after each
+    sequence's last position, which linear_attention_step (or a next call) goes on from.
+    States and sums are fp32.  Products run on the tensor unit: fp32 ones in three of tf32 parts, 3 to 20 roundings of 2^-24 off
+    by the head's size (plain fp32: 1.6 to 3); beside bf16 inputs what is fp32 (the state, the weighted pairs) in two bf16
+    parts, 2^-18 off.  A value that is not finite becomes NaN, infinities too, and may show in the results of up to 31 positions
+    before its own.  The gradients of q, k, v and state are deterministic; differentiable once, in reverse mode."""
     if log_decay.requires_grad and torch.is_grad_enabled():
         raise ValueError("linear_attention: log_decay takes no gradient (detach it)")
     scale = _head_scale(q) if scale is None else scale

@@ -167,7 +167,8 @@ BPC_API int bpc_embed_wgrad(const void* gy, const void* ids, int32_t id_bytes, v
  * contiguous, x's type or, for f32 x, a narrower one; stats (B, G, 2) fp32, 8-byte aligned: each group's mean
  * and 1 / sqrt(var + eps), written by the forward pass (or NULL), read by the backward pass; weight, bias (C) fp32 or
  * NULL (1, 0).  gy: y's type, any strides as x; dx (B, N, C) contiguous, x's type; dw, db (C) fp32; NULL where a gradient
- * is not wanted.  Statistics and sums are fp32 or wider, in a fixed order (deterministic), each result rounded once.  N
+ * is not wanted.  Statistics and sums are fp32 or wider, in a fixed order (deterministic), each result rounded once; the GELU's
+ * gradient is NaN where |z| passes 10^13.  N
  * <= 2^30, C <= 2^20; every buffer aligned to its type.
  * No buffer that is written overlaps another.  workspace: bpc_group_norm_workspace_size() bytes on the current device, 16-byte
  * aligned. */
@@ -195,12 +196,18 @@ BPC_API int bpc_group_norm_bwd(const void* gy, const void* x, const float* stats
  * forgets everything; no gradient of it is formed.  state, new_state, grad_state, dstate (B, H, dk, dv) fp32, 16-byte
  * aligned (4-byte for the step); a NULL state or grad_state is zero.  lengths (B) int32 or int64 (length_bytes 4 or 8) or
  * NULL (T each): positions at or behind a sequence's length are not read, and zero in o, dq, dk and dv.  1 <= dk, dv <=
- * 128, B H < 2^30, T <= 2^30.  States, products and sums are fp32, in a fixed order (deterministic).  No buffer that is
- * written overlaps another, but the step's new_state may be the state itself; states that overlap otherwise are refused.
+ * 128, B H < 2^30, T <= 2^30.  No buffer that is written overlaps another, but the step's new_state may be the state itself;
+ * states that overlap otherwise are refused.
+ * Arithmetic: states and sums are fp32, in a fixed order (deterministic).  Products of whole sequences run on the tensor unit:
+ * f32 operands in two tf32 parts (the root mean square of a result's error is 3 to 20 times 2^-24, by the head's size, where
+ * plain fp32 arithmetic makes 1.6 to 3); bf16 inputs as they are, and what is fp32 beside them (the state, the weighted pairs and
+ * rows) in two bf16 parts, off by 2^-18 of itself, rows that make a state handed out in three.  A step's products are fp32.
+ * Values that are not finite become NaN in these parts, infinities too, and so do f32 operands from 2^128 (1 - 2^-12) up (beside
+ * bf16 inputs from 2^128 (1 - 2^-9)).  They may show in the results of up to 31 positions on either side of their own, besides
+ * those that they belong to.
  * workspace: bpc_linear_attention_workspace_size() bytes on the current device, 16-byte aligned; fwd_workspace: the workspace
  * of bpc_linear_attention_fwd on the same inputs, as it was left (another than workspace), or NULL: what it holds is then
- * formed again.  A value that is not finite may show in the results of up to 31 positions on either side of its own, besides
- * those that it belongs to. */
+ * formed again. */
 BPC_API size_t bpc_linear_attention_workspace_size(int64_t B, int64_t T, int32_t H, int32_t dk, int32_t dv, int32_t dtype,
                                                    int32_t backward);
 BPC_API int bpc_linear_attention_fwd(const void* q, const void* k, const void* v, void* o, const float* log_decay,
