@@ -535,7 +535,8 @@ class CascadeNet(nn.Module):
     of other sizes); None: the `embed` module itself.  ops.embedding runs it and its weight gradient on the library's
     kernels (GPU only): the same values, a gradient that repeats bit for bit.
     norm="group": GroupNorm + SiLU in place of every BatchNorm + SiLU (CascadeBlock; gn_out before the read-out), GPU only;
-    eval then runs the composition of training."""
+    eval then runs the composition of training, in fp32 unless it is under autocast as training is (256 BB72 shots of 14 blocks of
+    512 channels: 758 ms, under bf16 autocast 9.6; with BatchNorm 3.7)."""
 
     def __init__(self, geo, H, L, det_t, det_typ, det_site, logicals, res="branch", embedding=None, norm="batch",
                  groups=32):
