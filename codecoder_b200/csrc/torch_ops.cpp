@@ -473,7 +473,7 @@ Tensor linear_attention_step(const Tensor& q_in, const Tensor& k_in, const Tenso
                              const Tensor& state, double scale, const std::optional<Tensor>& new_state) {
   at::NoGradGuard no_grad;
   const char* what = "linear_attention_step";
-  check_followed(what, {&q_in, &k_in, &v_in, &log_decay, &state});
+  check_followed(what, {&q_in, &k_in, &v_in, &log_decay, &state, new_state ? &*new_state : &state});
   const int32_t code = check_heads(q_in, k_in, v_in, log_decay, 3, what);
   const Tensor& to = new_state ? *new_state : state;
   for (const Tensor* s : {&state, &to}) {

@@ -43,3 +43,10 @@ def test_traces_are_refused(at):
     f, args, _ = list(calls())[at]
     with pytest.raises(RuntimeError, match="cannot be traced"):
         torch.jit.trace(lambda *a: f(*a), tuple(args), check_trace=False)
+
+
+def test_a_tangent_of_the_state_written_is_refused():
+    """It would be left beside a value that it no longer belongs to."""
+    q, g, state = torch.randn(2, 2, 4), -torch.ones(2), torch.zeros(2, 2, 4, 4)
+    with fwd.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+        ops.linear_attention_step(q, q, q, g, state, new_state=fwd.make_dual(state.clone(), state))
