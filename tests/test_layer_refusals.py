@@ -14,7 +14,7 @@ def test_the_fused_path_refuses_blocks_with_group_norm(H):
         CascadeStack.forward_blocks(blocks, h)
 
 
-@pytest.mark.parametrize("device,error,text", [("cpu", RuntimeError, "CUDA"), pytest.param("cuda", ValueError, "", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("device,error,text", [("cpu", RuntimeError, "CUDA"), pytest.param("cuda", ValueError, "head size", marks=pytest.mark.gpu)])
 def test_heads_of_no_size_are_refused_by_the_entry_points(device, error, text):
     from codecoder_b200 import ops
     g = torch.zeros(2, device=device)
